@@ -386,6 +386,94 @@ oxh_status oxh_adamw_multi_tensor_table_step(oxh_stream stream, float learning_r
                                              const uint32_t *device_chunk_starts,
                                              uint32_t count, uint64_t total_chunks);
 
+/* ------------------------------------------------------------------ sequence layers
+ * What a recurrent sequence model's blocks and their matrices train with; no counterpart in the
+ * reference, which has no layer along a sequence, no norm over one position's features and one
+ * optimizer.  Activations are float32 or bfloat16 (OXH_F32, OXH_BF16: contiguous, aligned to
+ * their elements), parameters, statistics, states and all arithmetic float32; an output is
+ * rounded once. */
+#define OXH_F32 0
+#define OXH_BF16 1
+
+/* Root-mean-square norm over the last dimension of input (+ residual, may be NULL):
+ *   s = input + residual;  q = 1 / sqrt(mean(s^2) + epsilon);  output = s * q * weight
+ * `sum` receives s and `inverse_rms` [rows] q (either may be NULL; the backward reads both; with
+ * no residual s is the input).  `sum` may be `input` or `residual` itself (a residual stream kept
+ * in place); nothing else may overlap. */
+oxh_status oxh_rms_norm_forward(oxh_stream stream, int dtype, uint64_t rows, uint64_t columns,
+                                float epsilon, const void *input, const void *residual,
+                                const float *weight, void *sum, void *output,
+                                float *inverse_rms);
+/* Its backward, from `gradient` (of the output) and `sum_gradient` (of s where it has other uses,
+ * the residual stream's own gradient; may be NULL), with u = s * q and d = gradient * weight:
+ *   input_gradient = sum_gradient + q * (d - u * mean(u * d))     (of input and of residual)
+ *   weight_gradient = sum over rows of gradient * u               (may be NULL)
+ * input_gradient may be sum_gradient itself.  The weight gradient's sums have a fixed order and
+ * take the workspace (may be NULL without it).  No rows: the weight gradient is 0. */
+oxh_status oxh_rms_norm_backward_workspace_size(uint64_t rows, uint64_t columns,
+                                                uint64_t *bytes);
+oxh_status oxh_rms_norm_backward(oxh_stream stream, int dtype, uint64_t rows, uint64_t columns,
+                                 const void *gradient, const void *sum_gradient,
+                                 const void *sum, const float *weight, const float *inverse_rms,
+                                 void *input_gradient, float *weight_gradient, void *workspace,
+                                 uint64_t workspace_bytes);
+
+/* Gated linear recurrence over [batch, time, channels], per batch row and channel:
+ *   a_t = sigmoid(gate_t);  h_t = a_t * h_{t-1} + (1 - a_t) * input_t
+ * from initial_state [batch, channels] (NULL: 0); output holds every h_t and final_state (may be
+ * NULL) the last.  lengths (device int32 [batch], may be NULL; clamped to 0..time): a row's steps
+ * at or past its length give 0 and leave the state, whatever input and gate hold there.
+ * final_state may be initial_state itself: single tokens are time 1 with the state in place. */
+oxh_status oxh_gated_recurrence_workspace_size(uint64_t batch, uint64_t time, uint64_t channels,
+                                               uint64_t *bytes);
+oxh_status oxh_gated_recurrence_forward(oxh_stream stream, int dtype, uint64_t batch,
+                                        uint64_t time, uint64_t channels, const void *input,
+                                        const void *gate, const float *initial_state,
+                                        const int32_t *lengths, void *output,
+                                        float *final_state, void *workspace,
+                                        uint64_t workspace_bytes);
+/* Its backward from `gradient` (of every h_t) and final_state_gradient (may be NULL), reading the
+ * forward's operands and output:
+ *   l_t = gradient_t + a_{t+1} * l_{t+1} (+ final_state_gradient at the last step)
+ *   input_gradient_t = (1 - a_t) * l_t
+ *   gate_gradient_t = a_t * (1 - a_t) * (h_{t-1} - input_t) * l_t
+ *   initial_state_gradient = a_1 * l_1   (may be NULL; may be final_state_gradient itself)
+ * Steps at or past a row's length take gradients of 0. */
+oxh_status oxh_gated_recurrence_backward(
+    oxh_stream stream, int dtype, uint64_t batch, uint64_t time, uint64_t channels,
+    const void *gradient, const void *input, const void *gate, const void *output,
+    const float *initial_state, const float *final_state_gradient, const int32_t *lengths,
+    void *input_gradient, void *gate_gradient, float *initial_state_gradient, void *workspace,
+    uint64_t workspace_bytes);
+
+/* Orthogonalises `count` matrices [rows, columns] (contiguous, float32) by Newton-Schulz
+ * products: X = V / (|V|_F + epsilon), then `rounds` times
+ *   A = X X';  B = b A + c A A;  X = a X + B X,   (a, b, c) = (3.4445, -4.7750, 2.0315)
+ * (the transposed iteration where rows > columns), which takes every singular value that is not
+ * tiny to about 1 (0.7 .. 1.21) and keeps the singular vectors.  A zero matrix gives zeros. */
+oxh_status oxh_orthogonalize_workspace_size(uint64_t count, uint64_t rows, uint64_t columns,
+                                            uint64_t *bytes);
+oxh_status oxh_orthogonalize(oxh_stream stream, uint64_t count, uint64_t rows, uint64_t columns,
+                             uint32_t rounds, float epsilon, const float *input, float *output,
+                             void *workspace, uint64_t workspace_bytes);
+/* Optimizer step of weight matrices by their orthogonalised momentum (a convolution's weight is
+ * the matrix [out, in * kh * kw]), in place:
+ *   M = momentum * M + G;  V = nesterov ? G + momentum * M : M;  X = V orthogonalised as above
+ *   W = W - learning_rate * (weight_decay * W + sqrt(max(1, rows / columns)) * X)
+ * `tensors` is host memory, read before the call returns. */
+typedef struct oxh_muon_tensor {
+  float *parameter;
+  const float *gradient;
+  float *momentum;
+  uint64_t rows, columns;
+} oxh_muon_tensor;
+oxh_status oxh_muon_workspace_size(const oxh_muon_tensor *tensors, uint32_t count,
+                                   uint64_t *bytes);
+oxh_status oxh_muon_multi_tensor(oxh_stream stream, float learning_rate, float weight_decay,
+                                 float momentum, int nesterov, float epsilon, uint32_t rounds,
+                                 const oxh_muon_tensor *tensors, uint32_t count, void *workspace,
+                                 uint64_t workspace_bytes);
+
 /* ------------------------------------------------------------------ conv2d / avg_pool2d
  * The layers around the hot path that a MobileNetV4-Conv-S training step needs.  Reference
  * kernels kernel_module.rs:359-490,558-825; CPU semantics evaluation.rs:334-445,

@@ -1,0 +1,487 @@
+// rms_norm.hip -- root-mean-square norm over the last dimension, of a residual sum where there is
+// one, and its gradients.
+//
+//   s = x + r;  q = 1 / sqrt(mean(s^2) + epsilon);  y = s q w
+//   d = dy w;   dx = dr = ds + q (d - s q mean(s q d));   dw = sum over rows of dy s q
+//
+// Rows are float32 or bfloat16; the sum, the statistics, both dot products and the weight
+// gradient are float32, and each output is rounded once (y from the unrounded s).  No counterpart
+// in the reference, whose only norm is BatchNorm2d.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <string>
+
+#include "common.h"
+#include "storage.h"
+
+namespace {
+
+using oxh::storage::bf16;
+using oxh::storage::load;
+using oxh::storage::store;
+
+// The sum over a row's Lanes threads (whole waves) in one fixed order, in every thread.  `slot`
+// is a buffer of 16 floats; consecutive calls alternate between two.
+template <int Lanes>
+__device__ __forceinline__ float row_sum(float v, float *slot) {
+  float one[1] = {v};
+  oxh::wave_sums_rows(one);
+  if constexpr (Lanes == 64) return one[0];
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) slot[wave] = one[0];
+  __syncthreads();
+  float total = 0.0f;
+#pragma unroll
+  for (int i = 0; i < Lanes / 64; ++i) total += slot[i];
+  return total;
+}
+
+template <typename T>
+struct Forward {
+  const T *x, *r;
+  const float *w;
+  T *s, *y;
+  float *q;
+  uint64_t rows;
+  uint32_t columns;
+  float inverse_columns, epsilon;
+};
+
+// One row per Lanes threads, kept in registers between its two uses: Chunks accesses of N values
+// per thread cover it.
+template <typename T, int N, int Lanes, int Chunks>
+__global__ __launch_bounds__(Lanes < 256 ? 256 : Lanes) void rms_norm_forward_kernel(
+    Forward<T> a) {
+  __shared__ float slot[16];
+  constexpr int kRows = Lanes < 256 ? 256 / Lanes : 1;
+  const uint32_t lane = threadIdx.x % Lanes;
+  const uint64_t row = static_cast<uint64_t>(blockIdx.x) * kRows + threadIdx.x / Lanes;
+  if (row >= a.rows) return;  // whole waves: Lanes == 64 when a block holds several rows
+  const uint64_t base = row * a.columns;
+  float v[Chunks][N];
+  float squares = 0.0f;
+#pragma unroll
+  for (int c = 0; c < Chunks; ++c) {
+    const uint32_t at = (c * Lanes + lane) * N;
+    if (at < a.columns) {
+      load<T, N>(a.x + base + at, v[c]);
+      if (a.r != nullptr) {
+        float r[N];
+        load<T, N>(a.r + base + at, r);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[c][i] += r[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[c][i] = 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) squares = fmaf(v[c][i], v[c][i], squares);
+  }
+  const float q =
+      1.0f / sqrtf(row_sum<Lanes>(squares, slot) * a.inverse_columns + a.epsilon);
+  if (lane == 0 && a.q != nullptr) a.q[row] = q;
+#pragma unroll
+  for (int c = 0; c < Chunks; ++c) {
+    const uint32_t at = (c * Lanes + lane) * N;
+    if (at >= a.columns) continue;
+    if (a.s != nullptr) store<T, N>(a.s + base + at, v[c]);
+    float w[N];
+    load<float, N>(a.w + at, w);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[c][i] = v[c][i] * q * w[i];
+    store<T, N>(a.y + base + at, v[c]);
+  }
+}
+
+// Rows longer than the registers of a block: two passes over the operands.  The second forms the
+// sum again (from x and r, not from the rounded one); a thread reads its elements before it writes
+// them, so s may be x or r here too.
+template <typename T>
+__global__ __launch_bounds__(1024) void rms_norm_forward_long_kernel(Forward<T> a) {
+  __shared__ float slot[16];
+  const uint64_t base = static_cast<uint64_t>(blockIdx.x) * a.columns;
+  float squares = 0.0f;
+  for (uint32_t at = threadIdx.x; at < a.columns; at += 1024) {
+    float v = oxh::storage::widen(a.x[base + at]);
+    if (a.r != nullptr) v += oxh::storage::widen(a.r[base + at]);
+    squares = fmaf(v, v, squares);
+  }
+  const float q = 1.0f / sqrtf(row_sum<1024>(squares, slot) * a.inverse_columns + a.epsilon);
+  if (threadIdx.x == 0 && a.q != nullptr) a.q[blockIdx.x] = q;
+  for (uint32_t at = threadIdx.x; at < a.columns; at += 1024) {
+    float v = oxh::storage::widen(a.x[base + at]);
+    if (a.r != nullptr) v += oxh::storage::widen(a.r[base + at]);
+    if (a.s != nullptr) a.s[base + at] = static_cast<T>(v);
+    a.y[base + at] = static_cast<T>(v * q * a.w[at]);
+  }
+}
+
+template <typename T>
+struct Backward {
+  const T *g, *sg, *s;
+  const float *w, *q;
+  T *dx;
+  float *partial;
+  uint64_t rows;
+  uint32_t columns;
+  float inverse_columns;
+};
+
+// Each group of Lanes threads takes every groups-th row and keeps its share of the weight
+// gradient in registers; the groups' shares go to `partial`, one row of columns each.
+template <typename T, int N, int Lanes, int Chunks>
+__global__ __launch_bounds__(Lanes < 256 ? 256 : Lanes) void rms_norm_backward_kernel(
+    Backward<T> a) {
+  __shared__ float slot[2][16];
+  constexpr int kRows = Lanes < 256 ? 256 / Lanes : 1;
+  const uint32_t lane = threadIdx.x % Lanes;
+  const uint64_t group = static_cast<uint64_t>(blockIdx.x) * kRows + threadIdx.x / Lanes;
+  const uint64_t groups = static_cast<uint64_t>(gridDim.x) * kRows;
+  float dw[Chunks][N], w[Chunks][N];
+#pragma unroll
+  for (int c = 0; c < Chunks; ++c) {
+    const uint32_t at = (c * Lanes + lane) * N;
+#pragma unroll
+    for (int i = 0; i < N; ++i) dw[c][i] = w[c][i] = 0.0f;
+    if (at < a.columns) load<float, N>(a.w + at, w[c]);
+  }
+  int turn = 0;
+  for (uint64_t row = group; row < a.rows; row += groups) {
+    const uint64_t base = row * a.columns;
+    const float q = a.q[row];
+    float unit[Chunks][N], d[Chunks][N];
+    float dot = 0.0f;
+#pragma unroll
+    for (int c = 0; c < Chunks; ++c) {
+      const uint32_t at = (c * Lanes + lane) * N;
+#pragma unroll
+      for (int i = 0; i < N; ++i) unit[c][i] = d[c][i] = 0.0f;
+      if (at >= a.columns) continue;
+      load<T, N>(a.s + base + at, unit[c]);
+      load<T, N>(a.g + base + at, d[c]);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        unit[c][i] *= q;
+        dw[c][i] = fmaf(d[c][i], unit[c][i], dw[c][i]);
+        d[c][i] *= w[c][i];
+        dot = fmaf(unit[c][i], d[c][i], dot);
+      }
+    }
+    const float mean = row_sum<Lanes>(dot, slot[turn]) * a.inverse_columns;
+    turn ^= 1;
+#pragma unroll
+    for (int c = 0; c < Chunks; ++c) {
+      const uint32_t at = (c * Lanes + lane) * N;
+      if (at >= a.columns) continue;
+      float out[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) out[i] = q * (d[c][i] - unit[c][i] * mean);
+      if (a.sg != nullptr) {
+        float sg[N];
+        load<T, N>(a.sg + base + at, sg);
+#pragma unroll
+        for (int i = 0; i < N; ++i) out[i] += sg[i];
+      }
+      store<T, N>(a.dx + base + at, out);
+    }
+  }
+  if (a.partial == nullptr) return;
+#pragma unroll
+  for (int c = 0; c < Chunks; ++c) {
+    const uint32_t at = (c * Lanes + lane) * N;
+    if (at < a.columns) store<float, N>(a.partial + group * a.columns + at, dw[c]);
+  }
+}
+
+// Rows longer than the registers of a block: two passes over a row, and the weight gradient's
+// share kept in `partial` itself.
+template <typename T>
+__global__ __launch_bounds__(1024) void rms_norm_backward_long_kernel(Backward<T> a) {
+  __shared__ float slot[2][16];
+  int turn = 0;
+  float *dw = a.partial == nullptr
+                  ? nullptr
+                  : a.partial + static_cast<uint64_t>(blockIdx.x) * a.columns;
+  for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const uint64_t base = row * a.columns;
+    const float q = a.q[row];
+    float dot = 0.0f;
+    for (uint32_t at = threadIdx.x; at < a.columns; at += 1024) {
+      const float g = oxh::storage::widen(a.g[base + at]);
+      const float unit = oxh::storage::widen(a.s[base + at]) * q;
+      dot = fmaf(unit, g * a.w[at], dot);
+    }
+    const float mean = row_sum<1024>(dot, slot[turn]) * a.inverse_columns;
+    turn ^= 1;
+    for (uint32_t at = threadIdx.x; at < a.columns; at += 1024) {
+      const float g = oxh::storage::widen(a.g[base + at]);
+      const float unit = oxh::storage::widen(a.s[base + at]) * q;
+      float out = q * (g * a.w[at] - unit * mean);
+      if (a.sg != nullptr) out += oxh::storage::widen(a.sg[base + at]);
+      a.dx[base + at] = static_cast<T>(out);
+      if (dw != nullptr) dw[at] = row == blockIdx.x ? g * unit : fmaf(g, unit, dw[at]);
+    }
+  }
+}
+
+// out[c] = sum over the partial rows, in row order within each of 16 strands, the strands added
+// in order.
+__global__ __launch_bounds__(1024) void rms_norm_weight_kernel(const float *partial, float *out,
+                                                               uint32_t rows, uint32_t columns) {
+  __shared__ float part[16][64];
+  const uint32_t column = blockIdx.x * 64 + (threadIdx.x & 63), strand = threadIdx.x >> 6;
+  float sum = 0.0f;
+  if (column < columns)
+    for (uint32_t r = strand; r < rows; r += 16)
+      sum += partial[static_cast<uint64_t>(r) * columns + column];
+  part[strand][threadIdx.x & 63] = sum;
+  __syncthreads();
+  if (strand != 0 || column >= columns) return;
+#pragma unroll
+  for (int i = 1; i < 16; ++i) sum += part[i][threadIdx.x];
+  out[column] = sum;
+}
+
+// Values that one row's registers cover at N values per access (8 accesses of 1024 threads).
+template <int N>
+constexpr uint64_t row_limit() {
+  return 1024ull * 8 * N;
+}
+
+template <int Lanes, int Chunks>
+struct Shape {
+  static constexpr int lanes = Lanes, chunks = Chunks;
+};
+
+// Calls run(Shape<lanes, chunks>) with the fewest threads per row that keep it within 8 accesses
+// each.
+template <int N, typename Run>
+void with_shape(uint64_t columns, Run run) {
+  const uint64_t packs = (columns + N - 1) / N;
+  if (packs <= 64) run(Shape<64, 1>());
+  else if (packs <= 128) run(Shape<64, 2>());
+  else if (packs <= 256) run(Shape<64, 4>());
+  else if (packs <= 512) run(Shape<256, 2>());
+  else if (packs <= 1024) run(Shape<256, 4>());
+  else if (packs <= 2048) run(Shape<256, 8>());
+  else if (packs <= 4096) run(Shape<1024, 4>());
+  else run(Shape<1024, 8>());
+}
+
+// Groups of rows that the backward's weight gradient is summed over (rows of `partial`, which
+// stays within 8 MB up to 8192 columns).
+uint64_t group_limit(uint64_t columns) {
+  return std::min<uint64_t>(2048, std::max<uint64_t>(256, (1ull << 21) / columns));
+}
+uint64_t backward_groups(uint64_t rows, uint64_t columns) {
+  return std::min<uint64_t>(rows, group_limit(columns));
+}
+
+oxh_status check_rows(const char *what, int dtype, uint64_t rows, uint64_t columns) {
+  OXH_REQUIRE(oxh::storage::valid(dtype), OXH_INVALID_SHAPE,
+              std::string(what) + ": dtype is neither OXH_F32 nor OXH_BF16");
+  OXH_REQUIRE(columns >= 1 && columns < (1ull << 31), OXH_INVALID_SHAPE,
+              std::string(what) + ": columns out of range");
+  OXH_REQUIRE(rows < (1ull << 31), OXH_INVALID_SHAPE, std::string(what) + ": too many rows");
+  OXH_REQUIRE(rows <= (1ull << 60) / columns, OXH_INVALID_SHAPE,
+              std::string(what) + ": element count overflow");
+  return oxh::ok();
+}
+
+bool aligned_to(const void *p, uint64_t bytes) {
+  return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0;
+}
+
+template <typename T>
+oxh_status forward(hipStream_t stream, const Forward<T> &a) {
+  constexpr int kPack = 16 / sizeof(T);
+  const bool packed = a.columns % kPack == 0 && oxh::aligned16(a.x) && oxh::aligned16(a.y) &&
+                      (a.r == nullptr || oxh::aligned16(a.r)) &&
+                      (a.s == nullptr || oxh::aligned16(a.s)) && oxh::aligned16(a.w);
+  const uint64_t limit = packed ? row_limit<kPack>() : row_limit<1>();
+  if (a.columns > limit) {
+    oxh::launch(rms_norm_forward_long_kernel<T>, dim3(static_cast<uint32_t>(a.rows)),
+                dim3(1024), 0, stream, a);
+    return oxh::launched("rms_norm_forward");
+  }
+  auto start = [&](auto pack) {
+    constexpr int N = decltype(pack)::value;
+    with_shape<N>(a.columns, [&](auto shape) {
+      using S = decltype(shape);
+      constexpr int threads = S::lanes < 256 ? 256 : S::lanes, per = threads / S::lanes;
+      oxh::launch(rms_norm_forward_kernel<T, N, S::lanes, S::chunks>,
+                  dim3(static_cast<uint32_t>((a.rows + per - 1) / per)), dim3(threads), 0,
+                  stream, a);
+    });
+  };
+  if (packed) start(std::integral_constant<int, kPack>());
+  else start(std::integral_constant<int, 1>());
+  return oxh::launched("rms_norm_forward");
+}
+
+template <typename T>
+oxh_status backward(hipStream_t stream, const Backward<T> &a, float *weight_gradient) {
+  constexpr int kPack = 16 / sizeof(T);
+  const bool packed = a.columns % kPack == 0 && oxh::aligned16(a.g) && oxh::aligned16(a.s) &&
+                      oxh::aligned16(a.dx) && (a.sg == nullptr || oxh::aligned16(a.sg)) &&
+                      oxh::aligned16(a.w);
+  const uint64_t limit = packed ? row_limit<kPack>() : row_limit<1>();
+  uint64_t groups = backward_groups(a.rows, a.columns);
+  if (a.columns > limit) {
+    oxh::launch(rms_norm_backward_long_kernel<T>, dim3(static_cast<uint32_t>(groups)),
+                dim3(1024), 0, stream, a);
+  } else {
+    auto start = [&](auto pack) {
+      constexpr int N = decltype(pack)::value;
+      with_shape<N>(a.columns, [&](auto shape) {
+        using S = decltype(shape);
+        constexpr int threads = S::lanes < 256 ? 256 : S::lanes, per = threads / S::lanes;
+        // whole blocks of groups: the last block's spare groups have no rows and add zeros
+        const uint64_t blocks = std::max<uint64_t>(1, std::min<uint64_t>(
+            (a.rows + per - 1) / per, group_limit(a.columns) / per));
+        groups = blocks * per;
+        oxh::launch(rms_norm_backward_kernel<T, N, S::lanes, S::chunks>,
+                    dim3(static_cast<uint32_t>(blocks)), dim3(threads), 0, stream, a);
+      });
+    };
+    if (packed) start(std::integral_constant<int, kPack>());
+    else start(std::integral_constant<int, 1>());
+  }
+  oxh_status st = oxh::launched("rms_norm_backward");
+  if (st != OXH_OK || weight_gradient == nullptr) return st;
+  oxh::launch(rms_norm_weight_kernel, dim3((a.columns + 63) / 64), dim3(1024), 0, stream,
+              static_cast<const float *>(a.partial), weight_gradient,
+              static_cast<uint32_t>(groups), a.columns);
+  return oxh::launched("rms_norm_weight_gradient");
+}
+
+}  // namespace
+
+extern "C" {
+
+oxh_status oxh_rms_norm_forward(oxh_stream stream, int dtype, uint64_t rows, uint64_t columns,
+                                float epsilon, const void *input, const void *residual,
+                                const float *weight, void *sum, void *output,
+                                float *inverse_rms) {
+  oxh_status st = check_rows("rms norm", dtype, rows, columns);
+  if (st != OXH_OK) return st;
+  OXH_REQUIRE(std::isfinite(epsilon) && epsilon >= 0.0f, OXH_EXECUTION,
+              "rms norm epsilon must be non-negative and finite");
+  if (rows == 0) return oxh::ok();
+  OXH_REQUIRE(input != nullptr && weight != nullptr && output != nullptr, OXH_INVALID_SHAPE,
+              "rms norm: null pointer");
+  const uint64_t bytes = rows * columns * oxh::storage::bytes_of(dtype);
+  const uint64_t element = oxh::storage::bytes_of(dtype);
+  OXH_REQUIRE(aligned_to(input, element) && aligned_to(residual, element) &&
+                  aligned_to(sum, element) && aligned_to(output, element) &&
+                  aligned_to(weight, 4) && aligned_to(inverse_rms, 4),
+              OXH_INVALID_SHAPE, "rms norm: a pointer is not aligned to its elements");
+  // the sum may be written over an operand, nothing else may overlap
+  auto apart = [&](const void *a, uint64_t an, const void *b, uint64_t bn) {
+    return a == nullptr || b == nullptr || !oxh::any_overlap(a, an, b, bn);
+  };
+  OXH_REQUIRE(apart(output, bytes, input, bytes) && apart(output, bytes, residual, bytes) &&
+                  apart(output, bytes, sum, bytes) && apart(output, bytes, weight, columns * 4) &&
+                  apart(sum, bytes, weight, columns * 4) &&
+                  apart(inverse_rms, rows * 4, output, bytes) &&
+                  apart(inverse_rms, rows * 4, sum, bytes) &&
+                  apart(inverse_rms, rows * 4, input, bytes) &&
+                  apart(inverse_rms, rows * 4, residual, bytes) &&
+                  apart(inverse_rms, rows * 4, weight, columns * 4),
+              OXH_INVALID_SHAPE, "rms norm: an output overlaps an operand or another output");
+  OXH_REQUIRE(sum == nullptr || (!oxh::partial_overlap(sum, input, bytes) &&
+                                 (residual == nullptr ||
+                                  !oxh::partial_overlap(sum, residual, bytes))),
+              OXH_INVALID_SHAPE, "rms norm: the sum partially overlaps an operand");
+  const uint32_t cols = static_cast<uint32_t>(columns);
+  const float inverse = 1.0f / static_cast<float>(columns);
+  if (dtype == OXH_F32)
+    return forward<float>(oxh::as_stream(stream),
+                          {static_cast<const float *>(input), static_cast<const float *>(residual),
+                           weight, static_cast<float *>(sum), static_cast<float *>(output),
+                           inverse_rms, rows, cols, inverse, epsilon});
+  return forward<bf16>(oxh::as_stream(stream),
+                       {static_cast<const bf16 *>(input), static_cast<const bf16 *>(residual),
+                        weight, static_cast<bf16 *>(sum), static_cast<bf16 *>(output),
+                        inverse_rms, rows, cols, inverse, epsilon});
+}
+
+oxh_status oxh_rms_norm_backward_workspace_size(uint64_t rows, uint64_t columns,
+                                                uint64_t *bytes) {
+  OXH_REQUIRE(bytes != nullptr, OXH_INVALID_SHAPE, "bytes is null");
+  oxh_status st = check_rows("rms norm", OXH_F32, rows, columns);
+  if (st != OXH_OK) return st;
+  // groups come in whole blocks of 4
+  *bytes = ((backward_groups(rows, columns) + 3) / 4 * 4 * columns * 4 + 255) / 256 * 256;
+  return oxh::ok();
+}
+
+oxh_status oxh_rms_norm_backward(oxh_stream stream, int dtype, uint64_t rows, uint64_t columns,
+                                 const void *gradient, const void *sum_gradient,
+                                 const void *sum, const float *weight, const float *inverse_rms,
+                                 void *input_gradient, float *weight_gradient, void *workspace,
+                                 uint64_t workspace_bytes) {
+  oxh_status st = check_rows("rms norm backward", dtype, rows, columns);
+  if (st != OXH_OK) return st;
+  if (rows == 0) {
+    if (weight_gradient == nullptr) return oxh::ok();
+    return oxh_memset0_async(weight_gradient, columns * 4, stream);
+  }
+  OXH_REQUIRE(gradient != nullptr && sum != nullptr && weight != nullptr &&
+                  inverse_rms != nullptr && input_gradient != nullptr,
+              OXH_INVALID_SHAPE, "rms norm backward: null pointer");
+  const uint64_t element = oxh::storage::bytes_of(dtype), bytes = rows * columns * element;
+  OXH_REQUIRE(aligned_to(gradient, element) && aligned_to(sum_gradient, element) &&
+                  aligned_to(sum, element) && aligned_to(input_gradient, element) &&
+                  aligned_to(weight, 4) && aligned_to(inverse_rms, 4) &&
+                  aligned_to(weight_gradient, 4),
+              OXH_INVALID_SHAPE, "rms norm backward: a pointer is not aligned to its elements");
+  uint64_t needed = 0;
+  if (weight_gradient != nullptr) {
+    st = oxh_rms_norm_backward_workspace_size(rows, columns, &needed);
+    if (st != OXH_OK) return st;
+    OXH_REQUIRE(workspace != nullptr && workspace_bytes >= needed && oxh::aligned16(workspace),
+                OXH_INVALID_SHAPE, "rms norm backward: workspace too small or misaligned");
+  }
+  struct Span {
+    const void *p;
+    uint64_t n;
+  };
+  const Span in[] = {{gradient, bytes}, {sum, bytes},           {weight, columns * 4},
+                     {inverse_rms, rows * 4}, {sum_gradient, bytes}};
+  const Span out[] = {{input_gradient, bytes}, {weight_gradient, columns * 4},
+                      {needed != 0 ? workspace : nullptr, needed}};
+  for (int o = 0; o < 3; ++o) {
+    if (out[o].p == nullptr) continue;
+    for (int i = 0; i < 5; ++i) {
+      if (in[i].p == nullptr || (o == 0 && i == 4 && in[i].p == out[o].p)) continue;
+      OXH_REQUIRE(!oxh::any_overlap(out[o].p, out[o].n, in[i].p, in[i].n), OXH_INVALID_SHAPE,
+                  "rms norm backward: an output or the workspace overlaps an operand");
+    }
+    for (int k = 0; k < o; ++k)
+      OXH_REQUIRE(out[k].p == nullptr ||
+                      !oxh::any_overlap(out[o].p, out[o].n, out[k].p, out[k].n),
+                  OXH_INVALID_SHAPE, "rms norm backward: two outputs overlap");
+  }
+  const uint32_t cols = static_cast<uint32_t>(columns);
+  const float inverse = 1.0f / static_cast<float>(columns);
+  float *partial = weight_gradient != nullptr ? static_cast<float *>(workspace) : nullptr;
+  if (dtype == OXH_F32)
+    return backward<float>(
+        oxh::as_stream(stream),
+        {static_cast<const float *>(gradient), static_cast<const float *>(sum_gradient),
+         static_cast<const float *>(sum), weight, inverse_rms,
+         static_cast<float *>(input_gradient), partial, rows, cols, inverse},
+        weight_gradient);
+  return backward<bf16>(
+      oxh::as_stream(stream),
+      {static_cast<const bf16 *>(gradient), static_cast<const bf16 *>(sum_gradient),
+       static_cast<const bf16 *>(sum), weight, inverse_rms, static_cast<bf16 *>(input_gradient),
+       partial, rows, cols, inverse},
+      weight_gradient);
+}
+
+}  // extern "C"

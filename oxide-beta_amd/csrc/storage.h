@@ -1,0 +1,61 @@
+// storage.h -- element types of the sequence operators (internal to the library): values are kept
+// as float32 or bfloat16, all arithmetic is float32, a stored bfloat16 is rounded once, to nearest
+// even.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <string>
+
+#include "common.h"
+
+namespace oxh {
+namespace storage {
+
+typedef __bf16 bf16;
+
+inline bool valid(int dtype) { return dtype == OXH_F32 || dtype == OXH_BF16; }
+inline uint64_t bytes_of(int dtype) { return dtype == OXH_BF16 ? 2 : 4; }
+
+template <typename T>
+__device__ __forceinline__ float widen(T v) {
+  return static_cast<float>(v);
+}
+
+// N consecutive values moved as one access (N * sizeof(T) bytes, up to 16; the address is a
+// multiple of that).
+template <typename T, int N>
+struct Pack {
+  typedef T type __attribute__((ext_vector_type(N)));
+};
+template <typename T>
+struct Pack<T, 1> {
+  typedef T type;
+};
+
+template <typename T, int N>
+__device__ __forceinline__ void load(const T *p, float (&v)[N]) {
+  if constexpr (N == 1) {
+    v[0] = widen(*p);
+  } else {
+    const typename Pack<T, N>::type x = *reinterpret_cast<const typename Pack<T, N>::type *>(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = widen(x[i]);
+  }
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store(T *p, const float (&v)[N]) {
+  if constexpr (N == 1) {
+    *p = static_cast<T>(v[0]);
+  } else {
+    typename Pack<T, N>::type x;
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = static_cast<T>(v[i]);
+    *reinterpret_cast<typename Pack<T, N>::type *>(p) = x;
+  }
+}
+
+}  // namespace storage
+}  // namespace oxh

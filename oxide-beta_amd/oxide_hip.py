@@ -64,6 +64,11 @@ class AdamWTensor(ctypes.Structure):
                 ("second_moment", _vp), ("n", _u64)]
 
 
+class MuonTensor(ctypes.Structure):
+    _fields_ = [("parameter", _vp), ("gradient", _vp), ("momentum", _vp), ("rows", _u64),
+                ("columns", _u64)]
+
+
 class Conv2dShape(ctypes.Structure):
     _fields_ = [(f, ctypes.c_uint64) for f in (
         "batch", "in_channels", "height", "width", "out_channels", "kernel_h", "kernel_w",
@@ -157,6 +162,17 @@ _SIGNATURES = {
                                                 _vp, _u32, _u64]),
     "oxh_adamw_multi_tensor_step": (_st, [_vp, _f32, _f32, _f32, _f32, _f32, _vp,
                                           ctypes.POINTER(AdamWTensor), _u32]),
+    "oxh_rms_norm_forward": (_st, [_vp, _int, _u64, _u64, _f32] + [_vp] * 6),
+    "oxh_rms_norm_backward_workspace_size": (_st, [_u64, _u64, ctypes.POINTER(_u64)]),
+    "oxh_rms_norm_backward": (_st, [_vp, _int, _u64, _u64] + [_vp] * 8 + [_u64]),
+    "oxh_gated_recurrence_workspace_size": (_st, [_u64, _u64, _u64, ctypes.POINTER(_u64)]),
+    "oxh_gated_recurrence_forward": (_st, [_vp, _int, _u64, _u64, _u64] + [_vp] * 7 + [_u64]),
+    "oxh_gated_recurrence_backward": (_st, [_vp, _int, _u64, _u64, _u64] + [_vp] * 11 + [_u64]),
+    "oxh_orthogonalize_workspace_size": (_st, [_u64, _u64, _u64, ctypes.POINTER(_u64)]),
+    "oxh_orthogonalize": (_st, [_vp, _u64, _u64, _u64, _u32, _f32, _vp, _vp, _vp, _u64]),
+    "oxh_muon_workspace_size": (_st, [ctypes.POINTER(MuonTensor), _u32, ctypes.POINTER(_u64)]),
+    "oxh_muon_multi_tensor": (_st, [_vp, _f32, _f32, _f32, _int, _f32, _u32,
+                                    ctypes.POINTER(MuonTensor), _u32, _vp, _u64]),
     "oxh_conv2d_output_size": (_st, [_CS, ctypes.POINTER(_u64), ctypes.POINTER(_u64)]),
     "oxh_conv2d_forward": (_st, [_vp, _CS, _vp, _vp, _vp, _vp]),
     "oxh_conv2d_forward_serial": (_int, [_CS]),
@@ -276,6 +292,46 @@ def _f32_tensor(t, name: str):
     return t
 
 
+F32, BF16 = 0, 1
+
+
+def _activation(tensors, shape, what: str) -> int:
+    """The dtype code of device tensors that share one type and one shape."""
+    import torch
+
+    first = tensors[0]
+    code = {torch.float32: F32, torch.bfloat16: BF16}.get(first.dtype)
+    if code is None or not first.is_cuda:
+        raise OxideError(INVALID_SHAPE, f"{what} takes float32 or bfloat16 device tensors")
+    for t in tensors:
+        if t is None:
+            continue
+        if t.dtype != first.dtype or t.device != first.device:
+            raise OxideError(INVALID_SHAPE, f"{what}: tensors differ in type or device")
+        if t.shape != shape:
+            raise OxideError(INVALID_SHAPE,
+                             f"{what}: shape {list(t.shape)} where {list(shape)} is expected")
+    return code
+
+
+def _shaped(t, shape, name: str):
+    """A float32 device tensor of ``shape``, or None."""
+    if t is not None and _f32_tensor(t, name).shape != shape:
+        raise OxideError(INVALID_SHAPE,
+                         f"{name}: shape {list(t.shape)} where {list(shape)} is expected")
+    return _ptr(t)
+
+
+def _lengths(t, batch: int):
+    import torch
+
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or not t.is_cuda or t.shape != (batch,):
+        raise OxideError(INVALID_SHAPE, "lengths must be an int32 device tensor [batch]")
+    return _ptr(t)
+
+
 def current_stream() -> int:
     import torch
 
@@ -320,6 +376,49 @@ def batch_norm_workspace_size(batch: int, channels: int, spatial: int) -> int:
 def cross_entropy_workspace_size(batch: int, classes: int) -> int:
     out = _u64()
     check(lib().oxh_cross_entropy_workspace_size(batch, classes, ctypes.byref(out)))
+    return out.value
+
+
+def rms_norm_backward_workspace_size(rows: int, columns: int) -> int:
+    out = _u64()
+    check(lib().oxh_rms_norm_backward_workspace_size(rows, columns, ctypes.byref(out)))
+    return out.value
+
+
+def gated_recurrence_workspace_size(batch: int, time: int, channels: int) -> int:
+    out = _u64()
+    check(lib().oxh_gated_recurrence_workspace_size(batch, time, channels, ctypes.byref(out)))
+    return out.value
+
+
+def orthogonalize_workspace_size(count: int, rows: int, columns: int) -> int:
+    out = _u64()
+    check(lib().oxh_orthogonalize_workspace_size(count, rows, columns, ctypes.byref(out)))
+    return out.value
+
+
+def muon_table(tensors):
+    """The C table of a sequence of (parameter, gradient, momentum): each a matrix
+    [shape[0], the rest] of float32 device values."""
+    table = (MuonTensor * len(tensors))()
+    for i, (p, g, m) in enumerate(tensors):
+        shape = tuple(p.shape)
+        if len(shape) < 2 or tuple(g.shape) != shape or tuple(m.shape) != shape:
+            raise OxideError(INVALID_SHAPE,
+                             "muon takes matrices: equal shapes of at least two dimensions")
+        for t in (p, g, m):
+            if hasattr(t, "dtype") and hasattr(t, "is_cuda"):
+                _f32_tensor(t, "a muon tensor")
+        columns = 1
+        for d in shape[1:]:
+            columns *= d
+        table[i] = MuonTensor(_ptr(p), _ptr(g), _ptr(m), shape[0], columns)
+    return table
+
+
+def muon_workspace_size(table) -> int:
+    out = _u64()
+    check(lib().oxh_muon_workspace_size(table, len(table), ctypes.byref(out)))
     return out.value
 
 
@@ -467,6 +566,7 @@ class LoadedModule:
         self._bn_ws = Workspace()
         self._ce_ws = Workspace()
         self._conv_ws = Workspace()
+        self._sequence_ws = Workspace()
 
     # -- elementwise (kernel_module.rs:8-34, 492-508, 1052-1059)
     def add(self, a, b, out, stream=None):
@@ -724,6 +824,94 @@ class LoadedModule:
             _ptr(step_counter), dev_table.data_ptr(), dev_starts.data_ptr(),
             count, total.value))
         return dev_table, dev_starts
+
+    # -- sequence layers (no counterpart in the reference)
+    def rms_norm_forward(self, x, weight, out, inverse_rms=None, residual=None, sum=None,  # noqa: A002
+                         epsilon=1e-6, stream=None):
+        """``out`` = s / rms(s) * weight over the last dimension, s = x + residual; ``sum``
+        receives s (it may be ``x`` or ``residual``) and ``inverse_rms`` [rows] what the
+        backward needs."""
+        code = _activation((x, out, residual, sum), x.shape, "rms_norm")
+        columns = x.shape[-1]
+        rows = x.numel() // max(columns, 1)
+        check(lib().oxh_rms_norm_forward(
+            _stream(stream), code, rows, columns, epsilon, _ptr(x), _ptr(residual),
+            _shaped(weight, (columns,), "weight"), _ptr(sum), _ptr(out),
+            _shaped(inverse_rms, (rows,), "inverse_rms")))
+
+    def rms_norm_backward(self, gradient, sum, weight, inverse_rms, input_gradient,  # noqa: A002
+                          weight_gradient=None, sum_gradient=None, stream=None):
+        """Gradients from the output's and, where the sum has other uses, ``sum_gradient``
+        (``input_gradient`` may be that tensor)."""
+        code = _activation((gradient, sum, input_gradient, sum_gradient), gradient.shape,
+                           "rms_norm_backward")
+        columns = gradient.shape[-1]
+        rows = gradient.numel() // max(columns, 1)
+        ws, wsb = (None, 0) if weight_gradient is None else self._sequence_ws.ptr_bytes(
+            rms_norm_backward_workspace_size(rows, columns))
+        check(lib().oxh_rms_norm_backward(
+            _stream(stream), code, rows, columns, _ptr(gradient), _ptr(sum_gradient), _ptr(sum),
+            _shaped(weight, (columns,), "weight"), _shaped(inverse_rms, (rows,), "inverse_rms"),
+            _ptr(input_gradient), _shaped(weight_gradient, (columns,), "weight_gradient"), ws,
+            wsb))
+
+    def gated_recurrence_forward(self, x, gate, out, initial_state=None, final_state=None,
+                                 lengths=None, stream=None):
+        """``out`` [batch, time, channels] of h_t = a_t h_{t-1} + (1 - a_t) x_t with
+        a_t = sigmoid(gate_t); states [batch, channels] float32 (the final one may be written
+        over the initial one), ``lengths`` [batch] int32."""
+        code = _activation((x, gate, out), x.shape, "gated_recurrence")
+        if x.dim() != 3:
+            raise OxideError(INVALID_SHAPE, "gated_recurrence expects [batch, time, channels]")
+        batch, time, channels = x.shape
+        ws, wsb = self._sequence_ws.ptr_bytes(
+            gated_recurrence_workspace_size(batch, time, channels))
+        states = (batch, channels)
+        check(lib().oxh_gated_recurrence_forward(
+            _stream(stream), code, batch, time, channels, _ptr(x), _ptr(gate),
+            _shaped(initial_state, states, "initial_state"), _lengths(lengths, batch),
+            _ptr(out), _shaped(final_state, states, "final_state"), ws, wsb))
+
+    def gated_recurrence_backward(self, gradient, x, gate, out, x_gradient, gate_gradient,
+                                  initial_state=None, final_state_gradient=None,
+                                  initial_state_gradient=None, lengths=None, stream=None):
+        """Gradients of ``gated_recurrence_forward``'s operands from its output's and its final
+        state's."""
+        code = _activation((gradient, x, gate, out, x_gradient, gate_gradient), x.shape,
+                           "gated_recurrence_backward")
+        if x.dim() != 3:
+            raise OxideError(INVALID_SHAPE, "gated_recurrence expects [batch, time, channels]")
+        batch, time, channels = x.shape
+        ws, wsb = self._sequence_ws.ptr_bytes(
+            gated_recurrence_workspace_size(batch, time, channels))
+        states = (batch, channels)
+        check(lib().oxh_gated_recurrence_backward(
+            _stream(stream), code, batch, time, channels, _ptr(gradient), _ptr(x), _ptr(gate),
+            _ptr(out), _shaped(initial_state, states, "initial_state"),
+            _shaped(final_state_gradient, states, "final_state_gradient"),
+            _lengths(lengths, batch), _ptr(x_gradient), _ptr(gate_gradient),
+            _shaped(initial_state_gradient, states, "initial_state_gradient"), ws, wsb))
+
+    def orthogonalize(self, x, out, rounds=5, epsilon=1e-7, stream=None):
+        """``out`` = the matrices of ``x`` ([rows, columns] or [count, rows, columns], float32)
+        orthogonalised by ``rounds`` Newton-Schulz rounds."""
+        if x.dim() not in (2, 3):
+            raise OxideError(INVALID_SHAPE, "orthogonalize expects a matrix or a stack of them")
+        count, (rows, columns) = (x.shape[0] if x.dim() == 3 else 1), x.shape[-2:]
+        ws, wsb = self._sequence_ws.ptr_bytes(orthogonalize_workspace_size(count, rows, columns))
+        check(lib().oxh_orthogonalize(_stream(stream), count, rows, columns, rounds, epsilon,
+                                      _shaped(x, x.shape, "x"), _shaped(out, x.shape, "out"), ws,
+                                      wsb))
+
+    def muon(self, learning_rate, weight_decay, momentum, tensors, nesterov=True, rounds=5,
+             epsilon=1e-7, stream=None):
+        """One optimizer step of ``tensors``, a sequence of (parameter, gradient, momentum):
+        the momentum and the parameter are updated in place."""
+        table = muon_table(tensors)
+        ws, wsb = self._sequence_ws.ptr_bytes(muon_workspace_size(table))
+        check(lib().oxh_muon_multi_tensor(_stream(stream), learning_rate, weight_decay, momentum,
+                                          int(bool(nesterov)), epsilon, rounds, table,
+                                          len(table), ws, wsb))
 
     # -- conv2d / avg_pool2d (kernel_module.rs:359-490, 558-825)
     def conv2d_forward(self, shape, x, weight, bias, out, stream=None):

@@ -1,0 +1,158 @@
+"""Newton-Schulz orthogonalisation and the optimizer step over it against the definition in float64.
+
+Tolerance.  An operand of a product keeps 22 bits, so each round perturbs X by about 2^-22 of its
+norm, and five rounds stretch what lies in the directions of the smallest singular values by at
+most 3.4445^5 = 485; the perturbation of a whole round in those directions is the float32 rounding
+of X alone, so 485 * 2^-22 = 1.2e-4 of the result's Frobenius norm is a bound that random matrices
+stay far below.  One round: 3.4445 * 2^-22 * 4."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import oxide_hip as ox
+
+pytestmark = pytest.mark.gpu
+A, B, C = 3.4445, -4.7750, 2.0315
+BOUND = A ** 5 * 2.0 ** -22
+SHAPES = [(1, 1), (1, 200), (200, 1), (2, 3), (31, 33), (32, 32), (33, 64), (64, 65), (96, 192),
+          (192, 96), (130, 127), (128, 512), (512, 96), (257, 300), (100, 1280), (10, 1280),
+          (700, 710), (300, 2000), (2000, 300)]
+
+
+def orthogonal(v, rounds=5, eps=1e-7):
+    x = v.T if v.shape[0] > v.shape[1] else v
+    x = x / (np.linalg.norm(x) + eps)
+    for _ in range(rounds):
+        gram = x @ x.T
+        x = A * x + (B * gram + C * (gram @ gram)) @ x
+    return x.T if v.shape[0] > v.shape[1] else x
+
+
+def matrix(shape, seed, scale=1e-3):
+    return (np.random.default_rng(seed).standard_normal(shape) * scale).astype(np.float32)
+
+
+def close(got, ref, bound, what=""):
+    off = np.linalg.norm(got.detach().cpu().double().numpy() - ref)
+    assert off <= bound * max(np.linalg.norm(ref), 1e-30), (what, off, np.linalg.norm(ref))
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_orthogonalize(module, dev, shape):
+    v = matrix(shape, 1)
+    x, out = torch.from_numpy(v).to(dev), torch.empty(shape, device=dev)
+    module.orthogonalize(x, out)
+    close(out, orthogonal(v.astype(np.float64)), BOUND)
+    singular = np.linalg.svd(orthogonal(v.astype(np.float64)), compute_uv=False)
+    assert singular.max() < 1.25
+
+
+@pytest.mark.parametrize("shape", [(40, 70), (70, 40), (200, 200)])
+@pytest.mark.parametrize("rounds", [1, 2, 3, 8])
+def test_rounds(module, dev, shape, rounds):
+    v = matrix(shape, 2)
+    out = torch.empty(shape, device=dev)
+    module.orthogonalize(torch.from_numpy(v).to(dev), out, rounds=rounds)
+    close(out, orthogonal(v.astype(np.float64), rounds), A ** min(rounds, 5) * 2.0 ** -20)
+
+
+@pytest.mark.parametrize("scale", [1e-15, 1e-6, 1.0, 1e15])
+def test_any_scale(module, dev, scale):
+    """The norm is taken first, so only its own range limits the values (the sum of squares is a
+    float32)."""
+    v = matrix((60, 90), 3, scale)
+    out = torch.empty(60, 90, device=dev)
+    module.orthogonalize(torch.from_numpy(v).to(dev), out, epsilon=1e-20)
+    close(out, orthogonal(v.astype(np.float64), eps=1e-20), BOUND)
+
+
+def test_low_rank_and_decaying_spectrum(module, dev):
+    """Directions far below the largest one: the ones that five rounds stretch most."""
+    r = np.random.default_rng(4)
+    v = ((r.standard_normal((150, 20)) * np.exp(-np.arange(20) / 4)) @
+         r.standard_normal((20, 260))).astype(np.float32)
+    out = torch.empty(150, 260, device=dev)
+    module.orthogonalize(torch.from_numpy(v).to(dev), out)
+    close(out, orthogonal(v.astype(np.float64)), BOUND)
+
+
+def test_stack_equals_its_matrices(module, dev):
+    """More matrices than one launch group takes, each with the bits it has alone."""
+    v = torch.from_numpy(matrix((70, 24, 40), 5)).to(dev)
+    out, one = torch.empty_like(v), torch.empty(24, 40, device=dev)
+    module.orthogonalize(v, out)
+    for i in (0, 31, 32, 69):
+        module.orthogonalize(v[i], one)
+        assert torch.equal(out[i], one)
+
+
+def test_zero_and_not_finite(module, dev):
+    v = torch.from_numpy(matrix((4, 50, 60), 6)).to(dev)
+    v[1] = 0.0
+    v[2, 3, 4] = float("nan")
+    out, clean = torch.empty_like(v), torch.empty(50, 60, device=dev)
+    module.orthogonalize(v, out)
+    assert (out[1] == 0).all() and out[2].isnan().all()
+    for i in (0, 3):
+        module.orthogonalize(v[i], clean)
+        assert torch.equal(out[i], clean)
+
+
+SETS = [[(96, 192)], [(192, 96, 1, 1)], [(32, 16, 3, 3), (10, 1280, 1, 1), (7, 5)],
+        [(300, 200), (200, 300), (64, 64), (1, 9)], [(24, 24 + i) for i in range(40)]]
+
+
+@pytest.mark.parametrize("shapes", SETS)
+@pytest.mark.parametrize("nesterov", [True, False])
+def test_step(module, dev, shapes, nesterov):
+    """Two steps over a list of matrices (convolution weights among them)."""
+    r = np.random.default_rng(7)
+    p, g, m = ([r.standard_normal(s).astype(np.float32) * k for s in shapes]
+               for k in (0.05, 1e-3, 1e-2))
+    dev_p, dev_g, dev_m = ([torch.from_numpy(a).to(dev) for a in t] for t in (p, g, m))
+    p, g, m = ([a.astype(np.float64).reshape(a.shape[0], -1) for a in t] for t in (p, g, m))
+    for _ in range(2):
+        module.muon(0.02, 0.1, 0.95, list(zip(dev_p, dev_g, dev_m)), nesterov=nesterov)
+        for i in range(len(p)):
+            m[i] = 0.95 * m[i] + g[i]
+            x = orthogonal(g[i] + 0.95 * m[i] if nesterov else m[i])
+            scale = math.sqrt(max(1.0, p[i].shape[0] / p[i].shape[1]))
+            moved = 0.02 * (0.1 * p[i] + scale * x)
+            p[i] = p[i] - moved
+            flat = lambda t: t.reshape(t.shape[0], -1)  # noqa: E731
+            close(flat(dev_m[i]), m[i], 4 * 2.0 ** -24, "momentum")
+            off = flat(dev_p[i]).cpu().double().numpy() - p[i]
+            tol = 2 * BOUND * np.linalg.norm(moved) + 4 * 2.0 ** -24 * np.linalg.norm(p[i])
+            assert np.linalg.norm(off) <= tol
+
+
+def test_another_stream_a_graph_and_repeats(module, dev):
+    shapes = [(96, 192), (130, 70), (512, 520)]
+    start = [[torch.from_numpy(matrix(s, 10 * i + j, k)).to(dev) for j, s in enumerate(shapes)]
+             for i, k in enumerate((0.05, 1e-3, 1e-2))]
+    p, g, m = ([t.clone() for t in ts] for ts in start)
+
+    def reset():
+        for now, then in zip((p, g, m), start):
+            for a, b in zip(now, then):
+                a.copy_(b)
+        torch.cuda.synchronize()
+
+    def step(stream=None):
+        module.muon(0.02, 0.01, 0.9, list(zip(p, g, m)), stream=stream)
+
+    step()
+    torch.cuda.synchronize()
+    want = [t.clone() for t in p + m]
+    stream = torch.cuda.Stream()
+    reset()
+    graph = ox.HipGraphExec.capture(stream, lambda: step(stream))
+    for run in (lambda: step(stream), lambda: graph.launch(stream), lambda: graph.launch(stream)):
+        reset()
+        run()
+        torch.cuda.synchronize()
+        for a, b in zip(p + m, want):
+            assert torch.equal(a, b)

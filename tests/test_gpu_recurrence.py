@@ -1,0 +1,326 @@
+"""The gated linear recurrence and its gradients on the device against the formulas in float64.
+
+Tolerances, with u = 2^-24.  A gate's two values carry the rounding of exp's scaled argument (|g|
+log2(e) u relative to exp(-|g|), which is at most 0.54 u log2(e) of the value itself for the larger
+one and |g| 1.45 u for the smaller), of exp, of the reciprocal and two products: below 24 u for the
+|g| <= 10 here.  Every step of a serial or composed sum adds two roundings.  So a term that passes
+through n steps has a relative error below 32 n u, and the error of h_t is below 32 u e_t with
+e_t = a_t e_{t-1} + (a_t |h_{t-1}| + (1 - a_t) |u_t|) in magnitudes; likewise for l_t backwards.  A
+bfloat16 result has half a unit of 2^-8 more."""
+
+import numpy as np
+import pytest
+import torch
+
+import oxide_hip as ox
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16}
+# batch, time, channels
+SHAPES = [(1, 1, 1), (3, 1, 65), (64, 1, 256), (2, 2, 64), (2, 7, 130), (1, 63, 33), (3, 64, 128),
+          (2, 65, 72), (1, 129, 1000), (5, 200, 31), (1, 2500, 24), (1, 4099, 96), (40, 17, 512),
+          (2, 1000, 2056), (1, 20000, 8)]
+
+
+def make(shape, dtype, dev, seed, scale=1.0, mean=0.0, offset=0):
+    g = torch.Generator().manual_seed(seed)
+    n = int(np.prod(shape))
+    flat = torch.zeros(n + offset, dtype=dtype, device=dev)
+    flat[offset:] = (torch.randn(n, generator=g) * scale + mean).to(dev).to(dtype)
+    return flat[offset:].view(shape)
+
+
+def f64(t):
+    return t.detach().cpu().double().numpy()
+
+
+def gates(shape, dtype, dev, seed, offset=0):
+    return make(shape, dtype, dev, seed, 1.5, 2.0, offset).clamp_(-10, 10)
+
+
+def lengths_of(batch, time, dev, seed=9):
+    n = np.random.default_rng(seed).integers(0, time + 1, batch)
+    n[0] = time
+    if batch > 1:
+        n[-1] = 0
+    return torch.from_numpy(n.astype(np.int32)).to(dev)
+
+
+def within(got, ref, magnitude, dtype, what):
+    tol = 32 * U * magnitude + (2.0 ** -8 * np.abs(ref) if dtype == torch.bfloat16 else 0.0)
+    bad = ~(np.abs(f64(got) - ref) <= tol + 1e-37)
+    assert not bad.any(), (what, int(bad.sum()), np.argwhere(bad)[:3],
+                           np.nanmax(np.abs(f64(got) - ref)))
+
+
+def forward_ref(u, g, state, lengths):
+    batch, time, channels = u.shape
+    u6, keep, take = f64(u), 1 / (1 + np.exp(-f64(g))), 1 / (1 + np.exp(f64(g)))
+    h = np.zeros((batch, channels)) if state is None else f64(state)
+    e, n = np.zeros_like(h), [time] * batch if lengths is None else lengths.tolist()
+    out, err = np.zeros_like(u6), np.zeros_like(u6)
+    for t in range(time):
+        for i in range(batch):
+            if t >= n[i]:
+                continue
+            e[i] = keep[i, t] * (e[i] + np.abs(h[i])) + take[i, t] * np.abs(u6[i, t])
+            h[i] = keep[i, t] * h[i] + take[i, t] * u6[i, t]
+            out[i, t], err[i, t] = h[i], e[i]
+    return out, err, h, e
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("ragged", [False, True])
+def test_forward(module, dev, shape, dtype, ragged):
+    t = TYPES[dtype]
+    u, g = make(shape, t, dev, 1), gates(shape, t, dev, 2)
+    state = make((shape[0], shape[2]), torch.float32, dev, 3)
+    lengths = lengths_of(shape[0], shape[1], dev) if ragged else None
+    h, final = torch.empty_like(u), torch.empty_like(state)
+    module.gated_recurrence_forward(u, g, h, initial_state=state, final_state=final,
+                                    lengths=lengths)
+    ref, err, ref_final, err_final = forward_ref(u, g, state, lengths)
+    within(h, ref, err, t, "output")
+    within(final, ref_final, err_final, torch.float32, "final state")
+
+
+def backward_ref(dh, u, g, h, state, dfinal, lengths):
+    batch, time, channels = u.shape
+    keep, take = 1 / (1 + np.exp(-f64(g))), 1 / (1 + np.exp(f64(g)))
+    dh6, u6, h6 = f64(dh), f64(u), f64(h)
+    s6 = np.zeros((batch, channels)) if state is None else f64(state)
+    back = np.zeros((batch, channels)) if dfinal is None else f64(dfinal)
+    size, err = np.abs(back), np.zeros_like(back)
+    n = [time] * batch if lengths is None else lengths.tolist()
+    out = [np.zeros_like(u6) for _ in range(4)]
+    for i in range(batch):
+        for t in range(n[i] - 1, -1, -1):
+            back[i] += dh6[i, t]
+            size[i] += np.abs(dh6[i, t])
+            err[i] += size[i]
+            before = h6[i, t - 1] if t else s6[i]
+            out[0][i, t] = take[i, t] * back[i]
+            out[1][i, t] = take[i, t] * err[i]
+            out[2][i, t] = keep[i, t] * take[i, t] * (before - u6[i, t]) * back[i]
+            out[3][i, t] = keep[i, t] * take[i, t] * (np.abs(before) + np.abs(u6[i, t])) * err[i]
+            back[i] *= keep[i, t]
+            size[i] *= keep[i, t]
+            err[i] = keep[i, t] * err[i]
+    return out, back, err + size
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("ragged", [False, True])
+def test_backward(module, dev, shape, dtype, ragged):
+    t = TYPES[dtype]
+    dh, u, g, h = (make(shape, t, dev, 1), make(shape, t, dev, 2), gates(shape, t, dev, 3),
+                   make(shape, t, dev, 4))
+    state, dfinal = (make((shape[0], shape[2]), torch.float32, dev, k) for k in (5, 6))
+    lengths = lengths_of(shape[0], shape[1], dev) if ragged else None
+    du, dg, ds = torch.empty_like(u), torch.empty_like(u), torch.empty_like(state)
+    module.gated_recurrence_backward(dh, u, g, h, du, dg, initial_state=state,
+                                     final_state_gradient=dfinal, initial_state_gradient=ds,
+                                     lengths=lengths)
+    (rdu, edu, rdg, edg), rds, eds = backward_ref(dh, u, g, h, state, dfinal, lengths)
+    within(du, rdu, edu, t, "input gradient")
+    within(dg, rdg, edg, t, "gate gradient")
+    within(ds, rds, eds, torch.float32, "state gradient")
+
+
+def test_without_states(module, dev):
+    shape = (3, 150, 70)
+    u, g = make(shape, torch.float32, dev, 1), gates(shape, torch.float32, dev, 2)
+    h = torch.empty_like(u)
+    module.gated_recurrence_forward(u, g, h)
+    ref, err, _, _ = forward_ref(u, g, None, None)
+    within(h, ref, err, torch.float32, "output")
+    dh, du, dg = make(shape, torch.float32, dev, 3), torch.empty_like(u), torch.empty_like(u)
+    module.gated_recurrence_backward(dh, u, g, h, du, dg)
+    (rdu, edu, rdg, edg), _, _ = backward_ref(dh, u, g, h, None, None, None)
+    within(du, rdu, edu, torch.float32, "input gradient")
+    within(dg, rdg, edg, torch.float32, "gate gradient")
+
+
+@pytest.mark.parametrize("shape", [(4, 1, 100), (2, 300, 64), (1, 5000, 40)])
+def test_state_in_place(module, dev, shape):
+    """The final state over the initial one, the state's gradient over the final's."""
+    u, g = make(shape, torch.float32, dev, 1), gates(shape, torch.float32, dev, 2)
+    state = make((shape[0], shape[2]), torch.float32, dev, 3)
+    want, h2 = torch.empty_like(state), torch.empty_like(u)
+    h, kept = torch.empty_like(u), state.clone()
+    module.gated_recurrence_forward(u, g, h2, initial_state=state, final_state=want)
+    module.gated_recurrence_forward(u, g, h, initial_state=kept, final_state=kept)
+    assert torch.equal(kept, want) and torch.equal(h, h2)
+    back, ds = state.clone(), torch.empty_like(state)
+    a, b = torch.empty_like(u), torch.empty_like(u)
+    module.gated_recurrence_backward(u, u, g, h, a, b, final_state_gradient=state,
+                                     initial_state_gradient=ds)
+    module.gated_recurrence_backward(u, u, g, h, a, b, final_state_gradient=back,
+                                     initial_state_gradient=back)
+    assert torch.equal(back, ds)
+
+
+def test_token_by_token_equals_the_whole(module, dev):
+    """A sequence in one call and one token at a time with the state in place."""
+    shape = (3, 40, 48)
+    u, g = make(shape, torch.float32, dev, 1), gates(shape, torch.float32, dev, 2)
+    h, final = torch.empty_like(u), torch.empty(3, 48, device=dev)
+    module.gated_recurrence_forward(u, g, h, final_state=final)
+    state, one = torch.zeros(3, 48, device=dev), torch.empty(3, 1, 48, device=dev)
+    _, err, _, _ = forward_ref(u, g, None, None)
+    for t in range(40):
+        module.gated_recurrence_forward(u[:, t:t + 1].contiguous(), g[:, t:t + 1].contiguous(),
+                                        one, initial_state=state, final_state=state)
+        within(one[:, 0], f64(h[:, t]), 2 * err[:, t], torch.float32, t)
+    within(state, f64(final), 2 * err[:, -1], torch.float32, "final state")
+
+
+@pytest.mark.parametrize("shape", [(4, 9, 50), (3, 700, 64), (2, 6000, 24)])
+@pytest.mark.parametrize("poison", [float("nan"), float("inf"), -3.4e38])
+def test_masked_places_may_hold_anything(module, dev, shape, poison):
+    u, g = make(shape, torch.float32, dev, 1), gates(shape, torch.float32, dev, 2)
+    state = make((shape[0], shape[2]), torch.float32, dev, 3)
+    n = lengths_of(shape[0], shape[1], dev)
+    dh, h = make(shape, torch.float32, dev, 4), torch.empty_like(u)
+    final, outs = torch.empty_like(state), [torch.empty_like(u) for _ in range(2)]
+    ds = torch.empty_like(state)
+    masked = (torch.arange(shape[1], device=dev)[None] >= n[:, None])[:, :, None]
+
+    def run(u, g, dh):
+        module.gated_recurrence_forward(u, g, h, initial_state=state, final_state=final,
+                                        lengths=n)
+        hp = torch.where(masked, poison, h)
+        module.gated_recurrence_backward(dh, u, g, hp, *outs, initial_state=state,
+                                         final_state_gradient=state, initial_state_gradient=ds,
+                                         lengths=n)
+        return [t.clone() for t in (h, final, *outs, ds)]
+
+    want = run(u, g, dh)
+    got = run(*(torch.where(masked, poison, t) for t in (u, g, dh)))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    assert (want[0][-1] == 0).all() and torch.equal(want[1][-1], state[-1])
+    assert torch.equal(want[4][-1], state[-1])
+
+
+def test_gates_at_their_limits(module, dev):
+    """A closed gate keeps the state, an open one takes the input; what is not finite stays in
+    its channel and does not reach earlier steps."""
+    u = make((1, 90, 64), torch.float32, dev, 1)
+    state = make((1, 64), torch.float32, dev, 2)
+    h = torch.empty_like(u)
+    for g, want in ((float("inf"), state[:, None].expand(1, 90, 64)), (float("-inf"), u),
+                    (200.0, state[:, None].expand(1, 90, 64)), (-200.0, u)):
+        module.gated_recurrence_forward(u, torch.full_like(u, g), h, initial_state=state)
+        assert torch.equal(h, want)
+    gate = gates((1, 90, 64), torch.float32, dev, 3)
+    clean = torch.empty_like(u)
+    module.gated_recurrence_forward(u, gate, clean, initial_state=state)
+    v = u.clone()
+    v[0, 40, 5] = float("nan")
+    module.gated_recurrence_forward(v, gate, h, initial_state=state)
+    hit = h.isnan()
+    assert hit[0, 40:, 5].all() and int(hit.sum()) == 50
+    assert torch.equal(h[~hit], clean[~hit])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("offset", [1, 2, 4])
+def test_other_alignments(module, dev, dtype, offset):
+    t, shape = TYPES[dtype], (2, 300, 64)
+    u, g = make(shape, t, dev, 1, offset=offset), gates(shape, t, dev, 2)
+    h = make(shape, t, dev, 3, offset=offset)
+    state = make((2, 64), torch.float32, dev, 4, offset=offset)
+    final = torch.empty(2, 64, device=dev)
+    module.gated_recurrence_forward(u, g, h, initial_state=state, final_state=final)
+    ref, err, ref_final, err_final = forward_ref(u, g, state, None)
+    within(h, ref, err, t, "output")
+    within(final, ref_final, err_final, torch.float32, "final state")
+    du, dg = make(shape, t, dev, 5, offset=offset), torch.empty_like(g)
+    dh = make(shape, t, dev, 6)
+    module.gated_recurrence_backward(dh, u, g, h, du, dg, initial_state=state)
+    (rdu, edu, rdg, edg), _, _ = backward_ref(dh, u, g, h, state, None, None)
+    within(du, rdu, edu, t, "input gradient")
+    within(dg, rdg, edg, t, "gate gradient")
+
+
+def test_gradient_against_differences(module, dev):
+    """The gradients of sum(c h) + sum(k final) along random directions against central
+    differences of the kernel's own forward: step 2^-7, truncation of the order of its square and
+    rounding of 64 u / step of the magnitudes; 1e-3 covers both."""
+    shape, step = (2, 60, 33), 2.0 ** -7
+    u, g = make(shape, torch.float32, dev, 1), gates(shape, torch.float32, dev, 2)
+    state = make((2, 33), torch.float32, dev, 3)
+    c, k = make(shape, torch.float32, dev, 4), make((2, 33), torch.float32, dev, 5)
+    vu, vg = make(shape, torch.float32, dev, 6), make(shape, torch.float32, dev, 7)
+    vs = make((2, 33), torch.float32, dev, 8)
+    h, final = torch.empty_like(u), torch.empty_like(state)
+
+    def loss(s):
+        module.gated_recurrence_forward(u + s * vu, g + s * vg, h, initial_state=state + s * vs,
+                                        final_state=final)
+        return float((f64(h) * f64(c)).sum() + (f64(final) * f64(k)).sum())
+
+    numeric = (loss(step) - loss(-step)) / (2 * step)
+    loss(0.0)
+    du, dg, ds = torch.empty_like(u), torch.empty_like(u), torch.empty_like(state)
+    module.gated_recurrence_backward(c, u, g, h, du, dg, initial_state=state,
+                                     final_state_gradient=k, initial_state_gradient=ds)
+    parts = [f64(a) * f64(b) for a, b in ((du, vu), (dg, vg), (ds, vs))]
+    assert abs(numeric - sum(p.sum() for p in parts)) <= \
+        1e-3 * sum(np.abs(p).sum() for p in parts)
+
+
+def test_empty(module, dev):
+    """No steps leave the state; no rows or channels do nothing; lengths are clamped."""
+    state, final = torch.randn(2, 8, device=dev), torch.empty(2, 8, device=dev)
+    nothing = torch.empty(2, 0, 8, device=dev)
+    module.gated_recurrence_forward(nothing, nothing, torch.empty_like(nothing),
+                                    initial_state=state, final_state=final)
+    assert torch.equal(state, final)
+    module.gated_recurrence_backward(nothing, nothing, nothing, nothing,
+                                     torch.empty_like(nothing), torch.empty_like(nothing),
+                                     final_state_gradient=state, initial_state_gradient=final)
+    assert torch.equal(state, final)
+    for shape in ((0, 5, 8), (2, 5, 0)):
+        z = torch.empty(shape, device=dev)
+        module.gated_recurrence_forward(z, z.clone(), z.clone())
+    u = torch.randn(2, 5, 8, device=dev)
+    h, want = torch.empty_like(u), torch.empty_like(u)
+    n = torch.tensor([-3, 1000], dtype=torch.int32, device=dev)
+    module.gated_recurrence_forward(u, u.clone(), want)
+    module.gated_recurrence_forward(u, u.clone(), h, lengths=n)
+    assert (h[0] == 0).all() and torch.equal(h[1], want[1])
+
+
+@pytest.mark.parametrize("shape", [(2, 500, 200), (1, 9000, 64)])
+def test_another_stream_a_graph_and_repeats(module, dev, shape):
+    u, g = make(shape, torch.bfloat16, dev, 1), gates(shape, torch.bfloat16, dev, 2)
+    state = make((shape[0], shape[2]), torch.float32, dev, 3)
+    h, final = torch.empty_like(u), torch.empty_like(state)
+    du, dg, ds = torch.empty_like(u), torch.empty_like(u), torch.empty_like(state)
+    outs = (h, final, du, dg, ds)
+
+    def both(stream=None):
+        module.gated_recurrence_forward(u, g, h, initial_state=state, final_state=final,
+                                        stream=stream)
+        module.gated_recurrence_backward(u, u, g, h, du, dg, initial_state=state,
+                                         final_state_gradient=state, initial_state_gradient=ds,
+                                         stream=stream)
+
+    both()
+    torch.cuda.synchronize()
+    want = [t.clone() for t in outs]
+    stream = torch.cuda.Stream()
+    graph = ox.HipGraphExec.capture(stream, lambda: both(stream))
+    for run in (lambda: both(stream), lambda: graph.launch(stream), lambda: graph.launch(stream)):
+        for t in outs:
+            t.zero_()
+        torch.cuda.synchronize()
+        run()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, want):
+            assert torch.equal(a, b)

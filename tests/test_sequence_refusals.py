@@ -1,0 +1,191 @@
+"""What the sequence operators refuse on the host, before any launch (the pointers are never
+followed)."""
+
+import ctypes
+
+import numpy as np
+import pytest
+
+import oxide_hip as ox
+
+BASE = 1 << 30
+STEP = 1 << 24
+
+
+def places(n):
+    return [BASE + i * STEP for i in range(n)]
+
+
+def refused(status, text, kind=ox.INVALID_SHAPE):
+    assert status == kind, (status, ox.lib().oxh_last_error())
+    assert text in ox.lib().oxh_last_error(), ox.lib().oxh_last_error()
+
+
+def norm_forward(**k):
+    x, r, w, s, y, q = places(6)
+    a = dict(dtype=0, rows=4, columns=8, epsilon=1e-6, x=x, r=r, w=w, s=s, y=y, q=q) | k
+    return ox.lib().oxh_rms_norm_forward(None, a["dtype"], a["rows"], a["columns"], a["epsilon"],
+                                         a["x"], a["r"], a["w"], a["s"], a["y"], a["q"])
+
+
+def test_rms_norm_forward():
+    x, r, w, s, y, q = places(6)
+    refused(norm_forward(dtype=2), b"dtype")
+    refused(norm_forward(columns=0), b"columns")
+    refused(norm_forward(rows=1 << 31), b"rows")
+    for eps in (-1e-6, float("nan"), float("inf")):
+        refused(norm_forward(epsilon=eps), b"epsilon", ox.EXECUTION)
+    for name in ("x", "w", "y"):
+        refused(norm_forward(**{name: None}), b"null")
+    refused(norm_forward(x=x + 2), b"aligned")
+    refused(norm_forward(dtype=1, y=y + 1), b"aligned")
+    refused(norm_forward(y=x), b"overlaps")
+    refused(norm_forward(y=s + 4), b"overlaps")
+    refused(norm_forward(s=x + 4), b"partially overlaps")
+    refused(norm_forward(s=r - 4), b"partially overlaps")
+    refused(norm_forward(q=y), b"overlaps")
+    assert norm_forward(rows=0, x=None, y=None) == ox.OK
+
+
+def norm_backward(**k):
+    g, sg, s, w, q, dx, dw, ws = places(8)
+    a = dict(dtype=0, rows=4, columns=8, g=g, sg=sg, s=s, w=w, q=q, dx=dx, dw=dw, ws=ws,
+             n=ox.rms_norm_backward_workspace_size(4, 8)) | k
+    return ox.lib().oxh_rms_norm_backward(None, a["dtype"], a["rows"], a["columns"], a["g"],
+                                          a["sg"], a["s"], a["w"], a["q"], a["dx"], a["dw"],
+                                          a["ws"], a["n"])
+
+
+def test_rms_norm_backward():
+    g, sg, s, w, q, dx, dw, ws = places(8)
+    for name in ("g", "s", "w", "q", "dx"):
+        refused(norm_backward(**{name: None}), b"null")
+    refused(norm_backward(n=0), b"workspace")
+    refused(norm_backward(ws=None), b"workspace")
+    refused(norm_backward(ws=ws + 4), b"workspace")
+    refused(norm_backward(dx=g), b"overlaps")
+    refused(norm_backward(dx=s), b"overlaps")
+    refused(norm_backward(dx=sg + 4), b"overlaps")
+    refused(norm_backward(dw=w), b"overlaps")
+    refused(norm_backward(dw=dx), b"overlap")
+    refused(norm_backward(ws=s), b"overlaps")
+    with pytest.raises(ox.OxideError):
+        ox.rms_norm_backward_workspace_size(4, 0)
+
+
+def scan_forward(**k):
+    u, g, st, n, h, f, ws = places(7)
+    a = dict(dtype=0, batch=2, time=3, channels=8, u=u, g=g, st=st, n=n, h=h, f=f, ws=ws,
+             bytes=ox.gated_recurrence_workspace_size(2, 3, 8)) | k
+    return ox.lib().oxh_gated_recurrence_forward(
+        None, a["dtype"], a["batch"], a["time"], a["channels"], a["u"], a["g"], a["st"], a["n"],
+        a["h"], a["f"], a["ws"], a["bytes"])
+
+
+def test_gated_recurrence_forward():
+    u, g, st, n, h, f, ws = places(7)
+    refused(scan_forward(dtype=7), b"dtype")
+    refused(scan_forward(batch=65536), b"batch")
+    refused(scan_forward(time=1 << 31), b"time")
+    refused(scan_forward(batch=65535, time=(1 << 31) - 1, channels=(1 << 31) - 1), b"overflow")
+    for name in ("u", "g", "h"):
+        refused(scan_forward(**{name: None}), b"null")
+    refused(scan_forward(u=u + 2), b"aligned")
+    refused(scan_forward(n=n + 2), b"aligned")
+    refused(scan_forward(bytes=0), b"workspace")
+    refused(scan_forward(h=u), b"overlaps")
+    refused(scan_forward(f=st + 4), b"overlaps")
+    refused(scan_forward(f=h), b"overlap")
+    refused(scan_forward(ws=g), b"overlap")
+    assert scan_forward(batch=0, u=None) == ox.OK
+    assert scan_forward(channels=0, u=None) == ox.OK
+
+
+def scan_backward(**k):
+    dh, u, g, h, st, df, n, du, dg, ds, ws = places(11)
+    a = dict(dtype=0, dh=dh, u=u, g=g, h=h, st=st, df=df, n=n, du=du, dg=dg, ds=ds, ws=ws,
+             bytes=ox.gated_recurrence_workspace_size(2, 3, 8)) | k
+    return ox.lib().oxh_gated_recurrence_backward(
+        None, a["dtype"], 2, 3, 8, a["dh"], a["u"], a["g"], a["h"], a["st"], a["df"], a["n"],
+        a["du"], a["dg"], a["ds"], a["ws"], a["bytes"])
+
+
+def test_gated_recurrence_backward():
+    dh, u, g, h, st, df, n, du, dg, ds, ws = places(11)
+    for name in ("dh", "u", "g", "h", "du", "dg"):
+        refused(scan_backward(**{name: None}), b"null")
+    refused(scan_backward(dtype=1, dg=dg + 1), b"aligned")
+    refused(scan_backward(ws=None), b"workspace")
+    for bad in (dh, u, g, h):
+        refused(scan_backward(du=bad), b"overlaps")
+        refused(scan_backward(dg=bad + 4), b"overlaps")
+    refused(scan_backward(du=dg), b"overlap")
+    refused(scan_backward(ds=df + 4), b"overlaps")
+    refused(scan_backward(ds=st), b"overlaps")
+
+
+def test_orthogonalize():
+    x, y, ws = places(3)
+    lib, need = ox.lib(), ox.orthogonalize_workspace_size(2, 30, 40)
+
+    def call(count=2, rows=30, columns=40, rounds=5, eps=1e-7, x=x, y=y, ws=ws, n=need):
+        return lib.oxh_orthogonalize(None, count, rows, columns, rounds, eps, x, y, ws, n)
+
+    refused(call(rows=0), b"empty")
+    refused(call(rows=65537, columns=65537), b"too large")
+    refused(call(rows=(1 << 20) + 1), b"too large")
+    refused(call(rows=8192, columns=(1 << 20)), b"too large")
+    refused(call(rounds=0), b"rounds")
+    refused(call(rounds=65), b"rounds")
+    for eps in (0.0, -1.0, float("nan")):
+        refused(call(eps=eps), b"epsilon", ox.EXECUTION)
+    refused(call(x=None), b"null")
+    refused(call(y=y + 2), b"misaligned")
+    refused(call(n=need - 1), b"workspace")
+    refused(call(ws=ws + 8), b"workspace")
+    refused(call(y=x), b"overlap")
+    refused(call(ws=x), b"overlap")
+    assert call(count=0, x=None, ws=None) == ox.OK
+
+
+def test_muon():
+    p, g, m, ws = places(4)
+    lib = ox.lib()
+
+    def call(entries=((p, g, m, 30, 40),), lr=0.1, wd=0.0, mu=0.9, eps=1e-7, rounds=5, ws=ws,
+             n=None):
+        table = (ox.MuonTensor * len(entries))(*[ox.MuonTensor(*e) for e in entries])
+        if n is None:
+            out = ctypes.c_uint64()
+            if lib.oxh_muon_workspace_size(table, len(entries), ctypes.byref(out)) != ox.OK:
+                return ox.INVALID_SHAPE
+            n = out.value
+        return lib.oxh_muon_multi_tensor(None, lr, wd, mu, 1, eps, rounds, table, len(entries), ws,
+                                         n)
+
+    for k in ({"lr": float("nan")}, {"wd": float("inf")}, {"mu": float("nan")}):
+        refused(call(**k), b"finite")
+    refused(call(eps=0.0), b"epsilon", ox.EXECUTION)
+    refused(call(rounds=0), b"rounds")
+    refused(call(((p, g, m, 0, 40),)), b"empty")
+    refused(call(((p, g, None, 30, 40),)), b"null")
+    refused(call(((p + 1, g, m, 30, 40),)), b"misaligned")
+    refused(call(n=16), b"workspace")
+    refused(call(((p, p, m, 30, 40),)), b"overlaps")
+    refused(call(((p, g, p + 400, 30, 40),)), b"overlaps")
+    refused(call(((p, g, m, 30, 40), (p + 4000, g + 8000, m + 8000, 30, 40))), b"overlaps")
+    refused(call(ws=m), b"overlaps")
+    assert call((), ws=None) == ox.OK
+
+
+def test_front_end_checks_shapes():
+    """The Python front end refuses before it reaches the library."""
+    torch = pytest.importorskip("torch")
+    z = torch.zeros
+    with pytest.raises(ox.OxideError):
+        ox.muon_table([(z(3), z(3), z(3))])
+    with pytest.raises(ox.OxideError):
+        ox.muon_table([(z(3, 4), z(3, 5), z(3, 4))])
+    with pytest.raises(ox.OxideError):  # host tensors
+        ox._activation((z(2, 3),), (2, 3), "rms_norm")
+    assert np.isfinite(ox.gated_recurrence_workspace_size(1, 1, 1))
