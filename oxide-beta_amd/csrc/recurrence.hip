@@ -10,7 +10,9 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <string>
+#include <type_traits>
 
 #include "common.h"
 #include "storage.h"
@@ -20,25 +22,32 @@ namespace {
 using oxh::storage::bf16;
 using oxh::storage::widen;
 
-// sigmoid(g) and 1 - sigmoid(g), each to a few roundings however small: with e = exp(-|g|), they
-// are 1 / (1 + e) and e / (1 + e), the larger one for the sign of g first.
+// sigmoid(g) and 1 - sigmoid(g), each to a few roundings however small: with e = exp(-g) they are
+// r = 1 / (1 + e) and e r, the latter as 1 - r (exact enough above 1/2) where g < 0, since e may
+// overflow there.
 struct Gate {
   float keep, take;
 };
 __device__ __forceinline__ Gate gate_of(float g) {
-  const float e = __expf(-fabsf(g));
-  const float large = __builtin_amdgcn_rcpf(1.0f + e), small = e * large;
-  return g >= 0.0f ? Gate{large, small} : Gate{small, large};
+  const float e = __builtin_amdgcn_exp2f(g * -1.44269504f);
+  const float r = __builtin_amdgcn_rcpf(1.0f + e);
+  return {r, g < 0.0f ? 1.0f - r : e * r};
 }
 
+// Both directions run h -> keep h + add over their steps in the order taken (backwards in time
+// for the gradients, where h is a_{t+1} l_{t+1}, the gradient that reaches step t from later ones,
+// and add = a_t dh_t).
 template <typename T>
-struct Forward {
-  const T *u, *g;
-  const float *state;
-  T *h;
-  float *final;
+struct Args {
+  const T *u, *g, *h, *dh;  // forward: u, g
+  T *out, *dg;              // h, or du and dg
+  const float *first;       // the state before the first step taken, or null
+  const float *origin;      // backward: h before step 0, or null
+  float *last;              // the one after the last, or null
   const int32_t *lengths;
-  uint32_t time, channels;
+  float *parts;  // per batch row: entry 0 the first state, entry s + 1 segment s's (keep, add)
+  uint32_t time, channels, groups;  // groups: blocks across the channels
+  uint32_t segments, steps;         // steps per segment
 };
 
 __device__ __forceinline__ uint32_t length_of(const int32_t *lengths, uint32_t row,
@@ -48,58 +57,346 @@ __device__ __forceinline__ uint32_t length_of(const int32_t *lengths, uint32_t r
   return n < 0 ? 0u : min(static_cast<uint32_t>(n), time);
 }
 
-template <typename T>
-__global__ __launch_bounds__(64) void recurrence_forward_kernel(Forward<T> a) {
-  const uint32_t c = blockIdx.x * 64 + threadIdx.x, row = blockIdx.y;
-  if (c >= a.channels) return;
-  const uint32_t n = length_of(a.lengths, row, a.time);
-  const uint64_t at = static_cast<uint64_t>(row) * a.channels + c;
-  uint64_t i = static_cast<uint64_t>(row) * a.time * a.channels + c;
-  float h = a.state != nullptr ? a.state[at] : 0.0f;
-  for (uint32_t t = 0; t < n; ++t, i += a.channels) {
-    const Gate k = gate_of(widen(a.g[i]));
-    h = fmaf(k.keep, h, k.take * widen(a.u[i]));
-    a.h[i] = static_cast<T>(h);
-  }
-  for (uint32_t t = n; t < a.time; ++t, i += a.channels) a.h[i] = static_cast<T>(0.0f);
-  if (a.final != nullptr) a.final[at] = h;
+template <typename T, int V>
+using Raw = typename oxh::storage::Pack<T, V>::type;
+
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> raw_load(const T *p) {
+  return *reinterpret_cast<const Raw<T, V> *>(p);
+}
+template <typename T, int V>
+__device__ __forceinline__ float part_of(const Raw<T, V> &x, int v) {
+  if constexpr (V == 1) return widen(x);
+  else return widen(x[v]);
 }
 
-template <typename T>
-struct Backward {
-  const T *dh, *u, *g, *h;
-  const float *state, *dfinal;
-  T *du, *dg;
-  float *dstate;
-  const int32_t *lengths;
-  uint32_t time, channels;
+// A map h -> a h + b of V channels.
+template <int V>
+struct Map {
+  float a[V], b[V];
+  __device__ __forceinline__ void identity() {
+#pragma unroll
+    for (int v = 0; v < V; ++v) a[v] = 1.0f, b[v] = 0.0f;
+  }
+  // this map after `before`
+  __device__ __forceinline__ void after(const Map &before) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      b[v] = fmaf(a[v], before.b[v], b[v]);
+      a[v] *= before.a[v];
+    }
+  }
 };
 
-template <typename T>
-__global__ __launch_bounds__(64) void recurrence_backward_kernel(Backward<T> a) {
-  const uint32_t c = blockIdx.x * 64 + threadIdx.x, row = blockIdx.y;
-  if (c >= a.channels) return;
+// The maps of all threads that share channels composed in time order.  A block is W waves of
+// 64 / Lanes time groups of Lanes threads; `mine` becomes the composition of the groups before
+// this thread's, and the whole block's is returned.  `shared` [W][2][Lanes * V]; two buffers in
+// turn need one barrier per call.
+template <int V, int Lanes, int W>
+__device__ __forceinline__ Map<V> scan_groups(Map<V> &mine, float *shared) {
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane % Lanes;
+  Map<V> upto = mine;
+#pragma unroll
+  for (int d = Lanes; d < 64; d *= 2) {
+    Map<V> before;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      before.a[v] = __shfl_up(upto.a[v], d);
+      before.b[v] = __shfl_up(upto.b[v], d);
+    }
+    if (lane >= static_cast<uint32_t>(d)) upto.after(before);
+  }
+  if constexpr (W > 1) {
+    if (lane >= 64 - Lanes) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        shared[(wave * 2) * Lanes * V + c * V + v] = upto.a[v];
+        shared[(wave * 2 + 1) * Lanes * V + c * V + v] = upto.b[v];
+      }
+    }
+  }
+  // exclusive within the wave
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    mine.a[v] = Lanes < 64 ? __shfl_up(upto.a[v], Lanes & 63) : 1.0f;
+    mine.b[v] = Lanes < 64 ? __shfl_up(upto.b[v], Lanes & 63) : 0.0f;
+  }
+  if (lane < Lanes) mine.identity();
+  if constexpr (W == 1) {
+    Map<V> all;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      all.a[v] = Lanes < 64 ? __shfl(upto.a[v], 64 - Lanes + c) : upto.a[v];
+      all.b[v] = Lanes < 64 ? __shfl(upto.b[v], 64 - Lanes + c) : upto.b[v];
+    }
+    return all;
+  } else {
+    __syncthreads();
+    Map<V> all;
+    all.identity();
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      if (w == static_cast<int>(wave)) mine.after(all);
+      Map<V> next;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        next.a[v] = shared[(w * 2) * Lanes * V + c * V + v];
+        next.b[v] = shared[(w * 2 + 1) * Lanes * V + c * V + v];
+      }
+      next.after(all);
+      all = next;
+    }
+    return all;
+  }
+}
+
+struct Place {
+  uint32_t row, segment, channel;
+  bool in;  // the thread's channels exist
+};
+template <int V, int Lanes>
+__device__ __forceinline__ Place place_of(uint32_t groups, uint32_t segments, uint32_t channels) {
+  const uint32_t group = blockIdx.x % groups, rest = blockIdx.x / groups;
+  Place p;
+  p.segment = rest % segments;
+  p.row = rest / segments;
+  p.channel = group * Lanes * V + (threadIdx.x % Lanes) * V;
+  p.in = p.channel < channels;
+  return p;
+}
+
+// The steps below the row's length, a range of the steps in the order taken.
+struct Live {
+  uint32_t begin, end;
+};
+template <bool Back, typename T>
+__device__ __forceinline__ Live live_of(const Args<T> &a, uint32_t row) {
   const uint32_t n = length_of(a.lengths, row, a.time);
-  const uint64_t at = static_cast<uint64_t>(row) * a.channels + c;
-  const uint64_t first = static_cast<uint64_t>(row) * a.time * a.channels + c;
-  for (uint32_t t = n; t < a.time; ++t) {
-    const uint64_t i = first + static_cast<uint64_t>(t) * a.channels;
-    a.du[i] = a.dg[i] = static_cast<T>(0.0f);
+  return Back ? Live{a.time - n, a.time} : Live{0, n};
+}
+
+// Offset of the thread's channels at time 0 (of channel 0 for threads without, whose loads then
+// stay in bounds and whose results go nowhere), and of the k-th step taken behind it.
+template <int V, typename T>
+__device__ __forceinline__ uint64_t row_start(const Args<T> &a, const Place &p) {
+  return static_cast<uint64_t>(p.row) * a.time * a.channels + (p.in ? p.channel : 0);
+}
+template <bool Back, typename T>
+__device__ __forceinline__ uint64_t row_of(const Args<T> &a, uint32_t k) {
+  return static_cast<uint64_t>(Back ? a.time - 1 - k : k) * a.channels;
+}
+
+template <int V>
+__device__ __forceinline__ void load_state(const float *p, float (&h)[V]) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) h[v] = p[v];
+}
+template <int V>
+__device__ __forceinline__ void store_state(float *p, const float (&h)[V]) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) p[v] = h[v];
+}
+
+// Where the time axis is split: segment s's map to entry s + 1 of `parts`, and the first state to
+// entry 0.  Each time group takes a run of the segment's steps of its own.
+template <typename T, int V, int Lanes, int W, int S, bool Back>
+__global__ __launch_bounds__(64 * W) void recurrence_parts_kernel(Args<T> a) {
+  __shared__ float shared[W * 2 * Lanes * V];
+  constexpr uint32_t kGroups = 64 / Lanes * W;
+  const Place p = place_of<V, Lanes>(a.groups, a.segments, a.channels);
+  const Live live = live_of<Back>(a, p.row);
+  const uint32_t share = (a.steps + kGroups - 1) / kGroups;
+  const uint32_t first = p.segment * a.steps + threadIdx.x / Lanes * share;
+  const uint32_t begin = max(first, live.begin);
+  const uint32_t end = min(min(first + share, (p.segment + 1) * a.steps), live.end);
+  const T *add = (Back ? a.dh : a.u) + row_start<V>(a, p), *gates = a.g + row_start<V>(a, p);
+  Map<V> map;
+  map.identity();
+  auto step = [&](const Raw<T, V> &x, const Raw<T, V> &g) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const Gate gate = gate_of(part_of<T, V>(g, v));
+      const float b = (Back ? gate.keep : gate.take) * part_of<T, V>(x, v);
+      map.b[v] = fmaf(gate.keep, map.b[v], b);
+      map.a[v] *= gate.keep;
+    }
+  };
+  uint32_t k = begin;
+  for (; k + S <= end; k += S) {
+    Raw<T, V> x[S], g[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const uint64_t at = row_of<Back>(a, k + s);
+      x[s] = raw_load<T, V>(add + at);
+      g[s] = raw_load<T, V>(gates + at);
+    }
+#pragma unroll
+    for (int s = 0; s < S; ++s) step(x[s], g[s]);
   }
-  float l = a.dfinal != nullptr ? a.dfinal[at] : 0.0f;
-  for (uint32_t t = n; t-- > 0;) {
-    const uint64_t i = first + static_cast<uint64_t>(t) * a.channels;
-    const Gate k = gate_of(widen(a.g[i]));
-    const float before = t != 0              ? widen(a.h[i - a.channels])
-                         : a.state != nullptr ? a.state[at]
-                                              : 0.0f;
-    l += widen(a.dh[i]);
-    const float taken = k.take * l;
-    a.du[i] = static_cast<T>(taken);
-    a.dg[i] = static_cast<T>(k.keep * taken * (before - widen(a.u[i])));
-    l *= k.keep;
+  for (; k < end; ++k) {
+    const uint64_t at = row_of<Back>(a, k);
+    step(raw_load<T, V>(add + at), raw_load<T, V>(gates + at));
   }
-  if (a.dstate != nullptr) a.dstate[at] = l;
+  const Map<V> all = scan_groups<V, Lanes, W>(map, shared);
+  if (!p.in || threadIdx.x >= Lanes) return;
+  float *entry = a.parts + (static_cast<uint64_t>(p.row) * (a.segments + 1) + p.segment + 1) * 2 *
+                               a.channels + p.channel;
+  store_state<V>(entry, all.a);
+  store_state<V>(entry + a.channels, all.b);
+  if (p.segment == 0) {
+    float h[V] = {};
+    if (a.first != nullptr)
+      load_state<V>(a.first + static_cast<uint64_t>(p.row) * a.channels + p.channel, h);
+    store_state<V>(entry - a.channels, h);
+  }
+}
+
+// The recurrence over one segment (the whole time axis where it is not split), in tiles of
+// kGroups * S steps: each thread composes its S steps, the block scans the compositions, and each
+// thread runs its steps again from the state that reaches them.  The next tile's operands are
+// loaded before the present one's work.
+template <typename T, int V, int Lanes, int W, int S, bool Back>
+__global__ __launch_bounds__(64 * W) void recurrence_kernel(Args<T> a) {
+  __shared__ float shared[2][W * 2 * Lanes * V];
+  constexpr uint32_t kGroups = 64 / Lanes * W, kTile = kGroups * S;
+  const Place p = place_of<V, Lanes>(a.groups, a.segments, a.channels);
+  const Live live = live_of<Back>(a, p.row);
+  const uint32_t group = threadIdx.x / Lanes;
+  const uint64_t row = row_start<V>(a, p);
+  const uint64_t state = static_cast<uint64_t>(p.row) * a.channels + (p.in ? p.channel : 0);
+  float h[V] = {};  // before the tile
+  int turn = 0;
+  if (a.segments > 1) {
+    // the entries before this segment, shared out among the time groups
+    const float *entry = a.parts + static_cast<uint64_t>(p.row) * (a.segments + 1) * 2 * a.channels +
+                         (p.in ? p.channel : 0);
+    const uint32_t share = (p.segment + kGroups - 1) / kGroups;
+    const uint32_t begin = group * share, end = min(begin + share, p.segment);
+    Map<V> map;
+    map.identity();
+    for (uint32_t s = begin; s < end; ++s) {
+      const float *e = entry + static_cast<uint64_t>(s + 1) * 2 * a.channels;
+      Map<V> next;
+      load_state<V>(e, next.a);
+      load_state<V>(e + a.channels, next.b);
+      next.after(map);
+      map = next;
+    }
+    load_state<V>(entry + a.channels, h);
+    const Map<V> all = scan_groups<V, Lanes, W>(map, shared[turn]);
+    turn ^= 1;
+#pragma unroll
+    for (int v = 0; v < V; ++v) h[v] = fmaf(all.a[v], h[v], all.b[v]);
+  } else if (a.first != nullptr) {
+    load_state<V>(a.first + state, h);
+  }
+
+  const uint32_t begin = p.segment * a.steps, end = min(begin + a.steps, a.time);
+  const uint32_t live_end = min(end, live.end);
+  constexpr int kOperands = Back ? 4 : 2;
+  Raw<T, V> next[kOperands][S];
+  auto load_step = [&](int s, uint32_t k) {
+    const uint64_t at = row + row_of<Back>(a, k);
+    next[0][s] = raw_load<T, V>((Back ? a.dh : a.u) + at);
+    next[1][s] = raw_load<T, V>(a.g + at);
+    if constexpr (Back) {
+      next[2][s] = raw_load<T, V>(a.u + at);
+      if (k + 1 != a.time) next[3][s] = raw_load<T, V>(a.h + at - a.channels);
+    }
+  };
+  // whether every step of a tile is live (and, backwards, has a step before it)
+  auto whole = [&](uint32_t tile) {
+    return tile >= live.begin && tile + kTile <= live_end &&
+           (!Back || tile + kTile < a.time);
+  };
+  auto fetch = [&](uint32_t tile) {
+    const uint32_t k = tile + group * S;
+    if (whole(tile)) {
+#pragma unroll
+      for (int s = 0; s < S; ++s) load_step(s, k + s);
+    } else {
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+        if (k + s >= live.begin && k + s < live_end) load_step(s, k + s);
+    }
+  };
+  float keep[S][V], add[S][V], take[S][V], slope[S][V];
+  Map<V> map;
+  auto compose = [&](uint32_t tile, auto all_live) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const uint32_t k = tile + group * S + s;
+      const bool on = decltype(all_live)::value ||
+                      (k >= live.begin && k < live_end);
+      const bool oldest = !decltype(all_live)::value && Back && k + 1 == a.time;
+      float before[V] = {};
+      if (oldest && a.origin != nullptr) load_state<V>(a.origin + state, before);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const Gate gate = gate_of(part_of<T, V>(next[1][s], v));
+        const float x = part_of<T, V>(next[0][s], v);
+        keep[s][v] = on ? gate.keep : 1.0f;
+        if constexpr (Back) {
+          const float prev = oldest ? before[v] : part_of<T, V>(next[3][s], v);
+          add[s][v] = on ? x : 0.0f;  // dh
+          take[s][v] = on ? gate.take : 0.0f;
+          slope[s][v] = on ? prev - part_of<T, V>(next[2][s], v) : 0.0f;
+          map.b[v] = keep[s][v] * (map.b[v] + add[s][v]);
+        } else {
+          add[s][v] = on ? gate.take * x : 0.0f;
+          map.b[v] = fmaf(keep[s][v], map.b[v], add[s][v]);
+        }
+        map.a[v] *= keep[s][v];
+      }
+    }
+  };
+  if (begin < end) fetch(begin);
+  for (uint32_t tile = begin; tile < end; tile += kTile) {
+    const bool all_live = whole(tile);
+    map.identity();
+    if (all_live) compose(tile, std::true_type());
+    else compose(tile, std::false_type());
+    if (tile + kTile < end) fetch(tile + kTile);
+    const Map<V> all = scan_groups<V, Lanes, W>(map, shared[turn]);
+    turn ^= 1;
+    float x[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      x[v] = fmaf(map.a[v], h[v], map.b[v]);
+      h[v] = fmaf(all.a[v], h[v], all.b[v]);
+    }
+    if (!p.in) continue;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const uint32_t k = tile + group * S + s;
+      const bool on = all_live || (k >= live.begin && k < live_end);
+      if (!all_live && k >= end) continue;
+      const uint64_t at = row + row_of<Back>(a, k);
+      float y[V], z[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if constexpr (Back) {  // 0 beyond the length: take and slope are
+          const float l = x[v] + add[s][v];
+          y[v] = take[s][v] * l;
+          z[v] = keep[s][v] * y[v] * slope[s][v];
+          x[v] = keep[s][v] * l;
+        } else {
+          x[v] = fmaf(keep[s][v], x[v], add[s][v]);
+          y[v] = on ? x[v] : 0.0f;
+        }
+      }
+      oxh::storage::store<T, V>(a.out + at, y);
+      if constexpr (Back) oxh::storage::store<T, V>(a.dg + at, z);
+    }
+  }
+  // every thread has read the first state, which may lie where the last one goes
+  __syncthreads();
+  if (a.last != nullptr && p.in && p.segment + 1 == a.segments && group == 0)
+    store_state<V>(a.last + state, h);
+}
+
+std::string message(const char *what, const char *problem) {
+  return std::string(what) + problem;
 }
 
 struct Span {
@@ -109,7 +406,7 @@ struct Span {
 
 // Outputs distinct from the operands and from each other; `same` names pairs that may be the same
 // buffer (not overlap partly).
-oxh_status check_apart(const std::string &what, const Span *in, int ins, const Span *out,
+oxh_status check_apart(const char *what, const Span *in, int ins, const Span *out,
                        int outs, int same_in, int same_out) {
   for (int o = 0; o < outs; ++o) {
     if (out[o].p == nullptr || out[o].n == 0) continue;
@@ -117,12 +414,12 @@ oxh_status check_apart(const std::string &what, const Span *in, int ins, const S
       if (in[i].p == nullptr || in[i].n == 0) continue;
       if (i == same_in && o == same_out && in[i].p == out[o].p) continue;
       OXH_REQUIRE(!oxh::any_overlap(out[o].p, out[o].n, in[i].p, in[i].n), OXH_INVALID_SHAPE,
-                  what + ": an output overlaps an operand");
+                  message(what, ": an output overlaps an operand"));
     }
     for (int k = 0; k < o; ++k)
       OXH_REQUIRE(out[k].p == nullptr || out[k].n == 0 ||
                       !oxh::any_overlap(out[o].p, out[o].n, out[k].p, out[k].n),
-                  OXH_INVALID_SHAPE, what + ": two outputs overlap");
+                  OXH_INVALID_SHAPE, message(what, ": two outputs overlap"));
   }
   return oxh::ok();
 }
@@ -131,32 +428,145 @@ bool aligned_to(const void *p, uint64_t bytes) {
   return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0;
 }
 
-oxh_status check_shape(const std::string &what, int dtype, uint64_t batch, uint64_t time,
+oxh_status check_shape(const char *what, int dtype, uint64_t batch, uint64_t time,
                        uint64_t channels) {
   OXH_REQUIRE(oxh::storage::valid(dtype), OXH_INVALID_SHAPE,
-              what + ": dtype is neither OXH_F32 nor OXH_BF16");
-  OXH_REQUIRE(batch <= 65535, OXH_INVALID_SHAPE, what + ": batch above 65535");
+              message(what, ": dtype is neither OXH_F32 nor OXH_BF16"));
+  OXH_REQUIRE(batch <= 65535, OXH_INVALID_SHAPE, message(what, ": batch above 65535"));
   OXH_REQUIRE(time < (1ull << 31) && channels < (1ull << 31), OXH_INVALID_SHAPE,
-              what + ": time or channels too large");
+              message(what, ": time or channels too large"));
   OXH_REQUIRE(channels == 0 || batch * time <= (1ull << 58) / channels, OXH_INVALID_SHAPE,
-              what + ": element count overflow");
+              message(what, ": element count overflow"));
   return oxh::ok();
 }
 
-template <typename T>
-oxh_status forward(hipStream_t stream, uint64_t batch, const Forward<T> &a) {
-  oxh::launch(recurrence_forward_kernel<T>,
-              dim3((a.channels + 63) / 64, static_cast<uint32_t>(batch)), dim3(64), 0, stream,
-              a);
-  return oxh::launched("gated_recurrence_forward");
+// How a call is laid out: the channels per thread and per block, the steps per thread and tile,
+// and the segments of the time axis.
+struct Plan {
+  int values, lanes;
+  bool brief;
+  uint32_t groups, segments, steps;
+};
+
+constexpr int kBriefTime = 16;
+constexpr int kWaves = 4;
+// steps per thread and tile
+constexpr int steps_of(int values, bool back) { return (values == 1 ? 16 : 8) / (back ? 2 : 1); }
+
+
+Plan plan_of(uint64_t batch, uint64_t time, uint64_t channels, bool packed, bool back) {
+  Plan p;
+  p.values = packed ? 4 : 1;
+  p.brief = time <= kBriefTime;
+  p.lanes = p.brief ? 64 : packed ? (channels <= 32 ? 8 : 16) : (channels <= 32 ? 32 : 64);
+  p.groups = static_cast<uint32_t>((channels + p.lanes * p.values - 1) / (p.lanes * p.values));
+  p.segments = 1;
+  p.steps = static_cast<uint32_t>(time);
+  if (p.brief) return p;
+  const uint64_t tile = 64 / p.lanes * kWaves * steps_of(p.values, back);
+  const uint64_t blocks = batch * p.groups, target = 512;
+  if (blocks >= oxh::kComputeUnits) return p;
+  const uint64_t tiles = (time + tile - 1) / tile;
+  const uint64_t wanted = std::min((target + blocks - 1) / blocks, (tiles + 1) / 2);
+  if (wanted < 2) return p;
+  const uint64_t per = (tiles + wanted - 1) / wanted;
+  p.steps = static_cast<uint32_t>(per * tile);
+  p.segments = static_cast<uint32_t>((tiles + per - 1) / per);
+  return p;
+}
+
+uint64_t parts_bytes(const Plan &p, uint64_t batch, uint64_t channels) {
+  return p.segments == 1 ? 0 : batch * (p.segments + 1) * 2 * channels * 4;
+}
+
+template <typename T, int V, int Lanes, bool Back>
+oxh_status run_split(hipStream_t stream, uint64_t batch, Args<T> a, const char *what) {
+  constexpr int S = steps_of(V, Back);
+  const uint64_t blocks = batch * a.groups * a.segments;
+  if (a.segments > 1) {
+    oxh::launch(recurrence_parts_kernel<T, V, Lanes, kWaves, S, Back>,
+                dim3(static_cast<uint32_t>(blocks)), dim3(64 * kWaves), 0, stream, a);
+    oxh_status st = oxh::launched(what);
+    if (st != OXH_OK) return st;
+  }
+  oxh::launch(recurrence_kernel<T, V, Lanes, kWaves, S, Back>,
+              dim3(static_cast<uint32_t>(blocks)), dim3(64 * kWaves), 0, stream, a);
+  return oxh::launched(what);
+}
+
+template <typename T, bool Back>
+oxh_status run(hipStream_t stream, uint64_t batch, Args<T> a, bool packed, const char *what) {
+  const Plan p = plan_of(batch, a.time, a.channels, packed, Back);
+  a.groups = p.groups;
+  a.segments = p.segments;
+  a.steps = p.steps;
+  const uint64_t blocks = batch * p.groups * p.segments;
+  OXH_REQUIRE(blocks < (1ull << 31), OXH_INVALID_SHAPE, std::string(what) + ": too many rows");
+  if (p.brief) {
+    const dim3 grid(static_cast<uint32_t>(blocks));
+    if (packed) oxh::launch(recurrence_kernel<T, 4, 64, 1, 4, Back>, grid, dim3(64), 0, stream, a);
+    else oxh::launch(recurrence_kernel<T, 1, 64, 1, 4, Back>, grid, dim3(64), 0, stream, a);
+    return oxh::launched(what);
+  }
+  if (packed)
+    switch (p.lanes) { case 8: return run_split<T, 4, 8, Back>(stream, batch, a, what);
+      case 16: return run_split<T, 4, 16, Back>(stream, batch, a, what);
+      case 32: return run_split<T, 4, 32, Back>(stream, batch, a, what);
+      default: return run_split<T, 4, 64, Back>(stream, batch, a, what);}
+  return p.lanes == 32 ? run_split<T, 1, 32, Back>(stream, batch, a, what)
+                       : run_split<T, 1, 64, Back>(stream, batch, a, what);
+}
+
+// Whether four channels can move as one access.
+bool packs(uint64_t channels, uint64_t element, std::initializer_list<const void *> pointers) {
+  if (channels % 4 != 0) return false;
+  for (const void *p : pointers)
+    if (!aligned_to(p, 4 * element)) return false;
+  return true;
 }
 
 template <typename T>
-oxh_status backward(hipStream_t stream, uint64_t batch, const Backward<T> &a) {
-  oxh::launch(recurrence_backward_kernel<T>,
-              dim3((a.channels + 63) / 64, static_cast<uint32_t>(batch)), dim3(64), 0, stream,
-              a);
-  return oxh::launched("gated_recurrence_backward");
+oxh_status forward(hipStream_t stream, uint64_t batch, const void *input, const void *gate,
+                   const float *initial_state, const int32_t *lengths, void *output,
+                   float *final_state, void *workspace, uint32_t time, uint32_t channels) {
+  Args<T> a{};
+  a.u = static_cast<const T *>(input);
+  a.g = static_cast<const T *>(gate);
+  a.out = static_cast<T *>(output);
+  a.first = initial_state;
+  a.last = final_state;
+  a.lengths = lengths;
+  a.parts = static_cast<float *>(workspace);
+  a.time = time;
+  a.channels = channels;
+  return run<T, false>(stream, batch, a, packs(channels, sizeof(T), {input, gate, output}),
+                       "gated_recurrence_forward");
+}
+
+template <typename T>
+oxh_status backward(hipStream_t stream, uint64_t batch, const void *gradient, const void *input,
+                    const void *gate, const void *output, const float *initial_state,
+                    const float *final_state_gradient, const int32_t *lengths,
+                    void *input_gradient, void *gate_gradient, float *initial_state_gradient,
+                    void *workspace, uint32_t time, uint32_t channels) {
+  Args<T> a{};
+  a.dh = static_cast<const T *>(gradient);
+  a.u = static_cast<const T *>(input);
+  a.g = static_cast<const T *>(gate);
+  a.h = static_cast<const T *>(output);
+  a.out = static_cast<T *>(input_gradient);
+  a.dg = static_cast<T *>(gate_gradient);
+  a.first = final_state_gradient;
+  a.origin = initial_state;
+  a.last = initial_state_gradient;
+  a.lengths = lengths;
+  a.parts = static_cast<float *>(workspace);
+  a.time = time;
+  a.channels = channels;
+  return run<T, true>(
+      stream, batch, a,
+      packs(channels, sizeof(T), {gradient, input, gate, output, input_gradient, gate_gradient}),
+      "gated_recurrence_backward");
 }
 
 }  // namespace
@@ -168,7 +578,13 @@ oxh_status oxh_gated_recurrence_workspace_size(uint64_t batch, uint64_t time, ui
   OXH_REQUIRE(bytes != nullptr, OXH_INVALID_SHAPE, "bytes is null");
   oxh_status st = check_shape("gated recurrence", OXH_F32, batch, time, channels);
   if (st != OXH_OK) return st;
-  *bytes = 256;
+  *bytes = 0;
+  if (batch == 0 || channels == 0) return oxh::ok();
+  for (const bool packed : {false, true})
+    for (const bool back : {false, true})
+      *bytes = std::max(*bytes, parts_bytes(plan_of(batch, time, channels, packed, back), batch,
+                                            channels));
+  *bytes = (*bytes + 255) / 256 * 256;
   return oxh::ok();
 }
 
@@ -178,36 +594,32 @@ oxh_status oxh_gated_recurrence_forward(oxh_stream stream, int dtype, uint64_t b
                                         const int32_t *lengths, void *output,
                                         float *final_state, void *workspace,
                                         uint64_t workspace_bytes) {
-  const std::string what = "gated recurrence";
+  const char *const what = "gated recurrence";
   oxh_status st = check_shape(what, dtype, batch, time, channels);
   if (st != OXH_OK) return st;
   if (batch == 0 || channels == 0) return oxh::ok();
   const uint64_t element = oxh::storage::bytes_of(dtype),
                  bytes = batch * time * channels * element, states = batch * channels * 4;
   OXH_REQUIRE(time == 0 || (input != nullptr && gate != nullptr && output != nullptr),
-              OXH_INVALID_SHAPE, what + ": null pointer");
+              OXH_INVALID_SHAPE, message(what, ": null pointer"));
   OXH_REQUIRE(aligned_to(input, element) && aligned_to(gate, element) &&
                   aligned_to(output, element) && aligned_to(initial_state, 4) &&
                   aligned_to(final_state, 4) && aligned_to(lengths, 4),
-              OXH_INVALID_SHAPE, what + ": a pointer is not aligned to its elements");
+              OXH_INVALID_SHAPE, message(what, ": a pointer is not aligned to its elements"));
   uint64_t needed = 0;
   st = oxh_gated_recurrence_workspace_size(batch, time, channels, &needed);
   if (st != OXH_OK) return st;
-  OXH_REQUIRE(workspace != nullptr && workspace_bytes >= needed && oxh::aligned16(workspace),
-              OXH_INVALID_SHAPE, what + ": workspace too small or misaligned");
+  OXH_REQUIRE(needed == 0 || (workspace != nullptr && workspace_bytes >= needed &&
+                              oxh::aligned16(workspace)),
+              OXH_INVALID_SHAPE, message(what, ": workspace too small or misaligned"));
   const Span in[] = {{input, bytes}, {gate, bytes}, {initial_state, states}, {lengths, batch * 4}};
   const Span out[] = {{output, bytes}, {final_state, states}, {workspace, needed}};
   st = check_apart(what, in, 4, out, 3, 2, 1);
   if (st != OXH_OK) return st;
   const uint32_t t = static_cast<uint32_t>(time), c = static_cast<uint32_t>(channels);
-  if (dtype == OXH_F32)
-    return forward<float>(oxh::as_stream(stream), batch,
-                          {static_cast<const float *>(input), static_cast<const float *>(gate),
-                           initial_state, static_cast<float *>(output), final_state, lengths, t,
-                           c});
-  return forward<bf16>(oxh::as_stream(stream), batch,
-                       {static_cast<const bf16 *>(input), static_cast<const bf16 *>(gate),
-                        initial_state, static_cast<bf16 *>(output), final_state, lengths, t, c});
+  const auto run_typed = dtype == OXH_F32 ? forward<float> : forward<bf16>;
+  return run_typed(oxh::as_stream(stream), batch, input, gate, initial_state, lengths, output,
+                   final_state, workspace, t, c);
 }
 
 oxh_status oxh_gated_recurrence_backward(
@@ -216,7 +628,7 @@ oxh_status oxh_gated_recurrence_backward(
     const float *initial_state, const float *final_state_gradient, const int32_t *lengths,
     void *input_gradient, void *gate_gradient, float *initial_state_gradient, void *workspace,
     uint64_t workspace_bytes) {
-  const std::string what = "gated recurrence backward";
+  const char *const what = "gated recurrence backward";
   oxh_status st = check_shape(what, dtype, batch, time, channels);
   if (st != OXH_OK) return st;
   if (batch == 0 || channels == 0) return oxh::ok();
@@ -225,18 +637,19 @@ oxh_status oxh_gated_recurrence_backward(
   OXH_REQUIRE(time == 0 || (gradient != nullptr && input != nullptr && gate != nullptr &&
                             output != nullptr && input_gradient != nullptr &&
                             gate_gradient != nullptr),
-              OXH_INVALID_SHAPE, what + ": null pointer");
+              OXH_INVALID_SHAPE, message(what, ": null pointer"));
   OXH_REQUIRE(aligned_to(gradient, element) && aligned_to(input, element) &&
                   aligned_to(gate, element) && aligned_to(output, element) &&
                   aligned_to(input_gradient, element) && aligned_to(gate_gradient, element) &&
                   aligned_to(initial_state, 4) && aligned_to(final_state_gradient, 4) &&
                   aligned_to(initial_state_gradient, 4) && aligned_to(lengths, 4),
-              OXH_INVALID_SHAPE, what + ": a pointer is not aligned to its elements");
+              OXH_INVALID_SHAPE, message(what, ": a pointer is not aligned to its elements"));
   uint64_t needed = 0;
   st = oxh_gated_recurrence_workspace_size(batch, time, channels, &needed);
   if (st != OXH_OK) return st;
-  OXH_REQUIRE(workspace != nullptr && workspace_bytes >= needed && oxh::aligned16(workspace),
-              OXH_INVALID_SHAPE, what + ": workspace too small or misaligned");
+  OXH_REQUIRE(needed == 0 || (workspace != nullptr && workspace_bytes >= needed &&
+                              oxh::aligned16(workspace)),
+              OXH_INVALID_SHAPE, message(what, ": workspace too small or misaligned"));
   const Span in[] = {{gradient, bytes},       {input, bytes},
                      {gate, bytes},           {output, bytes},
                      {initial_state, states}, {final_state_gradient, states},
@@ -248,19 +661,10 @@ oxh_status oxh_gated_recurrence_backward(
   st = check_apart(what, in, 7, out, 4, 5, 2);
   if (st != OXH_OK) return st;
   const uint32_t t = static_cast<uint32_t>(time), c = static_cast<uint32_t>(channels);
-  if (dtype == OXH_F32)
-    return backward<float>(
-        oxh::as_stream(stream), batch,
-        {static_cast<const float *>(gradient), static_cast<const float *>(input),
-         static_cast<const float *>(gate), static_cast<const float *>(output), initial_state,
-         final_state_gradient, static_cast<float *>(input_gradient),
-         static_cast<float *>(gate_gradient), initial_state_gradient, lengths, t, c});
-  return backward<bf16>(
-      oxh::as_stream(stream), batch,
-      {static_cast<const bf16 *>(gradient), static_cast<const bf16 *>(input),
-       static_cast<const bf16 *>(gate), static_cast<const bf16 *>(output), initial_state,
-       final_state_gradient, static_cast<bf16 *>(input_gradient),
-       static_cast<bf16 *>(gate_gradient), initial_state_gradient, lengths, t, c});
+  const auto run_typed = dtype == OXH_F32 ? backward<float> : backward<bf16>;
+  return run_typed(oxh::as_stream(stream), batch, gradient, input, gate, output, initial_state,
+                   final_state_gradient, lengths, input_gradient, gate_gradient,
+                   initial_state_gradient, workspace, t, c);
 }
 
 }  // extern "C"

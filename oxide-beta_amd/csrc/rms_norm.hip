@@ -227,22 +227,26 @@ __global__ __launch_bounds__(1024) void rms_norm_backward_long_kernel(Backward<T
   }
 }
 
-// out[c] = sum over the partial rows, in row order within each of 16 strands, the strands added
-// in order.
+// out[c] = sum over the partial rows: 16 columns per block, 64 strands of rows each, a strand's
+// rows in order and the strands by halves.
 __global__ __launch_bounds__(1024) void rms_norm_weight_kernel(const float *partial, float *out,
                                                                uint32_t rows, uint32_t columns) {
-  __shared__ float part[16][64];
-  const uint32_t column = blockIdx.x * 64 + (threadIdx.x & 63), strand = threadIdx.x >> 6;
+  __shared__ float part[64][17];
+  const uint32_t c = threadIdx.x & 15, strand = threadIdx.x >> 4, column = blockIdx.x * 16 + c;
   float sum = 0.0f;
-  if (column < columns)
-    for (uint32_t r = strand; r < rows; r += 16)
+  if (column < columns) {
+#pragma unroll 8
+    for (uint32_t r = strand; r < rows; r += 64)
       sum += partial[static_cast<uint64_t>(r) * columns + column];
-  part[strand][threadIdx.x & 63] = sum;
+  }
+  part[strand][c] = sum;
   __syncthreads();
-  if (strand != 0 || column >= columns) return;
 #pragma unroll
-  for (int i = 1; i < 16; ++i) sum += part[i][threadIdx.x];
-  out[column] = sum;
+  for (uint32_t half = 32; half != 0; half /= 2) {
+    if (strand < half) part[strand][c] += part[strand + half][c];
+    __syncthreads();
+  }
+  if (strand == 0 && column < columns) out[column] = part[0][c];
 }
 
 // Values that one row's registers cover at N values per access (8 accesses of 1024 threads).
@@ -352,7 +356,7 @@ oxh_status backward(hipStream_t stream, const Backward<T> &a, float *weight_grad
   }
   oxh_status st = oxh::launched("rms_norm_backward");
   if (st != OXH_OK || weight_gradient == nullptr) return st;
-  oxh::launch(rms_norm_weight_kernel, dim3((a.columns + 63) / 64), dim3(1024), 0, stream,
+  oxh::launch(rms_norm_weight_kernel, dim3((a.columns + 15) / 16), dim3(1024), 0, stream,
               static_cast<const float *>(a.partial), weight_gradient,
               static_cast<uint32_t>(groups), a.columns);
   return oxh::launched("rms_norm_weight_gradient");

@@ -24,6 +24,7 @@ Errors raise ``OxideError`` whose ``kind`` names the reference's Error variant
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import re
 from pathlib import Path
@@ -293,49 +294,66 @@ def _f32_tensor(t, name: str):
 
 
 F32, BF16 = 0, 1
+_activation_codes = None  # torch dtype -> F32 / BF16, filled at the first use
 
 
 def _activation(tensors, shape, what: str) -> int:
-    """The dtype code of device tensors that share one type and one shape."""
-    import torch
+    """The dtype code of device tensors that share one type and one shape (None: absent)."""
+    global _activation_codes
+    if _activation_codes is None:
+        import torch
 
-    first = tensors[0]
-    code = {torch.float32: F32, torch.bfloat16: BF16}.get(first.dtype)
-    if code is None or not first.is_cuda:
-        raise OxideError(INVALID_SHAPE, f"{what} takes float32 or bfloat16 device tensors")
+        _activation_codes = {torch.float32: F32, torch.bfloat16: BF16}
+    dtype = tensors[0].dtype
+    code = _activation_codes.get(dtype)
+    if code is None:
+        raise OxideError(INVALID_SHAPE, f"{what} takes float32 or bfloat16 tensors")
     for t in tensors:
-        if t is None:
-            continue
-        if t.dtype != first.dtype or t.device != first.device:
-            raise OxideError(INVALID_SHAPE, f"{what}: tensors differ in type or device")
-        if t.shape != shape:
+        if t is not None and (t.dtype is not dtype or not t.is_cuda or t.shape != shape):
             raise OxideError(INVALID_SHAPE,
-                             f"{what}: shape {list(t.shape)} where {list(shape)} is expected")
+                             f"{what} takes device tensors of one type and of shape "
+                             f"{list(shape)}: got {t.dtype} {list(t.shape)} on {t.device}")
     return code
 
 
 def _shaped(t, shape, name: str):
-    """A float32 device tensor of ``shape``, or None."""
-    if t is not None and _f32_tensor(t, name).shape != shape:
+    """Address of a contiguous float32 device tensor of ``shape``, or None."""
+    if t is None:
+        return None
+    if _f32_tensor(t, name).shape != shape:
         raise OxideError(INVALID_SHAPE,
                          f"{name}: shape {list(t.shape)} where {list(shape)} is expected")
     return _ptr(t)
 
 
 def _lengths(t, batch: int):
-    import torch
-
     if t is None:
         return None
+    import torch
+
     if t.dtype != torch.int32 or not t.is_cuda or t.shape != (batch,):
         raise OxideError(INVALID_SHAPE, "lengths must be an int32 device tensor [batch]")
     return _ptr(t)
 
 
-def current_stream() -> int:
-    import torch
+_raw_stream = None  # () -> address of torch's current stream, set at the first use
 
-    return torch.cuda.current_stream().cuda_stream
+
+def current_stream() -> int:
+    """Address of torch's current stream (by torch's own raw accessor where it has one: 0.1 us,
+    2.8 us through a stream object)."""
+    global _raw_stream
+    if _raw_stream is None:
+        import torch
+
+        raw, device = (getattr(torch._C, name, None)
+                       for name in ("_cuda_getCurrentRawStream", "_cuda_getDevice"))
+        if raw is not None and device is not None:
+            torch.cuda.current_stream()  # initialises torch's device state
+            _raw_stream = lambda: raw(device())  # noqa: E731
+        else:
+            _raw_stream = lambda: torch.cuda.current_stream().cuda_stream  # noqa: E731
+    return _raw_stream()
 
 
 def _stream(stream) -> int | None:
@@ -379,18 +397,21 @@ def cross_entropy_workspace_size(batch: int, classes: int) -> int:
     return out.value
 
 
+@functools.lru_cache(maxsize=4096)
 def rms_norm_backward_workspace_size(rows: int, columns: int) -> int:
     out = _u64()
     check(lib().oxh_rms_norm_backward_workspace_size(rows, columns, ctypes.byref(out)))
     return out.value
 
 
+@functools.lru_cache(maxsize=4096)
 def gated_recurrence_workspace_size(batch: int, time: int, channels: int) -> int:
     out = _u64()
     check(lib().oxh_gated_recurrence_workspace_size(batch, time, channels, ctypes.byref(out)))
     return out.value
 
 
+@functools.lru_cache(maxsize=4096)
 def orthogonalize_workspace_size(count: int, rows: int, columns: int) -> int:
     out = _u64()
     check(lib().oxh_orthogonalize_workspace_size(count, rows, columns, ctypes.byref(out)))
@@ -826,13 +847,17 @@ class LoadedModule:
         return dev_table, dev_starts
 
     # -- sequence layers (no counterpart in the reference)
+    def _sequence_workspace(self, nbytes: int) -> tuple[int | None, int]:
+        return self._sequence_ws.ptr_bytes(nbytes) if nbytes else (None, 0)
+
     def rms_norm_forward(self, x, weight, out, inverse_rms=None, residual=None, sum=None,  # noqa: A002
                          epsilon=1e-6, stream=None):
         """``out`` = s / rms(s) * weight over the last dimension, s = x + residual; ``sum``
         receives s (it may be ``x`` or ``residual``) and ``inverse_rms`` [rows] what the
         backward needs."""
-        code = _activation((x, out, residual, sum), x.shape, "rms_norm")
-        columns = x.shape[-1]
+        shape = x.shape
+        code = _activation((x, out, residual, sum), shape, "rms_norm")
+        columns = shape[-1] if shape else 0
         rows = x.numel() // max(columns, 1)
         check(lib().oxh_rms_norm_forward(
             _stream(stream), code, rows, columns, epsilon, _ptr(x), _ptr(residual),
@@ -843,12 +868,13 @@ class LoadedModule:
                           weight_gradient=None, sum_gradient=None, stream=None):
         """Gradients from the output's and, where the sum has other uses, ``sum_gradient``
         (``input_gradient`` may be that tensor)."""
-        code = _activation((gradient, sum, input_gradient, sum_gradient), gradient.shape,
+        shape = gradient.shape
+        code = _activation((gradient, sum, input_gradient, sum_gradient), shape,
                            "rms_norm_backward")
-        columns = gradient.shape[-1]
+        columns = shape[-1] if shape else 0
         rows = gradient.numel() // max(columns, 1)
-        ws, wsb = (None, 0) if weight_gradient is None else self._sequence_ws.ptr_bytes(
-            rms_norm_backward_workspace_size(rows, columns))
+        ws, wsb = self._sequence_workspace(
+            0 if weight_gradient is None else rms_norm_backward_workspace_size(rows, columns))
         check(lib().oxh_rms_norm_backward(
             _stream(stream), code, rows, columns, _ptr(gradient), _ptr(sum_gradient), _ptr(sum),
             _shaped(weight, (columns,), "weight"), _shaped(inverse_rms, (rows,), "inverse_rms"),
@@ -860,13 +886,13 @@ class LoadedModule:
         """``out`` [batch, time, channels] of h_t = a_t h_{t-1} + (1 - a_t) x_t with
         a_t = sigmoid(gate_t); states [batch, channels] float32 (the final one may be written
         over the initial one), ``lengths`` [batch] int32."""
-        code = _activation((x, gate, out), x.shape, "gated_recurrence")
-        if x.dim() != 3:
+        shape = x.shape
+        if len(shape) != 3:
             raise OxideError(INVALID_SHAPE, "gated_recurrence expects [batch, time, channels]")
-        batch, time, channels = x.shape
-        ws, wsb = self._sequence_ws.ptr_bytes(
-            gated_recurrence_workspace_size(batch, time, channels))
+        code = _activation((x, gate, out), shape, "gated_recurrence")
+        batch, time, channels = shape
         states = (batch, channels)
+        ws, wsb = self._sequence_workspace(gated_recurrence_workspace_size(batch, time, channels))
         check(lib().oxh_gated_recurrence_forward(
             _stream(stream), code, batch, time, channels, _ptr(x), _ptr(gate),
             _shaped(initial_state, states, "initial_state"), _lengths(lengths, batch),
@@ -877,14 +903,14 @@ class LoadedModule:
                                   initial_state_gradient=None, lengths=None, stream=None):
         """Gradients of ``gated_recurrence_forward``'s operands from its output's and its final
         state's."""
-        code = _activation((gradient, x, gate, out, x_gradient, gate_gradient), x.shape,
-                           "gated_recurrence_backward")
-        if x.dim() != 3:
+        shape = x.shape
+        if len(shape) != 3:
             raise OxideError(INVALID_SHAPE, "gated_recurrence expects [batch, time, channels]")
-        batch, time, channels = x.shape
-        ws, wsb = self._sequence_ws.ptr_bytes(
-            gated_recurrence_workspace_size(batch, time, channels))
+        code = _activation((gradient, x, gate, out, x_gradient, gate_gradient), shape,
+                           "gated_recurrence_backward")
+        batch, time, channels = shape
         states = (batch, channels)
+        ws, wsb = self._sequence_workspace(gated_recurrence_workspace_size(batch, time, channels))
         check(lib().oxh_gated_recurrence_backward(
             _stream(stream), code, batch, time, channels, _ptr(gradient), _ptr(x), _ptr(gate),
             _ptr(out), _shaped(initial_state, states, "initial_state"),
@@ -898,7 +924,7 @@ class LoadedModule:
         if x.dim() not in (2, 3):
             raise OxideError(INVALID_SHAPE, "orthogonalize expects a matrix or a stack of them")
         count, (rows, columns) = (x.shape[0] if x.dim() == 3 else 1), x.shape[-2:]
-        ws, wsb = self._sequence_ws.ptr_bytes(orthogonalize_workspace_size(count, rows, columns))
+        ws, wsb = self._sequence_workspace(orthogonalize_workspace_size(count, rows, columns))
         check(lib().oxh_orthogonalize(_stream(stream), count, rows, columns, rounds, epsilon,
                                       _shaped(x, x.shape, "x"), _shaped(out, x.shape, "out"), ws,
                                       wsb))
@@ -908,7 +934,7 @@ class LoadedModule:
         """One optimizer step of ``tensors``, a sequence of (parameter, gradient, momentum):
         the momentum and the parameter are updated in place."""
         table = muon_table(tensors)
-        ws, wsb = self._sequence_ws.ptr_bytes(muon_workspace_size(table))
+        ws, wsb = self._sequence_workspace(muon_workspace_size(table))
         check(lib().oxh_muon_multi_tensor(_stream(stream), learning_rate, weight_decay, momentum,
                                           int(bool(nesterov)), epsilon, rounds, table,
                                           len(table), ws, wsb))

@@ -75,8 +75,8 @@ def test_rms_norm_backward():
 
 def scan_forward(**k):
     u, g, st, n, h, f, ws = places(7)
-    a = dict(dtype=0, batch=2, time=3, channels=8, u=u, g=g, st=st, n=n, h=h, f=f, ws=ws,
-             bytes=ox.gated_recurrence_workspace_size(2, 3, 8)) | k
+    a = dict(dtype=0, batch=2, time=2000, channels=8, u=u, g=g, st=st, n=n, h=h, f=f, ws=ws,
+             bytes=ox.gated_recurrence_workspace_size(2, 2000, 8)) | k
     return ox.lib().oxh_gated_recurrence_forward(
         None, a["dtype"], a["batch"], a["time"], a["channels"], a["u"], a["g"], a["st"], a["n"],
         a["h"], a["f"], a["ws"], a["bytes"])
@@ -104,9 +104,9 @@ def test_gated_recurrence_forward():
 def scan_backward(**k):
     dh, u, g, h, st, df, n, du, dg, ds, ws = places(11)
     a = dict(dtype=0, dh=dh, u=u, g=g, h=h, st=st, df=df, n=n, du=du, dg=dg, ds=ds, ws=ws,
-             bytes=ox.gated_recurrence_workspace_size(2, 3, 8)) | k
+             bytes=ox.gated_recurrence_workspace_size(2, 2000, 8)) | k
     return ox.lib().oxh_gated_recurrence_backward(
-        None, a["dtype"], 2, 3, 8, a["dh"], a["u"], a["g"], a["h"], a["st"], a["df"], a["n"],
+        None, a["dtype"], 2, 2000, 8, a["dh"], a["u"], a["g"], a["h"], a["st"], a["df"], a["n"],
         a["du"], a["dg"], a["ds"], a["ws"], a["bytes"])
 
 
@@ -126,9 +126,9 @@ def test_gated_recurrence_backward():
 
 def test_orthogonalize():
     x, y, ws = places(3)
-    lib, need = ox.lib(), ox.orthogonalize_workspace_size(2, 30, 40)
+    lib, need = ox.lib(), ox.orthogonalize_workspace_size(2, 300, 400)
 
-    def call(count=2, rows=30, columns=40, rounds=5, eps=1e-7, x=x, y=y, ws=ws, n=need):
+    def call(count=2, rows=300, columns=400, rounds=5, eps=1e-7, x=x, y=y, ws=ws, n=need):
         return lib.oxh_orthogonalize(None, count, rows, columns, rounds, eps, x, y, ws, n)
 
     refused(call(rows=0), b"empty")
@@ -152,7 +152,7 @@ def test_muon():
     p, g, m, ws = places(4)
     lib = ox.lib()
 
-    def call(entries=((p, g, m, 30, 40),), lr=0.1, wd=0.0, mu=0.9, eps=1e-7, rounds=5, ws=ws,
+    def call(entries=((p, g, m, 300, 400),), lr=0.1, wd=0.0, mu=0.9, eps=1e-7, rounds=5, ws=ws,
              n=None):
         table = (ox.MuonTensor * len(entries))(*[ox.MuonTensor(*e) for e in entries])
         if n is None:
@@ -167,13 +167,13 @@ def test_muon():
         refused(call(**k), b"finite")
     refused(call(eps=0.0), b"epsilon", ox.EXECUTION)
     refused(call(rounds=0), b"rounds")
-    refused(call(((p, g, m, 0, 40),)), b"empty")
-    refused(call(((p, g, None, 30, 40),)), b"null")
-    refused(call(((p + 1, g, m, 30, 40),)), b"misaligned")
+    refused(call(((p, g, m, 0, 400),)), b"empty")
+    refused(call(((p, g, None, 300, 400),)), b"null")
+    refused(call(((p + 1, g, m, 300, 400),)), b"misaligned")
     refused(call(n=16), b"workspace")
-    refused(call(((p, p, m, 30, 40),)), b"overlaps")
-    refused(call(((p, g, p + 400, 30, 40),)), b"overlaps")
-    refused(call(((p, g, m, 30, 40), (p + 4000, g + 8000, m + 8000, 30, 40))), b"overlaps")
+    refused(call(((p, p, m, 300, 400),)), b"overlaps")
+    refused(call(((p, g, p + 400, 300, 400),)), b"overlaps")
+    refused(call(((p, g, m, 300, 400), (p + 4000, g + 500000, m + 500000, 300, 400))), b"overlaps")
     refused(call(ws=m), b"overlaps")
     assert call((), ws=None) == ox.OK
 
