@@ -21,6 +21,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <exception>
 #include <string>
 #include <vector>
 
@@ -31,6 +32,9 @@ namespace {
 typedef _Float16 f16;
 typedef f16 f16x4 __attribute__((ext_vector_type(4)));
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
@@ -38,8 +42,9 @@ constexpr float kScale = 16384.0f, kUnscale = 1.0f / (16384.0f * 16384.0f);
 
 // A matrix of a launch group.  Short = min(rows, columns) and Long are the sides of X; ps and pl
 // the same rounded up to the tile, the padding zero throughout.  `scratch` holds, in order:
-//   x [ps][pl] float32; xs: X in halves; xt0, xt1: X' in halves (one is read while the other is
-//   written); ga [ps][ps] float32: A; gs, bs: A and B in halves; the norm's partial sums.
+//   x [pl][ps] float32: X'; xs: X in halves; xt0, xt1: X' in halves (one is read while the other
+//   is written); ga [ps][ps] float32: A (its lower tiles, transposed); gs, bs: A and B in halves;
+//   the norm's partial sums.
 // Halves of a matrix with k columns: per row, blocks of 32 columns, 32 hi then 32 lo.
 struct Matrix {
   const float *gradient;
@@ -125,6 +130,32 @@ __device__ __forceinline__ uint64_t halves_at(uint32_t row, uint32_t column, uin
   return (static_cast<uint64_t>(row) * k + (column & ~31u)) * 2 + (column & 31u);
 }
 
+// Both halves in one word, hi below.
+__device__ __forceinline__ uint32_t halves_word(float v) {
+  f16 hi, lo;
+  halves_of(v, hi, lo);
+  return static_cast<uint32_t>(__builtin_bit_cast(uint16_t, hi)) |
+         static_cast<uint32_t>(__builtin_bit_cast(uint16_t, lo)) << 16;
+}
+// 16 consecutive such words to their place in halves.
+__device__ __forceinline__ void store_line(const uint32_t *words, f16 *to) {
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const u32x4 w0 = *reinterpret_cast<const u32x4 *>(words + 8 * e);
+    const u32x4 w1 = *reinterpret_cast<const u32x4 *>(words + 8 * e + 4);
+    u32x4 hi, lo;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      hi[k] = (w0[2 * k] & 0xFFFFu) | w0[2 * k + 1] << 16;
+      lo[k] = w0[2 * k] >> 16 | (w0[2 * k + 1] & 0xFFFF0000u);
+      hi[2 + k] = (w1[2 * k] & 0xFFFFu) | w1[2 * k + 1] << 16;
+      lo[2 + k] = w1[2 * k] >> 16 | (w1[2 * k + 1] & 0xFFFF0000u);
+    }
+    *reinterpret_cast<u32x4 *>(to + 8 * e) = hi;
+    *reinterpret_cast<u32x4 *>(to + 8 * e + 32) = lo;
+  }
+}
+
 // X = V / (|V| + epsilon) in its three forms, a 32 x 32 tile per block.
 __global__ __launch_bounds__(256) void muon_start_kernel(Group g) {
   __shared__ float tile[32][33];
@@ -159,7 +190,7 @@ __global__ __launch_bounds__(256) void muon_start_kernel(Group g) {
   for (uint32_t k = ty; k < 32; k += 8) {
     f16 hi, lo;
     const float v = tile[k][tx], t = tile[tx][k];
-    x[static_cast<uint64_t>(i0 + k) * m.pl + j0 + tx] = v;
+    x[static_cast<uint64_t>(j0 + k) * m.ps + i0 + tx] = t;
     halves_of(v, hi, lo);
     f16 *p = xs + halves_at(i0 + k, j0 + tx, m.pl);
     p[0] = hi;
@@ -173,29 +204,63 @@ __global__ __launch_bounds__(256) void muon_start_kernel(Group g) {
 
 enum class Step { Gram, Poly, Apply, Last };
 
-// One of a round's three products, a tile of 2 x 2 waves by T x T blocks of 32 x 32 per block of
-// threads.  Both operands are halves with the summed index along the rows.  A and B are
-// symmetric: only tiles on and below the diagonal are summed, the others are their mirrors.
-template <Step S, int T>
-__global__ __launch_bounds__(256) void muon_product_kernel(Group g, int odd) {
-  constexpr int kTile = 64 * T;
-  // per operand row: 32 summed values, 8 pieces of 16 bytes (hi 0..3, lo 4..7), each at its place
-  // exclusive-or the row's low bits, so that 8 rows' same piece lie in 8 different bank groups
-  __shared__ __attribute__((aligned(16))) char stage[2][kTile * 128];
-  const Matrix &m = matrix_of(g, blockIdx.x);
-  const Layout l = layout_of(m.ps, m.pl);
-  const uint32_t b = blockIdx.x - m.first_block;
-  uint32_t ti, tj;
-  if constexpr (S == Step::Gram || S == Step::Poly) {
-    ti = static_cast<uint32_t>((sqrtf(8.0f * b + 1.0f) - 1.0f) * 0.5f);
-    while (ti * (ti + 1) / 2 > b) --ti;
-    while ((ti + 1) * (ti + 2) / 2 <= b) ++ti;
-    tj = b - ti * (ti + 1) / 2;
+// The block shapes of the products: Groups times WM x WN waves of TM x TN blocks of 32 x 32, and
+// K blocks of 32 summed values per stage, of whose 2 K halves each group takes every Groups-th.
+template <int WM_, int WN_, int TM_, int TN_, int K_, int Groups_>
+struct Shape {
+  static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, K = K_, Groups = Groups_;
+  static constexpr int threads = WM * WN * Groups * 64, tile = WM * TM * 32;
+  static_assert(WM * TM == WN * TN && 2 * K % Groups == 0, "square tiles, whole halves");
+};
+using Wide = Shape<2, 2, 3, 3, 1, 2>;    // 192 x 192
+using Medium = Shape<2, 2, 2, 2, 1, 2>;  // 128 x 128
+using Small = Shape<2, 2, 1, 1, 2, 2>;   // 64 x 64
+
+// The tile of index b among rows x columns tiles, or (Symmetric) among those on and below the
+// diagonal of rows x rows: bands of four tile rows, each taken column by column, so that the run
+// of tiles that one XCD computes shares few operand rows in its L2.
+struct Tile {
+  uint32_t row, column;
+};
+template <bool Symmetric>
+__device__ __forceinline__ Tile tile_at(uint32_t b, uint32_t rows, uint32_t columns) {
+  uint32_t band, at;
+  if constexpr (Symmetric) {
+    // a band's full columns and its triangle: 16 band + 10 tiles, 8 band^2 + 2 band before it
+    band = static_cast<uint32_t>((sqrtf(8.0f * b + 1.0f) - 1.0f) * 0.125f);
+    while (8 * band * band + 2 * band > b) --band;
+    while (8 * (band + 1) * (band + 1) + 2 * (band + 1) <= b) ++band;
+    at = b - (8 * band * band + 2 * band);
   } else {
-    const uint32_t across = m.pl / kTile;
-    ti = b / across;
-    tj = b % across;
+    band = b / (4 * columns);
+    at = b - band * 4 * columns;
   }
+  const uint32_t height = min(4u, rows - 4 * band);
+  const uint32_t full = Symmetric ? height * (4 * band + 1) : ~0u;
+  if (at < full) return {4 * band + at % height, at / height};
+  at -= full;  // the triangle's columns right of its first: height - 1, height - 2, ... tiles
+  uint32_t column = 1;
+  while (at >= height - column) at -= height - column, ++column;
+  return {4 * band + column + at, 4 * band + column};
+}
+
+// One of a round's three products, a square tile per block of threads.  Both operands are halves
+// with the summed index along the rows.  A and B are symmetric: only tiles on and below the
+// diagonal are summed, the others are their mirrors.
+template <Step S, class Sh>
+__global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int odd) {
+  constexpr int kTile = Sh::tile, TM = Sh::TM, TN = Sh::TN, K = Sh::K;
+  // per operand row and K block: 32 summed values, 8 pieces of 16 bytes (hi 0..3, lo 4..7), each
+  // at its place exclusive-or bits 1 to 3 of the row: the 16 rows that one pass of a fragment's reads takes lie
+  // in different banks (with bits 0 to 2, two and two share them: 1.05 times the time)
+  constexpr int kStage = kTile * 128 * K;
+  __shared__ __attribute__((aligned(16))) char stage[2 * 2 * kStage];  // [turn][a, b][K][row][128]
+  const uint32_t id = oxh::xcd_contiguous(blockIdx.x, gridDim.x);
+  const Matrix &m = matrix_of(g, id);
+  const Layout l = layout_of(m.ps, m.pl);
+  constexpr bool kSymmetric = S == Step::Gram || S == Step::Poly;
+  const Tile t = tile_at<kSymmetric>(id - m.first_block, m.ps / kTile, m.pl / kTile);
+  const uint32_t ti = t.row, tj = t.column;
   const uint32_t k_total = S == Step::Gram ? m.pl : m.ps;
   const f16 *pa, *pb;
   f16 *gs = reinterpret_cast<f16 *>(m.scratch + l.gs), *bs = reinterpret_cast<f16 *>(m.scratch + l.bs);
@@ -209,88 +274,160 @@ __global__ __launch_bounds__(256) void muon_product_kernel(Group g, int odd) {
   const char *sb = reinterpret_cast<const char *>(pb) + static_cast<uint64_t>(tj) * kTile * k_total * 4;
 
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t wi = wave >> 1, wj = wave & 1;
-  constexpr int kLoads = kTile * 8 / 256;  // 16-byte pieces per thread per operand
-  uint4 ra[kLoads], rb[kLoads];
-  auto fetch = [&](uint32_t k) {
+  const uint32_t group = wave / (Sh::WM * Sh::WN), place = wave % (Sh::WM * Sh::WN);
+  const uint32_t wi = place / Sh::WN, wj = place % Sh::WN;
+  // this thread's 16-byte pieces of a stage: piece c0 of rows r0, r0 + kStep, ... of the operands'
+  // K blocks one after the other
+  constexpr int kStep = Sh::threads / 8, kLoads = 2 * K * kTile / kStep;
+  static_assert(K * kTile % kStep == 0, "an operand is whole passes");
+  const uint32_t r0 = threadIdx.x >> 3, c0 = threadIdx.x & 7;
+  u32x4 held[kLoads];
+  const uint32_t blocks = k_total / 32;
+  auto fetch = [&](uint32_t block) {
+    if (block >= blocks) return;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const uint32_t piece = i * 256 + threadIdx.x, row = piece >> 3, c = piece & 7;
-      const uint64_t at = static_cast<uint64_t>(row) * k_total * 4 + k * 4 + c * 16;
-      ra[i] = *reinterpret_cast<const uint4 *>(sa + at);
-      rb[i] = *reinterpret_cast<const uint4 *>(sb + at);
+      const uint32_t r = (i * kStep) % (K * kTile) + r0, row = r % kTile, k = block + r / kTile;
+      const char *p = (i * kStep < K * kTile ? sa : sb) +
+                      static_cast<uint64_t>(row) * k_total * 4 + k * 128 + c0 * 16;
+      held[i] = K == 1 || k < blocks ? *reinterpret_cast<const u32x4 *>(p) : u32x4{0, 0, 0, 0};
     }
   };
-  f32x16 acc[T][T];
-#pragma unroll
-  for (int i = 0; i < T; ++i)
-#pragma unroll
-    for (int j = 0; j < T; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-  fetch(0);
-  for (uint32_t k = 0; k < k_total; k += 32) {
-    __syncthreads();
+  auto put = [&](char *to_stage) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const uint32_t piece = i * 256 + threadIdx.x, row = piece >> 3, c = piece & 7;
-      *reinterpret_cast<uint4 *>(stage[0] + row * 128 + ((c ^ (row & 7)) * 16)) = ra[i];
-      *reinterpret_cast<uint4 *>(stage[1] + row * 128 + ((c ^ (row & 7)) * 16)) = rb[i];
+      const uint32_t r = i * kStep + r0;
+      *reinterpret_cast<u32x4 *>(to_stage + r * 128 + ((c0 ^ (r >> 1 & 7)) * 16)) = held[i];
+    }
+  };
+  f32x16 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+  // Operands pass from memory to registers two stages ahead, and on to the buffer that is not
+  // being read one stage ahead, behind the first fragments' reads (its own last readers passed the
+  // barrier).  Loading further ahead, or more per stage, changed nothing.
+  fetch(0);
+  put(stage);
+  fetch(K);
+  __syncthreads();
+  int turn = 0;
+  for (uint32_t block = 0; block < blocks; block += K) {
+    const char *now = stage + turn * 2 * kStage;
+    turn ^= 1;
+#pragma unroll
+    for (int part = 0; part < 2 * K / Sh::Groups; ++part) {
+      f16x8 ah[TM], al[TM], bh[TN], bl[TN];
+      const uint32_t half = part * Sh::Groups + group;
+      const uint32_t c = (half & 1) * 2 + (lane >> 5);
+      const char *in_a = now + (half >> 1) * kTile * 128, *in_b = in_a + kStage;
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        const uint32_t row = (wi * TM + i) * 32 + (lane & 31);
+        ah[i] = *reinterpret_cast<const f16x8 *>(in_a + row * 128 + ((c ^ (row >> 1 & 7)) * 16));
+        al[i] =
+            *reinterpret_cast<const f16x8 *>(in_a + row * 128 + (((c + 4) ^ (row >> 1 & 7)) * 16));
+      }
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const uint32_t row = (wj * TN + j) * 32 + (lane & 31);
+        bh[j] = *reinterpret_cast<const f16x8 *>(in_b + row * 128 + ((c ^ (row >> 1 & 7)) * 16));
+        bl[j] =
+            *reinterpret_cast<const f16x8 *>(in_b + row * 128 + (((c + 4) ^ (row >> 1 & 7)) * 16));
+      }
+      if (part == 0 && block + K < blocks) {
+        put(stage + turn * 2 * kStage);
+        fetch(block + 2 * K);
+      }
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], acc[i][j], 0, 0, 0);
     }
     __syncthreads();
-    if (k + 32 < k_total) fetch(k + 32);
+  }
+
+  // The groups' sums meet: block t of a wave's TM x TN is finished by group t % Groups, which adds
+  // the groups' in their order; one block per group and turn goes through the shared memory.
+  if constexpr (Sh::Groups > 1) {
+    constexpr int kGroups = Sh::Groups, kBlocks = TM * TN;
+    constexpr int kTurn = kBlocks < kGroups ? kBlocks : kGroups;
+    static_assert(Sh::WM * Sh::WN * kTurn * kGroups * 4096 <= 4 * kStage, "exchange space");
+    float *space = reinterpret_cast<float *>(stage);
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      f16x8 ah[T], al[T], bh[T], bl[T];
-      const uint32_t c = half * 2 + (lane >> 5);
+    for (int t0 = 0; t0 < kBlocks; t0 += kGroups) {
 #pragma unroll
-      for (int i = 0; i < T; ++i) {
-        const uint32_t row = (wi * T + i) * 32 + (lane & 31);
-        ah[i] = *reinterpret_cast<f16x8 *>(stage[0] + row * 128 + ((c ^ (row & 7)) * 16));
-        al[i] = *reinterpret_cast<f16x8 *>(stage[0] + row * 128 + (((c + 4) ^ (row & 7)) * 16));
+      for (int o = 0; o < kGroups; ++o) {
+        if (t0 + o >= kBlocks) continue;
+        float *slot = space + ((place * kTurn + o) * kGroups + group) * 1024 + lane * 4;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<f32x4 *>(slot + q * 256) =
+              f32x4{acc[(t0 + o) / TN][(t0 + o) % TN][4 * q], acc[(t0 + o) / TN][(t0 + o) % TN][4 * q + 1],
+                    acc[(t0 + o) / TN][(t0 + o) % TN][4 * q + 2], acc[(t0 + o) / TN][(t0 + o) % TN][4 * q + 3]};
       }
+      __syncthreads();
 #pragma unroll
-      for (int j = 0; j < T; ++j) {
-        const uint32_t row = (wj * T + j) * 32 + (lane & 31);
-        bh[j] = *reinterpret_cast<f16x8 *>(stage[1] + row * 128 + ((c ^ (row & 7)) * 16));
-        bl[j] = *reinterpret_cast<f16x8 *>(stage[1] + row * 128 + (((c + 4) ^ (row & 7)) * 16));
-      }
+      for (int o = 0; o < kGroups; ++o) {
+        if (t0 + o >= kBlocks || o != static_cast<int>(group)) continue;
 #pragma unroll
-      for (int i = 0; i < T; ++i)
+        for (int q = 0; q < 4; ++q) {
+          f32x4 sum{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int j = 0; j < T; ++j) {
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], acc[i][j], 0, 0, 0);
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], acc[i][j], 0, 0, 0);
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], acc[i][j], 0, 0, 0);
+          for (int other = 0; other < kGroups; ++other)
+            sum += *reinterpret_cast<const f32x4 *>(
+                space + ((place * kTurn + o) * kGroups + other) * 1024 + lane * 4 + q * 256);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[(t0 + o) / TN][(t0 + o) % TN][4 * q + r] = sum[r];
         }
+      }
+      __syncthreads();
     }
   }
 
   // Lane l holds column l % 32 and, in register r, row 8 (r / 4) + 4 (l / 32) + r % 4 of each
-  // 32 x 32 block: four consecutive rows per register quad.
+  // 32 x 32 block: four consecutive rows per register quad, which x and ga, kept transposed, move
+  // at once.  The halves go through the wave's own part of the shared memory (whose operands have
+  // been read: a barrier ended the sums), by rows and then by columns, and leave as whole lines: 32
+  // hi and 32 lo of a row.
   float *x = reinterpret_cast<float *>(m.scratch + l.x), *ga = reinterpret_cast<float *>(m.scratch + l.ga);
+  constexpr uint32_t kPitch = 36;  // words per line of the wave's 32 x 32 words
+  constexpr int kFinishing = TM * TN < Sh::Groups ? TM * TN : Sh::Groups;  // groups with a block
+  static_assert(Sh::WM * Sh::WN * kFinishing * 32 * kPitch * 4 <= 4 * kStage, "turning space");
+  uint32_t *turned = reinterpret_cast<uint32_t *>(stage) + wave * 32 * kPitch;
 #pragma unroll
-  for (int i = 0; i < T; ++i)
+  for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int j = 0; j < T; ++j) {
-      const uint32_t column = tj * kTile + (wj * T + j) * 32 + (lane & 31);
+    for (int j = 0; j < TN; ++j) {
+      if (Sh::Groups > 1 && (i * TN + j) % Sh::Groups != static_cast<int>(group)) continue;
+      const uint32_t row0 = ti * kTile + (wi * TM + i) * 32, column0 = tj * kTile + (wj * TN + j) * 32;
+      const uint32_t column = column0 + (lane & 31);
+      u32x4 words[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const uint32_t row = ti * kTile + (wi * T + i) * 32 + 8 * q + 4 * (lane >> 5);
-        float v[4];
-        f16x4 hi, lo;
+        const uint32_t at = 8 * q + 4 * (lane >> 5), row = row0 + at;
+        const uint64_t turned_at = static_cast<uint64_t>(column) * m.ps + row;
+        f32x4 v;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          v[r] = acc[i][j][4 * q + r] * kUnscale;
-          if constexpr (S == Step::Poly)
-            v[r] = kB * ga[static_cast<uint64_t>(row + r) * m.ps + column] + kC * v[r];
-          if constexpr (S == Step::Apply || S == Step::Last)
-            v[r] += kA * x[static_cast<uint64_t>(row + r) * m.pl + column];
-          f16 h, w;
-          halves_of(v[r], h, w);
-          hi[r] = h;
-          lo[r] = w;
-        }
+        for (int r = 0; r < 4; ++r) v[r] = acc[i][j][4 * q + r] * kUnscale;
+        if constexpr (S == Step::Poly)
+          v = kB * *reinterpret_cast<const f32x4 *>(ga + turned_at) + kC * v;
+        if constexpr (S == Step::Apply || S == Step::Last)
+          v += kA * *reinterpret_cast<const f32x4 *>(x + turned_at);
         if constexpr (S == Step::Last) {
           const bool tall = m.rows > m.columns;
 #pragma unroll
@@ -301,31 +438,326 @@ __global__ __launch_bounds__(256) void muon_product_kernel(Group g, int odd) {
             *t = m.momentum == nullptr ? v[r] : *t - g.lr * (g.decay * *t + m.scale * v[r]);
           }
         } else {
-          // along the rows, and the transposed entry, four of a row at once
-          f16 *straight = S == Step::Gram ? gs : S == Step::Poly ? bs : xs;
-          f16 *mirror = S == Step::Apply ? to : straight;
-          const uint32_t k_straight = S == Step::Apply ? m.pl : m.ps;
+          if constexpr (S == Step::Apply) *reinterpret_cast<f32x4 *>(x + turned_at) = v;
+          if constexpr (S == Step::Gram) *reinterpret_cast<f32x4 *>(ga + turned_at) = v;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            f16 *p = straight + halves_at(row + r, column, k_straight);
-            p[0] = hi[r];
-            p[32] = lo[r];
-            if constexpr (S == Step::Apply)
-              x[static_cast<uint64_t>(row + r) * m.pl + column] = v[r];
-            if constexpr (S == Step::Gram)
-              ga[static_cast<uint64_t>(row + r) * m.ps + column] = v[r];
-          }
-          if (S == Step::Apply || ti != tj) {
-            f16 *p = mirror + halves_at(column, row, m.ps);
-            *reinterpret_cast<f16x4 *>(p) = hi;
-            *reinterpret_cast<f16x4 *>(p + 32) = lo;
-            if constexpr (S == Step::Gram)
-              *reinterpret_cast<float4 *>(ga + static_cast<uint64_t>(column) * m.ps + row) =
-                  make_float4(v[0], v[1], v[2], v[3]);
+            words[q][r] = halves_word(v[r]);
+            turned[(at + r) * kPitch + (lane & 31)] = words[q][r];
           }
         }
       }
+      if constexpr (S != Step::Last) {
+        f16 *straight = S == Step::Gram ? gs : S == Step::Poly ? bs : xs;
+        f16 *mirror = S == Step::Apply ? to : straight;
+        __builtin_amdgcn_wave_barrier();
+        const uint32_t *line = turned + (lane >> 1) * kPitch + (lane & 1) * 16;
+        store_line(line,
+                   straight + halves_at(row0 + (lane >> 1), column0 + (lane & 1) * 16,
+                                        S == Step::Apply ? m.pl : m.ps));
+        __builtin_amdgcn_wave_barrier();
+        if (S == Step::Apply || ti != tj) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<u32x4 *>(turned + (lane & 31) * kPitch + 8 * q + 4 * (lane >> 5)) =
+                words[q];
+          __builtin_amdgcn_wave_barrier();
+          store_line(line,
+                     mirror + halves_at(column0 + (lane >> 1), row0 + (lane & 1) * 16, m.ps));
+          __builtin_amdgcn_wave_barrier();
+        }
+      }
     }
+}
+
+// ---------------------------------------------------------------- one block per matrix
+//
+// A matrix whose X' in halves fits the shared memory of a compute unit is stepped from start to end
+// by one block of 12 waves, X staying in registers.  Each wave owns blocks of 16 columns of X
+// (along its long side), as 16 x 16 results of the matrix cores: lane l holds column l % 16 and, of
+// row block r, rows 16 r + 4 (l / 16) .. + 3.  Summed indexes are taken 32 at a time in the order
+// 16 r + 4 (l / 16) + i that this gives: a pair of row blocks is then an operand of B X as it lies,
+// and transposed reads of the shared memory (16 lanes fetch 4 rows of 16 float16 and each gets a
+// column of 4) give the same order for X X'.
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+constexpr int kWhole = 163840;  // bytes of shared memory, the last for the norm's parts
+constexpr int kWholeWaves = 12;
+// X': bytes of a row of PS values in halves (hi, then lo), an odd number of 32-byte steps, so that
+// eight rows lie in different banks; every other eight rows have the 16-byte halves of each step
+// exchanged, so that sixteen rows' stores do too.
+constexpr int whole_pitch(int ps) { return ps * 4 + 32; }
+// A and B: for each lane quad the rows' pieces of 16 bytes that it reads (per 32 summed values, hi
+// and lo), an odd number of them to a row.
+constexpr int square_pitch(int ps) { return (ps / 16 + 1) * 16; }
+constexpr int square_bytes(int ps) { return 4 * ps * square_pitch(ps); }
+
+__device__ __forceinline__ f16x8 join(s16x4 a, s16x4 b) {
+  return __builtin_bit_cast(f16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+// Four values as hi and lo.
+__device__ __forceinline__ void halves_of(const f32x4 &v, s16x4 &hi, s16x4 &lo) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    f16 h, w;
+    halves_of(v[r], h, w);
+    hi[r] = __builtin_bit_cast(short, h);
+    lo[r] = __builtin_bit_cast(short, w);
+  }
+}
+
+// acc += a b' in halves.
+__device__ __forceinline__ void multiply(const f16x8 (&a)[2], const f16x8 (&b)[2], f32x4 &acc) {
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[1], b[0], acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[0], b[1], acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[0], b[0], acc, 0, 0, 0);
+}
+
+template <int PS, int Blocks>
+__global__ __launch_bounds__(64 * kWholeWaves) void muon_whole_kernel(Group g, uint32_t rounds) {
+  __shared__ __attribute__((aligned(16))) char shared[kWhole];
+  float *const parts = reinterpret_cast<float *>(shared + kWhole - 4 * kWholeWaves);
+  constexpr int kRowBlocks = PS / 16, kPitch = whole_pitch(PS), kSquare = square_pitch(PS);
+  constexpr int kSide = PS / 32, kTiles = kSide * (kSide + 1) / 2;  // of 32 x 32, lower ones of A
+  constexpr int kSplits = kWholeWaves / kTiles;                     // of the sums of A
+  // X' first; then, over it, the sums to be joined, A and B
+  char *const sums = shared, *const sa = shared + kTiles * (kSplits - 1) * 4096,
+              *const sb = sa + square_bytes(PS);
+  static_assert(kTiles * (kSplits - 1) * 4096 + 2 * square_bytes(PS) <= kWhole, "shared memory");
+  const Matrix &m = g.m[blockIdx.x];
+  const bool tall = m.rows > m.columns;
+  const uint32_t s = tall ? m.columns : m.rows, n = tall ? m.rows : m.columns;
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
+  const uint32_t column_blocks = (n + 31) / 32 * 2;
+  // The matrix lies in the shared memory as in memory, its rows an odd number of words apart, on
+  // the way in and out: fn(offset there, offset in memory) for each of this thread's elements.
+  float *const words = reinterpret_cast<float *>(shared);
+  const uint32_t pitch = m.columns | 1;
+  auto each = [&](auto fn) {
+    constexpr uint32_t kThreads = 64 * kWholeWaves;
+    const uint32_t rows_on = kThreads / m.columns, columns_on = kThreads % m.columns;
+    uint32_t row = threadIdx.x / m.columns, column = threadIdx.x % m.columns;
+    for (uint32_t at = threadIdx.x; at < m.rows * m.columns; at += kThreads) {
+      fn(row * pitch + column, at);
+      row += rows_on;
+      column += columns_on;
+      if (column >= m.columns) column -= m.columns, ++row;
+    }
+  };
+  const uint32_t step_i = tall ? 1 : pitch, step_j = tall ? pitch : 1;
+
+  float squares = 0.0f;
+  each([&](uint32_t to, uint32_t at) {
+    float v = m.gradient[at];
+    if (m.momentum != nullptr) {
+      const float now = g.momentum * m.momentum[at] + v;
+      m.momentum[at] = now;
+      v = g.nesterov ? v + g.momentum * now : now;
+    }
+    words[to] = v;
+    squares = fmaf(v, v, squares);
+  });
+  float one[1] = {squares};
+  oxh::wave_sums_rows(one);
+  if (lane == 0) parts[wave] = one[0];
+  __syncthreads();
+  float total = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kWholeWaves; ++w) total += parts[w];
+  const float norm = sqrtf(total) + g.epsilon;
+  f32x4 x[Blocks][kRowBlocks];
+#pragma unroll
+  for (int c = 0; c < Blocks; ++c) {
+    const uint32_t j = (c * kWholeWaves + wave) * 16 + col;
+#pragma unroll
+    for (int r = 0; r < kRowBlocks; ++r)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t i = 16 * r + 4 * quad + e;
+        x[c][r][e] = i < s && j < n ? words[i * step_i + j * step_j] / norm : 0.0f;
+      }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  __syncthreads();
+
+  // this wave's tile of A and its share of the sum
+  const uint32_t tile = wave % kTiles, split = wave / kTiles;
+  uint32_t ti = 0;
+  while ((ti + 1) * (ti + 2) / 2 <= tile) ++ti;
+  const uint32_t tj = tile - ti * (ti + 1) / 2;
+
+  for (uint32_t round = 0; round < rounds; ++round) {
+#pragma unroll
+    for (int c = 0; c < Blocks; ++c) {
+      const uint32_t block = c * kWholeWaves + wave;
+      if (block >= column_blocks) continue;
+      char *row = shared + (block * 16 + col) * kPitch + ((quad * 8) ^ ((col & 8) * 2));
+#pragma unroll
+      for (int r = 0; r < kRowBlocks; ++r) {
+        s16x4 hi, lo;
+        halves_of(x[c][r], hi, lo);
+        *reinterpret_cast<s16x4 *>(row + 32 * r) = hi;
+        *reinterpret_cast<s16x4 *>(row + 2 * PS + 32 * r) = lo;
+      }
+    }
+    __syncthreads();
+
+    f32x4 acc[2][2] = {};
+    if (split < kSplits) {
+      // rows 32 t + 16 b of X as an operand: column 16 b + .. of the rows of X' in shared memory
+      auto operand = [&](uint32_t k, uint32_t t, int b, f16x8(&out)[2]) {
+        const char *p = shared + (k * 32 + quad * 4 + (col >> 2)) * kPitch + (t * 32 + b * 16) * 2 +
+                        (((col & 3) * 8) ^ ((quad & 2) * 8));
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          out[h] = join(__builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (lds_s16x4 *)(p + h * 2 * PS)),
+                        __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (lds_s16x4 *)(p + h * 2 * PS + 16 * kPitch)));
+      };
+      for (uint32_t k = split; k < column_blocks / 2; k += kSplits) {
+        f16x8 a[2][2], b[2][2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) operand(k, ti, i, a[i]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) operand(k, tj, j, b[j]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) multiply(a[i], b[j], acc[i][j]);
+      }
+    }
+    __syncthreads();
+    if constexpr (kSplits > 1) {
+      f32x4 *mine = reinterpret_cast<f32x4 *>(sums) + ((split - 1) * kTiles + tile) * 256 + lane;
+      if (split != 0 && split < kSplits) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) mine[q * 64] = acc[q >> 1][q & 1];
+      }
+      __syncthreads();
+      if (split == 0) {
+        const f32x4 *other = reinterpret_cast<const f32x4 *>(sums) + tile * 256 + lane;
+#pragma unroll
+        for (int p = 0; p < kSplits - 1; ++p)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) acc[q >> 1][q & 1] += other[p * kTiles * 256 + q * 64];
+      }
+    }
+    // block (i, j) of this wave's tile of A or B to the columns' rows of `to` and, off the
+    // diagonal, to the rows' rows: there two lanes with neighbouring columns share their four rows'
+    // words
+    auto keep = [&](char *to, const f32x4 &v, int i, int j) {
+      s16x4 hi, lo;
+      halves_of(v, hi, lo);
+      char *p = to + (quad * PS + tj * 32 + j * 16 + col) * kSquare + ti * 32 + i * 8;
+      *reinterpret_cast<s16x4 *>(p) = hi;
+      *reinterpret_cast<s16x4 *>(p + 16) = lo;
+      if (ti == tj) return;  // both lie in this tile
+      const u32x2 mine[2] = {__builtin_bit_cast(u32x2, hi), __builtin_bit_cast(u32x2, lo)};
+      const bool odd = col & 1;
+      char *q = to + ((col >> 2) * PS + ti * 32 + i * 16 + quad * 4 + (odd ? 2 : 0)) * kSquare +
+                tj * 32 + j * 8 + (col & 2) * 2;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        // the pair of rows this lane stores, of its own column and the neighbour's
+        const uint32_t kept = odd ? mine[h][1] : mine[h][0], sent = odd ? mine[h][0] : mine[h][1];
+        const uint32_t got = static_cast<uint32_t>(
+            __builtin_amdgcn_update_dpp(0, static_cast<int>(sent), 0xB1, 0xF, 0xF, false));
+        const uint32_t first = odd ? got : kept, second = odd ? kept : got;
+        *reinterpret_cast<uint32_t *>(q + h * 16) = (first & 0xFFFFu) | second << 16;
+        *reinterpret_cast<uint32_t *>(q + h * 16 + kSquare) = first >> 16 | (second & 0xFFFF0000u);
+      }
+    };
+    // 16 rows of A or B as an operand
+    auto rows_of = [&](const char *from, uint32_t row, int k, f16x8(&out)[2]) {
+      const char *p = from + (quad * PS + row + col) * kSquare + k * 32;
+      out[0] = *reinterpret_cast<const f16x8 *>(p);
+      out[1] = *reinterpret_cast<const f16x8 *>(p + 16);
+    };
+    if (split == 0) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          acc[i][j] *= kUnscale;
+          keep(sa, acc[i][j], i, j);
+        }
+    }
+    __syncthreads();
+    if (split == 0) {
+      f32x4 square[2][2] = {};
+#pragma unroll
+      for (int k = 0; k < kSide; ++k) {
+        f16x8 a[2][2], b[2][2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) rows_of(sa, ti * 32 + i * 16, k, a[i]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) rows_of(sa, tj * 32 + j * 16, k, b[j]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) multiply(a[i], b[j], square[i][j]);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          keep(sb, kB * acc[i][j] + kC * (square[i][j] * kUnscale), i, j);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < Blocks; ++c) {
+      if (static_cast<uint32_t>(c * kWholeWaves) + wave >= column_blocks) continue;
+      f16x8 b[kSide][2];
+#pragma unroll
+      for (int k = 0; k < kSide; ++k) {
+        s16x4 h0, l0, h1, l1;
+        halves_of(x[c][2 * k], h0, l0);
+        halves_of(x[c][2 * k + 1], h1, l1);
+        b[k][0] = join(h0, h1);
+        b[k][1] = join(l0, l1);
+      }
+#pragma unroll
+      for (int r = 0; r < kRowBlocks; ++r) {
+        f32x4 sum = {};
+#pragma unroll
+        for (int k = 0; k < kSide; ++k) {
+          f16x8 a[2];
+          rows_of(sb, r * 16, k, a);
+          multiply(a, b[k], sum);
+        }
+        x[c][r] = kA * x[c][r] + sum * kUnscale;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __syncthreads();
+  }
+  uint32_t again = col;  // so that no offset is kept from the way in
+  asm volatile("" : "+v"(again));
+#pragma unroll
+  for (int c = 0; c < Blocks; ++c) {
+    const uint32_t j = (c * kWholeWaves + wave) * 16 + again;
+#pragma unroll
+    for (int r = 0; r < kRowBlocks; ++r)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t i = 16 * r + 4 * quad + e;
+        if (i < s && j < n) words[i * step_i + j * step_j] = x[c][r][e];
+      }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  __syncthreads();
+  each([&](uint32_t from, uint32_t at) {
+    const float v = words[from];
+    if (m.momentum == nullptr) {
+      m.target[at] = v;
+    } else {
+      const float w = m.target[at];
+      m.target[at] = w - g.lr * (g.decay * w + m.scale * v);
+    }
+  });
 }
 
 // ---------------------------------------------------------------- host
@@ -338,15 +770,34 @@ struct Item {
 
 uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
 
-// Tile side for a launch group: 128 where its products then still have a tile for every compute
-// unit, else 64.
+// Whether one block steps the whole matrix: the rows of the shared memory that hold X', and at most
+// Blocks column blocks per wave.
+constexpr int whole_blocks(int ps) { return ps == 32 ? 6 : ps == 64 ? 3 : 2; }
+bool whole(const Item &it) {
+  const uint64_t s = std::min(it.rows, it.columns), n = std::max(it.rows, it.columns);
+  if (s > 128) return false;
+  const int ps = static_cast<int>(round_up(s, 32));
+  return round_up(n, 32) * whole_pitch(ps) <= kWhole - 4 * kWholeWaves &&
+         round_up(n, 32) <= 16ull * kWholeWaves * whole_blocks(ps);
+}
+
+// Tile side for a launch group, by the tiles that A has (the product that fills the chip least):
+// 128 where it has at least one for every other compute unit (12 x 1024 x 1024: 1325 us, 1558 with
+// 64; 2048 x 2048 with 136 tiles: 821 and 1027), else 64 (1536 x 1536 with 78: 541 us, 581 with
+// 128; 1000 x 1280: 280 and 441); 192 where its tiles just fill one round of one block per compute
+// unit (4096 x 4096 with 253: 4.49 ms, 4.97 with 128; 6144 x 6144 with 528: 14.96 and 14.71).
 uint32_t tile_of(const Item *items, size_t count) {
-  uint64_t tiles = 0;
-  for (size_t i = 0; i < count; ++i) {
-    const uint64_t s = round_up(std::min(items[i].rows, items[i].columns), 128) / 128;
-    tiles += s * (s + 1) / 2;
-  }
-  return tiles >= oxh::kComputeUnits ? 128 : 64;
+  auto tiles = [&](uint64_t tile) {
+    uint64_t n = 0;
+    for (size_t i = 0; i < count; ++i) {
+      const uint64_t s = round_up(std::min(items[i].rows, items[i].columns), tile) / tile;
+      n += s * (s + 1) / 2;
+    }
+    return n;
+  };
+  const uint64_t wide = tiles(Wide::tile), units = oxh::kComputeUnits;
+  if (wide <= units && wide * 8 >= units * 7) return Wide::tile;
+  return tiles(Medium::tile) * 2 >= units ? Medium::tile : Small::tile;
 }
 
 uint64_t scratch_of(const Item *items, size_t count) {
@@ -360,10 +811,20 @@ uint64_t scratch_of(const Item *items, size_t count) {
   return total;
 }
 
-uint64_t scratch_of_all(const std::vector<Item> &items) {
-  uint64_t most = 256;
-  for (size_t at = 0; at < items.size(); at += kGroup)
-    most = std::max(most, scratch_of(&items[at], std::min<size_t>(kGroup, items.size() - at)));
+// The matrices that one block does not take, and those it takes.
+struct Parted {
+  std::vector<Item> large, small;
+};
+Parted part(const std::vector<Item> &items) {
+  Parted p;
+  for (const Item &it : items) (whole(it) ? p.small : p.large).push_back(it);
+  return p;
+}
+
+uint64_t scratch_of_all(const std::vector<Item> &large) {
+  uint64_t most = 0;
+  for (size_t at = 0; at < large.size(); at += kGroup)
+    most = std::max(most, scratch_of(&large[at], std::min<size_t>(kGroup, large.size() - at)));
   return most;
 }
 
@@ -375,10 +836,14 @@ oxh_status product(hipStream_t stream, Group &g, uint32_t tile, int odd, const c
     g.m[i].first_block = g.blocks;
     g.blocks += S == Step::Gram || S == Step::Poly ? s * (s + 1) / 2 : s * l;
   }
-  if (tile == 128)
-    oxh::launch(muon_product_kernel<S, 2>, dim3(g.blocks), dim3(256), 0, stream, g, odd);
-  else
-    oxh::launch(muon_product_kernel<S, 1>, dim3(g.blocks), dim3(256), 0, stream, g, odd);
+  auto start = [&](auto shape) {
+    using Sh = decltype(shape);
+    oxh::launch(muon_product_kernel<S, Sh>, dim3(g.blocks), dim3(Sh::threads), 0, stream,
+                g, odd);
+  };
+  if (tile == Wide::tile) start(Wide());
+  else if (tile == Medium::tile) start(Medium());
+  else start(Small());
   return oxh::launched(what);
 }
 
@@ -410,38 +875,78 @@ struct Hyper {
   bool nesterov;
 };
 
-oxh_status run_all(hipStream_t stream, const std::vector<Item> &items, const Hyper &h,
-                   uint32_t rounds, char *workspace) {
-  for (size_t at = 0; at < items.size(); at += kGroup) {
-    const size_t count = std::min<size_t>(kGroup, items.size() - at);
-    const uint32_t tile = tile_of(&items[at], count);
-    Group g{};
+void describe(const Item &it, Matrix &m) {
+  m.gradient = it.gradient;
+  m.momentum = it.momentum;
+  m.target = it.target;
+  m.rows = static_cast<uint32_t>(it.rows);
+  m.columns = static_cast<uint32_t>(it.columns);
+  m.scale =
+      std::sqrt(std::max(1.0f, static_cast<float>(it.rows) / static_cast<float>(it.columns)));
+}
+
+// Launches the small matrices with sides in this class, a group at a time.
+template <int PS, int Blocks>
+oxh_status run_whole(hipStream_t stream, const std::vector<Item> &small, Group g,
+                     uint32_t rounds) {
+  g.count = 0;
+  auto flush = [&]() {
+    if (g.count == 0) return oxh::ok();
+    oxh::launch(muon_whole_kernel<PS, Blocks>, dim3(g.count), dim3(64 * kWholeWaves), 0, stream, g,
+                rounds);
+    g.count = 0;
+    return oxh::launched("muon_whole");
+  };
+  for (const Item &it : small) {
+    const uint64_t s = std::min(it.rows, it.columns), n = std::max(it.rows, it.columns);
+    const bool few = round_up(n, 32) <= 16ull * kWholeWaves;
+    if (round_up(s, 32) != PS || few != (Blocks == 1)) continue;
+    describe(it, g.m[g.count++]);
+    if (g.count == kGroup) {
+      oxh_status st = flush();
+      if (st != OXH_OK) return st;
+    }
+  }
+  return flush();
+}
+
+oxh_status run_all(hipStream_t stream, const Parted &items, const Hyper &h, uint32_t rounds,
+                   char *workspace) {
+  Group g{};
+  g.momentum = h.momentum;
+  g.lr = h.lr;
+  g.decay = h.decay;
+  g.epsilon = h.epsilon;
+  g.nesterov = h.nesterov ? 1 : 0;
+  oxh_status st = oxh::ok();
+  const std::vector<Item> &small = items.small, &large = items.large;
+  if (!small.empty()) {
+    st = run_whole<32, 1>(stream, small, g, rounds);
+    if (st == OXH_OK) st = run_whole<32, whole_blocks(32)>(stream, small, g, rounds);
+    if (st == OXH_OK) st = run_whole<64, 1>(stream, small, g, rounds);
+    if (st == OXH_OK) st = run_whole<64, whole_blocks(64)>(stream, small, g, rounds);
+    if (st == OXH_OK) st = run_whole<96, 1>(stream, small, g, rounds);
+    if (st == OXH_OK) st = run_whole<96, whole_blocks(96)>(stream, small, g, rounds);
+    if (st == OXH_OK) st = run_whole<128, 1>(stream, small, g, rounds);
+    if (st == OXH_OK) st = run_whole<128, whole_blocks(128)>(stream, small, g, rounds);
+  }
+  for (size_t at = 0; at < large.size() && st == OXH_OK; at += kGroup) {
+    const size_t count = std::min<size_t>(kGroup, large.size() - at);
+    const uint32_t tile = tile_of(&large[at], count);
     g.count = static_cast<uint32_t>(count);
-    g.momentum = h.momentum;
-    g.lr = h.lr;
-    g.decay = h.decay;
-    g.epsilon = h.epsilon;
-    g.nesterov = h.nesterov ? 1 : 0;
     uint64_t offset = 0;
     for (size_t i = 0; i < count; ++i) {
-      const Item &it = items[at + i];
+      const Item &it = large[at + i];
       Matrix &m = g.m[i];
-      m.gradient = it.gradient;
-      m.momentum = it.momentum;
-      m.target = it.target;
+      describe(it, m);
       m.scratch = workspace + offset;
-      m.rows = static_cast<uint32_t>(it.rows);
-      m.columns = static_cast<uint32_t>(it.columns);
       m.ps = static_cast<uint32_t>(round_up(std::min(it.rows, it.columns), tile));
       m.pl = static_cast<uint32_t>(round_up(std::max(it.rows, it.columns), tile));
-      m.scale = std::sqrt(std::max(1.0f, static_cast<float>(it.rows) /
-                                             static_cast<float>(it.columns)));
       offset += round_up(layout_of(m.ps, m.pl).total, 256);
     }
-    oxh_status st = run_group(stream, g, tile, rounds);
-    if (st != OXH_OK) return st;
+    st = run_group(stream, g, tile, rounds);
   }
-  return oxh::ok();
+  return st;
 }
 
 // Sides whose tiles and block counts fit 32 bits.
@@ -466,8 +971,19 @@ oxh_status items_of(const oxh_muon_tensor *tensors, uint32_t count, std::vector<
 
 bool aligned4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 
+// Runs a C entry's body; what its containers may throw becomes a status.
+template <typename Body>
+oxh_status guarded(Body body) {
+  try {
+    return body();
+  } catch (const std::exception &e) {
+    return oxh::fail(OXH_EXECUTION, e.what());
+  }
+}
+
 oxh_status check_workspace(uint64_t needed, const void *workspace, uint64_t bytes) {
-  OXH_REQUIRE(workspace != nullptr && bytes >= needed && oxh::aligned16(workspace),
+  OXH_REQUIRE(needed == 0 || (workspace != nullptr && bytes >= needed &&
+                              oxh::aligned16(workspace)),
               OXH_INVALID_SHAPE, "muon: workspace too small or misaligned");
   return oxh::ok();
 }
@@ -478,104 +994,114 @@ extern "C" {
 
 oxh_status oxh_orthogonalize_workspace_size(uint64_t count, uint64_t rows, uint64_t columns,
                                             uint64_t *bytes) {
-  OXH_REQUIRE(bytes != nullptr, OXH_INVALID_SHAPE, "bytes is null");
-  *bytes = 256;
-  if (count == 0) return oxh::ok();
-  oxh_status st = check_sides(rows, columns);
-  if (st != OXH_OK) return st;
-  OXH_REQUIRE(count <= 65536, OXH_INVALID_SHAPE, "orthogonalize: too many matrices");
-  *bytes = scratch_of_all(std::vector<Item>(count, Item{nullptr, nullptr, nullptr, rows, columns}));
-  return oxh::ok();
+  return guarded([&]() -> oxh_status {
+    OXH_REQUIRE(bytes != nullptr, OXH_INVALID_SHAPE, "bytes is null");
+    *bytes = 0;
+    if (count == 0) return oxh::ok();
+    oxh_status st = check_sides(rows, columns);
+    if (st != OXH_OK) return st;
+    OXH_REQUIRE(count <= 65536, OXH_INVALID_SHAPE, "orthogonalize: too many matrices");
+    *bytes = scratch_of_all(
+        part(std::vector<Item>(count, Item{nullptr, nullptr, nullptr, rows, columns})).large);
+    return oxh::ok();
+  });
 }
 
 oxh_status oxh_orthogonalize(oxh_stream stream, uint64_t count, uint64_t rows, uint64_t columns,
                              uint32_t rounds, float epsilon, const float *input, float *output,
                              void *workspace, uint64_t workspace_bytes) {
-  uint64_t needed = 0;
-  oxh_status st = oxh_orthogonalize_workspace_size(count, rows, columns, &needed);
-  if (st != OXH_OK) return st;
-  OXH_REQUIRE(rounds >= 1 && rounds <= 64, OXH_INVALID_SHAPE,
-              "orthogonalize: rounds outside 1..64");
-  OXH_REQUIRE(std::isfinite(epsilon) && epsilon > 0.0f, OXH_EXECUTION,
-              "orthogonalize: epsilon must be positive and finite");
-  if (count == 0) return oxh::ok();
-  OXH_REQUIRE(input != nullptr && output != nullptr && aligned4(input) && aligned4(output),
-              OXH_INVALID_SHAPE, "orthogonalize: null or misaligned pointer");
-  st = check_workspace(needed, workspace, workspace_bytes);
-  if (st != OXH_OK) return st;
-  const uint64_t bytes = count * rows * columns * 4;
-  OXH_REQUIRE(!oxh::any_overlap(input, bytes, output, bytes) &&
-                  !oxh::any_overlap(workspace, needed, input, bytes) &&
-                  !oxh::any_overlap(workspace, needed, output, bytes),
-              OXH_INVALID_SHAPE, "orthogonalize: buffers overlap");
-  std::vector<Item> items;
-  for (uint64_t i = 0; i < count; ++i)
-    items.push_back({input + i * rows * columns, nullptr, output + i * rows * columns, rows,
-                     columns});
-  return run_all(oxh::as_stream(stream), items, {0.0f, 0.0f, 0.0f, epsilon, false}, rounds,
-                 static_cast<char *>(workspace));
+  return guarded([&]() -> oxh_status {
+    uint64_t needed = 0;
+    oxh_status st = oxh_orthogonalize_workspace_size(count, rows, columns, &needed);
+    if (st != OXH_OK) return st;
+    OXH_REQUIRE(rounds >= 1 && rounds <= 64, OXH_INVALID_SHAPE,
+                "orthogonalize: rounds outside 1..64");
+    OXH_REQUIRE(std::isfinite(epsilon) && epsilon > 0.0f, OXH_EXECUTION,
+                "orthogonalize: epsilon must be positive and finite");
+    if (count == 0) return oxh::ok();
+    OXH_REQUIRE(input != nullptr && output != nullptr && aligned4(input) && aligned4(output),
+                OXH_INVALID_SHAPE, "orthogonalize: null or misaligned pointer");
+    st = check_workspace(needed, workspace, workspace_bytes);
+    if (st != OXH_OK) return st;
+    const uint64_t bytes = count * rows * columns * 4;
+    OXH_REQUIRE(!oxh::any_overlap(input, bytes, output, bytes) &&
+                    (needed == 0 || (!oxh::any_overlap(workspace, needed, input, bytes) &&
+                                     !oxh::any_overlap(workspace, needed, output, bytes))),
+                OXH_INVALID_SHAPE, "orthogonalize: buffers overlap");
+    std::vector<Item> items;
+    for (uint64_t i = 0; i < count; ++i)
+      items.push_back({input + i * rows * columns, nullptr, output + i * rows * columns, rows,
+                       columns});
+    return run_all(oxh::as_stream(stream), part(items), {0.0f, 0.0f, 0.0f, epsilon, false}, rounds,
+                   static_cast<char *>(workspace));
+  });
 }
 
 oxh_status oxh_muon_workspace_size(const oxh_muon_tensor *tensors, uint32_t count,
                                    uint64_t *bytes) {
-  OXH_REQUIRE(bytes != nullptr, OXH_INVALID_SHAPE, "bytes is null");
-  std::vector<Item> items;
-  oxh_status st = items_of(tensors, count, items);
-  if (st != OXH_OK) return st;
-  *bytes = scratch_of_all(items);
-  return oxh::ok();
+  return guarded([&]() -> oxh_status {
+    OXH_REQUIRE(bytes != nullptr, OXH_INVALID_SHAPE, "bytes is null");
+    std::vector<Item> items;
+    oxh_status st = items_of(tensors, count, items);
+    if (st != OXH_OK) return st;
+    *bytes = scratch_of_all(part(items).large);
+    return oxh::ok();
+  });
 }
 
 oxh_status oxh_muon_multi_tensor(oxh_stream stream, float learning_rate, float weight_decay,
                                  float momentum, int nesterov, float epsilon, uint32_t rounds,
                                  const oxh_muon_tensor *tensors, uint32_t count, void *workspace,
                                  uint64_t workspace_bytes) {
-  OXH_REQUIRE(std::isfinite(learning_rate) && std::isfinite(weight_decay) &&
-                  std::isfinite(momentum),
-              OXH_INVALID_SHAPE, "muon: hyper-parameters must be finite");
-  OXH_REQUIRE(rounds >= 1 && rounds <= 64, OXH_INVALID_SHAPE, "muon: rounds outside 1..64");
-  OXH_REQUIRE(std::isfinite(epsilon) && epsilon > 0.0f, OXH_EXECUTION,
-              "muon: epsilon must be positive and finite");
-  std::vector<Item> items;
-  oxh_status st = items_of(tensors, count, items);
-  if (st != OXH_OK) return st;
-  if (count == 0) return oxh::ok();
-  const uint64_t needed = scratch_of_all(items);
-  st = check_workspace(needed, workspace, workspace_bytes);
-  if (st != OXH_OK) return st;
-  // every written range against every other range: sorted by address, neighbours may not meet
-  // unless both are read only
-  struct Range {
-    uintptr_t begin, end;
-    bool written;
-  };
-  std::vector<Range> ranges;
-  auto add = [&](const void *p, uint64_t bytes, bool written) {
-    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
-    ranges.push_back({at, at + bytes, written});
-  };
-  add(workspace, needed, true);
-  for (const Item &it : items) {
-    OXH_REQUIRE(it.gradient != nullptr && it.momentum != nullptr && it.target != nullptr &&
-                    aligned4(it.gradient) && aligned4(it.momentum) && aligned4(it.target),
-                OXH_INVALID_SHAPE, "muon: null or misaligned pointer");
-    const uint64_t bytes = it.rows * it.columns * 4;
-    add(it.gradient, bytes, false);
-    add(it.momentum, bytes, true);
-    add(it.target, bytes, true);
-  }
-  std::sort(ranges.begin(), ranges.end(),
-            [](const Range &a, const Range &b) { return a.begin < b.begin; });
-  uintptr_t end_any = 0, end_written = 0;
-  for (const Range &r : ranges) {
-    OXH_REQUIRE(r.begin >= end_written && (!r.written || r.begin >= end_any), OXH_INVALID_SHAPE,
-                "muon: a buffer that is written overlaps another");
-    end_any = std::max(end_any, r.end);
-    if (r.written) end_written = std::max(end_written, r.end);
-  }
-  return run_all(oxh::as_stream(stream), items,
-                 {learning_rate, weight_decay, momentum, epsilon, nesterov != 0}, rounds,
-                 static_cast<char *>(workspace));
+  return guarded([&]() -> oxh_status {
+    OXH_REQUIRE(std::isfinite(learning_rate) && std::isfinite(weight_decay) &&
+                    std::isfinite(momentum),
+                OXH_INVALID_SHAPE, "muon: hyper-parameters must be finite");
+    OXH_REQUIRE(rounds >= 1 && rounds <= 64, OXH_INVALID_SHAPE, "muon: rounds outside 1..64");
+    OXH_REQUIRE(std::isfinite(epsilon) && epsilon > 0.0f, OXH_EXECUTION,
+                "muon: epsilon must be positive and finite");
+    std::vector<Item> items;
+    oxh_status st = items_of(tensors, count, items);
+    if (st != OXH_OK) return st;
+    if (count == 0) return oxh::ok();
+    const Parted parted = part(items);
+    const uint64_t needed = scratch_of_all(parted.large);
+    st = check_workspace(needed, workspace, workspace_bytes);
+    if (st != OXH_OK) return st;
+    // every written range against every other range: sorted by address, neighbours may not meet
+    // unless both are read only
+    struct Range {
+      uintptr_t begin, end;
+      bool written;
+    };
+    std::vector<Range> ranges;
+    auto add = [&](const void *p, uint64_t bytes, bool written) {
+      const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+      ranges.push_back({at, at + bytes, written});
+    };
+    if (needed != 0) add(workspace, needed, true);
+    for (const Item &it : items) {
+      OXH_REQUIRE(it.gradient != nullptr && it.momentum != nullptr && it.target != nullptr &&
+                      aligned4(it.gradient) && aligned4(it.momentum) && aligned4(it.target),
+                  OXH_INVALID_SHAPE, "muon: null or misaligned pointer");
+      const uint64_t bytes = it.rows * it.columns * 4;
+      add(it.gradient, bytes, false);
+      add(it.momentum, bytes, true);
+      add(it.target, bytes, true);
+    }
+    std::sort(ranges.begin(), ranges.end(),
+              [](const Range &a, const Range &b) { return a.begin < b.begin; });
+    uintptr_t end_any = 0, end_written = 0;
+    for (const Range &r : ranges) {
+      OXH_REQUIRE(r.begin >= end_written && (!r.written || r.begin >= end_any), OXH_INVALID_SHAPE,
+                  "muon: a buffer that is written overlaps another");
+      end_any = std::max(end_any, r.end);
+      if (r.written) end_written = std::max(end_written, r.end);
+    }
+    return run_all(oxh::as_stream(stream), parted,
+                   {learning_rate, weight_decay, momentum, epsilon, nesterov != 0}, rounds,
+                   static_cast<char *>(workspace));
+  });
 }
 
 }  // extern "C"
