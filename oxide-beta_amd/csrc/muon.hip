@@ -97,26 +97,58 @@ __device__ __forceinline__ float direction(const Group &g, const Matrix &m, uint
   return g.nesterov ? grad + g.momentum * mom : mom;
 }
 
-// M = mu M + G, and the partial sums of V^2: block p of a matrix's kNormParts (or fewer, the
-// others then 0) takes every parts-th run of 256 elements.
-__global__ __launch_bounds__(256) void muon_norm_kernel(Group g) {
-  __shared__ float wave[4];
+// M = mu M + G, and the partial sums of V^2: block p of a matrix's kNormParts takes every parts-th
+// run of a block's elements, four per thread where `packed` (the pointers are 16-byte aligned; the
+// last n % 4 elements are the first block's).
+constexpr int kNormThreads = 1024;
+__global__ __launch_bounds__(kNormThreads) void muon_norm_kernel(Group g) {
+  __shared__ float wave[kNormThreads / 64];
   const Matrix &m = matrix_of(g, blockIdx.x);
   const uint32_t part = blockIdx.x - m.first_block;
   const uint64_t n = static_cast<uint64_t>(m.rows) * m.columns;
+  const bool packed = ((reinterpret_cast<uintptr_t>(m.gradient) |
+                        reinterpret_cast<uintptr_t>(m.momentum)) & 15u) == 0;
   float sum = 0.0f;
-  for (uint64_t i = part * 256ull + threadIdx.x; i < n; i += kNormParts * 256ull) {
-    if (m.momentum != nullptr) m.momentum[i] = g.momentum * m.momentum[i] + m.gradient[i];
-    const float v = direction(g, m, i);
+  auto take = [&](float grad, float &mom) {
+    float v = grad;
+    if (m.momentum != nullptr) {
+      mom = g.momentum * mom + grad;
+      v = g.nesterov ? grad + g.momentum * mom : mom;
+    }
     sum = fmaf(v, v, sum);
+  };
+  const uint64_t packs = packed ? n / 4 : 0;
+  const f32x4 *gradient = reinterpret_cast<const f32x4 *>(m.gradient);
+  f32x4 *momentum = reinterpret_cast<f32x4 *>(m.momentum);
+#pragma unroll 4
+  for (uint64_t i = part * static_cast<uint64_t>(kNormThreads) + threadIdx.x; i < packs;
+       i += static_cast<uint64_t>(kNormParts) * kNormThreads) {
+    f32x4 mom{0.0f, 0.0f, 0.0f, 0.0f};
+    const f32x4 grad = gradient[i];
+    if (momentum != nullptr) mom = momentum[i];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float one = mom[e];
+      take(grad[e], one);
+      mom[e] = one;
+    }
+    if (momentum != nullptr) momentum[i] = mom;
+  }
+  for (uint64_t i = packs * 4 + part * static_cast<uint64_t>(kNormThreads) + threadIdx.x; i < n;
+       i += static_cast<uint64_t>(kNormParts) * kNormThreads) {
+    float mom = m.momentum != nullptr ? m.momentum[i] : 0.0f;
+    take(m.gradient[i], mom);
+    if (m.momentum != nullptr) m.momentum[i] = mom;
   }
   float one[1] = {sum};
   oxh::wave_sums_rows(one);
   if ((threadIdx.x & 63) == 0) wave[threadIdx.x >> 6] = one[0];
   __syncthreads();
   if (threadIdx.x == 0) {
-    float *parts = reinterpret_cast<float *>(m.scratch + layout_of(m.ps, m.pl).parts);
-    parts[part] = (wave[0] + wave[1]) + (wave[2] + wave[3]);
+    float total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kNormThreads / 64; ++w) total += wave[w];
+    reinterpret_cast<float *>(m.scratch + layout_of(m.ps, m.pl).parts)[part] = total;
   }
 }
 
@@ -174,6 +206,7 @@ __global__ __launch_bounds__(256) void muon_start_kernel(Group g) {
   const uint32_t s = tall ? m.columns : m.rows, n = tall ? m.rows : m.columns;
   const uint32_t tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   // read along the rows of V
+#pragma unroll
   for (uint32_t k = ty; k < 32; k += 8) {
     const uint32_t i = tall ? i0 + tx : i0 + k, j = tall ? j0 + k : j0 + tx;
     float v = 0.0f;
@@ -184,22 +217,26 @@ __global__ __launch_bounds__(256) void muon_start_kernel(Group g) {
     else tile[k][tx] = v;
   }
   __syncthreads();
+  // 16 bytes of a row of each form per thread: four values, or eight hi or lo
   float *x = reinterpret_cast<float *>(m.scratch + l.x);
   f16 *xs = reinterpret_cast<f16 *>(m.scratch + l.xs);
   f16 *xt = reinterpret_cast<f16 *>(m.scratch + l.xt0);
-  for (uint32_t k = ty; k < 32; k += 8) {
+  const uint32_t row = threadIdx.x >> 3, piece = threadIdx.x & 7, first = (piece & 3) * 8;
+  f32x4 values;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) values[e] = tile[piece * 4 + e][row];
+  *reinterpret_cast<f32x4 *>(x + static_cast<uint64_t>(j0 + row) * m.ps + i0 + piece * 4) = values;
+  f16x8 straight, turned;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
     f16 hi, lo;
-    const float v = tile[k][tx], t = tile[tx][k];
-    x[static_cast<uint64_t>(j0 + k) * m.ps + i0 + tx] = t;
-    halves_of(v, hi, lo);
-    f16 *p = xs + halves_at(i0 + k, j0 + tx, m.pl);
-    p[0] = hi;
-    p[32] = lo;
-    halves_of(t, hi, lo);
-    f16 *q = xt + halves_at(j0 + k, i0 + tx, m.ps);
-    q[0] = hi;
-    q[32] = lo;
+    halves_of(tile[row][first + e], hi, lo);
+    straight[e] = piece < 4 ? hi : lo;
+    halves_of(tile[first + e][row], hi, lo);
+    turned[e] = piece < 4 ? hi : lo;
   }
+  *reinterpret_cast<f16x8 *>(xs + halves_at(i0 + row, j0, m.pl) + piece * 8) = straight;
+  *reinterpret_cast<f16x8 *>(xt + halves_at(j0 + row, i0, m.ps) + piece * 8) = turned;
 }
 
 enum class Step { Gram, Poly, Apply, Last };
@@ -215,6 +252,7 @@ struct Shape {
 using Wide = Shape<2, 2, 3, 3, 1, 2>;    // 192 x 192
 using Medium = Shape<2, 2, 2, 2, 1, 2>;  // 128 x 128
 using Small = Shape<2, 2, 1, 1, 2, 2>;   // 64 x 64
+using Tiny = Shape<1, 1, 1, 1, 4, 8>;    // 32 x 32
 
 // The tile of index b among rows x columns tiles, or (Symmetric) among those on and below the
 // diagonal of rows x rows: bands of four tile rows, each taken column by column, so that the run
@@ -430,12 +468,23 @@ __global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int 
           v += kA * *reinterpret_cast<const f32x4 *>(x + turned_at);
         if constexpr (S == Step::Last) {
           const bool tall = m.rows > m.columns;
+          const uint32_t wr0 = tall ? column : row, wc0 = tall ? row : column;
+          float *t = m.target + static_cast<uint64_t>(wr0) * m.columns + wc0;
+          const uint64_t next = tall ? 1 : m.columns;
+          // entries past the sides are read from the last ones, and not written
+          const uint32_t left = tall ? (wr0 < m.rows && wc0 < m.columns ? m.columns - wc0 : 0u)
+                                     : (wc0 < m.columns && wr0 < m.rows ? m.rows - wr0 : 0u);
+          if (left != 0) {
+            if (m.momentum != nullptr) {
+              f32x4 w;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const uint32_t wr = tall ? column : row + r, wc = tall ? row + r : column;
-            if (wr >= m.rows || wc >= m.columns) continue;
-            float *t = m.target + static_cast<uint64_t>(wr) * m.columns + wc;
-            *t = m.momentum == nullptr ? v[r] : *t - g.lr * (g.decay * *t + m.scale * v[r]);
+              for (uint32_t r = 0; r < 4; ++r) w[r] = t[min(r, left - 1) * next];
+#pragma unroll
+              for (int r = 0; r < 4; ++r) v[r] = w[r] - g.lr * (g.decay * w[r] + m.scale * v[r]);
+            }
+#pragma unroll
+            for (uint32_t r = 0; r < 4; ++r)
+              if (r < left) t[r * next] = v[r];
           }
         } else {
           if constexpr (S == Step::Apply) *reinterpret_cast<f32x4 *>(x + turned_at) = v;
@@ -781,31 +830,60 @@ bool whole(const Item &it) {
          round_up(n, 32) <= 16ull * kWholeWaves * whole_blocks(ps);
 }
 
-// Tile side for a launch group, by the tiles that A has (the product that fills the chip least):
-// 128 where it has at least one for every other compute unit (12 x 1024 x 1024: 1325 us, 1558 with
-// 64; 2048 x 2048 with 136 tiles: 821 and 1027), else 64 (1536 x 1536 with 78: 541 us, 581 with
-// 128; 1000 x 1280: 280 and 441); 192 where its tiles just fill one round of one block per compute
-// unit (4096 x 4096 with 253: 4.49 ms, 4.97 with 128; 6144 x 6144 with 528: 14.96 and 14.71).
-uint32_t tile_of(const Item *items, size_t count) {
-  auto tiles = [&](uint64_t tile) {
-    uint64_t n = 0;
-    for (size_t i = 0; i < count; ++i) {
-      const uint64_t s = round_up(std::min(items[i].rows, items[i].columns), tile) / tile;
-      n += s * (s + 1) / 2;
-    }
-    return n;
+// Tile sides of a launch group: `square` of A and B, of which the tiles on and below the diagonal
+// are summed, and `apply` of B X.
+struct Tiles {
+  uint32_t square, apply;
+  uint32_t pad() const { return std::max(square, apply); }
+};
+
+// Small tiles spread a product over more compute units, large ones load less per product.  Each
+// product takes
+//   32 where its tiles of 32 are at most one per compute unit (512 x 512: 119 us, 157 with 64;
+//     1024 x 1024: 327 and 245; 512 x 2048, whose B X has 1024 such tiles: 208 with 32 for both
+//     products, 179 with 32 and 64, 240 with 64);
+//   128 where there is one for every other compute unit (B X of 1536 x 1536, 144 tiles: 493 us, 523
+//     with 64; 1000 x 1280, 80 tiles: 311 and 284; all of 2048 x 2048, 136 and 256 tiles: 794 and
+//     958) and padding to 128 adds at most a tenth (32 matrices of 300 x 1200, padded 1.26 times:
+//     992 and 739);
+//   64 otherwise;
+// and both take 192 where the square products just fill one round of a block per compute unit, with
+// the same limit on padding (4096 x 4096, 253 tiles: 4.43 ms, 4.87 with 128; 6144 x 6144, 528
+// tiles: 14.96 and 14.71; 12 x 1024 x 1024, 252 tiles padded 1.27 times: 1645 us and 1300).
+Tiles tiles_of(const Item *items, size_t count) {
+  struct Count {
+    uint64_t square = 0, apply = 0, area = 0;
   };
-  const uint64_t wide = tiles(Wide::tile), units = oxh::kComputeUnits;
-  if (wide <= units && wide * 8 >= units * 7) return Wide::tile;
-  return tiles(Medium::tile) * 2 >= units ? Medium::tile : Small::tile;
+  auto of = [&](uint64_t tile) {
+    Count c;
+    for (size_t i = 0; i < count; ++i) {
+      const uint64_t s = round_up(std::min(items[i].rows, items[i].columns), tile) / tile,
+                     n = round_up(std::max(items[i].rows, items[i].columns), tile) / tile;
+      c.square += s * (s + 1) / 2;
+      c.apply += s * n;
+      c.area += s * n * tile * tile;
+    }
+    return c;
+  };
+  const uint64_t units = oxh::kComputeUnits;
+  const Count tiny = of(Tiny::tile), small = of(Small::tile), medium = of(Medium::tile),
+              wide = of(Wide::tile);
+  auto fits = [&](const Count &c) { return c.area * 10 <= small.area * 11; };
+  if (wide.square <= units && wide.square * 8 >= units * 7 && fits(wide))
+    return {Wide::tile, Wide::tile};
+  auto pick = [&](uint64_t in_tiny, uint64_t in_medium) -> uint32_t {
+    if (in_tiny <= units) return Tiny::tile;
+    return fits(medium) && in_medium * 2 >= units ? Medium::tile : Small::tile;
+  };
+  return {pick(tiny.square, medium.square), pick(tiny.apply, medium.apply)};
 }
 
 uint64_t scratch_of(const Item *items, size_t count) {
-  const uint32_t tile = tile_of(items, count);
+  const uint32_t pad = tiles_of(items, count).pad();
   uint64_t total = 0;
   for (size_t i = 0; i < count; ++i)
-    total += round_up(layout_of(round_up(std::min(items[i].rows, items[i].columns), tile),
-                                round_up(std::max(items[i].rows, items[i].columns), tile))
+    total += round_up(layout_of(round_up(std::min(items[i].rows, items[i].columns), pad),
+                                round_up(std::max(items[i].rows, items[i].columns), pad))
                           .total,
                       256);
   return total;
@@ -843,14 +921,15 @@ oxh_status product(hipStream_t stream, Group &g, uint32_t tile, int odd, const c
   };
   if (tile == Wide::tile) start(Wide());
   else if (tile == Medium::tile) start(Medium());
-  else start(Small());
+  else if (tile == Small::tile) start(Small());
+  else start(Tiny());
   return oxh::launched(what);
 }
 
-oxh_status run_group(hipStream_t stream, Group &g, uint32_t tile, uint32_t rounds) {
+oxh_status run_group(hipStream_t stream, Group &g, const Tiles &tiles, uint32_t rounds) {
   g.blocks = 0;
   for (uint32_t i = 0; i < g.count; ++i) g.m[i].first_block = g.blocks, g.blocks += kNormParts;
-  oxh::launch(muon_norm_kernel, dim3(g.blocks), dim3(256), 0, stream, g);
+  oxh::launch(muon_norm_kernel, dim3(g.blocks), dim3(kNormThreads), 0, stream, g);
   oxh_status st = oxh::launched("muon_norm");
   if (st != OXH_OK) return st;
   g.blocks = 0;
@@ -861,11 +940,11 @@ oxh_status run_group(hipStream_t stream, Group &g, uint32_t tile, uint32_t round
   oxh::launch(muon_start_kernel, dim3(g.blocks), dim3(256), 0, stream, g);
   st = oxh::launched("muon_start");
   for (uint32_t r = 0; r < rounds && st == OXH_OK; ++r) {
-    st = product<Step::Gram>(stream, g, tile, r & 1, "muon_gram");
-    if (st == OXH_OK) st = product<Step::Poly>(stream, g, tile, r & 1, "muon_poly");
+    st = product<Step::Gram>(stream, g, tiles.square, r & 1, "muon_gram");
+    if (st == OXH_OK) st = product<Step::Poly>(stream, g, tiles.square, r & 1, "muon_poly");
     if (st != OXH_OK) return st;
-    st = r + 1 < rounds ? product<Step::Apply>(stream, g, tile, r & 1, "muon_apply")
-                        : product<Step::Last>(stream, g, tile, r & 1, "muon_last");
+    st = r + 1 < rounds ? product<Step::Apply>(stream, g, tiles.apply, r & 1, "muon_apply")
+                        : product<Step::Last>(stream, g, tiles.apply, r & 1, "muon_last");
   }
   return st;
 }
@@ -932,7 +1011,8 @@ oxh_status run_all(hipStream_t stream, const Parted &items, const Hyper &h, uint
   }
   for (size_t at = 0; at < large.size() && st == OXH_OK; at += kGroup) {
     const size_t count = std::min<size_t>(kGroup, large.size() - at);
-    const uint32_t tile = tile_of(&large[at], count);
+    const Tiles tiles = tiles_of(&large[at], count);
+    const uint32_t pad = tiles.pad();
     g.count = static_cast<uint32_t>(count);
     uint64_t offset = 0;
     for (size_t i = 0; i < count; ++i) {
@@ -940,11 +1020,11 @@ oxh_status run_all(hipStream_t stream, const Parted &items, const Hyper &h, uint
       Matrix &m = g.m[i];
       describe(it, m);
       m.scratch = workspace + offset;
-      m.ps = static_cast<uint32_t>(round_up(std::min(it.rows, it.columns), tile));
-      m.pl = static_cast<uint32_t>(round_up(std::max(it.rows, it.columns), tile));
+      m.ps = static_cast<uint32_t>(round_up(std::min(it.rows, it.columns), pad));
+      m.pl = static_cast<uint32_t>(round_up(std::max(it.rows, it.columns), pad));
       offset += round_up(layout_of(m.ps, m.pl).total, 256);
     }
-    st = run_group(stream, g, tile, rounds);
+    st = run_group(stream, g, tiles, rounds);
   }
   return st;
 }
