@@ -45,16 +45,20 @@ __device__ __forceinline__ void load(const T *p, float (&v)[N]) {
   }
 }
 
-template <typename T, int N>
+// Once: past the caches.
+template <typename T, int N, bool Once = false>
 __device__ __forceinline__ void store(T *p, const float (&v)[N]) {
+  typename Pack<T, N>::type x;
   if constexpr (N == 1) {
-    *p = static_cast<T>(v[0]);
+    x = static_cast<T>(v[0]);
   } else {
-    typename Pack<T, N>::type x;
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = static_cast<T>(v[i]);
-    *reinterpret_cast<typename Pack<T, N>::type *>(p) = x;
   }
+  if constexpr (Once)
+    __builtin_nontemporal_store(x, reinterpret_cast<typename Pack<T, N>::type *>(p));
+  else
+    *reinterpret_cast<typename Pack<T, N>::type *>(p) = x;
 }
 
 }  // namespace storage
