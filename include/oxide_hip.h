@@ -890,10 +890,29 @@ oxh_status oxh_net_batch_norm2d(oxh_net *net, uint32_t x, uint32_t weight, uint3
  * holding class indices as f32; a one-element loss (the batch mean). */
 oxh_status oxh_net_cross_entropy(oxh_net *net, uint32_t logits, uint32_t targets,
                                  uint32_t *node);
+/* RMS norm over the last dimension (weight [last dimension]; epsilon non-negative and finite, else
+ * OXH_EXECUTION) and the gated recurrence over [batch, time, channels] from a zero state.  A norm
+ * of an add's value runs in the add's launch, which writes the sum and the norm. */
+oxh_status oxh_net_rms_norm(oxh_net *net, uint32_t x, uint32_t weight, float epsilon,
+                            uint32_t *node);
+oxh_status oxh_net_gated_recurrence(oxh_net *net, uint32_t x, uint32_t gate, uint32_t *node);
 oxh_status oxh_net_forward_program(const oxh_net *net, uint32_t output, oxh_program **program);
 /* adamw NULL: forward + backward only (the gradients stay in the program's buffers). */
 oxh_status oxh_net_training_program(const oxh_net *net, uint32_t root,
                                     const oxh_adamw_config *adamw, oxh_program **program);
+/* A training program that updates the `count` parameters of nodes `matrices` (at least two
+ * dimensions, the first one the rows) by oxh_muon_multi_tensor and the others by AdamW (`adamw`
+ * NULL: they keep their values).  Learning rate positive, weight decay non-negative, momentum in
+ * [0, 1), all finite, else OXH_EXECUTION. */
+typedef struct oxh_muon_config {
+  float learning_rate, weight_decay, momentum, epsilon;
+  int nesterov;
+  uint32_t rounds;
+} oxh_muon_config;
+oxh_status oxh_net_training_program_muon(const oxh_net *net, uint32_t root,
+                                         const oxh_muon_config *muon, const uint32_t *matrices,
+                                         uint32_t count, const oxh_adamw_config *adamw,
+                                         oxh_program **program);
 /* Device buffer of a node's value in the program (inputs: where to write them). */
 oxh_status oxh_program_value(const oxh_program *program, uint32_t node, float **device);
 /* Device buffer of a node's gradient after a training program ran (Tensor::grad,

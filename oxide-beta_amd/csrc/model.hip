@@ -362,7 +362,7 @@ oxh_status build_trainer(oxh_trainer &t, float learning_rate, float weight_decay
   if (st == OXH_OK) st = net::cross_entropy(t.g, t.logits, t.targets, &t.loss_node);
   if (st != OXH_OK) return st;
   const net::AdamConfig adam{learning_rate, weight_decay, 0.9f, 0.999f, 1e-8f};
-  return net::build_training(t.g, t.loss_node, &adam, t.program);
+  return net::build_training(t.g, t.loss_node, &adam, nullptr, t.program);
 }
 
 oxh_status build_evaluator(oxh_evaluator &e) {

@@ -5,7 +5,8 @@
 // order, which is a topological order: leaves (inputs fed per run, trainable parameters,
 // constants; caller-owned device values) and Conv2d / BatchNorm2d / ReLU / Add / Mul /
 // AvgPool2d / Reshape / CrossEntropy nodes with the builders' shape rules
-// (tensor/mod.rs:103-389).  A program is a fixed list of launch groups over buffers carved
+// (tensor/mod.rs:103-389), and the RmsNorm / Recurrence nodes of sequence models, which the
+// reference has not.  A program is a fixed list of launch groups over buffers carved
 // from one device allocation:
 //   * forward program: the eager device evaluation of a node (runtime.rs:125-379), used for
 //     inference and for JIT plans the fused-plan compiler cannot take (jit.rs:205-207,226-243);
@@ -53,7 +54,9 @@ struct Arena {
 
 // ---------------------------------------------------------------- graph
 
-enum class Op { Input, Param, Constant, Conv, Bn, Relu, Add, Mul, Pool, Reshape, CrossEntropy };
+enum class Op {
+  Input, Param, Constant, Conv, Bn, Relu, Add, Mul, Pool, Reshape, CrossEntropy, RmsNorm, Recurrence
+};
 
 struct Node {
   Node(Op o, std::vector<int> i) : op(o), in(std::move(i)) {}
@@ -100,10 +103,21 @@ oxh_status batch_norm2d(Graph &g, int x, int weight, int bias, float *running_me
                         float *running_variance, bool training, float momentum, float epsilon,
                         int *node);
 oxh_status cross_entropy(Graph &g, int logits, int targets, int *node);
+// Root-mean-square norm over the last dimension; the gated recurrence over [batch, time, channels].
+oxh_status rms_norm(Graph &g, int x, int weight, float epsilon, int *node);
+oxh_status gated_recurrence(Graph &g, int x, int gate, int *node);
 
 struct AdamConfig {
   float learning_rate = 1e-3f, weight_decay = 0.01f, beta1 = 0.9f, beta2 = 0.999f,
         epsilon = 1e-8f;
+};
+
+// The optimizer of the parameters `matrices` names (nodes); the others take AdamW.
+struct MuonConfig {
+  float learning_rate = 0.02f, weight_decay = 0.0f, momentum = 0.95f, epsilon = 1e-7f;
+  int nesterov = 1;
+  uint32_t rounds = 5;
+  std::vector<int> matrices;
 };
 
 // ---------------------------------------------------------------- launch records
@@ -157,6 +171,9 @@ struct oxh_program {
   uint64_t adam_chunks = 0;
   int32_t *step = nullptr;
   uint32_t *error_flag = nullptr;  // raised by a cross entropy with an invalid target
+  // matrices that take the orthogonalised update
+  oxh::net::MuonConfig muon_config;
+  std::vector<oxh_muon_tensor> muon;
   // chunk sums the program's convolutions leave to the optimizer group, recorded by each run
   std::vector<oxh::ChunkSum> deferred_sums;
 
@@ -172,7 +189,8 @@ namespace net {
 // Programs over `g` (which must outlive nothing: the program copies what it needs).  The
 // program's stream must be set before building.
 oxh_status build_forward(const Graph &g, int output, oxh_program &p);
-oxh_status build_training(const Graph &g, int root, const AdamConfig *adam, oxh_program &p);
+oxh_status build_training(const Graph &g, int root, const AdamConfig *adam,
+                          const MuonConfig *muon, oxh_program &p);
 
 }  // namespace net
 }  // namespace oxh

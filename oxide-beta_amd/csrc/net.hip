@@ -246,6 +246,37 @@ oxh_status cross_entropy(Graph &g, int logits, int targets, int *node) {
   return oxh::ok();
 }
 
+oxh_status rms_norm(Graph &g, int x, int weight, float epsilon, int *node) {
+  oxh_status st = node_index(g, x, "rms_norm");
+  if (st == OXH_OK) st = node_index(g, weight, "rms_norm");
+  if (st != OXH_OK) return st;
+  const Node &in = g.nodes[x], &w = g.nodes[weight];
+  OXH_REQUIRE(w.rank == 1 && w.shape[0] == in.shape[in.rank - 1] && w.shape[0] != 0,
+              OXH_INVALID_SHAPE, "rms_norm weight must match the last dimension");
+  OXH_REQUIRE(std::isfinite(epsilon) && epsilon >= 0.0f, OXH_EXECUTION,
+              "rms_norm epsilon must be non-negative and finite");
+  Node n{Op::RmsNorm, {x, weight}};
+  n.rank = in.rank;
+  n.shape = in.shape;
+  n.epsilon = epsilon;
+  *node = g.add(n);
+  return oxh::ok();
+}
+
+oxh_status gated_recurrence(Graph &g, int x, int gate, int *node) {
+  oxh_status st = node_index(g, x, "gated_recurrence");
+  if (st == OXH_OK) st = node_index(g, gate, "gated_recurrence");
+  if (st != OXH_OK) return st;
+  const Node &in = g.nodes[x];
+  OXH_REQUIRE(in.rank == 3 && same_shape(in, g.nodes[gate]), OXH_INVALID_SHAPE,
+              "gated_recurrence expects [batch, time, channels] and a gate of that shape");
+  Node n{Op::Recurrence, {x, gate}};
+  n.rank = in.rank;
+  n.shape = in.shape;
+  *node = g.add(n);
+  return oxh::ok();
+}
+
 // ---------------------------------------------------------------- program helpers
 
 namespace {
@@ -272,6 +303,9 @@ TensorRef ref_flat(const char *role, void *data, uint64_t count, int access, int
 }
 
 uint64_t node_bytes(const Node &n) { return n.numel() * 4; }
+
+// Rows that an RMS norm of this shape takes.
+uint64_t norm_rows(const Node &n) { return n.numel() / n.shape[n.rank - 1]; }
 
 oxh_conv2d_shape conv_shape(const Graph &g, const Node &n) {
   const Node &x = g.nodes[n.in[0]], &w = g.nodes[n.in[1]];
@@ -333,6 +367,10 @@ oxh_status plan_workspace(const Graph &g, const std::vector<char> &active, uint6
     } else if (n.op == Op::CrossEntropy) {
       const Node &l = g.nodes[n.in[0]];
       st = oxh_cross_entropy_workspace_size(l.shape[0], l.shape[1], &b);
+    } else if (n.op == Op::RmsNorm) {
+      st = oxh_rms_norm_backward_workspace_size(norm_rows(n), n.shape[n.rank - 1], &b);
+    } else if (n.op == Op::Recurrence) {
+      st = oxh_gated_recurrence_workspace_size(n.shape[0], n.shape[1], n.shape[2], &b);
     }
     if (st != OXH_OK) return st;
     if (b > bytes) bytes = b;
@@ -395,6 +433,69 @@ OpRec pool_forward_op(const Graph &g, const std::vector<float *> &value, size_t 
   op.tensors = {ref("x", const_cast<float *>(xi), g.nodes[x.in[0]], 0), ref("y", out, x, 1)};
   op.attrs = pool_attrs(x);
   op.launch = [ps, xi, out](hipStream_t st) { return oxh_avg_pool2d_forward(st, &ps, xi, out); };
+  return op;
+}
+
+// For each residual add the RMS norm that its launch forms with its sum (-1: none): the first norm
+// of the add's value, whose weight must exist by then (a leaf).
+std::vector<int64_t> norms_of_adds(const Graph &g, const std::vector<char> &active) {
+  std::vector<int64_t> norm(g.nodes.size(), -1);
+  for (size_t i = 0; i < g.nodes.size(); ++i) {
+    const Node &x = g.nodes[i];
+    if (!active[i] || x.op != Op::RmsNorm || !g.nodes[x.in[1]].leaf()) continue;
+    if (g.nodes[x.in[0]].op == Op::Add && norm[x.in[0]] < 0)
+      norm[x.in[0]] = static_cast<int64_t>(i);
+  }
+  return norm;
+}
+
+// The norm of node i; `add` >= 0: with the residual add in front, whose sum the launch writes too.
+OpRec norm_forward_op(const Graph &g, const std::vector<float *> &value, float *inverse_rms,
+                      size_t i, int add) {
+  const Node &x = g.nodes[i];
+  const Node &in = g.nodes[x.in[0]];
+  const float *a = add >= 0 ? value[g.nodes[add].in[0]] : value[x.in[0]];
+  const float *b = add >= 0 ? value[g.nodes[add].in[1]] : nullptr;
+  float *sum = add >= 0 ? value[add] : nullptr, *out = value[i];
+  const float *w = value[x.in[1]];
+  const uint64_t rows = norm_rows(x), columns = x.shape[x.rank - 1];
+  const float eps = x.epsilon;
+  OpRec op;
+  op.kind = add >= 0 ? "add_rms_norm_forward" : "rms_norm_forward";
+  op.name = (add >= 0 ? "add" + std::to_string(add) + "+" : std::string()) + "norm" +
+            std::to_string(i);
+  if (add >= 0) {
+    op.tensors = {ref("a", const_cast<float *>(a), g.nodes[g.nodes[add].in[0]], 0),
+                  ref("b", const_cast<float *>(b), g.nodes[g.nodes[add].in[1]], 0),
+                  ref("sum", sum, g.nodes[add], 1)};
+  } else {
+    op.tensors = {ref("x", const_cast<float *>(a), in, 0)};
+  }
+  op.tensors.push_back(ref("weight", const_cast<float *>(w), g.nodes[x.in[1]], 0));
+  op.tensors.push_back(ref("y", out, x, 1));
+  op.tensors.push_back(ref_flat("inverse_rms", inverse_rms, rows, 1));
+  op.attrs = {{"epsilon", eps}};
+  op.launch = [=](hipStream_t st) {
+    return oxh_rms_norm_forward(st, OXH_F32, rows, columns, eps, a, b, w, sum, out, inverse_rms);
+  };
+  return op;
+}
+
+OpRec recurrence_forward_op(const Graph &g, const std::vector<float *> &value, void *ws,
+                            uint64_t wsb, size_t i) {
+  const Node &x = g.nodes[i];
+  const float *xi = value[x.in[0]], *gate = value[x.in[1]];
+  float *out = value[i];
+  const uint64_t batch = x.shape[0], time = x.shape[1], channels = x.shape[2];
+  OpRec op;
+  op.kind = "gated_recurrence_forward";
+  op.name = "recurrence" + std::to_string(i);
+  op.tensors = {ref("x", const_cast<float *>(xi), g.nodes[x.in[0]], 0),
+                ref("gate", const_cast<float *>(gate), g.nodes[x.in[1]], 0), ref("y", out, x, 1)};
+  op.launch = [=](hipStream_t st) {
+    return oxh_gated_recurrence_forward(st, OXH_F32, batch, time, channels, xi, gate, nullptr,
+                                        nullptr, out, nullptr, ws, wsb);
+  };
   return op;
 }
 
@@ -484,6 +585,7 @@ oxh_status build_forward(const Graph &g, int output, oxh_program &p) {
       soff[i] = a.reserve(x.shape[1] * 4);
       ioff[i] = a.reserve(x.shape[1] * 4);
     }
+    if (x.op == Op::RmsNorm) ioff[i] = a.reserve(norm_rows(x) * 4);
   }
   const uint64_t flag_off = a.reserve(4);
   uint64_t ws_bytes = 0;
@@ -509,6 +611,8 @@ oxh_status build_forward(const Graph &g, int output, oxh_program &p) {
   void *ws = a.at<void>(ws_off);
   const uint64_t wsb = ws_bytes;
   std::vector<char> formed(n, 0);  // values an inference BatchNorm's launch forms with its own
+  const std::vector<int64_t> norm_of = norms_of_adds(g, active);
+  std::vector<char> normed(n, 0);  // norms formed with their residual adds
   for (size_t i = 0; i < n; ++i) {
     const Node &x = g.nodes[i];
     if (!active[i] || x.leaf() || is_view(g, x)) continue;
@@ -516,8 +620,21 @@ oxh_status build_forward(const Graph &g, int output, oxh_program &p) {
       case Op::Conv:
         p.ops.push_back(conv_forward_op(g, p.value, i));
         break;
-      case Op::Relu:
+      case Op::RmsNorm:
+        if (!normed[i]) p.ops.push_back(norm_forward_op(g, p.value, p.saved_inv[i], i, -1));
+        break;
+      case Op::Recurrence:
+        p.ops.push_back(recurrence_forward_op(g, p.value, ws, wsb, i));
+        break;
       case Op::Add:
+        if (norm_of[i] >= 0 && !formed[i]) {
+          const size_t j = static_cast<size_t>(norm_of[i]);
+          normed[j] = 1;
+          p.ops.push_back(norm_forward_op(g, p.value, p.saved_inv[j], j, static_cast<int>(i)));
+          break;
+        }
+        [[fallthrough]];
+      case Op::Relu:
       case Op::Mul:
         p.ops.push_back(elementwise_forward_op(g, p.value, i));
         if (formed[i]) p.ops.back().program_launch = [](hipStream_t) { return oxh::ok(); };
@@ -584,7 +701,8 @@ oxh_status build_forward(const Graph &g, int output, oxh_program &p) {
 
 // ---------------------------------------------------------------- training program
 
-oxh_status build_training(const Graph &g, int root, const AdamConfig *adam, oxh_program &p) {
+oxh_status build_training(const Graph &g, int root, const AdamConfig *adam,
+                          const MuonConfig *muon, oxh_program &p) {
   const size_t n = g.nodes.size();
   OXH_REQUIRE(root >= 0 && static_cast<size_t>(root) < n, OXH_INVALID_SHAPE,
               "root node out of range");
@@ -599,6 +717,27 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam, oxh_
     OXH_REQUIRE(std::isfinite(adam->beta1) && std::isfinite(adam->beta2) &&
                     std::isfinite(adam->epsilon),
                 OXH_INVALID_SHAPE, "AdamW betas and epsilon must be finite");
+  }
+  // parameters that take the orthogonalised update in place of AdamW's
+  std::vector<char> matrix(n, 0);
+  if (muon != nullptr) {
+    OXH_REQUIRE(std::isfinite(muon->learning_rate) && muon->learning_rate > 0.0f, OXH_EXECUTION,
+                "Muon learning rate must be positive and finite");
+    OXH_REQUIRE(std::isfinite(muon->weight_decay) && muon->weight_decay >= 0.0f, OXH_EXECUTION,
+                "Muon weight decay must be non-negative and finite");
+    OXH_REQUIRE(std::isfinite(muon->momentum) && muon->momentum >= 0.0f && muon->momentum < 1.0f,
+                OXH_EXECUTION, "Muon momentum must be in 0..1");
+    OXH_REQUIRE(std::isfinite(muon->epsilon) && muon->epsilon > 0.0f, OXH_EXECUTION,
+                "Muon epsilon must be positive and finite");
+    OXH_REQUIRE(muon->rounds >= 1 && muon->rounds <= 64, OXH_INVALID_SHAPE,
+                "Muon rounds outside 1..64");
+    for (int i : muon->matrices) {
+      oxh_status st = node_index(g, i, "Muon");
+      if (st != OXH_OK) return st;
+      OXH_REQUIRE(g.nodes[i].op == Op::Param && g.nodes[i].rank >= 2 && g.nodes[i].numel() != 0,
+                  OXH_INVALID_SHAPE, "Muon takes parameters of at least two dimensions");
+      matrix[i] = 1;
+    }
   }
   const std::vector<char> active = ancestors(g, root);
 
@@ -737,6 +876,7 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam, oxh_
       continue;
     }
     if (!active[i]) continue;
+    if (x.op == Op::RmsNorm) sioff[i] = a.reserve(norm_rows(x) * 4);
     if (x.op == Op::Bn) {  // saved statistics, also for a BN fused with its ReLU
       smoff[i] = a.reserve(x.shape[1] * 4);
       sioff[i] = a.reserve(x.shape[1] * 4);
@@ -755,10 +895,14 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam, oxh_
   std::vector<std::array<int64_t, 3>> poff(trained.size());
   for (size_t k = 0; k < trained.size(); ++k) {
     const uint64_t bytes = node_bytes(g.nodes[trained[k]]);
+    // a matrix has one moment, its momentum
+    const bool first = matrix[trained[k]] || adam, second = !matrix[trained[k]] && adam;
     poff[k] = {static_cast<int64_t>(a.reserve(bytes)),
-               adam ? static_cast<int64_t>(a.reserve(bytes)) : -1,
-               adam ? static_cast<int64_t>(a.reserve(bytes)) : -1};
+               first ? static_cast<int64_t>(a.reserve(bytes)) : -1,
+               second ? static_cast<int64_t>(a.reserve(bytes)) : -1};
   }
+  bool adam_any = false;  // whether AdamW has a parameter to update
+  for (int pn : trained) adam_any = adam_any || (adam != nullptr && !matrix[pn]);
   const uint64_t scratch_off = a.reserve(largest * 4), one_off = a.reserve(4),
                  step_off = a.reserve(4), flag_off = a.reserve(4);
   const uint64_t table_off = a.reserve(std::max<size_t>(trained.size(), 1) *
@@ -770,7 +914,9 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam, oxh_
   constexpr int kDiscardSlots = 6;
   bool discards = false;
   for (size_t i = 0; i < n; ++i)
-    if (want(static_cast<int>(i)) && (g.nodes[i].op == Op::Bn || dw_conv[i]))
+    if (want(static_cast<int>(i)) &&
+        (g.nodes[i].op == Op::Bn || g.nodes[i].op == Op::RmsNorm ||
+         g.nodes[i].op == Op::Recurrence || dw_conv[i]))
       for (int k : g.nodes[i].in) discards = discards || !want(k);
   const uint64_t discard_off = a.reserve(discards ? kDiscardSlots * largest * 4 : 4);
   // A gradient a launch forms beside its main contribution (a convolution's or BatchNorm's
@@ -780,7 +926,9 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam, oxh_
   bool sides = false;
   for (size_t i = 0; i < n; ++i) {
     const Node &x = g.nodes[i];
-    if (!active[i] || (x.op != Op::Conv && x.op != Op::Bn)) continue;
+    if (!active[i] || (x.op != Op::Conv && x.op != Op::Bn && x.op != Op::RmsNorm &&
+                       x.op != Op::Recurrence))
+      continue;
     for (size_t k = 1; k < x.in.size(); ++k)
       sides = sides || (want(x.in[k]) && consumers[x.in[k]] > 1);
   }
@@ -788,13 +936,22 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam, oxh_
   uint64_t ws_bytes = 0;
   oxh_status st = plan_workspace(g, active, ws_bytes);
   if (st != OXH_OK) return st;
+  std::vector<oxh_muon_tensor> shapes;  // the buffers follow once they are allocated
+  for (int pn : trained)
+    if (matrix[pn])
+      shapes.push_back({nullptr, nullptr, nullptr, g.nodes[pn].shape[0],
+                        g.nodes[pn].numel() / g.nodes[pn].shape[0]});
+  uint64_t muon_bytes = 0;
+  st = oxh_muon_workspace_size(shapes.data(), static_cast<uint32_t>(shapes.size()), &muon_bytes);
+  if (st != OXH_OK) return st;
+  ws_bytes = std::max(ws_bytes, muon_bytes);
   const uint64_t ws_off = a.reserve(ws_bytes);
   // A convolution whose parameters feed it alone takes a workspace of its own when the program
   // ends with AdamW: its weight-gradient chunk partials then stay put until the optimizer
   // group, which sums every such convolution's in one launch (with the step counter advance).
   std::vector<int64_t> defer_off(n, -1);
   std::vector<uint64_t> defer_bytes(n, 0);
-  if (adam != nullptr) {
+  if (adam_any) {
     for (size_t i = 0; i < n; ++i) {
       const Node &x = g.nodes[i];
       if (!active[i] || x.op != Op::Conv || !want(x.in[1])) continue;
@@ -832,10 +989,8 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam, oxh_
   std::vector<float *> pm(n, nullptr), pv(n, nullptr);
   for (size_t k = 0; k < trained.size(); ++k) {
     p.grad[trained[k]] = a.at<float>(poff[k][0]);
-    if (adam) {
-      pm[trained[k]] = a.at<float>(poff[k][1]);
-      pv[trained[k]] = a.at<float>(poff[k][2]);
-    }
+    if (poff[k][1] >= 0) pm[trained[k]] = a.at<float>(poff[k][1]);
+    if (poff[k][2] >= 0) pv[trained[k]] = a.at<float>(poff[k][2]);
   }
   float *scratch = a.at<float>(scratch_off), *discard = a.at<float>(discard_off);
   float *side_base = a.at<float>(side_off);
@@ -982,6 +1137,8 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam, oxh_
   };
 
   // forward
+  const std::vector<int64_t> norm_of = norms_of_adds(g, active);
+  std::vector<char> normed(n, 0);  // norms formed with their residual adds
   for (size_t i = 0; i < n; ++i) {
     const Node &x = g.nodes[i];
     if (!active[i] || x.leaf() || is_view(g, x) || fused_bn[i] || dw_conv[i] || pre_fused[i])
@@ -1024,9 +1181,21 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam, oxh_
           ops.push_back(std::move(op));
           break;
         }
+        if (norm_of[i] >= 0) {
+          const size_t j = static_cast<size_t>(norm_of[i]);
+          normed[j] = 1;
+          ops.push_back(norm_forward_op(g, p.value, p.saved_inv[j], j, static_cast<int>(i)));
+          break;
+        }
         [[fallthrough]];
       case Op::Mul:
         ops.push_back(elementwise_forward_op(g, p.value, i));
+        break;
+      case Op::RmsNorm:
+        if (!normed[i]) ops.push_back(norm_forward_op(g, p.value, p.saved_inv[i], i, -1));
+        break;
+      case Op::Recurrence:
+        ops.push_back(recurrence_forward_op(g, p.value, ws, wsb, i));
         break;
       case Op::Relu:
         if (!fused_relu[i]) {
@@ -1609,6 +1778,64 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam, oxh_
         });
         break;
       }
+      case Op::RmsNorm: {
+        // the input's other contributions, made by now or waiting as an add's, are added in the
+        // same pass
+        const int xin = x.in[0];
+        const float *xi = p.value[xin], *w = p.value[x.in[1]], *si = p.saved_inv[r];
+        const uint64_t rows = norm_rows(x), columns = x.shape[x.rank - 1];
+        float *dw = nullptr, *dst = nullptr, *acc = nullptr;
+        const float *addend = nullptr;
+        if (want(x.in[1])) side(x.in[1], dw, "weight_gradient");
+        if (want(xin) && !written[xin] && pending[xin].gradient != nullptr) {
+          addend = pending[xin].gradient;
+          op.tensors.push_back(ref("addend", const_cast<float *>(addend),
+                                   g.nodes[pending[xin].add], 0));
+          pending[xin] = Pending{};
+          written[xin] = 1;
+          dst = p.grad[xin];
+        } else if (want(xin) && written[xin]) {
+          addend = dst = p.grad[xin];
+        } else {
+          contribution(xin, dst, acc);
+        }
+        op.kind = "rms_norm_backward";
+        op.name = name("norm", r) + ".backward";
+        op.tensors.push_back(ref("gradient", const_cast<float *>(gr), x, 0));
+        op.tensors.push_back(ref("x", const_cast<float *>(xi), g.nodes[xin], 0));
+        op.tensors.push_back(ref("weight", const_cast<float *>(w), g.nodes[x.in[1]], 0));
+        op.tensors.push_back(ref_flat("inverse_rms", const_cast<float *>(si), rows, 0));
+        op.tensors.push_back(addend == dst ? ref("input_gradient", dst, g.nodes[xin], 2)
+                                           : ref("contribution", dst, g.nodes[xin], 1));
+        if (dw != nullptr) op.tensors.push_back(ref_flat("weight_gradient", dw, columns, 1));
+        emit(std::move(op), acc, g.nodes[xin], [=](hipStream_t st) {
+          return oxh_rms_norm_backward(st, OXH_F32, rows, columns, gr, addend, xi, w, si, dst, dw,
+                                       ws, wsb);
+        });
+        break;
+      }
+      case Op::Recurrence: {
+        const int xin = x.in[0];
+        const float *xi = p.value[xin], *gate = p.value[x.in[1]], *y = p.value[r];
+        const uint64_t batch = x.shape[0], time = x.shape[1], channels = x.shape[2];
+        float *dst, *acc, *dgate;
+        contribution(xin, dst, acc);
+        side(x.in[1], dgate, "gate_gradient");
+        op.kind = "gated_recurrence_backward";
+        op.name = name("recurrence", r) + ".backward";
+        op.tensors = {ref("gradient", const_cast<float *>(gr), x, 0),
+                      ref("x", const_cast<float *>(xi), g.nodes[xin], 0),
+                      ref("gate", const_cast<float *>(gate), g.nodes[x.in[1]], 0),
+                      ref("y", const_cast<float *>(y), x, 0),
+                      ref("contribution", dst, g.nodes[xin], 1),
+                      ref("gate_gradient", dgate, g.nodes[x.in[1]], 1)};
+        emit(std::move(op), acc, g.nodes[xin], [=](hipStream_t st) {
+          return oxh_gated_recurrence_backward(st, OXH_F32, batch, time, channels, gr, xi, gate, y,
+                                               nullptr, nullptr, nullptr, dst, dgate, nullptr, ws,
+                                               wsb);
+        });
+        break;
+      }
       default:
         return oxh::fail(OXH_TRACE, "no backward for a traced node");
     }
@@ -1618,8 +1845,8 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam, oxh_
   OXH_REQUIRE(!side_unplanned && side_adds.empty(), OXH_EXECUTION,
               "internal: unplanned side contribution");
 
-  // AdamW over every parameter that received a gradient (creation order)
-  if (adam != nullptr && !trained.empty()) {
+  // AdamW over every parameter that received a gradient (creation order), matrices aside
+  if (adam_any) {
     p.has_adam = true;
     p.adam_config = *adam;
     p.adam.clear();
@@ -1627,6 +1854,7 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam, oxh_
     op.kind = "adamw";
     op.name = "adamw";
     for (int pn : trained) {
+      if (matrix[pn]) continue;
       const Node &pr = g.nodes[pn];
       p.adam.push_back(oxh_adamw_tensor{pr.data, p.grad[pn], pm[pn], pv[pn], pr.numel()});
       op.tensors.push_back(ref_flat("parameter", pr.data, pr.numel(), 2));
@@ -1664,6 +1892,32 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam, oxh_
             self->adam_table, self->adam_starts, static_cast<uint32_t>(self->adam.size()),
             self->adam_chunks);
       };
+    ops.push_back(std::move(op));
+  }
+  // the orthogonalised update of the matrices (behind the convolutions' chunk sums)
+  if (!shapes.empty()) {
+    p.muon_config = *muon;
+    p.muon.clear();
+    OpRec op;
+    op.kind = op.name = "muon";
+    for (int pn : trained) {
+      if (!matrix[pn]) continue;
+      const Node &pr = g.nodes[pn];
+      p.muon.push_back(oxh_muon_tensor{pr.data, p.grad[pn], pm[pn], pr.shape[0],
+                                       pr.numel() / pr.shape[0]});
+      op.tensors.push_back(ref("parameter", pr.data, pr, 2));
+      op.tensors.push_back(ref("gradient", p.grad[pn], pr, 0));
+      op.tensors.push_back(ref("momentum", pm[pn], pr, 2));
+    }
+    op.attrs = {{"learning_rate", muon->learning_rate}, {"weight_decay", muon->weight_decay},
+                {"momentum", muon->momentum}, {"nesterov", muon->nesterov},
+                {"epsilon", muon->epsilon}, {"rounds", muon->rounds}};
+    op.launch = [self, ws, wsb](hipStream_t s) {
+      const MuonConfig &c = self->muon_config;
+      return oxh_muon_multi_tensor(s, c.learning_rate, c.weight_decay, c.momentum, c.nesterov,
+                                   c.epsilon, c.rounds, self->muon.data(),
+                                   static_cast<uint32_t>(self->muon.size()), ws, wsb);
+    };
     ops.push_back(std::move(op));
   }
   return p.finalize();
@@ -1746,7 +2000,8 @@ int as_index(uint32_t node) {
 }
 
 oxh_status make_program(const oxh_net *net, uint32_t node, bool training,
-                        const oxh_adamw_config *adamw, oxh_program **program) {
+                        const oxh_adamw_config *adamw, const oxh::net::MuonConfig *muon,
+                        oxh_program **program) {
   OXH_REQUIRE(net != nullptr && program != nullptr, OXH_INVALID_SHAPE, "null argument");
   *program = nullptr;
   std::unique_ptr<oxh_program> p(new oxh_program());
@@ -1756,7 +2011,7 @@ oxh_status make_program(const oxh_net *net, uint32_t node, bool training,
     cfg = oxh::net::AdamConfig{adamw->learning_rate, adamw->weight_decay, adamw->beta1,
                                adamw->beta2, adamw->epsilon};
   oxh_status st = training ? oxh::net::build_training(net->graph, as_index(node),
-                                                      adamw != nullptr ? &cfg : nullptr, *p)
+                                                      adamw != nullptr ? &cfg : nullptr, muon, *p)
                            : oxh::net::build_forward(net->graph, as_index(node), *p);
   if (st == OXH_OK) st = oxh::net::make_stream(p->stream);
   if (st != OXH_OK) return st;
@@ -1858,6 +2113,15 @@ oxh_status oxh_net_batch_norm2d(oxh_net *net, uint32_t x, uint32_t weight, uint3
                                        training != 0, momentum, epsilon, &index));
 }
 
+oxh_status oxh_net_rms_norm(oxh_net *net, uint32_t x, uint32_t weight, float epsilon,
+                            uint32_t *node) {
+  OXH_NET_BUILD(oxh::net::rms_norm(net->graph, as_index(x), as_index(weight), epsilon, &index));
+}
+
+oxh_status oxh_net_gated_recurrence(oxh_net *net, uint32_t x, uint32_t gate, uint32_t *node) {
+  OXH_NET_BUILD(oxh::net::gated_recurrence(net->graph, as_index(x), as_index(gate), &index));
+}
+
 oxh_status oxh_net_cross_entropy(oxh_net *net, uint32_t logits, uint32_t targets,
                                  uint32_t *node) {
   OXH_NET_BUILD(oxh::net::cross_entropy(net->graph, as_index(logits), as_index(targets), &index));
@@ -1866,12 +2130,33 @@ oxh_status oxh_net_cross_entropy(oxh_net *net, uint32_t logits, uint32_t targets
 #undef OXH_NET_BUILD
 
 oxh_status oxh_net_forward_program(const oxh_net *net, uint32_t output, oxh_program **program) {
-  return make_program(net, output, false, nullptr, program);
+  return make_program(net, output, false, nullptr, nullptr, program);
 }
 
 oxh_status oxh_net_training_program(const oxh_net *net, uint32_t root,
                                     const oxh_adamw_config *adamw, oxh_program **program) {
-  return make_program(net, root, true, adamw, program);
+  return make_program(net, root, true, adamw, nullptr, program);
+}
+
+oxh_status oxh_net_training_program_muon(const oxh_net *net, uint32_t root,
+                                         const oxh_muon_config *muon, const uint32_t *matrices,
+                                         uint32_t count, const oxh_adamw_config *adamw,
+                                         oxh_program **program) {
+  OXH_REQUIRE(muon != nullptr && (matrices != nullptr || count == 0), OXH_INVALID_SHAPE,
+              "null argument");
+  try {
+    oxh::net::MuonConfig cfg;
+    cfg.learning_rate = muon->learning_rate;
+    cfg.weight_decay = muon->weight_decay;
+    cfg.momentum = muon->momentum;
+    cfg.epsilon = muon->epsilon;
+    cfg.nesterov = muon->nesterov;
+    cfg.rounds = muon->rounds;
+    for (uint32_t i = 0; i < count; ++i) cfg.matrices.push_back(as_index(matrices[i]));
+    return make_program(net, root, true, adamw, &cfg, program);
+  } catch (const std::exception &e) {
+    return oxh::fail(OXH_EXECUTION, e.what());
+  }
 }
 
 oxh_status oxh_program_destroy(oxh_program *program) {

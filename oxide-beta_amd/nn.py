@@ -177,6 +177,56 @@ class FusedInvertedBottleneck(Module):
         return y.add(x) if self.residual else y
 
 
+class RMSNorm(Module):
+    """Root-mean-square norm over the last dimension, weight 1 (no counterpart in the reference)."""
+
+    def __init__(self, features, epsilon=1e-6):
+        if features == 0:
+            raise ox.OxideError(ox.INVALID_SHAPE, "RMSNorm features must be non-zero")
+        self.weight = Parameter(np.ones(features, np.float32))
+        self.epsilon = epsilon
+
+    def own_parameters(self):
+        return [self.weight]
+
+    def forward(self, x):
+        return x.rms_norm(self.weight.tensor(), self.epsilon)
+
+
+class Linear(Module):
+    """A 1 x 1 convolution over the last dimension of [batch, time, features]."""
+
+    def __init__(self, in_features, out_features):
+        self.conv = Conv2d(in_features, out_features, 1)
+
+    def children(self):
+        return [self.conv]
+
+    def forward(self, x):
+        batch, time, features = x.shape
+        y = self.conv(x.reshape((batch * time, features, 1, 1)))
+        return y.reshape((batch, time, y.shape[1]))
+
+
+class GatedRecurrentBlock(Module):
+    """x + project(gated recurrence of two projections of rms_norm(x)) over [batch, time,
+    features]; the gates start at ``gate_bias``, which keeps sigmoid(gate_bias) of the state per
+    step (no counterpart in the reference)."""
+
+    def __init__(self, features, gate_bias=2.0):
+        self.norm = RMSNorm(features)
+        self.value, self.gate = Linear(features, features), Linear(features, features)
+        self.project = Linear(features, features)
+        self.gate.conv.bias = Parameter(np.full(features, gate_bias, np.float32))
+
+    def children(self):
+        return [self.norm, self.value, self.gate, self.project]
+
+    def forward(self, x):
+        y = self.norm(x)
+        return x.add(self.project(self.value(y).gated_recurrence(self.gate(y))))
+
+
 class GlobalAveragePool(Module):
     def forward(self, x):
         return x.global_avg_pool2d()
@@ -231,3 +281,28 @@ class AdamW:
                                 "AdamW weight decay must be non-negative and finite")
         self.learning_rate, self.weight_decay = float(lr), float(wd)
         self.betas, self.epsilon = (0.9, 0.999), 1e-8
+
+
+class Muon:
+    """The update by an orthogonalised momentum (``oxh_muon_multi_tensor``) for the matrices among
+    ``parameters`` -- those of at least two dimensions whose rows and columns both exceed 1, less
+    ``others`` (an output layer, say) -- and ``adamw`` for every other parameter."""
+
+    def __init__(self, parameters, adamw: AdamW, learning_rate: float = 0.02,
+                 weight_decay: float = 0.0, momentum: float = 0.95, nesterov: bool = True,
+                 others=(), rounds: int = 5, epsilon: float = 1e-7):
+        lr, wd, mu = np.float32(learning_rate), np.float32(weight_decay), np.float32(momentum)
+        if not np.isfinite(lr) or lr <= 0:
+            raise ox.OxideError(ox.EXECUTION, "Muon learning rate must be positive and finite")
+        if not np.isfinite(wd) or wd < 0:
+            raise ox.OxideError(ox.EXECUTION,
+                                "Muon weight decay must be non-negative and finite")
+        if not np.isfinite(mu) or not 0 <= mu < 1:
+            raise ox.OxideError(ox.EXECUTION, "Muon momentum must be in 0..1")
+        skipped = {id(p) for p in others}
+        self.matrices = [p for p in parameters
+                         if id(p) not in skipped and len(p.shape) >= 2 and p.shape[0] > 1
+                         and int(np.prod(p.shape[1:])) > 1]
+        self.learning_rate, self.weight_decay, self.momentum = float(lr), float(wd), float(mu)
+        self.nesterov, self.rounds, self.epsilon = bool(nesterov), int(rounds), float(epsilon)
+        self.adamw = adamw

@@ -6,7 +6,8 @@ liboxide_hip net (``oxh_net_*``) and run as device programs (``oxh_program_*``):
   which is also what a JIT plan the fused-plan compiler cannot take runs (jit.rs:205-243);
 * ``training_program(loss, adamw)`` -- forward, reverse mode from a one-element root
   (``Tensor::backward``, tensor/mod.rs:399-422 -> runtime.rs:1198-1217) and optionally one
-  AdamW step over every parameter the loss reaches (optim.rs:78-152).
+  AdamW step over every parameter the loss reaches (optim.rs:78-152), or an ``nn.Muon`` step over
+  its matrices with AdamW over the others.
 
 A ``Program`` exposes each node's value and gradient buffer (``Tensor::grad``,
 tensor/mod.rs:429-444), runs eagerly or from one captured hipGraph, and lists its launch groups
@@ -32,6 +33,11 @@ class AdamWConfig(ctypes.Structure):
                 ("beta2", _f32), ("epsilon", _f32)]
 
 
+class MuonConfig(ctypes.Structure):
+    _fields_ = [("learning_rate", _f32), ("weight_decay", _f32), ("momentum", _f32),
+                ("epsilon", _f32), ("nesterov", _int), ("rounds", _u32)]
+
+
 _P = ctypes.POINTER
 _SIGNATURES = {
     "oxh_net_create": [_P(_vp)],
@@ -49,8 +55,12 @@ _SIGNATURES = {
     "oxh_net_avg_pool2d": [_vp, _u32, _u64, _u64, _u64, _u64, _P(_u32)],
     "oxh_net_batch_norm2d": [_vp, _u32, _u32, _u32, _vp, _vp, _int, _f32, _f32, _P(_u32)],
     "oxh_net_cross_entropy": [_vp, _u32, _u32, _P(_u32)],
+    "oxh_net_rms_norm": [_vp, _u32, _u32, _f32, _P(_u32)],
+    "oxh_net_gated_recurrence": [_vp, _u32, _u32, _P(_u32)],
     "oxh_net_forward_program": [_vp, _u32, _P(_vp)],
     "oxh_net_training_program": [_vp, _u32, _P(AdamWConfig), _P(_vp)],
+    "oxh_net_training_program_muon": [_vp, _u32, _P(MuonConfig), _P(_u32), _u32,
+                                      _P(AdamWConfig), _P(_vp)],
     "oxh_program_value": [_vp, _u32, _P(_vp)],
     "oxh_program_gradient": [_vp, _u32, _P(_vp)],
     "oxh_program_destroy": [_vp],
@@ -234,6 +244,24 @@ class Tensor:
                        "cross_entropy expects [batch, classes] logits and [batch] targets")
         return Tensor((1,), "cross_entropy", (self, targets))
 
+    # the layers of sequence models (no counterpart in the reference)
+    def rms_norm(self, weight, epsilon: float = 1e-6):
+        """s / rms(s) * weight over the last dimension; of an add's value, in its launch."""
+        if weight.shape != self.shape[-1:] or self.shape[-1] == 0:
+            raise _err(ox.INVALID_SHAPE, "rms_norm weight must match the last dimension")
+        e32 = np.float32(epsilon)
+        if not np.isfinite(e32) or e32 < 0.0:
+            raise _err(ox.EXECUTION, "rms_norm epsilon must be non-negative and finite")
+        return Tensor(self.shape, "rms_norm", (self, weight), epsilon=float(e32))
+
+    def gated_recurrence(self, gate):
+        """h_t = a_t h_{t-1} + (1 - a_t) x_t, a_t = sigmoid(gate_t), over [batch, time,
+        channels] from a zero state."""
+        if len(self.shape) != 3 or gate.shape != self.shape:
+            raise _err(ox.INVALID_SHAPE,
+                       "gated_recurrence expects [batch, time, channels] and a gate of that shape")
+        return Tensor(self.shape, "gated_recurrence", (self, gate))
+
 
 def input(shape, requires_grad: bool = False) -> Tensor:  # noqa: A001 - Tensor::placeholder
     """A value fed per run (a placeholder, tensor/mod.rs:520-522; ``requires_grad`` gives it a
@@ -342,6 +370,11 @@ class Net:
             _call("oxh_net_batch_norm2d", h, n(t.args[0]), n(t.args[1]), n(t.args[2]),
                   st.running_mean.data_ptr(), st.running_variance.data_ptr(),
                   int(a["training"]), a["momentum"], a["epsilon"], ctypes.byref(out))
+        elif t.kind == "rms_norm":
+            _call("oxh_net_rms_norm", h, n(t.args[0]), n(t.args[1]), t.attrs["epsilon"],
+                  ctypes.byref(out))
+        elif t.kind == "gated_recurrence":
+            _call("oxh_net_gated_recurrence", h, n(t.args[0]), n(t.args[1]), ctypes.byref(out))
         elif t.kind == "cross_entropy":
             _call("oxh_net_cross_entropy", h, n(t.args[0]), n(t.args[1]), ctypes.byref(out))
         else:
@@ -442,13 +475,25 @@ def forward_program(output: Tensor, inputs: Sequence[Tensor] = ()) -> Program:
 
 def training_program(loss: Tensor, adamw=None) -> Program:
     """Forward, reverse mode from the one-element ``loss`` (Tensor::backward), and with an
-    ``nn.AdamW`` one optimizer step over every parameter the loss reaches."""
+    ``nn.AdamW`` (or an ``nn.Muon``) one optimizer step over every parameter the loss reaches."""
     net = Net([loss])
     h = _vp()
+    matrices, optimizer = getattr(adamw, "matrices", None), adamw
+    if matrices is not None:
+        adamw = optimizer.adamw
     cfg = None
     if adamw is not None:
         cfg = AdamWConfig(adamw.learning_rate, adamw.weight_decay, adamw.betas[0],
                           adamw.betas[1], adamw.epsilon)
-    _call("oxh_net_training_program", net.handle, net.node[loss.id],
-          ctypes.byref(cfg) if cfg is not None else None, ctypes.byref(h))
+    adamw_cfg = ctypes.byref(cfg) if cfg is not None else None
+    if matrices is None:
+        _call("oxh_net_training_program", net.handle, net.node[loss.id], adamw_cfg,
+              ctypes.byref(h))
+    else:
+        nodes = [net._params[id(p)] for p in matrices if id(p) in net._params]
+        muon = MuonConfig(optimizer.learning_rate, optimizer.weight_decay, optimizer.momentum,
+                          optimizer.epsilon, int(optimizer.nesterov), optimizer.rounds)
+        _call("oxh_net_training_program_muon", net.handle, net.node[loss.id],
+              ctypes.byref(muon), (_u32 * max(len(nodes), 1))(*nodes), len(nodes), adamw_cfg,
+              ctypes.byref(h))
     return Program(h.value, net)

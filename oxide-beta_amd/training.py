@@ -472,7 +472,8 @@ class EvalForward:
 def op_bytes(op: Op) -> tuple[str, int]:
     """(category, algorithmic HBM bytes) of one launch group: every tensor it must read or
     write, once (fp32).  Categories: the hot-path kernel families (batch_norm2d, elementwise,
-    cross_entropy, adamw) and the layers around them (conv2d, avg_pool2d)."""
+    cross_entropy, adamw), the layers around them (conv2d, avg_pool2d) and those of sequence models
+    (rms_norm, gated_recurrence, muon)."""
     nb = lambda t: t.numel() * 4  # noqa: E731
     acc = 3 * nb(op.accumulate_into) if op.accumulate_into is not None else 0
     k = op.kind
@@ -513,6 +514,18 @@ def op_bytes(op: Op) -> tuple[str, int]:
         return "cross_entropy", 2 * nb(op.reads["logits"])
     if k == "adamw":
         return "adamw", sum(7 * nb(t[0]) for t in op.attrs["tensors"])
+    if k == "muon":  # parameter and momentum in and out, gradient in; no fp16 halves
+        return "muon", sum(5 * nb(t) for t in op.by_role["gradient"])
+    if k == "rms_norm_forward":
+        return "rms_norm", 2 * nb(op.reads["x"])
+    if k == "add_rms_norm_forward":
+        return "rms_norm", 4 * nb(op.reads["a"])                           # a, b in; sum, y out
+    if k == "rms_norm_backward":
+        return "rms_norm", 3 * nb(op.reads["gradient"]) + acc              # g, x in; dx out
+    if k == "gated_recurrence_forward":
+        return "gated_recurrence", 3 * nb(op.reads["x"])                   # x, gate in; y out
+    if k == "gated_recurrence_backward":
+        return "gated_recurrence", 6 * nb(op.reads["x"]) + acc     # g, x, gate, y in; dx, dgate out
     if k.startswith("avg_pool2d"):
         return "avg_pool2d", 0
     return "conv2d", 0

@@ -324,3 +324,24 @@ def test_another_stream_a_graph_and_repeats(module, dev, shape):
         torch.cuda.synchronize()
         for a, b in zip(outs, want):
             assert torch.equal(a, b)
+
+
+def test_more_than_the_caches_hold(module, dev):
+    """Inputs and outputs of over 256 MB, whose accesses bypass the caches: a few channels against
+    the formulas."""
+    t = torch.float32
+    u, g = make((1, 46001, 512), t, dev, 1), gates((1, 46001, 512), t, dev, 2)
+    h = torch.empty_like(u)
+    module.gated_recurrence_forward(u, g, h)
+    some = [0, 3, 130, 509, 511]
+    pick = lambda x: x[:, :, some].contiguous()  # noqa: E731
+    ref, err, _, _ = forward_ref(pick(u), pick(g), None, None)
+    within(pick(h), ref, err, t, "output")
+    n = 23003
+    u, g, h = u[:, :n].contiguous(), g[:, :n].contiguous(), h[:, :n].contiguous()
+    dh = make(u.shape, t, dev, 4)
+    du, dg = torch.empty_like(u), torch.empty_like(g)
+    module.gated_recurrence_backward(dh, u, g, h, du, dg)
+    out, _, _ = backward_ref(pick(dh), pick(u), pick(g), pick(h), None, None, None)
+    within(pick(du), out[0], out[1], t, "input gradient")
+    within(pick(dg), out[2], out[3], t, "gate gradient")

@@ -189,3 +189,64 @@ def test_front_end_checks_shapes():
     with pytest.raises(ox.OxideError):  # host tensors
         ox._activation((z(2, 3),), (2, 3), "rms_norm")
     assert np.isfinite(ox.gated_recurrence_workspace_size(1, 1, 1))
+
+
+def test_net_builders():
+    """oxh_net_* of the sequence layers and of the optimizer, before anything is allocated."""
+    import tensor
+
+    L, h, u32 = tensor._lib(), ctypes.c_void_p(), ctypes.c_uint32
+    shape = lambda *d: (ctypes.c_uint64 * len(d))(*d)  # noqa: E731
+    assert L.oxh_net_create(ctypes.byref(h)) == ox.OK
+
+    def leaf(*d, parameter=False):
+        n = u32()
+        if parameter:
+            st = L.oxh_net_parameter(h, len(d), shape(*d), BASE, ctypes.byref(n))
+        else:
+            st = L.oxh_net_input(h, len(d), shape(*d), 0, ctypes.byref(n))
+        assert st == ox.OK
+        return n.value
+
+    x, other, flat = leaf(2, 3, 8), leaf(2, 4, 8), leaf(6, 8)
+    w, short, square = leaf(8, parameter=True), leaf(7, parameter=True), leaf(8, 8, parameter=True)
+    n = u32()
+    out = ctypes.byref(n)
+    for a, b in ((x, short), (x, square), (x, 99), (99, w)):
+        assert L.oxh_net_rms_norm(h, a, b, 1e-6, out) == ox.INVALID_SHAPE
+    for eps in (-1.0, float("nan"), float("inf")):
+        refused(L.oxh_net_rms_norm(h, x, w, eps, out), b"epsilon", ox.EXECUTION)
+    for a, b in ((x, other), (flat, flat), (x, 99), (99, x)):
+        assert L.oxh_net_gated_recurrence(h, a, b, out) == ox.INVALID_SHAPE
+    assert L.oxh_net_rms_norm(h, x, w, 0.0, out) == ox.OK
+    assert L.oxh_net_gated_recurrence(h, n.value, x, out) == ox.OK
+    rank, dims = u32(), (ctypes.c_uint64 * 4)()
+    assert L.oxh_net_node_shape(h, n.value, ctypes.byref(rank), dims) == ox.OK
+    assert rank.value == 3 and list(dims)[:3] == [2, 3, 8]
+    assert L.oxh_net_rms_norm(None, x, w, 0.0, out) == ox.INVALID_SHAPE
+    assert L.oxh_net_gated_recurrence(h, x, x, None) == ox.INVALID_SHAPE
+
+    targets = leaf(6)
+    assert L.oxh_net_cross_entropy(h, flat, targets, out) == ox.OK
+    loss, program = n.value, ctypes.c_void_p()
+
+    def muon(nodes=(square,), root=loss, config=True, **k):
+        a = dict(learning_rate=0.1, weight_decay=0.0, momentum=0.9, epsilon=1e-7, nesterov=1,
+                 rounds=5) | k
+        c = tensor.MuonConfig(**a)
+        return L.oxh_net_training_program_muon(
+            h, root, ctypes.byref(c) if config else None, (u32 * len(nodes))(*nodes), len(nodes),
+            None, ctypes.byref(program))
+
+    refused(muon(root=x), b"scalar", ox.EXECUTION)
+    refused(muon(config=False), b"null")
+    for k in (dict(learning_rate=0.0), dict(learning_rate=float("nan")), dict(weight_decay=-0.1),
+              dict(momentum=1.0), dict(momentum=float("nan")), dict(epsilon=0.0),
+              dict(epsilon=float("inf"))):
+        assert muon(**k) == ox.EXECUTION, k
+    refused(muon(rounds=0), b"rounds")
+    refused(muon(rounds=65), b"rounds")
+    for node in (w, x, 99):
+        assert muon((node,)) == ox.INVALID_SHAPE
+    assert program.value is None
+    assert L.oxh_net_destroy(h) == ox.OK
