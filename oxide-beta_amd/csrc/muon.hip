@@ -13,10 +13,14 @@
 // Products.  An operand value v is held as two float16 numbers, hi = f16(S v) and lo =
 // f16(S v - hi) with S = 2^14, which together keep 22 bits of it; a product is summed as hi hi' +
 // hi lo' + lo hi' in float32 on the matrix cores (the omitted lo lo' is below 2^-22 of the
-// product).  No entry overflows: |X| and |A| stay below 1.5 and |B| below 2.9 for |X|_F <= 1.  The
-// term a X is taken from a float32 copy of X: the error of X itself is what grows from round to
-// round (by up to a = 3.4445 in the directions of small singular values), that of the products
-// stays relative to B X.
+// product).  No entry overflows: |X| and |A| stay below 1.5 and |B| below 2.9 for |X|_F <= 1.
+//
+// X itself is kept as halves too, and a X and b A are added to the summed products from them.  The
+// error of X grows from round to round (by up to a = 3.4445 in the directions of small singular
+// values): with 22 bits in place of float32's 24 the result of five rounds on 1000 x 1280 matrices
+// of rank 125 is 9.5e-6 of its norm off, with a float32 copy beside the halves 8.6e-6, and the
+// copies made B X of 12 x 512 x 2048 move 250 MB in place of 100.  B + a I as the factor would
+// save the addition, but then a X has the error of a factor's halves: 3.0e-5.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -36,15 +40,16 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 constexpr float kScale = 16384.0f, kUnscale = 1.0f / (16384.0f * 16384.0f);
 
 // A matrix of a launch group.  Short = min(rows, columns) and Long are the sides of X; ps and pl
 // the same rounded up to the tile, the padding zero throughout.  `scratch` holds, in order:
-//   x [pl][ps] float32: X'; xs: X in halves; xt0, xt1: X' in halves (one is read while the other
-//   is written); ga [ps][ps] float32: A (its lower tiles, transposed); gs, bs: A and B in halves;
-//   the norm's partial sums.
+//   xt0, xt1 [pl][ps]: X' in halves (one is read while the other is written); gs, bs [ps][ps]: A
+//   and B in halves; the norm's partial sums.
 // Halves of a matrix with k columns: per row, blocks of 32 columns, 32 hi then 32 lo.
 struct Matrix {
   const float *gradient;
@@ -66,17 +71,14 @@ struct Group {
 constexpr uint32_t kNormParts = 256;
 
 struct Layout {
-  uint64_t x, xs, xt0, xt1, ga, gs, bs, parts, total;
+  uint64_t xt0, xt1, gs, bs, parts, total;
 };
 __host__ __device__ inline Layout layout_of(uint64_t ps, uint64_t pl) {
   const uint64_t wide = ps * pl * 4, square = ps * ps * 4;
   Layout l;
-  l.x = 0;
-  l.xs = wide;
-  l.xt0 = 2 * wide;
-  l.xt1 = 3 * wide;
-  l.ga = 4 * wide;
-  l.gs = l.ga + square;
+  l.xt0 = 0;
+  l.xt1 = wide;
+  l.gs = 2 * wide;
   l.bs = l.gs + square;
   l.parts = l.bs + square;
   l.total = l.parts + kNormParts * 4;
@@ -188,7 +190,7 @@ __device__ __forceinline__ void store_line(const uint32_t *words, f16 *to) {
   }
 }
 
-// X = V / (|V| + epsilon) in its three forms, a 32 x 32 tile per block.
+// X' = (V / (|V| + epsilon))' in halves, a 32 x 32 tile per block.
 __global__ __launch_bounds__(256) void muon_start_kernel(Group g) {
   __shared__ float tile[32][33];
   __shared__ float wave[4];
@@ -217,26 +219,21 @@ __global__ __launch_bounds__(256) void muon_start_kernel(Group g) {
     else tile[k][tx] = v;
   }
   __syncthreads();
-  // 16 bytes of a row of each form per thread: four values, or eight hi or lo
-  float *x = reinterpret_cast<float *>(m.scratch + l.x);
-  f16 *xs = reinterpret_cast<f16 *>(m.scratch + l.xs);
+  // 16 bytes of a row per thread: eight hi or lo
   f16 *xt = reinterpret_cast<f16 *>(m.scratch + l.xt0);
   const uint32_t row = threadIdx.x >> 3, piece = threadIdx.x & 7, first = (piece & 3) * 8;
-  f32x4 values;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) values[e] = tile[piece * 4 + e][row];
-  *reinterpret_cast<f32x4 *>(x + static_cast<uint64_t>(j0 + row) * m.ps + i0 + piece * 4) = values;
-  f16x8 straight, turned;
+  f16x8 turned;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     f16 hi, lo;
-    halves_of(tile[row][first + e], hi, lo);
-    straight[e] = piece < 4 ? hi : lo;
     halves_of(tile[first + e][row], hi, lo);
     turned[e] = piece < 4 ? hi : lo;
   }
-  *reinterpret_cast<f16x8 *>(xs + halves_at(i0 + row, j0, m.pl) + piece * 8) = straight;
   *reinterpret_cast<f16x8 *>(xt + halves_at(j0 + row, i0, m.ps) + piece * 8) = turned;
+}
+
+__device__ __forceinline__ f16x8 join(s16x4 a, s16x4 b) {
+  return __builtin_bit_cast(f16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
 enum class Step { Gram, Poly, Apply, Last };
@@ -282,9 +279,40 @@ __device__ __forceinline__ Tile tile_at(uint32_t b, uint32_t rows, uint32_t colu
   return {4 * band + column + at, 4 * band + column};
 }
 
-// One of a round's three products, a square tile per block of threads.  Both operands are halves
-// with the summed index along the rows.  A and B are symmetric: only tiles on and below the
-// diagonal are summed, the others are their mirrors.
+// The lane's four consecutive rows, in each quad q (rows 8 q + 4 (lane / 32) ..), of a column whose
+// 32 values lie at `line` as halves: each lane loads 16-byte pieces 2 h and 2 h + 1 of hi and lo, h
+// = lane / 32, and exchanges with lane ^ 32 the half of each that the other's rows are.
+__device__ __forceinline__ void column_of(const f16 *line, uint32_t lane, f32x4 (&value)[4]) {
+  u32x4 hi[2], lo[2];
+  const f16 *p = line + (lane >> 5) * 16;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    hi[e] = *reinterpret_cast<const u32x4 *>(p + 8 * e);
+    lo[e] = *reinterpret_cast<const u32x4 *>(p + 32 + 8 * e);
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const auto h = __builtin_amdgcn_permlane32_swap(hi[e][k], hi[e][k + 2], false, false);
+      const auto l = __builtin_amdgcn_permlane32_swap(lo[e][k], lo[e][k + 2], false, false);
+#pragma unroll
+      for (int o = 0; o < 2; ++o) {
+        // hi + lo has at most 23 bits
+        const uint32_t hw = h[o], lw = l[o];
+        value[2 * o + e][2 * k] = static_cast<float>(__builtin_bit_cast(f16, static_cast<uint16_t>(hw))) +
+                                  static_cast<float>(__builtin_bit_cast(f16, static_cast<uint16_t>(lw)));
+        value[2 * o + e][2 * k + 1] =
+            static_cast<float>(__builtin_bit_cast(f16, static_cast<uint16_t>(hw >> 16))) +
+            static_cast<float>(__builtin_bit_cast(f16, static_cast<uint16_t>(lw >> 16)));
+      }
+    }
+}
+
+// One of a round's three products, a square tile per block of threads.  A A and B X sum along the
+// rows of their operands, which pass through shared memory as they lie; A = X X' sums along the
+// columns of X', which transposed reads of the shared memory turn.  A and B are symmetric: only
+// tiles on and below the diagonal are summed, the others are their mirrors.
 template <Step S, class Sh>
 __global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int odd) {
   constexpr int kTile = Sh::tile, TM = Sh::TM, TN = Sh::TN, K = Sh::K;
@@ -302,14 +330,15 @@ __global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int 
   const uint32_t k_total = S == Step::Gram ? m.pl : m.ps;
   const f16 *pa, *pb;
   f16 *gs = reinterpret_cast<f16 *>(m.scratch + l.gs), *bs = reinterpret_cast<f16 *>(m.scratch + l.bs);
-  f16 *xs = reinterpret_cast<f16 *>(m.scratch + l.xs);
   f16 *from = reinterpret_cast<f16 *>(m.scratch + (odd ? l.xt1 : l.xt0));
   f16 *to = reinterpret_cast<f16 *>(m.scratch + (odd ? l.xt0 : l.xt1));
-  if constexpr (S == Step::Gram) pa = pb = xs;
+  if constexpr (S == Step::Gram) pa = pb = from;
   else if constexpr (S == Step::Poly) pa = pb = gs;
   else pa = bs, pb = from;
-  const char *sa = reinterpret_cast<const char *>(pa) + static_cast<uint64_t>(ti) * kTile * k_total * 4;
-  const char *sb = reinterpret_cast<const char *>(pb) + static_cast<uint64_t>(tj) * kTile * k_total * 4;
+  // of the operands' rows ti kTile .., or (Gram) columns
+  const uint64_t tile_bytes = S == Step::Gram ? kTile * 4 : static_cast<uint64_t>(kTile) * k_total * 4;
+  const char *sa = reinterpret_cast<const char *>(pa) + ti * tile_bytes;
+  const char *sb = reinterpret_cast<const char *>(pb) + tj * tile_bytes;
 
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t group = wave / (Sh::WM * Sh::WN), place = wave % (Sh::WM * Sh::WN);
@@ -321,21 +350,70 @@ __global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int 
   const uint32_t r0 = threadIdx.x >> 3, c0 = threadIdx.x & 7;
   u32x4 held[kLoads];
   const uint32_t blocks = k_total / 32;
+  // Gram: lines of 256 bytes, which are 64 columns of a row, or 32 of two rows where a tile has no
+  // more.  A line's 32-byte pieces lie at their places exclusive-or a number of the line (`turn_of`),
+  // so that the pieces of four rows that 32 lanes read together, or of eight rows, lie in different
+  // banks.
+  constexpr int kLineRows = kTile == 32 ? 2 : 1;
+  auto turn_of = [](uint32_t line) {
+    return kLineRows == 2 ? (line & 1) << 1 | (line >> 1 & 1) : (line & 3) << 1 | (line >> 2 & 1);
+  };
+  const uint32_t line0 = threadIdx.x >> 4, piece0 = threadIdx.x & 15;
   auto fetch = [&](uint32_t block) {
     if (block >= blocks) return;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const uint32_t r = (i * kStep) % (K * kTile) + r0, row = r % kTile, k = block + r / kTile;
-      const char *p = (i * kStep < K * kTile ? sa : sb) +
-                      static_cast<uint64_t>(row) * k_total * 4 + k * 128 + c0 * 16;
-      held[i] = K == 1 || k < blocks ? *reinterpret_cast<const u32x4 *>(p) : u32x4{0, 0, 0, 0};
+      if constexpr (S == Step::Gram) {
+        // passes of 32 lines: for each 32 rows the tile's columns 64 by 64
+        static_assert(Sh::threads == 512, "32 lines a pass");
+        constexpr int kAcross = kTile >= 64 ? kTile / 64 : 1;
+        const uint32_t pass = i % (kLoads / 2), across = kLineRows == 2 ? 0 : pass % kAcross;
+        const uint32_t row = pass / kAcross * 32 * kLineRows + line0 * kLineRows + piece0 / (16 / kLineRows);
+        const char *p = (i < kLoads / 2 ? sa : sb) +
+                        (static_cast<uint64_t>(block) * 32 + row) * m.ps * 4 + across * 256 +
+                        piece0 % (16 / kLineRows) * 16;
+        held[i] = K == 1 || block + row / 32 < blocks ? *reinterpret_cast<const u32x4 *>(p)
+                                                      : u32x4{0, 0, 0, 0};
+      } else {
+        const uint32_t r = (i * kStep) % (K * kTile) + r0, row = r % kTile, k = block + r / kTile;
+        const char *p = (i * kStep < K * kTile ? sa : sb) +
+                        static_cast<uint64_t>(row) * k_total * 4 + k * 128 + c0 * 16;
+        held[i] = K == 1 || k < blocks ? *reinterpret_cast<const u32x4 *>(p) : u32x4{0, 0, 0, 0};
+      }
     }
   };
   auto put = [&](char *to_stage) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const uint32_t r = i * kStep + r0;
-      *reinterpret_cast<u32x4 *>(to_stage + r * 128 + ((c0 ^ (r >> 1 & 7)) * 16)) = held[i];
+      if constexpr (S == Step::Gram) {
+        *reinterpret_cast<u32x4 *>(to_stage + (i * 32 + line0) * 256 +
+                                   ((piece0 >> 1 ^ turn_of(line0)) << 5 | (piece0 & 1) << 4)) = held[i];
+      } else {
+        const uint32_t r = i * kStep + r0;
+        *reinterpret_cast<u32x4 *>(to_stage + r * 128 + ((c0 ^ (r >> 1 & 7)) * 16)) = held[i];
+      }
+    }
+  };
+  // hi and lo of rows (Gram: columns) 32 t .. of an operand's stage, 16 summed values
+  auto operand = [&](const char *in, uint32_t t, uint32_t half, f16x8 &hi, f16x8 &lo) {
+    if constexpr (S == Step::Gram) {
+      const uint32_t row = half * 16 + (lane >> 5) * 4 + (lane >> 2 & 3), line = row / kLineRows % 32;
+      const uint32_t pass = kLineRows == 2 ? row / 64 : row / 32 * (kTile / 64) + t / 2;
+      const uint32_t part = (kLineRows == 2 ? row & 1 : t & 1) * 4 + (lane >> 4 & 1);
+      const char *p = in + (pass * 32 + line) * 256 + (lane & 3) * 8;
+      constexpr int kEight = 8 / kLineRows * 256;  // eight rows further: the same turn
+      auto read = [&](uint32_t at) {
+        const char *q = p + ((at ^ turn_of(line)) << 5);
+        return join(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)q),
+                    __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(q + kEight)));
+      };
+      hi = read(part);
+      lo = read(part + 2);
+    } else {
+      const uint32_t row = t * 32 + (lane & 31), c = (half & 1) * 2 + (lane >> 5);
+      const char *p = in + (half >> 1) * kTile * 128 + row * 128;
+      hi = *reinterpret_cast<const f16x8 *>(p + ((c ^ (row >> 1 & 7)) * 16));
+      lo = *reinterpret_cast<const f16x8 *>(p + (((c + 4) ^ (row >> 1 & 7)) * 16));
     }
   };
   f32x16 acc[TM][TN];
@@ -360,22 +438,10 @@ __global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int 
     for (int part = 0; part < 2 * K / Sh::Groups; ++part) {
       f16x8 ah[TM], al[TM], bh[TN], bl[TN];
       const uint32_t half = part * Sh::Groups + group;
-      const uint32_t c = (half & 1) * 2 + (lane >> 5);
-      const char *in_a = now + (half >> 1) * kTile * 128, *in_b = in_a + kStage;
 #pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        const uint32_t row = (wi * TM + i) * 32 + (lane & 31);
-        ah[i] = *reinterpret_cast<const f16x8 *>(in_a + row * 128 + ((c ^ (row >> 1 & 7)) * 16));
-        al[i] =
-            *reinterpret_cast<const f16x8 *>(in_a + row * 128 + (((c + 4) ^ (row >> 1 & 7)) * 16));
-      }
+      for (int i = 0; i < TM; ++i) operand(now, wi * TM + i, half, ah[i], al[i]);
 #pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const uint32_t row = (wj * TN + j) * 32 + (lane & 31);
-        bh[j] = *reinterpret_cast<const f16x8 *>(in_b + row * 128 + ((c ^ (row >> 1 & 7)) * 16));
-        bl[j] =
-            *reinterpret_cast<const f16x8 *>(in_b + row * 128 + (((c + 4) ^ (row >> 1 & 7)) * 16));
-      }
+      for (int j = 0; j < TN; ++j) operand(now + kStage, wj * TN + j, half, bh[j], bl[j]);
       if (part == 0 && block + K < blocks) {
         put(stage + turn * 2 * kStage);
         fetch(block + 2 * K);
@@ -438,11 +504,9 @@ __global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int 
   }
 
   // Lane l holds column l % 32 and, in register r, row 8 (r / 4) + 4 (l / 32) + r % 4 of each
-  // 32 x 32 block: four consecutive rows per register quad, which x and ga, kept transposed, move
-  // at once.  The halves go through the wave's own part of the shared memory (whose operands have
-  // been read: a barrier ended the sums), by rows and then by columns, and leave as whole lines: 32
-  // hi and 32 lo of a row.
-  float *x = reinterpret_cast<float *>(m.scratch + l.x), *ga = reinterpret_cast<float *>(m.scratch + l.ga);
+  // 32 x 32 block: four consecutive rows per register quad.  The halves go through the wave's own
+  // part of the shared memory (whose operands have been read: a barrier ended the sums), by columns
+  // and (A and B off the diagonal) by rows, and leave as whole lines: 32 hi and 32 lo of a row.
   constexpr uint32_t kPitch = 36;  // words per line of the wave's 32 x 32 words
   constexpr int kFinishing = TM * TN < Sh::Groups ? TM * TN : Sh::Groups;  // groups with a block
   static_assert(Sh::WM * Sh::WN * kFinishing * 32 * kPitch * 4 <= 4 * kStage, "turning space");
@@ -454,18 +518,18 @@ __global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int 
       if (Sh::Groups > 1 && (i * TN + j) % Sh::Groups != static_cast<int>(group)) continue;
       const uint32_t row0 = ti * kTile + (wi * TM + i) * 32, column0 = tj * kTile + (wj * TN + j) * 32;
       const uint32_t column = column0 + (lane & 31);
+      // X or A at this place: among the operand rows just read
+      f32x4 addend[4];
+      if constexpr (S != Step::Gram) column_of(pb + halves_at(column, row0, m.ps), lane, addend);
       u32x4 words[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const uint32_t at = 8 * q + 4 * (lane >> 5), row = row0 + at;
-        const uint64_t turned_at = static_cast<uint64_t>(column) * m.ps + row;
         f32x4 v;
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] = acc[i][j][4 * q + r] * kUnscale;
-        if constexpr (S == Step::Poly)
-          v = kB * *reinterpret_cast<const f32x4 *>(ga + turned_at) + kC * v;
-        if constexpr (S == Step::Apply || S == Step::Last)
-          v += kA * *reinterpret_cast<const f32x4 *>(x + turned_at);
+        if constexpr (S == Step::Poly) v = kB / kScale * addend[q] + kC * v;
+        if constexpr (S == Step::Apply || S == Step::Last) v += kA / kScale * addend[q];
         if constexpr (S == Step::Last) {
           const bool tall = m.rows > m.columns;
           const uint32_t wr0 = tall ? column : row, wc0 = tall ? row : column;
@@ -487,32 +551,25 @@ __global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int 
               if (r < left) t[r * next] = v[r];
           }
         } else {
-          if constexpr (S == Step::Apply) *reinterpret_cast<f32x4 *>(x + turned_at) = v;
-          if constexpr (S == Step::Gram) *reinterpret_cast<f32x4 *>(ga + turned_at) = v;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            words[q][r] = halves_word(v[r]);
-            turned[(at + r) * kPitch + (lane & 31)] = words[q][r];
-          }
+          for (int r = 0; r < 4; ++r) words[q][r] = halves_word(v[r]);
+          *reinterpret_cast<u32x4 *>(turned + (lane & 31) * kPitch + at) = words[q];
         }
       }
       if constexpr (S != Step::Last) {
-        f16 *straight = S == Step::Gram ? gs : S == Step::Poly ? bs : xs;
-        f16 *mirror = S == Step::Apply ? to : straight;
-        __builtin_amdgcn_wave_barrier();
+        f16 *result = S == Step::Gram ? gs : S == Step::Poly ? bs : to;
         const uint32_t *line = turned + (lane >> 1) * kPitch + (lane & 1) * 16;
-        store_line(line,
-                   straight + halves_at(row0 + (lane >> 1), column0 + (lane & 1) * 16,
-                                        S == Step::Apply ? m.pl : m.ps));
         __builtin_amdgcn_wave_barrier();
-        if (S == Step::Apply || ti != tj) {
+        store_line(line, result + halves_at(column0 + (lane >> 1), row0 + (lane & 1) * 16, m.ps));
+        __builtin_amdgcn_wave_barrier();
+        if (kSymmetric && ti != tj) {
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<u32x4 *>(turned + (lane & 31) * kPitch + 8 * q + 4 * (lane >> 5)) =
-                words[q];
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              turned[(8 * q + 4 * (lane >> 5) + r) * kPitch + (lane & 31)] = words[q][r];
           __builtin_amdgcn_wave_barrier();
-          store_line(line,
-                     mirror + halves_at(column0 + (lane >> 1), row0 + (lane & 1) * 16, m.ps));
+          store_line(line, result + halves_at(row0 + (lane >> 1), column0 + (lane & 1) * 16, m.ps));
           __builtin_amdgcn_wave_barrier();
         }
       }
@@ -529,9 +586,6 @@ __global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int 
 // and transposed reads of the shared memory (16 lanes fetch 4 rows of 16 float16 and each gets a
 // column of 4) give the same order for X X'.
 
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-
 constexpr int kWhole = 163840;  // bytes of shared memory, the last for the norm's parts
 constexpr int kWholeWaves = 12;
 // X': bytes of a row of PS values in halves (hi, then lo), an odd number of 32-byte steps, so that
@@ -543,9 +597,6 @@ constexpr int whole_pitch(int ps) { return ps * 4 + 32; }
 constexpr int square_pitch(int ps) { return (ps / 16 + 1) * 16; }
 constexpr int square_bytes(int ps) { return 4 * ps * square_pitch(ps); }
 
-__device__ __forceinline__ f16x8 join(s16x4 a, s16x4 b) {
-  return __builtin_bit_cast(f16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
-}
 // Four values as hi and lo.
 __device__ __forceinline__ void halves_of(const f32x4 &v, s16x4 &hi, s16x4 &lo) {
 #pragma unroll
