@@ -240,16 +240,23 @@ enum class Step { Gram, Poly, Apply, Last };
 
 // The block shapes of the products: Groups times WM x WN waves of TM x TN blocks of 32 x 32, and
 // K blocks of 32 summed values per stage, of whose 2 K halves each group takes every Groups-th.
-template <int WM_, int WN_, int TM_, int TN_, int K_, int Groups_>
+// Direct loads (from memory straight to shared memory, one stage ahead) need fewer registers than
+// loads through registers (two stages ahead), so that two blocks share a compute unit where there
+// are two: 12 x 512 x 2048, of 128 and 64, 604 us and 687.  One block alone waits longer for them:
+// 4096 x 4096, of 192, 4.63 ms and 4.02; 1000 x 1280, of 64, 270 us and 230, and 222 with four
+// groups; 1091 x 87, of 32, 108 us and 98.
+template <int WM_, int WN_, int TM_, int TN_, int K_, int Groups_, bool Direct_>
 struct Shape {
+  static constexpr bool Direct = Direct_;
   static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, K = K_, Groups = Groups_;
   static constexpr int threads = WM * WN * Groups * 64, tile = WM * TM * 32;
   static_assert(WM * TM == WN * TN && 2 * K % Groups == 0, "square tiles, whole halves");
 };
-using Wide = Shape<2, 2, 3, 3, 1, 2>;    // 192 x 192
-using Medium = Shape<2, 2, 2, 2, 1, 2>;  // 128 x 128
-using Small = Shape<2, 2, 1, 1, 2, 2>;   // 64 x 64
-using Tiny = Shape<1, 1, 1, 1, 4, 8>;    // 32 x 32
+using Wide = Shape<2, 2, 3, 3, 1, 2, false>;    // 192 x 192
+using Medium = Shape<2, 2, 2, 2, 1, 2, true>;   // 128 x 128
+using Small = Shape<2, 2, 1, 1, 2, 2, true>;    // 64 x 64
+using Few = Shape<2, 2, 1, 1, 2, 4, false>;     // 64 x 64, where no compute unit has two
+using Tiny = Shape<1, 1, 1, 1, 4, 8, false>;    // 32 x 32
 
 // The tile of index b among rows x columns tiles, or (Symmetric) among those on and below the
 // diagonal of rows x rows: bands of four tile rows, each taken column by column, so that the run
@@ -340,59 +347,71 @@ __global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int 
   const char *sa = reinterpret_cast<const char *>(pa) + ti * tile_bytes;
   const char *sb = reinterpret_cast<const char *>(pb) + tj * tile_bytes;
 
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t group = wave / (Sh::WM * Sh::WN), place = wave % (Sh::WM * Sh::WN);
   const uint32_t wi = place / Sh::WN, wj = place % Sh::WN;
-  // this thread's 16-byte pieces of a stage: piece c0 of rows r0, r0 + kStep, ... of the operands'
-  // K blocks one after the other
-  constexpr int kStep = Sh::threads / 8, kLoads = 2 * K * kTile / kStep;
-  static_assert(K * kTile % kStep == 0, "an operand is whole passes");
-  const uint32_t r0 = threadIdx.x >> 3, c0 = threadIdx.x & 7;
-  u32x4 held[kLoads];
-  const uint32_t blocks = k_total / 32;
   // Gram: lines of 256 bytes, which are 64 columns of a row, or 32 of two rows where a tile has no
   // more.  A line's 32-byte pieces lie at their places exclusive-or a number of the line (`turn_of`),
   // so that the pieces of four rows that 32 lanes read together, or of eight rows, lie in different
   // banks.
-  constexpr int kLineRows = kTile == 32 ? 2 : 1;
+  constexpr int kLineRows = kTile == 32 ? 2 : 1, kAcross = kTile >= 64 ? kTile / 64 : 1;
   auto turn_of = [](uint32_t line) {
     return kLineRows == 2 ? (line & 1) << 1 | (line >> 1 & 1) : (line & 3) << 1 | (line >> 2 & 1);
   };
-  const uint32_t line0 = threadIdx.x >> 4, piece0 = threadIdx.x & 15;
-  auto fetch = [&](uint32_t block) {
-    if (block >= blocks) return;
+  // Direct: operands pass from memory to shared memory without a stop in registers.  Each load of a
+  // wave fills 1024 bytes there in the order of its lanes, so a lane loads the piece that belongs at
+  // its place (both ways do).
+  constexpr int kLoads = 2 * K * kTile * 8 / Sh::threads, kRows = Sh::threads / 8;
+  static_assert(kLoads % 2 == 0 && (kRows == 64 || (kRows == 128 && kTile == 64 && K == 2)),
+                "passes of rows, or of lines");
+  u32x4 held[kLoads];
+  const uint32_t blocks = k_total / 32;  // a multiple of the tile's
+  constexpr bool kTail = kTile < 32 * K;
+  const uint32_t r0 = threadIdx.x >> 3, c0 = (threadIdx.x & 7) ^ (r0 >> 1 & 7);
+  const uint32_t line0 = threadIdx.x >> 4,
+                 piece0 = ((threadIdx.x >> 1 & 7) ^ turn_of(line0)) << 1 | (threadIdx.x & 1);
+  auto fetch = [&](uint32_t block, char *to_stage) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
+      const uint32_t pass = i % (kLoads / 2);
+      const char *p = i < kLoads / 2 ? sa : sb;
+      // The source is a block of 32 summed values, the same for the wave; past the last one (whose
+      // products are left out) the last is read again
+      auto source = [&](uint32_t ahead) {
+        return static_cast<uint64_t>(kTail ? min(block + ahead, blocks - 1) : block + ahead) * 128;
+      };
       if constexpr (S == Step::Gram) {
-        // passes of 32 lines: for each 32 rows the tile's columns 64 by 64
-        static_assert(Sh::threads == 512, "32 lines a pass");
-        constexpr int kAcross = kTile >= 64 ? kTile / 64 : 1;
-        const uint32_t pass = i % (kLoads / 2), across = kLineRows == 2 ? 0 : pass % kAcross;
-        const uint32_t row = pass / kAcross * 32 * kLineRows + line0 * kLineRows + piece0 / (16 / kLineRows);
-        const char *p = (i < kLoads / 2 ? sa : sb) +
-                        (static_cast<uint64_t>(block) * 32 + row) * m.ps * 4 + across * 256 +
-                        piece0 % (16 / kLineRows) * 16;
-        held[i] = K == 1 || block + row / 32 < blocks ? *reinterpret_cast<const u32x4 *>(p)
-                                                      : u32x4{0, 0, 0, 0};
+        // passes of lines: for each 32 rows the tile's columns 64 by 64
+        const uint32_t line = pass * (kRows / 2) + line0, lines = line / 32;
+        const uint32_t row = line % 32 * kLineRows + piece0 / (16 / kLineRows);
+        p += source((pass * (kRows / 2) + wave * 4) / 32 / kAcross * kLineRows + wave * 4 % 32 * kLineRows / 32) * m.ps;
+        p += row % 32 * m.ps * 4 + lines % kAcross * 256 + piece0 % (16 / kLineRows) * 16;
       } else {
-        const uint32_t r = (i * kStep) % (K * kTile) + r0, row = r % kTile, k = block + r / kTile;
-        const char *p = (i * kStep < K * kTile ? sa : sb) +
-                        static_cast<uint64_t>(row) * k_total * 4 + k * 128 + c0 * 16;
-        held[i] = K == 1 || k < blocks ? *reinterpret_cast<const u32x4 *>(p) : u32x4{0, 0, 0, 0};
+        const uint32_t row = kTile % kRows == 0 ? pass * kRows % kTile + r0 : (pass * kRows + r0) % kTile;
+        p += source((pass * kRows + wave * 8) / kTile);
+        p += row * k_total * 4 + c0 * 16;
+      }
+      if constexpr (Sh::Direct) {
+        __builtin_amdgcn_global_load_lds(
+            (const __attribute__((address_space(1))) void *)p,
+            (__attribute__((address_space(3))) void *)(to_stage + (i * Sh::threads + wave * 64) * 16), 16, 0, 0);
+      } else {
+        held[i] = *reinterpret_cast<const u32x4 *>(p);
       }
     }
   };
   auto put = [&](char *to_stage) {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      if constexpr (S == Step::Gram) {
-        *reinterpret_cast<u32x4 *>(to_stage + (i * 32 + line0) * 256 +
-                                   ((piece0 >> 1 ^ turn_of(line0)) << 5 | (piece0 & 1) << 4)) = held[i];
-      } else {
-        const uint32_t r = i * kStep + r0;
-        *reinterpret_cast<u32x4 *>(to_stage + r * 128 + ((c0 ^ (r >> 1 & 7)) * 16)) = held[i];
-      }
+    for (int i = 0; i < kLoads; ++i)
+      *reinterpret_cast<u32x4 *>(to_stage + (i * Sh::threads + threadIdx.x) * 16) = held[i];
+  };
+  // Ends with every thread's operands there.
+  auto arrive = [] {
+    if constexpr (Sh::Direct) {
+      __builtin_amdgcn_sched_barrier(0);  // behind the products
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
+    __syncthreads();
   };
   // hi and lo of rows (Gram: columns) 32 t .. of an operand's stage, 16 summed values
   auto operand = [&](const char *in, uint32_t t, uint32_t half, f16x8 &hi, f16x8 &lo) {
@@ -423,29 +442,37 @@ __global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int 
     for (int j = 0; j < TN; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-  // Operands pass from memory to registers two stages ahead, and on to the buffer that is not
-  // being read one stage ahead, behind the first fragments' reads (its own last readers passed the
-  // barrier).  Loading further ahead, or more per stage, changed nothing.
-  fetch(0);
-  put(stage);
-  fetch(K);
-  __syncthreads();
+  // A stage is loaded while the one before is multiplied, from behind its last fragments' reads into
+  // the buffer whose readers passed the barrier.
+  fetch(0, stage);
+  if constexpr (!Sh::Direct) {
+    put(stage);
+    if (K < blocks) fetch(K, stage);
+  }
+  arrive();
   int turn = 0;
   for (uint32_t block = 0; block < blocks; block += K) {
     const char *now = stage + turn * 2 * kStage;
     turn ^= 1;
+    constexpr int kParts = 2 * K / Sh::Groups;
 #pragma unroll
-    for (int part = 0; part < 2 * K / Sh::Groups; ++part) {
+    for (int part = 0; part < kParts; ++part) {
       f16x8 ah[TM], al[TM], bh[TN], bl[TN];
       const uint32_t half = part * Sh::Groups + group;
+      const bool within = !kTail || block + half / 2 < blocks;
+      if (within) {
 #pragma unroll
-      for (int i = 0; i < TM; ++i) operand(now, wi * TM + i, half, ah[i], al[i]);
+        for (int i = 0; i < TM; ++i) operand(now, wi * TM + i, half, ah[i], al[i]);
 #pragma unroll
-      for (int j = 0; j < TN; ++j) operand(now + kStage, wj * TN + j, half, bh[j], bl[j]);
-      if (part == 0 && block + K < blocks) {
-        put(stage + turn * 2 * kStage);
-        fetch(block + 2 * K);
+        for (int j = 0; j < TN; ++j) operand(now + kStage, wj * TN + j, half, bh[j], bl[j]);
       }
+      if constexpr (Sh::Direct) {
+        if (part == kParts - 1 && block + K < blocks) fetch(block + K, stage + turn * 2 * kStage);
+      } else if (part == 0 && block + K < blocks) {
+        put(stage + turn * 2 * kStage);
+        if (block + 2 * K < blocks) fetch(block + 2 * K, stage);
+      }
+      if (!within) continue;
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -462,7 +489,7 @@ __global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int 
         for (int j = 0; j < TN; ++j)
           acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], acc[i][j], 0, 0, 0);
     }
-    __syncthreads();
+    arrive();
   }
 
   // The groups' sums meet: block t of a wave's TM x TN is finished by group t % Groups, which adds
@@ -890,17 +917,18 @@ struct Tiles {
 
 // Small tiles spread a product over more compute units, large ones load less per product.  Each
 // product takes
-//   32 where its tiles of 32 are at most one per compute unit (512 x 512: 119 us, 157 with 64;
-//     1024 x 1024: 327 and 245; 512 x 2048, whose B X has 1024 such tiles: 208 with 32 for both
-//     products, 179 with 32 and 64, 240 with 64);
-//   128 where there is one for every other compute unit (B X of 1536 x 1536, 144 tiles: 493 us, 523
-//     with 64; 1000 x 1280, 80 tiles: 311 and 284; all of 2048 x 2048, 136 and 256 tiles: 794 and
-//     958) and padding to 128 adds at most a tenth (32 matrices of 300 x 1200, padded 1.26 times:
-//     992 and 739);
-//   64 otherwise;
+//   32 where its tiles of 32 are at most one per compute unit (512 x 512: 101 us, 135 with 64;
+//     1024 x 1024: 282 and 201; 512 x 2048, whose B X has 1024 such tiles: 166 with 32 for both
+//     products, 145 with 32 and 64, 190 with 64);
+//   128 where there is one for every other compute unit (B X of 1000 x 4000, 256 tiles: 422 us, 443
+//     with 64; of 1536 x 1536, 144 tiles: 524 both; of 1000 x 1280, 80 tiles: 302 and 230; all of
+//     2560 x 2560, 210 and 400 tiles: 1367 and 1608) and padding to 128 adds at most a tenth (32
+//     matrices of 300 x 1200, padded 1.26 times: 739 and 618);
+//   64 otherwise (`Few` up to a block per compute unit: 1024 x 1024, 136 and 256 tiles, 201 us and
+//     254 without; everywhere, 12 x 512 x 2048 takes 716 and 657 without);
 // and both take 192 where the square products just fill one round of a block per compute unit, with
-// the same limit on padding (4096 x 4096, 253 tiles: 4.43 ms, 4.87 with 128; 6144 x 6144, 528
-// tiles: 14.96 and 14.71; 12 x 1024 x 1024, 252 tiles padded 1.27 times: 1645 us and 1300).
+// the same limit on padding (4096 x 4096, 253 tiles: 4.06 ms, 4.80 with 128; 2560 x 2560, 105 tiles:
+// 1641 and 1367 us; 12 x 1024 x 1024, 252 tiles padded 1.27 times: 1330 and 1079).
 Tiles tiles_of(const Item *items, size_t count) {
   struct Count {
     uint64_t square = 0, apply = 0, area = 0;
@@ -972,6 +1000,7 @@ oxh_status product(hipStream_t stream, Group &g, uint32_t tile, int odd, const c
   };
   if (tile == Wide::tile) start(Wide());
   else if (tile == Medium::tile) start(Medium());
+  else if (tile == Small::tile && g.blocks <= oxh::kComputeUnits) start(Few());
   else if (tile == Small::tile) start(Small());
   else start(Tiny());
   return oxh::launched(what);

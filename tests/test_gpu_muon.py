@@ -156,3 +156,39 @@ def test_another_stream_a_graph_and_repeats(module, dev):
         torch.cuda.synchronize()
         for a, b in zip(p + m, want):
             assert torch.equal(a, b)
+
+
+# sides at which tiles of 64 fill the compute units once or more often, of 128, and of 192
+LARGE = [(1000, 1280), (520, 2050), (1537, 1660), (4000, 1030), (2050, 2300), (3900, 3870)]
+
+
+def orthogonal_on(v, rounds=5, eps=1e-7):
+    """``orthogonal`` of a float64 tensor where it lies."""
+    x = v.T.contiguous() if v.shape[0] > v.shape[1] else v
+    x = x / (x.norm() + eps)
+    for _ in range(rounds):
+        gram = x @ x.T.contiguous()
+        x = A * x + (B * gram + C * (gram @ gram)) @ x
+    return x.T.contiguous() if v.shape[0] > v.shape[1] else x
+
+
+@pytest.mark.parametrize("shape", LARGE)
+def test_large(module, dev, shape):
+    """Both entry points, with a spectrum that falls by 10^4 over an eighth of the directions."""
+    g = torch.Generator().manual_seed(11)
+    rank = min(shape) // 8
+    left = torch.randn(shape[0], rank, generator=g) * torch.logspace(0, -4, rank)
+    v = (left @ torch.randn(rank, shape[1], generator=g) +
+         1e-4 * torch.randn(*shape, generator=g)).to(dev)
+    out = torch.empty_like(v)
+    module.orthogonalize(v, out)
+    ref = orthogonal_on(v.double())
+    assert (out.double() - ref).norm() <= BOUND * ref.norm()
+    p = torch.randn(*shape, generator=g).to(dev)
+    m = torch.zeros_like(p)
+    moved = 0.1 * math.sqrt(max(1.0, shape[0] / shape[1])) * ref
+    want = p.double() - moved
+    module.muon(0.1, 0.0, 0.9, [(p, v, m)], nesterov=False)
+    assert torch.equal(m, v)
+    tol = BOUND * moved.norm() + 4 * 2.0 ** -24 * want.norm()
+    assert (p.double() - want).norm() <= tol
