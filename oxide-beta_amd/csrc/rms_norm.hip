@@ -19,8 +19,10 @@
 namespace {
 
 using oxh::storage::bf16;
-using oxh::storage::load;
-using oxh::storage::store;
+using oxh::storage::load_places;
+using oxh::storage::Places;
+using oxh::storage::places_at;
+using oxh::storage::store_places;
 
 // The sum over a row's Lanes threads (whole waves) in one fixed order, in every thread.  `slot`
 // is a buffer of 16 floats; consecutive calls alternate between two.
@@ -51,7 +53,7 @@ struct Forward {
 
 // One row per Lanes threads, kept in registers between its two uses: Chunks accesses of N values
 // per thread cover it.
-template <typename T, int N, int Lanes, int Chunks>
+template <typename T, int N, int Lanes, int Chunks, bool Ragged>
 __global__ __launch_bounds__(Lanes < 256 ? 256 : Lanes) void rms_norm_forward_kernel(
     Forward<T> a) {
   __shared__ float slot[16];
@@ -66,10 +68,11 @@ __global__ __launch_bounds__(Lanes < 256 ? 256 : Lanes) void rms_norm_forward_ke
   for (int c = 0; c < Chunks; ++c) {
     const uint32_t at = (c * Lanes + lane) * N;
     if (at < a.columns) {
-      load<T, N>(a.x + base + at, v[c]);
+      const Places here = places_at<N, Ragged>(at, a.columns);
+      load_places<T, N, Ragged>(a.x + base, here, v[c]);
       if (a.r != nullptr) {
         float r[N];
-        load<T, N>(a.r + base + at, r);
+        load_places<T, N, Ragged>(a.r + base, here, r);
 #pragma unroll
         for (int i = 0; i < N; ++i) v[c][i] += r[i];
       }
@@ -87,12 +90,13 @@ __global__ __launch_bounds__(Lanes < 256 ? 256 : Lanes) void rms_norm_forward_ke
   for (int c = 0; c < Chunks; ++c) {
     const uint32_t at = (c * Lanes + lane) * N;
     if (at >= a.columns) continue;
-    if (a.s != nullptr) store<T, N>(a.s + base + at, v[c]);
+    const Places here = places_at<N, Ragged>(at, a.columns);
+    if (a.s != nullptr) store_places<T, N, Ragged>(a.s + base, here, v[c]);
     float w[N];
-    load<float, N>(a.w + at, w);
+    load_places<float, N, Ragged>(a.w, here, w);
 #pragma unroll
     for (int i = 0; i < N; ++i) v[c][i] = v[c][i] * q * w[i];
-    store<T, N>(a.y + base + at, v[c]);
+    store_places<T, N, Ragged>(a.y + base, here, v[c]);
   }
 }
 
@@ -131,25 +135,26 @@ struct Backward {
 };
 
 // Each group of Lanes threads takes every groups-th row and keeps its share of the weight
-// gradient in registers; the groups' shares go to `partial`, one row of columns each.
-template <typename T, int N, int Lanes, int Chunks>
+// gradient in registers; a block's groups add theirs in shared memory, in order, and each block's
+// sum goes to its row of `partial`.
+template <typename T, int N, int Lanes, int Chunks, bool Ragged>
 __global__ __launch_bounds__(Lanes < 256 ? 256 : Lanes) void rms_norm_backward_kernel(
     Backward<T> a) {
   __shared__ float slot[2][16];
-  constexpr int kRows = Lanes < 256 ? 256 / Lanes : 1;
-  const uint32_t lane = threadIdx.x % Lanes;
-  const uint64_t group = static_cast<uint64_t>(blockIdx.x) * kRows + threadIdx.x / Lanes;
-  const uint64_t groups = static_cast<uint64_t>(gridDim.x) * kRows;
+  constexpr int kGroups = Lanes < 256 ? 256 / Lanes : 1;  // of a block
+  const uint32_t lane = threadIdx.x % Lanes, own = threadIdx.x / Lanes;
+  const uint64_t groups = static_cast<uint64_t>(gridDim.x) * kGroups;
   float dw[Chunks][N], w[Chunks][N];
 #pragma unroll
   for (int c = 0; c < Chunks; ++c) {
     const uint32_t at = (c * Lanes + lane) * N;
 #pragma unroll
     for (int i = 0; i < N; ++i) dw[c][i] = w[c][i] = 0.0f;
-    if (at < a.columns) load<float, N>(a.w + at, w[c]);
+    if (at < a.columns) load_places<float, N, Ragged>(a.w, places_at<N, Ragged>(at, a.columns), w[c]);
   }
   int turn = 0;
-  for (uint64_t row = group; row < a.rows; row += groups) {
+  for (uint64_t row = static_cast<uint64_t>(blockIdx.x) * kGroups + own; row < a.rows;
+       row += groups) {
     const uint64_t base = row * a.columns;
     const float q = a.q[row];
     float unit[Chunks][N], d[Chunks][N];
@@ -160,8 +165,9 @@ __global__ __launch_bounds__(Lanes < 256 ? 256 : Lanes) void rms_norm_backward_k
 #pragma unroll
       for (int i = 0; i < N; ++i) unit[c][i] = d[c][i] = 0.0f;
       if (at >= a.columns) continue;
-      load<T, N>(a.s + base + at, unit[c]);
-      load<T, N>(a.g + base + at, d[c]);
+      const Places here = places_at<N, Ragged>(at, a.columns);
+      load_places<T, N, Ragged>(a.s + base, here, unit[c]);
+      load_places<T, N, Ragged>(a.g + base, here, d[c]);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         unit[c][i] *= q;
@@ -176,23 +182,43 @@ __global__ __launch_bounds__(Lanes < 256 ? 256 : Lanes) void rms_norm_backward_k
     for (int c = 0; c < Chunks; ++c) {
       const uint32_t at = (c * Lanes + lane) * N;
       if (at >= a.columns) continue;
+      const Places here = places_at<N, Ragged>(at, a.columns);
       float out[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) out[i] = q * (d[c][i] - unit[c][i] * mean);
       if (a.sg != nullptr) {
         float sg[N];
-        load<T, N>(a.sg + base + at, sg);
+        load_places<T, N, Ragged>(a.sg + base, here, sg);
 #pragma unroll
         for (int i = 0; i < N; ++i) out[i] += sg[i];
       }
-      store<T, N>(a.dx + base + at, out);
+      store_places<T, N, Ragged>(a.dx + base, here, out);
     }
   }
   if (a.partial == nullptr) return;
+  float *to = a.partial + static_cast<uint64_t>(blockIdx.x) * a.columns;
+  if constexpr (kGroups == 1) {
 #pragma unroll
-  for (int c = 0; c < Chunks; ++c) {
-    const uint32_t at = (c * Lanes + lane) * N;
-    if (at < a.columns) store<float, N>(a.partial + group * a.columns + at, dw[c]);
+    for (int c = 0; c < Chunks; ++c) {
+      const uint32_t at = (c * Lanes + lane) * N;
+      if (at >= a.columns) continue;
+      store_places<float, N, Ragged>(to, places_at<N, Ragged>(at, a.columns), dw[c]);
+    }
+  } else {
+    __shared__ float shares[kGroups][Lanes * Chunks * N];
+#pragma unroll
+    for (int c = 0; c < Chunks; ++c) {
+      const uint32_t at = (c * Lanes + lane) * N;
+      if (at >= a.columns) continue;
+      store_places<float, N, Ragged>(shares[own], places_at<N, Ragged>(at, a.columns), dw[c]);
+    }
+    __syncthreads();
+    for (uint32_t at = threadIdx.x; at < a.columns; at += 256) {
+      float sum = shares[0][at];
+#pragma unroll
+      for (int i = 1; i < kGroups; ++i) sum += shares[i][at];
+      to[at] = sum;
+    }
   }
 }
 
@@ -249,39 +275,53 @@ __global__ __launch_bounds__(1024) void rms_norm_weight_kernel(const float *part
   if (strand == 0 && column < columns) out[column] = part[0][c];
 }
 
-// Values that one row's registers cover at N values per access (8 accesses of 1024 threads).
-template <int N>
-constexpr uint64_t row_limit() {
-  return 1024ull * 8 * N;
+// Values of a row that a block's registers hold.  The backward keeps five per value of its row and
+// its masks need more: past these limits the registers spill, and two passes are faster (bfloat16
+// 1024 x 32769: 146 us, 441 in registers; float32 512 x 20001: 53 and 105; within the limits
+// bfloat16 1024 x 16383: 46 us, 74 in two passes; float32 1024 x 16384: 40 and 79).
+template <typename T>
+constexpr uint64_t forward_limit() {
+  return 1024 * 8 * (16 / sizeof(T));
 }
+constexpr uint64_t backward_limit(bool ragged) { return ragged ? 16384 : 32768; }
 
 template <int Lanes, int Chunks>
 struct Shape {
   static constexpr int lanes = Lanes, chunks = Chunks;
 };
 
-// Calls run(Shape<lanes, chunks>) with the fewest threads per row that keep it within 8 accesses
-// each.
-template <int N, typename Run>
+// Calls run(Shape<lanes, chunks>) with the fewest threads per row that keep it within 8 accesses,
+// and where that is one wave within 32 values, each.  Limit: columns never exceed it.
+template <int N, uint64_t Limit, typename Run>
 void with_shape(uint64_t columns, Run run) {
   const uint64_t packs = (columns + N - 1) / N;
-  if (packs <= 64) run(Shape<64, 1>());
-  else if (packs <= 128) run(Shape<64, 2>());
-  else if (packs <= 256) run(Shape<64, 4>());
-  else if (packs <= 512) run(Shape<256, 2>());
-  else if (packs <= 1024) run(Shape<256, 4>());
-  else if (packs <= 2048) run(Shape<256, 8>());
-  else if (packs <= 4096) run(Shape<1024, 4>());
-  else run(Shape<1024, 8>());
+  if constexpr (N == 1) return run(Shape<64, 1>());  // rows of fewer values than an access
+  if (packs <= 64) return run(Shape<64, 1>());
+  if (packs <= 128) return run(Shape<64, 2>());
+  if (packs <= 256) return run(Shape<64, 4>());
+  if (packs <= 512) return run(std::conditional_t<N <= 4, Shape<64, 8>, Shape<256, 2>>());
+  if (packs <= 1024) return run(Shape<256, 4>());
+  if (Limit / N <= 2048 || packs <= 2048) return run(Shape<256, 8>());
+  if constexpr (Limit / N > 2048)
+    if (Limit / N <= 4096 || packs <= 4096) return run(Shape<1024, 4>());
+  if constexpr (Limit / N > 4096) run(Shape<1024, 8>());
 }
 
-// Groups of rows that the backward's weight gradient is summed over (rows of `partial`, which
-// stays within 8 MB up to 8192 columns).
-uint64_t group_limit(uint64_t columns) {
-  return std::min<uint64_t>(2048, std::max<uint64_t>(256, (1ull << 21) / columns));
+// Calls run(pack, ragged) for rows of these columns: 16 bytes per access, or one value where a row
+// has fewer.
+template <typename T, typename Run>
+void with_pack(uint64_t columns, Run run) {
+  constexpr int kPack = 16 / sizeof(T);
+  typedef std::integral_constant<int, kPack> Packed;
+  if (columns % kPack == 0) run(Packed(), std::false_type());
+  else if (columns > kPack) run(Packed(), std::true_type());
+  else run(std::integral_constant<int, 1>(), std::false_type());
 }
-uint64_t backward_groups(uint64_t rows, uint64_t columns) {
-  return std::min<uint64_t>(rows, group_limit(columns));
+
+// Blocks that the backward's weight gradient is summed over (rows of `partial`, which stays within
+// 8 MB up to 8192 columns).
+uint64_t block_limit(uint64_t columns) {
+  return std::min<uint64_t>(2048, std::max<uint64_t>(256, (1ull << 21) / columns));
 }
 
 oxh_status check_rows(const char *what, int dtype, uint64_t rows, uint64_t columns) {
@@ -301,64 +341,51 @@ bool aligned_to(const void *p, uint64_t bytes) {
 
 template <typename T>
 oxh_status forward(hipStream_t stream, const Forward<T> &a) {
-  constexpr int kPack = 16 / sizeof(T);
-  const bool packed = a.columns % kPack == 0 && oxh::aligned16(a.x) && oxh::aligned16(a.y) &&
-                      (a.r == nullptr || oxh::aligned16(a.r)) &&
-                      (a.s == nullptr || oxh::aligned16(a.s)) && oxh::aligned16(a.w);
-  const uint64_t limit = packed ? row_limit<kPack>() : row_limit<1>();
-  if (a.columns > limit) {
+  if (a.columns > forward_limit<T>()) {
     oxh::launch(rms_norm_forward_long_kernel<T>, dim3(static_cast<uint32_t>(a.rows)),
                 dim3(1024), 0, stream, a);
     return oxh::launched("rms_norm_forward");
   }
-  auto start = [&](auto pack) {
+  with_pack<T>(a.columns, [&](auto pack, auto ragged) {
     constexpr int N = decltype(pack)::value;
-    with_shape<N>(a.columns, [&](auto shape) {
+    with_shape<N, forward_limit<T>()>(a.columns, [&](auto shape) {
       using S = decltype(shape);
       constexpr int threads = S::lanes < 256 ? 256 : S::lanes, per = threads / S::lanes;
-      oxh::launch(rms_norm_forward_kernel<T, N, S::lanes, S::chunks>,
+      oxh::launch(rms_norm_forward_kernel<T, N, S::lanes, S::chunks, decltype(ragged)::value>,
                   dim3(static_cast<uint32_t>((a.rows + per - 1) / per)), dim3(threads), 0,
                   stream, a);
     });
-  };
-  if (packed) start(std::integral_constant<int, kPack>());
-  else start(std::integral_constant<int, 1>());
+  });
   return oxh::launched("rms_norm_forward");
 }
 
 template <typename T>
 oxh_status backward(hipStream_t stream, const Backward<T> &a, float *weight_gradient) {
-  constexpr int kPack = 16 / sizeof(T);
-  const bool packed = a.columns % kPack == 0 && oxh::aligned16(a.g) && oxh::aligned16(a.s) &&
-                      oxh::aligned16(a.dx) && (a.sg == nullptr || oxh::aligned16(a.sg)) &&
-                      oxh::aligned16(a.w);
-  const uint64_t limit = packed ? row_limit<kPack>() : row_limit<1>();
-  uint64_t groups = backward_groups(a.rows, a.columns);
-  if (a.columns > limit) {
-    oxh::launch(rms_norm_backward_long_kernel<T>, dim3(static_cast<uint32_t>(groups)),
+  uint64_t blocks = std::min<uint64_t>(a.rows, block_limit(a.columns));
+  if (a.columns > backward_limit(a.columns % (16 / sizeof(T)) != 0)) {
+    oxh::launch(rms_norm_backward_long_kernel<T>, dim3(static_cast<uint32_t>(blocks)),
                 dim3(1024), 0, stream, a);
   } else {
-    auto start = [&](auto pack) {
+    with_pack<T>(a.columns, [&](auto pack, auto ragged) {
       constexpr int N = decltype(pack)::value;
-      with_shape<N>(a.columns, [&](auto shape) {
+      with_shape<N, backward_limit(decltype(ragged)::value)>(a.columns, [&](auto shape) {
         using S = decltype(shape);
         constexpr int threads = S::lanes < 256 ? 256 : S::lanes, per = threads / S::lanes;
-        // whole blocks of groups: the last block's spare groups have no rows and add zeros
-        const uint64_t blocks = std::max<uint64_t>(1, std::min<uint64_t>(
-            (a.rows + per - 1) / per, group_limit(a.columns) / per));
-        groups = blocks * per;
-        oxh::launch(rms_norm_backward_kernel<T, N, S::lanes, S::chunks>,
+        // two blocks per compute unit (float32 3584 x 1280: 16.8 us, 20.5 with one, 19.3 with four),
+        // and every group the same number of rows, but for the last ones
+        const uint64_t most = std::min<uint64_t>(block_limit(a.columns), 512),
+                       rounds = (a.rows + most * per - 1) / (most * per);
+        blocks = (a.rows + rounds * per - 1) / (rounds * per);
+        oxh::launch(rms_norm_backward_kernel<T, N, S::lanes, S::chunks, decltype(ragged)::value>,
                     dim3(static_cast<uint32_t>(blocks)), dim3(threads), 0, stream, a);
       });
-    };
-    if (packed) start(std::integral_constant<int, kPack>());
-    else start(std::integral_constant<int, 1>());
+    });
   }
   oxh_status st = oxh::launched("rms_norm_backward");
   if (st != OXH_OK || weight_gradient == nullptr) return st;
   oxh::launch(rms_norm_weight_kernel, dim3((a.columns + 15) / 16), dim3(1024), 0, stream,
               static_cast<const float *>(a.partial), weight_gradient,
-              static_cast<uint32_t>(groups), a.columns);
+              static_cast<uint32_t>(blocks), a.columns);
   return oxh::launched("rms_norm_weight_gradient");
 }
 
@@ -418,8 +445,7 @@ oxh_status oxh_rms_norm_backward_workspace_size(uint64_t rows, uint64_t columns,
   OXH_REQUIRE(bytes != nullptr, OXH_INVALID_SHAPE, "bytes is null");
   oxh_status st = check_rows("rms norm", OXH_F32, rows, columns);
   if (st != OXH_OK) return st;
-  // groups come in whole blocks of 4
-  *bytes = ((backward_groups(rows, columns) + 3) / 4 * 4 * columns * 4 + 255) / 256 * 256;
+  *bytes = (std::min(rows, block_limit(columns)) * columns * 4 + 255) / 256 * 256;
   return oxh::ok();
 }
 

@@ -200,3 +200,36 @@ def test_another_stream_a_graph_and_repeats(module, dev):
         torch.cuda.synchronize()
         for a, b in zip((y, q, dx, dw), want):
             assert torch.equal(a, b)
+
+
+# columns that are no multiple of an access: less than one, one and a value, one short of what a
+# wave, four, and sixteen hold, past the registers; rows that make several turns of every group
+RAGGED = [(3, 2), (5, 5), (9, 9), (4100, 33), (6, 255), (3, 513), (2100, 1283), (700, 2047),
+          (4, 4095), (3, 8191), (2, 12001), (2, 16383), (2, 16385), (2, 32767), (2, 65535)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", RAGGED)
+def test_ragged_rows(module, dev, shape, dtype):
+    """Both directions, the sum over its operand and the gradient over the stream's, and nothing
+    written behind or before an output."""
+    t, rows = TYPES[dtype], shape[0]
+    size = int(np.prod(shape))
+    r, w = make(shape, t, dev, 2), make(shape[-1:], torch.float32, dev, 3) + 1.0
+    x = make(shape, t, dev, 1)
+    s_ref, q_ref, y_ref = forward_ref(x, r, w, 1e-6)
+    around = torch.full((size + 64,), 7.0, dtype=t, device=dev)
+    y = around[32:32 + size].view(shape)
+    q = torch.empty(rows, device=dev)
+    module.rms_norm_forward(x, w, y, q, residual=r, sum=x)
+    within(x, s_ref, np.abs(s_ref), 1, t, "sum")
+    within(q, q_ref, q_ref, 64, torch.float32, "inverse rms")
+    within(y, y_ref, np.abs(y_ref), 64, t, "output")
+    assert (around[:32] == 7).all() and (around[32 + size:] == 7).all()
+    g, sg = make(shape, t, dev, 4), make(shape, t, dev, 5)
+    dx = around[33:33 + size].view(shape)
+    dx.copy_(sg)
+    around[32], dw = 7.0, torch.empty_like(w)
+    module.rms_norm_backward(g, x, w, q, dx, dw, sum_gradient=dx)
+    check_backward(x, g, w, sg, q, dx, dw, t)
+    assert (around[:33] == 7).all() and (around[33 + size:] == 7).all()
