@@ -10,7 +10,6 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <initializer_list>
 #include <string>
 #include <type_traits>
 
@@ -153,9 +152,10 @@ __device__ __forceinline__ Map<V> scan_groups(Map<V> &mine, float *shared) {
 
 struct Place {
   uint32_t row, segment, channel;
-  bool in;  // the thread's channels exist
+  bool in;        // the thread's channels exist
+  uint32_t skip;  // the first ones that are another thread's
 };
-template <int V, int Lanes>
+template <int V, int Lanes, bool Ragged>
 __device__ __forceinline__ Place place_of(uint32_t groups, uint32_t segments, uint32_t channels) {
   const uint32_t group = blockIdx.x % groups, rest = blockIdx.x / groups;
   Place p;
@@ -163,6 +163,12 @@ __device__ __forceinline__ Place place_of(uint32_t groups, uint32_t segments, ui
   p.row = rest / segments;
   p.channel = group * Lanes * V + (threadIdx.x % Lanes) * V;
   p.in = p.channel < channels;
+  p.skip = 0;
+  if (Ragged && p.in) {
+    const oxh::storage::Places at = oxh::storage::places_at<V, Ragged>(p.channel, channels);
+    p.channel = at.start;
+    p.skip = at.skip;
+  }
   return p;
 }
 
@@ -193,18 +199,19 @@ __device__ __forceinline__ void load_state(const float *p, float (&h)[V]) {
   for (int v = 0; v < V; ++v) h[v] = p[v];
 }
 template <int V>
-__device__ __forceinline__ void store_state(float *p, const float (&h)[V]) {
+__device__ __forceinline__ void store_state(float *p, uint32_t skip, const float (&h)[V]) {
 #pragma unroll
-  for (int v = 0; v < V; ++v) p[v] = h[v];
+  for (uint32_t v = 0; v < V; ++v)
+    if (v >= skip) p[v] = h[v];
 }
 
 // Where the time axis is split: segment s's map to entry s + 1 of `parts`, and the first state to
 // entry 0.  Each time group takes a run of the segment's steps of its own.
-template <typename T, int V, int Lanes, int W, int S, bool Back>
+template <typename T, int V, int Lanes, int W, int S, bool Back, bool Ragged>
 __global__ __launch_bounds__(64 * W) void recurrence_parts_kernel(Args<T> a) {
   __shared__ float shared[W * 2 * Lanes * V];
   constexpr uint32_t kGroups = 64 / Lanes * W;
-  const Place p = place_of<V, Lanes>(a.groups, a.segments, a.channels);
+  const Place p = place_of<V, Lanes, Ragged>(a.groups, a.segments, a.channels);
   const Live live = live_of<Back>(a, p.row);
   const uint32_t share = (a.steps + kGroups - 1) / kGroups;
   const uint32_t first = p.segment * a.steps + threadIdx.x / Lanes * share;
@@ -242,13 +249,13 @@ __global__ __launch_bounds__(64 * W) void recurrence_parts_kernel(Args<T> a) {
   if (!p.in || threadIdx.x >= Lanes) return;
   float *entry = a.parts + (static_cast<uint64_t>(p.row) * (a.segments + 1) + p.segment + 1) * 2 *
                                a.channels + p.channel;
-  store_state<V>(entry, all.a);
-  store_state<V>(entry + a.channels, all.b);
+  store_state<V>(entry, p.skip, all.a);
+  store_state<V>(entry + a.channels, p.skip, all.b);
   if (p.segment == 0) {
     float h[V] = {};
     if (a.first != nullptr)
       load_state<V>(a.first + static_cast<uint64_t>(p.row) * a.channels + p.channel, h);
-    store_state<V>(entry - a.channels, h);
+    store_state<V>(entry - a.channels, p.skip, h);
   }
 }
 
@@ -257,11 +264,11 @@ __global__ __launch_bounds__(64 * W) void recurrence_parts_kernel(Args<T> a) {
 // thread runs its steps again from the state that reaches them.  The next tile's operands are
 // loaded before the present one's work.
 // Once: what it moves is far more than the caches hold, and bypasses them.
-template <typename T, int V, int Lanes, int W, int S, bool Back, bool Once = false>
+template <typename T, int V, int Lanes, int W, int S, bool Back, bool Ragged, bool Once = false>
 __global__ __launch_bounds__(64 * W) void recurrence_kernel(Args<T> a) {
   __shared__ float shared[2][W * 2 * Lanes * V];
   constexpr uint32_t kGroups = 64 / Lanes * W, kTile = kGroups * S;
-  Place p = place_of<V, Lanes>(a.groups, a.segments, a.channels);
+  Place p = place_of<V, Lanes, Ragged>(a.groups, a.segments, a.channels);
   const Live live = live_of<Back>(a, p.row);
   const uint32_t group = threadIdx.x / Lanes;
   const uint64_t row = row_start<V>(a, p);
@@ -387,14 +394,15 @@ __global__ __launch_bounds__(64 * W) void recurrence_kernel(Args<T> a) {
           y[v] = on ? x[v] : 0.0f;
         }
       }
-      oxh::storage::store<T, V, Once>(a.out + at, y);
-      if constexpr (Back) oxh::storage::store<T, V, Once>(a.dg + at, z);
+      const oxh::storage::Places here{0, p.skip};
+      oxh::storage::store_places<T, V, Ragged, Once>(a.out + at, here, y);
+      if constexpr (Back) oxh::storage::store_places<T, V, Ragged, Once>(a.dg + at, here, z);
     }
   }
   // every thread has read the first state, which may lie where the last one goes
   __syncthreads();
   if (a.last != nullptr && p.in && p.segment + 1 == a.segments && group == 0)
-    store_state<V>(a.last + state, h);
+    store_state<V>(a.last + state, p.skip, h);
 }
 
 std::string message(const char *what, const char *problem) {
@@ -451,29 +459,48 @@ struct Plan {
 };
 
 constexpr int kBriefTime = 16;
-constexpr int kWaves = 4;
-// steps per thread and tile
-constexpr int steps_of(int values, bool back) { return (values == 1 ? 16 : 8) / (back ? 2 : 1); }
+// Waves per block, and steps per thread and tile.  Eight waves of four steps (backward: two) hold
+// the bytes in flight of four waves of eight in half the registers each, and more of them hide more
+// (forward 8 x 2048 x 2048 float32 87 us, 94 with four; 10 x 356 x 855 12.6 and 15.7; backward 8 x
+// 2048 x 2048 167 and 171; 1 x 131072 x 512 bfloat16 237 and 244).
+constexpr int kWaves = 8;
+constexpr int steps_of(int values, bool back) { return (values == 1 ? 8 : 4) / (back ? 2 : 1); }
 
-
-Plan plan_of(uint64_t batch, uint64_t time, uint64_t channels, bool packed, bool back) {
+// A tile takes about as long as 9 MB moved (3 us), a second launch as two tiles, and it reads half
+// the operands again.  So the time axis is taken whole where blocks across rows and channels give
+// every compute unit one, or where its tiles are at most two and one more for each 3 MB of a tensor
+// (8 x 2048 x 512 float32, 8 tiles: 24.6 us whole, 28.7 split; 2 x 512 x 1024, 2 tiles: 7.6 and 12;
+// 5 x 1537 x 333 bfloat16, 7 tiles: 23.7 and 14.2; 1 x 4096 x 2048 float32, 16 tiles: 41 and 30);
+// there 32 channels per block where 64 leave more than half of the units without (8 x 2048 x 512,
+// 64 blocks: 24.6 and 39; 10 x 356 x 855, 140 blocks: 15.4 and 12.6).  Otherwise it is split for two
+// blocks per unit, a tile at least per segment (3 x 700 x 130: 10.5 us with one, 16.3 with two).
+Plan plan_of(uint64_t batch, uint64_t time, uint64_t channels, uint64_t element, bool back) {
   Plan p;
-  p.values = packed ? 4 : 1;
+  p.values = channels < 4 ? 1 : 4;
   p.brief = time <= kBriefTime;
-  p.lanes = p.brief ? 64 : packed ? (channels <= 32 ? 8 : 16) : (channels <= 32 ? 32 : 64);
-  p.groups = static_cast<uint32_t>((channels + p.lanes * p.values - 1) / (p.lanes * p.values));
+  auto across = [&](int lanes) {
+    p.lanes = lanes;
+    p.groups = static_cast<uint32_t>((channels + lanes * p.values - 1) / (lanes * p.values));
+    return batch * p.groups;
+  };
+  auto tiles = [&](uint64_t &tile) {
+    tile = 64 / p.lanes * kWaves * steps_of(p.values, back);
+    return (time + tile - 1) / tile;
+  };
   p.segments = 1;
   p.steps = static_cast<uint32_t>(time);
-  if (p.brief) return p;
-  const uint64_t tile = 64 / p.lanes * kWaves * steps_of(p.values, back);
-  const uint64_t blocks = batch * p.groups, target = 512;
-  if (blocks >= oxh::kComputeUnits) return p;
-  const uint64_t tiles = (time + tile - 1) / tile;
-  const uint64_t wanted = std::min((target + blocks - 1) / blocks, (tiles + 1) / 2);
-  if (wanted < 2) return p;
-  const uint64_t per = (tiles + wanted - 1) / wanted;
+  const int lanes = p.brief ? 64 : p.values == 1 ? 32 : channels <= 32 ? 8 : 16;
+  const uint64_t blocks = across(lanes), units = oxh::kComputeUnits;
+  if (p.brief || blocks >= units) return p;
+  uint64_t tile;
+  if (p.values == 4 && blocks * 2 < units) across(8);
+  if (tiles(tile) <= 2 + batch * time * channels * element / (3u << 20)) return p;
+  across(lanes);
+  const uint64_t all = tiles(tile);
+  const uint64_t wanted = std::min((2 * units + blocks - 1) / blocks, all);
+  const uint64_t per = (all + wanted - 1) / wanted;
   p.steps = static_cast<uint32_t>(per * tile);
-  p.segments = static_cast<uint32_t>((tiles + per - 1) / per);
+  p.segments = static_cast<uint32_t>((all + per - 1) / per);
   return p;
 }
 
@@ -481,12 +508,12 @@ uint64_t parts_bytes(const Plan &p, uint64_t batch, uint64_t channels) {
   return p.segments == 1 ? 0 : batch * (p.segments + 1) * 2 * channels * 4;
 }
 
-template <typename T, int V, int Lanes, bool Back>
+template <typename T, int V, int Lanes, bool Back, bool Ragged>
 oxh_status run_split(hipStream_t stream, uint64_t batch, Args<T> a, const char *what) {
   constexpr int S = steps_of(V, Back);
   const uint64_t blocks = batch * a.groups * a.segments;
   if (a.segments > 1) {
-    oxh::launch(recurrence_parts_kernel<T, V, Lanes, kWaves, S, Back>,
+    oxh::launch(recurrence_parts_kernel<T, V, Lanes, kWaves, S, Back, Ragged>,
                 dim3(static_cast<uint32_t>(blocks)), dim3(64 * kWaves), 0, stream, a);
     oxh_status st = oxh::launched(what);
     if (st != OXH_OK) return st;
@@ -498,43 +525,43 @@ oxh_status run_split(hipStream_t stream, uint64_t batch, Args<T> a, const char *
   const uint64_t moved = batch * a.time * a.channels * sizeof(T) * (Back ? 6 : 3);
   if constexpr (V == 4 && Lanes == 16) {
     if (moved > kCached) {
-      oxh::launch(recurrence_kernel<T, V, Lanes, kWaves, S, Back, true>,
+      oxh::launch(recurrence_kernel<T, V, Lanes, kWaves, S, Back, Ragged, true>,
                   dim3(static_cast<uint32_t>(blocks)), dim3(64 * kWaves), 0, stream, a);
       return oxh::launched(what);
     }
   }
-  oxh::launch(recurrence_kernel<T, V, Lanes, kWaves, S, Back>,
+  oxh::launch(recurrence_kernel<T, V, Lanes, kWaves, S, Back, Ragged>,
               dim3(static_cast<uint32_t>(blocks)), dim3(64 * kWaves), 0, stream, a);
   return oxh::launched(what);
 }
 
+template <typename T, bool Back, int V, bool Ragged>
+oxh_status run_plan(hipStream_t stream, uint64_t batch, const Args<T> &a, const Plan &p,
+                    const char *what) {
+  if (p.brief) {
+    const dim3 grid(static_cast<uint32_t>(batch * p.groups));
+    oxh::launch(recurrence_kernel<T, V, 64, 1, 4, Back, Ragged>, grid, dim3(64), 0, stream, a);
+    return oxh::launched(what);
+  }
+  if constexpr (V == 1) {
+    return run_split<T, 1, 32, Back, Ragged>(stream, batch, a, what);
+  } else {
+    return p.lanes == 8 ? run_split<T, 4, 8, Back, Ragged>(stream, batch, a, what)
+                        : run_split<T, 4, 16, Back, Ragged>(stream, batch, a, what);
+  }
+}
+
 template <typename T, bool Back>
-oxh_status run(hipStream_t stream, uint64_t batch, Args<T> a, bool packed, const char *what) {
-  const Plan p = plan_of(batch, a.time, a.channels, packed, Back);
+oxh_status run(hipStream_t stream, uint64_t batch, Args<T> a, const char *what) {
+  const Plan p = plan_of(batch, a.time, a.channels, sizeof(T), Back);
   a.groups = p.groups;
   a.segments = p.segments;
   a.steps = p.steps;
-  const uint64_t blocks = batch * p.groups * p.segments;
-  OXH_REQUIRE(blocks < (1ull << 31), OXH_INVALID_SHAPE, std::string(what) + ": too many rows");
-  if (p.brief) {
-    const dim3 grid(static_cast<uint32_t>(blocks));
-    if (packed) oxh::launch(recurrence_kernel<T, 4, 64, 1, 4, Back>, grid, dim3(64), 0, stream, a);
-    else oxh::launch(recurrence_kernel<T, 1, 64, 1, 4, Back>, grid, dim3(64), 0, stream, a);
-    return oxh::launched(what);
-  }
-  if (packed)
-    return p.lanes == 8 ? run_split<T, 4, 8, Back>(stream, batch, a, what)
-                        : run_split<T, 4, 16, Back>(stream, batch, a, what);
-  return p.lanes == 32 ? run_split<T, 1, 32, Back>(stream, batch, a, what)
-                       : run_split<T, 1, 64, Back>(stream, batch, a, what);
-}
-
-// Whether four channels can move as one access.
-bool packs(uint64_t channels, uint64_t element, std::initializer_list<const void *> pointers) {
-  if (channels % 4 != 0) return false;
-  for (const void *p : pointers)
-    if (!aligned_to(p, 4 * element)) return false;
-  return true;
+  OXH_REQUIRE(batch * p.groups * p.segments < (1ull << 31), OXH_INVALID_SHAPE,
+              std::string(what) + ": too many rows");
+  if (p.values == 1) return run_plan<T, Back, 1, false>(stream, batch, a, p, what);
+  return a.channels % 4 == 0 ? run_plan<T, Back, 4, false>(stream, batch, a, p, what)
+                             : run_plan<T, Back, 4, true>(stream, batch, a, p, what);
 }
 
 template <typename T>
@@ -551,8 +578,7 @@ oxh_status forward(hipStream_t stream, uint64_t batch, const void *input, const 
   a.parts = static_cast<float *>(workspace);
   a.time = time;
   a.channels = channels;
-  return run<T, false>(stream, batch, a, packs(channels, sizeof(T), {input, gate, output}),
-                       "gated_recurrence_forward");
+  return run<T, false>(stream, batch, a, "gated_recurrence_forward");
 }
 
 template <typename T>
@@ -575,10 +601,7 @@ oxh_status backward(hipStream_t stream, uint64_t batch, const void *gradient, co
   a.parts = static_cast<float *>(workspace);
   a.time = time;
   a.channels = channels;
-  return run<T, true>(
-      stream, batch, a,
-      packs(channels, sizeof(T), {gradient, input, gate, output, input_gradient, gate_gradient}),
-      "gated_recurrence_backward");
+  return run<T, true>(stream, batch, a, "gated_recurrence_backward");
 }
 
 }  // namespace
@@ -592,9 +615,9 @@ oxh_status oxh_gated_recurrence_workspace_size(uint64_t batch, uint64_t time, ui
   if (st != OXH_OK) return st;
   *bytes = 0;
   if (batch == 0 || channels == 0) return oxh::ok();
-  for (const bool packed : {false, true})
+  for (const uint64_t element : {2, 4})
     for (const bool back : {false, true})
-      *bytes = std::max(*bytes, parts_bytes(plan_of(batch, time, channels, packed, back), batch,
+      *bytes = std::max(*bytes, parts_bytes(plan_of(batch, time, channels, element, back), batch,
                                             channels));
   *bytes = (*bytes + 255) / 256 * 256;
   return oxh::ok();

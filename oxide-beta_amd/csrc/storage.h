@@ -85,10 +85,10 @@ __device__ __forceinline__ void store(T *p, const float (&v)[N]) {
 }
 
 // Skipped values are not stored.
-template <typename T, int N, bool Ragged>
+template <typename T, int N, bool Ragged, bool Once = false>
 __device__ __forceinline__ void store_places(T *row, Places at, const float (&v)[N]) {
   if (!Ragged || at.skip == 0) {
-    store<T, N>(row + at.start, v);
+    store<T, N, Once>(row + at.start, v);
   } else {
 #pragma unroll
     for (uint32_t i = 0; i < N; ++i)

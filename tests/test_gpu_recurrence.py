@@ -345,3 +345,35 @@ def test_more_than_the_caches_hold(module, dev):
     out, _, _ = backward_ref(pick(dh), pick(u), pick(g), pick(h), None, None, None)
     within(pick(du), out[0], out[1], t, "input gradient")
     within(pick(dg), out[2], out[3], t, "gate gradient")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(2, 5, 65), (3, 40, 5), (2, 300, 65), (1, 3000, 67), (2, 9, 2051),
+                                   (300, 20, 7), (2, 300, 3)])
+def test_ragged_channels(module, dev, shape, dtype):
+    """Channels that are no multiple of an access, of one in another block among them: the state
+    where it lay, and nothing written before or behind an output."""
+    t, size = TYPES[dtype], int(np.prod(shape))
+    u, g = make(shape, t, dev, 1), gates(shape, t, dev, 2)
+    first = make((shape[0], shape[2]), torch.float32, dev, 3)
+    lengths = lengths_of(shape[0], shape[1], dev)
+    ref, err, ref_final, err_final = forward_ref(u, g, first, lengths)
+    around = torch.full((size + 40,), 7.0, dtype=t, device=dev)
+    more = torch.full((size + 40,), 7.0, dtype=t, device=dev)
+    h, state = around[21:21 + size].view(shape), first.clone()
+    module.gated_recurrence_forward(u, g, h, initial_state=state, final_state=state,
+                                    lengths=lengths)
+    within(h, ref, err, t, "output")
+    within(state, ref_final, err_final, torch.float32, "state")
+    dh, dfinal = make(shape, t, dev, 4), make((shape[0], shape[2]), torch.float32, dev, 5)
+    h = h.clone()
+    du, dg, ds = around[21:21 + size].view(shape), more[21:21 + size].view(shape), dfinal.clone()
+    module.gated_recurrence_backward(dh, u, g, h, du, dg, initial_state=first,
+                                     final_state_gradient=ds, initial_state_gradient=ds,
+                                     lengths=lengths)
+    (rdu, edu, rdg, edg), rds, eds = backward_ref(dh, u, g, h, first, dfinal, lengths)
+    within(du, rdu, edu, t, "input gradient")
+    within(dg, rdg, edg, t, "gate gradient")
+    within(ds, rds, eds, torch.float32, "state gradient")
+    for b in (around, more):
+        assert (b[:21] == 7).all() and (b[21 + size:] == 7).all()
