@@ -36,8 +36,13 @@ __device__ __forceinline__ Gate gate_of(float g) {
 // Both directions run h -> keep h + add over their steps in the order taken (backwards in time
 // for the gradients, where h is a_{t+1} l_{t+1}, the gradient that reaches step t from later ones,
 // and add = a_t dh_t).
+struct Layout {
+  uint32_t time, channels, groups;  // groups: blocks across the channels
+  uint32_t segments, steps;         // steps per segment
+  bool lines;                       // every group's channels of a step are whole lines of memory
+};
 template <typename T>
-struct Args {
+struct Args : Layout {
   const T *u, *g, *h, *dh;  // forward: u, g
   T *out, *dg;              // h, or du and dg
   const float *first;       // the state before the first step taken, or null
@@ -45,8 +50,6 @@ struct Args {
   float *last;              // the one after the last, or null
   const int32_t *lengths;
   float *parts;  // per batch row: entry 0 the first state, entry s + 1 segment s's (keep, add)
-  uint32_t time, channels, groups;  // groups: blocks across the channels
-  uint32_t segments, steps;         // steps per segment
 };
 
 __device__ __forceinline__ uint32_t length_of(const int32_t *lengths, uint32_t row,
@@ -156,11 +159,12 @@ struct Place {
   uint32_t skip;  // the first ones that are another thread's
 };
 template <int V, int Lanes, bool Ragged>
-__device__ __forceinline__ Place place_of(uint32_t groups, uint32_t segments, uint32_t channels) {
-  const uint32_t group = blockIdx.x % groups, rest = blockIdx.x / groups;
+__device__ __forceinline__ Place place_of(const Layout &l) {
+  const uint32_t id = l.lines ? blockIdx.x : oxh::xcd_contiguous(blockIdx.x, gridDim.x);
+  const uint32_t group = id % l.groups, rest = id / l.groups, channels = l.channels;
   Place p;
-  p.segment = rest % segments;
-  p.row = rest / segments;
+  p.segment = rest % l.segments;
+  p.row = rest / l.segments;
   p.channel = group * Lanes * V + (threadIdx.x % Lanes) * V;
   p.in = p.channel < channels;
   p.skip = 0;
@@ -211,7 +215,7 @@ template <typename T, int V, int Lanes, int W, int S, bool Back, bool Ragged>
 __global__ __launch_bounds__(64 * W) void recurrence_parts_kernel(Args<T> a) {
   __shared__ float shared[W * 2 * Lanes * V];
   constexpr uint32_t kGroups = 64 / Lanes * W;
-  const Place p = place_of<V, Lanes, Ragged>(a.groups, a.segments, a.channels);
+  const Place p = place_of<V, Lanes, Ragged>(a);
   const Live live = live_of<Back>(a, p.row);
   const uint32_t share = (a.steps + kGroups - 1) / kGroups;
   const uint32_t first = p.segment * a.steps + threadIdx.x / Lanes * share;
@@ -268,7 +272,7 @@ template <typename T, int V, int Lanes, int W, int S, bool Back, bool Ragged, bo
 __global__ __launch_bounds__(64 * W) void recurrence_kernel(Args<T> a) {
   __shared__ float shared[2][W * 2 * Lanes * V];
   constexpr uint32_t kGroups = 64 / Lanes * W, kTile = kGroups * S;
-  Place p = place_of<V, Lanes, Ragged>(a.groups, a.segments, a.channels);
+  Place p = place_of<V, Lanes, Ragged>(a);
   const Live live = live_of<Back>(a, p.row);
   const uint32_t group = threadIdx.x / Lanes;
   const uint64_t row = row_start<V>(a, p);
@@ -518,13 +522,14 @@ oxh_status run_split(hipStream_t stream, uint64_t batch, Args<T> a, const char *
     oxh_status st = oxh::launched(what);
     if (st != OXH_OK) return st;
   }
-  // What passes beyond the 256 MB last-level cache is not kept there (backward 8 x 2048 x 2048
-  // float32, 805 MB: 160 us, 172 with the default policy; forward 1 x 131072 x 512 bfloat16, 403
-  // MB: 128 and 152); smaller calls leave their results to the next one.
+  // What passes beyond the 256 MB last-level cache is not kept there, where blocks write whole lines
+  // (backward 8 x 2048 x 2048 float32, 805 MB: 160 us, 172 with the default policy; forward 1 x
+  // 131072 x 512 bfloat16, 403 MB: 128 and 152; off lines it costs: backward 8 x 2048 x 2048
+  // bfloat16 161 us, 118 with the default); smaller calls leave their results to the next one.
   constexpr uint64_t kCached = 256ull << 20;
   const uint64_t moved = batch * a.time * a.channels * sizeof(T) * (Back ? 6 : 3);
   if constexpr (V == 4 && Lanes == 16) {
-    if (moved > kCached) {
+    if (moved > kCached && a.lines) {
       oxh::launch(recurrence_kernel<T, V, Lanes, kWaves, S, Back, Ragged, true>,
                   dim3(static_cast<uint32_t>(blocks)), dim3(64 * kWaves), 0, stream, a);
       return oxh::launched(what);
@@ -557,6 +562,16 @@ oxh_status run(hipStream_t stream, uint64_t batch, Args<T> a, const char *what) 
   a.groups = p.groups;
   a.segments = p.segments;
   a.steps = p.steps;
+  // Lines that two groups share stay in one L2 if neighbouring blocks are on one XCD (forward 8 x
+  // 2048 x 2048 bfloat16 16 bytes off a line: 42 us, 60 without; backward 1 x 5824 x 955 24 and 34); those of their own are better
+  // spread over the XCDs (forward 16 x 1024 x 4096 bfloat16: 83 us, 104 together).
+  constexpr uint64_t kLine = 128;
+  a.lines = a.channels * sizeof(T) % kLine == 0 &&
+            p.lanes * p.values * sizeof(T) % kLine == 0;
+  for (const void *x : {static_cast<const void *>(a.u), static_cast<const void *>(a.g),
+                        static_cast<const void *>(a.h), static_cast<const void *>(a.dh),
+                        static_cast<const void *>(a.out), static_cast<const void *>(a.dg)})
+    a.lines = a.lines && aligned_to(x, kLine);
   OXH_REQUIRE(batch * p.groups * p.segments < (1ull << 31), OXH_INVALID_SHAPE,
               std::string(what) + ": too many rows");
   if (p.values == 1) return run_plan<T, Back, 1, false>(stream, batch, a, p, what);
