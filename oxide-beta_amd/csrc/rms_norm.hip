@@ -158,6 +158,9 @@ __global__ __launch_bounds__(Lanes < 256 ? 256 : Lanes) void rms_norm_backward_k
     const uint64_t base = row * a.columns;
     const float q = a.q[row];
     float unit[Chunks][N], d[Chunks][N];
+    // the stream's gradient, loaded with the rest where the registers allow it
+    constexpr bool kEarly = Chunks * N <= 32 && Lanes < 1024;
+    typename oxh::storage::Pack<T, N>::type stream[kEarly ? Chunks : 1];
     float dot = 0.0f;
 #pragma unroll
     for (int c = 0; c < Chunks; ++c) {
@@ -168,6 +171,8 @@ __global__ __launch_bounds__(Lanes < 256 ? 256 : Lanes) void rms_norm_backward_k
       const Places here = places_at<N, Ragged>(at, a.columns);
       load_places<T, N, Ragged>(a.s + base, here, unit[c]);
       load_places<T, N, Ragged>(a.g + base, here, d[c]);
+      if (kEarly && a.sg != nullptr)
+        stream[kEarly ? c : 0] = oxh::storage::raw<T, N>(a.sg + base + here.start);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         unit[c][i] *= q;
@@ -188,9 +193,10 @@ __global__ __launch_bounds__(Lanes < 256 ? 256 : Lanes) void rms_norm_backward_k
       for (int i = 0; i < N; ++i) out[i] = q * (d[c][i] - unit[c][i] * mean);
       if (a.sg != nullptr) {
         float sg[N];
-        load_places<T, N, Ragged>(a.sg + base, here, sg);
+        oxh::storage::widen_all<T, N>(kEarly ? stream[kEarly ? c : 0]
+                                             : oxh::storage::raw<T, N>(a.sg + base + here.start), sg);
 #pragma unroll
-        for (int i = 0; i < N; ++i) out[i] += sg[i];
+        for (int i = 0; i < N; ++i) out[i] += sg[i];  // skipped ones are not stored
       }
       store_places<T, N, Ragged>(a.dx + base, here, out);
     }
@@ -295,16 +301,19 @@ struct Shape {
 template <int N, uint64_t Limit, typename Run>
 void with_shape(uint64_t columns, Run run) {
   const uint64_t packs = (columns + N - 1) / N;
-  if constexpr (N == 1) return run(Shape<64, 1>());  // rows of fewer values than an access
-  if (packs <= 64) return run(Shape<64, 1>());
-  if (packs <= 128) return run(Shape<64, 2>());
-  if (packs <= 256) return run(Shape<64, 4>());
-  if (packs <= 512) return run(std::conditional_t<N <= 4, Shape<64, 8>, Shape<256, 2>>());
-  if (packs <= 1024) return run(Shape<256, 4>());
-  if (Limit / N <= 2048 || packs <= 2048) return run(Shape<256, 8>());
-  if constexpr (Limit / N > 2048)
-    if (Limit / N <= 4096 || packs <= 4096) return run(Shape<1024, 4>());
-  if constexpr (Limit / N > 4096) run(Shape<1024, 8>());
+  if constexpr (N == 1) {  // rows of fewer values than an access
+    run(Shape<64, 1>());
+  } else {
+    if (packs <= 64) return run(Shape<64, 1>());
+    if (packs <= 128) return run(Shape<64, 2>());
+    if (packs <= 256) return run(Shape<64, 4>());
+    if (packs <= 512) return run(std::conditional_t<N <= 4, Shape<64, 8>, Shape<256, 2>>());
+    if (packs <= 1024) return run(Shape<256, 4>());
+    if (Limit / N <= 2048 || packs <= 2048) return run(Shape<256, 8>());
+    if constexpr (Limit / N > 2048)
+      if (Limit / N <= 4096 || packs <= 4096) return run(Shape<1024, 4>());
+    if constexpr (Limit / N > 4096) run(Shape<1024, 8>());
+  }
 }
 
 // Calls run(pack, ragged) for rows of these columns: 16 bytes per access, or one value where a row

@@ -36,14 +36,21 @@ struct Pack<T, 1> {
 };
 
 template <typename T, int N>
-__device__ __forceinline__ void load(const T *p, float (&v)[N]) {
+__device__ __forceinline__ typename Pack<T, N>::type raw(const T *p) {
+  return *reinterpret_cast<const typename Pack<T, N>::type *>(p);
+}
+template <typename T, int N>
+__device__ __forceinline__ void widen_all(const typename Pack<T, N>::type &x, float (&v)[N]) {
   if constexpr (N == 1) {
-    v[0] = widen(*p);
+    v[0] = widen(x);
   } else {
-    const typename Pack<T, N>::type x = *reinterpret_cast<const typename Pack<T, N>::type *>(p);
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = widen(x[i]);
   }
+}
+template <typename T, int N>
+__device__ __forceinline__ void load(const T *p, float (&v)[N]) {
+  widen_all<T, N>(raw<T, N>(p), v);
 }
 
 // The places of a row that N consecutive ones from `at` (< columns) stand for, columns >= N.  Ragged
