@@ -898,8 +898,10 @@ struct Item {
 uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
 
 // Whether one block steps the whole matrix: the rows of the shared memory that hold X', and at most
-// Blocks column blocks per wave.
-constexpr int whole_blocks(int ps) { return ps == 32 ? 6 : ps == 64 ? 3 : 2; }
+// this many column blocks per wave (one matrix of 96 x 192 43 us, 72 in launches; of 96 x 384 83 and
+// 75, but 16 of them 84 and 143; of 128 x 192 60 and 73; of 128 x 256, whose two column blocks spill,
+// 180 and 74, 16 of them 181 and 140).
+constexpr int whole_blocks(int ps) { return ps == 32 ? 6 : ps == 64 ? 3 : ps == 96 ? 2 : 1; }
 bool whole(const Item &it) {
   const uint64_t s = std::min(it.rows, it.columns), n = std::max(it.rows, it.columns);
   if (s > 128) return false;
@@ -1087,7 +1089,6 @@ oxh_status run_all(hipStream_t stream, const Parted &items, const Hyper &h, uint
     if (st == OXH_OK) st = run_whole<96, 1>(stream, small, g, rounds);
     if (st == OXH_OK) st = run_whole<96, whole_blocks(96)>(stream, small, g, rounds);
     if (st == OXH_OK) st = run_whole<128, 1>(stream, small, g, rounds);
-    if (st == OXH_OK) st = run_whole<128, whole_blocks(128)>(stream, small, g, rounds);
   }
   for (size_t at = 0; at < large.size() && st == OXH_OK; at += kGroup) {
     const size_t count = std::min<size_t>(kGroup, large.size() - at);
