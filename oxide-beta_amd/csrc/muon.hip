@@ -2,7 +2,8 @@
 // moves each weight matrix by its orthogonalised momentum.
 //
 //   M = mu M + G;  V = G + mu M (Nesterov) or M;  X = V / (|V|_F + epsilon)
-//   rounds times:  A = X X';  B = b A + c A A;  X = a X + B X,   (a, b, c) = (3.4445, -4.775, 2.0315)
+//   rounds times:  A = X X';  B = b A + c A A;  X = a X + B X
+//   (a, b, c) = (3.4445, -4.775, 2.0315)
 //   W = W - lr (wd W + sqrt(max(1, rows / columns)) X)
 //
 // with X transposed where rows > columns, so A is the smaller Gram matrix.  Every singular value s
@@ -21,6 +22,13 @@
 // of rank 125 is 9.5e-6 of its norm off, with a float32 copy beside the halves 8.6e-6, and the
 // copies made B X of 12 x 512 x 2048 move 250 MB in place of 100.  B + a I as the factor would
 // save the addition, but then a X has the error of a factor's halves: 3.0e-5.
+//
+// Bound.  Three matrix instructions for each of the plain product's, half of A and of A A: 5 (s^2 n
+// + s^3 + 2 s^2 n) multiply-adds for X of s x n.  Large matrices come near the matrix cores' rate:
+// 4096 x 4096 in 4.1 ms, 335 TFLOP/s or 1005 of float16 (a library's largest float16 products reach
+// 1092 here); 12 x 512 x 2048 in 612 us (three launches a round, which leave the cores a part of
+// the time), and 1000 x 1280 in 225 us, where each of 17 launches takes 9 to 18 us: 136 tiles on
+// 256 compute units, each a chain of loads.  Matrices that fit one compute unit take none of it.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -34,7 +42,6 @@
 namespace {
 
 typedef _Float16 f16;
-typedef f16 f16x4 __attribute__((ext_vector_type(4)));
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -307,11 +314,11 @@ __device__ __forceinline__ void column_of(const f16 *line, uint32_t lane, f32x4 
       for (int o = 0; o < 2; ++o) {
         // hi + lo has at most 23 bits
         const uint32_t hw = h[o], lw = l[o];
-        value[2 * o + e][2 * k] = static_cast<float>(__builtin_bit_cast(f16, static_cast<uint16_t>(hw))) +
-                                  static_cast<float>(__builtin_bit_cast(f16, static_cast<uint16_t>(lw)));
-        value[2 * o + e][2 * k + 1] =
-            static_cast<float>(__builtin_bit_cast(f16, static_cast<uint16_t>(hw >> 16))) +
-            static_cast<float>(__builtin_bit_cast(f16, static_cast<uint16_t>(lw >> 16)));
+        auto half = [](uint32_t word) {
+          return static_cast<float>(__builtin_bit_cast(f16, static_cast<uint16_t>(word)));
+        };
+        value[2 * o + e][2 * k] = half(hw) + half(lw);
+        value[2 * o + e][2 * k + 1] = half(hw >> 16) + half(lw >> 16);
       }
     }
 }
@@ -324,8 +331,9 @@ template <Step S, class Sh>
 __global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int odd) {
   constexpr int kTile = Sh::tile, TM = Sh::TM, TN = Sh::TN, K = Sh::K;
   // per operand row and K block: 32 summed values, 8 pieces of 16 bytes (hi 0..3, lo 4..7), each
-  // at its place exclusive-or bits 1 to 3 of the row: the 16 rows that one pass of a fragment's reads takes lie
-  // in different banks (with bits 0 to 2, two and two share them: 1.05 times the time)
+  // at its place exclusive-or bits 1 to 3 of the row: the 16 rows that one pass of a fragment's
+  // reads takes lie in different banks (with bits 0 to 2, two and two share them: 1.05 times the
+  // time)
   constexpr int kStage = kTile * 128 * K;
   __shared__ __attribute__((aligned(16))) char stage[2 * 2 * kStage];  // [turn][a, b][K][row][128]
   const uint32_t id = oxh::xcd_contiguous(blockIdx.x, gridDim.x);
@@ -336,14 +344,15 @@ __global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int 
   const uint32_t ti = t.row, tj = t.column;
   const uint32_t k_total = S == Step::Gram ? m.pl : m.ps;
   const f16 *pa, *pb;
-  f16 *gs = reinterpret_cast<f16 *>(m.scratch + l.gs), *bs = reinterpret_cast<f16 *>(m.scratch + l.bs);
+  f16 *gs = reinterpret_cast<f16 *>(m.scratch + l.gs);
+  f16 *bs = reinterpret_cast<f16 *>(m.scratch + l.bs);
   f16 *from = reinterpret_cast<f16 *>(m.scratch + (odd ? l.xt1 : l.xt0));
   f16 *to = reinterpret_cast<f16 *>(m.scratch + (odd ? l.xt0 : l.xt1));
   if constexpr (S == Step::Gram) pa = pb = from;
   else if constexpr (S == Step::Poly) pa = pb = gs;
   else pa = bs, pb = from;
   // of the operands' rows ti kTile .., or (Gram) columns
-  const uint64_t tile_bytes = S == Step::Gram ? kTile * 4 : static_cast<uint64_t>(kTile) * k_total * 4;
+  const uint64_t tile_bytes = kTile * 4 * (S == Step::Gram ? uint64_t{1} : k_total);
   const char *sa = reinterpret_cast<const char *>(pa) + ti * tile_bytes;
   const char *sb = reinterpret_cast<const char *>(pb) + tj * tile_bytes;
 
@@ -351,16 +360,16 @@ __global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int 
   const uint32_t group = wave / (Sh::WM * Sh::WN), place = wave % (Sh::WM * Sh::WN);
   const uint32_t wi = place / Sh::WN, wj = place % Sh::WN;
   // Gram: lines of 256 bytes, which are 64 columns of a row, or 32 of two rows where a tile has no
-  // more.  A line's 32-byte pieces lie at their places exclusive-or a number of the line (`turn_of`),
-  // so that the pieces of four rows that 32 lanes read together, or of eight rows, lie in different
-  // banks.
+  // more.  A line's 32-byte pieces lie at their places exclusive-or a number of the line
+  // (`turn_of`), so that the pieces of four rows that 32 lanes read together, or of eight rows, lie
+  // in different banks.
   constexpr int kLineRows = kTile == 32 ? 2 : 1, kAcross = kTile >= 64 ? kTile / 64 : 1;
   auto turn_of = [](uint32_t line) {
     return kLineRows == 2 ? (line & 1) << 1 | (line >> 1 & 1) : (line & 3) << 1 | (line >> 2 & 1);
   };
-  // Direct: operands pass from memory to shared memory without a stop in registers.  Each load of a
-  // wave fills 1024 bytes there in the order of its lanes, so a lane loads the piece that belongs at
-  // its place (both ways do).
+  // Direct: operands pass from memory to shared memory without a stop in registers.  Each load of
+  // a wave fills 1024 bytes there in the order of its lanes, so a lane loads the piece that belongs
+  // at its place (both ways do).
   constexpr int kLoads = 2 * K * kTile * 8 / Sh::threads, kRows = Sh::threads / 8;
   static_assert(kLoads % 2 == 0 && (kRows == 64 || (kRows == 128 && kTile == 64 && K == 2)),
                 "passes of rows, or of lines");
@@ -375,8 +384,8 @@ __global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int 
     for (int i = 0; i < kLoads; ++i) {
       const uint32_t pass = i % (kLoads / 2);
       const char *p = i < kLoads / 2 ? sa : sb;
-      // The source is a block of 32 summed values, the same for the wave; past the last one (whose
-      // products are left out) the last is read again
+      // a block of 32 summed values, the same for the wave; past the last one (whose products are
+      // left out) the last is read again
       auto source = [&](uint32_t ahead) {
         return static_cast<uint64_t>(kTail ? min(block + ahead, blocks - 1) : block + ahead) * 128;
       };
@@ -384,17 +393,21 @@ __global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int 
         // passes of lines: for each 32 rows the tile's columns 64 by 64
         const uint32_t line = pass * (kRows / 2) + line0, lines = line / 32;
         const uint32_t row = line % 32 * kLineRows + piece0 / (16 / kLineRows);
-        p += source((pass * (kRows / 2) + wave * 4) / 32 / kAcross * kLineRows + wave * 4 % 32 * kLineRows / 32) * m.ps;
+        p += source((pass * (kRows / 2) + wave * 4) / 32 / kAcross * kLineRows +
+                    wave * 4 % 32 * kLineRows / 32) * m.ps;
         p += row % 32 * m.ps * 4 + lines % kAcross * 256 + piece0 % (16 / kLineRows) * 16;
       } else {
-        const uint32_t row = kTile % kRows == 0 ? pass * kRows % kTile + r0 : (pass * kRows + r0) % kTile;
+        const uint32_t row = kTile % kRows == 0 ? pass * kRows % kTile + r0
+                                                : (pass * kRows + r0) % kTile;
         p += source((pass * kRows + wave * 8) / kTile);
         p += row * k_total * 4 + c0 * 16;
       }
       if constexpr (Sh::Direct) {
         __builtin_amdgcn_global_load_lds(
             (const __attribute__((address_space(1))) void *)p,
-            (__attribute__((address_space(3))) void *)(to_stage + (i * Sh::threads + wave * 64) * 16), 16, 0, 0);
+            (__attribute__((address_space(3))) void *)(to_stage +
+                                                       (i * Sh::threads + wave * 64) * 16),
+            16, 0, 0);
       } else {
         held[i] = *reinterpret_cast<const u32x4 *>(p);
       }
@@ -416,7 +429,8 @@ __global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int 
   // hi and lo of rows (Gram: columns) 32 t .. of an operand's stage, 16 summed values
   auto operand = [&](const char *in, uint32_t t, uint32_t half, f16x8 &hi, f16x8 &lo) {
     if constexpr (S == Step::Gram) {
-      const uint32_t row = half * 16 + (lane >> 5) * 4 + (lane >> 2 & 3), line = row / kLineRows % 32;
+      const uint32_t row = half * 16 + (lane >> 5) * 4 + (lane >> 2 & 3);
+      const uint32_t line = row / kLineRows % 32;
       const uint32_t pass = kLineRows == 2 ? row / 64 : row / 32 * (kTile / 64) + t / 2;
       const uint32_t part = (kLineRows == 2 ? row & 1 : t & 1) * 4 + (lane >> 4 & 1);
       const char *p = in + (pass * 32 + line) * 256 + (lane & 3) * 8;
@@ -442,8 +456,10 @@ __global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int 
     for (int j = 0; j < TN; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-  // A stage is loaded while the one before is multiplied, from behind its last fragments' reads into
-  // the buffer whose readers passed the barrier.
+  // Direct: a stage is loaded while the one before is multiplied, from behind its last fragments'
+  // reads into the buffer whose readers passed the barrier.  Through registers: loaded two stages
+  // ahead, and written to that buffer behind the first fragments' reads.  Loading further ahead, or
+  // more per stage, changed nothing.
   fetch(0, stage);
   if constexpr (!Sh::Direct) {
     put(stage);
@@ -505,11 +521,11 @@ __global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int 
       for (int o = 0; o < kGroups; ++o) {
         if (t0 + o >= kBlocks) continue;
         float *slot = space + ((place * kTurn + o) * kGroups + group) * 1024 + lane * 4;
+        const f32x16 &sums = acc[(t0 + o) / TN][(t0 + o) % TN];
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           *reinterpret_cast<f32x4 *>(slot + q * 256) =
-              f32x4{acc[(t0 + o) / TN][(t0 + o) % TN][4 * q], acc[(t0 + o) / TN][(t0 + o) % TN][4 * q + 1],
-                    acc[(t0 + o) / TN][(t0 + o) % TN][4 * q + 2], acc[(t0 + o) / TN][(t0 + o) % TN][4 * q + 3]};
+              f32x4{sums[4 * q], sums[4 * q + 1], sums[4 * q + 2], sums[4 * q + 3]};
       }
       __syncthreads();
 #pragma unroll
@@ -543,7 +559,8 @@ __global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int 
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       if (Sh::Groups > 1 && (i * TN + j) % Sh::Groups != static_cast<int>(group)) continue;
-      const uint32_t row0 = ti * kTile + (wi * TM + i) * 32, column0 = tj * kTile + (wj * TN + j) * 32;
+      const uint32_t row0 = ti * kTile + (wi * TM + i) * 32;
+      const uint32_t column0 = tj * kTile + (wj * TN + j) * 32;
       const uint32_t column = column0 + (lane & 31);
       // X or A at this place: among the operand rows just read
       f32x4 addend[4];
@@ -656,7 +673,8 @@ __global__ __launch_bounds__(64 * kWholeWaves) void muon_whole_kernel(Group g, u
   const Matrix &m = g.m[blockIdx.x];
   const bool tall = m.rows > m.columns;
   const uint32_t s = tall ? m.columns : m.rows, n = tall ? m.rows : m.columns;
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t col = lane & 15, quad = lane >> 4;
   const uint32_t column_blocks = (n + 31) / 32 * 2;
   // The matrix lies in the shared memory as in memory, its rows an odd number of words apart, on
   // the way in and out: fn(offset there, offset in memory) for each of this thread's elements.
@@ -898,9 +916,9 @@ struct Item {
 uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
 
 // Whether one block steps the whole matrix: the rows of the shared memory that hold X', and at most
-// this many column blocks per wave (one matrix of 96 x 192 43 us, 72 in launches; of 96 x 384 83 and
-// 75, but 16 of them 84 and 143; of 128 x 192 60 and 73; of 128 x 256, whose two column blocks spill,
-// 180 and 74, 16 of them 181 and 140).
+// this many column blocks per wave (one matrix of 96 x 192 43 us, 72 in launches; of 96 x 384 83
+// and 75, but 16 of them 84 and 143; of 128 x 192 60 and 73; of 128 x 256, whose two column blocks
+// spill, 180 and 74, 16 of them 181 and 140).
 constexpr int whole_blocks(int ps) { return ps == 32 ? 6 : ps == 64 ? 3 : ps == 96 ? 2 : 1; }
 bool whole(const Item &it) {
   const uint64_t s = std::min(it.rows, it.columns), n = std::max(it.rows, it.columns);
@@ -929,8 +947,8 @@ struct Tiles {
 //   64 otherwise (`Few` up to a block per compute unit: 1024 x 1024, 136 and 256 tiles, 201 us and
 //     254 without; everywhere, 12 x 512 x 2048 takes 716 and 657 without);
 // and both take 192 where the square products just fill one round of a block per compute unit, with
-// the same limit on padding (4096 x 4096, 253 tiles: 4.06 ms, 4.80 with 128; 2560 x 2560, 105 tiles:
-// 1641 and 1367 us; 12 x 1024 x 1024, 252 tiles padded 1.27 times: 1330 and 1079).
+// the same limit on padding (4096 x 4096, 253 tiles: 4.06 ms, 4.80 with 128; 2560 x 2560, 105
+// tiles: 1641 and 1367 us; 12 x 1024 x 1024, 252 tiles padded 1.27 times: 1330 and 1079).
 Tiles tiles_of(const Item *items, size_t count) {
   struct Count {
     uint64_t square = 0, apply = 0, area = 0;

@@ -7,6 +7,14 @@
 //
 // A row's steps at or past its length give 0, take no gradient and leave the state.  No
 // counterpart in the reference, which has no layer along a sequence.
+//
+// Composing two steps' maps h -> a h + b is associative, so time is cut into tiles that a block
+// scans, and into segments where rows and channels alone leave compute units idle.  The bound is
+// memory: forward 8 x 2048 x 2048 float32 takes 82 us (4.9 TB/s), backward 153 us (5.3 TB/s).
+// Split, the operands are read twice: forward 1 x 131072 x 512 bfloat16 takes 52 us for the
+// segments' maps and 72 us for the states, 671 MB at 5.4 TB/s (one pass over its 403 MB would need
+// the segments' states handed on inside one launch).  A single step of 64 x 2048 takes 3.4 us, a
+// launch.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -281,8 +289,8 @@ __global__ __launch_bounds__(64 * W) void recurrence_kernel(Args<T> a) {
   int turn = 0;
   if (a.segments > 1) {
     // the entries before this segment, shared out among the time groups
-    const float *entry = a.parts + static_cast<uint64_t>(p.row) * (a.segments + 1) * 2 * a.channels +
-                         (p.in ? p.channel : 0);
+    const float *entry = a.parts + (p.in ? p.channel : 0) +
+                         static_cast<uint64_t>(p.row) * (a.segments + 1) * 2 * a.channels;
     const uint32_t share = (p.segment + kGroups - 1) / kGroups;
     const uint32_t begin = group * share, end = min(begin + share, p.segment);
     Map<V> map;
@@ -462,7 +470,6 @@ struct Plan {
   uint32_t groups, segments, steps;
 };
 
-constexpr int kBriefTime = 16;
 // Waves per block, and steps per thread and tile.  Eight waves of four steps (backward: two) hold
 // the bytes in flight of four waves of eight in half the registers each, and more of them hide more
 // (forward 8 x 2048 x 2048 float32 87 us, 94 with four; 10 x 356 x 855 12.6 and 15.7; backward 8 x
@@ -476,12 +483,12 @@ constexpr int steps_of(int values, bool back) { return (values == 1 ? 8 : 4) / (
 // (8 x 2048 x 512 float32, 8 tiles: 24.6 us whole, 28.7 split; 2 x 512 x 1024, 2 tiles: 7.6 and 12;
 // 5 x 1537 x 333 bfloat16, 7 tiles: 23.7 and 14.2; 1 x 4096 x 2048 float32, 16 tiles: 41 and 30);
 // there 32 channels per block where 64 leave more than half of the units without (8 x 2048 x 512,
-// 64 blocks: 24.6 and 39; 10 x 356 x 855, 140 blocks: 15.4 and 12.6).  Otherwise it is split for two
-// blocks per unit, a tile at least per segment (3 x 700 x 130: 10.5 us with one, 16.3 with two).
+// 64 blocks: 24.6 and 39; 10 x 356 x 855, 140 blocks: 15.4 and 12.6).  Otherwise it is split for
+// two blocks per unit, a tile at least per segment (3 x 700 x 130: 10.5 us with one, 16.3 with
+// two).
 Plan plan_of(uint64_t batch, uint64_t time, uint64_t channels, uint64_t element, bool back) {
   Plan p;
   p.values = channels < 4 ? 1 : 4;
-  p.brief = time <= kBriefTime;
   auto across = [&](int lanes) {
     p.lanes = lanes;
     p.groups = static_cast<uint32_t>((channels + lanes * p.values - 1) / (lanes * p.values));
@@ -493,8 +500,17 @@ Plan plan_of(uint64_t batch, uint64_t time, uint64_t channels, uint64_t element,
   };
   p.segments = 1;
   p.steps = static_cast<uint32_t>(time);
-  const int lanes = p.brief ? 64 : p.values == 1 ? 32 : channels <= 32 ? 8 : 16;
-  const uint64_t blocks = across(lanes), units = oxh::kComputeUnits;
+  // 32 channels per block where there are no more (1 x 65536 x 32 bfloat16: 11.2 us, 16.8 with 64
+  // per block) or up to 64 in few rows (1 x 65536 x 64: 14.0 and 16.2; 1000 x 33 x 64: 16.8 and
+  // 10.1)
+  const uint64_t units = oxh::kComputeUnits;
+  const int lanes = p.values == 1 ? 32 : channels <= (batch < units ? 64 : 32) ? 8 : 16;
+  const uint64_t blocks = across(lanes);
+  // Few steps: one wave steps 256 channels one after the other, 4 loads ahead, at about 0.3 us a
+  // step (64 x 4 x 2048 float32: 3.8 us, 16 in tiles; 4 x 16 x 1024 bfloat16: 6.2 and 5.0), while a
+  // tile of idle steps takes as long as a full one (256 x 32 x 4096: 110 us, 33 by waves).
+  p.brief = time <= std::min<uint64_t>(64, std::max<uint64_t>(8, blocks / 64));
+  if (p.brief) across(64);
   if (p.brief || blocks >= units) return p;
   uint64_t tile;
   if (p.values == 4 && blocks * 2 < units) across(8);
@@ -522,9 +538,9 @@ oxh_status run_split(hipStream_t stream, uint64_t batch, Args<T> a, const char *
     oxh_status st = oxh::launched(what);
     if (st != OXH_OK) return st;
   }
-  // What passes beyond the 256 MB last-level cache is not kept there, where blocks write whole lines
-  // (backward 8 x 2048 x 2048 float32, 805 MB: 160 us, 172 with the default policy; forward 1 x
-  // 131072 x 512 bfloat16, 403 MB: 128 and 152; off lines it costs: backward 8 x 2048 x 2048
+  // What passes beyond the 256 MB last-level cache is not kept there, where blocks write whole
+  // lines (backward 8 x 2048 x 2048 float32, 805 MB: 160 us, 172 with the default policy; forward
+  // 1 x 131072 x 512 bfloat16, 403 MB: 128 and 152; off lines it costs: backward 8 x 2048 x 2048
   // bfloat16 161 us, 118 with the default); smaller calls leave their results to the next one.
   constexpr uint64_t kCached = 256ull << 20;
   const uint64_t moved = batch * a.time * a.channels * sizeof(T) * (Back ? 6 : 3);
@@ -563,8 +579,9 @@ oxh_status run(hipStream_t stream, uint64_t batch, Args<T> a, const char *what) 
   a.segments = p.segments;
   a.steps = p.steps;
   // Lines that two groups share stay in one L2 if neighbouring blocks are on one XCD (forward 8 x
-  // 2048 x 2048 bfloat16 16 bytes off a line: 42 us, 60 without; backward 1 x 5824 x 955 24 and 34); those of their own are better
-  // spread over the XCDs (forward 16 x 1024 x 4096 bfloat16: 83 us, 104 together).
+  // 2048 x 2048 bfloat16 16 bytes off a line: 42 us, 60 without; backward 1 x 5824 x 955 24 and
+  // 34); those of their own are better spread over the XCDs (forward 16 x 1024 x 4096 bfloat16: 83
+  // us, 104 together).
   constexpr uint64_t kLine = 128;
   a.lines = a.channels * sizeof(T) % kLine == 0 &&
             p.lanes * p.values * sizeof(T) % kLine == 0;

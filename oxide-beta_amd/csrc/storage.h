@@ -53,9 +53,9 @@ __device__ __forceinline__ void load(const T *p, float (&v)[N]) {
   widen_all<T, N>(raw<T, N>(p), v);
 }
 
-// The places of a row that N consecutive ones from `at` (< columns) stand for, columns >= N.  Ragged
-// rows, whose columns are no multiple of N, end in an access that begins early enough to stay within
-// the row: its first `skip` values are the access's before it.
+// The places of a row that N consecutive ones from `at` (< columns) stand for, columns >= N.
+// Ragged rows, whose columns are no multiple of N, end in an access that begins early enough to
+// stay within the row: its first `skip` values are the access's before it.
 struct Places {
   uint32_t start, skip;
 };

@@ -348,8 +348,8 @@ def test_more_than_the_caches_hold(module, dev):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("shape", [(2, 5, 65), (3, 40, 5), (2, 300, 65), (1, 3000, 67), (2, 9, 2051),
-                                   (300, 20, 7), (2, 300, 3)])
+@pytest.mark.parametrize("shape", [(2, 5, 65), (3, 40, 5), (2, 300, 65), (1, 3000, 67),
+                                   (2, 9, 2051), (300, 20, 7), (2, 300, 3)])
 def test_ragged_channels(module, dev, shape, dtype):
     """Channels that are no multiple of an access, of one in another block among them: the state
     where it lay, and nothing written before or behind an output."""
