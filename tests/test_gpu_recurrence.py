@@ -377,3 +377,21 @@ def test_ragged_channels(module, dev, shape, dtype):
     within(ds, rds, eds, torch.float32, "state gradient")
     for b in (around, more):
         assert (b[:21] == 7).all() and (b[21 + size:] == 7).all()
+
+
+def test_offsets_past_32_bits(module, dev):
+    """More than 2^31 elements: the last steps against the formulas from 40 steps before them, which
+    reach no further (keep is below 0.02 there: 0.02^30 of anything is below the tolerance)."""
+    t, shape, n = torch.bfloat16, (1, 4200001, 512), 40
+    u = torch.randn(shape, dtype=t, device=dev)
+    g = torch.randn(shape, dtype=t, device=dev).sub_(8).clamp_(-10, -4)
+    h = torch.empty_like(u)
+    module.gated_recurrence_forward(u, g, h)
+    tail = lambda x: x[:, -n:].contiguous()  # noqa: E731
+    ref, err, _, _ = forward_ref(tail(u), tail(g), None, None)
+    within(tail(h)[:, 30:], ref[:, 30:], err[:, 30:], t, "output")
+    du, dg = torch.empty_like(u), torch.empty_like(u)
+    module.gated_recurrence_backward(u, u, g, h, du, dg)
+    out, _, _ = backward_ref(tail(u), tail(u), tail(g), tail(h), None, None, None)
+    within(tail(du)[:, 1:], out[0][:, 1:], out[1][:, 1:], t, "input gradient")
+    within(tail(dg)[:, 1:], out[2][:, 1:], out[3][:, 1:], t, "gate gradient")

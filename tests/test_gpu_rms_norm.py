@@ -233,3 +233,18 @@ def test_ragged_rows(module, dev, shape, dtype):
     module.rms_norm_backward(g, x, w, q, dx, dw, sum_gradient=dx)
     check_backward(x, g, w, sg, q, dx, dw, t)
     assert (around[:33] == 7).all() and (around[33 + size:] == 7).all()
+
+
+def test_offsets_past_32_bits(module, dev):
+    """More than 2^31 elements: the last rows against the formulas."""
+    t, shape = torch.bfloat16, (70001, 32765)
+    x = torch.randn(shape, dtype=t, device=dev)
+    w = torch.randn(shape[1], device=dev)
+    y, q = torch.empty_like(x), torch.empty(shape[0], device=dev)
+    module.rms_norm_forward(x, w, y, q)
+    s_ref, q_ref, y_ref = forward_ref(x[-3:], None, w, 1e-6)
+    within(q[-3:], q_ref, q_ref, 64, torch.float32, "inverse rms")
+    within(y[-3:], y_ref, np.abs(y_ref), 64, t, "output")
+    dx = torch.empty_like(x)
+    module.rms_norm_backward(y, x, w, q, dx, None)
+    check_backward(x[-3:], y[-3:], w, None, q[-3:], dx[-3:], None, t)
