@@ -285,27 +285,25 @@ def _ptr(t) -> int | None:
     return t.data_ptr()
 
 
-def _f32_tensor(t, name: str):
+F32, BF16 = 0, 1
+_codes = {}  # torch dtype -> F32 / BF16, filled at the first use (with _float32 and _int32)
+_float32 = _int32 = None
+
+
+def _know_types() -> None:
+    global _float32, _int32
     import torch
 
-    if t.dtype != torch.float32 or not t.is_cuda:
-        raise OxideError(INVALID_SHAPE, f"{name} must be a float32 device tensor")
-    return t
-
-
-F32, BF16 = 0, 1
-_activation_codes = None  # torch dtype -> F32 / BF16, filled at the first use
+    _float32, _int32 = torch.float32, torch.int32
+    _codes.update({torch.float32: F32, torch.bfloat16: BF16})
 
 
 def _activation(tensors, shape, what: str) -> int:
     """The dtype code of device tensors that share one type and one shape (None: absent)."""
-    global _activation_codes
-    if _activation_codes is None:
-        import torch
-
-        _activation_codes = {torch.float32: F32, torch.bfloat16: BF16}
+    if _float32 is None:
+        _know_types()
     dtype = tensors[0].dtype
-    code = _activation_codes.get(dtype)
+    code = _codes.get(dtype)
     if code is None:
         raise OxideError(INVALID_SHAPE, f"{what} takes float32 or bfloat16 tensors")
     for t in tensors:
@@ -320,7 +318,11 @@ def _shaped(t, shape, name: str):
     """Address of a contiguous float32 device tensor of ``shape``, or None."""
     if t is None:
         return None
-    if _f32_tensor(t, name).shape != shape:
+    if _float32 is None:
+        _know_types()
+    if t.dtype is not _float32 or not t.is_cuda:
+        raise OxideError(INVALID_SHAPE, f"{name} must be a float32 device tensor")
+    if t.shape != shape:
         raise OxideError(INVALID_SHAPE,
                          f"{name}: shape {list(t.shape)} where {list(shape)} is expected")
     return _ptr(t)
@@ -329,9 +331,9 @@ def _shaped(t, shape, name: str):
 def _lengths(t, batch: int):
     if t is None:
         return None
-    import torch
-
-    if t.dtype != torch.int32 or not t.is_cuda or t.shape != (batch,):
+    if _float32 is None:
+        _know_types()
+    if t.dtype is not _int32 or not t.is_cuda or t.shape != (batch,):
         raise OxideError(INVALID_SHAPE, "lengths must be an int32 device tensor [batch]")
     return _ptr(t)
 
@@ -385,6 +387,33 @@ class Workspace:
         return b.data_ptr(), b.numel()
 
 
+class StreamWorkspaces:
+    """Device scratch, a buffer for each stream, so that calls on two streams share none.  One that
+    has become too small is kept, since a captured graph may hold its address, and its successor is
+    twice its size at least."""
+
+    def __init__(self):
+        self._bufs = {}  # stream -> buffers, the last in use
+
+    def ptr_bytes(self, nbytes: int, stream: int) -> tuple[int | None, int]:
+        if nbytes == 0:
+            return None, 0
+        bufs = self._bufs.get(stream)
+        if bufs is None or bufs[-1].numel() < nbytes:
+            import torch
+
+            size = max(nbytes, 2 * bufs[-1].numel() if bufs else 256)
+            if stream == current_stream():
+                buf = torch.empty(size, dtype=torch.uint8, device="cuda")
+            else:  # of the stream's own memory: what it frees waits for its kernels
+                with torch.cuda.stream(torch.cuda.ExternalStream(stream) if stream
+                                       else torch.cuda.default_stream()):
+                    buf = torch.empty(size, dtype=torch.uint8, device="cuda")
+            bufs = self._bufs.setdefault(stream, [])
+            bufs.append(buf)
+        return bufs[-1].data_ptr(), bufs[-1].numel()
+
+
 def batch_norm_workspace_size(batch: int, channels: int, spatial: int) -> int:
     out = _u64()
     check(lib().oxh_batch_norm_workspace_size(batch, channels, spatial, ctypes.byref(out)))
@@ -421,6 +450,8 @@ def orthogonalize_workspace_size(count: int, rows: int, columns: int) -> int:
 def muon_table(tensors):
     """The C table of a sequence of (parameter, gradient, momentum): each a matrix
     [shape[0], the rest] of float32 device values."""
+    if _float32 is None:
+        _know_types()
     table = (MuonTensor * len(tensors))()
     for i, (p, g, m) in enumerate(tensors):
         shape = tuple(p.shape)
@@ -428,8 +459,8 @@ def muon_table(tensors):
             raise OxideError(INVALID_SHAPE,
                              "muon takes matrices: equal shapes of at least two dimensions")
         for t in (p, g, m):
-            if hasattr(t, "dtype") and hasattr(t, "is_cuda"):
-                _f32_tensor(t, "a muon tensor")
+            if t.dtype is not _float32 or not t.is_cuda:
+                raise OxideError(INVALID_SHAPE, "a muon tensor must be a float32 device tensor")
         columns = 1
         for d in shape[1:]:
             columns *= d
@@ -587,7 +618,7 @@ class LoadedModule:
         self._bn_ws = Workspace()
         self._ce_ws = Workspace()
         self._conv_ws = Workspace()
-        self._sequence_ws = Workspace()
+        self._sequence_ws = StreamWorkspaces()
 
     # -- elementwise (kernel_module.rs:8-34, 492-508, 1052-1059)
     def add(self, a, b, out, stream=None):
@@ -847,9 +878,6 @@ class LoadedModule:
         return dev_table, dev_starts
 
     # -- sequence layers (no counterpart in the reference)
-    def _sequence_workspace(self, nbytes: int) -> tuple[int | None, int]:
-        return self._sequence_ws.ptr_bytes(nbytes) if nbytes else (None, 0)
-
     def rms_norm_forward(self, x, weight, out, inverse_rms=None, residual=None, sum=None,  # noqa: A002
                          epsilon=1e-6, stream=None):
         """``out`` = s / rms(s) * weight over the last dimension, s = x + residual; ``sum``
@@ -873,10 +901,12 @@ class LoadedModule:
                            "rms_norm_backward")
         columns = shape[-1] if shape else 0
         rows = gradient.numel() // max(columns, 1)
-        ws, wsb = self._sequence_workspace(
-            0 if weight_gradient is None else rms_norm_backward_workspace_size(rows, columns))
+        stream = _stream(stream)
+        ws, wsb = self._sequence_ws.ptr_bytes(
+            0 if weight_gradient is None else rms_norm_backward_workspace_size(rows, columns),
+            stream)
         check(lib().oxh_rms_norm_backward(
-            _stream(stream), code, rows, columns, _ptr(gradient), _ptr(sum_gradient), _ptr(sum),
+            stream, code, rows, columns, _ptr(gradient), _ptr(sum_gradient), _ptr(sum),
             _shaped(weight, (columns,), "weight"), _shaped(inverse_rms, (rows,), "inverse_rms"),
             _ptr(input_gradient), _shaped(weight_gradient, (columns,), "weight_gradient"), ws,
             wsb))
@@ -892,9 +922,11 @@ class LoadedModule:
         code = _activation((x, gate, out), shape, "gated_recurrence")
         batch, time, channels = shape
         states = (batch, channels)
-        ws, wsb = self._sequence_workspace(gated_recurrence_workspace_size(batch, time, channels))
+        stream = _stream(stream)
+        ws, wsb = self._sequence_ws.ptr_bytes(
+            gated_recurrence_workspace_size(batch, time, channels), stream)
         check(lib().oxh_gated_recurrence_forward(
-            _stream(stream), code, batch, time, channels, _ptr(x), _ptr(gate),
+            stream, code, batch, time, channels, _ptr(x), _ptr(gate),
             _shaped(initial_state, states, "initial_state"), _lengths(lengths, batch),
             _ptr(out), _shaped(final_state, states, "final_state"), ws, wsb))
 
@@ -910,9 +942,11 @@ class LoadedModule:
                            "gated_recurrence_backward")
         batch, time, channels = shape
         states = (batch, channels)
-        ws, wsb = self._sequence_workspace(gated_recurrence_workspace_size(batch, time, channels))
+        stream = _stream(stream)
+        ws, wsb = self._sequence_ws.ptr_bytes(
+            gated_recurrence_workspace_size(batch, time, channels), stream)
         check(lib().oxh_gated_recurrence_backward(
-            _stream(stream), code, batch, time, channels, _ptr(gradient), _ptr(x), _ptr(gate),
+            stream, code, batch, time, channels, _ptr(gradient), _ptr(x), _ptr(gate),
             _ptr(out), _shaped(initial_state, states, "initial_state"),
             _shaped(final_state_gradient, states, "final_state_gradient"),
             _lengths(lengths, batch), _ptr(x_gradient), _ptr(gate_gradient),
@@ -924,8 +958,10 @@ class LoadedModule:
         if x.dim() not in (2, 3):
             raise OxideError(INVALID_SHAPE, "orthogonalize expects a matrix or a stack of them")
         count, (rows, columns) = (x.shape[0] if x.dim() == 3 else 1), x.shape[-2:]
-        ws, wsb = self._sequence_workspace(orthogonalize_workspace_size(count, rows, columns))
-        check(lib().oxh_orthogonalize(_stream(stream), count, rows, columns, rounds, epsilon,
+        stream = _stream(stream)
+        ws, wsb = self._sequence_ws.ptr_bytes(orthogonalize_workspace_size(count, rows, columns),
+                                              stream)
+        check(lib().oxh_orthogonalize(stream, count, rows, columns, rounds, epsilon,
                                       _shaped(x, x.shape, "x"), _shaped(out, x.shape, "out"), ws,
                                       wsb))
 
@@ -934,8 +970,9 @@ class LoadedModule:
         """One optimizer step of ``tensors``, a sequence of (parameter, gradient, momentum):
         the momentum and the parameter are updated in place."""
         table = muon_table(tensors)
-        ws, wsb = self._sequence_workspace(muon_workspace_size(table))
-        check(lib().oxh_muon_multi_tensor(_stream(stream), learning_rate, weight_decay, momentum,
+        stream = _stream(stream)
+        ws, wsb = self._sequence_ws.ptr_bytes(muon_workspace_size(table), stream)
+        check(lib().oxh_muon_multi_tensor(stream, learning_rate, weight_decay, momentum,
                                           int(bool(nesterov)), epsilon, rounds, table,
                                           len(table), ws, wsb))
 

@@ -395,3 +395,37 @@ def test_offsets_past_32_bits(module, dev):
     out, _, _ = backward_ref(tail(u), tail(u), tail(g), tail(h), None, None, None)
     within(tail(du)[:, 1:], out[0][:, 1:], out[1][:, 1:], t, "input gradient")
     within(tail(dg)[:, 1:], out[2][:, 1:], out[3][:, 1:], t, "gate gradient")
+
+
+def test_workspaces_of_streams_and_graphs(module, dev):
+    """Streams share no scratch memory, and a captured call keeps its own when the stream's next
+    ones need more."""
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    ws = ox.StreamWorkspaces()
+    a, b = (ws.ptr_bytes(1000, s.cuda_stream)[0] for s in (one, two))
+    c, size = ws.ptr_bytes(1001, one.cuda_stream)
+    assert len({a, b, c}) == 3 and size >= 2000
+    assert ws.ptr_bytes(10, one.cuda_stream) == (c, size)
+    assert ws.ptr_bytes(0, one.cuda_stream) == (None, 0)
+
+    t, shape = torch.float32, (1, 3000, 24)
+    u, g = make(shape, t, dev, 1), gates(shape, t, dev, 2)
+    want, h = torch.empty_like(u), torch.empty_like(u)
+    own = ox.load_kernels(0)
+    own.gated_recurrence_forward(u, g, want)
+    run = lambda: own.gated_recurrence_forward(u, g, h, stream=one)  # noqa: E731
+    torch.cuda.synchronize()
+    run()
+    graph = ox.HipGraphExec.capture(one, run)
+    large = make((1, 60000, 96), t, dev, 3)
+    out = torch.empty_like(large)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        own.gated_recurrence_forward(large, large, out, stream=one)
+        fill = torch.full((1 << 20,), 3.0, device=dev)  # takes memory that was given back
+        torch.cuda.synchronize()
+        h.zero_()
+        torch.cuda.synchronize()
+        graph.launch(one)
+        torch.cuda.synchronize()
+        assert torch.equal(h, want) and (fill == 3).all()
