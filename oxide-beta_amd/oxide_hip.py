@@ -298,20 +298,28 @@ def _know_types() -> None:
     _codes.update({torch.float32: F32, torch.bfloat16: BF16})
 
 
-def _activation(tensors, shape, what: str) -> int:
-    """The dtype code of device tensors that share one type and one shape (None: absent)."""
+def _activations(tensors, shape, what: str) -> tuple:
+    """The dtype code of contiguous device tensors that share one type and one shape (None:
+    absent), and their addresses."""
     if _float32 is None:
         _know_types()
     dtype = tensors[0].dtype
     code = _codes.get(dtype)
     if code is None:
         raise OxideError(INVALID_SHAPE, f"{what} takes float32 or bfloat16 tensors")
+    out = [code]
     for t in tensors:
-        if t is not None and (t.dtype is not dtype or not t.is_cuda or t.shape != shape):
+        if t is None:
+            out.append(None)
+            continue
+        if t.dtype is not dtype or not t.is_cuda or t.shape != shape:
             raise OxideError(INVALID_SHAPE,
                              f"{what} takes device tensors of one type and of shape "
                              f"{list(shape)}: got {t.dtype} {list(t.shape)} on {t.device}")
-    return code
+        if not t.is_contiguous():
+            raise OxideError(INVALID_SHAPE, "tensors must be contiguous")
+        out.append(t.data_ptr())
+    return out
 
 
 def _shaped(t, shape, name: str):
@@ -325,7 +333,9 @@ def _shaped(t, shape, name: str):
     if t.shape != shape:
         raise OxideError(INVALID_SHAPE,
                          f"{name}: shape {list(t.shape)} where {list(shape)} is expected")
-    return _ptr(t)
+    if not t.is_contiguous():
+        raise OxideError(INVALID_SHAPE, "tensors must be contiguous")
+    return t.data_ptr()
 
 
 def _lengths(t, batch: int):
@@ -884,12 +894,13 @@ class LoadedModule:
         receives s (it may be ``x`` or ``residual``) and ``inverse_rms`` [rows] what the
         backward needs."""
         shape = x.shape
-        code = _activation((x, out, residual, sum), shape, "rms_norm")
+        code, x_at, out_at, residual_at, sum_at = _activations((x, out, residual, sum), shape,
+                                                               "rms_norm")
         columns = shape[-1] if shape else 0
         rows = x.numel() // max(columns, 1)
         check(lib().oxh_rms_norm_forward(
-            _stream(stream), code, rows, columns, epsilon, _ptr(x), _ptr(residual),
-            _shaped(weight, (columns,), "weight"), _ptr(sum), _ptr(out),
+            _stream(stream), code, rows, columns, epsilon, x_at, residual_at,
+            _shaped(weight, (columns,), "weight"), sum_at, out_at,
             _shaped(inverse_rms, (rows,), "inverse_rms")))
 
     def rms_norm_backward(self, gradient, sum, weight, inverse_rms, input_gradient,  # noqa: A002
@@ -897,8 +908,8 @@ class LoadedModule:
         """Gradients from the output's and, where the sum has other uses, ``sum_gradient``
         (``input_gradient`` may be that tensor)."""
         shape = gradient.shape
-        code = _activation((gradient, sum, input_gradient, sum_gradient), shape,
-                           "rms_norm_backward")
+        code, gradient_at, sum_at, input_at, stream_at = _activations(
+            (gradient, sum, input_gradient, sum_gradient), shape, "rms_norm_backward")
         columns = shape[-1] if shape else 0
         rows = gradient.numel() // max(columns, 1)
         stream = _stream(stream)
@@ -906,10 +917,9 @@ class LoadedModule:
             0 if weight_gradient is None else rms_norm_backward_workspace_size(rows, columns),
             stream)
         check(lib().oxh_rms_norm_backward(
-            stream, code, rows, columns, _ptr(gradient), _ptr(sum_gradient), _ptr(sum),
+            stream, code, rows, columns, gradient_at, stream_at, sum_at,
             _shaped(weight, (columns,), "weight"), _shaped(inverse_rms, (rows,), "inverse_rms"),
-            _ptr(input_gradient), _shaped(weight_gradient, (columns,), "weight_gradient"), ws,
-            wsb))
+            input_at, _shaped(weight_gradient, (columns,), "weight_gradient"), ws, wsb))
 
     def gated_recurrence_forward(self, x, gate, out, initial_state=None, final_state=None,
                                  lengths=None, stream=None):
@@ -919,16 +929,16 @@ class LoadedModule:
         shape = x.shape
         if len(shape) != 3:
             raise OxideError(INVALID_SHAPE, "gated_recurrence expects [batch, time, channels]")
-        code = _activation((x, gate, out), shape, "gated_recurrence")
+        code, x_at, gate_at, out_at = _activations((x, gate, out), shape, "gated_recurrence")
         batch, time, channels = shape
         states = (batch, channels)
         stream = _stream(stream)
         ws, wsb = self._sequence_ws.ptr_bytes(
             gated_recurrence_workspace_size(batch, time, channels), stream)
         check(lib().oxh_gated_recurrence_forward(
-            stream, code, batch, time, channels, _ptr(x), _ptr(gate),
+            stream, code, batch, time, channels, x_at, gate_at,
             _shaped(initial_state, states, "initial_state"), _lengths(lengths, batch),
-            _ptr(out), _shaped(final_state, states, "final_state"), ws, wsb))
+            out_at, _shaped(final_state, states, "final_state"), ws, wsb))
 
     def gated_recurrence_backward(self, gradient, x, gate, out, x_gradient, gate_gradient,
                                   initial_state=None, final_state_gradient=None,
@@ -938,18 +948,18 @@ class LoadedModule:
         shape = x.shape
         if len(shape) != 3:
             raise OxideError(INVALID_SHAPE, "gated_recurrence expects [batch, time, channels]")
-        code = _activation((gradient, x, gate, out, x_gradient, gate_gradient), shape,
-                           "gated_recurrence_backward")
+        code, *at = _activations((gradient, x, gate, out, x_gradient, gate_gradient), shape,
+                                 "gated_recurrence_backward")
         batch, time, channels = shape
         states = (batch, channels)
         stream = _stream(stream)
         ws, wsb = self._sequence_ws.ptr_bytes(
             gated_recurrence_workspace_size(batch, time, channels), stream)
         check(lib().oxh_gated_recurrence_backward(
-            stream, code, batch, time, channels, _ptr(gradient), _ptr(x), _ptr(gate),
-            _ptr(out), _shaped(initial_state, states, "initial_state"),
+            stream, code, batch, time, channels, *at[:4],
+            _shaped(initial_state, states, "initial_state"),
             _shaped(final_state_gradient, states, "final_state_gradient"),
-            _lengths(lengths, batch), _ptr(x_gradient), _ptr(gate_gradient),
+            _lengths(lengths, batch), at[4], at[5],
             _shaped(initial_state_gradient, states, "initial_state_gradient"), ws, wsb))
 
     def orthogonalize(self, x, out, rounds=5, epsilon=1e-7, stream=None):

@@ -187,7 +187,7 @@ def test_front_end_checks_shapes():
     with pytest.raises(ox.OxideError):
         ox.muon_table([(z(3, 4), z(3, 5), z(3, 4))])
     with pytest.raises(ox.OxideError):  # host tensors
-        ox._activation((z(2, 3),), (2, 3), "rms_norm")
+        ox._activations((z(2, 3),), (2, 3), "rms_norm")
     assert np.isfinite(ox.gated_recurrence_workspace_size(1, 1, 1))
 
 
