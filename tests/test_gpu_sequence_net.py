@@ -13,6 +13,7 @@ import pytest
 import torch
 import torch.nn.functional as F
 
+import jit
 import nn
 import oxide_hip as ox
 import sequence
@@ -244,3 +245,33 @@ def test_builders_refuse():
     for bad in (dict(learning_rate=0.0), dict(weight_decay=-1.0), dict(momentum=1.0)):
         with pytest.raises(ox.OxideError):
             nn.Muon([], nn.AdamW(1e-3, 0.0), **bad)
+
+
+def test_compiled_block():
+    """jit.compile of a block: no fused plan takes it, so it runs as a program."""
+    block, x = nn.GatedRecurrentBlock(24), randn(2, 11, 24, seed=1)
+    module = jit.compile(block, x)
+    with torch.no_grad():
+        X = torch.tensor(x, dtype=torch.float64)
+        weight = lambda m: torch.tensor(m.conv.weight.host()[:, :, 0, 0].astype(np.float64))  # noqa: E731
+        linear = lambda m, v: v @ weight(m).T + torch.tensor(m.conv.bias.host().astype(np.float64))  # noqa: E731
+        y = norm64(X, torch.tensor(block.norm.weight.host().astype(np.float64)))
+        ref = X + linear(block.project, recurrence64(linear(block.value, y), linear(block.gate, y)))
+    for _ in range(2):
+        close(np.asarray(module.run([x])).reshape(x.shape), ref, "block")
+
+
+def test_adamw_alone_over_sequence_layers():
+    images, labels = images_of(16)
+    model, step = step_of(update=nn.AdamW(1e-2, 0.1))
+    before = [p.host().copy() for p in model.parameters()]
+    step.images.copy_from(images.astype(np.float32).reshape(16, 1, 28, 28) / 255)
+    step.labels.copy_from(labels.astype(np.float32))
+    step.step()
+    assert np.isfinite(step.loss()) and step.program.steps() == 1
+    c1, c2 = ox.adamw_corrections(0.9, 0.999, 1)
+    for p, old in zip(model.parameters(), before):
+        g = step.program.gradient(p.tensor()).host().astype(np.float64)
+        moved = 1e-2 * ((0.1 * g / c1) / (np.sqrt(0.001 * g * g / c2) + 1e-8) + 0.1 * old)
+        off = np.linalg.norm(p.host() - (old - moved))
+        assert off <= 1e-3 * np.linalg.norm(moved) + 1e-7 * np.linalg.norm(old), p.shape
