@@ -41,14 +41,14 @@ __device__ __forceinline__ Gate gate_of(float g) {
   return {r, g < 0.0f ? 1.0f - r : e * r};
 }
 
-// Both directions run h -> keep h + add over their steps in the order taken (backwards in time
-// for the gradients, where h is a_{t+1} l_{t+1}, the gradient that reaches step t from later ones,
-// and add = a_t dh_t).
 struct Layout {
   uint32_t time, channels, groups;  // groups: blocks across the channels
   uint32_t segments, steps;         // steps per segment
   bool lines;                       // every group's channels of a step are whole lines of memory
 };
+// Both directions run h -> keep h + add over their steps in the order taken (backwards in time
+// for the gradients, where h is a_{t+1} l_{t+1}, the gradient that reaches step t from later ones,
+// and add = a_t dh_t).
 template <typename T>
 struct Args : Layout {
   const T *u, *g, *h, *dh;  // forward: u, g
