@@ -35,6 +35,7 @@
 #include <cmath>
 #include <exception>
 #include <string>
+#include <type_traits>
 #include <vector>
 
 #include "common.h"
@@ -629,6 +630,11 @@ __global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int 
 // 16 r + 4 (l / 16) + i that this gives: a pair of row blocks is then an operand of B X as it lies,
 // and transposed reads of the shared memory (16 lanes fetch 4 rows of 16 float16 and each gets a
 // column of 4) give the same order for X X'.
+//
+// The bound is one compute unit's shared memory and its barriers: of the 92000 cycles that 96 x 192
+// takes (38 us), a round is 14500: X X' 3000 (its operands are 2250 of the shared memory's), A and A
+// A 4600 with their halves, shared among the waves that summed a tile, B X 4700 (3400), X' in halves
+// 2000.  The way in is 14000: twelve loads at a time, 7000 where eight took 9300.
 
 constexpr int kWhole = 163840;  // bytes of shared memory, the last for the norm's parts
 constexpr int kWholeWaves = 12;
@@ -666,10 +672,13 @@ __global__ __launch_bounds__(64 * kWholeWaves) void muon_whole_kernel(Group g, u
   constexpr int kRowBlocks = PS / 16, kPitch = whole_pitch(PS), kSquare = square_pitch(PS);
   constexpr int kSide = PS / 32, kTiles = kSide * (kSide + 1) / 2;  // of 32 x 32, lower ones of A
   constexpr int kSplits = kWholeWaves / kTiles;                     // of the sums of A
+  // the waves that finish a tile's four 16 x 16 blocks, and how many each
+  constexpr int kShare = kSplits >= 4 ? 4 : kSplits >= 2 ? 2 : 1, kOwn = 4 / kShare;
+  constexpr int kOwnRows = kShare == 1 ? 2 : 1, kOwnColumns = kOwn / kOwnRows;
   // X' first; then, over it, the sums to be joined, A and B
-  char *const sums = shared, *const sa = shared + kTiles * (kSplits - 1) * 4096,
-              *const sb = sa + square_bytes(PS);
-  static_assert(kTiles * (kSplits - 1) * 4096 + 2 * square_bytes(PS) <= kWhole, "shared memory");
+  constexpr int kSums = kSplits > 1 ? kTiles * 4 * kSplits * 1024 : 0;
+  char *const sums = shared, *const sa = shared + kSums, *const sb = sa + square_bytes(PS);
+  static_assert(kSums + 2 * square_bytes(PS) <= kWhole, "shared memory");
   const Matrix &m = g.m[blockIdx.x];
   const bool tall = m.rows > m.columns;
   const uint32_t s = tall ? m.columns : m.rows, n = tall ? m.rows : m.columns;
@@ -677,27 +686,45 @@ __global__ __launch_bounds__(64 * kWholeWaves) void muon_whole_kernel(Group g, u
   const uint32_t col = lane & 15, quad = lane >> 4;
   const uint32_t column_blocks = (n + 31) / 32 * 2;
   // The matrix lies in the shared memory as in memory, its rows an odd number of words apart, on
-  // the way in and out: fn(offset there, offset in memory) for each of this thread's elements.
+  // the way in and out.  A thread moves kBatch of its elements at a time: load(b, offset in memory)
+  // for each, then use(b, offset there, offset in memory).
   float *const words = reinterpret_cast<float *>(shared);
   const uint32_t pitch = m.columns | 1;
-  auto each = [&](auto fn) {
+  constexpr int kBatch = 12;
+  auto each = [&](auto load, auto use) {
     constexpr uint32_t kThreads = 64 * kWholeWaves;
     const uint32_t rows_on = kThreads / m.columns, columns_on = kThreads % m.columns;
+    const uint32_t all = m.rows * m.columns;
     uint32_t row = threadIdx.x / m.columns, column = threadIdx.x % m.columns;
-    for (uint32_t at = threadIdx.x; at < m.rows * m.columns; at += kThreads) {
-      fn(row * pitch + column, at);
-      row += rows_on;
-      column += columns_on;
-      if (column >= m.columns) column -= m.columns, ++row;
-    }
+    auto batch = [&](uint32_t at, auto whole) {
+      constexpr bool kWholeBatch = decltype(whole)::value;
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b)
+        if (kWholeBatch || at + b * kThreads < all) load(b, at + b * kThreads);
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        if (kWholeBatch || at + b * kThreads < all)
+          use(b, row * pitch + column, at + b * kThreads);
+        row += rows_on;
+        column += columns_on;
+        if (column >= m.columns) column -= m.columns, ++row;
+      }
+    };
+    uint32_t at = threadIdx.x;
+    for (; at + (kBatch - 1) * kThreads < all; at += kBatch * kThreads)
+      batch(at, std::true_type());
+    if (at < all) batch(at, std::false_type());
   };
   const uint32_t step_i = tall ? 1 : pitch, step_j = tall ? pitch : 1;
 
-  float squares = 0.0f;
-  each([&](uint32_t to, uint32_t at) {
-    float v = m.gradient[at];
+  float squares = 0.0f, grad[kBatch], mom[kBatch];
+  each([&](int b, uint32_t at) {
+    grad[b] = m.gradient[at];
+    if (m.momentum != nullptr) mom[b] = m.momentum[at];
+  }, [&](int b, uint32_t to, uint32_t at) {
+    float v = grad[b];
     if (m.momentum != nullptr) {
-      const float now = g.momentum * m.momentum[at] + v;
+      const float now = g.momentum * mom[b] + v;
       m.momentum[at] = now;
       v = g.nesterov ? v + g.momentum * now : now;
     }
@@ -711,7 +738,7 @@ __global__ __launch_bounds__(64 * kWholeWaves) void muon_whole_kernel(Group g, u
   float total = 0.0f;
 #pragma unroll
   for (int w = 0; w < kWholeWaves; ++w) total += parts[w];
-  const float norm = sqrtf(total) + g.epsilon;
+  const float inverse = 1.0f / (sqrtf(total) + g.epsilon);
   f32x4 x[Blocks][kRowBlocks];
 #pragma unroll
   for (int c = 0; c < Blocks; ++c) {
@@ -721,7 +748,7 @@ __global__ __launch_bounds__(64 * kWholeWaves) void muon_whole_kernel(Group g, u
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint32_t i = 16 * r + 4 * quad + e;
-        x[c][r][e] = i < s && j < n ? words[i * step_i + j * step_j] / norm : 0.0f;
+        x[c][r][e] = i < s && j < n ? words[i * step_i + j * step_j] * inverse : 0.0f;
       }
     __builtin_amdgcn_sched_barrier(0);
   }
@@ -775,25 +802,35 @@ __global__ __launch_bounds__(64 * kWholeWaves) void muon_whole_kernel(Group g, u
       }
     }
     __syncthreads();
+    // this wave's blocks of A, and the first one's place in the tile
+    f32x4 own[kOwnRows][kOwnColumns];
+    const uint32_t i0 = kShare == 1 ? 0 : kShare == 2 ? split : split >> 1;
+    const uint32_t j0 = kShare == 4 ? split & 1 : 0;
     if constexpr (kSplits > 1) {
-      f32x4 *mine = reinterpret_cast<f32x4 *>(sums) + ((split - 1) * kTiles + tile) * 256 + lane;
-      if (split != 0 && split < kSplits) {
+      f32x4 *slot = reinterpret_cast<f32x4 *>(sums) + tile * 4 * kSplits * 64 + lane;
+      if (split < kSplits) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) mine[q * 64] = acc[q >> 1][q & 1];
+        for (uint32_t q = 0; q < 4; ++q)
+          if (q / kOwn != split) slot[(q * kSplits + split) * 64] = acc[q >> 1][q & 1];
       }
       __syncthreads();
-      if (split == 0) {
-        const f32x4 *other = reinterpret_cast<const f32x4 *>(sums) + tile * 256 + lane;
 #pragma unroll
-        for (int p = 0; p < kSplits - 1; ++p)
+      for (uint32_t q = 0; q < 4; ++q) {
+        if (q / kOwn != split) continue;
+        f32x4 sum = {};
 #pragma unroll
-          for (int q = 0; q < 4; ++q) acc[q >> 1][q & 1] += other[p * kTiles * 256 + q * 64];
+        for (uint32_t p = 0; p < kSplits; ++p)
+          sum += p == split ? acc[q >> 1][q & 1] : slot[(q * kSplits + p) * 64];
+        own[q % kOwn / kOwnColumns][q % kOwn % kOwnColumns] = sum;
       }
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) own[q >> 1][q & 1] = acc[q >> 1][q & 1];
     }
     // block (i, j) of this wave's tile of A or B to the columns' rows of `to` and, off the
     // diagonal, to the rows' rows: there two lanes with neighbouring columns share their four rows'
     // words
-    auto keep = [&](char *to, const f32x4 &v, int i, int j) {
+    auto keep = [&](char *to, const f32x4 &v, uint32_t i, uint32_t j) {
       s16x4 hi, lo;
       halves_of(v, hi, lo);
       char *p = to + (quad * PS + tj * 32 + j * 16 + col) * kSquare + ti * 32 + i * 8;
@@ -821,35 +858,35 @@ __global__ __launch_bounds__(64 * kWholeWaves) void muon_whole_kernel(Group g, u
       out[0] = *reinterpret_cast<const f16x8 *>(p);
       out[1] = *reinterpret_cast<const f16x8 *>(p + 16);
     };
-    if (split == 0) {
+    if (split < kShare) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < kOwnRows; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          acc[i][j] *= kUnscale;
-          keep(sa, acc[i][j], i, j);
+        for (int j = 0; j < kOwnColumns; ++j) {
+          own[i][j] *= kUnscale;
+          keep(sa, own[i][j], i0 + i, j0 + j);
         }
     }
     __syncthreads();
-    if (split == 0) {
-      f32x4 square[2][2] = {};
+    if (split < kShare) {
+      f32x4 square[kOwnRows][kOwnColumns] = {};
 #pragma unroll
       for (int k = 0; k < kSide; ++k) {
-        f16x8 a[2][2], b[2][2];
+        f16x8 a[kOwnRows][2], b[kOwnColumns][2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) rows_of(sa, ti * 32 + i * 16, k, a[i]);
+        for (int i = 0; i < kOwnRows; ++i) rows_of(sa, ti * 32 + (i0 + i) * 16, k, a[i]);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) rows_of(sa, tj * 32 + j * 16, k, b[j]);
+        for (int j = 0; j < kOwnColumns; ++j) rows_of(sa, tj * 32 + (j0 + j) * 16, k, b[j]);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < kOwnRows; ++i)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) multiply(a[i], b[j], square[i][j]);
+          for (int j = 0; j < kOwnColumns; ++j) multiply(a[i], b[j], square[i][j]);
       }
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < kOwnRows; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          keep(sb, kB * acc[i][j] + kC * (square[i][j] * kUnscale), i, j);
+        for (int j = 0; j < kOwnColumns; ++j)
+          keep(sb, kB * own[i][j] + kC * (square[i][j] * kUnscale), i0 + i, j0 + j);
     }
     __syncthreads();
 #pragma unroll
@@ -894,14 +931,13 @@ __global__ __launch_bounds__(64 * kWholeWaves) void muon_whole_kernel(Group g, u
     __builtin_amdgcn_sched_barrier(0);
   }
   __syncthreads();
-  each([&](uint32_t from, uint32_t at) {
+  float w[kBatch];
+  each([&](int b, uint32_t at) {
+    if (m.momentum != nullptr) w[b] = m.target[at];
+  }, [&](int b, uint32_t from, uint32_t at) {
     const float v = words[from];
-    if (m.momentum == nullptr) {
-      m.target[at] = v;
-    } else {
-      const float w = m.target[at];
-      m.target[at] = w - g.lr * (g.decay * w + m.scale * v);
-    }
+    m.target[at] =
+        m.momentum == nullptr ? v : w[b] - g.lr * (g.decay * w[b] + m.scale * v);
   });
 }
 
@@ -916,9 +952,9 @@ struct Item {
 uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
 
 // Whether one block steps the whole matrix: the rows of the shared memory that hold X', and at most
-// this many column blocks per wave (one matrix of 96 x 192 43 us, 72 in launches; of 96 x 384 83
-// and 75, but 16 of them 84 and 143; of 128 x 192 60 and 73; of 128 x 256, whose two column blocks
-// spill, 180 and 74, 16 of them 181 and 140).
+// this many column blocks per wave (one matrix of 96 x 192 38 us, 72 in launches; of 96 x 384 67
+// and 75; of 128 x 192 58 and 73; of 128 x 256, whose two column blocks spill, 116 and 74, 16 of
+// them 117 and 140).
 constexpr int whole_blocks(int ps) { return ps == 32 ? 6 : ps == 64 ? 3 : ps == 96 ? 2 : 1; }
 bool whole(const Item &it) {
   const uint64_t s = std::min(it.rows, it.columns), n = std::max(it.rows, it.columns);
