@@ -631,7 +631,7 @@ __global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int 
 // and transposed reads of the shared memory (16 lanes fetch 4 rows of 16 float16 and each gets a
 // column of 4) give the same order for X X'.
 //
-// The bound is one compute unit's shared memory and its barriers: of the 92000 cycles that 96 x 192
+// The bound is one compute unit's shared memory and its barriers: of the 88000 cycles that 96 x 192
 // takes (38 us), a round is 14500: X X' 3000 (its operands are 2250 of the shared memory's), A and A
 // A 4600 with their halves, shared among the waves that summed a tile, B X 4700 (3400), X' in halves
 // 2000.  The way in is 14000: twelve loads at a time, 7000 where eight took 9300.

@@ -19,6 +19,7 @@ import oxide_hip as ox
 import sequence
 import tensor as tn
 import training
+from test_data_checkpoint import _idx_images, _idx_labels
 from test_gpu_muon import orthogonal
 
 pytestmark = pytest.mark.gpu
@@ -275,3 +276,15 @@ def test_adamw_alone_over_sequence_layers():
         moved = 1e-2 * ((0.1 * g / c1) / (np.sqrt(0.001 * g * g / c2) + 1e-8) + 0.1 * old)
         off = np.linalg.norm(p.host() - (old - moved))
         assert off <= 1e-3 * np.linalg.norm(moved) + 1e-7 * np.linalg.norm(old), p.shape
+
+
+def test_example_on_idx_files(tmp_path, capsys):
+    """The example's command: IDX files in, a line per epoch and the test accuracy out."""
+    for name, count, seed in (("train", 384, 0), ("t10k", 200, 1)):
+        images, labels = images_of(count, seed)
+        (tmp_path / f"{name}-images-idx3-ubyte").write_bytes(_idx_images(images))
+        (tmp_path / f"{name}-labels-idx1-ubyte").write_bytes(_idx_labels(labels))
+    sequence.main(str(tmp_path), 2)
+    lines = capsys.readouterr().out.splitlines()
+    assert [line.split()[0] for line in lines] == ["epoch", "epoch", "test"]
+    assert math.isfinite(float(lines[1].split()[-1])) and 0 <= float(lines[2].split()[-1]) <= 1
