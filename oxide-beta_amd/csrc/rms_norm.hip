@@ -374,10 +374,22 @@ oxh_status forward(hipStream_t stream, const Forward<T> &a) {
   return oxh::launched("rms_norm_forward");
 }
 
+// Rows that one block takes by itself, whose share is the weight gradient: a second launch is about
+// as long as three more rows of a wave, or one of a block (bfloat16 16 x 1024: 7.2 us a call, 10.1
+// with two launches; 32 x 1024: 8.3 and 10.1, but 9.3 and 6.0 on the device; float32 2 x 4096: 7.4
+// and 10.1; 8 x 4096: 13.7 and 10.2).
+constexpr uint64_t rows_alone(int groups) { return groups > 1 ? 4 * groups : 2; }
+
 template <typename T>
-oxh_status backward(hipStream_t stream, const Backward<T> &a, float *weight_gradient) {
+oxh_status backward(hipStream_t stream, Backward<T> a, float *weight_gradient) {
   uint64_t blocks = std::min<uint64_t>(a.rows, block_limit(a.columns));
+  // a single block's share is the weight gradient
+  auto choose = [&](uint64_t count) {
+    blocks = count;
+    if (blocks == 1 && weight_gradient != nullptr) a.partial = weight_gradient;
+  };
   if (a.columns > backward_limit(a.columns % (16 / sizeof(T)) != 0)) {
+    choose(blocks);
     oxh::launch(rms_norm_backward_long_kernel<T>, dim3(static_cast<uint32_t>(blocks)),
                 dim3(1024), 0, stream, a);
   } else {
@@ -390,14 +402,14 @@ oxh_status backward(hipStream_t stream, const Backward<T> &a, float *weight_grad
         // four), and every group the same number of rows, but for the last ones
         const uint64_t most = std::min<uint64_t>(block_limit(a.columns), 512),
                        rounds = (a.rows + most * per - 1) / (most * per);
-        blocks = (a.rows + rounds * per - 1) / (rounds * per);
+        choose(a.rows <= rows_alone(per) ? 1 : (a.rows + rounds * per - 1) / (rounds * per));
         oxh::launch(rms_norm_backward_kernel<T, N, S::lanes, S::chunks, decltype(ragged)::value>,
                     dim3(static_cast<uint32_t>(blocks)), dim3(threads), 0, stream, a);
       });
     });
   }
   oxh_status st = oxh::launched("rms_norm_backward");
-  if (st != OXH_OK || weight_gradient == nullptr) return st;
+  if (st != OXH_OK || weight_gradient == nullptr || blocks == 1) return st;
   oxh::launch(rms_norm_weight_kernel, dim3((a.columns + 15) / 16), dim3(1024), 0, stream,
               static_cast<const float *>(a.partial), weight_gradient,
               static_cast<uint32_t>(blocks), a.columns);

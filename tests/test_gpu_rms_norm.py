@@ -248,3 +248,18 @@ def test_offsets_past_32_bits(module, dev):
     dx = torch.empty_like(x)
     module.rms_norm_backward(y, x, w, q, dx, None)
     check_backward(x[-3:], y[-3:], w, None, q[-3:], dx[-3:], None, t)
+
+
+@pytest.mark.parametrize("shape", [(1, 1024), (16, 1024), (17, 1024), (16, 33), (5, 7), (2, 4096),
+                                   (3, 4096), (1, 40000)])
+def test_few_rows(module, dev, shape):
+    """The weight gradient that one block writes by itself, and the row counts beside it."""
+    t = torch.float32
+    s, g = make(shape, t, dev, 1), make(shape, t, dev, 2)
+    w = make(shape[-1:], t, dev, 3) + 1.0
+    q = torch.from_numpy(1.0 / np.sqrt((f64(s) ** 2).mean(-1) + 1e-6)).float().to(dev)
+    dx, around = torch.empty_like(s), torch.full((shape[1] + 20,), 7.0, device=dev)
+    dw = around[9:9 + shape[1]]
+    module.rms_norm_backward(g, s, w, q, dx, dw)
+    check_backward(s, g, w, None, q, dx, dw, t)
+    assert (around[:9] == 7).all() and (around[9 + shape[1]:] == 7).all()
