@@ -474,7 +474,13 @@ struct Plan {
 // the bytes in flight of four waves of eight in half the registers each, and more of them hide more
 // (forward 8 x 2048 x 2048 float32 87 us, 94 with four; 10 x 356 x 855 12.6 and 15.7; backward 8 x
 // 2048 x 2048 167 and 171; 1 x 131072 x 512 bfloat16 237 and 244).
+// Backward over segments takes four waves of two and twice the blocks, whose waits overlap freely (5
+// x 1537 x 333 bfloat16 15.0 us, 18.5 with eight waves; 1 x 5824 x 955 22.7 and 24.2; 1 x 131072 x
+// 512 199 and 200; forward gains nothing).
 constexpr int kWaves = 8;
+constexpr int waves_of(int values, bool back, bool split) {
+  return back && split && values != 1 ? 4 : kWaves;
+}
 constexpr int steps_of(int values, bool back) { return (values == 1 ? 8 : 4) / (back ? 2 : 1); }
 
 // A tile takes about as long as 9 MB moved (3 us), a second launch as two tiles, and it reads half
@@ -494,8 +500,8 @@ Plan plan_of(uint64_t batch, uint64_t time, uint64_t channels, uint64_t element,
     p.groups = static_cast<uint32_t>((channels + lanes * p.values - 1) / (lanes * p.values));
     return batch * p.groups;
   };
-  auto tiles = [&](uint64_t &tile) {
-    tile = 64 / p.lanes * kWaves * steps_of(p.values, back);
+  auto tiles = [&](bool split, uint64_t &tile) {
+    tile = 64 / p.lanes * waves_of(p.values, back, split) * steps_of(p.values, back);
     return (time + tile - 1) / tile;
   };
   p.segments = 1;
@@ -514,10 +520,15 @@ Plan plan_of(uint64_t batch, uint64_t time, uint64_t channels, uint64_t element,
   if (p.brief || blocks >= units) return p;
   uint64_t tile;
   if (p.values == 4 && blocks * 2 < units) across(8);
-  if (tiles(tile) <= 2 + batch * time * channels * element / (3u << 20)) return p;
+  if (tiles(false, tile) <= 2 + batch * time * channels * element / (3u << 20)) return p;
   across(lanes);
-  const uint64_t all = tiles(tile);
-  const uint64_t wanted = std::min((2 * units + blocks - 1) / blocks, all);
+  const uint64_t all = tiles(true, tile);
+  // at most 256 segments, whose maps a block goes through (backward 1 x 30000 x 100 float32: 24 us,
+  // 28 with 469)
+  const uint64_t per_unit = 16 / waves_of(p.values, back, true);
+  const uint64_t wanted =
+      std::min({(per_unit * units + blocks - 1) / blocks, all, uint64_t{256}});
+  if (wanted < 2) return p;
   const uint64_t per = (all + wanted - 1) / wanted;
   p.steps = static_cast<uint32_t>(per * tile);
   p.segments = static_cast<uint32_t>((all + per - 1) / per);
@@ -528,13 +539,13 @@ uint64_t parts_bytes(const Plan &p, uint64_t batch, uint64_t channels) {
   return p.segments == 1 ? 0 : batch * (p.segments + 1) * 2 * channels * 4;
 }
 
-template <typename T, int V, int Lanes, bool Back, bool Ragged>
-oxh_status run_split(hipStream_t stream, uint64_t batch, Args<T> a, const char *what) {
+template <typename T, int V, int Lanes, bool Back, bool Ragged, int W>
+oxh_status run_tiles(hipStream_t stream, uint64_t batch, Args<T> a, const char *what) {
   constexpr int S = steps_of(V, Back);
   const uint64_t blocks = batch * a.groups * a.segments;
   if (a.segments > 1) {
-    oxh::launch(recurrence_parts_kernel<T, V, Lanes, kWaves, S, Back, Ragged>,
-                dim3(static_cast<uint32_t>(blocks)), dim3(64 * kWaves), 0, stream, a);
+    oxh::launch(recurrence_parts_kernel<T, V, Lanes, W, S, Back, Ragged>,
+                dim3(static_cast<uint32_t>(blocks)), dim3(64 * W), 0, stream, a);
     oxh_status st = oxh::launched(what);
     if (st != OXH_OK) return st;
   }
@@ -546,14 +557,22 @@ oxh_status run_split(hipStream_t stream, uint64_t batch, Args<T> a, const char *
   const uint64_t moved = batch * a.time * a.channels * sizeof(T) * (Back ? 6 : 3);
   if constexpr (V == 4 && Lanes == 16) {
     if (moved > kCached && a.lines) {
-      oxh::launch(recurrence_kernel<T, V, Lanes, kWaves, S, Back, Ragged, true>,
-                  dim3(static_cast<uint32_t>(blocks)), dim3(64 * kWaves), 0, stream, a);
+      oxh::launch(recurrence_kernel<T, V, Lanes, W, S, Back, Ragged, true>,
+                  dim3(static_cast<uint32_t>(blocks)), dim3(64 * W), 0, stream, a);
       return oxh::launched(what);
     }
   }
-  oxh::launch(recurrence_kernel<T, V, Lanes, kWaves, S, Back, Ragged>,
-              dim3(static_cast<uint32_t>(blocks)), dim3(64 * kWaves), 0, stream, a);
+  oxh::launch(recurrence_kernel<T, V, Lanes, W, S, Back, Ragged>,
+              dim3(static_cast<uint32_t>(blocks)), dim3(64 * W), 0, stream, a);
   return oxh::launched(what);
+}
+
+template <typename T, int V, int Lanes, bool Back, bool Ragged>
+oxh_status run_split(hipStream_t stream, uint64_t batch, const Args<T> &a, const char *what) {
+  constexpr int kWhole = waves_of(V, Back, false), kSplit = waves_of(V, Back, true);
+  if (kSplit != kWhole && a.segments > 1)
+    return run_tiles<T, V, Lanes, Back, Ragged, kSplit>(stream, batch, a, what);
+  return run_tiles<T, V, Lanes, Back, Ragged, kWhole>(stream, batch, a, what);
 }
 
 template <typename T, bool Back, int V, bool Ragged>
