@@ -472,11 +472,10 @@ struct Plan {
 
 // Waves per block, and steps per thread and tile.  Eight waves of four steps (backward: two) hold
 // the bytes in flight of four waves of eight in half the registers each, and more of them hide more
-// (forward 8 x 2048 x 2048 float32 87 us, 94 with four; 10 x 356 x 855 12.6 and 15.7; backward 8 x
-// 2048 x 2048 167 and 171; 1 x 131072 x 512 bfloat16 237 and 244).
-// Backward over segments takes four waves of two and twice the blocks, whose waits overlap freely (5
-// x 1537 x 333 bfloat16 15.0 us, 18.5 with eight waves; 1 x 5824 x 955 22.7 and 24.2; 1 x 131072 x
-// 512 199 and 200; forward gains nothing).
+// (forward 8 x 2048 x 2048 float32 87 us, 94 with four; 10 x 356 x 855 12.6 and 15.7; over segments
+// 5 x 1537 x 333 bfloat16 14.2 and 14.6; backward 8 x 2048 x 2048 float32 167 and 171).  Backward
+// over segments takes four waves of two and twice the blocks, whose waits overlap freely (5 x 1537 x
+// 333 15.6 us, 18.3 with eight waves; 1 x 5824 x 955 23.1 and 24.2; 1 x 131072 x 512 198 and 200).
 constexpr int kWaves = 8;
 constexpr int waves_of(int values, bool back, bool split) {
   return back && split && values != 1 ? 4 : kWaves;
@@ -490,8 +489,8 @@ constexpr int steps_of(int values, bool back) { return (values == 1 ? 8 : 4) / (
 // 5 x 1537 x 333 bfloat16, 7 tiles: 23.7 and 14.2; 1 x 4096 x 2048 float32, 16 tiles: 41 and 30);
 // there 32 channels per block where 64 leave more than half of the units without (8 x 2048 x 512,
 // 64 blocks: 24.6 and 39; 10 x 356 x 855, 140 blocks: 15.4 and 12.6).  Otherwise it is split for
-// two blocks per unit, a tile at least per segment (3 x 700 x 130: 10.5 us with one, 16.3 with
-// two).
+// two blocks of eight waves per unit, or four of four, a tile at least per segment (3 x 700 x 130:
+// 10.5 us with one, 16.3 with two).
 Plan plan_of(uint64_t batch, uint64_t time, uint64_t channels, uint64_t element, bool back) {
   Plan p;
   p.values = channels < 4 ? 1 : 4;
