@@ -474,8 +474,9 @@ struct Plan {
 // the bytes in flight of four waves of eight in half the registers each, and more of them hide more
 // (forward 8 x 2048 x 2048 float32 87 us, 94 with four; 10 x 356 x 855 12.6 and 15.7; over segments
 // 5 x 1537 x 333 bfloat16 14.2 and 14.6; backward 8 x 2048 x 2048 float32 167 and 171).  Backward
-// over segments takes four waves of two and twice the blocks, whose waits overlap freely (5 x 1537 x
-// 333 15.6 us, 18.3 with eight waves; 1 x 5824 x 955 23.1 and 24.2; 1 x 131072 x 512 198 and 200).
+// over segments takes four waves of two and twice the blocks, whose waits overlap freely (5 x 1537
+// x 333 15.6 us, 18.3 with eight waves; 1 x 5824 x 955 23.1 and 24.2; 1 x 131072 x 512 198 and
+// 200).
 constexpr int kWaves = 8;
 constexpr int waves_of(int values, bool back, bool split) {
   return back && split && values != 1 ? 4 : kWaves;
