@@ -28,7 +28,8 @@
 // 4096 x 4096 in 4.1 ms, 335 TFLOP/s or 1005 of float16 (a library's largest float16 products reach
 // 1092 here); 12 x 512 x 2048 in 612 us (three launches a round, which leave the cores a part of
 // the time), and 1000 x 1280 in 225 us, where each of 17 launches takes 9 to 18 us: 136 tiles on
-// 256 compute units, each a chain of loads.  Matrices that fit one compute unit take none of it.
+// 256 compute units, each a chain of loads.  Short sides of up to 128 take fewer launches: one for
+// a matrix that a compute unit holds, seven in slabs of its columns.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -64,6 +65,7 @@ struct Matrix {
   float *momentum;  // null: orthogonalize
   float *target;    // the parameter, or the output
   char *scratch;
+  uint64_t parts;  // offset of the norm's partial sums
   uint32_t rows, columns, ps, pl;
   uint32_t first_block;  // of this launch
   float scale;
@@ -158,7 +160,7 @@ __global__ __launch_bounds__(kNormThreads) void muon_norm_kernel(Group g) {
     float total = 0.0f;
 #pragma unroll
     for (int w = 0; w < kNormThreads / 64; ++w) total += wave[w];
-    reinterpret_cast<float *>(m.scratch + layout_of(m.ps, m.pl).parts)[part] = total;
+    reinterpret_cast<float *>(m.scratch + m.parts)[part] = total;
   }
 }
 
@@ -665,8 +667,26 @@ __device__ __forceinline__ void multiply(const f16x8 (&a)[2], const f16x8 (&b)[2
   acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[0], b[0], acc, 0, 0, 0);
 }
 
-template <int PS, int Blocks>
-__global__ __launch_bounds__(64 * kWholeWaves) void muon_whole_kernel(Group g, uint32_t rounds) {
+//
+// Slab: the same for a matrix of too many columns, in slabs of 12 x 16 of them, a block each, and a
+// launch for each round: it adds the slabs' shares of A in order, takes its columns of X through B,
+// and leaves its share of the next A.  Launch 0 makes X, launch `rounds` the result.
+constexpr uint32_t kSlabColumns = 16 * kWholeWaves;
+struct SlabLayout {
+  uint64_t shares, parts, total;  // X lies first
+};
+__host__ __device__ inline SlabLayout slab_layout(uint64_t ps, uint64_t slabs) {
+  const uint64_t side = ps / 32, tiles = side * (side + 1) / 2;
+  SlabLayout l;
+  l.shares = slabs * ps * kSlabColumns * 4;
+  l.parts = l.shares + 2 * slabs * tiles * 4096;
+  l.total = l.parts + kNormParts * 4;
+  return l;
+}
+
+template <int PS, int Blocks, bool Slab>
+__global__ __launch_bounds__(64 * kWholeWaves) void muon_whole_kernel(Group g, uint32_t rounds,
+                                                                      uint32_t round) {
   __shared__ __attribute__((aligned(16))) char shared[kWhole];
   float *const parts = reinterpret_cast<float *>(shared + kWhole - 4 * kWholeWaves);
   constexpr int kRowBlocks = PS / 16, kPitch = whole_pitch(PS), kSquare = square_pitch(PS);
@@ -679,12 +699,29 @@ __global__ __launch_bounds__(64 * kWholeWaves) void muon_whole_kernel(Group g, u
   constexpr int kSums = kSplits > 1 ? kTiles * 4 * kSplits * 1024 : 0;
   char *const sums = shared, *const sa = shared + kSums, *const sb = sa + square_bytes(PS);
   static_assert(kSums + 2 * square_bytes(PS) <= kWhole, "shared memory");
-  const Matrix &m = g.m[blockIdx.x];
+  const Matrix &m = Slab ? matrix_of(g, blockIdx.x) : g.m[blockIdx.x];
   const bool tall = m.rows > m.columns;
-  const uint32_t s = tall ? m.columns : m.rows, n = tall ? m.rows : m.columns;
+  const uint32_t s = tall ? m.columns : m.rows, n_all = tall ? m.rows : m.columns;
+  const uint32_t slab = Slab ? blockIdx.x - m.first_block : 0, column0 = slab * kSlabColumns;
+  const uint32_t n = Slab ? min(n_all - column0, kSlabColumns) : n_all;
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t col = lane & 15, quad = lane >> 4;
   const uint32_t column_blocks = (n + 31) / 32 * 2;
+  f32x4 x[Blocks][kRowBlocks];
+  // Slab: X as the threads hold it; the shares of A, of even and of odd launches
+  const uint32_t slabs = (n_all + kSlabColumns - 1) / kSlabColumns;
+  const SlabLayout sl = slab_layout(PS, slabs);
+  f32x4 *const kept_x = reinterpret_cast<f32x4 *>(m.scratch) +
+                        slab * kRowBlocks * 64 * kWholeWaves + threadIdx.x;
+  auto shares = [&](uint32_t launch, uint32_t of) {
+    return reinterpret_cast<f32x4 *>(m.scratch + sl.shares) +
+           ((launch & 1) * slabs + of) * kTiles * 4 * 64 + lane;
+  };
+  // offset of (i, j) of X in the matrix
+  auto place = [&](uint32_t i, uint32_t j) {
+    return tall ? static_cast<uint64_t>(column0 + j) * m.columns + i
+                : static_cast<uint64_t>(i) * m.columns + column0 + j;
+  };
   // The matrix lies in the shared memory as in memory, its rows an odd number of words apart, on
   // the way in and out.  A thread moves kBatch of its elements at a time: load(b, offset in memory)
   // for each, then use(b, offset there, offset in memory).
@@ -717,6 +754,30 @@ __global__ __launch_bounds__(64 * kWholeWaves) void muon_whole_kernel(Group g, u
   };
   const uint32_t step_i = tall ? 1 : pitch, step_j = tall ? pitch : 1;
 
+  if constexpr (Slab) {
+    if (round != 0) {
+#pragma unroll
+      for (int r = 0; r < kRowBlocks; ++r) x[0][r] = kept_x[r * 64 * kWholeWaves];
+    } else {
+      const float *norms = reinterpret_cast<const float *>(m.scratch + sl.parts);
+      float one[1] = {threadIdx.x < kNormParts ? norms[threadIdx.x] : 0.0f};
+      oxh::wave_sums_rows(one);
+      if (lane == 0) parts[wave] = one[0];
+      __syncthreads();
+      float total = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWholeWaves; ++w) total += parts[w];
+      const float inverse = 1.0f / (sqrtf(total) + g.epsilon);
+      const uint32_t j = wave * 16 + col;
+#pragma unroll
+      for (int r = 0; r < kRowBlocks; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t i = 16 * r + 4 * quad + e;
+          x[0][r][e] = i < s && j < n ? direction(g, m, place(i, j)) * inverse : 0.0f;
+        }
+    }
+  } else {
   float squares = 0.0f, grad[kBatch], mom[kBatch];
   each([&](int b, uint32_t at) {
     grad[b] = m.gradient[at];
@@ -739,7 +800,6 @@ __global__ __launch_bounds__(64 * kWholeWaves) void muon_whole_kernel(Group g, u
 #pragma unroll
   for (int w = 0; w < kWholeWaves; ++w) total += parts[w];
   const float inverse = 1.0f / (sqrtf(total) + g.epsilon);
-  f32x4 x[Blocks][kRowBlocks];
 #pragma unroll
   for (int c = 0; c < Blocks; ++c) {
     const uint32_t j = (c * kWholeWaves + wave) * 16 + col;
@@ -753,6 +813,7 @@ __global__ __launch_bounds__(64 * kWholeWaves) void muon_whole_kernel(Group g, u
     __builtin_amdgcn_sched_barrier(0);
   }
   __syncthreads();
+  }
 
   // this wave's tile of A and its share of the sum
   const uint32_t tile = wave % kTiles, split = wave / kTiles;
@@ -760,7 +821,12 @@ __global__ __launch_bounds__(64 * kWholeWaves) void muon_whole_kernel(Group g, u
   while ((ti + 1) * (ti + 2) / 2 <= tile) ++ti;
   const uint32_t tj = tile - ti * (ti + 1) / 2;
 
-  for (uint32_t round = 0; round < rounds; ++round) {
+  // this wave's blocks of A, and the first one's place in the tile
+  f32x4 own[kOwnRows][kOwnColumns];
+  const uint32_t i0 = kShare == 1 ? 0 : kShare == 2 ? split : split >> 1;
+  const uint32_t j0 = kShare == 4 ? split & 1 : 0;
+  // own = the products of X's columns here
+  auto gram = [&]() {
 #pragma unroll
     for (int c = 0; c < Blocks; ++c) {
       const uint32_t block = c * kWholeWaves + wave;
@@ -802,10 +868,6 @@ __global__ __launch_bounds__(64 * kWholeWaves) void muon_whole_kernel(Group g, u
       }
     }
     __syncthreads();
-    // this wave's blocks of A, and the first one's place in the tile
-    f32x4 own[kOwnRows][kOwnColumns];
-    const uint32_t i0 = kShare == 1 ? 0 : kShare == 2 ? split : split >> 1;
-    const uint32_t j0 = kShare == 4 ? split & 1 : 0;
     if constexpr (kSplits > 1) {
       f32x4 *slot = reinterpret_cast<f32x4 *>(sums) + tile * 4 * kSplits * 64 + lane;
       if (split < kSplits) {
@@ -827,6 +889,9 @@ __global__ __launch_bounds__(64 * kWholeWaves) void muon_whole_kernel(Group g, u
 #pragma unroll
       for (int q = 0; q < 4; ++q) own[q >> 1][q & 1] = acc[q >> 1][q & 1];
     }
+  };
+  // X = a X + (b A + c A A) X
+  auto apply = [&]() {
     // block (i, j) of this wave's tile of A or B to the columns' rows of `to` and, off the
     // diagonal, to the rows' rows: there two lanes with neighbouring columns share their four rows'
     // words
@@ -915,6 +980,47 @@ __global__ __launch_bounds__(64 * kWholeWaves) void muon_whole_kernel(Group g, u
       __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();
+  };
+  if constexpr (Slab) {
+    auto each_own = [&](auto use) {
+      if (split >= kShare) return;
+#pragma unroll
+      for (int i = 0; i < kOwnRows; ++i)
+#pragma unroll
+        for (int j = 0; j < kOwnColumns; ++j)
+          use(own[i][j], (tile * 4 + (i0 + i) * 2 + j0 + j) * 64);
+    };
+    if (round != 0) {
+      each_own([&](f32x4 &sum, uint32_t at) {
+        sum = shares(round + 1, 0)[at];
+#pragma unroll 8
+        for (uint32_t p = 1; p < slabs; ++p) sum += shares(round + 1, p)[at];
+      });
+      apply();
+    }
+    if (round != rounds) {
+#pragma unroll
+      for (int r = 0; r < kRowBlocks; ++r) kept_x[r * 64 * kWholeWaves] = x[0][r];
+      gram();
+      each_own([&](f32x4 &share, uint32_t at) { shares(round, slab)[at] = share; });
+    } else {
+      const uint32_t j = wave * 16 + col;
+#pragma unroll
+      for (int r = 0; r < kRowBlocks; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t i = 16 * r + 4 * quad + e;
+          if (i >= s || j >= n) continue;
+          float *to = m.target + place(i, j);
+          *to = m.momentum == nullptr ? x[0][r][e]
+                                      : *to - g.lr * (g.decay * *to + m.scale * x[0][r][e]);
+        }
+    }
+    return;
+  }
+  for (uint32_t turn = 0; turn < rounds; ++turn) {
+    gram();
+    apply();
   }
   uint32_t again = col;  // so that no offset is kept from the way in
   asm volatile("" : "+v"(again));
@@ -952,16 +1058,26 @@ struct Item {
 uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
 
 // Whether one block steps the whole matrix: the rows of the shared memory that hold X', and at most
-// this many column blocks per wave (one matrix of 96 x 192 38 us, 72 in launches; of 96 x 384 67
-// and 75; of 128 x 192 58 and 73; of 128 x 256, whose two column blocks spill, 116 and 74, 16 of
-// them 117 and 140).
-constexpr int whole_blocks(int ps) { return ps == 32 ? 6 : ps == 64 ? 3 : ps == 96 ? 2 : 1; }
+// this many column blocks per wave (one matrix of 96 x 192 38 us, 72 in tiles; of 64 x 384 45, 47 in
+// slabs; of 128 x 192 58, 73 in tiles; of 96 x 384 and 128 x 256, whose two column blocks spill, 92
+// and 116, and 60 in slabs and 74 in tiles).
+constexpr int whole_blocks(int ps) { return ps == 32 ? 6 : ps == 64 ? 3 : 1; }
 bool whole(const Item &it) {
   const uint64_t s = std::min(it.rows, it.columns), n = std::max(it.rows, it.columns);
   if (s > 128) return false;
   const int ps = static_cast<int>(round_up(s, 32));
   return round_up(n, 32) * whole_pitch(ps) <= kWhole - 4 * kWholeWaves &&
          round_up(n, 32) <= 16ull * kWholeWaves * whole_blocks(ps);
+}
+
+// Whether a matrix goes in slabs: 7 launches in place of the tiles' 17, but the least work per launch
+// is a slab's round, and every block adds all slabs' shares (64 x 1000: 50 us, 84 in tiles; 20 x
+// 10000: 48 and 247; four of 69 x 2045: 85 and 128; 128 x 512: 92 and 80; 128 x 2000: 107 and 108;
+// 128 x 19000: 280 and 434).
+constexpr uint64_t kMostSlabs = 100;
+bool slabbed(const Item &it) {
+  const uint64_t s = std::min(it.rows, it.columns), n = std::max(it.rows, it.columns);
+  return (s <= 96 || (s <= 128 && n >= 2048)) && n <= kMostSlabs * kSlabColumns;
 }
 
 // Tile sides of a launch group: `square` of A and B, of which the tiles on and below the diagonal
@@ -1024,20 +1140,53 @@ uint64_t scratch_of(const Item *items, size_t count) {
   return total;
 }
 
-// The matrices that one block does not take, and those it takes.
+// The matrices that one block takes, those that go in slabs, and the others.
 struct Parted {
-  std::vector<Item> large, small;
+  std::vector<Item> large, slabs, small;
 };
 Parted part(const std::vector<Item> &items) {
   Parted p;
-  for (const Item &it : items) (whole(it) ? p.small : p.large).push_back(it);
+  for (const Item &it : items)
+    (whole(it) ? p.small : slabbed(it) ? p.slabs : p.large).push_back(it);
   return p;
 }
 
-uint64_t scratch_of_all(const std::vector<Item> &large) {
+uint64_t side_of(const Item &it) { return round_up(std::min(it.rows, it.columns), 32); }
+uint64_t slabs_of(const Item &it) {
+  return (std::max(it.rows, it.columns) + kSlabColumns - 1) / kSlabColumns;
+}
+// Calls run(group) with the slabbed matrices of this side, a launch group at a time.
+template <typename Run>
+oxh_status slab_groups(const std::vector<Item> &slabs, uint64_t side, Run run) {
+  std::vector<Item> group;
+  auto flush = [&]() {
+    if (group.empty()) return oxh::ok();
+    const oxh_status st = run(group);
+    group.clear();
+    return st;
+  };
+  for (const Item &it : slabs) {
+    if (side_of(it) != side) continue;
+    group.push_back(it);
+    if (group.size() < kGroup) continue;
+    oxh_status st = flush();
+    if (st != OXH_OK) return st;
+  }
+  return flush();
+}
+
+uint64_t scratch_of_all(const Parted &items) {
   uint64_t most = 0;
+  const std::vector<Item> &large = items.large;
   for (size_t at = 0; at < large.size(); at += kGroup)
     most = std::max(most, scratch_of(&large[at], std::min<size_t>(kGroup, large.size() - at)));
+  for (uint64_t side = 32; side <= 128; side += 32)
+    slab_groups(items.slabs, side, [&](const std::vector<Item> &group) {
+      uint64_t total = 0;
+      for (const Item &it : group) total += round_up(slab_layout(side, slabs_of(it)).total, 256);
+      most = std::max(most, total);
+      return oxh::ok();
+    });
   return most;
 }
 
@@ -1062,11 +1211,15 @@ oxh_status product(hipStream_t stream, Group &g, uint32_t tile, int odd, const c
   return oxh::launched(what);
 }
 
-oxh_status run_group(hipStream_t stream, Group &g, const Tiles &tiles, uint32_t rounds) {
+oxh_status run_norm(hipStream_t stream, Group &g) {
   g.blocks = 0;
   for (uint32_t i = 0; i < g.count; ++i) g.m[i].first_block = g.blocks, g.blocks += kNormParts;
   oxh::launch(muon_norm_kernel, dim3(g.blocks), dim3(kNormThreads), 0, stream, g);
-  oxh_status st = oxh::launched("muon_norm");
+  return oxh::launched("muon_norm");
+}
+
+oxh_status run_group(hipStream_t stream, Group &g, const Tiles &tiles, uint32_t rounds) {
+  oxh_status st = run_norm(stream, g);
   if (st != OXH_OK) return st;
   g.blocks = 0;
   for (uint32_t i = 0; i < g.count; ++i) {
@@ -1107,8 +1260,8 @@ oxh_status run_whole(hipStream_t stream, const std::vector<Item> &small, Group g
   g.count = 0;
   auto flush = [&]() {
     if (g.count == 0) return oxh::ok();
-    oxh::launch(muon_whole_kernel<PS, Blocks>, dim3(g.count), dim3(64 * kWholeWaves), 0, stream, g,
-                rounds);
+    oxh::launch(muon_whole_kernel<PS, Blocks, false>, dim3(g.count), dim3(64 * kWholeWaves), 0,
+                stream, g, rounds, 0u);
     g.count = 0;
     return oxh::launched("muon_whole");
   };
@@ -1123,6 +1276,35 @@ oxh_status run_whole(hipStream_t stream, const std::vector<Item> &small, Group g
     }
   }
   return flush();
+}
+
+// The slabbed matrices of this side.
+template <int PS>
+oxh_status run_slabs(hipStream_t stream, const std::vector<Item> &slabs, Group g, uint32_t rounds,
+                     char *workspace) {
+  return slab_groups(slabs, PS, [&](const std::vector<Item> &group) {
+    g.count = static_cast<uint32_t>(group.size());
+    uint64_t offset = 0;
+    for (uint32_t i = 0; i < g.count; ++i) {
+      const SlabLayout l = slab_layout(PS, slabs_of(group[i]));
+      describe(group[i], g.m[i]);
+      g.m[i].scratch = workspace + offset;
+      g.m[i].parts = l.parts;
+      offset += round_up(l.total, 256);
+    }
+    oxh_status st = run_norm(stream, g);
+    uint32_t blocks = 0;
+    for (uint32_t i = 0; i < g.count; ++i) {
+      g.m[i].first_block = blocks;
+      blocks += static_cast<uint32_t>(slabs_of(group[i]));
+    }
+    for (uint32_t round = 0; round <= rounds && st == OXH_OK; ++round) {
+      oxh::launch(muon_whole_kernel<PS, 1, true>, dim3(blocks), dim3(64 * kWholeWaves), 0, stream,
+                  g, rounds, round);
+      st = oxh::launched("muon_slab");
+    }
+    return st;
+  });
 }
 
 oxh_status run_all(hipStream_t stream, const Parted &items, const Hyper &h, uint32_t rounds,
@@ -1141,8 +1323,13 @@ oxh_status run_all(hipStream_t stream, const Parted &items, const Hyper &h, uint
     if (st == OXH_OK) st = run_whole<64, 1>(stream, small, g, rounds);
     if (st == OXH_OK) st = run_whole<64, whole_blocks(64)>(stream, small, g, rounds);
     if (st == OXH_OK) st = run_whole<96, 1>(stream, small, g, rounds);
-    if (st == OXH_OK) st = run_whole<96, whole_blocks(96)>(stream, small, g, rounds);
     if (st == OXH_OK) st = run_whole<128, 1>(stream, small, g, rounds);
+  }
+  if (!items.slabs.empty()) {
+    if (st == OXH_OK) st = run_slabs<32>(stream, items.slabs, g, rounds, workspace);
+    if (st == OXH_OK) st = run_slabs<64>(stream, items.slabs, g, rounds, workspace);
+    if (st == OXH_OK) st = run_slabs<96>(stream, items.slabs, g, rounds, workspace);
+    if (st == OXH_OK) st = run_slabs<128>(stream, items.slabs, g, rounds, workspace);
   }
   for (size_t at = 0; at < large.size() && st == OXH_OK; at += kGroup) {
     const size_t count = std::min<size_t>(kGroup, large.size() - at);
@@ -1157,6 +1344,7 @@ oxh_status run_all(hipStream_t stream, const Parted &items, const Hyper &h, uint
       m.scratch = workspace + offset;
       m.ps = static_cast<uint32_t>(round_up(std::min(it.rows, it.columns), pad));
       m.pl = static_cast<uint32_t>(round_up(std::max(it.rows, it.columns), pad));
+      m.parts = layout_of(m.ps, m.pl).parts;
       offset += round_up(layout_of(m.ps, m.pl).total, 256);
     }
     st = run_group(stream, g, tiles, rounds);
@@ -1217,7 +1405,7 @@ oxh_status oxh_orthogonalize_workspace_size(uint64_t count, uint64_t rows, uint6
     if (st != OXH_OK) return st;
     OXH_REQUIRE(count <= 65536, OXH_INVALID_SHAPE, "orthogonalize: too many matrices");
     *bytes = scratch_of_all(
-        part(std::vector<Item>(count, Item{nullptr, nullptr, nullptr, rows, columns})).large);
+        part(std::vector<Item>(count, Item{nullptr, nullptr, nullptr, rows, columns})));
     return oxh::ok();
   });
 }
@@ -1259,7 +1447,7 @@ oxh_status oxh_muon_workspace_size(const oxh_muon_tensor *tensors, uint32_t coun
     std::vector<Item> items;
     oxh_status st = items_of(tensors, count, items);
     if (st != OXH_OK) return st;
-    *bytes = scratch_of_all(part(items).large);
+    *bytes = scratch_of_all(part(items));
     return oxh::ok();
   });
 }
@@ -1280,7 +1468,7 @@ oxh_status oxh_muon_multi_tensor(oxh_stream stream, float learning_rate, float w
     if (st != OXH_OK) return st;
     if (count == 0) return oxh::ok();
     const Parted parted = part(items);
-    const uint64_t needed = scratch_of_all(parted.large);
+    const uint64_t needed = scratch_of_all(parted);
     st = check_workspace(needed, workspace, workspace_bytes);
     if (st != OXH_OK) return st;
     // every written range against every other range: sorted by address, neighbours may not meet

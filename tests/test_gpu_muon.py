@@ -192,3 +192,59 @@ def test_large(module, dev, shape):
     assert torch.equal(m, v)
     tol = BOUND * moved.norm() + 4 * 2.0 ** -24 * want.norm()
     assert (p.double() - want).norm() <= tol
+
+
+# short sides of up to 128 with more columns than one block takes
+SLABS = [(87, 1091), (1091, 87), (1, 4000), (20, 1500), (32, 1025), (64, 700), (700, 61), (96, 193),
+         (193, 96), (90, 384), (385, 70), (128, 2049), (2500, 100), (96, 19200), (33, 19201)]
+
+
+@pytest.mark.parametrize("shape", SLABS)
+@pytest.mark.parametrize("rounds", [1, 2, 5])
+def test_slabs(module, dev, shape, rounds):
+    v = matrix(shape, 13)
+    x, out = torch.from_numpy(v).to(dev), torch.empty(shape, device=dev)
+    module.orthogonalize(x, out, rounds=rounds)
+    ref = orthogonal_on(x.double(), rounds).cpu().numpy()
+    close(out, ref, A ** rounds * 2.0 ** -22 if rounds == 5 else A ** rounds * 2.0 ** -20)
+
+
+def test_step_of_every_kind(module, dev):
+    """One list with matrices that a block takes, that go in slabs (more than a launch group of one
+    side, and of several) and in tiles; each moves as it does alone, and a replay repeats it."""
+    shapes = [(30, 40), (128, 150), (300, 310), (128, 600), (90, 700), (2100, 120)] + \
+        [(64, 600 + 7 * i) for i in range(34)] + [(1300, 33)]
+    r = np.random.default_rng(14)
+    start = [[torch.from_numpy(r.standard_normal(s).astype(np.float32) * k).to(dev)
+              for s in shapes] for k in (0.05, 1e-3, 1e-2)]
+    alone = [[t.clone() for t in ts] for ts in start]
+    for one in zip(*alone):
+        module.muon(0.02, 0.01, 0.9, [one])
+    for i, (p, g, m) in enumerate(zip(*start)):
+        want = orthogonal_on((g + 0.9 * (0.9 * m + g)).double())
+        scale = math.sqrt(max(1.0, shapes[i][0] / shapes[i][1]))
+        moved = 0.02 * (0.01 * p.double() + scale * want)
+        off = (alone[0][i].double() - (p.double() - moved)).norm()
+        assert off <= BOUND * moved.norm() + 4 * 2.0 ** -24 * p.double().norm(), shapes[i]
+    p, g, m = ([t.clone() for t in ts] for ts in start)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def step():
+        module.muon(0.02, 0.01, 0.9, list(zip(p, g, m)), stream=stream)
+
+    step()
+    torch.cuda.synchronize()
+    graph = ox.HipGraphExec.capture(stream, step)
+    for _ in range(2):
+        for now, then in zip((p, g, m), start):
+            for a, b in zip(now, then):
+                a.copy_(b)
+        torch.cuda.synchronize()
+        graph.launch(stream)
+        torch.cuda.synchronize()
+        for a, b in zip(p + m, alone[0] + alone[2]):
+            # tiles are chosen for a list, so (128, 600) and (300, 310) may differ in rounding
+            assert (a - b).norm() <= 1e-5 * b.norm()
+            if a.shape[0] not in (128, 300):
+                assert torch.equal(a, b)
