@@ -633,10 +633,10 @@ __global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int 
 // and transposed reads of the shared memory (16 lanes fetch 4 rows of 16 float16 and each gets a
 // column of 4) give the same order for X X'.
 //
-// The bound is one compute unit's shared memory and its barriers: of the 88000 cycles that 96 x 192
-// takes (38 us), a round is 14500: X X' 3000 (its operands are 2250 of the shared memory's), A and A
-// A 4600 with their halves, shared among the waves that summed a tile, B X 4700 (3400), X' in halves
-// 2000.  The way in is 14000: twelve loads at a time, 7000 where eight took 9300.
+// The bound is one compute unit's shared memory and its barriers: of the 88000 cycles that 96 x
+// 192 takes (38 us), a round is 14500: X X' 3000 (its operands are 2250 of the shared memory's), A
+// and A A 4600 with their halves, shared among the waves that summed a tile, B X 4700 (3400), X' in
+// halves 2000.  The way in is 14000: twelve loads at a time, 7000 where eight took 9300.
 
 constexpr int kWhole = 163840;  // bytes of shared memory, the last for the norm's parts
 constexpr int kWholeWaves = 12;
@@ -1058,9 +1058,9 @@ struct Item {
 uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
 
 // Whether one block steps the whole matrix: the rows of the shared memory that hold X', and at most
-// this many column blocks per wave (one matrix of 96 x 192 38 us, 72 in tiles; of 64 x 384 45, 47 in
-// slabs; of 128 x 192 58, 73 in tiles; of 96 x 384 and 128 x 256, whose two column blocks spill, 92
-// and 116, and 60 in slabs and 74 in tiles).
+// this many column blocks per wave (one matrix of 96 x 192 38 us, 72 in tiles; of 64 x 384 45, 47
+// in slabs; of 128 x 192 58, 73 in tiles; of 96 x 384 and 128 x 256, whose two column blocks spill,
+// 92 and 116, and 60 in slabs and 74 in tiles).
 constexpr int whole_blocks(int ps) { return ps == 32 ? 6 : ps == 64 ? 3 : 1; }
 bool whole(const Item &it) {
   const uint64_t s = std::min(it.rows, it.columns), n = std::max(it.rows, it.columns);
@@ -1070,10 +1070,10 @@ bool whole(const Item &it) {
          round_up(n, 32) <= 16ull * kWholeWaves * whole_blocks(ps);
 }
 
-// Whether a matrix goes in slabs: 7 launches in place of the tiles' 17, but the least work per launch
-// is a slab's round, and every block adds all slabs' shares (64 x 1000: 50 us, 84 in tiles; 20 x
-// 10000: 48 and 247; four of 69 x 2045: 85 and 128; 128 x 512: 92 and 80; 128 x 2000: 107 and 108;
-// 128 x 19000: 280 and 434).
+// Whether a matrix goes in slabs: 7 launches in place of the tiles' 17, but the least work per
+// launch is a slab's round, and every block adds all slabs' shares (64 x 1000: 50 us, 84 in tiles;
+// 20 x 10000: 48 and 247; four of 69 x 2045: 85 and 128; 128 x 512: 92 and 80; 128 x 2000: 107 and
+// 108; 128 x 19000: 280 and 434).
 constexpr uint64_t kMostSlabs = 100;
 bool slabbed(const Item &it) {
   const uint64_t s = std::min(it.rows, it.columns), n = std::max(it.rows, it.columns);
