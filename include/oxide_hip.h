@@ -70,6 +70,8 @@ oxh_status oxh_device_count(int *count);
 oxh_status oxh_stream_create(oxh_stream *stream);
 oxh_status oxh_stream_destroy(oxh_stream stream);
 oxh_status oxh_stream_synchronize(oxh_stream stream);
+/* Whether what is enqueued on the stream is being recorded into a graph. */
+oxh_status oxh_stream_is_capturing(oxh_stream stream, int *capturing);
 
 /* DeviceBuffer::{zeroed, uninitialized_async, from_host, copy_from_host_async_unchecked,
  * to_host_vec} (runtime.rs:83-105, cuda/jit.rs:34-45,93,97). */

@@ -86,6 +86,16 @@ oxh_status oxh_stream_synchronize(oxh_stream stream) {
   return oxh::ok();
 }
 
+oxh_status oxh_stream_is_capturing(oxh_stream stream, int *capturing) {
+  OXH_REQUIRE(capturing != nullptr, OXH_INVALID_SHAPE, "capturing is null");
+  *capturing = 0;
+  if (stream == nullptr) return oxh::ok();  // cannot be captured
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  OXH_HIP_CHECK(hipStreamIsCapturing(oxh::as_stream(stream), &status));
+  *capturing = status != hipStreamCaptureStatusNone;
+  return oxh::ok();
+}
+
 oxh_status oxh_alloc(void **ptr, uint64_t bytes) {
   OXH_REQUIRE(ptr != nullptr, OXH_INVALID_SHAPE, "ptr is null");
   *ptr = nullptr;

@@ -27,6 +27,8 @@ import ctypes
 import functools
 import os
 import re
+import sys
+import threading
 from pathlib import Path
 from typing import Callable
 
@@ -97,6 +99,7 @@ _SIGNATURES = {
     "oxh_stream_create": (_st, [ctypes.POINTER(_vp)]),
     "oxh_stream_destroy": (_st, [_vp]),
     "oxh_stream_synchronize": (_st, [_vp]),
+    "oxh_stream_is_capturing": (_st, [_vp, ctypes.POINTER(_int)]),
     "oxh_alloc": (_st, [ctypes.POINTER(_vp), _u64]),
     "oxh_free": (_st, [_vp]),
     "oxh_memset0_async": (_st, [_vp, _u64, _vp]),
@@ -397,31 +400,82 @@ class Workspace:
         return b.data_ptr(), b.numel()
 
 
+_recording = threading.local()  # .scratch: the scratch of the graph that this thread records
+_unfreed = []  # scratch of graphs that ended while another capture allowed no wait for their runs
+
+
+def _capturing(stream: int) -> bool:
+    out = _int()
+    check(lib().oxh_stream_is_capturing(stream, ctypes.byref(out)))
+    return out.value != 0
+
+
+def _free_after_runs(scratch: list) -> None:
+    """Drops a graph's scratch once its replays have ended, on whatever streams they ran."""
+    import torch
+
+    recording = getattr(_recording, "scratch", None)
+    if recording is not None:  # no wait during a capture: the next graph's to free
+        recording.extend(scratch)
+    elif torch.cuda.is_current_stream_capturing():
+        _unfreed.extend(scratch)
+    else:
+        torch.cuda.synchronize()
+
+
 class StreamWorkspaces:
-    """Device scratch, a buffer for each stream, so that calls on two streams share none.  One that
-    has become too small is kept, since a captured graph may hold its address, and its successor is
-    twice its size at least."""
+    """Device scratch.  Eager calls share a buffer for each stream; a call recorded into a graph,
+    which may be replayed on any stream beside any other, takes one of its own, which lives as long
+    as the graph (``HipGraphExec``, or torch's, whose captures allocate from the graph's pool) or,
+    in a capture by other means, as long as this object."""
+
+    _AHEAD = 64 << 20  # bytes that a successor may have beyond what is asked for
 
     def __init__(self):
-        self._bufs = {}  # stream -> buffers, the last in use
+        self._bufs = {}  # stream -> buffer
+        self._kept = []  # of captures without an owner
+        self._pooled = None  # of torch's graphs the last, until its launches have been recorded
 
     def ptr_bytes(self, nbytes: int, stream: int) -> tuple[int | None, int]:
         if nbytes == 0:
             return None, 0
-        bufs = self._bufs.get(stream)
-        if bufs is None or bufs[-1].numel() < nbytes:
-            import torch
+        self._pooled = None
+        if stream and _capturing(stream):
+            buf = self._allocate(nbytes, stream)
+            recording = getattr(_recording, "scratch", None)
+            if recording is not None:
+                recording.append(buf)
+            elif _in_graph_pool(buf):
+                self._pooled = buf
+            else:
+                self._kept.append(buf)
+            return buf.data_ptr(), buf.numel()
+        buf = self._bufs.get(stream)
+        if buf is None or buf.numel() < nbytes:
+            size = 256 if buf is None else min(2 * buf.numel(), buf.numel() + self._AHEAD)
+            # the outgrown one goes back to the stream it was allocated on, behind its kernels
+            buf = self._bufs[stream] = self._allocate(max(nbytes, size), stream)
+        return buf.data_ptr(), buf.numel()
 
-            size = max(nbytes, 2 * bufs[-1].numel() if bufs else 256)
-            if stream == current_stream():
-                buf = torch.empty(size, dtype=torch.uint8, device="cuda")
-            else:  # of the stream's own memory: what it frees waits for its kernels
-                with torch.cuda.stream(torch.cuda.ExternalStream(stream) if stream
-                                       else torch.cuda.default_stream()):
-                    buf = torch.empty(size, dtype=torch.uint8, device="cuda")
-            bufs = self._bufs.setdefault(stream, [])
-            bufs.append(buf)
-        return bufs[-1].data_ptr(), bufs[-1].numel()
+    @staticmethod
+    def _allocate(nbytes: int, stream: int):
+        """Of the stream's own memory: what it frees waits for its kernels."""
+        import torch
+
+        if stream == current_stream():
+            return torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream) if stream
+                               else torch.cuda.default_stream()):
+            return torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+
+
+def _in_graph_pool(buf) -> bool:
+    """Whether a buffer lies in the memory pool of one of torch's graphs."""
+    import torch
+
+    at = buf.data_ptr()
+    return any(tuple(s["segment_pool_id"]) != (0, 0) and s["address"] <= at < s["address"] +
+               s["total_size"] for s in torch.cuda.memory_snapshot())
 
 
 def batch_norm_workspace_size(batch: int, channels: int, spatial: int) -> int:
@@ -1115,13 +1169,16 @@ def load_kernels(device: int = 0) -> LoadedModule:
 class HipGraphExec:
     """``CudaGraphExec`` (cuda_graph.rs:30-179): capture once, launch many times."""
 
-    def __init__(self, handle: int):
+    def __init__(self, handle: int, scratch=()):
         self._handle = handle
+        self._scratch = list(scratch)  # device buffers of the recorded launches
 
     @classmethod
     def capture(cls, stream, record: Callable[[], None]) -> "HipGraphExec":
         s = _stream(stream)
         check(lib().oxh_graph_begin(s))
+        outer, scratch = getattr(_recording, "scratch", None), []
+        _recording.scratch = scratch
         try:
             record()
         except Exception as exc:
@@ -1130,14 +1187,18 @@ class HipGraphExec:
             if isinstance(exc, OxideError):
                 raise OxideError(EXECUTION, f"graph recording failed: {exc}") from exc
             raise OxideError(EXECUTION, f"graph recording failed: {exc}") from exc
+        finally:
+            _recording.scratch = outer
         handle = _vp()
         check(lib().oxh_graph_end(s, ctypes.byref(handle)))
-        return cls(handle.value)
+        return cls(handle.value, scratch)
 
     def launch(self, stream) -> None:
         check(lib().oxh_graph_launch(self._handle, _stream(stream)))
 
     def __del__(self):
+        if getattr(self, "_scratch", None) and not sys.is_finalizing():
+            _free_after_runs(self._scratch)
         if getattr(self, "_handle", None) and _lib is not None:
             _lib.oxh_graph_destroy(self._handle)
             self._handle = None
