@@ -427,11 +427,15 @@ class StreamWorkspaces:
     """Device scratch.  Eager calls share a buffer for each stream; a call recorded into a graph,
     which may be replayed on any stream beside any other, takes one of its own, which lives as long
     as the graph (``HipGraphExec``, or torch's, whose captures allocate from the graph's pool) or,
-    in a capture by other means, as long as this object."""
+    in a capture by other means, as long as this object.
+
+    A call holds ``lock`` from ``ptr_bytes`` to its last launch, so that host threads on one stream
+    take turns: the launches of two calls interleaved would write what the other's later ones read."""
 
     _AHEAD = 64 << 20  # bytes that a successor may have beyond what is asked for
 
     def __init__(self):
+        self.lock = threading.Lock()
         self._bufs = {}  # stream -> buffer
         self._kept = []  # of captures without an owner
         self._pooled = None  # of torch's graphs the last, until its launches have been recorded
@@ -967,13 +971,15 @@ class LoadedModule:
         columns = shape[-1] if shape else 0
         rows = gradient.numel() // max(columns, 1)
         stream = _stream(stream)
-        ws, wsb = self._sequence_ws.ptr_bytes(
-            0 if weight_gradient is None else rms_norm_backward_workspace_size(rows, columns),
-            stream)
-        check(lib().oxh_rms_norm_backward(
-            stream, code, rows, columns, gradient_at, stream_at, sum_at,
-            _shaped(weight, (columns,), "weight"), _shaped(inverse_rms, (rows,), "inverse_rms"),
-            input_at, _shaped(weight_gradient, (columns,), "weight_gradient"), ws, wsb))
+        scratch = self._sequence_ws
+        with scratch.lock:
+            ws, wsb = scratch.ptr_bytes(
+                0 if weight_gradient is None else rms_norm_backward_workspace_size(rows, columns),
+                stream)
+            check(lib().oxh_rms_norm_backward(
+                stream, code, rows, columns, gradient_at, stream_at, sum_at,
+                _shaped(weight, (columns,), "weight"), _shaped(inverse_rms, (rows,), "inverse_rms"),
+                input_at, _shaped(weight_gradient, (columns,), "weight_gradient"), ws, wsb))
 
     def gated_recurrence_forward(self, x, gate, out, initial_state=None, final_state=None,
                                  lengths=None, stream=None):
@@ -987,12 +993,14 @@ class LoadedModule:
         batch, time, channels = shape
         states = (batch, channels)
         stream = _stream(stream)
-        ws, wsb = self._sequence_ws.ptr_bytes(
-            gated_recurrence_workspace_size(batch, time, channels), stream)
-        check(lib().oxh_gated_recurrence_forward(
-            stream, code, batch, time, channels, x_at, gate_at,
-            _shaped(initial_state, states, "initial_state"), _lengths(lengths, batch),
-            out_at, _shaped(final_state, states, "final_state"), ws, wsb))
+        scratch = self._sequence_ws
+        with scratch.lock:
+            ws, wsb = scratch.ptr_bytes(gated_recurrence_workspace_size(batch, time, channels),
+                                        stream)
+            check(lib().oxh_gated_recurrence_forward(
+                stream, code, batch, time, channels, x_at, gate_at,
+                _shaped(initial_state, states, "initial_state"), _lengths(lengths, batch),
+                out_at, _shaped(final_state, states, "final_state"), ws, wsb))
 
     def gated_recurrence_backward(self, gradient, x, gate, out, x_gradient, gate_gradient,
                                   initial_state=None, final_state_gradient=None,
@@ -1007,14 +1015,16 @@ class LoadedModule:
         batch, time, channels = shape
         states = (batch, channels)
         stream = _stream(stream)
-        ws, wsb = self._sequence_ws.ptr_bytes(
-            gated_recurrence_workspace_size(batch, time, channels), stream)
-        check(lib().oxh_gated_recurrence_backward(
-            stream, code, batch, time, channels, *at[:4],
-            _shaped(initial_state, states, "initial_state"),
-            _shaped(final_state_gradient, states, "final_state_gradient"),
-            _lengths(lengths, batch), at[4], at[5],
-            _shaped(initial_state_gradient, states, "initial_state_gradient"), ws, wsb))
+        scratch = self._sequence_ws
+        with scratch.lock:
+            ws, wsb = scratch.ptr_bytes(gated_recurrence_workspace_size(batch, time, channels),
+                                        stream)
+            check(lib().oxh_gated_recurrence_backward(
+                stream, code, batch, time, channels, *at[:4],
+                _shaped(initial_state, states, "initial_state"),
+                _shaped(final_state_gradient, states, "final_state_gradient"),
+                _lengths(lengths, batch), at[4], at[5],
+                _shaped(initial_state_gradient, states, "initial_state_gradient"), ws, wsb))
 
     def orthogonalize(self, x, out, rounds=5, epsilon=1e-7, stream=None):
         """``out`` = the matrices of ``x`` ([rows, columns] or [count, rows, columns], float32)
@@ -1023,11 +1033,12 @@ class LoadedModule:
             raise OxideError(INVALID_SHAPE, "orthogonalize expects a matrix or a stack of them")
         count, (rows, columns) = (x.shape[0] if x.dim() == 3 else 1), x.shape[-2:]
         stream = _stream(stream)
-        ws, wsb = self._sequence_ws.ptr_bytes(orthogonalize_workspace_size(count, rows, columns),
-                                              stream)
-        check(lib().oxh_orthogonalize(stream, count, rows, columns, rounds, epsilon,
-                                      _shaped(x, x.shape, "x"), _shaped(out, x.shape, "out"), ws,
-                                      wsb))
+        scratch = self._sequence_ws
+        with scratch.lock:
+            ws, wsb = scratch.ptr_bytes(orthogonalize_workspace_size(count, rows, columns), stream)
+            check(lib().oxh_orthogonalize(stream, count, rows, columns, rounds, epsilon,
+                                          _shaped(x, x.shape, "x"), _shaped(out, x.shape, "out"),
+                                          ws, wsb))
 
     def muon(self, learning_rate, weight_decay, momentum, tensors, nesterov=True, rounds=5,
              epsilon=1e-7, stream=None):
@@ -1035,10 +1046,12 @@ class LoadedModule:
         the momentum and the parameter are updated in place."""
         table = muon_table(tensors)
         stream = _stream(stream)
-        ws, wsb = self._sequence_ws.ptr_bytes(muon_workspace_size(table), stream)
-        check(lib().oxh_muon_multi_tensor(stream, learning_rate, weight_decay, momentum,
-                                          int(bool(nesterov)), epsilon, rounds, table,
-                                          len(table), ws, wsb))
+        scratch = self._sequence_ws
+        with scratch.lock:
+            ws, wsb = scratch.ptr_bytes(muon_workspace_size(table), stream)
+            check(lib().oxh_muon_multi_tensor(stream, learning_rate, weight_decay, momentum,
+                                              int(bool(nesterov)), epsilon, rounds, table,
+                                              len(table), ws, wsb))
 
     # -- conv2d / avg_pool2d (kernel_module.rs:359-490, 558-825)
     def conv2d_forward(self, shape, x, weight, bias, out, stream=None):

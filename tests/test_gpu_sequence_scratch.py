@@ -3,6 +3,7 @@ stream a graph is replayed on.  The operators have a fixed order of sums, so res
 bit for bit."""
 
 import gc
+import threading
 
 import pytest
 import torch
@@ -158,3 +159,31 @@ def test_outgrown_buffers_are_given_back(dev):
         assert size <= got <= size + (64 << 20)
         assert torch.cuda.memory_allocated() - start <= got + 512
     torch.cuda.synchronize()
+
+
+def test_threads_on_one_stream(dev):
+    """Host threads that call one module on one stream, each with operands of its own."""
+    module = ox.load_kernels(0)
+    sets = [Calls(module, dev, 60 + 10 * i) for i in range(4)]
+    stream, wrong = torch.cuda.Stream(), []
+
+    def work(calls):
+        try:
+            for _ in range(20):
+                calls.run(stream)
+        except Exception as error:  # noqa: BLE001 - reported below
+            wrong.append(error)
+
+    for _ in range(3):
+        for calls in sets:
+            calls.clear()
+        torch.cuda.synchronize()
+        threads = [threading.Thread(target=work, args=(calls,)) for calls in sets]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        assert not wrong
+        for calls in sets:
+            calls.check()
