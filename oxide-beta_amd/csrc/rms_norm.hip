@@ -265,12 +265,14 @@ __global__ __launch_bounds__(1024) void rms_norm_backward_long_kernel(Backward<T
   }
 }
 
-// out[c] = sum over the partial rows: 16 columns per block, 64 strands of rows each, a strand's
-// rows in order and the strands by halves.
+// out[c] = sum over the partial rows: 16 columns per block (from `first` on), 64 strands of rows
+// each, a strand's rows in order and the strands by halves.
 __global__ __launch_bounds__(1024) void rms_norm_weight_kernel(const float *partial, float *out,
-                                                               uint32_t rows, uint32_t columns) {
+                                                               uint32_t rows, uint32_t columns,
+                                                               uint32_t first) {
   __shared__ float part[64][17];
-  const uint32_t c = threadIdx.x & 15, strand = threadIdx.x >> 4, column = blockIdx.x * 16 + c;
+  const uint32_t c = threadIdx.x & 15, strand = threadIdx.x >> 4;
+  const uint32_t column = first + blockIdx.x * 16 + c;
   float sum = 0.0f;
   if (column < columns) {
 #pragma unroll 8
@@ -354,11 +356,32 @@ bool aligned_to(const void *p, uint64_t bytes) {
   return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0;
 }
 
+// Blocks of so many threads that one launch takes: it numbers its threads with 32 bits.
+constexpr uint64_t most_blocks(uint64_t threads) { return (1ull << 31) / threads; }
+
+// The rows in as many launches as that asks for (two from 2^25 rows of a wave each), `per` rows a
+// block: run(blocks, rows' arguments).
+template <typename T, typename Run>
+void by_launches(Forward<T> a, uint64_t threads, uint64_t per, Run run) {
+  const uint64_t most = most_blocks(threads) * per;
+  for (uint64_t left = a.rows; left != 0; left -= a.rows) {
+    a.rows = std::min(left, most);
+    run(dim3(static_cast<uint32_t>((a.rows + per - 1) / per)), a);
+    const uint64_t on = a.rows * a.columns;
+    a.x += on;
+    a.y += on;
+    if (a.r != nullptr) a.r += on;
+    if (a.s != nullptr) a.s += on;
+    if (a.q != nullptr) a.q += a.rows;
+  }
+}
+
 template <typename T>
 oxh_status forward(hipStream_t stream, const Forward<T> &a) {
   if (a.columns > forward_limit<T>()) {
-    oxh::launch(rms_norm_forward_long_kernel<T>, dim3(static_cast<uint32_t>(a.rows)),
-                dim3(1024), 0, stream, a);
+    by_launches(a, 1024, 1, [&](dim3 blocks, const Forward<T> &part) {
+      oxh::launch(rms_norm_forward_long_kernel<T>, blocks, dim3(1024), 0, stream, part);
+    });
     return oxh::launched("rms_norm_forward");
   }
   with_pack<T>(a.columns, [&](auto pack, auto ragged) {
@@ -366,9 +389,10 @@ oxh_status forward(hipStream_t stream, const Forward<T> &a) {
     with_shape<N, forward_limit<T>()>(a.columns, [&](auto shape) {
       using S = decltype(shape);
       constexpr int threads = S::lanes < 256 ? 256 : S::lanes, per = threads / S::lanes;
-      oxh::launch(rms_norm_forward_kernel<T, N, S::lanes, S::chunks, decltype(ragged)::value>,
-                  dim3(static_cast<uint32_t>((a.rows + per - 1) / per)), dim3(threads), 0,
-                  stream, a);
+      by_launches(a, threads, per, [&](dim3 blocks, const Forward<T> &part) {
+        oxh::launch(rms_norm_forward_kernel<T, N, S::lanes, S::chunks, decltype(ragged)::value>,
+                    blocks, dim3(threads), 0, stream, part);
+      });
     });
   });
   return oxh::launched("rms_norm_forward");
@@ -410,9 +434,11 @@ oxh_status backward(hipStream_t stream, Backward<T> a, float *weight_gradient) {
   }
   oxh_status st = oxh::launched("rms_norm_backward");
   if (st != OXH_OK || weight_gradient == nullptr || blocks == 1) return st;
-  oxh::launch(rms_norm_weight_kernel, dim3((a.columns + 15) / 16), dim3(1024), 0, stream,
-              static_cast<const float *>(a.partial), weight_gradient,
-              static_cast<uint32_t>(blocks), a.columns);
+  constexpr uint32_t most = static_cast<uint32_t>(most_blocks(1024)) * 16;
+  for (uint32_t first = 0; first < a.columns; first += most)
+    oxh::launch(rms_norm_weight_kernel, dim3((std::min(a.columns - first, most) + 15) / 16),
+                dim3(1024), 0, stream, static_cast<const float *>(a.partial), weight_gradient,
+                static_cast<uint32_t>(blocks), a.columns, first);
   return oxh::launched("rms_norm_weight_gradient");
 }
 

@@ -263,3 +263,43 @@ def test_few_rows(module, dev, shape):
     module.rms_norm_backward(g, s, w, q, dx, dw)
     check_backward(s, g, w, None, q, dx, dw, t)
     assert (around[:9] == 7).all() and (around[9 + shape[1]:] == 7).all()
+
+
+def test_more_rows_than_a_launch_takes(module, dev):
+    """2^26 rows and a few, 64 threads each: more than 2^32, which one launch cannot number.  The
+    rows beside every 2^25th and the last ones, the sum where its operand lay."""
+    t, shape = torch.bfloat16, ((1 << 26) + 5, 8)
+    x, w = torch.randn(shape, dtype=t, device=dev), make((8,), torch.float32, dev, 2) + 1.0
+    r = torch.randn(shape, dtype=t, device=dev)
+    some = [0, 1, (1 << 25) - 1, 1 << 25, (1 << 25) + 1, (1 << 26) - 1, 1 << 26, (1 << 26) + 4]
+    ref = forward_ref(x[some], r[some], w, 1e-6)
+    y, q = torch.zeros_like(x), torch.zeros(shape[0], device=dev)
+    module.rms_norm_forward(x, w, y, q, residual=r, sum=x)
+    within(x[some], ref[0], np.abs(ref[0]), 1, t, "sum")
+    within(q[some], ref[1], ref[1], 64, torch.float32, "inverse rms")
+    within(y[some], ref[2], np.abs(ref[2]), 64, t, "output")
+    assert bool((q > 0).all())
+    dx = torch.empty_like(x)
+    module.rms_norm_backward(y, x, w, q, dx, None, sum_gradient=r)
+    check_backward(x[some], y[some], w, r[some], q[some], dx[some], None, t)
+
+
+def test_more_columns_than_a_launch_takes(module, dev):
+    """The weight gradient of 2^26 columns and a few, 64 threads each.  A row's dot product is a
+    chain of 2^26 / 1024 terms per thread, and its error's part in dx is q unit times it over the
+    columns: 2^16 u of the mean magnitude, which 128 u of dx's other terms leave out."""
+    t, shape = torch.float32, (3, (1 << 26) + 3)
+    s, g = torch.randn(shape, device=dev), torch.randn(shape, device=dev)
+    w, q = torch.ones(shape[1], device=dev), torch.rsqrt(s.square().mean(1))
+    dx, dw = torch.empty_like(s), torch.zeros(shape[1], device=dev)
+    module.rms_norm_backward(g, s, w, q, dx, dw)
+    some = [0, 15, 16, (1 << 25) - 1, 1 << 25, (1 << 25) + 16, (1 << 26) - 1, 1 << 26, (1 << 26) + 2]
+    unit = f64(s[:, some]) * f64(q)[:, None]
+    terms = f64(g[:, some]) * unit
+    within(dw[some], terms.sum(0), np.abs(terms).sum(0), 256, t, "weight gradient")
+    inner = (s.double() * g.double()).mean(1).cpu().numpy() * f64(q)
+    size = (s.double() * g.double()).abs().mean(1).cpu().numpy() * f64(q)
+    ref = f64(q)[:, None] * (f64(g[:, some]) - unit * inner[:, None])
+    bound = f64(q)[:, None] * (128 * U * (np.abs(f64(g[:, some])) + np.abs(unit) * size[:, None]) +
+                               2.0 ** 16 * U * np.abs(unit) * size[:, None])
+    assert (np.abs(f64(dx[:, some]) - ref) <= bound).all()
