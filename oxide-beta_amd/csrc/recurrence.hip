@@ -608,8 +608,10 @@ oxh_status run(hipStream_t stream, uint64_t batch, Args<T> a, const char *what) 
                         static_cast<const void *>(a.h), static_cast<const void *>(a.dh),
                         static_cast<const void *>(a.out), static_cast<const void *>(a.dg)})
     a.lines = a.lines && aligned_to(x, kLine);
-  OXH_REQUIRE(batch * p.groups * p.segments < (1ull << 31), OXH_INVALID_SHAPE,
-              std::string(what) + ": too many rows");
+  // a launch numbers its threads with 32 bits
+  const uint64_t waves = p.brief ? 1 : waves_of(p.values, Back, p.segments > 1);
+  OXH_REQUIRE(batch * p.groups * p.segments * 64 * waves < (1ull << 32), OXH_INVALID_SHAPE,
+              std::string(what) + ": too many rows and channels for one launch");
   if (p.values == 1) return run_plan<T, Back, 1, false>(stream, batch, a, p, what);
   return a.channels % 4 == 0 ? run_plan<T, Back, 4, false>(stream, batch, a, p, what)
                              : run_plan<T, Back, 4, true>(stream, batch, a, p, what);

@@ -250,3 +250,26 @@ def test_net_builders():
         assert muon((node,)) == ox.INVALID_SHAPE
     assert program.value is None
     assert L.oxh_net_destroy(h) == ox.OK
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_gated_recurrence_of_more_than_a_launch_takes(dtype):
+    """2^32 threads and more, which a launch cannot number: 256 channels a wave for a few steps, 64
+    a block of 8 waves for more.  Refused before any launch, where blocks alone still fit 31 bits."""
+    at = [i << 46 for i in range(1, 8)]
+
+    def forward(batch, time, channels):
+        need = ox.gated_recurrence_workspace_size(batch, time, channels)
+        return ox.lib().oxh_gated_recurrence_forward(None, dtype, batch, time, channels, at[0],
+                                                     at[1], None, None, at[2], None, at[3], need)
+
+    def backward(batch, time, channels):
+        need = ox.gated_recurrence_workspace_size(batch, time, channels)
+        return ox.lib().oxh_gated_recurrence_backward(None, dtype, batch, time, channels, *at[:4],
+                                                      None, None, None, at[4], at[5], None, at[6],
+                                                      need)
+
+    for call in (forward, backward):
+        for batch, time, channels in ((65535, 1, 1 << 19), (1 << 12, 8, 1 << 22),
+                                      (1, 100, 1 << 29), (60000, 65, 9000)):
+            refused(call(batch, time, channels), b"too many rows and channels")
