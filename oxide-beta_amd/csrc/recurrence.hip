@@ -396,9 +396,9 @@ __global__ __launch_bounds__(64 * W) void recurrence_kernel(Args<T> a) {
       float y[V], z[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        if constexpr (Back) {  // 0 beyond the length: take and slope are
+        if constexpr (Back) {  // beyond the length take and slope are 0, but l need not be finite
           const float l = x[v] + add[s][v];
-          y[v] = take[s][v] * l;
+          y[v] = on ? take[s][v] * l : 0.0f;
           z[v] = keep[s][v] * y[v] * slope[s][v];
           x[v] = keep[s][v] * l;
         } else {

@@ -429,3 +429,24 @@ def test_workspaces_of_streams_and_graphs(module, dev):
         graph.launch(one)
         torch.cuda.synchronize()
         assert torch.equal(h, want) and (fill == 3).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(4, 9, 50), (3, 700, 64), (2, 6000, 24), (300, 3, 5)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_masked_steps_beside_a_final_gradient_that_is_not_finite(module, dev, shape, dtype, bad):
+    """Steps at or past a row's length take gradients of 0 whatever reaches the row's last step."""
+    t = TYPES[dtype]
+    u, g = make(shape, t, dev, 1), gates(shape, t, dev, 2)
+    n = lengths_of(shape[0], shape[1], dev)
+    du, dg = torch.ones_like(u), torch.ones_like(u)
+    ds, final = torch.empty(shape[0], shape[2], device=dev), torch.zeros(shape[0], shape[2],
+                                                                         device=dev)
+    final[:, 1::2] = bad
+    module.gated_recurrence_backward(u, u, g, u, du, dg, final_state_gradient=final,
+                                     initial_state_gradient=ds, lengths=n)
+    masked = (torch.arange(shape[1], device=dev)[None] >= n[:, None])[:, :, None].expand(shape)
+    assert (du[masked] == 0).all() and (dg[masked] == 0).all()
+    assert torch.equal(ds[-1].nan_to_num(7.0), final[-1].nan_to_num(7.0))  # a row of no steps
+    assert du[:, :, ::2].isfinite().all() and dg[:, :, ::2].isfinite().all()
+    assert not du[0, -1, 1::2].isfinite().any()  # the first row is whole
