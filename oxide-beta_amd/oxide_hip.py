@@ -404,12 +404,6 @@ _recording = threading.local()  # .scratch: the scratch of the graph that this t
 _unfreed = []  # scratch of graphs that ended while another capture allowed no wait for their runs
 
 
-def _capturing(stream: int) -> bool:
-    out = _int()
-    check(lib().oxh_stream_is_capturing(stream, ctypes.byref(out)))
-    return out.value != 0
-
-
 def _free_after_runs(scratch: list) -> None:
     """Drops a graph's scratch once its replays have ended, on whatever streams they ran."""
     import torch
@@ -436,7 +430,9 @@ class StreamWorkspaces:
 
     def __init__(self):
         self.lock = threading.Lock()
-        self._bufs = {}  # stream -> buffer
+        self._bufs = {}  # stream -> (address, bytes, buffer)
+        self._capturing = _int()
+        self._capturing_at = ctypes.byref(self._capturing)
         self._kept = []  # of captures without an owner
         self._pooled = None  # of torch's graphs the last, until its launches have been recorded
 
@@ -444,7 +440,9 @@ class StreamWorkspaces:
         if nbytes == 0:
             return None, 0
         self._pooled = None
-        if stream and _capturing(stream):
+        if stream:
+            check(lib().oxh_stream_is_capturing(stream, self._capturing_at))
+        if stream and self._capturing.value:
             buf = self._allocate(nbytes, stream)
             recording = getattr(_recording, "scratch", None)
             if recording is not None:
@@ -454,12 +452,13 @@ class StreamWorkspaces:
             else:
                 self._kept.append(buf)
             return buf.data_ptr(), buf.numel()
-        buf = self._bufs.get(stream)
-        if buf is None or buf.numel() < nbytes:
-            size = 256 if buf is None else min(2 * buf.numel(), buf.numel() + self._AHEAD)
+        at, size, _ = self._bufs.get(stream, (None, 0, None))
+        if size < nbytes:
             # the outgrown one goes back to the stream it was allocated on, behind its kernels
-            buf = self._bufs[stream] = self._allocate(max(nbytes, size), stream)
-        return buf.data_ptr(), buf.numel()
+            buf = self._allocate(max(nbytes, min(2 * size, size + self._AHEAD), 256), stream)
+            at, size = buf.data_ptr(), buf.numel()
+            self._bufs[stream] = at, size, buf
+        return at, size
 
     @staticmethod
     def _allocate(nbytes: int, stream: int):
