@@ -297,8 +297,10 @@ def _know_types() -> None:
     global _float32, _int32
     import torch
 
-    _float32, _int32 = torch.float32, torch.int32
+    # _float32 last: other threads take it for all of them
     _codes.update({torch.float32: F32, torch.bfloat16: BF16})
+    _int32 = torch.int32
+    _float32 = torch.float32
 
 
 def _activations(tensors, shape, what: str) -> tuple:

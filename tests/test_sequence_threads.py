@@ -102,3 +102,33 @@ def test_threads_on_one_stream_take_turns(monkeypatch, call):
     for t in threads:
         t.join()
     assert not errors and library.calls == 12 and not library.met
+
+
+def test_types_are_known_before_they_are_said_to_be(monkeypatch):
+    """A thread whose first call comes while another's fills the table of types: what it reads as
+    ready is whole."""
+    class Table(dict):
+        def update(self, *arguments):
+            began.set()
+            late.wait(0.5)
+            super().update(*arguments)
+
+    began, late, seen = threading.Event(), threading.Event(), []
+    monkeypatch.setattr(ox, "_codes", Table())
+    monkeypatch.setattr(ox, "_float32", None)
+    monkeypatch.setattr(ox, "_int32", None)
+
+    def second():
+        began.wait(5)
+        x = Device(2, 3)
+        try:
+            seen.append(ox._activations((x,), x.shape, "rms_norm")[0])
+        except ox.OxideError as error:
+            seen.append(error)
+        late.set()
+
+    thread = threading.Thread(target=second)
+    thread.start()
+    assert ox._activations((Device(2, 3),), torch.Size((2, 3)), "rms_norm")[0] == ox.F32
+    thread.join()
+    assert seen == [ox.F32]
