@@ -1786,7 +1786,6 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam,
         const uint64_t rows = norm_rows(x), columns = x.shape[x.rank - 1];
         float *dw = nullptr, *dst = nullptr, *acc = nullptr;
         const float *addend = nullptr;
-        if (want(x.in[1])) side(x.in[1], dw, "weight_gradient");
         if (want(xin) && !written[xin] && pending[xin].gradient != nullptr) {
           addend = pending[xin].gradient;
           op.tensors.push_back(ref("addend", const_cast<float *>(addend),
@@ -1799,6 +1798,8 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam,
         } else {
           contribution(xin, dst, acc);
         }
+        // behind the input's: a value that is its own weight takes this one beside that
+        if (want(x.in[1])) side(x.in[1], dw, "weight_gradient");
         op.kind = "rms_norm_backward";
         op.name = name("norm", r) + ".backward";
         op.tensors.push_back(ref("gradient", const_cast<float *>(gr), x, 0));

@@ -288,3 +288,31 @@ def test_example_on_idx_files(tmp_path, capsys):
     lines = capsys.readouterr().out.splitlines()
     assert [line.split()[0] for line in lines] == ["epoch", "epoch", "test"]
     assert math.isfinite(float(lines[1].split()[-1])) and 0 <= float(lines[2].split()[-1]) <= 1
+
+
+@pytest.mark.parametrize("uses", ["alone", "added", "multiplied"])
+def test_norm_of_a_value_by_itself(uses):
+    """A value that is input and weight of a norm takes both gradients, beside those of other uses
+    (an add's waits for the norm's, a product's is there before it)."""
+    D = 24
+    wv, cv = 1 + 0.3 * randn(D, seed=5), randn(D, seed=6)
+    w, t = nn.Parameter(wv), tn.input((1,))
+    v = w.tensor()
+    y = v.rms_norm(v)
+    if uses == "added":
+        y = y.add(v)
+    if uses == "multiplied":
+        y = y.mul(v)
+    loss = y.mul(tn.constant(cv)).reshape((1, D)).cross_entropy(t)
+    program = tn.training_program(loss)
+    program.feed(t, np.array([3], np.float32))
+    run_checked(program)
+    W = leaf(wv)
+    Y = norm64(W, W)
+    Y = {"alone": Y, "added": Y + W, "multiplied": Y * W}[uses]
+    F.cross_entropy((Y * torch.tensor(cv, dtype=torch.float64)).reshape(1, D),
+                    torch.tensor([3])).backward()
+    close(program.gradient(v).host(), W.grad, "gradient")
+    for _ in range(2):
+        program.run()
+    close(program.gradient(v).host(), W.grad, "gradient of the whole program")
