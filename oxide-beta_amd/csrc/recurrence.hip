@@ -29,9 +29,13 @@ namespace {
 using oxh::storage::bf16;
 using oxh::storage::widen;
 
-// sigmoid(g) and 1 - sigmoid(g), each to a few roundings however small: with e = exp(-g) they are
-// r = 1 / (1 + e) and e r, the latter as 1 - r (exact enough above 1/2) where g < 0, since e may
-// overflow there.
+// sigmoid(g) and 1 - sigmoid(g): with e = exp(-g) they are r = 1 / (1 + e) and e r, the latter as
+// 1 - r (exact enough above 1/2) where g < 0, since e may overflow there.  With u = 2^-24 the larger
+// one is within 4 u; the smaller within (8 + 1.25 |g|) u, as exp2 takes g log2(e) rounded (measured
+// 64 u at |g| = 86), and 0 beyond |g| = 88, where it would be denormal.  That rounding carried along
+// (three operations a gate) leaves 3 u at any gate and costs what the caches or few waves do not
+// hide: backward bfloat16 8 x 2048 x 2048 115 us and 110, 6 x 11621 x 112 27.8 and 25.1, forward 1 x
+// 131072 x 512 125 and 120, float32 55 x 39 x 2907 19.6 and 18.3.
 struct Gate {
   float keep, take;
 };

@@ -450,3 +450,53 @@ def test_masked_steps_beside_a_final_gradient_that_is_not_finite(module, dev, sh
     assert torch.equal(ds[-1].nan_to_num(7.0), final[-1].nan_to_num(7.0))  # a row of no steps
     assert du[:, :, ::2].isfinite().all() and dg[:, :, ::2].isfinite().all()
     assert not du[0, -1, 1::2].isfinite().any()  # the first row is whole
+
+
+@pytest.mark.parametrize("time", [1, 100])
+@pytest.mark.parametrize("closed", [True, False])
+def test_small_gate_values(module, dev, time, closed):
+    """What a nearly closed gate takes and a nearly open one keeps, in a single step between steps
+    that add nothing and keep all, up to the smallest normal numbers.  exp2's argument g log2(e)
+    carries the constant's rounding (0.22 u) and its own (u), |g| times as much in the result; exp2
+    and the reciprocal are within a unit in the last place (2 u each), 1 + e and the product within
+    u: (8 + 1.25 |g|) u with what is of second order."""
+    g = torch.linspace(0, 86.5, 20001, device=dev) * (1.0 if closed else -1.0)
+    gate = torch.full((1, time, g.numel()), 200.0, device=dev)
+    u, at = torch.zeros_like(gate), time // 2
+    gate[0, at] = g
+    u[0, at] = 1.0 if closed else 0.0
+    state = torch.full((1, g.numel()), 0.0 if closed else 1.0, device=dev)
+    h, final = torch.empty_like(u), torch.empty_like(state)
+    module.gated_recurrence_forward(u, gate, h, initial_state=state, final_state=final)
+    small, bound = 1 / (1 + np.exp(np.abs(f64(g)))), (8 + 1.25 * np.abs(f64(g))) * U
+    for got in (h[0, at], final[0]):
+        assert (np.abs(f64(got) / small - 1) <= bound).all()
+    # gate gradient: keep take (h_{t-1} - u_t) l, of l = 1 here: the larger value's 4 u and three
+    # products more
+    dh, du, dg = torch.zeros_like(u), torch.empty_like(u), torch.empty_like(u)
+    dh[0, at] = 1.0
+    module.gated_recurrence_backward(dh, u, gate, h, du, dg, initial_state=state)
+    large = 1 / (1 + np.exp(-np.abs(f64(g))))
+    want = small * large * (-1.0 if closed else 1.0)
+    assert (np.abs(f64(dg[0, at]) / want - 1) <= bound + 8 * U).all()
+    take = small if closed else large
+    assert (np.abs(f64(du[0, at]) / take - 1) <= (bound if closed else 4 * U) + U).all()
+
+
+@pytest.mark.parametrize("time", [1, 100])
+def test_gates_that_are_not_finite(module, dev, time):
+    """A NaN gate gives NaN; infinite ones keep or take exactly, also of large values."""
+    u = make((1, time, 8), torch.float32, dev, 1)
+    u[0, -1, 5] = 3e38
+    gate, state = gates((1, time, 8), torch.float32, dev, 2), make((1, 8), torch.float32, dev, 3)
+    state[0, 6] = 3e38
+    gate[0, -1, 0], gate[0, -1, 1] = float("nan"), -float("nan")
+    gate[0, -1, 2:5:2] = float("inf")
+    gate[0, -1, 3] = gate[0, -1, 6] = float("-inf")
+    gate[0, -1, 5] = float("inf")
+    h = torch.empty_like(u)
+    module.gated_recurrence_forward(u, gate, h, initial_state=state)
+    assert h[0, -1, :2].isnan().all()
+    before = state if time == 1 else h[:, -2]
+    assert torch.equal(h[0, -1, [2, 4, 5]], before[0, [2, 4, 5]])
+    assert torch.equal(h[0, -1, [3, 6]], u[0, -1, [3, 6]])
