@@ -375,27 +375,13 @@ __global__ __launch_bounds__(64 * W) void recurrence_kernel(Args<T> a) {
       }
     }
   };
-  if (begin < end) fetch(begin);
-  for (uint32_t tile = begin; tile < end; tile += kTile) {
-    const bool all_live = whole(tile);
-    map.identity();
-    if (all_live) compose(tile, std::true_type());
-    else compose(tile, std::false_type());
-    if (tile + kTile < end) fetch(tile + kTile);
-    const Map<V> all = scan_groups<V, Lanes, W>(map, shared[turn]);
-    turn ^= 1;
-    float x[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      x[v] = fmaf(map.a[v], h[v], map.b[v]);
-      h[v] = fmaf(all.a[v], h[v], all.b[v]);
-    }
-    if (!p.in) continue;
+  // x: the state before this thread's steps
+  auto finish = [&](uint32_t tile, float (&x)[V], auto all_live) {
 #pragma unroll
     for (int s = 0; s < S; ++s) {
       const uint32_t k = tile + group * S + s;
-      const bool on = all_live || (k >= live.begin && k < live_end);
-      if (!all_live && k >= end) continue;
+      const bool on = decltype(all_live)::value || (k >= live.begin && k < live_end);
+      if (!decltype(all_live)::value && k >= end) continue;
       const uint64_t at = row + row_of<Back>(a, k);
       float y[V], z[V];
 #pragma unroll
@@ -414,6 +400,25 @@ __global__ __launch_bounds__(64 * W) void recurrence_kernel(Args<T> a) {
       oxh::storage::store_places<T, V, Ragged, Once>(a.out + at, here, y);
       if constexpr (Back) oxh::storage::store_places<T, V, Ragged, Once>(a.dg + at, here, z);
     }
+  };
+  if (begin < end) fetch(begin);
+  for (uint32_t tile = begin; tile < end; tile += kTile) {
+    const bool all_live = whole(tile);
+    map.identity();
+    if (all_live) compose(tile, std::true_type());
+    else compose(tile, std::false_type());
+    if (tile + kTile < end) fetch(tile + kTile);
+    const Map<V> all = scan_groups<V, Lanes, W>(map, shared[turn]);
+    turn ^= 1;
+    float x[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      x[v] = fmaf(map.a[v], h[v], map.b[v]);
+      h[v] = fmaf(all.a[v], h[v], all.b[v]);
+    }
+    if (!p.in) continue;
+    if (all_live) finish(tile, x, std::true_type());
+    else finish(tile, x, std::false_type());
   }
   // every thread has read the first state, which may lie where the last one goes
   __syncthreads();
