@@ -54,11 +54,13 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 constexpr float kScale = 16384.0f, kUnscale = 1.0f / (16384.0f * 16384.0f);
+// A small X keeps its bits down to |V|_F = 2^-32 epsilon; 8^30 and S^2 stay within float32.
+constexpr int kMostShift = 30;
 
 // A matrix of a launch group.  Short = min(rows, columns) and Long are the sides of X; ps and pl
 // the same rounded up to the tile, the padding zero throughout.  `scratch` holds, in order:
 //   xt0, xt1 [pl][ps]: X' in halves (one is read while the other is written); gs, bs [ps][ps]: A
-//   and B in halves; the norm's partial sums.
+//   and B in halves; the norm's partial sums; |X|_F before the first round.
 // Halves of a matrix with k columns: per row, blocks of 32 columns, 32 hi then 32 lo.
 struct Matrix {
   const float *gradient;
@@ -81,7 +83,7 @@ struct Group {
 constexpr uint32_t kNormParts = 256;
 
 struct Layout {
-  uint64_t xt0, xt1, gs, bs, parts, total;
+  uint64_t xt0, xt1, gs, bs, parts, length, total;
 };
 __host__ __device__ inline Layout layout_of(uint64_t ps, uint64_t pl) {
   const uint64_t wide = ps * pl * 4, square = ps * ps * 4;
@@ -91,7 +93,8 @@ __host__ __device__ inline Layout layout_of(uint64_t ps, uint64_t pl) {
   l.gs = 2 * wide;
   l.bs = l.gs + square;
   l.parts = l.bs + square;
-  l.total = l.parts + kNormParts * 4;
+  l.length = l.parts + kNormParts * 4;
+  l.total = l.length + 4;
   return l;
 }
 
@@ -200,6 +203,14 @@ __device__ __forceinline__ void store_line(const uint32_t *words, f16 *to) {
   }
 }
 
+// A small X is kept as 2^k X, and A and B as 4^k A and 4^k B, so that their entries do not fall below
+// the halves' range: k is 0 unless |X|_F = |V|_F / (|V|_F + epsilon) is below 1/4, and then leaves
+// `length`, which bounds X, between 1/4 and 1/2 (4^k B below 1.3).  A round takes a singular value of
+// up to 1.5 to at most 3.4445 times itself, so before round r the length is |X|_F 3.4445^r.
+__device__ __forceinline__ int shift_of(float length) {
+  return min(max(-1 - __builtin_amdgcn_frexp_expf(length), 0), kMostShift);
+}
+
 // X' = (V / (|V| + epsilon))' in halves, a 32 x 32 tile per block.
 __global__ __launch_bounds__(256) void muon_start_kernel(Group g) {
   __shared__ float tile[32][33];
@@ -211,7 +222,11 @@ __global__ __launch_bounds__(256) void muon_start_kernel(Group g) {
   oxh::wave_sums_rows(one);
   if ((threadIdx.x & 63) == 0) wave[threadIdx.x >> 6] = one[0];
   __syncthreads();
-  const float norm = sqrtf((wave[0] + wave[1]) + (wave[2] + wave[3])) + g.epsilon;
+  const float size = sqrtf((wave[0] + wave[1]) + (wave[2] + wave[3]));
+  const float norm = size + g.epsilon, length = size / norm;
+  const float scale = ldexpf(1.0f, shift_of(length));
+  if (blockIdx.x == m.first_block && threadIdx.x == 0)
+    *reinterpret_cast<float *>(m.scratch + l.length) = length;
   const uint32_t tiles = m.pl / 32, b = blockIdx.x - m.first_block;
   const uint32_t i0 = b / tiles * 32, j0 = b % tiles * 32;
   const bool tall = m.rows > m.columns;
@@ -224,7 +239,7 @@ __global__ __launch_bounds__(256) void muon_start_kernel(Group g) {
     float v = 0.0f;
     if (i < s && j < n)
       v = direction(g, m, tall ? static_cast<uint64_t>(j) * m.columns + i
-                               : static_cast<uint64_t>(i) * m.columns + j) / norm;
+                               : static_cast<uint64_t>(i) * m.columns + j) / norm * scale;
     if (tall) tile[tx][k] = v;
     else tile[k][tx] = v;
   }
@@ -329,9 +344,10 @@ __device__ __forceinline__ void column_of(const f16 *line, uint32_t lane, f32x4 
 // One of a round's three products, a square tile per block of threads.  A A and B X sum along the
 // rows of their operands, which pass through shared memory as they lie; A = X X' sums along the
 // columns of X', which transposed reads of the shared memory turn.  A and B are symmetric: only
-// tiles on and below the diagonal are summed, the others are their mirrors.
+// tiles on and below the diagonal are summed, the others are their mirrors.  growth: 3.4445 to the
+// number of rounds before.
 template <Step S, class Sh>
-__global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int odd) {
+__global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int odd, float growth) {
   constexpr int kTile = Sh::tile, TM = Sh::TM, TN = Sh::TN, K = Sh::K;
   // per operand row and K block: 32 summed values, 8 pieces of 16 bytes (hi 0..3, lo 4..7), each
   // at its place exclusive-or bits 1 to 3 of the row: the 16 rows that one pass of a fragment's
@@ -557,6 +573,15 @@ __global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int 
   constexpr int kFinishing = TM * TN < Sh::Groups ? TM * TN : Sh::Groups;  // groups with a block
   static_assert(Sh::WM * Sh::WN * kFinishing * 32 * kPitch * 4 <= 4 * kStage, "turning space");
   uint32_t *turned = reinterpret_cast<uint32_t *>(stage) + wave * 32 * kPitch;
+  // `again` takes 4^k out of the product of operands kept larger, `next` turns 2^k X into 2^k' X, as
+  // the next round has it, or X
+  float again = 1.0f, next = 1.0f;
+  if constexpr (S != Step::Gram) {
+    const float length = *reinterpret_cast<const float *>(m.scratch + l.length) * growth;
+    const int k = shift_of(length);
+    again = ldexpf(1.0f, -2 * k);
+    next = ldexpf(1.0f, (S == Step::Apply ? shift_of(length * kA) : 0) - k);
+  }
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -574,9 +599,10 @@ __global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int 
         const uint32_t at = 8 * q + 4 * (lane >> 5), row = row0 + at;
         f32x4 v;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = acc[i][j][4 * q + r] * kUnscale;
+        for (int r = 0; r < 4; ++r) v[r] = acc[i][j][4 * q + r] * (kUnscale * again);
         if constexpr (S == Step::Poly) v = kB / kScale * addend[q] + kC * v;
-        if constexpr (S == Step::Apply || S == Step::Last) v += kA / kScale * addend[q];
+        if constexpr (S == Step::Apply || S == Step::Last)
+          v = (v + kA / kScale * addend[q]) * next;
         if constexpr (S == Step::Last) {
           const bool tall = m.rows > m.columns;
           const uint32_t wr0 = tall ? column : row, wc0 = tall ? row : column;
@@ -1191,7 +1217,8 @@ uint64_t scratch_of_all(const Parted &items) {
 }
 
 template <Step S>
-oxh_status product(hipStream_t stream, Group &g, uint32_t tile, int odd, const char *what) {
+oxh_status product(hipStream_t stream, Group &g, uint32_t tile, int odd, float growth,
+                   const char *what) {
   g.blocks = 0;
   for (uint32_t i = 0; i < g.count; ++i) {
     const uint32_t s = g.m[i].ps / tile, l = g.m[i].pl / tile;
@@ -1201,7 +1228,7 @@ oxh_status product(hipStream_t stream, Group &g, uint32_t tile, int odd, const c
   auto start = [&](auto shape) {
     using Sh = decltype(shape);
     oxh::launch(muon_product_kernel<S, Sh>, dim3(g.blocks), dim3(Sh::threads), 0, stream,
-                g, odd);
+                g, odd, growth);
   };
   if (tile == Wide::tile) start(Wide());
   else if (tile == Medium::tile) start(Medium());
@@ -1228,12 +1255,15 @@ oxh_status run_group(hipStream_t stream, Group &g, const Tiles &tiles, uint32_t 
   }
   oxh::launch(muon_start_kernel, dim3(g.blocks), dim3(256), 0, stream, g);
   st = oxh::launched("muon_start");
+  float growth = 1.0f;
   for (uint32_t r = 0; r < rounds && st == OXH_OK; ++r) {
-    st = product<Step::Gram>(stream, g, tiles.square, r & 1, "muon_gram");
-    if (st == OXH_OK) st = product<Step::Poly>(stream, g, tiles.square, r & 1, "muon_poly");
+    const uint32_t square = tiles.square, apply = tiles.apply;
+    st = product<Step::Gram>(stream, g, square, r & 1, growth, "muon_gram");
+    if (st == OXH_OK) st = product<Step::Poly>(stream, g, square, r & 1, growth, "muon_poly");
     if (st != OXH_OK) return st;
-    st = r + 1 < rounds ? product<Step::Apply>(stream, g, tiles.apply, r & 1, "muon_apply")
-                        : product<Step::Last>(stream, g, tiles.apply, r & 1, "muon_last");
+    st = r + 1 < rounds ? product<Step::Apply>(stream, g, apply, r & 1, growth, "muon_apply")
+                        : product<Step::Last>(stream, g, apply, r & 1, growth, "muon_last");
+    growth *= kA;
   }
   return st;
 }

@@ -248,3 +248,40 @@ def test_step_of_every_kind(module, dev):
             assert (a - b).norm() <= 1e-5 * b.norm()
             if a.shape[0] not in (128, 300):
                 assert torch.equal(a, b)
+
+
+# sides that a block takes, that go in slabs and in tiles of each size
+SMALL_NORMS = [(60, 90), (96, 700), (257, 300), (300, 200), (700, 710), (520, 2050), (2050, 2300)]
+
+
+@pytest.mark.parametrize("shape", SMALL_NORMS)
+@pytest.mark.parametrize("norm", [2e-8, 1e-8, 1e-9, 1e-11, 1e-13, 1e-15])
+def test_norms_below_epsilon(module, dev, shape, norm):
+    """|V|_F / (|V|_F + epsilon) far below 1: X starts small and keeps its bits.  From 1e-11 on X stays
+    below 485e-4, where a round multiplies it by 3.4445 but for a part of 3.3e-3 at most: its
+    rounding to 22 bits, of which half a unit is 2^-23, the product's in float32 and the entries'
+    floor (2^-39 of an X of at least 1/4) add up, below 2^-22 a round."""
+    g = torch.Generator().manual_seed(21)
+    v = torch.randn(*shape, generator=g).double()
+    v = (v / v.norm() * norm).float().to(dev)
+    out = torch.empty_like(v)
+    module.orthogonalize(v, out)
+    ref = orthogonal_on(v.double())
+    bound = BOUND if norm > 1e-11 else 5 * 2.0 ** -22
+    assert (out.double() - ref).norm() <= bound * ref.norm()
+
+
+@pytest.mark.parametrize("norm", [1.0, 9e-8, 6e-8, 4e-8, 3.4e-8, 2e-8, 1e-8, 1e-9, 1e-12])
+@pytest.mark.parametrize("rounds", [1, 5])
+def test_one_direction_at_any_norm(module, dev, norm, rounds):
+    """A matrix of rank 1, whose whole norm is one singular value: the largest entries that A and B
+    can have."""
+    left, right = torch.randn(300, 1, generator=torch.Generator().manual_seed(22)), \
+        torch.ones(1, 310)
+    left[7], right[0, 9] = 300.0, 300.0  # one entry holds most of it
+    v = (left @ right).double()
+    v = (v / v.norm() * norm).float().to(dev)
+    out = torch.empty_like(v)
+    module.orthogonalize(v, out, rounds=rounds)
+    ref = orthogonal_on(v.double(), rounds)
+    assert (out.double() - ref).norm() <= BOUND * ref.norm()
