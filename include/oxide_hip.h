@@ -392,8 +392,8 @@ oxh_status oxh_adamw_multi_tensor_table_step(oxh_stream stream, float learning_r
  * What a recurrent sequence model's blocks and their matrices train with; no counterpart in the
  * reference, which has no layer along a sequence, no norm over one position's features and one
  * optimizer.  Activations are float32 or bfloat16 (OXH_F32, OXH_BF16: contiguous, aligned to
- * their elements), parameters, statistics, states and all arithmetic float32; an output is
- * rounded once. */
+ * their elements), parameters, statistics, states and arithmetic float32 (the orthogonalisation's
+ * products: below); an output is rounded once. */
 #define OXH_F32 0
 #define OXH_BF16 1
 
@@ -452,7 +452,10 @@ oxh_status oxh_gated_recurrence_backward(
  * products: X = V / (|V|_F + epsilon), then `rounds` times
  *   A = X X';  B = b A + c A A;  X = a X + B X,   (a, b, c) = (3.4445, -4.7750, 2.0315)
  * (the transposed iteration where rows > columns), which takes every singular value that is not
- * tiny to about 1 (0.7 .. 1.21) and keeps the singular vectors.  A zero matrix gives zeros. */
+ * tiny to about 1 (0.7 .. 1.21) and keeps the singular vectors.  A zero matrix gives zeros.
+ * Products sum in float32 over operands of 22 bits, entries of X below 2^-17 over an absolute 2^-39:
+ * a round is within about 2^-21 of the result's Frobenius norm, but rows or columns of less than
+ * 1e-5 of the largest ones' size keep fewer bits of their own. */
 oxh_status oxh_orthogonalize_workspace_size(uint64_t count, uint64_t rows, uint64_t columns,
                                             uint64_t *bytes);
 oxh_status oxh_orthogonalize(oxh_stream stream, uint64_t count, uint64_t rows, uint64_t columns,

@@ -12,9 +12,15 @@
 // AdamW.
 //
 // Products.  An operand value v is held as two float16 numbers, hi = f16(S v) and lo =
-// f16(S v - hi) with S = 2^14, which together keep 22 bits of it; a product is summed as hi hi' +
-// hi lo' + lo hi' in float32 on the matrix cores (the omitted lo lo' is below 2^-22 of the
-// product).  No entry overflows: |X| and |A| stay below 1.5 and |B| below 2.9 for |X|_F <= 1.
+// f16(S v - hi) with S = 2^14, which together keep 22 bits of it from |v| = 2^-17 on, and below an
+// absolute 2^-39; a product is summed as hi hi' + hi lo' + lo hi' in float32 on the matrix cores
+// (the omitted lo lo' is below 2^-22 of the product).  No entry overflows: |X| and |A| stay below
+// 1.5 and |B| below 2.9 for |X|_F <= 1.
+//
+// The absolute part is of the largest rows' scale, not a small row's own: in a matrix of 1000 x 1280
+// in which some rows are 1e-6 of the others, entries start near 2^-30, and those rows of the result
+// are 1.2e-3 of themselves off (1.3e-6 of the whole result, as any).  A scale for each row would not
+// do: A A and B X sum over rows.
 //
 // X itself is kept as halves too, and a X and b A are added to the summed products from them.  The
 // error of X grows from round to round (by up to a = 3.4445 in the directions of small singular

@@ -285,3 +285,19 @@ def test_one_direction_at_any_norm(module, dev, norm, rounds):
     module.orthogonalize(v, out, rounds=rounds)
     ref = orthogonal_on(v.double(), rounds)
     assert (out.double() - ref).norm() <= BOUND * ref.norm()
+
+
+@pytest.mark.parametrize("shape", [(100, 130), (64, 700), (300, 310), (700, 710), (1000, 1280)])
+def test_small_rows(module, dev, shape):
+    """Eight rows of 1e-6 of the others: what they lose to the halves' floor.  A round leaves them
+    2^-39 an entry of X off, and as much of A and of B (b and 1 times), each of which a round's X of
+    norm 1 turns into rows: sqrt(8 columns) (a + b + 2) 2^-39 at most, and every later round takes
+    3.4445 times it on: 684 (1 + a + .. + a^5) times that in all, beside the bound on the whole."""
+    v = torch.randn(*shape, generator=torch.Generator().manual_seed(24)).to(dev)
+    v[:8] *= 1e-6
+    out = torch.empty_like(v)
+    module.orthogonalize(v, out)
+    ref = orthogonal_on(v.double())
+    floor = 684 * (A - B + 2) * 2.0 ** -39 * math.sqrt(8 * shape[1])
+    assert (out[:8].double() - ref[:8]).norm() <= floor + BOUND * ref[:8].norm()
+    assert (out.double() - ref).norm() <= BOUND * ref.norm()
