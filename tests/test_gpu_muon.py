@@ -301,3 +301,17 @@ def test_small_rows(module, dev, shape):
     floor = 684 * (A - B + 2) * 2.0 ** -39 * math.sqrt(8 * shape[1])
     assert (out[:8].double() - ref[:8]).norm() <= floor + BOUND * ref[:8].norm()
     assert (out.double() - ref).norm() <= BOUND * ref.norm()
+
+
+@pytest.mark.parametrize("shape", [(60, 90), (96, 700), (300, 310), (700, 710), (1000, 1280),
+                                   (2050, 2300), (3900, 3870)])
+def test_bits_of_one_round(module, dev, shape):
+    """A round's bound from its operands' bits, 2^-23 each (half a unit of 22): a X has a (1 more for
+    its rounding); A of |A|_F <= 1 two of them, its rounding, and b A and B's rounding after it, c A A
+    two A's and their rounding, and B X those of B and of X, for |B|_F <= b + c: in all a + 1 + 4 b +
+    8 c + 2 (b + c) = 54 units of 2^-23 in the worst case, were all errors of one sign.  They are
+    independent, and a sum of thousands of them is below an eighth of that."""
+    v = torch.randn(*shape, generator=torch.Generator().manual_seed(23)).to(dev)
+    out = torch.empty_like(v)
+    module.orthogonalize(v, out, rounds=1)
+    assert (out.double() - orthogonal_on(v.double(), 1)).norm() <= 54 / 8 * 2.0 ** -23
