@@ -521,7 +521,9 @@ def op_bytes(op: Op) -> tuple[str, int]:
     if k == "add_rms_norm_forward":
         return "rms_norm", 4 * nb(op.reads["a"])                           # a, b in; sum, y out
     if k == "rms_norm_backward":
-        return "rms_norm", 3 * nb(op.reads["gradient"]) + acc              # g, x in; dx out
+        # g, x in; dx out; the input's other gradient in, a waiting add's or the one in place
+        other = "addend" in op.reads or "input_gradient" in op.by_role
+        return "rms_norm", (3 + other) * nb(op.reads["gradient"]) + acc
     if k == "gated_recurrence_forward":
         return "gated_recurrence", 3 * nb(op.reads["x"])                   # x, gate in; y out
     if k == "gated_recurrence_backward":

@@ -316,3 +316,23 @@ def test_norm_of_a_value_by_itself(uses):
     for _ in range(2):
         program.run()
     close(program.gradient(v).host(), W.grad, "gradient of the whole program")
+
+
+def test_bytes_of_norm_backwards():
+    """A norm's backward counts the other gradient of its input that it reads: a waiting add's, or
+    the one it adds to in place; none where the norm is the only use."""
+    B, T, D = 2, 3, 16
+    a, b, c = (tn.input((B, T, D), requires_grad=True) for _ in range(3))
+    w, t = nn.Parameter(1 + 0.1 * randn(D, seed=1)), tn.input((B,))
+    s = a.add(b)
+    added = s.add(s.rms_norm(w.tensor()))            # s takes the add's gradient
+    p = added.mul(c)
+    in_place = p.mul(p.rms_norm(w.tensor()))         # p takes the product's first
+    alone = in_place.rms_norm(w.tensor())
+    loss = alone.reshape((B, T * D)).cross_entropy(t)
+    program = tn.training_program(loss)
+    ops = [op for op in program.ops if op.kind == "rms_norm_backward"]
+    assert [("addend" in op.reads, "input_gradient" in op.by_role) for op in ops] == \
+        [(False, False), (False, True), (True, False)]
+    assert [training.op_bytes(op) for op in ops] == \
+        [("rms_norm", n * 4 * B * T * D) for n in (3, 4, 4)]
