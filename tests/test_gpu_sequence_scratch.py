@@ -2,6 +2,7 @@
 stream a graph is replayed on.  The operators have a fixed order of sums, so results are compared
 bit for bit."""
 
+import ctypes
 import gc
 import threading
 
@@ -91,6 +92,24 @@ def test_graphs_of_one_stream_on_several(dev, monkeypatch):
         torch.cuda.synchronize()
         for calls in sets:
             calls.check()
+
+
+def test_a_stream_says_whether_it_is_captured(dev):
+    one, two, said = torch.cuda.Stream(), torch.cuda.Stream(), []
+
+    def ask():
+        for s in (one, two):
+            out = ctypes.c_int(7)
+            ox.check(ox.lib().oxh_stream_is_capturing(s.cuda_stream, ctypes.byref(out)))
+            said.append(out.value)
+
+    ask()
+    with torch.cuda.stream(one):
+        x = torch.zeros(8, device=dev)
+        graph = ox.HipGraphExec.capture(one, lambda: (x.add_(1), ask()))
+    ask()
+    assert said == [0, 0, 1, 0, 0, 0]
+    del graph
 
 
 def test_scratch_lives_with_its_graph(dev, monkeypatch):

@@ -273,3 +273,9 @@ def test_gated_recurrence_of_more_than_a_launch_takes(dtype):
         for batch, time, channels in ((65535, 1, 1 << 19), (1 << 12, 8, 1 << 22),
                                       (1, 100, 1 << 29), (60000, 65, 9000)):
             refused(call(batch, time, channels), b"too many rows and channels")
+
+
+def test_stream_is_capturing():
+    out = ctypes.c_int(7)
+    assert ox.lib().oxh_stream_is_capturing(None, ctypes.byref(out)) == ox.OK and out.value == 0
+    refused(ox.lib().oxh_stream_is_capturing(None, None), b"null")
