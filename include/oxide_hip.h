@@ -425,7 +425,8 @@ oxh_status oxh_rms_norm_backward(oxh_stream stream, int dtype, uint64_t rows, ui
  * from initial_state [batch, channels] (NULL: 0); output holds every h_t and final_state (may be
  * NULL) the last.  lengths (device int32 [batch], may be NULL; clamped to 0..time): a row's steps
  * at or past its length give 0 and leave the state, whatever input and gate hold there.
- * final_state may be initial_state itself: single tokens are time 1 with the state in place. */
+ * final_state may be initial_state itself: single tokens are time 1 with the state in place.
+ * OXH_INVALID_SHAPE above a batch of 65535, or where one launch cannot number the threads. */
 oxh_status oxh_gated_recurrence_workspace_size(uint64_t batch, uint64_t time, uint64_t channels,
                                                uint64_t *bytes);
 oxh_status oxh_gated_recurrence_forward(oxh_stream stream, int dtype, uint64_t batch,

@@ -32,8 +32,8 @@
 // Bound.  Three matrix instructions for each of the plain product's, half of A and of A A: 5 (s^2 n
 // + s^3 + 2 s^2 n) multiply-adds for X of s x n.  Large matrices come near the matrix cores' rate:
 // 4096 x 4096 in 4.1 ms, 335 TFLOP/s or 1005 of float16 (a library's largest float16 products reach
-// 1092 here); 12 x 512 x 2048 in 612 us (three launches a round, which leave the cores a part of
-// the time), and 1000 x 1280 in 225 us, where each of 17 launches takes 9 to 18 us: 136 tiles on
+// 1092 here); 12 x 512 x 2048 in 602 us (three launches a round, which leave the cores a part of
+// the time), and 1000 x 1280 in 223 us, where each of 15 products takes 12 to 18 us: 136 tiles on
 // 256 compute units, each a chain of loads.  Short sides of up to 128 take fewer launches: one for
 // a matrix that a compute unit holds, seven in slabs of its columns.
 #include <hip/hip_runtime.h>
@@ -666,7 +666,7 @@ __global__ __launch_bounds__(Sh::threads) void muon_product_kernel(Group g, int 
 // column of 4) give the same order for X X'.
 //
 // The bound is one compute unit's shared memory and its barriers: of the 88000 cycles that 96 x
-// 192 takes (38 us), a round is 14500: X X' 3000 (its operands are 2250 of the shared memory's), A
+// 192 takes (40 us), a round is 14500: X X' 3000 (its operands are 2250 of the shared memory's), A
 // and A A 4600 with their halves, shared among the waves that summed a tile, B X 4700 (3400), X' in
 // halves 2000.  The way in is 14000: twelve loads at a time, 7000 where eight took 9300.
 
@@ -1090,7 +1090,7 @@ struct Item {
 uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
 
 // Whether one block steps the whole matrix: the rows of the shared memory that hold X', and at most
-// this many column blocks per wave (one matrix of 96 x 192 38 us, 72 in tiles; of 64 x 384 45, 47
+// this many column blocks per wave (one matrix of 96 x 192 40 us, 72 in tiles; of 64 x 384 45, 47
 // in slabs; of 128 x 192 58, 73 in tiles; of 96 x 384 and 128 x 256, whose two column blocks spill,
 // 92 and 116, and 60 in slabs and 74 in tiles).
 constexpr int whole_blocks(int ps) { return ps == 32 ? 6 : ps == 64 ? 3 : 1; }
@@ -1132,7 +1132,10 @@ struct Tiles {
 //     254 without; everywhere, 12 x 512 x 2048 takes 716 and 657 without);
 // and both take 192 where the square products just fill one round of a block per compute unit, with
 // the same limit on padding (4096 x 4096, 253 tiles: 4.06 ms, 4.80 with 128; 2560 x 2560, 105
-// tiles: 1641 and 1367 us; 12 x 1024 x 1024, 252 tiles padded 1.27 times: 1330 and 1079).
+// tiles: 1641 and 1367 us; 12 x 1024 x 1024, 252 tiles padded 1.27 times: 1330 and 1079).  That is
+// one matrix of a short side of 3841 to 4224; more rounds than one were not measured with 192, and a
+// list of such matrices is slower than they are one by one (two of 4096 x 4096 8.8 ms and 8.1, three
+// 13.0 and 12.1).
 Tiles tiles_of(const Item *items, size_t count) {
   struct Count {
     uint64_t square = 0, apply = 0, area = 0;

@@ -10,9 +10,9 @@
 //
 // Composing two steps' maps h -> a h + b is associative, so time is cut into tiles that a block
 // scans, and into segments where rows and channels alone leave compute units idle.  The bound is
-// memory: forward 8 x 2048 x 2048 float32 takes 82 us (4.9 TB/s), backward 153 us (5.3 TB/s).
-// Split, the operands are read twice: forward 1 x 131072 x 512 bfloat16 takes 52 us for the
-// segments' maps and 72 us for the states, 671 MB at 5.4 TB/s (one pass over its 403 MB would need
+// memory: forward 8 x 2048 x 2048 float32 takes 80 us (5.0 TB/s), backward 153 us (5.3 TB/s).
+// Split, the operands are read twice: forward 1 x 131072 x 512 bfloat16 takes 56 us for the
+// segments' maps and 68 us for the states, 671 MB at 5.4 TB/s (one pass over its 403 MB would need
 // the segments' states handed on inside one launch).  A single step of 64 x 2048 takes 3.4 us, a
 // launch.
 #include <hip/hip_runtime.h>
