@@ -402,28 +402,31 @@ class Workspace:
         return b.data_ptr(), b.numel()
 
 
-_recording = threading.local()  # .scratch: the scratch of the graph that this thread records
+# .scratch: the scratch of the graph that this thread records, buffers by the stream they are for
+_recording = threading.local()
 _unfreed = []  # scratch of graphs that ended while another capture allowed no wait for their runs
 
 
-def _free_after_runs(scratch: list) -> None:
+def _free_after_runs(scratch: dict) -> None:
     """Drops a graph's scratch once its replays have ended, on whatever streams they ran."""
     import torch
 
     recording = getattr(_recording, "scratch", None)
     if recording is not None:  # no wait during a capture: the next graph's to free
-        recording.extend(scratch)
+        recording.setdefault(None, []).append(scratch)
     elif torch.cuda.is_current_stream_capturing():
-        _unfreed.extend(scratch)
+        _unfreed.append(scratch)
     else:
         torch.cuda.synchronize()
+        _unfreed.clear()
 
 
 class StreamWorkspaces:
-    """Device scratch.  Eager calls share a buffer for each stream; a call recorded into a graph,
-    which may be replayed on any stream beside any other, takes one of its own, which lives as long
-    as the graph (``HipGraphExec``, or torch's, whose captures allocate from the graph's pool) or,
-    in a capture by other means, as long as this object.
+    """Device scratch.  Eager calls share a buffer for each stream.  A graph may be replayed on any
+    stream beside any other, so calls recorded into it take buffers of its own, which live as long
+    as it does: those of a ``HipGraphExec`` share one for each stream of its capture, those of
+    torch's graphs allocate from the graph's pool.  A call captured by other means takes one that
+    lives as long as this object.
 
     A call holds ``lock`` from ``ptr_bytes`` to its last launch, so that host threads on one stream
     take turns: the launches of two calls interleaved would write what the other's later ones read."""
@@ -445,14 +448,18 @@ class StreamWorkspaces:
         if stream:
             check(lib().oxh_stream_is_capturing(stream, self._capturing_at))
         if stream and self._capturing.value:
-            buf = self._allocate(nbytes, stream)
             recording = getattr(_recording, "scratch", None)
             if recording is not None:
-                recording.append(buf)
-            elif _in_graph_pool(buf):
-                self._pooled = buf
+                bufs = recording.setdefault(stream, [])
+                if not bufs or bufs[-1].numel() < nbytes:
+                    bufs.append(self._allocate(nbytes, stream))
+                buf = bufs[-1]
             else:
-                self._kept.append(buf)
+                buf = self._allocate(nbytes, stream)
+                if _in_graph_pool(buf):
+                    self._pooled = buf
+                else:
+                    self._kept.append(buf)
             return buf.data_ptr(), buf.numel()
         at, size, _ = self._bufs.get(stream, (None, 0, None))
         if size < nbytes:
@@ -1183,15 +1190,15 @@ def load_kernels(device: int = 0) -> LoadedModule:
 class HipGraphExec:
     """``CudaGraphExec`` (cuda_graph.rs:30-179): capture once, launch many times."""
 
-    def __init__(self, handle: int, scratch=()):
+    def __init__(self, handle: int, scratch: dict | None = None):
         self._handle = handle
-        self._scratch = list(scratch)  # device buffers of the recorded launches
+        self._scratch = scratch  # device buffers of the recorded launches
 
     @classmethod
     def capture(cls, stream, record: Callable[[], None]) -> "HipGraphExec":
         s = _stream(stream)
         check(lib().oxh_graph_begin(s))
-        outer, scratch = getattr(_recording, "scratch", None), []
+        outer, scratch = getattr(_recording, "scratch", None), {}
         _recording.scratch = scratch
         try:
             record()

@@ -133,7 +133,30 @@ def test_scratch_lives_with_its_graph(dev, monkeypatch):
     held = torch.cuda.memory_allocated()
     del graph
     gc.collect()
-    assert held - torch.cuda.memory_allocated() >= sum(b - a for a, b in mine)
+    assert held - torch.cuda.memory_allocated() >= max(b - a for a, b in mine)
+
+
+def test_calls_of_one_graph_share_scratch(dev, monkeypatch):
+    """Recorded calls on one stream run in their order, so a graph of many takes no more than the
+    largest and the smaller ones before it."""
+    module = ox.load_kernels(0)
+    calls, stream = Calls(module, dev, 7), torch.cuda.Stream()
+    ranges = recorded(monkeypatch)
+
+    def several():
+        for _ in range(10):
+            calls.run(stream)
+
+    start = torch.cuda.memory_allocated()
+    graph = ox.HipGraphExec.capture(stream, several)
+    used = torch.cuda.memory_allocated() - start
+    assert len(ranges) == 40 and used <= sum(b - a for a, b in set(ranges)) + 4 * 512
+    assert len(set(ranges)) <= 4 and len(set(ranges[4:])) == 1
+    calls.clear()
+    torch.cuda.synchronize()
+    graph.launch(torch.cuda.current_stream())
+    torch.cuda.synchronize()
+    calls.check()
 
 
 def test_graphs_of_torch(dev, monkeypatch):
@@ -206,3 +229,33 @@ def test_threads_on_one_stream(dev):
         assert not wrong
         for calls in sets:
             calls.check()
+
+
+def test_graphs_that_end_during_a_capture(dev):
+    """No wait is made while another graph is captured: its scratch is freed with that one, or with
+    the next that ends."""
+    module = ox.load_kernels(0)
+    calls, stream = Calls(module, dev, 9), torch.cuda.Stream()
+    capture = lambda: ox.HipGraphExec.capture(stream, lambda: calls.run(stream))  # noqa: E731
+    start, first = torch.cuda.memory_allocated(), [capture()]
+    other = torch.cuda.Stream()
+    with torch.cuda.stream(other):
+        x = torch.zeros(8, device=dev)
+        second = ox.HipGraphExec.capture(other, lambda: (first.clear(), x.add_(1)))
+    assert torch.cuda.memory_allocated() > start + 512
+    del second
+    gc.collect()
+    assert torch.cuda.memory_allocated() <= start + 512  # x
+    first.append(capture())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        first.clear()
+        x.add_(1)
+    assert len(ox._unfreed) == 1
+    graph.replay()
+    third = capture()
+    del third
+    gc.collect()
+    assert ox._unfreed == []
+    torch.cuda.synchronize()
+    assert float(x[0]) == 1
