@@ -417,7 +417,9 @@ __global__ __launch_bounds__(64 * W) void recurrence_kernel(Args<T> a) {
       h[v] = fmaf(all.a[v], h[v], all.b[v]);
     }
     if (!p.in) continue;
-    if (all_live) finish(tile, x, std::true_type());
+    // whole tiles without their lengths' questions; backward over segments, of few tiles each, one
+    // form is faster (5 x 1537 x 333 bfloat16 14.1 us and 14.4; 8 x 2048 x 2048 whole 112.0 and 110.7)
+    if (!(Back && W == 4) && all_live) finish(tile, x, std::true_type());
     else finish(tile, x, std::false_type());
   }
   // every thread has read the first state, which may lie where the last one goes

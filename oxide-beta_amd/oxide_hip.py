@@ -1001,10 +1001,9 @@ class LoadedModule:
         batch, time, channels = shape
         states = (batch, channels)
         stream = _stream(stream)
-        scratch = self._sequence_ws
+        scratch, size = self._sequence_ws, gated_recurrence_workspace_size(batch, time, channels)
         with scratch.lock:
-            ws, wsb = scratch.ptr_bytes(gated_recurrence_workspace_size(batch, time, channels),
-                                        stream)
+            ws, wsb = scratch.ptr_bytes(size, stream) if size else (None, 0)
             check(lib().oxh_gated_recurrence_forward(
                 stream, code, batch, time, channels, x_at, gate_at,
                 _shaped(initial_state, states, "initial_state"), _lengths(lengths, batch),
@@ -1023,10 +1022,9 @@ class LoadedModule:
         batch, time, channels = shape
         states = (batch, channels)
         stream = _stream(stream)
-        scratch = self._sequence_ws
+        scratch, size = self._sequence_ws, gated_recurrence_workspace_size(batch, time, channels)
         with scratch.lock:
-            ws, wsb = scratch.ptr_bytes(gated_recurrence_workspace_size(batch, time, channels),
-                                        stream)
+            ws, wsb = scratch.ptr_bytes(size, stream) if size else (None, 0)
             check(lib().oxh_gated_recurrence_backward(
                 stream, code, batch, time, channels, *at[:4],
                 _shaped(initial_state, states, "initial_state"),
