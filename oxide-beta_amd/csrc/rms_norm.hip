@@ -11,7 +11,7 @@
 // The bound is memory, so a row is read once and kept in registers: forward of a bfloat16 sum of
 // 16384 x 4096 moves 537 MB in 97 us (5.5 TB/s, a large copy's rate); backward of float32 3584 x
 // 1280 moves 73 MB in 15 us (4.8 TB/s) and sums the weight gradient's shares in 4 us more.  Small
-// calls are launches: one row of 1024 takes 2.4 us, backward of bfloat16 1021 x 1537 9.3 and 3.9.
+// calls are launches: one row of 1024 takes 2.4 us, backward of bfloat16 1021 x 1537 9.2 and 2.8.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
