@@ -449,6 +449,97 @@ oxh_status oxh_gated_recurrence_backward(
     void *input_gradient, void *gate_gradient, float *initial_state_gradient, void *workspace,
     uint64_t workspace_bytes);
 
+/* Layer norm over the last dimension of input (+ residual, may be NULL):
+ *   s = input + residual;  m = mean(s);  q = 1 / sqrt(mean((s - m)^2) + epsilon)
+ *   output = (s - m) * q * weight + bias   (bias may be NULL: 0)
+ * `sum` receives s, `mean` and `inverse_deviation` [rows] m and q (each may be NULL; the backward
+ * reads all three; with no residual s is the input).  `sum` may be `input` or `residual` itself;
+ * nothing else may overlap. */
+oxh_status oxh_layer_norm_forward(oxh_stream stream, int dtype, uint64_t rows, uint64_t columns,
+                                  float epsilon, const void *input, const void *residual,
+                                  const float *weight, const float *bias, void *sum, void *output,
+                                  float *mean, float *inverse_deviation);
+/* Its backward, from `gradient` (of the output) and `sum_gradient` (of s where it has other uses;
+ * may be NULL), with u = (s - m) * q and d = gradient * weight:
+ *   input_gradient = sum_gradient + q * (d - mean(d) - u * mean(u * d))   (of input and residual)
+ *   weight_gradient = sum over rows of gradient * u   (may be NULL)
+ *   bias_gradient = sum over rows of gradient         (may be NULL)
+ * input_gradient may be sum_gradient itself.  The parameters' sums have a fixed order and take the
+ * workspace (may be NULL without them).  No rows: they are 0. */
+oxh_status oxh_layer_norm_backward_workspace_size(uint64_t rows, uint64_t columns,
+                                                  uint64_t *bytes);
+oxh_status oxh_layer_norm_backward(oxh_stream stream, int dtype, uint64_t rows, uint64_t columns,
+                                   const void *gradient, const void *sum_gradient,
+                                   const void *sum, const float *weight, const float *mean,
+                                   const float *inverse_deviation, void *input_gradient,
+                                   float *weight_gradient, float *bias_gradient, void *workspace,
+                                   uint64_t workspace_bytes);
+
+/* Gated delta rule: per batch row and head a state S [key_dim, value_dim], float32, whose answer
+ * to a key each step moves towards a value:
+ *   a_t = sigmoid(gate_t);  b_t = sigmoid(write_t)
+ *   P = a_t S_{t-1};  S_t = P + b_t k_t (v_t - P' k_t)';  output_t = scale S_t' q_t
+ * query and key [batch, time, key_heads, key_dim], value and output [batch, time, heads,
+ * value_dim], gate and write [batch, time, heads], states [batch, heads, key_dim, value_dim]; head
+ * h reads key head h / (heads / key_heads).  From initial_state (NULL: 0); final_state (may be
+ * NULL) receives the last one and may be initial_state itself: single tokens are time 1 with the
+ * state in place.  lengths (device int32 [batch], may be NULL; clamped to 0..time): a row's steps
+ * at or past its length give 0 and leave the state, whatever the operands hold there.
+ * Keys of length 1 (or less) keep the state bounded.  A value of a row's own steps that is not
+ * finite may reach the outputs of its whole chunk of 64 steps.  bfloat16 operands: the state's own
+ * products keep 16 bits of what is formed on the way, the output's 8.
+ * `saved` (may be NULL) receives what the backward reads; a call without it takes up to 16 steps
+ * one by one, in float32.  OXH_INVALID_SHAPE above a key_dim of 128, a value_dim of 4096 or a
+ * batch of 65535, or where one launch cannot number the threads. */
+typedef struct oxh_delta_shape {
+  uint64_t batch, time, key_heads, heads, key_dim, value_dim;
+} oxh_delta_shape;
+oxh_status oxh_gated_delta_rule_saved_size(int dtype, const oxh_delta_shape *shape,
+                                           uint64_t *bytes);
+/* saves: whether the call passes `saved`. */
+oxh_status oxh_gated_delta_rule_workspace_size(int dtype, const oxh_delta_shape *shape, int saves,
+                                               uint64_t *bytes);
+oxh_status oxh_gated_delta_rule_forward(oxh_stream stream, int dtype, const oxh_delta_shape *shape,
+                                        float scale, const void *query, const void *key,
+                                        const void *value, const void *gate, const void *write,
+                                        const float *initial_state, const int32_t *lengths,
+                                        void *output, float *final_state, void *saved,
+                                        uint64_t saved_size, void *workspace,
+                                        uint64_t workspace_bytes);
+
+/* Its backward from `gradient` (of every output) and final_state_gradient (may be NULL), reading the
+ * forward's operands and what it saved.  initial_state_gradient may be NULL, or
+ * final_state_gradient itself.  Gradients of a key head's query and key are the sums over its value
+ * heads.  Steps at or past a row's length take gradients of 0. */
+oxh_status oxh_gated_delta_rule_backward_workspace_size(int dtype, const oxh_delta_shape *shape,
+                                                        uint64_t *bytes);
+oxh_status oxh_gated_delta_rule_backward(
+    oxh_stream stream, int dtype, const oxh_delta_shape *shape, float scale, const void *gradient,
+    const void *query, const void *key, const void *value, const void *gate, const void *write,
+    const void *saved, uint64_t saved_size, const float *final_state_gradient,
+    const int32_t *lengths, void *query_gradient, void *key_gradient, void *value_gradient,
+    void *gate_gradient, void *write_gradient, float *initial_state_gradient, void *workspace,
+    uint64_t workspace_bytes);
+
+/* Clipped policy loss with a KL term over rows of logits, from the action that was taken in each
+ * (a class index as float32, as cross entropy's targets), its log probability under the policy
+ * that took it, its advantage and, for kl > 0, its log probability under a reference:
+ *   l = log softmax(logits)[action];  r = exp(l - old);  d = reference - l
+ *   loss = sum of weight * (-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl (exp(d) - d - 1))
+ * weights NULL: 1 / rows each.  A row of weight 0 is not read.  Any of loss [1], log_probs [rows]
+ * (l; 0 for a row of weight 0) and gradient (of the logits, times outer_gradient[0]) may be NULL.
+ * The clip's borders belong to its inside.  An action that is no class index makes the loss, its
+ * row's gradient and log probability NaN and sets error_flag (may be NULL).  The workspace is the
+ * loss's. */
+oxh_status oxh_policy_loss_workspace_size(uint64_t rows, uint64_t classes, uint64_t *bytes);
+oxh_status oxh_policy_loss(oxh_stream stream, int dtype, uint64_t rows, uint64_t classes,
+                           float clip_low, float clip_high, float kl, const void *logits,
+                           const float *actions, const float *old_log_probs,
+                           const float *advantages, const float *reference_log_probs,
+                           const float *weights, const float *outer_gradient, float *loss,
+                           float *log_probs, void *gradient, uint32_t *error_flag,
+                           void *workspace, uint64_t workspace_bytes);
+
 /* Orthogonalises `count` matrices [rows, columns] (contiguous, float32) by Newton-Schulz
  * products: X = V / (|V|_F + epsilon), then `rounds` times
  *   A = X X';  B = b A + c A A;  X = a X + B X,   (a, b, c) = (3.4445, -4.7750, 2.0315)

@@ -24,8 +24,12 @@
 #include <string>
 
 #include "common.h"
+#include "softmax.h"
 
 namespace {
+
+using oxh::softmax::exp_nonpos;
+using oxh::softmax::target_index;
 
 // Row block shape for wide rows (overridable at build time for tuning sweeps): lanes per row
 // and the minimum waves per SIMD the register budget must allow.
@@ -68,16 +72,6 @@ struct CeArgs {
   double *row_loss;                       // workspace [batch]
   uint64_t batch, classes;
 };
-
-// evaluation.rs:622-636: finite, non-negative, integral and below `classes`.
-__device__ __forceinline__ bool target_index(float t, uint64_t classes, uint64_t &index) {
-  if (!isfinite(t) || t < 0.0f || t - truncf(t) != 0.0f) return false;
-  if (t >= 18446744073709551616.0f) return false;
-  const uint64_t i = static_cast<uint64_t>(t);
-  if (i >= classes) return false;
-  index = i;
-  return true;
-}
 
 // Block max: within each row of 16 lanes through DPP moves (xor 1, xor 2, mirrored half, mirrored
 // row: every lane then holds its row's max), the four rows through lane reads, then the waves
@@ -147,21 +141,6 @@ __global__ __launch_bounds__(kMeanBlock) void ce_mean_kernel(const double *__res
   }
   s = block_sum<kMeanBlock>(s, lds);
   if (threadIdx.x == 0) *loss = static_cast<float>(s) / static_cast<float>(batch);
-}
-
-// exp(d) for d = x - rowmax <= 0, within ~1.5 ulp: 2^(d * log2 e) with the product carried as
-// hi + lo (an exact fma residual plus d times the tail of log2 e), the hardware 2^x (v_exp_f32,
-// 1 ulp) on the fraction |f| <= 0.5 + 2^-24, and the integer part applied by ldexp.  NaN
-// propagates; d below -200 (including -inf) gives 0, as expf does.
-__device__ __forceinline__ float exp_nonpos(float d) {
-  constexpr float kLog2eHi = 1.44269502162933349609375f;  // nearest float to log2(e)
-  constexpr float kLog2eLo = 1.925963033500011e-08f;      // log2(e) - kLog2eHi
-  d = d < -200.0f ? -200.0f : d;
-  const float hi = d * kLog2eHi;
-  const float lo = fmaf(d, kLog2eLo, fmaf(d, kLog2eHi, -hi));
-  const float n = rintf(hi);
-  const float f = (hi - n) + lo;  // hi - n is exact
-  return ldexpf(__builtin_amdgcn_exp2f(f), static_cast<int>(n));
 }
 
 __device__ __forceinline__ float4 exp4_nonpos(const float4 &x, float m) {

@@ -1,0 +1,417 @@
+// delta_rule.h -- the gated delta rule's tiles (internal to the library): shapes, operands of the
+// matrix cores and where a call keeps them between its kernels.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <string>
+#include <type_traits>
+#include <vector>
+
+#include "common.h"
+#include "row_norm.h"
+#include "storage.h"
+
+namespace oxh {
+namespace delta {
+
+using storage::bf16;
+
+constexpr int kChunk = 64;  // steps of a chunk
+
+struct Dims {
+  uint32_t batch, time, key_heads, heads, keys, values;
+  uint32_t group, slabs;       // value heads of a key head; slabs of 16 value columns
+  uint32_t first, chunks;      // the chunks of this launch: [first, first + chunks)
+  const int32_t *lengths;      // may be null
+  float scale;
+};
+
+// Steps of batch row b.
+__device__ __forceinline__ uint32_t length_of(const Dims &d, uint32_t b) {
+  if (d.lengths == nullptr) return d.time;
+  const int32_t n = d.lengths[b];
+  return n <= 0 ? 0u : min(static_cast<uint32_t>(n), d.time);
+}
+
+// The matrix cores' 16 x 16 products take A as (row = lane % 16) and B as (column = lane % 16), both
+// with 8 values of the summed axis per lane, and leave C as (column = lane % 16, rows = 4 per lane
+// group of 16).  Which index of the summed axis a lane's values stand for is free as long as A and
+// B agree, and which index a row of a tile stands for is free altogether.  With rows numbered as
+// below, the C tiles 2 m and 2 m + 1 of a lane are its 8 consecutive indexes 32 m + 8 group + 0..7:
+// the result of one product is the B operand of the next as it stands, in the same registers.
+__device__ __forceinline__ uint32_t index_of(uint32_t tile, uint32_t row) {
+  return 32 * (tile >> 1) + ((row >> 2) << 3) + ((tile & 1) << 2) + (row & 3);
+}
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+// 8 values of a lane.
+template <typename T>
+struct Operand;
+template <>
+struct Operand<bf16> {
+  typedef bf16x8 type;
+};
+template <>
+struct Operand<float> {
+  typedef f32x8 type;
+};
+template <typename T>
+using operand = typename Operand<T>::type;
+
+// c + a b over 32 indexes.
+__device__ __forceinline__ f32x4 product(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 product(f32x8 a, f32x8 b, f32x4 c) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+  return c;
+}
+
+template <typename T>
+__device__ __forceinline__ operand<T> rounded(f32x8 v) {
+  return __builtin_convertvector(v, operand<T>);
+}
+__device__ __forceinline__ f32x8 widened(bf16x8 v) { return __builtin_convertvector(v, f32x8); }
+__device__ __forceinline__ f32x8 widened(f32x8 v) { return v; }
+
+// A float32 operand as bfloat16 ones that add up to it: to 2^-17 of each value with two.
+template <typename T, int Parts>
+struct Split {
+  operand<T> part[Parts];
+  __device__ __forceinline__ explicit Split(f32x8 v) {
+#pragma unroll
+    for (int p = 0; p < Parts; ++p) {
+      part[p] = rounded<T>(v);
+      if (p + 1 < Parts) v -= widened(part[p]);
+    }
+  }
+};
+template <typename T, int Parts>
+__device__ __forceinline__ f32x4 product(operand<T> a, const Split<T, Parts> &b, f32x4 c) {
+#pragma unroll
+  for (int p = Parts - 1; p >= 0; --p) c = product(a, b.part[p], c);
+  return c;
+}
+
+__device__ __forceinline__ f32x8 join(f32x4 low, f32x4 high) {
+  return __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// 8 consecutive values of a row of `count`, from place `at` on; those past its end are 0.
+template <typename T, bool Whole>
+__device__ __forceinline__ operand<T> load_row(const T *row, uint32_t at, uint32_t count) {
+  if (Whole || at + 8 <= count) {
+    operand<T> v;
+    if constexpr (sizeof(T) == 2) {
+      v = storage::raw<T, 8>(row + at);
+    } else {
+      const auto low = storage::raw<T, 4>(row + at), high = storage::raw<T, 4>(row + at + 4);
+      v = __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    return v;
+  }
+  operand<T> v = {};
+#pragma unroll
+  for (uint32_t i = 0; i < 8; ++i)
+    if (at + i < count) v[i] = row[at + i];
+  return v;
+}
+
+// Where the operands of a chunk lie, in units of a wave's operand (64 lanes, each its 8 values in
+// one piece).  Triangles of 64 x 64 are six operands: (tile, step) = (0,0) (1,0) (2,0) (2,1) (3,0)
+// (3,1) for the lower one, (0,0) (0,1) (1,0) (1,1) (2,1) (3,1) for its transpose.
+constexpr int kTriangle = 6;
+__device__ __forceinline__ int lower_place(int tile, int step) {
+  return tile < 2 ? tile : 2 * tile - 2 + step;
+}
+__device__ __forceinline__ int upper_place(int tile, int step) {
+  return tile < 2 ? 2 * tile + step : tile + 2;
+}
+
+// exp of the decay's sums of a chunk: from its start (`since`), to its end (`until`), and b.
+struct Gates {
+  float since[kChunk], until[kChunk], write[kChunk];
+};
+
+template <typename T>
+struct Chunk {  // per value head
+  static constexpr int kParts = sizeof(T) == 2 ? 2 : 1;
+  static constexpr uint64_t operand_bytes = 64 * 8 * sizeof(T);
+  static constexpr uint64_t gates = 0, system = sizeof(Gates),
+                            within = system + kTriangle * kParts * operand_bytes,
+                            bytes = within + kTriangle * operand_bytes;
+};
+
+__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
+// log sigmoid(x), not below -100: exp of it is 0 beside any other decay, and sums of it stay sums.
+__device__ __forceinline__ float log_sigmoid(float x) {
+  const float v = fminf(x, 0.0f) - log1pf(expf(-fabsf(x)));
+  return v < -100.0f ? -100.0f : x != x ? x : v;
+}
+
+// A chunk of a head: its rows, and where it lies among the rows' heads and the launch's chunks.
+struct Place {
+  uint32_t chunk, head, batch, key_head, begin, rows;
+  uint64_t row0, key_row, value_row;
+  __device__ __forceinline__ Place(const Dims &d, uint32_t chunk_, uint32_t head_, uint32_t batch_)
+      : chunk(chunk_), head(head_), batch(batch_), key_head(head_ / d.group) {
+    begin = (d.first + chunk) * kChunk;
+    const uint32_t length = length_of(d, batch);
+    rows = begin < length ? min(length - begin, static_cast<uint32_t>(kChunk)) : 0;
+    row0 = static_cast<uint64_t>(batch) * d.time + begin;
+    key_row = row0 * d.key_heads + key_head;  // times keys: the first row of its key head
+    value_row = row0 * d.heads + head;        // times values
+  }
+  __device__ __forceinline__ uint64_t head_chunk(const Dims &d) const {
+    return (static_cast<uint64_t>(batch) * d.heads + head) * d.chunks + chunk;
+  }
+  __device__ __forceinline__ uint64_t key_chunk(const Dims &d) const {
+    return (static_cast<uint64_t>(batch) * d.key_heads + key_head) * d.chunks + chunk;
+  }
+};
+
+template <typename T, int KT>
+struct System {
+  float mat[kChunk][68];  // A, then N
+  float inverse[4][16][20];
+  double sums[kChunk];
+  float betas[kChunk];
+  alignas(32) T tile[kChunk][32 * KT + 8];
+  __device__ __forceinline__ float between(uint32_t t, uint32_t i) const {
+    return expf(static_cast<float>(sums[t] - sums[i]));
+  }
+  __device__ __forceinline__ operand<T> key_row(uint32_t row, int step, uint32_t g) const {
+    return *reinterpret_cast<const operand<T> *>(&tile[row][32 * step + 8 * g]);
+  }
+};
+
+// The chunk's rows of a head of keys (or queries).  Steps past the row's length repeat its last one
+// with a decay of 1 and b = 0: nothing of them reaches a step of the row or the state.
+template <typename T, int KT, bool Whole>
+__device__ __forceinline__ void load_tile(T (&tile)[kChunk][32 * KT + 8], const Dims &d,
+                                          const Place &at, const T *from) {
+  const uint32_t r = threadIdx.x >> 2, part = threadIdx.x & 3;
+  const T *row = from + (at.key_row + static_cast<uint64_t>(min(r, at.rows - 1)) * d.key_heads) * d.keys;
+#pragma unroll
+  for (int i = 0; i < KT; ++i) {
+    const uint32_t k = (part + 4 * i) * 8;
+    *reinterpret_cast<operand<T> *>(&tile[r][k]) = load_row<T, Whole>(row, k, d.keys);
+  }
+}
+
+// Its transpose as operands: a lane its key index, 8 steps.
+template <typename T, int KT>
+__device__ __forceinline__ void store_transposed(const T (&tile)[kChunk][32 * KT + 8],
+                                                 operand<T> *to) {
+  const uint32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  for (int p = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); p < 4 * KT; p += 4) {
+    const uint32_t at = index_of(p >> 1, n), from = 32 * (p & 1) + 8 * g;
+    operand<T> v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = tile[from + i][at];
+    to[p * 64 + lane] = v;
+  }
+}
+
+// Leaves N of a chunk in m.mat (rows and columns in order), its keys in m.tile and its gates in
+// memory.  The last three of the block's four waves run `meanwhile` beside the first one's
+// inversions (keys and sums of the decay are there by then).
+template <typename T, int KT, bool Whole, typename Meanwhile>
+__device__ __forceinline__ void solve(System<T, KT> &m, const Dims &d, const Place &at,
+                                      const T *key, const T *gate, const T *write, Gates *gates,
+                                      Meanwhile meanwhile) {
+  const uint32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  load_tile<T, KT, Whole>(m.tile, d, at, key);
+  if (wave == 0) {
+    const uint64_t row = at.value_row + static_cast<uint64_t>(min(lane, at.rows - 1)) * d.heads;
+    const bool own = lane < at.rows;
+    const float decay = own ? log_sigmoid(storage::widen(gate[row])) : 0.0f;
+    const float beta = own ? sigmoid(storage::widen(write[row])) : 0.0f;
+    double sum = decay;
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) {
+      const double before = __shfl_up(sum, i);
+      if (lane >= static_cast<uint32_t>(i)) sum += before;
+    }
+    const double last = __shfl(sum, 63);
+    m.sums[lane] = sum;
+    m.betas[lane] = beta;
+    gates->since[lane] = expf(static_cast<float>(sum));
+    gates->until[lane] = expf(static_cast<float>(last - sum));
+    gates->write[lane] = beta;
+  }
+  __syncthreads();
+
+  // A: this wave's 16 steps against those of the tiles up to the end of their half
+  for (uint32_t it = 0; it <= (wave | 1); ++it) {
+    f32x4 acc = {};
+    if (it <= wave) {
+#pragma unroll
+      for (int s = 0; s < KT; ++s)
+        acc = product(m.key_row(16 * wave + n, s, g), m.key_row(16 * it + n, s, g), acc);
+    }
+    const uint32_t i = 16 * it + n;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const uint32_t t = 16 * wave + 4 * g + r;
+      m.mat[t][i] = i < t ? acc[r] * m.between(t, i) : 0.0f;
+    }
+  }
+  __syncthreads();
+
+  if (wave == 0) {
+    // (1 + A b) of each diagonal block of 16, inverted: a lane its column n of block g
+    float x[16];
+#pragma unroll
+    for (int t = 0; t < 16; ++t) {
+      x[t] = static_cast<uint32_t>(t) == n ? 1.0f : 0.0f;
+#pragma unroll
+      for (int i = 0; i < t; ++i)
+        x[t] = fmaf(-m.mat[16 * g + t][16 * g + i] * m.betas[16 * g + i], x[i], x[t]);
+      m.inverse[g][t][n] = x[t];
+    }
+  } else {
+    meanwhile();
+  }
+  __syncthreads();
+
+  // N by block rows, a wave its 16 columns: N_j = (1 + A b)_jj^-1 (A_j - sum over i < j of
+  // (A b)_ji N_i), the blocks above as they left the matrix cores
+  f32x4 solved[4];
+#pragma unroll
+  for (uint32_t j = 0; j < 4; ++j) {
+    if (j < wave) continue;
+    f32x4 acc;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) acc[r] = m.mat[16 * j + 4 * g + r][16 * wave + n];
+#pragma unroll
+    for (uint32_t i = 0; i < j; ++i) {
+      if (i < wave) continue;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t k = 16 * i + 4 * g + r;
+        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(-m.mat[16 * j + n][k] * m.betas[k],
+                                                   solved[i][r], acc, 0, 0, 0);
+      }
+    }
+    solved[j] = f32x4{};
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      solved[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(m.inverse[j][n][4 * g + r], acc[r],
+                                                       solved[j], 0, 0, 0);
+  }
+  __syncthreads();
+#pragma unroll
+  for (uint32_t j = 0; j < 4; ++j) {
+    if (j < wave) continue;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) m.mat[16 * j + 4 * g + r][16 * wave + n] = solved[j][r];
+  }
+  __syncthreads();
+}
+
+// ------------------------------------------------------------------------------------ host side
+
+constexpr uint64_t kMostKeys = 128;
+// Bytes of operands that a call prepares before it scans their chunks: what the last-level cache
+// holds beside the tensors.
+constexpr uint64_t kPrepared = 128ull << 20;
+
+inline uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
+
+struct Plan {
+  Dims d;
+  uint64_t all, segment, steps;  // chunks; those prepared at a time; 32 keys each
+  Plan(const oxh_delta_shape &s, float scale, const int32_t *lengths)
+      : d{static_cast<uint32_t>(s.batch), static_cast<uint32_t>(s.time),
+          static_cast<uint32_t>(s.key_heads), static_cast<uint32_t>(s.heads),
+          static_cast<uint32_t>(s.key_dim), static_cast<uint32_t>(s.value_dim),
+          static_cast<uint32_t>(s.heads / s.key_heads),
+          static_cast<uint32_t>((s.value_dim + 15) / 16), 0, 0, lengths, scale},
+        all((s.time + kChunk - 1) / kChunk), segment(0), steps(round_up(s.key_dim, 32) / 32) {}
+  uint64_t state_elements(const oxh_delta_shape &s) const {
+    return s.batch * s.heads * s.key_dim * s.value_dim;
+  }
+};
+
+// Calls run(32 keys each, whether they are whole).
+template <typename Run>
+void with_keys(uint64_t keys, Run run) {
+  auto whole = [&](auto steps) {
+    if (keys % 32 == 0) run(steps, std::true_type());
+    else run(steps, std::false_type());
+  };
+  if (keys <= 32) whole(std::integral_constant<int, 1>());
+  else if (keys <= 64) whole(std::integral_constant<int, 2>());
+  else if (keys <= 96) whole(std::integral_constant<int, 3>());
+  else whole(std::integral_constant<int, 4>());
+}
+
+inline oxh_status check_shape(int dtype, const oxh_delta_shape *s) {
+  OXH_REQUIRE(s != nullptr, OXH_INVALID_SHAPE, "gated delta rule: shape is null");
+  OXH_REQUIRE(storage::valid(dtype), OXH_INVALID_SHAPE,
+              "gated delta rule: dtype is neither OXH_F32 nor OXH_BF16");
+  OXH_REQUIRE(s->key_dim >= 1 && s->key_dim <= kMostKeys, OXH_INVALID_SHAPE,
+              "gated delta rule: key_dim must be 1..128");
+  OXH_REQUIRE(s->value_dim >= 1 && s->value_dim <= 4096, OXH_INVALID_SHAPE,
+              "gated delta rule: value_dim must be 1..4096");
+  OXH_REQUIRE(s->key_heads >= 1 && s->heads >= 1 && s->heads % s->key_heads == 0 &&
+                  s->heads <= 65535,
+              OXH_INVALID_SHAPE, "gated delta rule: heads must be a multiple of key_heads, at "
+                                 "most 65535");
+  OXH_REQUIRE(s->batch <= 65535, OXH_INVALID_SHAPE, "gated delta rule: batch above 65535");
+  OXH_REQUIRE(s->time < (1ull << 31) - kChunk, OXH_INVALID_SHAPE,
+              "gated delta rule: too many steps");
+  // one launch numbers its threads with 32 bits
+  const uint64_t heads = s->batch * s->heads;
+  OXH_REQUIRE(heads * std::max<uint64_t>((s->time + kChunk - 1) / kChunk, 1) <= (1ull << 23) &&
+                  heads * ((s->value_dim + 15) / 16) <= (1ull << 25),
+              OXH_INVALID_SHAPE, "gated delta rule: more heads and steps than one call takes");
+  return ok();
+}
+
+// Bytes of a call's tensors.
+struct Sizes {
+  uint64_t element, query, value, gate, state;
+  Sizes(int dtype, const oxh_delta_shape &s)
+      : element(storage::bytes_of(dtype)),
+        query(s.batch * s.time * s.key_heads * s.key_dim * element),
+        value(s.batch * s.time * s.heads * s.value_dim * element),
+        gate(s.batch * s.time * s.heads * element),
+        state(s.batch * s.heads * s.key_dim * s.value_dim * 4) {}
+};
+
+struct Span {
+  const void *p;
+  uint64_t bytes, align;
+};
+// Aligned to their elements; no output over an operand or another output.
+inline oxh_status check_apart(const std::vector<Span> &in, const std::vector<Span> &out) {
+  for (const auto *list : {&in, &out})
+    for (const Span &x : *list)
+      OXH_REQUIRE(row_norm::aligned_to(x.p, x.align), OXH_INVALID_SHAPE,
+                  "gated delta rule: a pointer is not aligned to its elements");
+  for (size_t o = 0; o < out.size(); ++o) {
+    if (out[o].p == nullptr) continue;
+    for (const Span &i : in)
+      OXH_REQUIRE(i.p == nullptr || !any_overlap(out[o].p, out[o].bytes, i.p, i.bytes),
+                  OXH_INVALID_SHAPE,
+                  "gated delta rule: an output, saved or the workspace overlaps an operand");
+    for (size_t k = 0; k < o; ++k)
+      OXH_REQUIRE(out[k].p == nullptr ||
+                      !any_overlap(out[o].p, out[o].bytes, out[k].p, out[k].bytes),
+                  OXH_INVALID_SHAPE, "gated delta rule: two outputs overlap");
+  }
+  return ok();
+}
+
+}  // namespace delta
+}  // namespace oxh

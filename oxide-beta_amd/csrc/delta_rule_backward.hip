@@ -1,0 +1,680 @@
+// delta_rule_backward.hip -- gradients of the gated delta rule (delta_rule.hip), by its chunks.
+//
+// With the notation there, u = b e, and the gradients do of the outputs and dS of the state behind
+// the chunk:
+//
+//   du = scale (G o q k')' do + exp(g_64 - g) k dS;  x = du - N' (b du);  dv = b x
+//   dS0 = exp(g_64) dS + scale q' (exp(g) do) - k' (exp(g) dv)
+//   M1 = scale G o (do u') (i <= t);  M2 = -G o (dv u') (i < t)
+//   dq = scale exp(g) do S0' + M1 k
+//   dk = -exp(g) dv S0' + exp(g_64 - g) u dS' + M1' q + (M2 + M2') k
+//   dwrite = (e . x) b (1 - b)
+//   dgate_s = (1 - a_s) (sum over t >= s of (q.dq - dk.k from S0) + over i < s of (k.dk from dS)
+//             + <dS, exp(g_64) S0> + over i < s <= t of H_ti),  H = G o (scale (do u') o q k'
+//             - (dv u') o k k')
+//
+// The last sum is that of (H's rows - its columns) over t >= s: the pairs that do not span s take
+// themselves away to the last bit, whatever their operands were rounded to.
+//
+// Three kernels: what depends on no state, for all chunks at once; the state's gradient from the
+// last chunk to the first, a wave for each 16 columns of values; and the products over the values,
+// a block per chunk and key head.  S0 and e are the forward's.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <string>
+#include <vector>
+
+#include "common.h"
+#include "delta_rule.h"
+#include "storage.h"
+
+namespace {
+
+using namespace oxh::delta;
+using oxh::storage::widen;
+
+// What a chunk's kernels leave each other, per value head; then per slab of 16 columns of values
+// dS as operands, the sums over its columns of e x, and <dS, exp(g_64) S0>.
+template <typename T>
+struct Back {
+  static constexpr uint64_t operand_bytes = Chunk<T>::operand_bytes, gates = 0,
+                            system = sizeof(Gates), within = system + kTriangle * operand_bytes,
+                            slabs = within + kTriangle * operand_bytes;
+  static __host__ __device__ constexpr uint64_t slab(uint64_t steps) {
+    return steps * operand_bytes + (kChunk + 8) * 4;
+  }
+  static __host__ __device__ constexpr uint64_t bytes(uint64_t steps, uint64_t count) {
+    return slabs + count * slab(steps);
+  }
+};
+
+template <typename T>
+struct Args {
+  Dims d;
+  const T *query, *key, *gate, *write, *gradient;
+  const char *saved;
+  char *heads, *keys;   // Back<T> of (batch, head, chunk); transposed keys, queries
+  const float *from;    // gradients of the states behind the launch's chunks, null: 0
+  float *to;            // and before them, may be null
+  T *dquery, *dkey, *dvalue, *dgate, *dwrite;
+  uint32_t all;         // chunks of the whole sequence
+};
+
+template <typename T, int KT, bool Whole>
+__global__ __launch_bounds__(256) void delta_backward_prepare_kernel(Args<T> a) {
+  using Op = operand<T>;
+  __shared__ System<T, KT> m;
+  const Dims &d = a.d;
+  const Place at(d, blockIdx.x, blockIdx.y, blockIdx.z);
+  if (at.rows == 0) return;
+  const uint32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const T *query = a.query + at.key_row * d.keys;
+  const uint64_t stride = static_cast<uint64_t>(d.key_heads) * d.keys;
+  char *out = a.heads + at.head_chunk(d) * Back<T>::bytes(KT, d.slabs);
+  solve<T, KT, Whole>(
+      m, d, at, a.key, a.gate, a.write, reinterpret_cast<Gates *>(out + Back<T>::gates), [&] {
+        // (G o q k')', a lane its key's step i, queries' steps t
+        const uint32_t first = wave == 1 ? 2 : wave - 2, last = wave == 1 ? 3 : wave - 2;
+        for (uint32_t ki = first; ki <= last; ++ki) {
+          const uint32_t i = index_of(ki, n);
+          for (int step = ki >> 1; step < 2; ++step) {
+            f32x4 half[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              f32x4 acc = {};
+              const T *row = query + min(index_of(2 * step + e, n), at.rows - 1) * stride;
+#pragma unroll
+              for (int s = 0; s < KT; ++s)
+                acc = product(load_row<T, Whole>(row, 32 * s + 8 * g, d.keys), m.key_row(i, s, g),
+                              acc);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const uint32_t t = 32 * step + 8 * g + 4 * e + r;
+                half[e][r] = i <= t ? acc[r] * m.between(t, i) * d.scale : 0.0f;
+              }
+            }
+            Op *to = reinterpret_cast<Op *>(out + Back<T>::within);
+            to[upper_place(ki, step) * 64 + lane] = rounded<T>(join(half[0], half[1]));
+          }
+        }
+      });
+  for (int p = wave; p < kTriangle; p += 4) {
+    const int ki = p < 4 ? p / 2 : p - 2, step = p < 4 ? p % 2 : 1;
+    const uint32_t i = index_of(ki, n);
+    f32x8 v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = m.mat[32 * step + 8 * g + j][i];
+    reinterpret_cast<Op *>(out + Back<T>::system)[p * 64 + lane] = rounded<T>(v);
+  }
+  if (at.head % d.group != 0) return;
+  Op *to = reinterpret_cast<Op *>(a.keys) + at.key_chunk(d) * (8 * KT * 64);
+  store_transposed<T, KT>(m.tile, to);
+  __syncthreads();
+  load_tile<T, KT, Whole>(m.tile, d, at, a.query);
+  __syncthreads();
+  store_transposed<T, KT>(m.tile, to + 4 * KT * 64);
+}
+
+// The sums over the 16 lanes of a group.
+__device__ __forceinline__ float row_total(float v) {
+  v += oxh::dpp_move<0xB1>(v);
+  v += oxh::dpp_move<0x4E>(v);
+  v += oxh::dpp_move<0x141>(v);
+  v += oxh::dpp_move<0x140>(v);
+  return v;
+}
+
+// A wave per 16 columns of a head's values, from the last chunk to the first.
+template <typename T, int KT, bool Whole>
+__global__ __launch_bounds__(256) void delta_backward_scan_kernel(Args<T> a) {
+  using Op = operand<T>;
+  const Dims &d = a.d;
+  const uint32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const uint32_t slab = blockIdx.x * (blockDim.x >> 6) +
+                        __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (slab >= d.slabs) return;
+  const uint32_t h = blockIdx.y, b = blockIdx.z;
+  const uint32_t column = 16 * slab + n;
+  const bool in = column < d.values;
+  const uint32_t col = in ? column : d.values - 1;
+  const uint64_t head = static_cast<uint64_t>(b) * d.heads + h;
+  const uint64_t stride = static_cast<uint64_t>(d.key_heads) * d.keys;
+  const uint64_t value_stride = static_cast<uint64_t>(d.heads) * d.values;
+  f32x4 ds[2 * KT];
+  const uint64_t state_at = head * d.keys * d.values + col;
+#pragma unroll
+  for (int i = 0; i < 2 * KT; ++i) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const uint32_t k = index_of(i, 4 * g + r);
+      ds[i][r] = a.from != nullptr && in && (Whole || k < d.keys)
+                     ? a.from[state_at + static_cast<uint64_t>(k) * d.values]
+                     : 0.0f;
+    }
+  }
+  for (uint32_t chunk = d.chunks; chunk-- != 0;) {
+    const Place at(d, chunk, h, b);
+    const uint32_t held = min(d.time - at.begin, static_cast<uint32_t>(kChunk)), rows = at.rows;
+    const uint64_t value_at = at.value_row * d.values + col;
+    T *dvalue = a.dvalue + value_at;
+    if (rows == 0) {
+      if (in)
+        for (uint32_t t = g; t < held; t += 4) dvalue[t * value_stride] = static_cast<T>(0.0f);
+      continue;
+    }
+    const T *key = a.key + at.key_row * d.keys;
+    const T *gradient = a.gradient + value_at;
+    char *block = a.heads + at.head_chunk(d) * Back<T>::bytes(KT, d.slabs);
+    const Gates *gates = reinterpret_cast<const Gates *>(block + Back<T>::gates);
+    const Op *system = reinterpret_cast<const Op *>(block + Back<T>::system) + lane;
+    const Op *within = reinterpret_cast<const Op *>(block + Back<T>::within) + lane;
+    const Op *keys = reinterpret_cast<const Op *>(a.keys) + at.key_chunk(d) * (8 * KT * 64) + lane;
+    const Op *queries = keys + 4 * KT * 64;
+    const Op *kept = reinterpret_cast<const Op *>(a.saved) +
+                     ((head * a.all + d.first + chunk) * d.slabs + slab) * ((KT + 2) * 64) + lane;
+    char *own = block + Back<T>::slabs + slab * Back<T>::slab(KT);
+    auto vec = [&](const float *v, int tile) {
+      return *reinterpret_cast<const f32x4 *>(v + 32 * (tile >> 1) + 8 * g + 4 * (tile & 1));
+    };
+
+    Op out[2], decayed[2];  // do, and scale exp(g) do
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      f32x8 v;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t t = 32 * s + 8 * g + j;
+        v[j] = t < rows && in ? widen(gradient[t * value_stride]) : 0.0f;
+      }
+      out[s] = rounded<T>(v);
+      decayed[s] = rounded<T>(v * join(vec(gates->since, 2 * s), vec(gates->since, 2 * s + 1)) *
+                              d.scale);
+    }
+    // the state's gradient as an operand, its dot product with the state and its product with keys
+    f32x4 w[4] = {};
+    float across = 0.0f;
+    const float whole = gates->since[kChunk - 1];
+#pragma unroll
+    for (int s = 0; s < KT; ++s) {
+      const f32x8 v = join(ds[2 * s], ds[2 * s + 1]), state = widened(kept[s * 64]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) across = fmaf(v[j], state[j], across);
+      const Op op = rounded<T>(v);
+      reinterpret_cast<Op *>(own)[s * 64 + lane] = op;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = product(load_row<T, Whole>(key + min(index_of(i, n), rows - 1) * stride,
+                                          32 * s + 8 * g, d.keys), op, w[i]);
+    }
+    across *= whole;
+    f32x4 x[4];
+    {
+      f32x4 du[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        du[i] = vec(gates->until, i) * w[i];
+#pragma unroll
+        for (int s = i >> 1; s < 2; ++s) du[i] = product(within[upper_place(i, s) * 64], out[s], du[i]);
+        x[i] = du[i];
+        du[i] *= -vec(gates->write, i);
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const Op weighted = rounded<T>(join(du[2 * s], du[2 * s + 1]));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if ((i >> 1) <= s) x[i] = product(system[upper_place(i, s) * 64], weighted, x[i]);
+      }
+    }
+    f32x4 dv[4], errors[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      dv[i] = vec(gates->write, i) * x[i];
+      const f32x8 e = widened(kept[(KT + (i >> 1)) * 64]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t t = index_of(i, 4 * g + r);
+        errors[i][r] = row_total(e[4 * (i & 1) + r] * x[i][r]);
+        if (t < held && in) dvalue[t * value_stride] = static_cast<T>(dv[i][r]);
+      }
+    }
+    {
+      float total[1] = {across};
+      oxh::wave_sums_rows(total);
+      float *sums = reinterpret_cast<float *>(own + KT * Back<T>::operand_bytes);
+      if (n == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<f32x4 *>(sums + index_of(i, 4 * g)) = errors[i];
+      }
+      if (lane == 0) sums[kChunk] = total[0];
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * KT; ++i) ds[i] *= whole;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const Op taken = rounded<T>(join(-vec(gates->since, 2 * s) * dv[2 * s],
+                                       -vec(gates->since, 2 * s + 1) * dv[2 * s + 1]));
+#pragma unroll
+      for (int i = 0; i < 2 * KT; ++i) {
+        ds[i] = product(queries[(2 * i + s) * 64], decayed[s], ds[i]);
+        ds[i] = product(keys[(2 * i + s) * 64], taken, ds[i]);
+      }
+    }
+  }
+  if (a.to == nullptr || !in) return;
+#pragma unroll
+  for (int i = 0; i < 2 * KT; ++i) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const uint32_t k = index_of(i, 4 * g + r);
+      if (Whole || k < d.keys) a.to[state_at + static_cast<uint64_t>(k) * d.values] = ds[i][r];
+    }
+  }
+}
+
+constexpr int kColumns = 32;  // of values that the products take at a time
+
+template <typename T, int KT>
+struct Products {
+  union {
+    struct {
+      alignas(32) T state[32 * KT][kColumns + 8], gradient[32 * KT][kColumns + 8];
+      alignas(32) T wrote[kChunk][kColumns + 8];
+    };
+    alignas(16) float rows[kChunk][32 * KT + 4];
+  };
+  alignas(32) T one[kChunk][kChunk + 8], one_t[kChunk][kChunk + 8], two[kChunk][kChunk + 8];
+  double sums[kChunk];
+  float rows_at[kChunk], columns_at[4][kChunk], before[kChunk];
+};
+
+// A block per chunk and key head, its value heads in turn; a wave 16 of the steps.
+template <typename T, int KT, bool Whole, bool WholeValues>
+__global__ __launch_bounds__(256) void delta_backward_products_kernel(Args<T> a) {
+  using Op = operand<T>;
+  __shared__ Products<T, KT> m;
+  const Dims &d = a.d;
+  const uint32_t chunk = blockIdx.x, kh = blockIdx.y, b = blockIdx.z;
+  const uint32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t row = threadIdx.x >> 2, part = threadIdx.x & 3;  // of the results' rows
+  const uint64_t stride = static_cast<uint64_t>(d.key_heads) * d.keys;
+  const uint64_t value_stride = static_cast<uint64_t>(d.heads) * d.values;
+  f32x8 dq[KT] = {}, dk[KT] = {};
+  const Place first(d, chunk, kh * d.group, b);
+  const uint32_t held = min(d.time - first.begin, static_cast<uint32_t>(kChunk)), rows = first.rows;
+  const Op *keys = reinterpret_cast<const Op *>(a.keys) + first.key_chunk(d) * (8 * KT * 64) + lane;
+  const Op *queries = keys + 4 * KT * 64;
+  for (uint32_t h = kh * d.group; h < (kh + 1) * d.group; ++h) {
+    const Place at(d, chunk, h, b);
+    if (rows == 0) {
+      if (threadIdx.x < held) {
+        const uint64_t to = at.value_row + static_cast<uint64_t>(threadIdx.x) * d.heads;
+        a.dgate[to] = a.dwrite[to] = static_cast<T>(0.0f);
+      }
+      continue;
+    }
+    const char *block = a.heads + at.head_chunk(d) * Back<T>::bytes(KT, d.slabs);
+    const Gates *gates = reinterpret_cast<const Gates *>(block + Back<T>::gates);
+    const uint64_t value_at = at.value_row * d.values;
+    const uint64_t head = static_cast<uint64_t>(b) * d.heads + h;
+    f32x4 one[4] = {}, two[4] = {}, q1[2 * KT] = {}, k1[2 * KT] = {}, k2[2 * KT] = {};
+    const uint32_t t_row = 16 * wave + n;  // this lane's row of the operands from the left
+    for (uint32_t v0 = 0; v0 < d.values; v0 += kColumns) {
+      __syncthreads();  // the columns before, or the rows of the head before
+      // two slabs of states, their gradients and errors; those past the last are 0
+      for (uint32_t i = wave; i < 2 * KT + 4; i += 4) {
+        const uint32_t s = i < 2 * KT ? i % KT : i & 1;
+        const uint32_t half = i < 2 * KT ? i / KT : (i - 2 * KT) >> 1, slab = v0 / 16 + half;
+        const bool there = slab < d.slabs;
+        const Op *kept = reinterpret_cast<const Op *>(a.saved) + lane +
+                         ((head * a.all + d.first + chunk) * d.slabs + slab) * ((KT + 2) * 64);
+        const uint32_t c = 16 * half + n;
+        if (i < 2 * KT) {
+          Op state = {}, gradient = {};
+          if (there) {
+            state = kept[s * 64];
+            gradient = reinterpret_cast<const Op *>(block + Back<T>::slabs +
+                                                    slab * Back<T>::slab(KT))[s * 64 + lane];
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            m.state[32 * s + 8 * g + j][c] = state[j];
+            m.gradient[32 * s + 8 * g + j][c] = gradient[j];
+          }
+        } else {
+          f32x8 e = {};
+          if (there) e = widened(kept[(KT + s) * 64]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t t = 32 * s + 8 * g + j;
+            m.wrote[t][c] = static_cast<T>(e[j] * gates->write[t]);
+          }
+        }
+      }
+      Op out = {}, dv = {};
+      if (t_row < rows) {
+        const uint64_t from = value_at + t_row * value_stride;
+        if (WholeValues || v0 + 8 * g < d.values) {
+          out = load_row<T, WholeValues>(a.gradient + from, v0 + 8 * g, d.values);
+          dv = load_row<T, WholeValues>(a.dvalue + from, v0 + 8 * g, d.values);
+        }
+      }
+      __syncthreads();
+      auto wrote = [&](uint32_t r) { return *reinterpret_cast<const Op *>(&m.wrote[r][8 * g]); };
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) {
+        if (i > wave) continue;
+        const Op u = wrote(16 * i + n);
+        one[i] = product(out, u, one[i]);
+        two[i] = product(dv, u, two[i]);
+      }
+      const Op own = wrote(t_row);
+#pragma unroll
+      for (int i = 0; i < 2 * KT; ++i) {
+        const uint32_t k = index_of(i, n);
+        const Op state = *reinterpret_cast<const Op *>(&m.state[k][8 * g]);
+        q1[i] = product(out, state, q1[i]);
+        k1[i] = product(dv, state, k1[i]);
+        k2[i] = product(own, *reinterpret_cast<const Op *>(&m.gradient[k][8 * g]), k2[i]);
+      }
+    }
+    if (threadIdx.x < kChunk) {
+      // the sums of the decay again, as the first kernel formed them
+      const uint64_t from = at.value_row + static_cast<uint64_t>(min(lane, rows - 1)) * d.heads;
+      double sum = lane < rows ? log_sigmoid(widen(a.gate[from])) : 0.0f;
+#pragma unroll
+      for (int i = 1; i < 64; i *= 2) {
+        const double before = __shfl_up(sum, i);
+        if (lane >= static_cast<uint32_t>(i)) sum += before;
+      }
+      m.sums[lane] = sum;
+    }
+    const T *query = a.query + at.key_row * d.keys, *key = a.key + at.key_row * d.keys;
+    auto operand_at = [&](const T *p, uint32_t r, int step) {
+      return load_row<T, Whole>(p + min(r, rows - 1) * stride, 32 * step + 8 * g, d.keys);
+    };
+    // q k' and k k' again, for what their pairs' decays are worth
+    f32x4 qk[4] = {}, kk[4] = {};
+#pragma unroll
+    for (int s = 0; s < KT; ++s) {
+      const Op q = operand_at(query, t_row, s), k = operand_at(key, t_row, s);
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) {
+        if (i > wave) continue;
+        const Op other = operand_at(key, 16 * i + n, s);
+        qk[i] = product(q, other, qk[i]);
+        kk[i] = product(k, other, kk[i]);
+      }
+    }
+    __syncthreads();
+    float across[4] = {};  // H's rows
+#pragma unroll
+    for (uint32_t it = 0; it < 4; ++it) {
+      const uint32_t i = 16 * it + n;
+      float down = 0.0f;  // and columns
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t t = 16 * wave + 4 * g + r;
+        const float between = i <= t ? expf(static_cast<float>(m.sums[t] - m.sums[i])) : 0.0f;
+        const float x = i <= t ? one[it][r] * between * d.scale : 0.0f;
+        m.one[t][i] = static_cast<T>(x);
+        m.one_t[i][t] = static_cast<T>(x);
+        if (i < t) {
+          const float y = -two[it][r] * between, pair = x * qk[it][r] + y * kk[it][r];
+          m.two[t][i] = static_cast<T>(y);
+          m.two[i][t] = static_cast<T>(y);
+          across[r] += pair;
+          down += pair;
+        } else if (i == t) {
+          m.two[t][t] = static_cast<T>(0.0f);
+        }
+      }
+      down += __shfl_xor(down, 16);
+      down += __shfl_xor(down, 32);
+      if (g == 0) m.columns_at[wave][i] = down;
+    }
+    const f32x4 since = *reinterpret_cast<const f32x4 *>(gates->since + 16 * wave + 4 * g);
+    const f32x4 until = *reinterpret_cast<const f32x4 *>(gates->until + 16 * wave + 4 * g);
+#pragma unroll
+    for (int i = 0; i < 2 * KT; ++i) {
+      q1[i] *= since * d.scale;
+      k1[i] *= -since;
+      k2[i] *= until;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const uint32_t t = 16 * wave + 4 * g + r;
+      const uint64_t from = min(t, rows - 1) * stride;
+      float after = across[r], before = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 2 * KT; ++i) {
+        const uint32_t k = index_of(i, n);
+        if (!Whole && k >= d.keys) continue;
+        const float own = widen(key[from + k]);
+        after = fmaf(widen(query[from + k]), q1[i][r], fmaf(own, k1[i][r], after));
+        before = fmaf(own, k2[i][r], before);
+      }
+      after = row_total(after);
+      before = row_total(before);
+      if (n == 0) {
+        m.rows_at[t] = after;
+        m.before[t] = before;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * KT; ++i) k1[i] += k2[i];
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const Op x = *reinterpret_cast<const Op *>(&m.one[t_row][32 * s + 8 * g]);
+      const Op xt = *reinterpret_cast<const Op *>(&m.one_t[t_row][32 * s + 8 * g]);
+      const Op y = *reinterpret_cast<const Op *>(&m.two[t_row][32 * s + 8 * g]);
+#pragma unroll
+      for (int i = 0; i < 2 * KT; ++i) {
+        const Op k = keys[(2 * i + s) * 64];
+        q1[i] = product(x, k, q1[i]);
+        k1[i] = product(y, k, k1[i]);
+        k1[i] = product(xt, queries[(2 * i + s) * 64], k1[i]);
+      }
+    }
+    // the rows whole: each thread 8 keys at a time of its row
+    auto rows_of = [&](const f32x4 (&v)[2 * KT]) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 2 * KT; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) m.rows[16 * wave + 4 * g + r][index_of(i, n)] = v[i][r];
+      __syncthreads();
+    };
+    auto piece = [&](int i) {
+      const float *p = &m.rows[row][(part + 4 * i) * 8];
+      return join(*reinterpret_cast<const f32x4 *>(p), *reinterpret_cast<const f32x4 *>(p + 4));
+    };
+    rows_of(q1);
+#pragma unroll
+    for (int i = 0; i < KT; ++i) dq[i] += piece(i);
+    rows_of(k1);
+#pragma unroll
+    for (int i = 0; i < KT; ++i) dk[i] += piece(i);
+    if (threadIdx.x < kChunk) {
+      float error = 0.0f, constant = 0.0f;
+      for (uint32_t slab = 0; slab < d.slabs; ++slab) {
+        const float *sums = reinterpret_cast<const float *>(
+            block + Back<T>::slabs + slab * Back<T>::slab(KT) + KT * Back<T>::operand_bytes);
+        error += sums[lane];
+        constant += sums[kChunk];
+      }
+      float after = m.rows_at[lane], before = m.before[lane];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) after -= m.columns_at[i][lane];
+      const float own = before;
+#pragma unroll
+      for (int i = 1; i < 64; i *= 2) {
+        const float x = __shfl_down(after, i), y = __shfl_up(before, i);
+        if (lane + i < 64) after += x;
+        if (lane >= static_cast<uint32_t>(i)) before += y;
+      }
+      if (lane < held) {
+        const uint64_t to = at.value_row + static_cast<uint64_t>(lane) * d.heads;
+        const bool live = lane < rows;
+        const float beta = gates->write[lane], decay = after + (before - own) + constant;
+        a.dgate[to] = static_cast<T>(live ? decay * sigmoid(-widen(a.gate[to])) : 0.0f);
+        a.dwrite[to] =
+            static_cast<T>(live ? error * beta * sigmoid(-widen(a.write[to])) : 0.0f);
+      }
+    }
+  }
+  if (row >= held) return;
+  const bool live = row < rows;
+  const uint64_t to = first.key_row * d.keys + row * stride;
+#pragma unroll
+  for (int i = 0; i < KT; ++i) {
+    const uint32_t k = (part + 4 * i) * 8;
+    const operand<T> x = rounded<T>(dq[i]), y = rounded<T>(dk[i]);
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) {
+      if (!Whole && k + j >= d.keys) continue;
+      a.dquery[to + k + j] = live ? x[j] : static_cast<T>(0.0f);
+      a.dkey[to + k + j] = live ? y[j] : static_cast<T>(0.0f);
+    }
+  }
+}
+
+template <typename T>
+struct BackPlan {
+  Plan p;
+  uint64_t head_bytes, key_bytes, state_bytes;
+  uint64_t bytes() const { return head_bytes + key_bytes + state_bytes; }
+  explicit BackPlan(const oxh_delta_shape &s, float scale, const int32_t *lengths)
+      : p(s, scale, lengths) {
+    const uint64_t head = s.batch * s.heads * Back<T>::bytes(p.steps, p.d.slabs);
+    const uint64_t key = s.batch * s.key_heads * p.steps * 8 * Chunk<T>::operand_bytes;
+    p.segment = std::min(p.all, std::max<uint64_t>(1, kPrepared / std::max<uint64_t>(1, head + key)));
+    head_bytes = round_up(p.segment * head, 256);
+    key_bytes = round_up(p.segment * key, 256);
+    state_bytes = p.segment < p.all ? round_up(p.state_elements(s) * 4, 256) : 0;
+  }
+};
+
+template <typename T>
+oxh_status backward(hipStream_t stream, const BackPlan<T> &plan, Args<T> a, const float *final,
+                    float *initial, char *workspace) {
+  a.heads = workspace;
+  a.keys = a.heads + plan.head_bytes;
+  float *between = reinterpret_cast<float *>(a.keys + plan.key_bytes);
+  const Plan &p = plan.p;
+  a.all = static_cast<uint32_t>(p.all);
+  const uint64_t launches = (p.all + p.segment - 1) / p.segment;
+  for (uint64_t i = launches; i-- != 0;) {
+    const uint64_t first = i * p.segment;
+    a.d = p.d;
+    a.d.first = static_cast<uint32_t>(first);
+    a.d.chunks = static_cast<uint32_t>(std::min(p.segment, p.all - first));
+    a.from = i + 1 == launches ? final : between;
+    a.to = i == 0 ? initial : between;
+    const Dims &d = a.d;
+    with_keys(d.keys, [&](auto steps, auto whole) {
+      constexpr int KT = decltype(steps)::value;
+      constexpr bool W = decltype(whole)::value;
+      oxh::launch(delta_backward_prepare_kernel<T, KT, W>, dim3(d.chunks, d.heads, d.batch),
+                  dim3(256), 0, stream, a);
+      oxh::launch(delta_backward_scan_kernel<T, KT, W>, dim3(d.slabs, d.heads, d.batch), dim3(64),
+                  0, stream, a);
+      const dim3 grid(d.chunks, d.key_heads, d.batch);
+      if (d.values % kColumns == 0)
+        oxh::launch(delta_backward_products_kernel<T, KT, W, true>, grid, dim3(256), 0, stream, a);
+      else
+        oxh::launch(delta_backward_products_kernel<T, KT, W, false>, grid, dim3(256), 0, stream, a);
+    });
+    oxh_status st = oxh::launched("gated_delta_rule_backward");
+    if (st != OXH_OK) return st;
+  }
+  return oxh::ok();
+}
+
+}  // namespace
+
+extern "C" {
+
+oxh_status oxh_gated_delta_rule_backward_workspace_size(int dtype, const oxh_delta_shape *shape,
+                                                        uint64_t *bytes) {
+  OXH_REQUIRE(bytes != nullptr, OXH_INVALID_SHAPE, "bytes is null");
+  oxh_status st = check_shape(dtype, shape);
+  if (st != OXH_OK) return st;
+  *bytes = dtype == OXH_F32 ? BackPlan<float>(*shape, 1.0f, nullptr).bytes()
+                            : BackPlan<bf16>(*shape, 1.0f, nullptr).bytes();
+  return oxh::ok();
+}
+
+oxh_status oxh_gated_delta_rule_backward(
+    oxh_stream stream, int dtype, const oxh_delta_shape *shape, float scale, const void *gradient,
+    const void *query, const void *key, const void *value, const void *gate, const void *write,
+    const void *saved, uint64_t saved_size, const float *final_state_gradient,
+    const int32_t *lengths, void *query_gradient, void *key_gradient, void *value_gradient,
+    void *gate_gradient, void *write_gradient, float *initial_state_gradient, void *workspace,
+    uint64_t workspace_bytes) {
+  oxh_status st = check_shape(dtype, shape);
+  if (st != OXH_OK) return st;
+  const oxh_delta_shape &s = *shape;
+  OXH_REQUIRE(std::isfinite(scale), OXH_EXECUTION, "gated delta rule: scale must be finite");
+  if (s.batch == 0) return oxh::ok();
+  const Sizes z(dtype, s);
+  uint64_t kept = 0, needed = 0;
+  st = oxh_gated_delta_rule_saved_size(dtype, shape, &kept);
+  if (st == OXH_OK) st = oxh_gated_delta_rule_backward_workspace_size(dtype, shape, &needed);
+  if (st != OXH_OK) return st;
+  std::vector<Span> in = {{gradient, z.value, z.element}, {query, z.query, z.element},
+                          {key, z.query, z.element},      {value, z.value, z.element},
+                          {gate, z.gate, z.element},      {write, z.gate, z.element},
+                          {saved, kept, 16}};
+  std::vector<Span> out = {{query_gradient, z.query, z.element}, {key_gradient, z.query, z.element},
+                           {value_gradient, z.value, z.element}, {gate_gradient, z.gate, z.element},
+                           {write_gradient, z.gate, z.element},  {workspace, needed, 16}};
+  for (const auto *list : {&in, &out})
+    for (const Span &x : *list)
+      OXH_REQUIRE(x.p != nullptr || x.bytes == 0, OXH_INVALID_SHAPE,
+                  "gated delta rule backward: null pointer");
+  OXH_REQUIRE(saved_size >= kept, OXH_INVALID_SHAPE,
+              "gated delta rule backward: saved is too small");
+  OXH_REQUIRE(workspace_bytes >= needed, OXH_INVALID_SHAPE,
+              "gated delta rule backward: workspace too small");
+  in.push_back({lengths, s.batch * 4, 4});
+  // the initial state's gradient may be written over the final one's
+  out.push_back({initial_state_gradient, z.state, 4});
+  if (final_state_gradient != initial_state_gradient) in.push_back({final_state_gradient, z.state, 4});
+  st = check_apart(in, out);
+  if (st != OXH_OK) return st;
+  hipStream_t on = oxh::as_stream(stream);
+  if (s.time == 0) {
+    if (initial_state_gradient == nullptr || initial_state_gradient == final_state_gradient)
+      return oxh::ok();
+    if (final_state_gradient == nullptr)
+      return oxh_memset0_async(initial_state_gradient, z.state, stream);
+    return oxh_memcpy_d2d_async(initial_state_gradient, final_state_gradient, z.state, stream);
+  }
+  auto run = [&](auto type) {
+    using T = decltype(type);
+    Args<T> a{};
+    a.query = static_cast<const T *>(query);
+    a.key = static_cast<const T *>(key);
+    a.gate = static_cast<const T *>(gate);
+    a.write = static_cast<const T *>(write);
+    a.gradient = static_cast<const T *>(gradient);
+    a.saved = static_cast<const char *>(saved);
+    a.dquery = static_cast<T *>(query_gradient);
+    a.dkey = static_cast<T *>(key_gradient);
+    a.dvalue = static_cast<T *>(value_gradient);
+    a.dgate = static_cast<T *>(gate_gradient);
+    a.dwrite = static_cast<T *>(write_gradient);
+    return backward<T>(on, BackPlan<T>(s, scale, lengths), a, final_state_gradient,
+                       initial_state_gradient, static_cast<char *>(workspace));
+  };
+  return dtype == OXH_F32 ? run(float()) : run(bf16());
+}
+
+}  // extern "C"

@@ -19,31 +19,17 @@
 #include <string>
 
 #include "common.h"
+#include "row_norm.h"
 #include "storage.h"
 
 namespace {
 
+using namespace oxh::row_norm;
 using oxh::storage::bf16;
 using oxh::storage::load_places;
 using oxh::storage::Places;
 using oxh::storage::places_at;
 using oxh::storage::store_places;
-
-// The sum over a row's Lanes threads (whole waves) in one fixed order, in every thread.  `slot`
-// is a buffer of 16 floats; consecutive calls alternate between two.
-template <int Lanes>
-__device__ __forceinline__ float row_sum(float v, float *slot) {
-  float one[1] = {v};
-  oxh::wave_sums_rows(one);
-  if constexpr (Lanes == 64) return one[0];
-  const int wave = threadIdx.x >> 6;
-  if ((threadIdx.x & 63) == 0) slot[wave] = one[0];
-  __syncthreads();
-  float total = 0.0f;
-#pragma unroll
-  for (int i = 0; i < Lanes / 64; ++i) total += slot[i];
-  return total;
-}
 
 template <typename T>
 struct Forward {
@@ -265,30 +251,6 @@ __global__ __launch_bounds__(1024) void rms_norm_backward_long_kernel(Backward<T
   }
 }
 
-// out[c] = sum over the partial rows: 16 columns per block (from `first` on), 64 strands of rows
-// each, a strand's rows in order and the strands by halves.
-__global__ __launch_bounds__(1024) void rms_norm_weight_kernel(const float *partial, float *out,
-                                                               uint32_t rows, uint32_t columns,
-                                                               uint32_t first) {
-  __shared__ float part[64][17];
-  const uint32_t c = threadIdx.x & 15, strand = threadIdx.x >> 4;
-  const uint32_t column = first + blockIdx.x * 16 + c;
-  float sum = 0.0f;
-  if (column < columns) {
-#pragma unroll 8
-    for (uint32_t r = strand; r < rows; r += 64)
-      sum += partial[static_cast<uint64_t>(r) * columns + column];
-  }
-  part[strand][c] = sum;
-  __syncthreads();
-#pragma unroll
-  for (uint32_t half = 32; half != 0; half /= 2) {
-    if (strand < half) part[strand][c] += part[strand + half][c];
-    __syncthreads();
-  }
-  if (strand == 0 && column < columns) out[column] = part[0][c];
-}
-
 // Values of a row that a block's registers hold.  The backward keeps five per value of its row and
 // its masks need more: past these limits the registers spill, and two passes are faster (bfloat16
 // 1024 x 32769: 146 us, 441 in registers; float32 512 x 20001: 53 and 105; within the limits
@@ -298,66 +260,6 @@ constexpr uint64_t forward_limit() {
   return 1024 * 8 * (16 / sizeof(T));
 }
 constexpr uint64_t backward_limit(bool ragged) { return ragged ? 16384 : 32768; }
-
-template <int Lanes, int Chunks>
-struct Shape {
-  static constexpr int lanes = Lanes, chunks = Chunks;
-};
-
-// Calls run(Shape<lanes, chunks>) with the fewest threads per row that keep it within 8 accesses,
-// and where that is one wave within 32 values, each.  Limit: columns never exceed it.
-template <int N, uint64_t Limit, typename Run>
-void with_shape(uint64_t columns, Run run) {
-  const uint64_t packs = (columns + N - 1) / N;
-  if constexpr (N == 1) {  // rows of fewer values than an access
-    run(Shape<64, 1>());
-  } else {
-    if (packs <= 64) return run(Shape<64, 1>());
-    if (packs <= 128) return run(Shape<64, 2>());
-    if (packs <= 256) return run(Shape<64, 4>());
-    if (packs <= 512) return run(std::conditional_t<N <= 4, Shape<64, 8>, Shape<256, 2>>());
-    if (packs <= 1024) return run(Shape<256, 4>());
-    if (Limit / N <= 2048 || packs <= 2048) return run(Shape<256, 8>());
-    if constexpr (Limit / N > 2048)
-      if (Limit / N <= 4096 || packs <= 4096) return run(Shape<1024, 4>());
-    if constexpr (Limit / N > 4096) run(Shape<1024, 8>());
-  }
-}
-
-// Calls run(pack, ragged) for rows of these columns: 16 bytes per access, or one value where a row
-// has fewer.
-template <typename T, typename Run>
-void with_pack(uint64_t columns, Run run) {
-  constexpr int kPack = 16 / sizeof(T);
-  typedef std::integral_constant<int, kPack> Packed;
-  if (columns % kPack == 0) run(Packed(), std::false_type());
-  else if (columns > kPack) run(Packed(), std::true_type());
-  else run(std::integral_constant<int, 1>(), std::false_type());
-}
-
-// Blocks that the backward's weight gradient is summed over (rows of `partial`, which stays within
-// 8 MB up to 8192 columns).
-uint64_t block_limit(uint64_t columns) {
-  return std::min<uint64_t>(2048, std::max<uint64_t>(256, (1ull << 21) / columns));
-}
-
-oxh_status check_rows(const char *what, int dtype, uint64_t rows, uint64_t columns) {
-  OXH_REQUIRE(oxh::storage::valid(dtype), OXH_INVALID_SHAPE,
-              std::string(what) + ": dtype is neither OXH_F32 nor OXH_BF16");
-  OXH_REQUIRE(columns >= 1 && columns < (1ull << 31), OXH_INVALID_SHAPE,
-              std::string(what) + ": columns out of range");
-  OXH_REQUIRE(rows < (1ull << 31), OXH_INVALID_SHAPE, std::string(what) + ": too many rows");
-  OXH_REQUIRE(rows <= (1ull << 60) / columns, OXH_INVALID_SHAPE,
-              std::string(what) + ": element count overflow");
-  return oxh::ok();
-}
-
-bool aligned_to(const void *p, uint64_t bytes) {
-  return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0;
-}
-
-// Blocks of so many threads that one launch takes: it numbers its threads with 32 bits.
-constexpr uint64_t most_blocks(uint64_t threads) { return (1ull << 31) / threads; }
 
 // The rows in as many launches as that asks for (two from 2^25 rows of a wave each), `per` rows a
 // block: run(blocks, rows' arguments).
@@ -398,12 +300,6 @@ oxh_status forward(hipStream_t stream, const Forward<T> &a) {
   return oxh::launched("rms_norm_forward");
 }
 
-// Rows that one block takes by itself, whose share is the weight gradient: a second launch is about
-// as long as three more rows of a wave, or one of a block (bfloat16 16 x 1024: 7.2 us a call, 10.1
-// with two launches; 32 x 1024: 8.3 and 10.1, but 9.3 and 6.0 on the device; float32 2 x 4096: 7.4
-// and 10.1; 8 x 4096: 13.7 and 10.2).
-constexpr uint64_t rows_alone(int groups) { return groups > 1 ? 4 * groups : 2; }
-
 template <typename T>
 oxh_status backward(hipStream_t stream, Backward<T> a, float *weight_gradient) {
   uint64_t blocks = std::min<uint64_t>(a.rows, block_limit(a.columns));
@@ -434,11 +330,8 @@ oxh_status backward(hipStream_t stream, Backward<T> a, float *weight_gradient) {
   }
   oxh_status st = oxh::launched("rms_norm_backward");
   if (st != OXH_OK || weight_gradient == nullptr || blocks == 1) return st;
-  constexpr uint32_t most = static_cast<uint32_t>(most_blocks(1024)) * 16;
-  for (uint32_t first = 0; first < a.columns; first += most)
-    oxh::launch(rms_norm_weight_kernel, dim3((std::min(a.columns - first, most) + 15) / 16),
-                dim3(1024), 0, stream, static_cast<const float *>(a.partial), weight_gradient,
-                static_cast<uint32_t>(blocks), a.columns, first);
+  launch_column_sums(stream, a.partial, weight_gradient, nullptr, a.columns,
+                     static_cast<uint32_t>(blocks), a.columns);
   return oxh::launched("rms_norm_weight_gradient");
 }
 

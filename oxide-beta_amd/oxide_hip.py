@@ -72,6 +72,11 @@ class MuonTensor(ctypes.Structure):
                 ("columns", _u64)]
 
 
+class DeltaShape(ctypes.Structure):
+    _fields_ = [(f, _u64) for f in ("batch", "time", "key_heads", "heads", "key_dim",
+                                    "value_dim")]
+
+
 class Conv2dShape(ctypes.Structure):
     _fields_ = [(f, ctypes.c_uint64) for f in (
         "batch", "in_channels", "height", "width", "out_channels", "kernel_h", "kernel_w",
@@ -90,6 +95,7 @@ class CheckpointTensor(ctypes.Structure):
 
 _CS = ctypes.POINTER(Conv2dShape)
 _PS = ctypes.POINTER(Pool2dShape)
+_DS = ctypes.POINTER(DeltaShape)
 
 _SIGNATURES = {
     "oxh_last_error": (ctypes.c_char_p, []),
@@ -172,6 +178,17 @@ _SIGNATURES = {
     "oxh_gated_recurrence_workspace_size": (_st, [_u64, _u64, _u64, ctypes.POINTER(_u64)]),
     "oxh_gated_recurrence_forward": (_st, [_vp, _int, _u64, _u64, _u64] + [_vp] * 7 + [_u64]),
     "oxh_gated_recurrence_backward": (_st, [_vp, _int, _u64, _u64, _u64] + [_vp] * 11 + [_u64]),
+    "oxh_layer_norm_forward": (_st, [_vp, _int, _u64, _u64, _f32] + [_vp] * 8),
+    "oxh_layer_norm_backward_workspace_size": (_st, [_u64, _u64, ctypes.POINTER(_u64)]),
+    "oxh_layer_norm_backward": (_st, [_vp, _int, _u64, _u64] + [_vp] * 10 + [_u64]),
+    "oxh_gated_delta_rule_saved_size": (_st, [_int, _DS, ctypes.POINTER(_u64)]),
+    "oxh_gated_delta_rule_workspace_size": (_st, [_int, _DS, _int, ctypes.POINTER(_u64)]),
+    "oxh_gated_delta_rule_backward_workspace_size": (_st, [_int, _DS, ctypes.POINTER(_u64)]),
+    "oxh_gated_delta_rule_backward": (_st, [_vp, _int, _DS, _f32] + [_vp] * 7 + [_u64] +
+                                      [_vp] * 9 + [_u64]),
+    "oxh_gated_delta_rule_forward": (_st, [_vp, _int, _DS, _f32] + [_vp] * 10 + [_u64, _vp, _u64]),
+    "oxh_policy_loss_workspace_size": (_st, [_u64, _u64, ctypes.POINTER(_u64)]),
+    "oxh_policy_loss": (_st, [_vp, _int, _u64, _u64, _f32, _f32, _f32] + [_vp] * 12 + [_u64]),
     "oxh_orthogonalize_workspace_size": (_st, [_u64, _u64, _u64, ctypes.POINTER(_u64)]),
     "oxh_orthogonalize": (_st, [_vp, _u64, _u64, _u64, _u32, _f32, _vp, _vp, _vp, _u64]),
     "oxh_muon_workspace_size": (_st, [ctypes.POINTER(MuonTensor), _u32, ctypes.POINTER(_u64)]),
@@ -514,6 +531,53 @@ def gated_recurrence_workspace_size(batch: int, time: int, channels: int) -> int
     out = _u64()
     check(lib().oxh_gated_recurrence_workspace_size(batch, time, channels, ctypes.byref(out)))
     return out.value
+
+
+@functools.lru_cache(maxsize=4096)
+def layer_norm_backward_workspace_size(rows: int, columns: int) -> int:
+    out = _u64()
+    check(lib().oxh_layer_norm_backward_workspace_size(rows, columns, ctypes.byref(out)))
+    return out.value
+
+
+@functools.lru_cache(maxsize=4096)
+def policy_loss_workspace_size(rows: int, classes: int) -> int:
+    out = _u64()
+    check(lib().oxh_policy_loss_workspace_size(rows, classes, ctypes.byref(out)))
+    return out.value
+
+
+@functools.lru_cache(maxsize=4096)
+def _delta_plan(code: int, *dims) -> tuple:
+    """A gated delta rule's shape for the C ABI (a reference to it) and bytes: its workspace
+    without and with what the backward reads, that, and the backward's workspace."""
+    shape, sizes = DeltaShape(*dims), []
+    for name, *saves in (("workspace", 0), ("workspace", 1), ("saved",), ("backward_workspace",)):
+        out = _u64()
+        check(getattr(lib(), f"oxh_gated_delta_rule_{name}_size")(code, ctypes.byref(shape), *saves,
+                                                                  ctypes.byref(out)))
+        sizes.append(out.value)
+    return ctypes.byref(shape), *sizes
+
+
+def _delta_dims(query, key, value) -> tuple:
+    if query.dim() != 4 or value.dim() != 4 or query.shape != key.shape \
+            or query.shape[:2] != value.shape[:2]:
+        raise OxideError(INVALID_SHAPE,
+                         "gated_delta_rule expects query and key [batch, time, key_heads, key_dim]"
+                         " and value [batch, time, heads, value_dim]")
+    batch, time, key_heads, keys = key.shape
+    return batch, time, key_heads, value.shape[2], keys, value.shape[3]
+
+
+def _saved_bytes(t, nbytes: int) -> tuple:
+    if t is None:
+        return None, 0
+    if not t.is_cuda or not t.is_contiguous() or t.element_size() != 1 or t.numel() < nbytes:
+        raise OxideError(INVALID_SHAPE,
+                         f"saved must be a device tensor of {nbytes} bytes "
+                         "(gated_delta_rule_saved)")
+    return t.data_ptr(), t.numel()
 
 
 @functools.lru_cache(maxsize=4096)
@@ -899,6 +963,34 @@ class LoadedModule:
                                                        _ptr(outer_gradient), _ptr(loss),
                                                        _ptr(grad), _ptr(error_flag), ws, wsb))
 
+    def policy_loss(self, logits, actions, old_log_probs, advantages, loss=None, gradient=None,
+                    outer_gradient=None, log_probs=None, reference_log_probs=None, weights=None,
+                    clip=(0.2, 0.2), kl=0.0, error_flag=None, stream=None):
+        """The clipped policy loss of ``logits`` [rows, classes] (float32 or bfloat16): ``loss``
+        [1] = sum of weight * (-min(r A, clip(r) A) + kl (exp(d) - d - 1)) with l = log
+        softmax(logits)[action], r = exp(l - old), d = reference - l; ``weights`` None: 1 / rows.
+        ``actions`` are class indexes in float32, as cross entropy's targets; ``log_probs`` [rows]
+        receives l, ``gradient`` the logits' gradient times ``outer_gradient`` [1]."""
+        shape = logits.shape
+        if len(shape) != 2:
+            raise OxideError(INVALID_SHAPE, "policy_loss expects [rows, classes] logits")
+        code, logits_at, gradient_at = _activations((logits, gradient), shape, "policy_loss")
+        rows, classes = shape
+        row = (rows,)
+        stream = _stream(stream)
+        scratch = self._sequence_ws
+        with scratch.lock:
+            ws, wsb = scratch.ptr_bytes(
+                0 if loss is None else policy_loss_workspace_size(rows, classes), stream)
+            check(lib().oxh_policy_loss(
+                stream, code, rows, classes, *clip, kl, logits_at,
+                _shaped(actions, row, "actions"), _shaped(old_log_probs, row, "old_log_probs"),
+                _shaped(advantages, row, "advantages"),
+                _shaped(reference_log_probs, row, "reference_log_probs"),
+                _shaped(weights, row, "weights"), _shaped(outer_gradient, (1,), "outer_gradient"),
+                _shaped(loss, (1,), "loss"), _shaped(log_probs, row, "log_probs"), gradient_at,
+                _ptr(error_flag), ws, wsb))
+
     # -- AdamW (kernel_module.rs:1094-1127)
     def adamw(self, learning_rate, weight_decay, beta1, beta2, first_correction,
               second_correction, epsilon, parameter, gradient, first_moment, second_moment,
@@ -1030,6 +1122,117 @@ class LoadedModule:
                 _shaped(initial_state, states, "initial_state"),
                 _shaped(final_state_gradient, states, "final_state_gradient"),
                 _lengths(lengths, batch), at[4], at[5],
+                _shaped(initial_state_gradient, states, "initial_state_gradient"), ws, wsb))
+
+    def layer_norm_forward(self, x, weight, bias, out, mean=None, inverse_deviation=None,
+                           residual=None, sum=None, epsilon=1e-5, stream=None):  # noqa: A002
+        """``out`` = (s - mean(s)) / deviation(s) * weight + bias over the last dimension, s = x +
+        residual (``bias`` None: 0); ``sum`` receives s (it may be ``x`` or ``residual``),
+        ``mean`` and ``inverse_deviation`` [rows] what the backward needs."""
+        shape = x.shape
+        code, x_at, out_at, residual_at, sum_at = _activations((x, out, residual, sum), shape,
+                                                               "layer_norm")
+        columns = shape[-1] if shape else 0
+        rows = x.numel() // max(columns, 1)
+        check(lib().oxh_layer_norm_forward(
+            _stream(stream), code, rows, columns, epsilon, x_at, residual_at,
+            _shaped(weight, (columns,), "weight"), _shaped(bias, (columns,), "bias"), sum_at,
+            out_at, _shaped(mean, (rows,), "mean"),
+            _shaped(inverse_deviation, (rows,), "inverse_deviation")))
+
+    def layer_norm_backward(self, gradient, sum, weight, mean, inverse_deviation,  # noqa: A002
+                            input_gradient, weight_gradient=None, bias_gradient=None,
+                            sum_gradient=None, stream=None):
+        """Gradients from the output's and, where the sum has other uses, ``sum_gradient``
+        (``input_gradient`` may be that tensor)."""
+        shape = gradient.shape
+        code, gradient_at, sum_at, input_at, stream_at = _activations(
+            (gradient, sum, input_gradient, sum_gradient), shape, "layer_norm_backward")
+        columns = shape[-1] if shape else 0
+        rows = gradient.numel() // max(columns, 1)
+        stream = _stream(stream)
+        scratch = self._sequence_ws
+        with scratch.lock:
+            ws, wsb = scratch.ptr_bytes(
+                0 if weight_gradient is None and bias_gradient is None
+                else layer_norm_backward_workspace_size(rows, columns), stream)
+            check(lib().oxh_layer_norm_backward(
+                stream, code, rows, columns, gradient_at, stream_at, sum_at,
+                _shaped(weight, (columns,), "weight"), _shaped(mean, (rows,), "mean"),
+                _shaped(inverse_deviation, (rows,), "inverse_deviation"), input_at,
+                _shaped(weight_gradient, (columns,), "weight_gradient"),
+                _shaped(bias_gradient, (columns,), "bias_gradient"), ws, wsb))
+
+    def gated_delta_rule_saved(self, key, value):
+        """A buffer for what ``gated_delta_rule_forward`` leaves for the backward of such keys and
+        values."""
+        import torch
+
+        if _float32 is None:
+            _know_types()
+        code = _codes.get(key.dtype)
+        if code is None:
+            raise OxideError(INVALID_SHAPE, "gated_delta_rule takes float32 or bfloat16 tensors")
+        size = _delta_plan(code, *_delta_dims(key, key, value))[3]
+        return torch.empty(size, dtype=torch.uint8, device=key.device)
+
+    def gated_delta_rule_forward(self, query, key, value, gate, write, out, initial_state=None,
+                                 final_state=None, saved=None, lengths=None, scale=None,
+                                 stream=None):
+        """``out`` [batch, time, heads, value_dim] of o_t = scale S_t' q_t with S_t = P + b_t k_t
+        (v_t - P' k_t)', P = a_t S_{t-1}, a_t = sigmoid(gate_t), b_t = sigmoid(write_t).
+        ``query`` and ``key`` [batch, time, key_heads, key_dim], ``gate`` and ``write`` [batch,
+        time, heads]; states [batch, heads, key_dim, value_dim] float32 (the final one may be
+        written over the initial one), ``lengths`` [batch] int32, ``scale`` key_dim ** -0.5 unless
+        given; ``saved`` (``gated_delta_rule_saved``) receives what the backward reads."""
+        dims = _delta_dims(query, key, value)
+        batch, time, _, heads, keys, values = dims
+        code, query_at, key_at = _activations((query, key), query.shape, "gated_delta_rule")
+        codes, *at = _activations((value, out), value.shape, "gated_delta_rule")
+        codeg, *gates = _activations((gate, write), (batch, time, heads), "gated_delta_rule")
+        if not code == codes == codeg:
+            raise OxideError(INVALID_SHAPE, "gated_delta_rule takes tensors of one type")
+        shape, alone, size, kept, _ = _delta_plan(code, *dims)
+        if saved is None:
+            size = alone
+        states = (batch, heads, keys, values)
+        stream = _stream(stream)
+        scratch = self._sequence_ws
+        with scratch.lock:
+            ws, wsb = scratch.ptr_bytes(size, stream) if size else (None, 0)
+            check(lib().oxh_gated_delta_rule_forward(
+                stream, code, shape, keys ** -0.5 if scale is None else scale, query_at, key_at,
+                at[0], *gates, _shaped(initial_state, states, "initial_state"),
+                _lengths(lengths, batch), at[1], _shaped(final_state, states, "final_state"),
+                *_saved_bytes(saved, kept), ws, wsb))
+
+    def gated_delta_rule_backward(self, gradient, query, key, value, gate, write, saved,
+                                  query_gradient, key_gradient, value_gradient, gate_gradient,
+                                  write_gradient, final_state_gradient=None,
+                                  initial_state_gradient=None, lengths=None, scale=None,
+                                  stream=None):
+        """Gradients of ``gated_delta_rule_forward``'s operands from its output's and its final
+        state's, with the ``lengths`` and ``scale`` of that call."""
+        dims = _delta_dims(query, key, value)
+        batch, time, _, heads, keys, values = dims
+        what = "gated_delta_rule_backward"
+        code, *of_keys = _activations((query, key, query_gradient, key_gradient), query.shape, what)
+        codev, *of_values = _activations((gradient, value, value_gradient), value.shape, what)
+        codeg, *of_gates = _activations((gate, write, gate_gradient, write_gradient),
+                                        (batch, time, heads), what)
+        if not code == codev == codeg:
+            raise OxideError(INVALID_SHAPE, f"{what} takes tensors of one type")
+        shape, _, _, kept, size = _delta_plan(code, *dims)
+        states = (batch, heads, keys, values)
+        stream = _stream(stream)
+        scratch = self._sequence_ws
+        with scratch.lock:
+            ws, wsb = scratch.ptr_bytes(size, stream) if size else (None, 0)
+            check(lib().oxh_gated_delta_rule_backward(
+                stream, code, shape, keys ** -0.5 if scale is None else scale, of_values[0],
+                *of_keys[:2], of_values[1], *of_gates[:2], *_saved_bytes(saved, kept),
+                _shaped(final_state_gradient, states, "final_state_gradient"),
+                _lengths(lengths, batch), *of_keys[2:], of_values[2], *of_gates[2:],
                 _shaped(initial_state_gradient, states, "initial_state_gradient"), ws, wsb))
 
     def orthogonalize(self, x, out, rounds=5, epsilon=1e-7, stream=None):
