@@ -85,6 +85,7 @@ __device__ __forceinline__ f32x8 widened(f32x8 v) { return v; }
 template <typename T, int Parts>
 struct Split {
   operand<T> part[Parts];
+  Split() = default;
   __device__ __forceinline__ explicit Split(f32x8 v) {
 #pragma unroll
     for (int p = 0; p < Parts; ++p) {
@@ -102,6 +103,15 @@ __device__ __forceinline__ f32x4 product(operand<T> a, const Split<T, Parts> &b,
 
 __device__ __forceinline__ f32x8 join(f32x4 low, f32x4 high) {
   return __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// A lane's load from `at` bytes behind an address that is the same for the wave (of memory, said so:
+// a load that might be of shared memory would have to wait for all others).
+template <typename V, int Align = alignof(V)>
+__device__ __forceinline__ V load_at(const void *base, uint32_t at) {
+  typedef V __attribute__((aligned(Align))) type;
+  typedef __attribute__((address_space(1))) const type *pointer;
+  return *(pointer)(reinterpret_cast<const char *>(base) + at);
 }
 
 // 8 consecutive values of a row of `count`, from place `at` on; those past its end are 0.
@@ -124,6 +134,24 @@ __device__ __forceinline__ operand<T> load_row(const T *row, uint32_t at, uint32
   return v;
 }
 
+// A lane's column of a state as the matrix cores' results, from `at` on (null: 0).
+template <int KT, bool Whole>
+__device__ __forceinline__ void load_state(f32x4 (&state)[2 * KT], const float *at, const Dims &d,
+                                           uint32_t g) {
+#pragma unroll
+  for (int i = 0; i < 2 * KT; ++i) state[i] = f32x4{};
+  if (at == nullptr) return;
+#pragma unroll
+  for (int i = 0; i < 2 * KT; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      // past the keys' end the last one again, and 0 in its place
+      const uint32_t k = index_of(i, 4 * g + r);
+      const float v = at[static_cast<uint64_t>(Whole ? k : min(k, d.keys - 1)) * d.values];
+      state[i][r] = Whole || k < d.keys ? v : 0.0f;
+    }
+}
+
 // Where the operands of a chunk lie, in units of a wave's operand (64 lanes, each its 8 values in
 // one piece).  Triangles of 64 x 64 are six operands: (tile, step) = (0,0) (1,0) (2,0) (2,1) (3,0)
 // (3,1) for the lower one, (0,0) (0,1) (1,0) (1,1) (2,1) (3,1) for its transpose.
@@ -135,18 +163,52 @@ __device__ __forceinline__ int upper_place(int tile, int step) {
   return tile < 2 ? 2 * tile + step : tile + 2;
 }
 
+// Where the block's waves see each other's shared memory; loads from memory stay on their way.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// Stores to places of a buffer that begins anywhere (the same for the wave); those past its bytes,
+// kNowhere among them, do not happen.
+constexpr uint32_t kNowhere = 0xFFFFFFF0u;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(void *p, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(p, 0, static_cast<int>(bytes), 0x00020000);
+}
+template <typename V>
+__device__ __forceinline__ void store_to(__amdgpu_buffer_rsrc_t to, uint32_t at, V v) {
+  typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  if constexpr (sizeof(V) == 2) {
+    __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, v), to, at, 0, 0);
+  } else if constexpr (sizeof(V) == 4) {
+    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), to, at, 0, 0);
+  } else if constexpr (sizeof(V) == 8) {
+    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, v), to, at, 0, 0);
+  } else if constexpr (sizeof(V) == 16) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), to, at, 0, 0);
+  } else {
+    struct Halves {
+      u32x4 low, high;
+    };
+    const Halves x = __builtin_bit_cast(Halves, v);
+    __builtin_amdgcn_raw_buffer_store_b128(x.low, to, at, 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b128(x.high, to, at == kNowhere ? at : at + 16, 0, 0);
+  }
+}
+
 // exp of the decay's sums of a chunk: from its start (`since`), to its end (`until`), and b.
 struct Gates {
   float since[kChunk], until[kChunk], write[kChunk];
 };
 
 template <typename T>
+constexpr uint64_t kOperandBytes = 64 * 8 * sizeof(T);
+
+template <typename T, int P>
 struct Chunk {  // per value head
-  static constexpr int kParts = sizeof(T) == 2 ? 2 : 1;
-  static constexpr uint64_t operand_bytes = 64 * 8 * sizeof(T);
   static constexpr uint64_t gates = 0, system = sizeof(Gates),
-                            within = system + kTriangle * kParts * operand_bytes,
-                            bytes = within + kTriangle * operand_bytes;
+                            within = system + kTriangle * P * kOperandBytes<T>,
+                            bytes = within + kTriangle * kOperandBytes<T>;
 };
 
 __device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
@@ -323,7 +385,7 @@ __device__ __forceinline__ void solve(System<T, KT> &m, const Dims &d, const Pla
 constexpr uint64_t kMostKeys = 128;
 // Bytes of operands that a call prepares before it scans their chunks: what the last-level cache
 // holds beside the tensors.
-constexpr uint64_t kPrepared = 128ull << 20;
+constexpr uint64_t kPrepared = 192ull << 20;
 
 inline uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
 
@@ -337,16 +399,22 @@ struct Plan {
           static_cast<uint32_t>(s.heads / s.key_heads),
           static_cast<uint32_t>((s.value_dim + 15) / 16), 0, 0, lengths, scale},
         all((s.time + kChunk - 1) / kChunk), segment(0), steps(round_up(s.key_dim, 32) / 32) {}
+  // Takes as many chunks at a time as `bytes` each allow, in equal parts.
+  void divide(uint64_t bytes) {
+    const uint64_t most = std::max<uint64_t>(1, kPrepared / std::max<uint64_t>(1, bytes));
+    const uint64_t parts = (all + most - 1) / most;
+    segment = parts == 0 ? 0 : (all + parts - 1) / parts;
+  }
   uint64_t state_elements(const oxh_delta_shape &s) const {
     return s.batch * s.heads * s.key_dim * s.value_dim;
   }
 };
 
-// Calls run(32 keys each, whether they are whole).
+// Calls run(32 keys each, whether rows are loaded without a look at their end).
 template <typename Run>
-void with_keys(uint64_t keys, Run run) {
+void with_keys(uint64_t keys, bool packed, Run run) {
   auto whole = [&](auto steps) {
-    if (keys % 32 == 0) run(steps, std::true_type());
+    if (packed) run(steps, std::true_type());
     else run(steps, std::false_type());
   };
   if (keys <= 32) whole(std::integral_constant<int, 1>());
@@ -370,6 +438,9 @@ inline oxh_status check_shape(int dtype, const oxh_delta_shape *s) {
   OXH_REQUIRE(s->batch <= 65535, OXH_INVALID_SHAPE, "gated delta rule: batch above 65535");
   OXH_REQUIRE(s->time < (1ull << 31) - kChunk, OXH_INVALID_SHAPE,
               "gated delta rule: too many steps");
+  // a chunk's rows lie within 32 bits of each other
+  OXH_REQUIRE(s->heads * s->value_dim < (1ull << 24), OXH_INVALID_SHAPE,
+              "gated delta rule: heads * value_dim must be below 2^24");
   // one launch numbers its threads with 32 bits
   const uint64_t heads = s->batch * s->heads;
   OXH_REQUIRE(heads * std::max<uint64_t>((s->time + kChunk - 1) / kChunk, 1) <= (1ull << 23) &&

@@ -20,6 +20,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstddef>
 #include <string>
 #include <vector>
 
@@ -38,11 +39,11 @@ struct PrepareArgs {
   Dims d;
   const T *query, *key, *gate, *write;
   char *heads;  // Chunk<T> of (batch, head, chunk)
-  char *keys;   // transposed keys of (batch, key head, chunk)
+  char *keys;   // operands of keys, queries and transposed keys of (batch, key head, chunk)
 };
 
 // A block per chunk and value head.
-template <typename T, int KT, bool Whole>
+template <typename T, int P, int KT, bool Whole>
 __global__ __launch_bounds__(256) void delta_prepare_kernel(PrepareArgs<T> a) {
   using Op = operand<T>;
   __shared__ System<T, KT> m;
@@ -53,9 +54,12 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(PrepareArgs<T> a) {
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const T *query = a.query + at.key_row * d.keys;
   const uint64_t stride = static_cast<uint64_t>(d.key_heads) * d.keys;
-  char *out = a.heads + at.head_chunk(d) * Chunk<T>::bytes;
+  char *out = a.heads + at.head_chunk(d) * Chunk<T, P>::bytes;
+  const bool first_head = at.head % d.group == 0;  // brings what its key head's others share
+  Op *keys = reinterpret_cast<Op *>(a.keys) + at.key_chunk(d) * (12 * KT * 64) + lane;
+  Op *queries = keys + 4 * KT * 64, *across = queries + 4 * KT * 64;
   solve<T, KT, Whole>(
-      m, d, at, a.key, a.gate, a.write, reinterpret_cast<Gates *>(out + Chunk<T>::gates), [&] {
+      m, d, at, a.key, a.gate, a.write, reinterpret_cast<Gates *>(out + Chunk<T, P>::gates), [&] {
         // G o q k', as the operand of a product from the left: a lane its step t, keys' steps i
         const uint32_t first = wave == 1 ? 0 : wave, last = wave == 1 ? 1 : wave;
         for (uint32_t ti = first; ti <= last; ++ti) {
@@ -64,6 +68,9 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(PrepareArgs<T> a) {
 #pragma unroll
           for (int s = 0; s < KT; ++s)
             q[s] = load_row<T, Whole>(query + min(t, at.rows - 1) * stride, 32 * s + 8 * g, d.keys);
+          if (first_head)
+#pragma unroll
+            for (int s = 0; s < KT; ++s) queries[(ti * KT + s) * 64] = q[s];
           for (int step = 0; step <= static_cast<int>(ti >> 1); ++step) {
             f32x4 half[2];
 #pragma unroll
@@ -78,7 +85,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(PrepareArgs<T> a) {
                 half[e][r] = i <= t ? acc[r] * m.between(t, i) * d.scale : 0.0f;
               }
             }
-            Op *to = reinterpret_cast<Op *>(out + Chunk<T>::within);
+            Op *to = reinterpret_cast<Op *>(out + Chunk<T, P>::within);
             to[lower_place(ti, step) * 64 + lane] = rounded<T>(join(half[0], half[1]));
           }
         }
@@ -89,20 +96,23 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(PrepareArgs<T> a) {
     f32x8 v;
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = row[i];
-    const Split<T, Chunk<T>::kParts> parts(v);
-    Op *to = reinterpret_cast<Op *>(out + Chunk<T>::system);
+    const Split<T, P> parts(v);
+    Op *to = reinterpret_cast<Op *>(out + Chunk<T, P>::system);
 #pragma unroll
-    for (int q = 0; q < Chunk<T>::kParts; ++q)
-      to[(p * Chunk<T>::kParts + q) * 64 + lane] = parts.part[q];
+    for (int q = 0; q < P; ++q)
+      to[(p * P + q) * 64 + lane] = parts.part[q];
   }
-  if (at.head % d.group == 0)
-    store_transposed<T, KT>(m.tile, reinterpret_cast<Op *>(a.keys) + at.key_chunk(d) * (4 * KT * 64));
+  if (!first_head) return;
+#pragma unroll
+  for (int s = 0; s < KT; ++s)
+    keys[(wave * KT + s) * 64] = m.key_row(index_of(wave, n), s, g);
+  store_transposed<T, KT>(m.tile, across - lane);
 }
 
 template <typename T>
 struct ScanArgs {
   Dims d;
-  const T *query, *key, *value;
+  const T *value;
   const char *heads, *keys;
   const float *from;  // states before the first chunk, null: 0
   float *to;          // and after the last, may be null
@@ -111,167 +121,304 @@ struct ScanArgs {
   uint32_t all;       // chunks of the whole sequence
 };
 
-// A wave per 16 columns of a head's values.
-template <typename T, int KT, bool Whole>
+// What the block's waves hand each other, as operands: the state, b y, b e and exp(g_64 - g) b e.
+template <typename T, int P, int KT, int C>
+struct Exchange {
+  operand<T> state[KT][C][P][64], weighted[2][C][P][64], wrote[2][C][P][64], left[2][C][P][64];
+};
+
+// A block of four waves per C slabs of 16 columns of a head's values.  A wave takes 16 of a chunk's
+// steps and 32 of the keys: whatever stands on the left of a product (keys, queries, the chunk's
+// matrices) is one wave's alone and goes from memory to its registers, a chunk ahead, as soon as the
+// present chunk's is used; what stands on the right goes through shared memory, three times a
+// chunk.
+template <typename T, int P, int KT, int C>
 __global__ __launch_bounds__(256) void delta_scan_kernel(ScanArgs<T> a) {
   using Op = operand<T>;
-  constexpr int P = Chunk<T>::kParts;
+  using Kept = Chunk<T, P>;
+  __shared__ Exchange<T, P, KT, C> m;
   const Dims &d = a.d;
   const uint32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-  const uint32_t slab = blockIdx.x * (blockDim.x >> 6) +
-                        __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (slab >= d.slabs) return;
-  const uint32_t h = blockIdx.y, b = blockIdx.z, kh = h / d.group;
-  const uint32_t column = 16 * slab + n;
-  const bool in = column < d.values;
-  const uint32_t col = in ? column : d.values - 1;
-  const uint32_t length = length_of(d, b);
+  const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = w & 1;
+  const int pair = w >> 1;  // of tiles of 16 steps: an operand of 32
+  // blocks of a head share what they read: on one XCD
+  const oxh::BlockTile block = oxh::xcd_block();
+  const uint32_t h = block.y, b = block.z, kh = h / d.group;
+  const uint32_t length = length_of(d, b), start = d.first * kChunk;
+  const uint32_t live =
+      length <= start ? 0 : min((length - start + kChunk - 1) / kChunk, d.chunks);
   const uint64_t head = static_cast<uint64_t>(b) * d.heads + h;
-  const uint64_t stride = static_cast<uint64_t>(d.key_heads) * d.keys;
   const uint64_t value_stride = static_cast<uint64_t>(d.heads) * d.values;
-
-  f32x4 state[2 * KT];
-  const uint64_t state_at = head * d.keys * d.values + col;
+  const uint64_t row0 = static_cast<uint64_t>(b) * d.time + start;
+  const T *values = a.value + row0 * value_stride + static_cast<uint64_t>(h) * d.values;
+  T *outs = a.out + row0 * value_stride + static_cast<uint64_t>(h) * d.values;
+  const char *chunks = a.heads + head * d.chunks * Kept::bytes;
+  constexpr uint32_t kOperand = 64 * sizeof(Op), kKeys = 4 * KT * kOperand;
+  const char *keys =
+      a.keys + (static_cast<uint64_t>(b) * d.key_heads + kh) * d.chunks * (3 * kKeys);
+  uint32_t cols[C];  // this lane's; those past the last are the last again, and not stored
+  bool in[C], own[C];
 #pragma unroll
-  for (int i = 0; i < 2 * KT; ++i) {
+  for (int c = 0; c < C; ++c) {
+    const uint32_t slab = block.x * C + c, column = 16 * slab + n;
+    own[c] = slab < d.slabs;
+    in[c] = column < d.values;
+    cols[c] = in[c] ? column : d.values - 1;
+  }
+  auto rows_of = [&](uint32_t chunk) -> uint32_t {
+    return min(length - start - chunk * kChunk, static_cast<uint32_t>(kChunk));
+  };
+  const bool holds = w < KT;  // keys 32 w on
+  const uint64_t state_at = head * d.keys * d.values;
+  auto key_at = [&](int tile, int r) { return 32 * w + index_of(tile, 4 * g + r); };
+  f32x4 state[2][C];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      state[i][c] = f32x4{};
+      if (a.from == nullptr || !holds) continue;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t k = key_at(i, r), there = min(k, d.keys - 1);
+        const float v = a.from[state_at + static_cast<uint64_t>(there) * d.values + cols[c]];
+        state[i][c][r] = k < d.keys ? v : 0.0f;
+      }
+    }
+
+  // The left operands of a chunk's four products and its values, each loaded where the chunk before
+  // has used its own (not before: their registers are the same).  No load or store of the loop is behind a branch, so that each use waits for
+  // its own loads alone: the last chunk loads itself again, and stores that are not to be go past
+  // their buffer's end.
+  Op key[KT], query[KT], solve[2][P], scores[2], back[2][2];
+  T value[C][4];
+  f32x4 since, until, write;
+  float whole = 0.0f;
+  const uint32_t value_bytes = static_cast<uint32_t>(value_stride * sizeof(T));
+  const uint32_t lane_at = lane * sizeof(Op);
+  auto load_keys = [&](uint32_t chunk) {
+    const char *from = keys + (chunk * uint64_t{3 * kKeys} + w * (KT * kOperand));
+#pragma unroll
+    for (int s = 0; s < KT; ++s) key[s] = load_at<Op>(from + s * kOperand, lane_at);
+#pragma unroll
+    for (int s = 0; s < KT; ++s) query[s] = load_at<Op>(from + kKeys + s * kOperand, lane_at);
+  };
+  auto load_values = [&](uint32_t chunk) {
+    const uint32_t last = rows_of(chunk) - 1;
+    const char *from = reinterpret_cast<const char *>(values + chunk * kChunk * value_stride);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const uint32_t k = index_of(i, 4 * g + r);
-      state[i][r] = a.from != nullptr && (Whole || k < d.keys)
-                        ? a.from[state_at + static_cast<uint64_t>(k) * d.values]
-                        : 0.0f;
-    }
-  }
-
-  for (uint32_t chunk = 0; chunk < d.chunks; ++chunk) {
-    const uint32_t begin = (d.first + chunk) * kChunk;
-    const uint64_t row0 = static_cast<uint64_t>(b) * d.time + begin;
-    T *out = a.out + row0 * value_stride + static_cast<uint64_t>(h) * d.values + col;
-    const uint32_t held = min(d.time - begin, static_cast<uint32_t>(kChunk));
-    if (begin >= length) {
-      if (in)
-        for (uint32_t t = g; t < held; t += 4) out[t * value_stride] = static_cast<T>(0.0f);
-      continue;
-    }
-    const uint32_t rows = min(length - begin, static_cast<uint32_t>(kChunk));
-    const T *key = a.key + row0 * stride + static_cast<uint64_t>(kh) * d.keys;
-    const T *query = a.query + row0 * stride + static_cast<uint64_t>(kh) * d.keys;
-    const T *value = a.value + row0 * value_stride + static_cast<uint64_t>(h) * d.values + col;
-    const char *operands = a.heads + (head * d.chunks + chunk) * Chunk<T>::bytes;
-    const Gates *gates = reinterpret_cast<const Gates *>(operands + Chunk<T>::gates);
-    const Op *system = reinterpret_cast<const Op *>(operands + Chunk<T>::system) + lane;
-    const Op *within = reinterpret_cast<const Op *>(operands + Chunk<T>::within) + lane;
-    const Op *keys = reinterpret_cast<const Op *>(a.keys) + lane +
-                     ((static_cast<uint64_t>(b) * d.key_heads + kh) * d.chunks + chunk) *
-                         (4 * KT * 64);
-    auto vec = [&](const float *v, int tile) {
-      return *reinterpret_cast<const f32x4 *>(v + 32 * (tile >> 1) + 8 * g + 4 * (tile & 1));
-    };
-
-    f32x4 y[4], q[4];
-    Op state_high[KT];
-    {
-      // the state as an operand, and its products with keys and queries
-      f32x4 held_by[4] = {};
+      const uint32_t row = min(index_of(w, 4 * g + r), last) * value_bytes;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) q[i] = f32x4{};
+      for (int c = 0; c < C; ++c)
+        value[c][r] = load_at<T>(from, row + cols[c] * static_cast<uint32_t>(sizeof(T)));
+    }
+  };
+  auto operands_of = [&](uint32_t chunk, uint64_t part) {
+    return chunks + (chunk * Kept::bytes + part);
+  };
+  auto load_system = [&](uint32_t chunk) {
+    const char *from = operands_of(chunk, Kept::system);
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+        solve[s][p] =
+            load_at<Op>(from + (lower_place(w, min(s, pair)) * P + p) * kOperand, lane_at);
+  };
+  auto load_rest = [&](uint32_t chunk) {
+    whole = load_at<float>(operands_of(chunk, Kept::gates) + offsetof(Gates, since),
+                           (kChunk - 1) * 4);
+    const char *from = operands_of(chunk, Kept::within);
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      scores[s] = load_at<Op>(from + lower_place(w, min(s, pair)) * kOperand, lane_at);
+    const char *k = keys + (chunk * uint64_t{3 * kKeys} + 2 * kKeys + 4 * min(w, KT - 1u) * kOperand);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        back[i][s] = load_at<Op>(k + (2 * i + s) * kOperand, lane_at);
+  };
+  auto load_gates = [&](uint32_t chunk) {
+    const char *gates = operands_of(chunk, Kept::gates);
+    const uint32_t at = index_of(w, 4 * g) * 4;
+    since = load_at<f32x4>(gates + offsetof(Gates, since), at);
+    until = load_at<f32x4>(gates + offsetof(Gates, until), at);
+    write = load_at<f32x4>(gates + offsetof(Gates, write), at);
+  };
+  typedef T quarter __attribute__((ext_vector_type(4)));
+  // a wave's half of an operand that two waves form, and the state's, which is its own
+  auto hand = [&](Op(&to)[P][64], f32x4 v) {
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const quarter q = __builtin_convertvector(v, quarter);
+      reinterpret_cast<quarter *>(&to[p][lane])[half] = q;
+      if (p + 1 < P) v -= __builtin_convertvector(q, f32x4);
+    }
+  };
+  // what the backward reads of a chunk: its slabs' states and errors
+  const uint32_t kept = d.slabs * (KT + 2) * kOperand;
+  auto saved_of = [&](uint32_t chunk) {
+    return buffer_of(a.saved + ((head * a.all + d.first + chunk) * kept), a.saved == nullptr ? 0 : kept);
+  };
+  auto saved_at = [&](int c, int place) {
+    return own[c] ? ((block.x * C + c) * (KT + 2) + place) * kOperand + lane_at : kNowhere;
+  };
+  auto hand_state = [&](uint32_t chunk) {
+    if (KT < 4 && !holds) return;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const Split<T, P> st(join(state[0][c], state[1][c]));
+#pragma unroll
+      for (int p = 0; p < P; ++p) m.state[w][c][p][lane] = st.part[p];
+      store_to(saved_of(chunk), saved_at(c, w), st.part[0]);
+    }
+  };
+  // right operands of 64 steps, all of them on their way before the first is used
+  auto read_pairs = [&](Op(&to)[2][C][P], const Op(&from)[2][C][P][64]) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int p = 0; p < P; ++p) to[s][c][p] = from[s][c][p][lane];
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if (live != 0) {
+    load_keys(0);
+    load_values(0);
+    load_gates(0);
+    load_system(0);
+    load_rest(0);
+    hand_state(0);
+  }
+  for (uint32_t chunk = 0; chunk < live; ++chunk) {
+    const uint32_t next = min(chunk + 1, live - 1);
+    lds_barrier();
+    f32x4 y[C] = {}, o[C] = {};
+    {
+      Op right[KT][C][P];
+#pragma unroll
+      for (int s = 0; s < KT; ++s)
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int p = 0; p < P; ++p) right[s][c][p] = m.state[s][c][p][lane];
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int s = 0; s < KT; ++s) {
-        const Split<T, P> st(join(state[2 * s], state[2 * s + 1]));
-        state_high[s] = st.part[0];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint64_t row = min(index_of(i, n), rows - 1) * stride;
-          held_by[i] =
-              product<T, P>(load_row<T, Whole>(key + row, 32 * s + 8 * g, d.keys), st, held_by[i]);
-          q[i] = product(load_row<T, Whole>(query + row, 32 * s + 8 * g, d.keys), st.part[0], q[i]);
-        }
-      }
+        for (int p = P - 1; p >= 0; --p)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f32x4 since = vec(gates->since, i);
+          for (int c = 0; c < C; ++c) y[c] = product(key[s], right[s][c][p], y[c]);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const uint32_t t = min(index_of(i, 4 * g + r), rows - 1);
-          y[i][r] = widen(value[t * value_stride]) - since[r] * held_by[i][r];
-        }
-        q[i] *= since * d.scale;
+        for (int c = 0; c < C; ++c) o[c] = product(query[s], right[s][c][0], o[c]);
       }
     }
-    if (a.saved != nullptr) {
-      Op *to = reinterpret_cast<Op *>(a.saved) +
-               ((head * a.all + d.first + chunk) * d.slabs + slab) * ((KT + 2) * 64) + lane;
+    __builtin_amdgcn_sched_barrier(0);
+    load_keys(next);
 #pragma unroll
-      for (int s = 0; s < KT; ++s) to[s * 64] = state_high[s];
+    for (int c = 0; c < C; ++c) {
+      f32x4 v;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = widen(value[c][r]);
+      y[c] = v - since * y[c];
+      o[c] *= since * d.scale;
+      hand(m.weighted[pair][c], -write * y[c]);
     }
+    __builtin_amdgcn_sched_barrier(0);
+    load_values(next);
+    lds_barrier();
     // e = y - N (b y)
-    f32x4 e[4];
     {
-      f32x4 weighted[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        weighted[i] = -vec(gates->write, i) * y[i];
-        e[i] = y[i];
-      }
+      Op right[2][C][P];
+      read_pairs(right, m.weighted);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const Split<T, P> w(join(weighted[2 * s], weighted[2 * s + 1]));
+        if (s > pair) continue;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if ((i >> 1) < s) continue;
-          const Op *from = system + lower_place(i, s) * P * 64;
-          if constexpr (P == 2) e[i] = product(from[64], w.part[0], e[i]);
-          e[i] = product<T, P>(from[0], w, e[i]);
-        }
+        for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+          for (int q = P - 1 - p; q >= 0; --q)
+#pragma unroll
+            for (int c = 0; c < C; ++c) y[c] = product(solve[s][p], right[s][c][q], y[c]);
       }
     }
-    if (a.saved != nullptr) {
-      Op *to = reinterpret_cast<Op *>(a.saved) +
-               ((head * a.all + d.first + chunk) * d.slabs + slab) * ((KT + 2) * 64) + lane;
+    __builtin_amdgcn_sched_barrier(0);
+    load_system(next);
 #pragma unroll
-      for (int s = 0; s < 2; ++s) to[(KT + s) * 64] = rounded<T>(join(e[2 * s], e[2 * s + 1]));
+    for (int c = 0; c < C; ++c) {
+      const uint32_t at = saved_at(c, KT + pair);
+      store_to(saved_of(chunk), own[c] ? at + half * static_cast<uint32_t>(sizeof(quarter)) : at,
+               __builtin_convertvector(y[c], quarter));
+      y[c] *= write;
+      hand(m.wrote[pair][c], y[c]);
+      hand(m.left[pair][c], until * y[c]);
     }
+    __builtin_amdgcn_sched_barrier(0);
+    load_gates(next);
+    lds_barrier();
     // o = exp(g) q S0 + (G o q k') (b e);  S = exp(g_64) S0 + k' (exp(g_64 - g) b e)
-    const float whole = gates->since[kChunk - 1];
+    Op left[2][C][P], wrote[2][C][P];
+    read_pairs(left, m.left);
+    read_pairs(wrote, m.wrote);
+    if (KT == 4 || holds) {
 #pragma unroll
-    for (int i = 0; i < 2 * KT; ++i) state[i] *= whole;
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int c = 0; c < C; ++c) state[i][c] *= whole;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+          for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) state[i][c] = product(back[i][s], left[s][c][p], state[i][c]);
+    }
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      f32x4 u[2], left[2];
+      if (s > pair) continue;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        u[i] = vec(gates->write, 2 * s + i) * e[2 * s + i];
-        left[i] = vec(gates->until, 2 * s + i) * u[i];
-      }
-      const Split<T, P> wrote(join(u[0], u[1]));
+      for (int p = P - 1; p >= 0; --p)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if ((i >> 1) >= s) q[i] = product<T, P>(within[lower_place(i, s) * 64], wrote, q[i]);
-      const Split<T, P> l(join(left[0], left[1]));
-#pragma unroll
-      for (int i = 0; i < 2 * KT; ++i)
-        state[i] = product<T, P>(keys[(2 * i + s) * 64], l, state[i]);
+        for (int c = 0; c < C; ++c) o[c] = product(scores[s], wrote[s][c][p], o[c]);
     }
-    if (in) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const uint32_t t = index_of(i, 4 * g + r);
-          if (t < held) out[t * value_stride] = static_cast<T>(t < rows ? q[i][r] : 0.0f);
-        }
-      }
-    }
-  }
-  if (a.to == nullptr || !in) return;
-#pragma unroll
-  for (int i = 0; i < 2 * KT; ++i) {
+    __builtin_amdgcn_sched_barrier(0);
+    load_rest(next);
+    const uint32_t rows = rows_of(chunk);
+    const auto to = buffer_of(outs + chunk * kChunk * value_stride, kChunk * value_bytes);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const uint32_t k = index_of(i, 4 * g + r);
-      if (Whole || k < d.keys) a.to[state_at + static_cast<uint64_t>(k) * d.values] = state[i][r];
+      const uint32_t t = index_of(w, 4 * g + r);
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        store_to(to, t < rows && in[c]
+                         ? t * value_bytes + cols[c] * static_cast<uint32_t>(sizeof(T))
+                         : kNowhere,
+                 static_cast<T>(o[c][r]));
     }
+    if (chunk + 1 < live) hand_state(chunk + 1);
   }
+  // steps past the row's end
+  const uint32_t end = min(d.time - start, d.chunks * kChunk);
+  for (uint32_t t = (length <= start ? 0 : length - start) + 4 * w + g; t < end; t += 16) {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (in[c]) outs[t * value_stride + cols[c]] = static_cast<T>(0.0f);
+  }
+  if (a.to == nullptr || !holds) return;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const uint32_t k = key_at(i, r);
+      if (k >= d.keys) continue;
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        if (in[c]) a.to[state_at + static_cast<uint64_t>(k) * d.values + cols[c]] = state[i][c][r];
+    }
 }
 
 template <typename T>
@@ -397,16 +544,16 @@ __global__ __launch_bounds__(256) void delta_step_kernel(StepArgs<T> a) {
 // Steps taken one by one where no backward is to follow.
 constexpr uint64_t kStepLimit = 16;
 
-template <typename T>
+template <typename T, int P>
 struct ForwardPlan {
   Plan p;
   uint64_t head_bytes, key_bytes, state_bytes;  // of the workspace
   uint64_t bytes() const { return head_bytes + key_bytes + state_bytes; }
   ForwardPlan(const oxh_delta_shape &s, float scale, const int32_t *lengths)
       : p(s, scale, lengths) {
-    const uint64_t head = s.batch * s.heads * Chunk<T>::bytes;
-    const uint64_t key = s.batch * s.key_heads * p.steps * 4 * Chunk<T>::operand_bytes;
-    p.segment = std::min(p.all, std::max<uint64_t>(1, kPrepared / std::max<uint64_t>(1, head + key)));
+    const uint64_t head = s.batch * s.heads * Chunk<T, P>::bytes;
+    const uint64_t key = s.batch * s.key_heads * p.steps * 12 * kOperandBytes<T>;
+    p.divide(head + key);
     head_bytes = round_up(p.segment * head, 256);
     key_bytes = round_up(p.segment * key, 256);
     state_bytes = p.segment < p.all ? round_up(p.state_elements(s) * 4, 256) : 0;
@@ -430,28 +577,36 @@ oxh_status by_steps(hipStream_t stream, const StepArgs<T> &a) {
   return oxh::launched("gated_delta_rule_steps");
 }
 
-template <typename T>
-oxh_status by_chunks(hipStream_t stream, const ForwardPlan<T> &plan, const T *query, const T *key, const T *value,
+template <typename T, int P>
+oxh_status by_chunks(hipStream_t stream, const ForwardPlan<T, P> &plan, const T *query, const T *key, const T *value,
                      const T *gate, const T *write, const float *initial, T *out, float *final,
                      char *saved, char *workspace) {
   const Plan &p = plan.p;
   char *heads = workspace, *keys = heads + plan.head_bytes;
   float *between = reinterpret_cast<float *>(keys + plan.key_bytes);
+  // slabs of a block: as many as leave a block for each compute unit
+  const uint64_t all_heads = static_cast<uint64_t>(p.d.batch) * p.d.heads;
+  auto blocks = [&](uint32_t slabs) { return (p.d.slabs + slabs - 1) / slabs; };
+  const bool two = all_heads * blocks(2) >= oxh::kComputeUnits;
   for (uint64_t first = 0; first < p.all; first += p.segment) {
     Dims d = p.d;
     d.first = static_cast<uint32_t>(first);
     d.chunks = static_cast<uint32_t>(std::min(p.segment, p.all - first));
     const bool last = first + p.segment >= p.all;
     const PrepareArgs<T> prepare{d, query, key, gate, write, heads, keys};
-    const ScanArgs<T> scan{d, query, key, value, heads, keys, first == 0 ? initial : between,
+    const ScanArgs<T> scan{d, value, heads, keys, first == 0 ? initial : between,
                            last ? final : between, out, saved, static_cast<uint32_t>(p.all)};
-    with_keys(d.keys, [&](auto steps, auto whole) {
+    with_keys(d.keys, d.keys % 32 == 0, [&](auto steps, auto whole) {
       constexpr int KT = decltype(steps)::value;
       constexpr bool W = decltype(whole)::value;
-      oxh::launch(delta_prepare_kernel<T, KT, W>, dim3(d.chunks, d.heads, d.batch), dim3(256), 0,
+      oxh::launch(delta_prepare_kernel<T, P, KT, W>, dim3(d.chunks, d.heads, d.batch), dim3(256), 0,
                   stream, prepare);
-      oxh::launch(delta_scan_kernel<T, KT, W>, dim3(d.slabs, d.heads, d.batch), dim3(64), 0,
-                  stream, scan);
+      if (two)
+        oxh::launch(delta_scan_kernel<T, P, KT, 2>, dim3(blocks(2), d.heads, d.batch), dim3(256), 0,
+                    stream, scan);
+      else
+        oxh::launch(delta_scan_kernel<T, P, KT, 1>, dim3(blocks(1), d.heads, d.batch), dim3(256), 0,
+                    stream, scan);
     });
     oxh_status st = oxh::launched("gated_delta_rule");
     if (st != OXH_OK) return st;
@@ -467,7 +622,7 @@ template <typename T>
 uint64_t saved_bytes(const oxh_delta_shape &s) {
   const uint64_t steps = round_up(s.key_dim, 32) / 32;
   return s.batch * s.heads * ((s.time + kChunk - 1) / kChunk) * ((s.value_dim + 15) / 16) *
-         (steps + 2) * Chunk<T>::operand_bytes;
+         (steps + 2) * kOperandBytes<T>;
 }
 
 }  // namespace
@@ -490,8 +645,8 @@ oxh_status oxh_gated_delta_rule_workspace_size(int dtype, const oxh_delta_shape 
   if (st != OXH_OK) return st;
   *bytes = 0;
   if (by_steps_alone(*shape, saves != 0)) return oxh::ok();
-  *bytes = dtype == OXH_F32 ? ForwardPlan<float>(*shape, 1.0f, nullptr).bytes()
-                            : ForwardPlan<bf16>(*shape, 1.0f, nullptr).bytes();
+  *bytes = dtype == OXH_F32 ? ForwardPlan<float, 1>(*shape, 1.0f, nullptr).bytes()
+                            : ForwardPlan<bf16, 2>(*shape, 1.0f, nullptr).bytes();
   return oxh::ok();
 }
 
@@ -550,18 +705,26 @@ oxh_status oxh_gated_delta_rule_forward(oxh_stream stream, int dtype, const oxh_
   auto run = [&](auto type) {
     using T = decltype(type);
     hipStream_t on = oxh::as_stream(stream);
-    const ForwardPlan<T> plan(s, scale, lengths);
     if (steps) {
-      const StepArgs<T> a{plan.p.d, static_cast<const T *>(query), static_cast<const T *>(key),
-                          static_cast<const T *>(value), static_cast<const T *>(gate),
-                          static_cast<const T *>(write), initial_state, final_state,
-                          static_cast<T *>(output)};
+      const StepArgs<T> a{Plan(s, scale, lengths).d, static_cast<const T *>(query),
+                          static_cast<const T *>(key), static_cast<const T *>(value),
+                          static_cast<const T *>(gate), static_cast<const T *>(write),
+                          initial_state, final_state, static_cast<T *>(output)};
       return by_steps(on, a);
     }
-    return by_chunks<T>(on, plan, static_cast<const T *>(query), static_cast<const T *>(key),
-                        static_cast<const T *>(value), static_cast<const T *>(gate),
-                        static_cast<const T *>(write), initial_state, static_cast<T *>(output),
-                        final_state, static_cast<char *>(saved), static_cast<char *>(workspace));
+    auto chunks = [&](auto parts) {
+      constexpr int P = decltype(parts)::value;
+      return by_chunks<T, P>(
+          on, ForwardPlan<T, P>(s, scale, lengths), static_cast<const T *>(query),
+          static_cast<const T *>(key), static_cast<const T *>(value), static_cast<const T *>(gate),
+          static_cast<const T *>(write), initial_state, static_cast<T *>(output), final_state,
+          static_cast<char *>(saved), static_cast<char *>(workspace));
+    };
+    // a state that is handed on keeps 16 bits of what is formed on its way, one that serves these
+    // outputs alone as many as they do
+    if constexpr (sizeof(T) == 2)
+      if (final_state != nullptr) return chunks(std::integral_constant<int, 2>());
+    return chunks(std::integral_constant<int, 1>());
   };
   return dtype == OXH_F32 ? run(float()) : run(bf16());
 }

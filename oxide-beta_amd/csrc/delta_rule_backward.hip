@@ -23,6 +23,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstddef>
 #include <string>
 #include <vector>
 
@@ -36,10 +37,11 @@ using namespace oxh::delta;
 using oxh::storage::widen;
 
 // What a chunk's kernels leave each other, per value head; then per slab of 16 columns of values
-// dS as operands, the sums over its columns of e x, and <dS, exp(g_64) S0>.
+// dS as operands, and for each block of slabs, at its first, the sums over its columns of e x and
+// (four parts of) <dS, exp(g_64) S0>.
 template <typename T>
 struct Back {
-  static constexpr uint64_t operand_bytes = Chunk<T>::operand_bytes, gates = 0,
+  static constexpr uint64_t operand_bytes = kOperandBytes<T>, gates = 0,
                             system = sizeof(Gates), within = system + kTriangle * operand_bytes,
                             slabs = within + kTriangle * operand_bytes;
   static __host__ __device__ constexpr uint64_t slab(uint64_t steps) {
@@ -55,11 +57,12 @@ struct Args {
   Dims d;
   const T *query, *key, *gate, *write, *gradient;
   const char *saved;
-  char *heads, *keys;   // Back<T> of (batch, head, chunk); transposed keys, queries
+  char *heads, *keys;   // Back<T> of (batch, head, chunk); keys, their transpose, queries' transpose
   const float *from;    // gradients of the states behind the launch's chunks, null: 0
   float *to;            // and before them, may be null
   T *dquery, *dkey, *dvalue, *dgate, *dwrite;
   uint32_t all;         // chunks of the whole sequence
+  uint32_t together;    // slabs of a block of the scan
 };
 
 template <typename T, int KT, bool Whole>
@@ -110,12 +113,15 @@ __global__ __launch_bounds__(256) void delta_backward_prepare_kernel(Args<T> a) 
     reinterpret_cast<Op *>(out + Back<T>::system)[p * 64 + lane] = rounded<T>(v);
   }
   if (at.head % d.group != 0) return;
-  Op *to = reinterpret_cast<Op *>(a.keys) + at.key_chunk(d) * (8 * KT * 64);
-  store_transposed<T, KT>(m.tile, to);
+  Op *to = reinterpret_cast<Op *>(a.keys) + at.key_chunk(d) * (12 * KT * 64);
+#pragma unroll
+  for (int s = 0; s < KT; ++s)
+    to[(wave * KT + s) * 64 + lane] = m.key_row(index_of(wave, n), s, g);
+  store_transposed<T, KT>(m.tile, to + 4 * KT * 64);
   __syncthreads();
   load_tile<T, KT, Whole>(m.tile, d, at, a.query);
   __syncthreads();
-  store_transposed<T, KT>(m.tile, to + 4 * KT * 64);
+  store_transposed<T, KT>(m.tile, to + 8 * KT * 64);
 }
 
 // The sums over the 16 lanes of a group.
@@ -127,153 +133,322 @@ __device__ __forceinline__ float row_total(float v) {
   return v;
 }
 
-// A wave per 16 columns of a head's values, from the last chunk to the first.
-template <typename T, int KT, bool Whole>
+// What the block's waves hand each other, as operands: dS, do and scale exp(g) do (of this chunk and
+// the next), -b du and -exp(g) dv.
+template <typename T, int KT, int C>
+struct Exchange {
+  operand<T> state[KT][C][64], out[2][2][C][64], decayed[2][2][C][64], weighted[2][C][64],
+      taken[2][C][64];
+};
+
+// A block of four waves per C slabs of 16 columns of a head's values, from the last chunk to the
+// first; the waves share a chunk as the forward's do.
+template <typename T, int KT, int C>
 __global__ __launch_bounds__(256) void delta_backward_scan_kernel(Args<T> a) {
   using Op = operand<T>;
+  using Kept = Back<T>;
+  __shared__ Exchange<T, KT, C> m;
   const Dims &d = a.d;
   const uint32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-  const uint32_t slab = blockIdx.x * (blockDim.x >> 6) +
-                        __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (slab >= d.slabs) return;
-  const uint32_t h = blockIdx.y, b = blockIdx.z;
-  const uint32_t column = 16 * slab + n;
-  const bool in = column < d.values;
-  const uint32_t col = in ? column : d.values - 1;
+  const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = w & 1;
+  const int pair = w >> 1;
+  const oxh::BlockTile block = oxh::xcd_block();
+  const uint32_t h = block.y, b = block.z, kh = h / d.group;
+  const uint32_t length = length_of(d, b), start = d.first * kChunk;
+  const uint32_t live =
+      length <= start ? 0 : min((length - start + kChunk - 1) / kChunk, d.chunks);
   const uint64_t head = static_cast<uint64_t>(b) * d.heads + h;
-  const uint64_t stride = static_cast<uint64_t>(d.key_heads) * d.keys;
   const uint64_t value_stride = static_cast<uint64_t>(d.heads) * d.values;
-  f32x4 ds[2 * KT];
-  const uint64_t state_at = head * d.keys * d.values + col;
+  const uint64_t value0 = (static_cast<uint64_t>(b) * d.time + start) * value_stride +
+                          static_cast<uint64_t>(h) * d.values;
+  const T *gradients = a.gradient + value0;
+  T *dvalues = a.dvalue + value0;
+  const uint64_t block_bytes = Kept::bytes(KT, d.slabs);
+  char *chunks = a.heads + head * d.chunks * block_bytes;
+  constexpr uint32_t kOperand = 64 * sizeof(Op), kKeys = 4 * KT * kOperand;
+  const char *keys =
+      a.keys + (static_cast<uint64_t>(b) * d.key_heads + kh) * d.chunks * (3 * kKeys);
+  uint32_t cols[C];  // this lane's; those past the last are the last again, with gradients of 0
+  bool in[C], own[C];
 #pragma unroll
-  for (int i = 0; i < 2 * KT; ++i) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const uint32_t k = index_of(i, 4 * g + r);
-      ds[i][r] = a.from != nullptr && in && (Whole || k < d.keys)
-                     ? a.from[state_at + static_cast<uint64_t>(k) * d.values]
-                     : 0.0f;
-    }
+  for (int c = 0; c < C; ++c) {
+    const uint32_t slab = block.x * C + c, column = 16 * slab + n;
+    own[c] = slab < d.slabs;
+    in[c] = column < d.values;
+    cols[c] = in[c] ? column : d.values - 1;
   }
-  for (uint32_t chunk = d.chunks; chunk-- != 0;) {
-    const Place at(d, chunk, h, b);
-    const uint32_t held = min(d.time - at.begin, static_cast<uint32_t>(kChunk)), rows = at.rows;
-    const uint64_t value_at = at.value_row * d.values + col;
-    T *dvalue = a.dvalue + value_at;
-    if (rows == 0) {
-      if (in)
-        for (uint32_t t = g; t < held; t += 4) dvalue[t * value_stride] = static_cast<T>(0.0f);
-      continue;
-    }
-    const T *key = a.key + at.key_row * d.keys;
-    const T *gradient = a.gradient + value_at;
-    char *block = a.heads + at.head_chunk(d) * Back<T>::bytes(KT, d.slabs);
-    const Gates *gates = reinterpret_cast<const Gates *>(block + Back<T>::gates);
-    const Op *system = reinterpret_cast<const Op *>(block + Back<T>::system) + lane;
-    const Op *within = reinterpret_cast<const Op *>(block + Back<T>::within) + lane;
-    const Op *keys = reinterpret_cast<const Op *>(a.keys) + at.key_chunk(d) * (8 * KT * 64) + lane;
-    const Op *queries = keys + 4 * KT * 64;
-    const Op *kept = reinterpret_cast<const Op *>(a.saved) +
-                     ((head * a.all + d.first + chunk) * d.slabs + slab) * ((KT + 2) * 64) + lane;
-    char *own = block + Back<T>::slabs + slab * Back<T>::slab(KT);
-    auto vec = [&](const float *v, int tile) {
-      return *reinterpret_cast<const f32x4 *>(v + 32 * (tile >> 1) + 8 * g + 4 * (tile & 1));
-    };
-
-    Op out[2], decayed[2];  // do, and scale exp(g) do
+  auto rows_of = [&](uint32_t chunk) -> uint32_t {
+    return min(length - start - chunk * kChunk, static_cast<uint32_t>(kChunk));
+  };
+  const bool holds = w < KT;  // keys 32 w on
+  const uint64_t state_at = head * d.keys * d.values;
+  auto key_at = [&](int tile, int r) { return 32 * w + index_of(tile, 4 * g + r); };
+  f32x4 ds[2][C];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      f32x8 v;
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t t = 32 * s + 8 * g + j;
-        v[j] = t < rows && in ? widen(gradient[t * value_stride]) : 0.0f;
-      }
-      out[s] = rounded<T>(v);
-      decayed[s] = rounded<T>(v * join(vec(gates->since, 2 * s), vec(gates->since, 2 * s + 1)) *
-                              d.scale);
-    }
-    // the state's gradient as an operand, its dot product with the state and its product with keys
-    f32x4 w[4] = {};
-    float across = 0.0f;
-    const float whole = gates->since[kChunk - 1];
-#pragma unroll
-    for (int s = 0; s < KT; ++s) {
-      const f32x8 v = join(ds[2 * s], ds[2 * s + 1]), state = widened(kept[s * 64]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) across = fmaf(v[j], state[j], across);
-      const Op op = rounded<T>(v);
-      reinterpret_cast<Op *>(own)[s * 64 + lane] = op;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        w[i] = product(load_row<T, Whole>(key + min(index_of(i, n), rows - 1) * stride,
-                                          32 * s + 8 * g, d.keys), op, w[i]);
-    }
-    across *= whole;
-    f32x4 x[4];
-    {
-      f32x4 du[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        du[i] = vec(gates->until, i) * w[i];
-#pragma unroll
-        for (int s = i >> 1; s < 2; ++s) du[i] = product(within[upper_place(i, s) * 64], out[s], du[i]);
-        x[i] = du[i];
-        du[i] *= -vec(gates->write, i);
-      }
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const Op weighted = rounded<T>(join(du[2 * s], du[2 * s + 1]));
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if ((i >> 1) <= s) x[i] = product(system[upper_place(i, s) * 64], weighted, x[i]);
-      }
-    }
-    f32x4 dv[4], errors[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      dv[i] = vec(gates->write, i) * x[i];
-      const f32x8 e = widened(kept[(KT + (i >> 1)) * 64]);
+    for (int c = 0; c < C; ++c) {
+      ds[i][c] = f32x4{};
+      if (a.from == nullptr || !holds) continue;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const uint32_t t = index_of(i, 4 * g + r);
-        errors[i][r] = row_total(e[4 * (i & 1) + r] * x[i][r]);
-        if (t < held && in) dvalue[t * value_stride] = static_cast<T>(dv[i][r]);
+        const uint32_t k = key_at(i, r), there = min(k, d.keys - 1);
+        const float v = a.from[state_at + static_cast<uint64_t>(there) * d.values + cols[c]];
+        ds[i][c][r] = k < d.keys && in[c] ? v : 0.0f;
       }
     }
-    {
-      float total[1] = {across};
-      oxh::wave_sums_rows(total);
-      float *sums = reinterpret_cast<float *>(own + KT * Back<T>::operand_bytes);
-      if (n == 0) {
+
+  // Loaded and stored as the forward's.
+  typedef T quarter __attribute__((ext_vector_type(4)));
+  Op key[KT], scores[2], solve[2], back[2][2], forth[2][2], before[C];
+  T gradient[C][4];
+  quarter error[C];
+  f32x4 since, until, write, since_next;
+  float whole = 0.0f;
+  const uint32_t value_bytes = static_cast<uint32_t>(value_stride * sizeof(T));
+  const uint32_t lane_at = lane * sizeof(Op);
+  auto operands_of = [&](uint32_t chunk, uint64_t part) {
+    return chunks + (chunk * block_bytes + part);
+  };
+  auto load_keys = [&](uint32_t chunk) {
+    const char *from = keys + (chunk * uint64_t{3 * kKeys} + w * (KT * kOperand));
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<f32x4 *>(sums + index_of(i, 4 * g)) = errors[i];
-      }
-      if (lane == 0) sums[kChunk] = total[0];
-    }
+    for (int s = 0; s < KT; ++s) key[s] = load_at<Op>(from + s * kOperand, lane_at);
+  };
+  auto load_triangle = [&](uint32_t chunk, uint64_t part, Op(&to)[2]) {
+    const char *from = operands_of(chunk, part);
 #pragma unroll
-    for (int i = 0; i < 2 * KT; ++i) ds[i] *= whole;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const Op taken = rounded<T>(join(-vec(gates->since, 2 * s) * dv[2 * s],
-                                       -vec(gates->since, 2 * s + 1) * dv[2 * s + 1]));
-#pragma unroll
-      for (int i = 0; i < 2 * KT; ++i) {
-        ds[i] = product(queries[(2 * i + s) * 64], decayed[s], ds[i]);
-        ds[i] = product(keys[(2 * i + s) * 64], taken, ds[i]);
-      }
-    }
-  }
-  if (a.to == nullptr || !in) return;
-#pragma unroll
-  for (int i = 0; i < 2 * KT; ++i) {
+    for (int s = 0; s < 2; ++s)
+      to[s] = load_at<Op>(from + upper_place(w, max(s, pair)) * kOperand, lane_at);
+  };
+  auto load_gradients = [&](uint32_t chunk) {
+    const uint32_t last = rows_of(chunk) - 1;
+    const char *from = reinterpret_cast<const char *>(gradients + chunk * kChunk * value_stride);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const uint32_t k = index_of(i, 4 * g + r);
-      if (Whole || k < d.keys) a.to[state_at + static_cast<uint64_t>(k) * d.values] = ds[i][r];
+      const uint32_t row = min(index_of(w, 4 * g + r), last) * value_bytes;
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        gradient[c][r] = load_at<T>(from, row + cols[c] * static_cast<uint32_t>(sizeof(T)));
     }
+    since_next = load_at<f32x4>(operands_of(chunk, Kept::gates) + offsetof(Gates, since),
+                                index_of(w, 4 * g) * 4);
+  };
+  auto load_gates = [&](uint32_t chunk) {
+    const char *gates = operands_of(chunk, Kept::gates);
+    const uint32_t at = index_of(w, 4 * g) * 4;
+    since = load_at<f32x4>(gates + offsetof(Gates, since), at);
+    until = load_at<f32x4>(gates + offsetof(Gates, until), at);
+    write = load_at<f32x4>(gates + offsetof(Gates, write), at);
+  };
+  // the forward's states and errors; a block's slabs past the last read the last one's
+  const uint32_t kept = d.slabs * (KT + 2) * kOperand;
+  auto saved_of = [&](uint32_t chunk) {
+    return a.saved + (head * a.all + d.first + chunk) * kept;
+  };
+  auto saved_at = [&](int c, int place) {
+    return (min(block.x * C + c, d.slabs - 1) * (KT + 2) + place) * kOperand + lane_at;
+  };
+  auto load_errors = [&](uint32_t chunk) {
+    const char *from = saved_of(chunk);
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      error[c] = load_at<quarter>(
+          from, saved_at(c, KT + pair) + half * static_cast<uint32_t>(sizeof(quarter)));
+  };
+  auto load_rest = [&](uint32_t chunk) {
+    whole = load_at<float>(operands_of(chunk, Kept::gates) + offsetof(Gates, since),
+                           (kChunk - 1) * 4);
+    const char *k = keys + (chunk * uint64_t{3 * kKeys} + kKeys + 4 * min(w, KT - 1u) * kOperand);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        back[i][s] = load_at<Op>(k + (2 * i + s) * kOperand, lane_at);
+        forth[i][s] = load_at<Op>(k + kKeys + (2 * i + s) * kOperand, lane_at);
+      }
+    const char *from = saved_of(chunk);
+#pragma unroll
+    for (int c = 0; c < C; ++c) before[c] = load_at<Op>(from, saved_at(c, min(w, KT - 1u)));
+  };
+  auto hand = [&](Op(&to)[64], f32x4 v) {
+    reinterpret_cast<quarter *>(&to[lane])[half] = __builtin_convertvector(v, quarter);
+  };
+  auto hand_gradients = [&](uint32_t chunk) {
+    const uint32_t rows = rows_of(chunk);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      f32x4 v;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        v[r] = in[c] && index_of(w, 4 * g + r) < rows ? widen(gradient[c][r]) : 0.0f;
+      hand(m.out[chunk & 1][pair][c], v);
+      hand(m.decayed[chunk & 1][pair][c], since_next * d.scale * v);
+    }
+  };
+  // dS of the chunk, for its products and for those of the kernel behind
+  auto slabs_of = [&](uint32_t chunk) {
+    return buffer_of(operands_of(chunk, Kept::slabs), d.slabs * Kept::slab(KT));
+  };
+  auto hand_state = [&](uint32_t chunk) {
+    if (KT < 4 && !holds) return;
+    const auto to = slabs_of(chunk);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const Op v = rounded<T>(join(ds[0][c], ds[1][c]));
+      m.state[w][c][lane] = v;
+      store_to(to, own[c] ? (block.x * C + c) * static_cast<uint32_t>(Kept::slab(KT)) +
+                                w * kOperand + lane_at
+                          : kNowhere, v);
+    }
+  };
+  auto read_pairs = [&](Op(&to)[2][C], const Op(&from)[2][C][64]) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int c = 0; c < C; ++c) to[s][c] = from[s][c][lane];
+  };
+  if (live != 0) {
+    const uint32_t last = live - 1;
+    load_gradients(last);
+    load_keys(last);
+    load_triangle(last, Kept::within, scores);
+    load_gates(last);
+    load_triangle(last, Kept::system, solve);
+    load_errors(last);
+    load_rest(last);
+    hand_gradients(last);
+    load_gradients(last == 0 ? 0 : last - 1);
+    hand_state(last);
   }
+  for (uint32_t chunk = live; chunk-- != 0;) {
+    const uint32_t next = chunk == 0 ? 0 : chunk - 1, after = next == 0 ? 0 : next - 1;
+    lds_barrier();
+    // du = scale (G o q k')' do + exp(g_64 - g) k dS
+    f32x4 x[C] = {};
+    {
+      Op right[KT][C], out[2][C];
+#pragma unroll
+      for (int s = 0; s < KT; ++s)
+#pragma unroll
+        for (int c = 0; c < C; ++c) right[s][c] = m.state[s][c][lane];
+      read_pairs(out, m.out[chunk & 1]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int s = 0; s < KT; ++s)
+#pragma unroll
+        for (int c = 0; c < C; ++c) x[c] = product(key[s], right[s][c], x[c]);
+#pragma unroll
+      for (int c = 0; c < C; ++c) x[c] *= until;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if (s < pair) continue;
+#pragma unroll
+        for (int c = 0; c < C; ++c) x[c] = product(scores[s], out[s][c], x[c]);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) hand(m.weighted[pair][c], -write * x[c]);
+    __builtin_amdgcn_sched_barrier(0);
+    load_keys(next);
+    load_triangle(next, Kept::within, scores);
+    lds_barrier();
+    // x = du - N' (b du);  dv = b x
+    {
+      Op right[2][C];
+      read_pairs(right, m.weighted);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if (s < pair) continue;
+#pragma unroll
+        for (int c = 0; c < C; ++c) x[c] = product(solve[s], right[s][c], x[c]);
+      }
+    }
+    f32x4 sums = {};
+    const uint32_t rows = rows_of(chunk);
+    const auto to = buffer_of(dvalues + chunk * kChunk * value_stride, kChunk * value_bytes);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      if (own[c]) sums += __builtin_convertvector(error[c], f32x4) * x[c];
+      x[c] *= write;
+      hand(m.taken[pair][c], -since * x[c]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t t = index_of(w, 4 * g + r);
+        store_to(to, t < rows && in[c]
+                         ? t * value_bytes + cols[c] * static_cast<uint32_t>(sizeof(T))
+                         : kNowhere,
+                 static_cast<T>(x[c][r]));
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sums[r] = row_total(sums[r]);
+    const auto slabs = slabs_of(chunk);
+    const uint32_t sums_at = block.x * C * static_cast<uint32_t>(Kept::slab(KT)) + KT * kOperand;
+    store_to(slabs, n == 0 ? sums_at + index_of(w, 4 * g) * 4 : kNowhere, sums);
+    // the next chunk's gradients of the outputs
+    hand_gradients(next);
+    __builtin_amdgcn_sched_barrier(0);
+    load_triangle(next, Kept::system, solve);
+    load_errors(next);
+    load_gates(next);
+    load_gradients(after);
+    lds_barrier();
+    // dS0 = exp(g_64) dS + scale q' (exp(g) do) - k' (exp(g) dv)
+    Op decayed[2][C], taken[2][C];
+    read_pairs(decayed, m.decayed[chunk & 1]);
+    read_pairs(taken, m.taken);
+    __builtin_amdgcn_sched_barrier(0);
+    float across[1] = {0.0f};
+    if (KT == 4 || holds) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          ds[i][c] *= whole;
+          const f32x8 s0 = widened(before[c]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            across[0] = fmaf(ds[i][c][r], own[c] ? s0[4 * i + r] : 0.0f, across[0]);
+        }
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) ds[i][c] = product(forth[i][s], decayed[s][c], ds[i][c]);
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) ds[i][c] = product(back[i][s], taken[s][c], ds[i][c]);
+    }
+    oxh::wave_sums_rows(across);
+    store_to(slabs, lane == 0 ? sums_at + (kChunk + w) * 4 : kNowhere, across[0]);
+    __builtin_amdgcn_sched_barrier(0);
+    load_rest(next);
+    if (chunk != 0) hand_state(next);
+  }
+  // steps past the row's end
+  const uint32_t end = min(d.time - start, d.chunks * kChunk);
+  for (uint32_t t = (length <= start ? 0 : length - start) + 4 * w + g; t < end; t += 16) {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (in[c]) dvalues[t * value_stride + cols[c]] = static_cast<T>(0.0f);
+  }
+  if (a.to == nullptr || !holds) return;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const uint32_t k = key_at(i, r);
+      if (k >= d.keys) continue;
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        if (in[c]) a.to[state_at + static_cast<uint64_t>(k) * d.values + cols[c]] = ds[i][c][r];
+    }
 }
 
 constexpr int kColumns = 32;  // of values that the products take at a time
@@ -307,7 +482,8 @@ __global__ __launch_bounds__(256) void delta_backward_products_kernel(Args<T> a)
   f32x8 dq[KT] = {}, dk[KT] = {};
   const Place first(d, chunk, kh * d.group, b);
   const uint32_t held = min(d.time - first.begin, static_cast<uint32_t>(kChunk)), rows = first.rows;
-  const Op *keys = reinterpret_cast<const Op *>(a.keys) + first.key_chunk(d) * (8 * KT * 64) + lane;
+  const Op *keys =
+      reinterpret_cast<const Op *>(a.keys) + (first.key_chunk(d) * 12 + 4) * (KT * 64) + lane;
   const Op *queries = keys + 4 * KT * 64;
   for (uint32_t h = kh * d.group; h < (kh + 1) * d.group; ++h) {
     const Place at(d, chunk, h, b);
@@ -503,11 +679,11 @@ __global__ __launch_bounds__(256) void delta_backward_products_kernel(Args<T> a)
     for (int i = 0; i < KT; ++i) dk[i] += piece(i);
     if (threadIdx.x < kChunk) {
       float error = 0.0f, constant = 0.0f;
-      for (uint32_t slab = 0; slab < d.slabs; ++slab) {
+      for (uint32_t slab = 0; slab < d.slabs; slab += a.together) {
         const float *sums = reinterpret_cast<const float *>(
             block + Back<T>::slabs + slab * Back<T>::slab(KT) + KT * Back<T>::operand_bytes);
         error += sums[lane];
-        constant += sums[kChunk];
+        constant += (sums[kChunk] + sums[kChunk + 1]) + (sums[kChunk + 2] + sums[kChunk + 3]);
       }
       float after = m.rows_at[lane], before = m.before[lane];
 #pragma unroll
@@ -553,8 +729,8 @@ struct BackPlan {
   explicit BackPlan(const oxh_delta_shape &s, float scale, const int32_t *lengths)
       : p(s, scale, lengths) {
     const uint64_t head = s.batch * s.heads * Back<T>::bytes(p.steps, p.d.slabs);
-    const uint64_t key = s.batch * s.key_heads * p.steps * 8 * Chunk<T>::operand_bytes;
-    p.segment = std::min(p.all, std::max<uint64_t>(1, kPrepared / std::max<uint64_t>(1, head + key)));
+    const uint64_t key = s.batch * s.key_heads * p.steps * 12 * kOperandBytes<T>;
+    p.divide(head + key);
     head_bytes = round_up(p.segment * head, 256);
     key_bytes = round_up(p.segment * key, 256);
     state_bytes = p.segment < p.all ? round_up(p.state_elements(s) * 4, 256) : 0;
@@ -570,6 +746,8 @@ oxh_status backward(hipStream_t stream, const BackPlan<T> &plan, Args<T> a, cons
   const Plan &p = plan.p;
   a.all = static_cast<uint32_t>(p.all);
   const uint64_t launches = (p.all + p.segment - 1) / p.segment;
+  auto blocks = [&](uint32_t slabs) { return (p.d.slabs + slabs - 1) / slabs; };
+  a.together = static_cast<uint64_t>(p.d.batch) * p.d.heads * blocks(2) >= oxh::kComputeUnits ? 2 : 1;
   for (uint64_t i = launches; i-- != 0;) {
     const uint64_t first = i * p.segment;
     a.d = p.d;
@@ -578,13 +756,16 @@ oxh_status backward(hipStream_t stream, const BackPlan<T> &plan, Args<T> a, cons
     a.from = i + 1 == launches ? final : between;
     a.to = i == 0 ? initial : between;
     const Dims &d = a.d;
-    with_keys(d.keys, [&](auto steps, auto whole) {
+    with_keys(d.keys, d.keys % 32 == 0, [&](auto steps, auto whole) {
       constexpr int KT = decltype(steps)::value;
       constexpr bool W = decltype(whole)::value;
       oxh::launch(delta_backward_prepare_kernel<T, KT, W>, dim3(d.chunks, d.heads, d.batch),
                   dim3(256), 0, stream, a);
-      oxh::launch(delta_backward_scan_kernel<T, KT, W>, dim3(d.slabs, d.heads, d.batch), dim3(64),
-                  0, stream, a);
+      const dim3 scan(blocks(a.together), d.heads, d.batch);
+      if (a.together == 2)
+        oxh::launch(delta_backward_scan_kernel<T, KT, 2>, scan, dim3(256), 0, stream, a);
+      else
+        oxh::launch(delta_backward_scan_kernel<T, KT, 1>, scan, dim3(256), 0, stream, a);
       const dim3 grid(d.chunks, d.key_heads, d.batch);
       if (d.values % kColumns == 0)
         oxh::launch(delta_backward_products_kernel<T, KT, W, true>, grid, dim3(256), 0, stream, a);
