@@ -134,6 +134,23 @@ __device__ __forceinline__ operand<T> load_row(const T *row, uint32_t at, uint32
   return v;
 }
 
+template <typename T, bool Whole>
+__device__ __forceinline__ void store_row(T *row, uint32_t at, uint32_t count, operand<T> v) {
+  if (Whole || at + 8 <= count) {
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<typename storage::Pack<T, 8>::type *>(row + at) = v;
+    } else {
+      typedef typename storage::Pack<T, 4>::type half;
+      *reinterpret_cast<half *>(row + at) = __builtin_shufflevector(v, v, 0, 1, 2, 3);
+      *reinterpret_cast<half *>(row + at + 4) = __builtin_shufflevector(v, v, 4, 5, 6, 7);
+    }
+    return;
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < 8; ++i)
+    if (at + i < count) row[at + i] = v[i];
+}
+
 // A lane's column of a state as the matrix cores' results, from `at` on (null: 0).
 template <int KT, bool Whole>
 __device__ __forceinline__ void load_state(f32x4 (&state)[2 * KT], const float *at, const Dims &d,
@@ -161,6 +178,43 @@ __device__ __forceinline__ int lower_place(int tile, int step) {
 }
 __device__ __forceinline__ int upper_place(int tile, int step) {
   return tile < 2 ? 2 * tile + step : tile + 2;
+}
+
+// Operands of two slabs of 16 columns in shared memory, the first one's from `first` on, the other's
+// `apart` behind: each lane a column, 8 rows.  From there the operand of their transpose, for sums
+// over the columns: a lane one of the 16 rows that index_of numbers for tile `half`, 8 of the 32
+// columns.
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+__device__ __forceinline__ bf16x8 turned(const bf16x8 *first, uint32_t apart, int half, uint32_t n,
+                                         uint32_t g) {
+  // 16 lanes read four columns' 16 rows, four of them each, and get a row of it
+  const bf16x8 *at = first + (g >> 1) * apart + (n & 3) * 16 + 8 * (g & 1) + (n >> 2);
+  s16x4 v[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    v[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_s16x4 *)(reinterpret_cast<const s16x4 *>(at + 4 * e) + half));
+  return __builtin_bit_cast(bf16x8, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
+}
+__device__ __forceinline__ f32x8 turned(const f32x8 *first, uint32_t apart, int half, uint32_t n,
+                                        uint32_t g) {
+  const f32x8 *at = first + (g >> 1) * apart + (n >> 2) * 16 + 8 * (g & 1);
+  f32x8 v;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    v[i] = reinterpret_cast<const float *>(at + i)[4 * half + (n & 3)];
+  return v;
+}
+
+// 16 bytes of each lane from memory to `to` + 16 * lane in shared memory, without a stop in
+// registers; they are there behind arrived().
+__device__ __forceinline__ void copy_16(const void *from, void *to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
+                                   (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+}
+__device__ __forceinline__ void arrived() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
 // Where the block's waves see each other's shared memory; loads from memory stay on their way.
@@ -388,6 +442,10 @@ constexpr uint64_t kMostKeys = 128;
 constexpr uint64_t kPrepared = 192ull << 20;
 
 inline uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
+
+// What the forward leaves the backward of a chunk and a pair of slabs: its state (tiles of 16 keys)
+// and its errors (tiles of 16 steps) as operands of sums over the values.
+inline uint64_t pairs_of(uint64_t values) { return (values + 31) / 32; }
 
 struct Plan {
   Dims d;

@@ -121,10 +121,12 @@ struct ScanArgs {
   uint32_t all;       // chunks of the whole sequence
 };
 
-// What the block's waves hand each other, as operands: the state, b y, b e and exp(g_64 - g) b e.
+// What the block's waves hand each other, as operands: the state, b y, b e, exp(g_64 - g) b e, and e
+// for the backward.
 template <typename T, int P, int KT, int C>
 struct Exchange {
-  operand<T> state[KT][C][P][64], weighted[2][C][P][64], wrote[2][C][P][64], left[2][C][P][64];
+  operand<T> state[KT][C][P][64], weighted[2][C][P][64], wrote[2][C][P][64], left[2][C][P][64],
+      error[2][C][64];
 };
 
 // A block of four waves per C slabs of 16 columns of a head's values.  A wave takes 16 of a chunk's
@@ -157,11 +159,10 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(ScanArgs<T> a) {
   const char *keys =
       a.keys + (static_cast<uint64_t>(b) * d.key_heads + kh) * d.chunks * (3 * kKeys);
   uint32_t cols[C];  // this lane's; those past the last are the last again, and not stored
-  bool in[C], own[C];
+  bool in[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const uint32_t slab = block.x * C + c, column = 16 * slab + n;
-    own[c] = slab < d.slabs;
+    const uint32_t column = 16 * (block.x * C + c) + n;
     in[c] = column < d.values;
     cols[c] = in[c] ? column : d.values - 1;
   }
@@ -257,13 +258,14 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(ScanArgs<T> a) {
       if (p + 1 < P) v -= __builtin_convertvector(q, f32x4);
     }
   };
-  // what the backward reads of a chunk: its slabs' states and errors
-  const uint32_t kept = d.slabs * (KT + 2) * kOperand;
+  // what the backward reads of a chunk; a block of one slab brings its half of the pair's lanes
+  const uint32_t kept = (d.slabs + 1) / 2 * (2 * KT + 4) * kOperand;
   auto saved_of = [&](uint32_t chunk) {
     return buffer_of(a.saved + ((head * a.all + d.first + chunk) * kept), a.saved == nullptr ? 0 : kept);
   };
-  auto saved_at = [&](int c, int place) {
-    return own[c] ? ((block.x * C + c) * (KT + 2) + place) * kOperand + lane_at : kNowhere;
+  const bool brings = C == 2 || (g >> 1) == (block.x & 1);
+  auto saved_at = [&](int place) {
+    return brings ? (block.x * C / 2 * (2 * KT + 4) + place) * kOperand + lane_at : kNowhere;
   };
   auto hand_state = [&](uint32_t chunk) {
     if (KT < 4 && !holds) return;
@@ -272,8 +274,12 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(ScanArgs<T> a) {
       const Split<T, P> st(join(state[0][c], state[1][c]));
 #pragma unroll
       for (int p = 0; p < P; ++p) m.state[w][c][p][lane] = st.part[p];
-      store_to(saved_of(chunk), saved_at(c, w), st.part[0]);
     }
+    if (a.saved == nullptr) return;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      store_to(saved_of(chunk), saved_at(2 * w + i),
+               turned(&m.state[w][0][0][0], C == 2 ? P * 64 : 0, i, n, g));
   };
   // right operands of 64 steps, all of them on their way before the first is used
   auto read_pairs = [&](Op(&to)[2][C][P], const Op(&from)[2][C][P][64]) {
@@ -349,9 +355,9 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(ScanArgs<T> a) {
     load_system(next);
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const uint32_t at = saved_at(c, KT + pair);
-      store_to(saved_of(chunk), own[c] ? at + half * static_cast<uint32_t>(sizeof(quarter)) : at,
-               __builtin_convertvector(y[c], quarter));
+      if (a.saved != nullptr)
+        reinterpret_cast<quarter *>(&m.error[pair][c][lane])[half] =
+            __builtin_convertvector(y[c], quarter);
       y[c] *= write;
       hand(m.wrote[pair][c], y[c]);
       hand(m.left[pair][c], until * y[c]);
@@ -385,6 +391,9 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(ScanArgs<T> a) {
 #pragma unroll
         for (int c = 0; c < C; ++c) o[c] = product(scores[s], wrote[s][c][p], o[c]);
     }
+    if (a.saved != nullptr)
+      store_to(saved_of(chunk), saved_at(2 * KT + w),
+               turned(&m.error[pair][0][0], C == 2 ? 64 : 0, half, n, g));
     __builtin_amdgcn_sched_barrier(0);
     load_rest(next);
     const uint32_t rows = rows_of(chunk);
@@ -586,8 +595,8 @@ oxh_status by_chunks(hipStream_t stream, const ForwardPlan<T, P> &plan, const T 
   float *between = reinterpret_cast<float *>(keys + plan.key_bytes);
   // slabs of a block: as many as leave a block for each compute unit
   const uint64_t all_heads = static_cast<uint64_t>(p.d.batch) * p.d.heads;
-  auto blocks = [&](uint32_t slabs) { return (p.d.slabs + slabs - 1) / slabs; };
-  const bool two = all_heads * blocks(2) >= oxh::kComputeUnits;
+  const uint32_t pairs = (p.d.slabs + 1) / 2;
+  const bool two = all_heads * pairs >= oxh::kComputeUnits;
   for (uint64_t first = 0; first < p.all; first += p.segment) {
     Dims d = p.d;
     d.first = static_cast<uint32_t>(first);
@@ -602,10 +611,10 @@ oxh_status by_chunks(hipStream_t stream, const ForwardPlan<T, P> &plan, const T 
       oxh::launch(delta_prepare_kernel<T, P, KT, W>, dim3(d.chunks, d.heads, d.batch), dim3(256), 0,
                   stream, prepare);
       if (two)
-        oxh::launch(delta_scan_kernel<T, P, KT, 2>, dim3(blocks(2), d.heads, d.batch), dim3(256), 0,
+        oxh::launch(delta_scan_kernel<T, P, KT, 2>, dim3(pairs, d.heads, d.batch), dim3(256), 0,
                     stream, scan);
       else
-        oxh::launch(delta_scan_kernel<T, P, KT, 1>, dim3(blocks(1), d.heads, d.batch), dim3(256), 0,
+        oxh::launch(delta_scan_kernel<T, P, KT, 1>, dim3(2 * pairs, d.heads, d.batch), dim3(256), 0,
                     stream, scan);
     });
     oxh_status st = oxh::launched("gated_delta_rule");
@@ -621,8 +630,8 @@ bool by_steps_alone(const oxh_delta_shape &s, bool saves) {
 template <typename T>
 uint64_t saved_bytes(const oxh_delta_shape &s) {
   const uint64_t steps = round_up(s.key_dim, 32) / 32;
-  return s.batch * s.heads * ((s.time + kChunk - 1) / kChunk) * ((s.value_dim + 15) / 16) *
-         (steps + 2) * kOperandBytes<T>;
+  return s.batch * s.heads * ((s.time + kChunk - 1) / kChunk) * pairs_of(s.value_dim) *
+         (2 * steps + 4) * kOperandBytes<T>;
 }
 
 }  // namespace

@@ -36,19 +36,18 @@ namespace {
 using namespace oxh::delta;
 using oxh::storage::widen;
 
-// What a chunk's kernels leave each other, per value head; then per slab of 16 columns of values
-// dS as operands, and for each block of slabs, at its first, the sums over its columns of e x and
-// (four parts of) <dS, exp(g_64) S0>.
+// What a chunk's kernels leave each other, per value head; then per pair of slabs dS (tiles of 16
+// keys) and x (tiles of 16 steps) as operands of sums over the values.
 template <typename T>
 struct Back {
-  static constexpr uint64_t operand_bytes = kOperandBytes<T>, gates = 0,
-                            system = sizeof(Gates), within = system + kTriangle * operand_bytes,
-                            slabs = within + kTriangle * operand_bytes;
-  static __host__ __device__ constexpr uint64_t slab(uint64_t steps) {
-    return steps * operand_bytes + (kChunk + 8) * 4;
+  static constexpr uint64_t gates = 0, system = sizeof(Gates),
+                            within = system + kTriangle * kOperandBytes<T>,
+                            pairs = within + kTriangle * kOperandBytes<T>;
+  static __host__ __device__ constexpr uint64_t pair(uint64_t steps) {
+    return (2 * steps + 4) * kOperandBytes<T>;
   }
   static __host__ __device__ constexpr uint64_t bytes(uint64_t steps, uint64_t count) {
-    return slabs + count * slab(steps);
+    return pairs + count * pair(steps);
   }
 };
 
@@ -61,8 +60,7 @@ struct Args {
   const float *from;    // gradients of the states behind the launch's chunks, null: 0
   float *to;            // and before them, may be null
   T *dquery, *dkey, *dvalue, *dgate, *dwrite;
-  uint32_t all;         // chunks of the whole sequence
-  uint32_t together;    // slabs of a block of the scan
+  uint32_t all, pairs;  // chunks of the whole sequence; pairs of slabs
 };
 
 template <typename T, int KT, bool Whole>
@@ -76,7 +74,7 @@ __global__ __launch_bounds__(256) void delta_backward_prepare_kernel(Args<T> a) 
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const T *query = a.query + at.key_row * d.keys;
   const uint64_t stride = static_cast<uint64_t>(d.key_heads) * d.keys;
-  char *out = a.heads + at.head_chunk(d) * Back<T>::bytes(KT, d.slabs);
+  char *out = a.heads + at.head_chunk(d) * Back<T>::bytes(KT, a.pairs);
   solve<T, KT, Whole>(
       m, d, at, a.key, a.gate, a.write, reinterpret_cast<Gates *>(out + Back<T>::gates), [&] {
         // (G o q k')', a lane its key's step i, queries' steps t
@@ -134,11 +132,12 @@ __device__ __forceinline__ float row_total(float v) {
 }
 
 // What the block's waves hand each other, as operands: dS, do and scale exp(g) do (of this chunk and
-// the next), -b du and -exp(g) dv.
+// the next), -b du, -exp(g) dv, and
+// x for the products.
 template <typename T, int KT, int C>
 struct Exchange {
   operand<T> state[KT][C][64], out[2][2][C][64], decayed[2][2][C][64], weighted[2][C][64],
-      taken[2][C][64];
+      taken[2][C][64], x[2][C][64];
 };
 
 // A block of four waves per C slabs of 16 columns of a head's values, from the last chunk to the
@@ -163,17 +162,16 @@ __global__ __launch_bounds__(256) void delta_backward_scan_kernel(Args<T> a) {
                           static_cast<uint64_t>(h) * d.values;
   const T *gradients = a.gradient + value0;
   T *dvalues = a.dvalue + value0;
-  const uint64_t block_bytes = Kept::bytes(KT, d.slabs);
+  const uint64_t block_bytes = Kept::bytes(KT, a.pairs);
   char *chunks = a.heads + head * d.chunks * block_bytes;
   constexpr uint32_t kOperand = 64 * sizeof(Op), kKeys = 4 * KT * kOperand;
   const char *keys =
       a.keys + (static_cast<uint64_t>(b) * d.key_heads + kh) * d.chunks * (3 * kKeys);
   uint32_t cols[C];  // this lane's; those past the last are the last again, with gradients of 0
-  bool in[C], own[C];
+  bool in[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const uint32_t slab = block.x * C + c, column = 16 * slab + n;
-    own[c] = slab < d.slabs;
+    const uint32_t column = 16 * (block.x * C + c) + n;
     in[c] = column < d.values;
     cols[c] = in[c] ? column : d.values - 1;
   }
@@ -200,9 +198,8 @@ __global__ __launch_bounds__(256) void delta_backward_scan_kernel(Args<T> a) {
 
   // Loaded and stored as the forward's.
   typedef T quarter __attribute__((ext_vector_type(4)));
-  Op key[KT], scores[2], solve[2], back[2][2], forth[2][2], before[C];
+  Op key[KT], scores[2], solve[2], back[2][2], forth[2][2];
   T gradient[C][4];
-  quarter error[C];
   f32x4 since, until, write, since_next;
   float whole = 0.0f;
   const uint32_t value_bytes = static_cast<uint32_t>(value_stride * sizeof(T));
@@ -241,21 +238,6 @@ __global__ __launch_bounds__(256) void delta_backward_scan_kernel(Args<T> a) {
     until = load_at<f32x4>(gates + offsetof(Gates, until), at);
     write = load_at<f32x4>(gates + offsetof(Gates, write), at);
   };
-  // the forward's states and errors; a block's slabs past the last read the last one's
-  const uint32_t kept = d.slabs * (KT + 2) * kOperand;
-  auto saved_of = [&](uint32_t chunk) {
-    return a.saved + (head * a.all + d.first + chunk) * kept;
-  };
-  auto saved_at = [&](int c, int place) {
-    return (min(block.x * C + c, d.slabs - 1) * (KT + 2) + place) * kOperand + lane_at;
-  };
-  auto load_errors = [&](uint32_t chunk) {
-    const char *from = saved_of(chunk);
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-      error[c] = load_at<quarter>(
-          from, saved_at(c, KT + pair) + half * static_cast<uint32_t>(sizeof(quarter)));
-  };
   auto load_rest = [&](uint32_t chunk) {
     whole = load_at<float>(operands_of(chunk, Kept::gates) + offsetof(Gates, since),
                            (kChunk - 1) * 4);
@@ -267,9 +249,6 @@ __global__ __launch_bounds__(256) void delta_backward_scan_kernel(Args<T> a) {
         back[i][s] = load_at<Op>(k + (2 * i + s) * kOperand, lane_at);
         forth[i][s] = load_at<Op>(k + kKeys + (2 * i + s) * kOperand, lane_at);
       }
-    const char *from = saved_of(chunk);
-#pragma unroll
-    for (int c = 0; c < C; ++c) before[c] = load_at<Op>(from, saved_at(c, min(w, KT - 1u)));
   };
   auto hand = [&](Op(&to)[64], f32x4 v) {
     reinterpret_cast<quarter *>(&to[lane])[half] = __builtin_convertvector(v, quarter);
@@ -286,21 +265,21 @@ __global__ __launch_bounds__(256) void delta_backward_scan_kernel(Args<T> a) {
       hand(m.decayed[chunk & 1][pair][c], since_next * d.scale * v);
     }
   };
-  // dS of the chunk, for its products and for those of the kernel behind
-  auto slabs_of = [&](uint32_t chunk) {
-    return buffer_of(operands_of(chunk, Kept::slabs), d.slabs * Kept::slab(KT));
+  // what the products read of a chunk; a block of one slab brings its half of the pair's lanes
+  const uint32_t kept = a.pairs * static_cast<uint32_t>(Kept::pair(KT));
+  auto pairs_at = [&](uint32_t chunk) { return buffer_of(operands_of(chunk, Kept::pairs), kept); };
+  const bool brings = C == 2 || (g >> 1) == (block.x & 1);
+  auto pair_at = [&](int place) {
+    return brings ? (block.x * C / 2 * (2 * KT + 4) + place) * kOperand + lane_at : kNowhere;
   };
   auto hand_state = [&](uint32_t chunk) {
     if (KT < 4 && !holds) return;
-    const auto to = slabs_of(chunk);
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const Op v = rounded<T>(join(ds[0][c], ds[1][c]));
-      m.state[w][c][lane] = v;
-      store_to(to, own[c] ? (block.x * C + c) * static_cast<uint32_t>(Kept::slab(KT)) +
-                                w * kOperand + lane_at
-                          : kNowhere, v);
-    }
+    for (int c = 0; c < C; ++c) m.state[w][c][lane] = rounded<T>(join(ds[0][c], ds[1][c]));
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      store_to(pairs_at(chunk), pair_at(2 * w + i),
+               turned(&m.state[w][0][0], C == 2 ? 64 : 0, i, n, g));
   };
   auto read_pairs = [&](Op(&to)[2][C], const Op(&from)[2][C][64]) {
 #pragma unroll
@@ -315,7 +294,6 @@ __global__ __launch_bounds__(256) void delta_backward_scan_kernel(Args<T> a) {
     load_triangle(last, Kept::within, scores);
     load_gates(last);
     load_triangle(last, Kept::system, solve);
-    load_errors(last);
     load_rest(last);
     hand_gradients(last);
     load_gradients(last == 0 ? 0 : last - 1);
@@ -365,12 +343,11 @@ __global__ __launch_bounds__(256) void delta_backward_scan_kernel(Args<T> a) {
         for (int c = 0; c < C; ++c) x[c] = product(solve[s], right[s][c], x[c]);
       }
     }
-    f32x4 sums = {};
     const uint32_t rows = rows_of(chunk);
     const auto to = buffer_of(dvalues + chunk * kChunk * value_stride, kChunk * value_bytes);
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      if (own[c]) sums += __builtin_convertvector(error[c], f32x4) * x[c];
+      hand(m.x[pair][c], x[c]);
       x[c] *= write;
       hand(m.taken[pair][c], -since * x[c]);
 #pragma unroll
@@ -382,16 +359,10 @@ __global__ __launch_bounds__(256) void delta_backward_scan_kernel(Args<T> a) {
                  static_cast<T>(x[c][r]));
       }
     }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) sums[r] = row_total(sums[r]);
-    const auto slabs = slabs_of(chunk);
-    const uint32_t sums_at = block.x * C * static_cast<uint32_t>(Kept::slab(KT)) + KT * kOperand;
-    store_to(slabs, n == 0 ? sums_at + index_of(w, 4 * g) * 4 : kNowhere, sums);
     // the next chunk's gradients of the outputs
     hand_gradients(next);
     __builtin_amdgcn_sched_barrier(0);
     load_triangle(next, Kept::system, solve);
-    load_errors(next);
     load_gates(next);
     load_gradients(after);
     lds_barrier();
@@ -400,18 +371,11 @@ __global__ __launch_bounds__(256) void delta_backward_scan_kernel(Args<T> a) {
     read_pairs(decayed, m.decayed[chunk & 1]);
     read_pairs(taken, m.taken);
     __builtin_amdgcn_sched_barrier(0);
-    float across[1] = {0.0f};
     if (KT == 4 || holds) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-          ds[i][c] *= whole;
-          const f32x8 s0 = widened(before[c]);
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            across[0] = fmaf(ds[i][c][r], own[c] ? s0[4 * i + r] : 0.0f, across[0]);
-        }
+        for (int c = 0; c < C; ++c) ds[i][c] *= whole;
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -425,8 +389,8 @@ __global__ __launch_bounds__(256) void delta_backward_scan_kernel(Args<T> a) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) ds[i][c] = product(back[i][s], taken[s][c], ds[i][c]);
     }
-    oxh::wave_sums_rows(across);
-    store_to(slabs, lane == 0 ? sums_at + (kChunk + w) * 4 : kNowhere, across[0]);
+    store_to(pairs_at(chunk), pair_at(2 * KT + w),
+             turned(&m.x[pair][0][0], C == 2 ? 64 : 0, half, n, g));
     __builtin_amdgcn_sched_barrier(0);
     load_rest(next);
     if (chunk != 0) hand_state(next);
@@ -451,41 +415,54 @@ __global__ __launch_bounds__(256) void delta_backward_scan_kernel(Args<T> a) {
     }
 }
 
-constexpr int kColumns = 32;  // of values that the products take at a time
+constexpr int kColumns = 32;  // of values that the products take at a time: a pair of slabs
 
 template <typename T, int KT>
 struct Products {
+  // of a pair of slabs the forward's state and errors, the state's gradient and x, as they were
+  // stored: tiles of 16 keys, then of 16 steps
+  struct Pair {
+    operand<T> kept[2 * KT + 4][64], back[2 * KT + 4][64];
+  };
   union {
-    struct {
-      alignas(32) T state[32 * KT][kColumns + 8], gradient[32 * KT][kColumns + 8];
-      alignas(32) T wrote[kChunk][kColumns + 8];
-    };
+    Pair pairs[2];
     alignas(16) float rows[kChunk][32 * KT + 4];
   };
+  // past a row's 64 columns: what is not to be written
   alignas(32) T one[kChunk][kChunk + 8], one_t[kChunk][kChunk + 8], two[kChunk][kChunk + 8];
   double sums[kChunk];
-  float rows_at[kChunk], columns_at[4][kChunk], before[kChunk];
+  float rows_at[kChunk], columns_at[4][kChunk], before[kChunk], errors[kChunk], across[4];
 };
 
-// A block per chunk and key head, its value heads in turn; a wave 16 of the steps.
-template <typename T, int KT, bool Whole, bool WholeValues>
-__global__ __launch_bounds__(256) void delta_backward_products_kernel(Args<T> a) {
+// A block per chunk and key head, its value heads in turn (Shared: more than one, whose sums take 64
+// registers more); a wave 16 of the steps.  Rows and columns
+// are numbered by index_of, so that a wave's values of keys and queries beside its results are those
+// of the operands that it multiplies them with.
+template <typename T, int KT, bool Whole, bool WholeValues, bool Shared>
+__global__ __launch_bounds__(256, sizeof(T) == 2 && !Shared ? 2 : 1) void delta_backward_products_kernel(
+    Args<T> a) {
   using Op = operand<T>;
+  using Pair = typename Products<T, KT>::Pair;
   __shared__ Products<T, KT> m;
   const Dims &d = a.d;
-  const uint32_t chunk = blockIdx.x, kh = blockIdx.y, b = blockIdx.z;
+  const oxh::BlockTile tile = oxh::xcd_block();
+  const uint32_t chunk = tile.x, kh = tile.y, b = tile.z;
   const uint32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int pair = w >> 1;
   const uint32_t row = threadIdx.x >> 2, part = threadIdx.x & 3;  // of the results' rows
   const uint64_t stride = static_cast<uint64_t>(d.key_heads) * d.keys;
   const uint64_t value_stride = static_cast<uint64_t>(d.heads) * d.values;
-  f32x8 dq[KT] = {}, dk[KT] = {};
+  constexpr uint32_t kOperand = 64 * sizeof(Op);
+  const uint32_t lane_at = lane * sizeof(Op);
+  f32x8 sums_q[Shared ? KT : 1] = {}, sums_k[Shared ? KT : 1] = {};
   const Place first(d, chunk, kh * d.group, b);
   const uint32_t held = min(d.time - first.begin, static_cast<uint32_t>(kChunk)), rows = first.rows;
-  const Op *keys =
-      reinterpret_cast<const Op *>(a.keys) + (first.key_chunk(d) * 12 + 4) * (KT * 64) + lane;
-  const Op *queries = keys + 4 * KT * 64;
-  for (uint32_t h = kh * d.group; h < (kh + 1) * d.group; ++h) {
+  const char *keys = a.keys + first.key_chunk(d) * (12 * KT * kOperand);
+  const uint32_t t_row = index_of(w, n), t_read = rows == 0 ? 0 : min(t_row, rows - 1);
+  const uint64_t to_keys = first.key_row * d.keys + row * stride;
+  for (uint32_t turn = 0; turn < (Shared ? d.group : 1); ++turn) {
+    const uint32_t h = kh * d.group + turn;
     const Place at(d, chunk, h, b);
     if (rows == 0) {
       if (threadIdx.x < held) {
@@ -494,71 +471,29 @@ __global__ __launch_bounds__(256) void delta_backward_products_kernel(Args<T> a)
       }
       continue;
     }
-    const char *block = a.heads + at.head_chunk(d) * Back<T>::bytes(KT, d.slabs);
-    const Gates *gates = reinterpret_cast<const Gates *>(block + Back<T>::gates);
-    const uint64_t value_at = at.value_row * d.values;
-    const uint64_t head = static_cast<uint64_t>(b) * d.heads + h;
+    const char *block = a.heads + at.head_chunk(d) * Back<T>::bytes(KT, a.pairs);
+    const char *gates = block + Back<T>::gates;
+    const uint64_t value_at = at.value_row * d.values + t_read * value_stride;
+    const char *saved = a.saved + ((static_cast<uint64_t>(b) * d.heads + h) * a.all + d.first + chunk) *
+                                      a.pairs * Back<T>::pair(KT);
     f32x4 one[4] = {}, two[4] = {}, q1[2 * KT] = {}, k1[2 * KT] = {}, k2[2 * KT] = {};
-    const uint32_t t_row = 16 * wave + n;  // this lane's row of the operands from the left
-    for (uint32_t v0 = 0; v0 < d.values; v0 += kColumns) {
-      __syncthreads();  // the columns before, or the rows of the head before
-      // two slabs of states, their gradients and errors; those past the last are 0
-      for (uint32_t i = wave; i < 2 * KT + 4; i += 4) {
-        const uint32_t s = i < 2 * KT ? i % KT : i & 1;
-        const uint32_t half = i < 2 * KT ? i / KT : (i - 2 * KT) >> 1, slab = v0 / 16 + half;
-        const bool there = slab < d.slabs;
-        const Op *kept = reinterpret_cast<const Op *>(a.saved) + lane +
-                         ((head * a.all + d.first + chunk) * d.slabs + slab) * ((KT + 2) * 64);
-        const uint32_t c = 16 * half + n;
-        if (i < 2 * KT) {
-          Op state = {}, gradient = {};
-          if (there) {
-            state = kept[s * 64];
-            gradient = reinterpret_cast<const Op *>(block + Back<T>::slabs +
-                                                    slab * Back<T>::slab(KT))[s * 64 + lane];
-          }
+    float across = 0.0f, errors = 0.0f;  // <dS, S0>, and of this lane's row e x
+    Op out_next;
+    auto fetch = [&](uint32_t i, Pair &to) {
+      const char *kept = saved + i * Back<T>::pair(KT);
+      const char *back = block + Back<T>::pairs + i * Back<T>::pair(KT);
+      constexpr int kPieces = Back<T>::pair(KT) / 1024;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            m.state[32 * s + 8 * g + j][c] = state[j];
-            m.gradient[32 * s + 8 * g + j][c] = gradient[j];
-          }
-        } else {
-          f32x8 e = {};
-          if (there) e = widened(kept[(KT + s) * 64]);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const uint32_t t = 32 * s + 8 * g + j;
-            m.wrote[t][c] = static_cast<T>(e[j] * gates->write[t]);
-          }
-        }
+      for (int q = 0; q < (kPieces + 3) / 4; ++q) {
+        const uint32_t p = 4 * q + w;
+        if (kPieces % 4 != 0 && p >= kPieces) continue;
+        copy_16(kept + p * 1024 + 16 * lane, reinterpret_cast<char *>(&to.kept[0][0]) + p * 1024);
+        copy_16(back + p * 1024 + 16 * lane, reinterpret_cast<char *>(&to.back[0][0]) + p * 1024);
       }
-      Op out = {}, dv = {};
-      if (t_row < rows) {
-        const uint64_t from = value_at + t_row * value_stride;
-        if (WholeValues || v0 + 8 * g < d.values) {
-          out = load_row<T, WholeValues>(a.gradient + from, v0 + 8 * g, d.values);
-          dv = load_row<T, WholeValues>(a.dvalue + from, v0 + 8 * g, d.values);
-        }
-      }
-      __syncthreads();
-      auto wrote = [&](uint32_t r) { return *reinterpret_cast<const Op *>(&m.wrote[r][8 * g]); };
-#pragma unroll
-      for (uint32_t i = 0; i < 4; ++i) {
-        if (i > wave) continue;
-        const Op u = wrote(16 * i + n);
-        one[i] = product(out, u, one[i]);
-        two[i] = product(dv, u, two[i]);
-      }
-      const Op own = wrote(t_row);
-#pragma unroll
-      for (int i = 0; i < 2 * KT; ++i) {
-        const uint32_t k = index_of(i, n);
-        const Op state = *reinterpret_cast<const Op *>(&m.state[k][8 * g]);
-        q1[i] = product(out, state, q1[i]);
-        k1[i] = product(dv, state, k1[i]);
-        k2[i] = product(own, *reinterpret_cast<const Op *>(&m.gradient[k][8 * g]), k2[i]);
-      }
-    }
+      out_next = load_row<T, WholeValues>(a.gradient + value_at, kColumns * i + 8 * g, d.values);
+    };
+    lds_barrier();  // the rows of the head before are read
+    fetch(0, m.pairs[0]);
     if (threadIdx.x < kChunk) {
       // the sums of the decay again, as the first kernel formed them
       const uint64_t from = at.value_row + static_cast<uint64_t>(min(lane, rows - 1)) * d.heads;
@@ -570,154 +505,209 @@ __global__ __launch_bounds__(256) void delta_backward_products_kernel(Args<T> a)
       }
       m.sums[lane] = sum;
     }
-    const T *query = a.query + at.key_row * d.keys, *key = a.key + at.key_row * d.keys;
-    auto operand_at = [&](const T *p, uint32_t r, int step) {
-      return load_row<T, Whole>(p + min(r, rows - 1) * stride, 32 * step + 8 * g, d.keys);
-    };
-    // q k' and k k' again, for what their pairs' decays are worth
-    f32x4 qk[4] = {}, kk[4] = {};
+    for (uint32_t i = 0; i < a.pairs; ++i) {
+      arrived();
+      const Op out = t_row < rows ? out_next : Op{};
+      if (i + 1 < a.pairs) fetch(i + 1, m.pairs[(i + 1) & 1]);
+      const Pair &s = m.pairs[i & 1];
+      const Op e = s.kept[2 * KT + w][lane], x = s.back[2 * KT + w][lane];
+      Op others[4];
 #pragma unroll
-    for (int s = 0; s < KT; ++s) {
-      const Op q = operand_at(query, t_row, s), k = operand_at(key, t_row, s);
+      for (int it = 0; it < 4; ++it) others[it] = s.kept[2 * KT + it][lane];
 #pragma unroll
-      for (uint32_t i = 0; i < 4; ++i) {
-        if (i > wave) continue;
-        const Op other = operand_at(key, 16 * i + n, s);
-        qk[i] = product(q, other, qk[i]);
-        kk[i] = product(k, other, kk[i]);
+      for (int j = 0; j < 8; ++j) errors = fmaf(widen(e[j]), widen(x[j]), errors);
+#pragma unroll
+      for (int it = 0; it < 4; ++it) {
+        if ((it >> 1) > pair) continue;
+        one[it] = product(out, others[it], one[it]);
+        two[it] = product(x, others[it], two[it]);
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        Op state[KT], gradient[KT];
+#pragma unroll
+        for (int k = 0; k < KT; ++k) {
+          state[k] = s.kept[half * KT + k][lane];
+          gradient[k] = s.back[half * KT + k][lane];
+        }
+#pragma unroll
+        for (int k = 0; k < KT; ++k) {
+          const int to = half * KT + k;
+          q1[to] = product(out, state[k], q1[to]);
+          k1[to] = product(x, state[k], k1[to]);
+          k2[to] = product(e, gradient[k], k2[to]);
+        }
+        // a quarter of the tiles each wave
+#pragma unroll
+        for (int k = 0; k < KT; ++k)
+          if (static_cast<uint32_t>(half * KT + k) % 4 == w)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) across = fmaf(widen(state[k][j]), widen(gradient[k][j]), across);
       }
     }
-    __syncthreads();
-    float across[4] = {};  // H's rows
+    // q k' and k k' again, for what their pairs' decays are worth
+    f32x4 qk[4] = {}, kk[4] = {};
+    {
+      const T *query = a.query + at.key_row * d.keys + t_read * stride;
+      Op q[KT], others[KT][4];
 #pragma unroll
-    for (uint32_t it = 0; it < 4; ++it) {
-      const uint32_t i = 16 * it + n;
+      for (int s = 0; s < KT; ++s) {
+        q[s] = load_row<T, Whole>(query, 32 * s + 8 * g, d.keys);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) others[s][i] = load_at<Op>(keys + (i * KT + s) * kOperand, lane_at);
+      }
+      if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int s = 0; s < KT; ++s) {
+        const Op k = w == 0 ? others[s][0] : w == 1 ? others[s][1] : w == 2 ? others[s][2] : others[s][3];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if ((i >> 1) > pair) continue;
+          qk[i] = product(q[s], others[s][i], qk[i]);
+          kk[i] = product(k, others[s][i], kk[i]);
+        }
+      }
+    }
+    const uint32_t t0 = index_of(w, 4 * g);  // this lane's first row of the results
+    const f32x4 since = load_at<f32x4>(gates + offsetof(Gates, since), t0 * 4);
+    const f32x4 until = load_at<f32x4>(gates + offsetof(Gates, until), t0 * 4);
+    const f32x4 write = load_at<f32x4>(gates + offsetof(Gates, write), t0 * 4);
+    float beta[4];
+#pragma unroll
+    for (int it = 0; it < 4; ++it)
+      beta[it] = load_at<float>(gates + offsetof(Gates, write), index_of(it, n) * 4);
+    errors += __shfl_xor(errors, 16);
+    errors += __shfl_xor(errors, 32);
+    if (g == 0) m.errors[t_row] = errors;
+    {
+      float total[1] = {across};
+      oxh::wave_sums_rows(total);
+      if (lane == 0) m.across[w] = total[0];
+    }
+    f32x4 after = {}, before = {};  // H's rows first
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+      const uint32_t i = index_of(it, n);
       float down = 0.0f;  // and columns
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const uint32_t t = 16 * wave + 4 * g + r;
-        const float between = i <= t ? expf(static_cast<float>(m.sums[t] - m.sums[i])) : 0.0f;
+        const uint32_t t = t0 + r;
+        // no decay between a step and a later one is asked for
+        const float between = beta[it] * expf(static_cast<float>(i <= t ? m.sums[t] - m.sums[i] : 0.0));
         const float x = i <= t ? one[it][r] * between * d.scale : 0.0f;
+        const float y = i < t ? -two[it][r] * write[r] * between : 0.0f;
+        const float worth = (i < t ? x * qk[it][r] : 0.0f) + y * kk[it][r];
         m.one[t][i] = static_cast<T>(x);
         m.one_t[i][t] = static_cast<T>(x);
-        if (i < t) {
-          const float y = -two[it][r] * between, pair = x * qk[it][r] + y * kk[it][r];
-          m.two[t][i] = static_cast<T>(y);
-          m.two[i][t] = static_cast<T>(y);
-          across[r] += pair;
-          down += pair;
-        } else if (i == t) {
-          m.two[t][t] = static_cast<T>(0.0f);
-        }
+        // the pairs the other way round are another lane's
+        m.two[t][i <= t ? i : kChunk] = static_cast<T>(y);
+        m.two[i][i <= t ? t : kChunk] = static_cast<T>(y);
+        after[r] += worth;
+        down += worth;
       }
       down += __shfl_xor(down, 16);
       down += __shfl_xor(down, 32);
-      if (g == 0) m.columns_at[wave][i] = down;
+      if (g == 0) m.columns_at[w][i] = down;
     }
-    const f32x4 since = *reinterpret_cast<const f32x4 *>(gates->since + 16 * wave + 4 * g);
-    const f32x4 until = *reinterpret_cast<const f32x4 *>(gates->until + 16 * wave + 4 * g);
+    lds_barrier();
+    // the rows of this wave of both matrices and of the first one's transpose
+    Op x[2], xt[2], y[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      x[s] = *reinterpret_cast<const Op *>(&m.one[t_row][32 * s + 8 * g]);
+      xt[s] = *reinterpret_cast<const Op *>(&m.one_t[t_row][32 * s + 8 * g]);
+      y[s] = *reinterpret_cast<const Op *>(&m.two[t_row][32 * s + 8 * g]);
+    }
 #pragma unroll
     for (int i = 0; i < 2 * KT; ++i) {
       q1[i] *= since * d.scale;
-      k1[i] *= -since;
-      k2[i] *= until;
+      k1[i] *= -since * write;
+      k2[i] *= until * write;
+      Op k[2], q[2];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        k[s] = load_at<Op>(keys + (4 * KT + 2 * i + s) * kOperand, lane_at);
+        q[s] = load_at<Op>(keys + (8 * KT + 2 * i + s) * kOperand, lane_at);
+      }
+      // of the wave's own steps: a lane's four are half of its 8
+      const Op own = pair == 0 ? k[0] : k[1], asked = pair == 0 ? q[0] : q[1];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float kr = widen(w & 1 ? own[4 + r] : own[r]), qr = widen(w & 1 ? asked[4 + r] : asked[r]);
+        after[r] = fmaf(qr, q1[i][r], fmaf(kr, k1[i][r], after[r]));
+        before[r] = fmaf(kr, k2[i][r], before[r]);
+      }
+      k1[i] += k2[i];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        q1[i] = product(x[s], k[s], q1[i]);
+        k1[i] = product(y[s], k[s], k1[i]);
+        k1[i] = product(xt[s], q[s], k1[i]);
+      }
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const uint32_t t = 16 * wave + 4 * g + r;
-      const uint64_t from = min(t, rows - 1) * stride;
-      float after = across[r], before = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 2 * KT; ++i) {
-        const uint32_t k = index_of(i, n);
-        if (!Whole && k >= d.keys) continue;
-        const float own = widen(key[from + k]);
-        after = fmaf(widen(query[from + k]), q1[i][r], fmaf(own, k1[i][r], after));
-        before = fmaf(own, k2[i][r], before);
-      }
-      after = row_total(after);
-      before = row_total(before);
-      if (n == 0) {
-        m.rows_at[t] = after;
-        m.before[t] = before;
-      }
+      after[r] = row_total(after[r]);
+      before[r] = row_total(before[r]);
     }
-#pragma unroll
-    for (int i = 0; i < 2 * KT; ++i) k1[i] += k2[i];
-    __syncthreads();
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const Op x = *reinterpret_cast<const Op *>(&m.one[t_row][32 * s + 8 * g]);
-      const Op xt = *reinterpret_cast<const Op *>(&m.one_t[t_row][32 * s + 8 * g]);
-      const Op y = *reinterpret_cast<const Op *>(&m.two[t_row][32 * s + 8 * g]);
-#pragma unroll
-      for (int i = 0; i < 2 * KT; ++i) {
-        const Op k = keys[(2 * i + s) * 64];
-        q1[i] = product(x, k, q1[i]);
-        k1[i] = product(y, k, k1[i]);
-        k1[i] = product(xt, queries[(2 * i + s) * 64], k1[i]);
-      }
+    if (n == 0) {
+      *reinterpret_cast<f32x4 *>(&m.rows_at[t0]) = after;
+      *reinterpret_cast<f32x4 *>(&m.before[t0]) = before;
     }
-    // the rows whole: each thread 8 keys at a time of its row
-    auto rows_of = [&](const f32x4 (&v)[2 * KT]) {
-      __syncthreads();
+    // the rows whole: each thread 8 keys at a time of its row, stored with the last head's
+    auto rows_of = [&](const f32x4(&v)[2 * KT], f32x8(&sums)[Shared ? KT : 1], T *to) {
+      lds_barrier();
 #pragma unroll
       for (int i = 0; i < 2 * KT; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) m.rows[16 * wave + 4 * g + r][index_of(i, n)] = v[i][r];
-      __syncthreads();
-    };
-    auto piece = [&](int i) {
-      const float *p = &m.rows[row][(part + 4 * i) * 8];
-      return join(*reinterpret_cast<const f32x4 *>(p), *reinterpret_cast<const f32x4 *>(p + 4));
-    };
-    rows_of(q1);
+        for (int r = 0; r < 4; ++r) m.rows[t0 + r][index_of(i, n)] = v[i][r];
+      lds_barrier();
 #pragma unroll
-    for (int i = 0; i < KT; ++i) dq[i] += piece(i);
-    rows_of(k1);
-#pragma unroll
-    for (int i = 0; i < KT; ++i) dk[i] += piece(i);
-    if (threadIdx.x < kChunk) {
-      float error = 0.0f, constant = 0.0f;
-      for (uint32_t slab = 0; slab < d.slabs; slab += a.together) {
-        const float *sums = reinterpret_cast<const float *>(
-            block + Back<T>::slabs + slab * Back<T>::slab(KT) + KT * Back<T>::operand_bytes);
-        error += sums[lane];
-        constant += (sums[kChunk] + sums[kChunk + 1]) + (sums[kChunk + 2] + sums[kChunk + 3]);
+      for (int i = 0; i < KT; ++i) {
+        const uint32_t k = (part + 4 * i) * 8;
+        const float *p = &m.rows[row][k];
+        f32x8 own = join(*reinterpret_cast<const f32x4 *>(p), *reinterpret_cast<const f32x4 *>(p + 4));
+        if constexpr (Shared) {
+          sums[i] += own;
+          if (turn + 1 < d.group) continue;
+          own = sums[i];
+        }
+        if (row < held)
+          store_row<T, Whole>(to + to_keys, k, d.keys, rounded<T>(row < rows ? own : f32x8{}));
       }
-      float after = m.rows_at[lane], before = m.before[lane];
+    };
+    rows_of(q1, sums_q, a.dquery);
+    rows_of(k1, sums_k, a.dkey);
+    if (threadIdx.x < kChunk) {
+      float later = m.rows_at[lane], earlier = m.before[lane];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) after -= m.columns_at[i][lane];
-      const float own = before;
+      for (int i = 0; i < 4; ++i) later -= m.columns_at[i][lane];
+      const float own = earlier;
 #pragma unroll
       for (int i = 1; i < 64; i *= 2) {
-        const float x = __shfl_down(after, i), y = __shfl_up(before, i);
-        if (lane + i < 64) after += x;
-        if (lane >= static_cast<uint32_t>(i)) before += y;
+        const float x = __shfl_down(later, i), y = __shfl_up(earlier, i);
+        if (lane + i < 64) later += x;
+        if (lane >= static_cast<uint32_t>(i)) earlier += y;
       }
       if (lane < held) {
         const uint64_t to = at.value_row + static_cast<uint64_t>(lane) * d.heads;
         const bool live = lane < rows;
-        const float beta = gates->write[lane], decay = after + (before - own) + constant;
+        const float beta = load_at<float>(gates + offsetof(Gates, write), lane * 4);
+        const float whole = load_at<float>(gates + offsetof(Gates, since), (kChunk - 1) * 4);
+        const float constant =
+            whole * ((m.across[0] + m.across[1]) + (m.across[2] + m.across[3]));
+        const float decay = later + (earlier - own) + constant;
         a.dgate[to] = static_cast<T>(live ? decay * sigmoid(-widen(a.gate[to])) : 0.0f);
         a.dwrite[to] =
-            static_cast<T>(live ? error * beta * sigmoid(-widen(a.write[to])) : 0.0f);
+            static_cast<T>(live ? m.errors[lane] * beta * sigmoid(-widen(a.write[to])) : 0.0f);
       }
     }
   }
-  if (row >= held) return;
-  const bool live = row < rows;
-  const uint64_t to = first.key_row * d.keys + row * stride;
+  if (rows != 0 || row >= held) return;
 #pragma unroll
   for (int i = 0; i < KT; ++i) {
-    const uint32_t k = (part + 4 * i) * 8;
-    const operand<T> x = rounded<T>(dq[i]), y = rounded<T>(dk[i]);
-#pragma unroll
-    for (uint32_t j = 0; j < 8; ++j) {
-      if (!Whole && k + j >= d.keys) continue;
-      a.dquery[to + k + j] = live ? x[j] : static_cast<T>(0.0f);
-      a.dkey[to + k + j] = live ? y[j] : static_cast<T>(0.0f);
-    }
+    store_row<T, Whole>(a.dquery + to_keys, (part + 4 * i) * 8, d.keys, Op{});
+    store_row<T, Whole>(a.dkey + to_keys, (part + 4 * i) * 8, d.keys, Op{});
   }
 }
 
@@ -728,7 +718,7 @@ struct BackPlan {
   uint64_t bytes() const { return head_bytes + key_bytes + state_bytes; }
   explicit BackPlan(const oxh_delta_shape &s, float scale, const int32_t *lengths)
       : p(s, scale, lengths) {
-    const uint64_t head = s.batch * s.heads * Back<T>::bytes(p.steps, p.d.slabs);
+    const uint64_t head = s.batch * s.heads * Back<T>::bytes(p.steps, pairs_of(s.value_dim));
     const uint64_t key = s.batch * s.key_heads * p.steps * 12 * kOperandBytes<T>;
     p.divide(head + key);
     head_bytes = round_up(p.segment * head, 256);
@@ -746,8 +736,8 @@ oxh_status backward(hipStream_t stream, const BackPlan<T> &plan, Args<T> a, cons
   const Plan &p = plan.p;
   a.all = static_cast<uint32_t>(p.all);
   const uint64_t launches = (p.all + p.segment - 1) / p.segment;
-  auto blocks = [&](uint32_t slabs) { return (p.d.slabs + slabs - 1) / slabs; };
-  a.together = static_cast<uint64_t>(p.d.batch) * p.d.heads * blocks(2) >= oxh::kComputeUnits ? 2 : 1;
+  a.pairs = (p.d.slabs + 1) / 2;
+  const bool two = static_cast<uint64_t>(p.d.batch) * p.d.heads * a.pairs >= oxh::kComputeUnits;
   for (uint64_t i = launches; i-- != 0;) {
     const uint64_t first = i * p.segment;
     a.d = p.d;
@@ -761,16 +751,24 @@ oxh_status backward(hipStream_t stream, const BackPlan<T> &plan, Args<T> a, cons
       constexpr bool W = decltype(whole)::value;
       oxh::launch(delta_backward_prepare_kernel<T, KT, W>, dim3(d.chunks, d.heads, d.batch),
                   dim3(256), 0, stream, a);
-      const dim3 scan(blocks(a.together), d.heads, d.batch);
-      if (a.together == 2)
-        oxh::launch(delta_backward_scan_kernel<T, KT, 2>, scan, dim3(256), 0, stream, a);
+      if (two)
+        oxh::launch(delta_backward_scan_kernel<T, KT, 2>, dim3(a.pairs, d.heads, d.batch), dim3(256),
+                    0, stream, a);
       else
-        oxh::launch(delta_backward_scan_kernel<T, KT, 1>, scan, dim3(256), 0, stream, a);
+        oxh::launch(delta_backward_scan_kernel<T, KT, 1>, dim3(2 * a.pairs, d.heads, d.batch),
+                    dim3(256), 0, stream, a);
       const dim3 grid(d.chunks, d.key_heads, d.batch);
-      if (d.values % kColumns == 0)
-        oxh::launch(delta_backward_products_kernel<T, KT, W, true>, grid, dim3(256), 0, stream, a);
-      else
-        oxh::launch(delta_backward_products_kernel<T, KT, W, false>, grid, dim3(256), 0, stream, a);
+      auto products = [&](auto values, auto shared) {
+        oxh::launch(delta_backward_products_kernel<T, KT, W, decltype(values)::value,
+                                                   decltype(shared)::value>,
+                    grid, dim3(256), 0, stream, a);
+      };
+      auto by_group = [&](auto values) {
+        if (d.group > 1) products(values, std::true_type());
+        else products(values, std::false_type());
+      };
+      if (d.values % kColumns == 0) by_group(std::true_type());
+      else by_group(std::false_type());
     });
     oxh_status st = oxh::launched("gated_delta_rule_backward");
     if (st != OXH_OK) return st;
