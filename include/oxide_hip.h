@@ -486,11 +486,12 @@ oxh_status oxh_layer_norm_backward(oxh_stream stream, int dtype, uint64_t rows, 
  * state in place.  lengths (device int32 [batch], may be NULL; clamped to 0..time): a row's steps
  * at or past its length give 0 and leave the state, whatever the operands hold there.
  * Keys of length 1 (or less) keep the state bounded.  A value of a row's own steps that is not
- * finite may reach the outputs of its whole chunk of 64 steps.  bfloat16 operands: the state's own
- * products keep 16 bits of what is formed on the way, the output's 8.
+ * finite may reach the outputs of its whole chunk of 64 steps.  bfloat16 operands: products keep 8
+ * bits of what is formed on the way, with a final_state 16 of what the state is made of.
  * `saved` (may be NULL) receives what the backward reads; a call without it takes up to 16 steps
- * one by one, in float32.  OXH_INVALID_SHAPE above a key_dim of 128, a value_dim of 4096 or a
- * batch of 65535, or where one launch cannot number the threads. */
+ * one by one, in float32.  OXH_INVALID_SHAPE above a key_dim of 128, a value_dim of 4096, a
+ * batch or heads of 65535 or heads * value_dim of 2^24 - 1, or where one launch cannot number the
+ * threads. */
 typedef struct oxh_delta_shape {
   uint64_t batch, time, key_heads, heads, key_dim, value_dim;
 } oxh_delta_shape;
@@ -993,6 +994,22 @@ oxh_status oxh_net_cross_entropy(oxh_net *net, uint32_t logits, uint32_t targets
 oxh_status oxh_net_rms_norm(oxh_net *net, uint32_t x, uint32_t weight, float epsilon,
                             uint32_t *node);
 oxh_status oxh_net_gated_recurrence(oxh_net *net, uint32_t x, uint32_t gate, uint32_t *node);
+/* Layer norm over the last dimension (weight and bias [last dimension]), which joins an add's launch
+ * as the RMS norm does; the gated delta rule over query and key [batch, time, key_heads, key_dim],
+ * value [batch, time, heads, value_dim], gate and write [batch, time, heads] from a zero state; the
+ * clipped policy loss of [batch, classes] logits with its other operands [batch] (mean over the
+ * rows without weights), which take no gradient.  reference_log_probs (needed for a positive kl)
+ * and weights may be OXH_NO_NODE.  OXH_EXECUTION for an epsilon, scale, clip or kl that is not
+ * finite or out of its range. */
+#define OXH_NO_NODE 0xffffffffu
+oxh_status oxh_net_layer_norm(oxh_net *net, uint32_t x, uint32_t weight, uint32_t bias,
+                              float epsilon, uint32_t *node);
+oxh_status oxh_net_gated_delta_rule(oxh_net *net, uint32_t query, uint32_t key, uint32_t value,
+                                    uint32_t gate, uint32_t write, float scale, uint32_t *node);
+oxh_status oxh_net_policy_loss(oxh_net *net, uint32_t logits, uint32_t actions,
+                               uint32_t old_log_probs, uint32_t advantages,
+                               uint32_t reference_log_probs, uint32_t weights, float clip_low,
+                               float clip_high, float kl, uint32_t *node);
 oxh_status oxh_net_forward_program(const oxh_net *net, uint32_t output, oxh_program **program);
 /* adamw NULL: forward + backward only (the gradients stay in the program's buffers). */
 oxh_status oxh_net_training_program(const oxh_net *net, uint32_t root,

@@ -5,8 +5,8 @@
 // order, which is a topological order: leaves (inputs fed per run, trainable parameters,
 // constants; caller-owned device values) and Conv2d / BatchNorm2d / ReLU / Add / Mul /
 // AvgPool2d / Reshape / CrossEntropy nodes with the builders' shape rules
-// (tensor/mod.rs:103-389), and the RmsNorm / Recurrence nodes of sequence models, which the
-// reference has not.  A program is a fixed list of launch groups over buffers carved
+// (tensor/mod.rs:103-389), and the RmsNorm / Recurrence / LayerNorm / DeltaRule nodes of sequence
+// models and the PolicyLoss of training by reward, which the reference has not.  A program is a fixed list of launch groups over buffers carved
 // from one device allocation:
 //   * forward program: the eager device evaluation of a node (runtime.rs:125-379), used for
 //     inference and for JIT plans the fused-plan compiler cannot take (jit.rs:205-207,226-243);
@@ -55,8 +55,12 @@ struct Arena {
 // ---------------------------------------------------------------- graph
 
 enum class Op {
-  Input, Param, Constant, Conv, Bn, Relu, Add, Mul, Pool, Reshape, CrossEntropy, RmsNorm, Recurrence
+  Input, Param, Constant, Conv, Bn, Relu, Add, Mul, Pool, Reshape, CrossEntropy, RmsNorm,
+  Recurrence, LayerNorm, DeltaRule, PolicyLoss
 };
+inline bool is_norm(Op op) { return op == Op::RmsNorm || op == Op::LayerNorm; }
+// Losses of rows of logits, whose gradient one pass forms with the value.
+inline bool is_loss(Op op) { return op == Op::CrossEntropy || op == Op::PolicyLoss; }
 
 struct Node {
   Node(Op o, std::vector<int> i) : op(o), in(std::move(i)) {}
@@ -71,6 +75,9 @@ struct Node {
   float *running_mean = nullptr, *running_variance = nullptr;          // Bn (device, in place)
   bool training = true;
   float momentum = 0.1f, epsilon = 1e-5f;
+  float scale = 1.0f;                                                  // DeltaRule
+  float clip_low = 0.0f, clip_high = 0.0f, kl = 0.0f;                  // PolicyLoss
+  bool reference = false, weights = false;                             // its optional operands
   uint64_t numel() const {
     uint64_t n = 1;
     for (uint32_t i = 0; i < rank; ++i) n *= shape[i];
@@ -106,6 +113,14 @@ oxh_status cross_entropy(Graph &g, int logits, int targets, int *node);
 // Root-mean-square norm over the last dimension; the gated recurrence over [batch, time, channels].
 oxh_status rms_norm(Graph &g, int x, int weight, float epsilon, int *node);
 oxh_status gated_recurrence(Graph &g, int x, int gate, int *node);
+oxh_status layer_norm(Graph &g, int x, int weight, int bias, float epsilon, int *node);
+oxh_status gated_delta_rule(Graph &g, int query, int key, int value, int gate, int write,
+                            float scale, int *node);
+// reference_log_probs and weights may be kNoNode.
+constexpr int kNoNode = -2;
+oxh_status policy_loss(Graph &g, int logits, int actions, int old_log_probs, int advantages,
+                       int reference_log_probs, int weights, float clip_low, float clip_high,
+                       float kl, int *node);
 
 struct AdamConfig {
   float learning_rate = 1e-3f, weight_decay = 0.01f, beta1 = 0.9f, beta2 = 0.999f,

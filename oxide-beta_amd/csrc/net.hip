@@ -277,6 +277,89 @@ oxh_status gated_recurrence(Graph &g, int x, int gate, int *node) {
   return oxh::ok();
 }
 
+oxh_status layer_norm(Graph &g, int x, int weight, int bias, float epsilon, int *node) {
+  oxh_status st = node_index(g, x, "layer_norm");
+  if (st == OXH_OK) st = node_index(g, weight, "layer_norm");
+  if (st == OXH_OK) st = node_index(g, bias, "layer_norm");
+  if (st != OXH_OK) return st;
+  const Node &in = g.nodes[x], &w = g.nodes[weight], &b = g.nodes[bias];
+  OXH_REQUIRE(w.rank == 1 && w.shape[0] == in.shape[in.rank - 1] && w.shape[0] != 0 &&
+                  same_shape(w, b),
+              OXH_INVALID_SHAPE, "layer_norm weight and bias must match the last dimension");
+  OXH_REQUIRE(std::isfinite(epsilon) && epsilon >= 0.0f, OXH_EXECUTION,
+              "layer_norm epsilon must be non-negative and finite");
+  Node n{Op::LayerNorm, {x, weight, bias}};
+  n.rank = in.rank;
+  n.shape = in.shape;
+  n.epsilon = epsilon;
+  *node = g.add(n);
+  return oxh::ok();
+}
+
+oxh_status gated_delta_rule(Graph &g, int query, int key, int value, int gate, int write,
+                            float scale, int *node) {
+  oxh_status st = oxh::ok();
+  for (int i : {query, key, value, gate, write})
+    if (st == OXH_OK) st = node_index(g, i, "gated_delta_rule");
+  if (st != OXH_OK) return st;
+  const Node &k = g.nodes[key], &v = g.nodes[value], &a = g.nodes[gate];
+  OXH_REQUIRE(k.rank == 4 && same_shape(k, g.nodes[query]) && v.rank == 4 &&
+                  v.shape[0] == k.shape[0] && v.shape[1] == k.shape[1],
+              OXH_INVALID_SHAPE,
+              "gated_delta_rule expects query and key [batch, time, key heads, key size] and value "
+              "[batch, time, heads, value size]");
+  OXH_REQUIRE(a.rank == 3 && a.shape[0] == v.shape[0] && a.shape[1] == v.shape[1] &&
+                  a.shape[2] == v.shape[2] && same_shape(a, g.nodes[write]),
+              OXH_INVALID_SHAPE, "gated_delta_rule expects gate and write [batch, time, heads]");
+  OXH_REQUIRE(std::isfinite(scale), OXH_EXECUTION, "gated_delta_rule scale must be finite");
+  Node n{Op::DeltaRule, {query, key, value, gate, write}};
+  n.rank = v.rank;
+  n.shape = v.shape;
+  n.scale = scale;
+  const oxh_delta_shape d{v.shape[0], v.shape[1], k.shape[2], v.shape[2], k.shape[3], v.shape[3]};
+  uint64_t bytes = 0;
+  st = oxh_gated_delta_rule_saved_size(OXH_F32, &d, &bytes);  // the launches' own limits
+  if (st != OXH_OK) return st;
+  *node = g.add(n);
+  return oxh::ok();
+}
+
+oxh_status policy_loss(Graph &g, int logits, int actions, int old_log_probs, int advantages,
+                       int reference_log_probs, int weights, float clip_low, float clip_high,
+                       float kl, int *node) {
+  oxh_status st = node_index(g, logits, "policy_loss");
+  if (st != OXH_OK) return st;
+  Node n{Op::PolicyLoss, {logits}};
+  const Node &l = g.nodes[logits];
+  OXH_REQUIRE(l.rank == 2, OXH_INVALID_SHAPE, "policy_loss expects [batch, classes] logits");
+  const int rows[] = {actions, old_log_probs, advantages, reference_log_probs, weights};
+  for (int i = 0; i < 5; ++i) {
+    if (i >= 3 && rows[i] == kNoNode) continue;
+    st = node_index(g, rows[i], "policy_loss");
+    if (st != OXH_OK) return st;
+    const Node &r = g.nodes[rows[i]];
+    OXH_REQUIRE(r.rank == 1 && r.shape[0] == l.shape[0], OXH_INVALID_SHAPE,
+                "policy_loss expects one action, log probability, advantage and weight a row");
+    n.in.push_back(rows[i]);
+  }
+  n.reference = reference_log_probs != kNoNode;
+  n.weights = weights != kNoNode;
+  OXH_REQUIRE(std::isfinite(clip_low) && clip_low >= 0.0f && clip_low <= 1.0f &&
+                  std::isfinite(clip_high) && clip_high >= 0.0f,
+              OXH_EXECUTION, "policy_loss clips must be finite and non-negative, the low one <= 1");
+  OXH_REQUIRE(std::isfinite(kl) && kl >= 0.0f, OXH_EXECUTION,
+              "policy_loss kl must be non-negative and finite");
+  OXH_REQUIRE(kl == 0.0f || n.reference, OXH_INVALID_SHAPE,
+              "policy_loss with a kl needs the reference's log probabilities");
+  n.clip_low = clip_low;
+  n.clip_high = clip_high;
+  n.kl = kl;
+  n.rank = 1;
+  n.shape = {1, 1, 1, 1};
+  *node = g.add(n);
+  return oxh::ok();
+}
+
 // ---------------------------------------------------------------- program helpers
 
 namespace {
@@ -352,7 +435,14 @@ std::vector<char> ancestors(const Graph &g, int root) {
   return active;
 }
 
-oxh_status plan_workspace(const Graph &g, const std::vector<char> &active, uint64_t &bytes) {
+oxh_delta_shape delta_shape(const Graph &g, const Node &n) {
+  const Node &k = g.nodes[n.in[1]], &v = g.nodes[n.in[2]];
+  return {v.shape[0], v.shape[1], k.shape[2], v.shape[2], k.shape[3], v.shape[3]};
+}
+
+// `trains`: for both passes of every operator, else for the forward alone.
+oxh_status plan_workspace(const Graph &g, const std::vector<char> &active, bool trains,
+                          uint64_t &bytes) {
   bytes = 256;
   for (size_t i = 0; i < g.nodes.size(); ++i) {
     if (!active[i]) continue;
@@ -371,6 +461,20 @@ oxh_status plan_workspace(const Graph &g, const std::vector<char> &active, uint6
       st = oxh_rms_norm_backward_workspace_size(norm_rows(n), n.shape[n.rank - 1], &b);
     } else if (n.op == Op::Recurrence) {
       st = oxh_gated_recurrence_workspace_size(n.shape[0], n.shape[1], n.shape[2], &b);
+    } else if (n.op == Op::LayerNorm) {
+      st = oxh_layer_norm_backward_workspace_size(norm_rows(n), n.shape[n.rank - 1], &b);
+    } else if (n.op == Op::DeltaRule) {
+      const oxh_delta_shape d = delta_shape(g, n);
+      st = oxh_gated_delta_rule_workspace_size(OXH_F32, &d, 0, &b);
+      uint64_t more[2] = {0, 0};
+      if (trains && st == OXH_OK)
+        st = oxh_gated_delta_rule_workspace_size(OXH_F32, &d, 1, &more[0]);
+      if (trains && st == OXH_OK)
+        st = oxh_gated_delta_rule_backward_workspace_size(OXH_F32, &d, &more[1]);
+      b = std::max(b, std::max(more[0], more[1]));
+    } else if (n.op == Op::PolicyLoss) {
+      const Node &l = g.nodes[n.in[0]];
+      st = oxh_policy_loss_workspace_size(l.shape[0], l.shape[1], &b);
     }
     if (st != OXH_OK) return st;
     if (b > bytes) bytes = b;
@@ -436,13 +540,16 @@ OpRec pool_forward_op(const Graph &g, const std::vector<float *> &value, size_t 
   return op;
 }
 
-// For each residual add the RMS norm that its launch forms with its sum (-1: none): the first norm
-// of the add's value, whose weight must exist by then (a leaf).
+// For each residual add the norm that its launch forms with its sum (-1: none): the first norm of
+// the add's value, whose parameters must exist by then (leaves).
 std::vector<int64_t> norms_of_adds(const Graph &g, const std::vector<char> &active) {
   std::vector<int64_t> norm(g.nodes.size(), -1);
   for (size_t i = 0; i < g.nodes.size(); ++i) {
     const Node &x = g.nodes[i];
-    if (!active[i] || x.op != Op::RmsNorm || !g.nodes[x.in[1]].leaf()) continue;
+    if (!active[i] || !is_norm(x.op)) continue;
+    bool leaves = true;
+    for (size_t k = 1; k < x.in.size(); ++k) leaves = leaves && g.nodes[x.in[k]].leaf();
+    if (!leaves) continue;
     if (g.nodes[x.in[0]].op == Op::Add && norm[x.in[0]] < 0)
       norm[x.in[0]] = static_cast<int64_t>(i);
   }
@@ -450,18 +557,20 @@ std::vector<int64_t> norms_of_adds(const Graph &g, const std::vector<char> &acti
 }
 
 // The norm of node i; `add` >= 0: with the residual add in front, whose sum the launch writes too.
-OpRec norm_forward_op(const Graph &g, const std::vector<float *> &value, float *inverse_rms,
-                      size_t i, int add) {
+OpRec norm_forward_op(const Graph &g, const std::vector<float *> &value, float *mean,
+                      float *inverse, size_t i, int add) {
   const Node &x = g.nodes[i];
   const Node &in = g.nodes[x.in[0]];
   const float *a = add >= 0 ? value[g.nodes[add].in[0]] : value[x.in[0]];
   const float *b = add >= 0 ? value[g.nodes[add].in[1]] : nullptr;
   float *sum = add >= 0 ? value[add] : nullptr, *out = value[i];
-  const float *w = value[x.in[1]];
+  const bool layer = x.op == Op::LayerNorm;
+  const float *w = value[x.in[1]], *bias = layer ? value[x.in[2]] : nullptr;
   const uint64_t rows = norm_rows(x), columns = x.shape[x.rank - 1];
   const float eps = x.epsilon;
   OpRec op;
-  op.kind = add >= 0 ? "add_rms_norm_forward" : "rms_norm_forward";
+  op.kind = std::string(add >= 0 ? "add_" : "") +
+            (layer ? "layer_norm_forward" : "rms_norm_forward");
   op.name = (add >= 0 ? "add" + std::to_string(add) + "+" : std::string()) + "norm" +
             std::to_string(i);
   if (add >= 0) {
@@ -472,11 +581,74 @@ OpRec norm_forward_op(const Graph &g, const std::vector<float *> &value, float *
     op.tensors = {ref("x", const_cast<float *>(a), in, 0)};
   }
   op.tensors.push_back(ref("weight", const_cast<float *>(w), g.nodes[x.in[1]], 0));
+  if (layer) op.tensors.push_back(ref("bias", const_cast<float *>(bias), g.nodes[x.in[2]], 0));
   op.tensors.push_back(ref("y", out, x, 1));
-  op.tensors.push_back(ref_flat("inverse_rms", inverse_rms, rows, 1));
+  if (layer) op.tensors.push_back(ref_flat("mean", mean, rows, 1));
+  op.tensors.push_back(ref_flat(layer ? "inverse_deviation" : "inverse_rms", inverse, rows, 1));
   op.attrs = {{"epsilon", eps}};
   op.launch = [=](hipStream_t st) {
-    return oxh_rms_norm_forward(st, OXH_F32, rows, columns, eps, a, b, w, sum, out, inverse_rms);
+    return layer ? oxh_layer_norm_forward(st, OXH_F32, rows, columns, eps, a, b, w, bias, sum, out,
+                                          mean, inverse)
+                 : oxh_rms_norm_forward(st, OXH_F32, rows, columns, eps, a, b, w, sum, out,
+                                        inverse);
+  };
+  return op;
+}
+
+// `saved` (null: none): what the backward reads.
+OpRec delta_forward_op(const Graph &g, const std::vector<float *> &value, float *saved,
+                       uint64_t saved_bytes, void *ws, uint64_t wsb, size_t i) {
+  const Node &x = g.nodes[i];
+  const oxh_delta_shape d = delta_shape(g, x);
+  static const char *const roles[] = {"query", "key", "value", "gate", "write"};
+  std::array<float *, 5> in;
+  OpRec op;
+  op.kind = "gated_delta_rule_forward";
+  op.name = "delta" + std::to_string(i);
+  for (int k = 0; k < 5; ++k) {
+    in[k] = value[x.in[k]];
+    op.tensors.push_back(ref(roles[k], in[k], g.nodes[x.in[k]], 0));
+  }
+  float *out = value[i];
+  op.tensors.push_back(ref("y", out, x, 1));
+  if (saved) op.tensors.push_back(ref_flat("saved", saved, saved_bytes / 4, 1));
+  const float scale = x.scale;
+  op.attrs = {{"scale", scale}};
+  op.launch = [=](hipStream_t st) {
+    return oxh_gated_delta_rule_forward(st, OXH_F32, &d, scale, in[0], in[1], in[2], in[3], in[4],
+                                        nullptr, nullptr, out, nullptr, saved,
+                                        saved ? saved_bytes : 0, ws, wsb);
+  };
+  return op;
+}
+
+// The loss (null: not formed) and the logits' gradient times `outer` (both null: not formed).
+OpRec policy_op(const Graph &g, const std::vector<float *> &value, float *loss, const float *outer,
+                float *gradient, uint32_t *flag, void *ws, uint64_t wsb, size_t i) {
+  const Node &x = g.nodes[i];
+  const Node &ln = g.nodes[x.in[0]];
+  const uint64_t rows = ln.shape[0], classes = ln.shape[1];
+  std::vector<const char *> roles = {"logits", "actions", "old_log_probs", "advantages"};
+  if (x.reference) roles.push_back("reference_log_probs");
+  if (x.weights) roles.push_back("weights");
+  OpRec op;
+  op.name = "policy" + std::to_string(i);
+  for (size_t k = 0; k < x.in.size(); ++k)
+    op.tensors.push_back(ref(roles[k], value[x.in[k]], g.nodes[x.in[k]], 0));
+  const float *lg = value[x.in[0]], *act = value[x.in[1]], *old = value[x.in[2]];
+  const float *adv = value[x.in[3]], *re = x.reference ? value[x.in[4]] : nullptr;
+  const float *wt = x.weights ? value[x.in[x.in.size() - 1]] : nullptr;
+  const float low = x.clip_low, high = x.clip_high, kl = x.kl;
+  if (outer)
+    op.tensors.push_back(ref_flat("outer_gradient", const_cast<float *>(outer), 1, 0));
+  if (loss) op.tensors.push_back(ref("loss", loss, x, 1));
+  if (gradient)
+    op.tensors.push_back(ref(loss ? "gradient" : "contribution", gradient, ln, 1));
+  op.tensors.push_back(ref_flat("error_flag", flag, 1, 2, 1));
+  op.attrs = {{"clip_low", low}, {"clip_high", high}, {"kl", kl}};
+  op.launch = [=](hipStream_t st) {
+    return oxh_policy_loss(st, OXH_F32, rows, classes, low, high, kl, lg, act, old, adv, re, wt,
+                           outer, loss, nullptr, gradient, flag, ws, wsb);
   };
   return op;
 }
@@ -585,11 +757,12 @@ oxh_status build_forward(const Graph &g, int output, oxh_program &p) {
       soff[i] = a.reserve(x.shape[1] * 4);
       ioff[i] = a.reserve(x.shape[1] * 4);
     }
-    if (x.op == Op::RmsNorm) ioff[i] = a.reserve(norm_rows(x) * 4);
+    if (is_norm(x.op)) ioff[i] = a.reserve(norm_rows(x) * 4);
+    if (x.op == Op::LayerNorm) soff[i] = a.reserve(norm_rows(x) * 4);
   }
   const uint64_t flag_off = a.reserve(4);
   uint64_t ws_bytes = 0;
-  oxh_status st = plan_workspace(g, active, ws_bytes);
+  oxh_status st = plan_workspace(g, active, false, ws_bytes);
   if (st != OXH_OK) return st;
   const uint64_t ws_off = a.reserve(ws_bytes);
   st = a.allocate();
@@ -621,16 +794,27 @@ oxh_status build_forward(const Graph &g, int output, oxh_program &p) {
         p.ops.push_back(conv_forward_op(g, p.value, i));
         break;
       case Op::RmsNorm:
-        if (!normed[i]) p.ops.push_back(norm_forward_op(g, p.value, p.saved_inv[i], i, -1));
+      case Op::LayerNorm:
+        if (!normed[i])
+          p.ops.push_back(norm_forward_op(g, p.value, p.saved_mean[i], p.saved_inv[i], i, -1));
         break;
       case Op::Recurrence:
         p.ops.push_back(recurrence_forward_op(g, p.value, ws, wsb, i));
+        break;
+      case Op::DeltaRule:
+        p.ops.push_back(delta_forward_op(g, p.value, nullptr, 0, ws, wsb, i));
+        break;
+      case Op::PolicyLoss:
+        p.ops.push_back(policy_op(g, p.value, p.value[i], nullptr, nullptr, p.error_flag, ws, wsb,
+                                  i));
+        p.ops.back().kind = "policy_loss_forward";
         break;
       case Op::Add:
         if (norm_of[i] >= 0 && !formed[i]) {
           const size_t j = static_cast<size_t>(norm_of[i]);
           normed[j] = 1;
-          p.ops.push_back(norm_forward_op(g, p.value, p.saved_inv[j], j, static_cast<int>(i)));
+          p.ops.push_back(norm_forward_op(g, p.value, p.saved_mean[j], p.saved_inv[j], j,
+                                          static_cast<int>(i)));
           break;
         }
         [[fallthrough]];
@@ -747,7 +931,7 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam,
     const Node &x = g.nodes[i];
     if (x.op == Op::Param) needs[i] = 1;
     else if (x.op == Op::Input) needs[i] = x.requires_grad ? 1 : 0;
-    else if (x.op == Op::CrossEntropy) needs[i] = needs[x.in[0]];  // targets take none
+    else if (is_loss(x.op)) needs[i] = needs[x.in[0]];  // the rows' other operands take none
     else
       for (int k : x.in) needs[i] = needs[i] || needs[k];
   }
@@ -841,8 +1025,7 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam,
   std::vector<char> has_grad(n, 0);
   std::vector<char> aliased(n, 0);      // an add's first operand using the add's buffer
   std::vector<char> view_alias(n, 0);  // a view (is_view) whose input uses its buffer
-  const bool root_fused_ce =
-      g.nodes[root].op == Op::CrossEntropy && want(g.nodes[root].in[0]);
+  const bool root_fused_ce = is_loss(g.nodes[root].op) && want(g.nodes[root].in[0]);
   for (size_t r = n; r-- > 0;) {
     const Node &x = g.nodes[r];
     if (!want(static_cast<int>(r)) || fused_bn[r] || pre_fused[r]) continue;
@@ -866,7 +1049,8 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam,
 
   // ---- plan the arena
   Arena &a = p.arena;
-  std::vector<int64_t> voff(n, -1), goff(n, -1), smoff(n, -1), sioff(n, -1);
+  std::vector<int64_t> voff(n, -1), goff(n, -1), smoff(n, -1), sioff(n, -1), deltaoff(n, -1);
+  std::vector<uint64_t> delta_bytes(n, 0);
   uint64_t largest = 1;
   for (size_t i = 0; i < n; ++i) {
     const Node &x = g.nodes[i];
@@ -876,14 +1060,21 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam,
       continue;
     }
     if (!active[i]) continue;
-    if (x.op == Op::RmsNorm) sioff[i] = a.reserve(norm_rows(x) * 4);
+    if (is_norm(x.op)) sioff[i] = a.reserve(norm_rows(x) * 4);
+    if (x.op == Op::LayerNorm) smoff[i] = a.reserve(norm_rows(x) * 4);
+    if (x.op == Op::DeltaRule && want(static_cast<int>(i))) {
+      const oxh_delta_shape d = delta_shape(g, x);
+      const oxh_status sized = oxh_gated_delta_rule_saved_size(OXH_F32, &d, &delta_bytes[i]);
+      if (sized != OXH_OK) return sized;
+      deltaoff[i] = a.reserve(delta_bytes[i]);
+    }
     if (x.op == Op::Bn) {  // saved statistics, also for a BN fused with its ReLU
       smoff[i] = a.reserve(x.shape[1] * 4);
       sioff[i] = a.reserve(x.shape[1] * 4);
     }
     if (x.leaf() || is_view(g, x) || fused_bn[i]) continue;
     voff[i] = a.reserve(node_bytes(x));
-    if (x.op != Op::CrossEntropy) largest = std::max(largest, x.numel());
+    if (!is_loss(x.op)) largest = std::max(largest, x.numel());
   }
   for (size_t i = 0; i < n; ++i)
     if (has_grad[i] && grad_of[i] < 0) goff[i] = a.reserve(node_bytes(g.nodes[i]));
@@ -915,8 +1106,8 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam,
   bool discards = false;
   for (size_t i = 0; i < n; ++i)
     if (want(static_cast<int>(i)) &&
-        (g.nodes[i].op == Op::Bn || g.nodes[i].op == Op::RmsNorm ||
-         g.nodes[i].op == Op::Recurrence || dw_conv[i]))
+        (g.nodes[i].op == Op::Bn || is_norm(g.nodes[i].op) ||
+         g.nodes[i].op == Op::Recurrence || g.nodes[i].op == Op::DeltaRule || dw_conv[i]))
       for (int k : g.nodes[i].in) discards = discards || !want(k);
   const uint64_t discard_off = a.reserve(discards ? kDiscardSlots * largest * 4 : 4);
   // A gradient a launch forms beside its main contribution (a convolution's or BatchNorm's
@@ -926,15 +1117,15 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam,
   bool sides = false;
   for (size_t i = 0; i < n; ++i) {
     const Node &x = g.nodes[i];
-    if (!active[i] || (x.op != Op::Conv && x.op != Op::Bn && x.op != Op::RmsNorm &&
-                       x.op != Op::Recurrence))
+    if (!active[i] || (x.op != Op::Conv && x.op != Op::Bn && !is_norm(x.op) &&
+                       x.op != Op::Recurrence && x.op != Op::DeltaRule))
       continue;
     for (size_t k = 1; k < x.in.size(); ++k)
       sides = sides || (want(x.in[k]) && consumers[x.in[k]] > 1);
   }
   const uint64_t side_off = a.reserve(sides ? kSideSlots * largest * 4 : 4);
   uint64_t ws_bytes = 0;
-  oxh_status st = plan_workspace(g, active, ws_bytes);
+  oxh_status st = plan_workspace(g, active, true, ws_bytes);
   if (st != OXH_OK) return st;
   std::vector<oxh_muon_tensor> shapes;  // the buffers follow once they are allocated
   for (int pn : trained)
@@ -1184,7 +1375,8 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam,
         if (norm_of[i] >= 0) {
           const size_t j = static_cast<size_t>(norm_of[i]);
           normed[j] = 1;
-          ops.push_back(norm_forward_op(g, p.value, p.saved_inv[j], j, static_cast<int>(i)));
+          ops.push_back(norm_forward_op(g, p.value, p.saved_mean[j], p.saved_inv[j], j,
+                                        static_cast<int>(i)));
           break;
         }
         [[fallthrough]];
@@ -1192,10 +1384,30 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam,
         ops.push_back(elementwise_forward_op(g, p.value, i));
         break;
       case Op::RmsNorm:
-        if (!normed[i]) ops.push_back(norm_forward_op(g, p.value, p.saved_inv[i], i, -1));
+      case Op::LayerNorm:
+        if (!normed[i])
+          ops.push_back(norm_forward_op(g, p.value, p.saved_mean[i], p.saved_inv[i], i, -1));
         break;
       case Op::Recurrence:
         ops.push_back(recurrence_forward_op(g, p.value, ws, wsb, i));
+        break;
+      case Op::DeltaRule:
+        ops.push_back(delta_forward_op(
+            g, p.value, deltaoff[i] >= 0 ? a.at<float>(deltaoff[i]) : nullptr, delta_bytes[i], ws,
+            wsb, i));
+        break;
+      case Op::PolicyLoss:
+        if (static_cast<int>(i) == root && root_fused_ce) {
+          // the root: loss and logit gradient in one pass, outer gradient 1
+          float *dl = nullptr, *acc = nullptr;
+          contribution(x.in[0], dl, acc);
+          op = policy_op(g, p.value, out, one, dl, p.error_flag, ws, wsb, i);
+          op.kind = "policy_loss";
+        } else {
+          op = policy_op(g, p.value, out, nullptr, nullptr, p.error_flag, ws, wsb, i);
+          op.kind = "policy_loss_forward";
+        }
+        ops.push_back(std::move(op));
         break;
       case Op::Relu:
         if (!fused_relu[i]) {
@@ -1362,7 +1574,7 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam,
   for (size_t r = n; r-- > 0;) {
     const Node &x = g.nodes[r];
     if (!want(static_cast<int>(r)) || x.leaf() || fused_bn[r] || pre_fused[r]) continue;
-    if (x.op == Op::CrossEntropy && static_cast<int>(r) == root && root_fused_ce) continue;
+    if (is_loss(x.op) && static_cast<int>(r) == root && root_fused_ce) continue;
     flush(static_cast<int>(r));  // a gradient still waiting for a second contribution
     OXH_REQUIRE(written[r], OXH_TRACE, "a traced value receives no gradient");
     const float *gr = p.grad[r];
@@ -1394,6 +1606,16 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam,
         emit(std::move(op), acc, ln, [=](hipStream_t st) {
           return oxh_cross_entropy_backward(st, rows, classes, lg, tg, gr, dst, flag);
         });
+        break;
+      }
+      case Op::PolicyLoss: {
+        float *dst, *acc;
+        contribution(x.in[0], dst, acc);
+        op = policy_op(g, p.value, nullptr, gr, dst, p.error_flag, ws, wsb, r);
+        op.kind = "policy_loss_backward";
+        op.name += ".backward";
+        auto body = std::move(op.launch);
+        emit(std::move(op), acc, g.nodes[x.in[0]], std::move(body));
         break;
       }
       case Op::Mul: {  // autograd.rs:123-138: d left = g * right, d right = g * left
@@ -1778,13 +2000,16 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam,
         });
         break;
       }
-      case Op::RmsNorm: {
+      case Op::RmsNorm:
+      case Op::LayerNorm: {
         // the input's other contributions, made by now or waiting as an add's, are added in the
         // same pass
         const int xin = x.in[0];
+        const bool layer = x.op == Op::LayerNorm;
         const float *xi = p.value[xin], *w = p.value[x.in[1]], *si = p.saved_inv[r];
+        const float *sm = p.saved_mean[r];
         const uint64_t rows = norm_rows(x), columns = x.shape[x.rank - 1];
-        float *dw = nullptr, *dst = nullptr, *acc = nullptr;
+        float *dw = nullptr, *db = nullptr, *dst = nullptr, *acc = nullptr;
         const float *addend = nullptr;
         if (want(xin) && !written[xin] && pending[xin].gradient != nullptr) {
           addend = pending[xin].gradient;
@@ -1800,16 +2025,23 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam,
         }
         // behind the input's: a value that is its own weight takes this one beside that
         if (want(x.in[1])) side(x.in[1], dw, "weight_gradient");
-        op.kind = "rms_norm_backward";
+        if (layer && want(x.in[2])) side(x.in[2], db, "bias_gradient");
+        op.kind = layer ? "layer_norm_backward" : "rms_norm_backward";
         op.name = name("norm", r) + ".backward";
         op.tensors.push_back(ref("gradient", const_cast<float *>(gr), x, 0));
         op.tensors.push_back(ref("x", const_cast<float *>(xi), g.nodes[xin], 0));
         op.tensors.push_back(ref("weight", const_cast<float *>(w), g.nodes[x.in[1]], 0));
-        op.tensors.push_back(ref_flat("inverse_rms", const_cast<float *>(si), rows, 0));
+        if (layer) op.tensors.push_back(ref_flat("mean", const_cast<float *>(sm), rows, 0));
+        op.tensors.push_back(ref_flat(layer ? "inverse_deviation" : "inverse_rms",
+                                      const_cast<float *>(si), rows, 0));
         op.tensors.push_back(addend == dst ? ref("input_gradient", dst, g.nodes[xin], 2)
                                            : ref("contribution", dst, g.nodes[xin], 1));
         if (dw != nullptr) op.tensors.push_back(ref_flat("weight_gradient", dw, columns, 1));
+        if (db != nullptr) op.tensors.push_back(ref_flat("bias_gradient", db, columns, 1));
         emit(std::move(op), acc, g.nodes[xin], [=](hipStream_t st) {
+          if (layer)
+            return oxh_layer_norm_backward(st, OXH_F32, rows, columns, gr, addend, xi, w, sm, si,
+                                           dst, dw, db, ws, wsb);
           return oxh_rms_norm_backward(st, OXH_F32, rows, columns, gr, addend, xi, w, si, dst, dw,
                                        ws, wsb);
         });
@@ -1834,6 +2066,36 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam,
           return oxh_gated_recurrence_backward(st, OXH_F32, batch, time, channels, gr, xi, gate, y,
                                                nullptr, nullptr, nullptr, dst, dgate, nullptr, ws,
                                                wsb);
+        });
+        break;
+      }
+      case Op::DeltaRule: {
+        const oxh_delta_shape d = delta_shape(g, x);
+        const float scale = x.scale;
+        const float *saved = a.at<float>(deltaoff[r]);
+        const uint64_t saved_bytes = delta_bytes[r];
+        static const char *const roles[] = {"query", "key", "value", "gate", "write"};
+        static const char *const sides_of[] = {"", "key_gradient", "value_gradient",
+                                               "gate_gradient", "write_gradient"};
+        std::array<const float *, 5> in;
+        std::array<float *, 5> grads;
+        float *acc;
+        contribution(x.in[0], grads[0], acc);
+        for (int k = 1; k < 5; ++k) side(x.in[k], grads[k], sides_of[k]);
+        op.kind = "gated_delta_rule_backward";
+        op.name = name("delta", r) + ".backward";
+        op.tensors.push_back(ref("gradient", const_cast<float *>(gr), x, 0));
+        for (int k = 0; k < 5; ++k) {
+          in[k] = p.value[x.in[k]];
+          op.tensors.push_back(ref(roles[k], const_cast<float *>(in[k]), g.nodes[x.in[k]], 0));
+        }
+        op.tensors.push_back(ref_flat("saved", const_cast<float *>(saved), saved_bytes / 4, 0));
+        for (int k = 0; k < 5; ++k)
+          op.tensors.push_back(ref(k ? sides_of[k] : "contribution", grads[k], g.nodes[x.in[k]], 1));
+        emit(std::move(op), acc, g.nodes[x.in[0]], [=](hipStream_t st) {
+          return oxh_gated_delta_rule_backward(
+              st, OXH_F32, &d, scale, gr, in[0], in[1], in[2], in[3], in[4], saved, saved_bytes,
+              nullptr, nullptr, grads[0], grads[1], grads[2], grads[3], grads[4], nullptr, ws, wsb);
         });
         break;
       }
@@ -2121,6 +2383,30 @@ oxh_status oxh_net_rms_norm(oxh_net *net, uint32_t x, uint32_t weight, float eps
 
 oxh_status oxh_net_gated_recurrence(oxh_net *net, uint32_t x, uint32_t gate, uint32_t *node) {
   OXH_NET_BUILD(oxh::net::gated_recurrence(net->graph, as_index(x), as_index(gate), &index));
+}
+
+oxh_status oxh_net_layer_norm(oxh_net *net, uint32_t x, uint32_t weight, uint32_t bias,
+                              float epsilon, uint32_t *node) {
+  OXH_NET_BUILD(oxh::net::layer_norm(net->graph, as_index(x), as_index(weight), as_index(bias),
+                                     epsilon, &index));
+}
+
+oxh_status oxh_net_gated_delta_rule(oxh_net *net, uint32_t query, uint32_t key, uint32_t value,
+                                    uint32_t gate, uint32_t write, float scale, uint32_t *node) {
+  OXH_NET_BUILD(oxh::net::gated_delta_rule(net->graph, as_index(query), as_index(key),
+                                           as_index(value), as_index(gate), as_index(write), scale,
+                                           &index));
+}
+
+oxh_status oxh_net_policy_loss(oxh_net *net, uint32_t logits, uint32_t actions,
+                               uint32_t old_log_probs, uint32_t advantages,
+                               uint32_t reference_log_probs, uint32_t weights, float clip_low,
+                               float clip_high, float kl, uint32_t *node) {
+  OXH_NET_BUILD(oxh::net::policy_loss(
+      net->graph, as_index(logits), as_index(actions), as_index(old_log_probs),
+      as_index(advantages),
+      reference_log_probs == OXH_NO_NODE ? oxh::net::kNoNode : as_index(reference_log_probs),
+      weights == OXH_NO_NODE ? oxh::net::kNoNode : as_index(weights), clip_low, clip_high, kl, &index));
 }
 
 oxh_status oxh_net_cross_entropy(oxh_net *net, uint32_t logits, uint32_t targets,

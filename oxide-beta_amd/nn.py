@@ -193,6 +193,23 @@ class RMSNorm(Module):
         return x.rms_norm(self.weight.tensor(), self.epsilon)
 
 
+class LayerNorm(Module):
+    """Layer norm over the last dimension, weight 1 and bias 0 (no counterpart in the reference)."""
+
+    def __init__(self, features, epsilon=1e-5):
+        if features == 0:
+            raise ox.OxideError(ox.INVALID_SHAPE, "LayerNorm features must be non-zero")
+        self.weight = Parameter(np.ones(features, np.float32))
+        self.bias = Parameter(np.zeros(features, np.float32))
+        self.epsilon = epsilon
+
+    def own_parameters(self):
+        return [self.weight, self.bias]
+
+    def forward(self, x):
+        return x.layer_norm(self.weight.tensor(), self.bias.tensor(), self.epsilon)
+
+
 class Linear(Module):
     """A 1 x 1 convolution over the last dimension of [batch, time, features]."""
 
@@ -225,6 +242,41 @@ class GatedRecurrentBlock(Module):
     def forward(self, x):
         y = self.norm(x)
         return x.add(self.project(self.value(y).gated_recurrence(self.gate(y))))
+
+
+class DeltaRuleBlock(Module):
+    """x + project(what a gated delta rule's state answers to queries) over [batch, time, features]:
+    queries, keys, values, gates and writes are projections of layer_norm(x), queries and keys of
+    length 1 (their root-mean-square norm times key_size ** -0.5).  ``heads`` states, each of a key
+    head of ``heads // key_heads`` of them; the gates start at ``gate_bias`` (no counterpart in the
+    reference)."""
+
+    def __init__(self, features, heads=4, key_heads=None, key_size=None, gate_bias=2.0):
+        key_heads = heads if key_heads is None else key_heads
+        if min(heads, key_heads) < 1 or features % heads or heads % key_heads:
+            raise ox.OxideError(ox.INVALID_SHAPE,
+                                "DeltaRuleBlock heads must divide the features, and key heads them")
+        key_size = features // heads if key_size is None else key_size
+        self.heads, self.key_heads, self.key_size = heads, key_heads, key_size
+        self.norm = LayerNorm(features)
+        self.query = Linear(features, key_heads * key_size)
+        self.key = Linear(features, key_heads * key_size)
+        self.value, self.project = Linear(features, features), Linear(features, features)
+        self.gate, self.write = Linear(features, heads), Linear(features, heads)
+        self.gate.conv.bias = Parameter(np.full(heads, gate_bias, np.float32))
+
+    def children(self):
+        return [self.norm, self.query, self.key, self.value, self.gate, self.write, self.project]
+
+    def forward(self, x):
+        batch, time, features = x.shape
+        y = self.norm(x)
+        unit = tn.constant(np.full(self.key_size, self.key_size ** -0.5))
+        query, key = (f(y).reshape((batch, time, self.key_heads, self.key_size)).rms_norm(unit)
+                      for f in (self.query, self.key))
+        value = self.value(y).reshape((batch, time, self.heads, features // self.heads))
+        answer = query.gated_delta_rule(key, value, self.gate(y), self.write(y), 1.0)
+        return x.add(self.project(answer.reshape((batch, time, features))))
 
 
 class GlobalAveragePool(Module):

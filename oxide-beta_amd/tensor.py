@@ -39,6 +39,7 @@ class MuonConfig(ctypes.Structure):
 
 
 _P = ctypes.POINTER
+NO_NODE = 0xffffffff  # OXH_NO_NODE
 _SIGNATURES = {
     "oxh_net_create": [_P(_vp)],
     "oxh_net_destroy": [_vp],
@@ -57,6 +58,9 @@ _SIGNATURES = {
     "oxh_net_cross_entropy": [_vp, _u32, _u32, _P(_u32)],
     "oxh_net_rms_norm": [_vp, _u32, _u32, _f32, _P(_u32)],
     "oxh_net_gated_recurrence": [_vp, _u32, _u32, _P(_u32)],
+    "oxh_net_layer_norm": [_vp, _u32, _u32, _u32, _f32, _P(_u32)],
+    "oxh_net_gated_delta_rule": [_vp, _u32, _u32, _u32, _u32, _u32, _f32, _P(_u32)],
+    "oxh_net_policy_loss": [_vp, _u32, _u32, _u32, _u32, _u32, _u32, _f32, _f32, _f32, _P(_u32)],
     "oxh_net_forward_program": [_vp, _u32, _P(_vp)],
     "oxh_net_training_program": [_vp, _u32, _P(AdamWConfig), _P(_vp)],
     "oxh_net_training_program_muon": [_vp, _u32, _P(MuonConfig), _P(_u32), _u32,
@@ -262,6 +266,67 @@ class Tensor:
                        "gated_recurrence expects [batch, time, channels] and a gate of that shape")
         return Tensor(self.shape, "gated_recurrence", (self, gate))
 
+    def layer_norm(self, weight, bias, epsilon: float = 1e-5):
+        """(s - mean(s)) / deviation(s) * weight + bias over the last dimension; of an add's value,
+        in its launch."""
+        if (weight.shape != self.shape[-1:] or bias.shape != weight.shape
+                or self.shape[-1] == 0):
+            raise _err(ox.INVALID_SHAPE,
+                       "layer_norm weight and bias must match the last dimension")
+        e32 = np.float32(epsilon)
+        if not np.isfinite(e32) or e32 < 0.0:
+            raise _err(ox.EXECUTION, "layer_norm epsilon must be non-negative and finite")
+        return Tensor(self.shape, "layer_norm", (self, weight, bias), epsilon=float(e32))
+
+    def gated_delta_rule(self, key, value, gate, write, scale: float | None = None):
+        """The answers to these queries of a state that each step fades by sigmoid(gate) and moves
+        by sigmoid(write) towards value at key, from a zero state; queries and keys [batch, time,
+        key heads, key size], values [batch, time, heads, value size], gate and write [batch, time,
+        heads].  ``scale``: key size ** -0.5."""
+        if (len(self.shape) != 4 or key.shape != self.shape or len(value.shape) != 4
+                or value.shape[:2] != key.shape[:2]):
+            raise _err(ox.INVALID_SHAPE,
+                       "gated_delta_rule expects query and key [batch, time, key heads, key size] "
+                       "and value [batch, time, heads, value size]")
+        if gate.shape != value.shape[:3] or write.shape != gate.shape:
+            raise _err(ox.INVALID_SHAPE,
+                       "gated_delta_rule expects gate and write [batch, time, heads]")
+        if not (1 <= self.shape[3] <= 128 and 1 <= value.shape[3] <= 4096 and self.shape[2]
+                and value.shape[2] and value.shape[2] % self.shape[2] == 0):
+            raise _err(ox.INVALID_SHAPE,
+                       "gated_delta_rule takes keys of 1 to 128 and values of 1 to 4096 entries, "
+                       "and heads in groups of the key heads")
+        s32 = np.float32(self.shape[3] ** -0.5 if scale is None else scale)
+        if not np.isfinite(s32):
+            raise _err(ox.EXECUTION, "gated_delta_rule scale must be finite")
+        return Tensor(value.shape, "gated_delta_rule", (self, key, value, gate, write),
+                      scale=float(s32))
+
+    def policy_loss(self, actions, old_log_probs, advantages, reference_log_probs=None,
+                    weights=None, clip=(0.2, 0.2), kl: float = 0.0):
+        """The clipped policy loss of these [batch, classes] logits (``oxh_policy_loss``), the
+        rows' mean or their sum by ``weights``, with the clip's (low, high) widths.  The other
+        operands take no gradient."""
+        rows = [t for t in (actions, old_log_probs, advantages, reference_log_probs, weights)
+                if t is not None]
+        if len(self.shape) != 2 or any(t.shape != self.shape[:1] for t in rows):
+            raise _err(ox.INVALID_SHAPE,
+                       "policy_loss expects [batch, classes] logits and one action, log "
+                       "probability, advantage and weight a row")
+        low, high = np.float32(clip)
+        if not (np.isfinite(low) and np.isfinite(high) and 0 <= low <= 1 and high >= 0):
+            raise _err(ox.EXECUTION, "policy_loss clips must be finite and non-negative, the low "
+                                     "one <= 1")
+        k32 = np.float32(kl)
+        if not np.isfinite(k32) or k32 < 0:
+            raise _err(ox.EXECUTION, "policy_loss kl must be non-negative and finite")
+        if k32 > 0 and reference_log_probs is None:
+            raise _err(ox.INVALID_SHAPE,
+                       "policy_loss with a kl needs the reference's log probabilities")
+        return Tensor((1,), "policy_loss", (self, *rows), clip_low=float(low),
+                      clip_high=float(high), kl=float(k32),
+                      referenced=reference_log_probs is not None, weighted=weights is not None)
+
 
 def input(shape, requires_grad: bool = False) -> Tensor:  # noqa: A001 - Tensor::placeholder
     """A value fed per run (a placeholder, tensor/mod.rs:520-522; ``requires_grad`` gives it a
@@ -375,6 +440,19 @@ class Net:
                   ctypes.byref(out))
         elif t.kind == "gated_recurrence":
             _call("oxh_net_gated_recurrence", h, n(t.args[0]), n(t.args[1]), ctypes.byref(out))
+        elif t.kind == "layer_norm":
+            _call("oxh_net_layer_norm", h, n(t.args[0]), n(t.args[1]), n(t.args[2]),
+                  t.attrs["epsilon"], ctypes.byref(out))
+        elif t.kind == "gated_delta_rule":
+            _call("oxh_net_gated_delta_rule", h, *(n(a) for a in t.args), t.attrs["scale"],
+                  ctypes.byref(out))
+        elif t.kind == "policy_loss":
+            a = t.attrs
+            rest = [n(x) for x in t.args[4:]]
+            reference = rest.pop(0) if a["referenced"] else NO_NODE
+            _call("oxh_net_policy_loss", h, *(n(x) for x in t.args[:4]), reference,
+                  rest.pop(0) if a["weighted"] else NO_NODE, a["clip_low"], a["clip_high"],
+                  a["kl"], ctypes.byref(out))
         elif t.kind == "cross_entropy":
             _call("oxh_net_cross_entropy", h, n(t.args[0]), n(t.args[1]), ctypes.byref(out))
         else:
@@ -448,7 +526,8 @@ class Program:
         ox.check(ox.lib().oxh_stream_synchronize(self.stream_handle))
 
     def check(self) -> None:
-        """Waits; InvalidShape if a cross entropy met a target that is not a class index."""
+        """Waits; InvalidShape if a cross entropy or policy loss met a target or action that
+        is not a class index."""
         _call("oxh_program_check", self.handle)
 
     def steps(self) -> int:

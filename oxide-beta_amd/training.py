@@ -472,8 +472,8 @@ class EvalForward:
 def op_bytes(op: Op) -> tuple[str, int]:
     """(category, algorithmic HBM bytes) of one launch group: every tensor it must read or
     write, once (fp32).  Categories: the hot-path kernel families (batch_norm2d, elementwise,
-    cross_entropy, adamw), the layers around them (conv2d, avg_pool2d) and those of sequence models
-    (rms_norm, gated_recurrence, muon)."""
+    cross_entropy, policy_loss, adamw), the layers around them (conv2d, avg_pool2d) and those of
+    sequence models (rms_norm, layer_norm, gated_recurrence, gated_delta_rule, muon)."""
     nb = lambda t: t.numel() * 4  # noqa: E731
     acc = 3 * nb(op.accumulate_into) if op.accumulate_into is not None else 0
     k = op.kind
@@ -516,14 +516,24 @@ def op_bytes(op: Op) -> tuple[str, int]:
         return "adamw", sum(7 * nb(t[0]) for t in op.attrs["tensors"])
     if k == "muon":  # parameter and momentum in and out, gradient in; no fp16 halves
         return "muon", sum(5 * nb(t) for t in op.by_role["gradient"])
-    if k == "rms_norm_forward":
-        return "rms_norm", 2 * nb(op.reads["x"])
-    if k == "add_rms_norm_forward":
-        return "rms_norm", 4 * nb(op.reads["a"])                           # a, b in; sum, y out
-    if k == "rms_norm_backward":
+    if k in ("policy_loss", "policy_loss_backward"):
+        return "policy_loss", 2 * nb(op.reads["logits"]) + acc
+    if k == "policy_loss_forward":
+        return "policy_loss", nb(op.reads["logits"])
+    if k in ("rms_norm_forward", "layer_norm_forward"):
+        return k[:-8], 2 * nb(op.reads["x"])
+    if k in ("add_rms_norm_forward", "add_layer_norm_forward"):
+        return k[4:-8], 4 * nb(op.reads["a"])                              # a, b in; sum, y out
+    if k in ("rms_norm_backward", "layer_norm_backward"):
         # g, x in; dx out; the input's other gradient in, a waiting add's or the one in place
         other = "addend" in op.reads or "input_gradient" in op.by_role
-        return "rms_norm", (3 + other) * nb(op.reads["gradient"]) + acc
+        return k[:-9], (3 + other) * nb(op.reads["gradient"]) + acc
+    if k.startswith("gated_delta_rule"):  # the operands in; y, or their gradients out; saved
+        operands = sum(nb(op.reads[r]) for r in ("query", "key", "value", "gate", "write"))
+        saved = sum(nb(t) for t in op.by_role.get("saved", ()))
+        if k.endswith("forward"):
+            return "gated_delta_rule", operands + nb(op.writes["y"]) + saved
+        return "gated_delta_rule", 2 * operands + nb(op.reads["gradient"]) + saved + acc
     if k == "gated_recurrence_forward":
         return "gated_recurrence", 3 * nb(op.reads["x"])                   # x, gate in; y out
     if k == "gated_recurrence_backward":

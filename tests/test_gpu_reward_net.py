@@ -1,0 +1,298 @@
+"""Layer norm, the gated delta rule and the clipped policy loss in traced graphs, together as a model
+that is trained by reward runs them: gradients against torch float64 autograd of the same graph,
+replays against eager steps, the example's commands.
+
+Tolerance of a gradient: at most 8 operators lie between it and the loss, each within 1024 * 2^-24
+of its terms' magnitudes (the operators' own tests), 4.9e-4 of the gradient's Frobenius norm: 5e-4,
+as the other sequence layers' graphs."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+import torch.nn.functional as F
+
+import jit
+import nn
+import oxide_hip as ox
+import sequence
+import tensor as tn
+import training
+from test_data_checkpoint import _idx_images, _idx_labels
+from test_gpu_sequence_net import (close, images_of, kinds, leaf, norm64, randn, run_checked)
+
+pytestmark = pytest.mark.gpu
+
+
+def layer64(x, w, b, eps=1e-5):
+    u = x - x.mean(-1, keepdim=True)
+    return u * torch.rsqrt(u.square().mean(-1, keepdim=True) + eps) * w + b
+
+
+def delta64(q, k, v, gate, write, scale=None):
+    group = v.shape[2] // k.shape[2]
+    q, k = (x.repeat_interleave(group, 2) for x in (q, k))
+    a, b, out = torch.sigmoid(gate), torch.sigmoid(write), []
+    s = torch.zeros(*v.shape[:1], v.shape[2], k.shape[3], v.shape[3], dtype=torch.float64)
+    for t in range(v.shape[1]):
+        p = a[:, t, :, None, None] * s
+        wrong = v[:, t] - (p * k[:, t, ..., None]).sum(2)
+        s = p + (b[:, t, :, None] * k[:, t])[..., None] * wrong[:, :, None]
+        out.append((s * q[:, t, ..., None]).sum(2))
+    return torch.stack(out, 1) * (k.shape[3] ** -0.5 if scale is None else scale)
+
+
+def policy64(logits, actions, old, advantages, reference=None, weights=None, clip=(0.2, 0.2),
+             kl=0.0):
+    rows = torch.arange(len(logits))
+    at = torch.log_softmax(logits, 1)[rows, torch.as_tensor(actions, dtype=torch.long)]
+    ratio = torch.exp(at - c64(old))
+    adv = c64(advantages)
+    loss = -torch.minimum(ratio * adv, ratio.clamp(1 - clip[0], 1 + clip[1]) * adv)
+    if reference is not None:
+        d = c64(reference) - at
+        loss = loss + kl * (torch.exp(d) - d - 1)
+    w = torch.full_like(loss, 1 / len(loss)) if weights is None else c64(weights)
+    return (loss * w).sum()
+
+
+def c64(v):
+    return torch.tensor(np.asarray(v, np.float64))
+
+
+def unit(v):
+    return v / np.linalg.norm(v, axis=-1, keepdims=True)
+
+
+def drawn(rows, classes, seed):
+    """Actions, old log probabilities, advantages, reference ones and weights."""
+    r = np.random.default_rng(seed)
+    f = lambda v: np.asarray(v, np.float32)  # noqa: E731
+    return (f(r.integers(0, classes, rows)), f(-2 + 0.3 * r.standard_normal(rows)),
+            f(r.standard_normal(rows)), f(-2 + 0.3 * r.standard_normal(rows)),
+            f(r.random(rows) / rows))
+
+
+@pytest.mark.parametrize("time,heads,key_heads", [(9, 2, 2), (70, 4, 2)])
+def test_norms_rule_and_policy(time, heads, key_heads):
+    """s1 = a + b, y1 = layer norm(s1) (one launch), values of the rule, s2 = s1 + answers, y2 (one
+    launch, the same parameters); the policy loss with a KL and weights is the root."""
+    B, D, K = 3, heads * 6, 5
+    av, bv = randn(B, time, D, seed=1), randn(B, time, D, seed=2)
+    qv, kv = (unit(randn(B, time, key_heads, K, seed=i)) for i in (3, 4))
+    gv, wv = 1.5 * randn(B, time, heads, seed=5) + 2, randn(B, time, heads, seed=6)
+    nw, nb, mv = 1 + 0.1 * randn(D, seed=7), 0.1 * randn(D, seed=8), randn(B, time, D, seed=9)
+    rows = drawn(B * D, time, 10)
+    a, b = (tn.input((B, time, D), requires_grad=True) for _ in range(2))
+    q, k = (tn.input((B, time, key_heads, K), requires_grad=True) for _ in range(2))
+    g, w = (tn.input((B, time, heads), requires_grad=True) for _ in range(2))
+    W, Bi = nn.Parameter(nw), nn.Parameter(nb)
+    s1 = a.add(b)
+    y1 = s1.layer_norm(W.tensor(), Bi.tensor())
+    v = y1.reshape((B, time, heads, D // heads))
+    s2 = s1.add(q.gated_delta_rule(k, v, g, w).reshape((B, time, D)))
+    y2 = s2.layer_norm(W.tensor(), Bi.tensor())
+    logits = y2.mul(tn.constant(mv)).reshape((B * D, time))
+    fed = [tn.input((B * D,)) for _ in rows]
+    loss = logits.policy_loss(*fed[:3], reference_log_probs=fed[3], weights=fed[4],
+                              clip=(0.1, 0.3), kl=0.2)
+    program = tn.training_program(loss)
+    assert kinds(program).count("add_layer_norm_forward") == 2
+    for once in ("policy_loss", "gated_delta_rule_forward", "gated_delta_rule_backward"):
+        assert kinds(program).count(once) == 1
+    assert not {"add_forward", "layer_norm_forward", "seed"} & set(kinds(program))
+    for node, value in zip((a, b, q, k, g, w, *fed), (av, bv, qv, kv, gv, wv, *rows)):
+        program.feed(node, value)
+    bytes_of = {op.kind: training.op_bytes(op) for op in program.ops}
+    assert bytes_of["add_layer_norm_forward"] == ("layer_norm", 4 * 4 * B * time * D)
+    assert bytes_of["policy_loss"] == ("policy_loss", 2 * 4 * B * time * D)
+    assert bytes_of["gated_delta_rule_backward"][0] == "gated_delta_rule"
+    run_checked(program)
+    A, Bt, Q, Ke, G, Wr, NW, NB = map(leaf, (av, bv, qv, kv, gv, wv, nw, nb))
+    S1 = A + Bt
+    V = layer64(S1, NW, NB).reshape(B, time, heads, -1)
+    S2 = S1 + delta64(Q, Ke, V, G, Wr).reshape(B, time, D)
+    Y2 = layer64(S2, NW, NB)
+    L = policy64((Y2 * c64(mv)).reshape(B * D, time), *rows[:3], rows[3], rows[4], (0.1, 0.3), 0.2)
+    L.backward()
+    close(program.value(s2).host(), S2, "second sum")
+    close(program.value(y2).host(), Y2, "second norm")
+    close(program.value(loss).host()[0], L, "loss")
+    for node, ref in ((a, A), (b, Bt), (q, Q), (k, Ke), (g, G), (w, Wr)):
+        close(program.gradient(node).host(), ref.grad, node)
+    close(program.gradient(W.tensor()).host(), NW.grad, "weight")
+    close(program.gradient(Bi.tensor()).host(), NB.grad, "bias")
+
+
+def test_one_value_in_many_places_and_a_loss_that_is_not_the_root():
+    """One value as query and key, one as gate and write, values that need no gradient, logits of
+    two losses that are added."""
+    B, T, H, K = 2, 20, 2, 4
+    kv = unit(randn(B, T, H, K, seed=1))
+    gv, vv = randn(B, T, H, seed=2), randn(B, T, H, K, seed=3)
+    rows = drawn(B * T, H * K, 4)
+    k, v = tn.input((B, T, H, K), requires_grad=True), tn.input((B, T, H, K))
+    g = tn.input((B, T, H), requires_grad=True)
+    fed = [tn.input((B * T,)) for _ in range(3)]
+    logits = k.gated_delta_rule(k, v, g, g, 0.7).reshape((B * T, H * K))
+    loss = logits.policy_loss(*fed).add(logits.cross_entropy(fed[0]))
+    program = tn.training_program(loss)
+    assert {"policy_loss_forward", "policy_loss_backward"} <= set(kinds(program))
+    for node, value in zip((k, v, g, *fed), (kv, vv, gv, *rows)):
+        program.feed(node, value)
+    run_checked(program)
+    Ke, G = leaf(kv), leaf(gv)
+    Lo = delta64(Ke, Ke, c64(vv), G, G, 0.7).reshape(B * T, H * K)
+    L = policy64(Lo, *rows[:3]) + F.cross_entropy(Lo, torch.tensor(rows[0], dtype=torch.long))
+    L.backward()
+    close(program.value(loss).host()[0], L, "loss")
+    close(program.gradient(k).host(), Ke.grad, "query and key")
+    close(program.gradient(g).host(), G.grad, "gate and write")
+    assert program.gradient(v) is None
+
+
+@pytest.mark.parametrize("uses", ["alone", "added"])
+def test_layer_norm_of_a_value_by_itself(uses):
+    """A value that is input, weight and bias of a norm takes all three gradients, beside an add's."""
+    D, wv, mv = 24, 1 + 0.3 * randn(24, seed=5), randn(24, seed=6)
+    w, t = nn.Parameter(wv), tn.input((1,))
+    v = w.tensor()
+    y = v.layer_norm(v, v, 1e-3)
+    out = y if uses == "alone" else y.add(v)
+    program = tn.training_program(out.mul(tn.constant(mv)).reshape((1, D)).cross_entropy(t))
+    program.feed(t, np.array([3], np.float32))
+    run_checked(program)
+    W = leaf(wv)
+    Y = layer64(W, W, W, 1e-3)
+    L = F.cross_entropy(((Y if uses == "alone" else Y + W) * c64(mv)).reshape(1, D),
+                        torch.tensor([3]))
+    L.backward()
+    close(program.gradient(v).host(), W.grad, uses)
+
+
+@pytest.mark.parametrize("time", [1, 16, 17, 150])
+def test_forward_program(time):
+    """Without gradients: steps one by one up to 16 of them, chunks above."""
+    k, v = tn.input((2, time, 1, 8)), tn.input((2, time, 3, 20))
+    g, w = tn.input((2, time, 3)), tn.input((2, time, 3))
+    s, W, Bi = tn.input((2, time, 3, 20)), randn(20, seed=1), randn(20, seed=2)
+    out = k.gated_delta_rule(k, v, g, w).add(s).layer_norm(tn.constant(W), tn.constant(Bi))
+    program = tn.forward_program(out, [k, v, g, w, s])
+    assert kinds(program) == ["gated_delta_rule_forward", "add_layer_norm_forward"]
+    values = [unit(randn(*k.shape, seed=3))] + [randn(*t.shape, seed=4 + i)
+                                                for i, t in enumerate((v, g, w, s))]
+    for node, value in zip((k, v, g, w, s), values):
+        program.feed(node, value)
+    program.run()
+    K, V, G, Wr, S = map(c64, values)
+    close(program.value(out).host(), layer64(delta64(K, K, V, G, Wr) + S, c64(W), c64(Bi)), "out")
+
+
+def model_of():
+    return sequence.RowClassifier(features=32, depth=2, block=nn.DeltaRuleBlock, norm=nn.LayerNorm)
+
+
+def model64(model, params, images):
+    """The model over float64 tensors in place of its parameters."""
+    p = {id(a): b for a, b in zip(model.parameters(), params)}
+
+    def linear(m, v):
+        return v @ p[id(m.conv.weight)].reshape(m.conv.weight.shape[:2]).T + p[id(m.conv.bias)]
+
+    def norm(m, v):
+        return layer64(v, p[id(m.weight)], p[id(m.bias)])
+
+    x = linear(model.widen, images)
+    for b in model.blocks:
+        y = norm(b.norm, x)
+        split = lambda v, n: v.reshape(*v.shape[:2], n, -1)  # noqa: E731
+        q, k = (norm64(split(linear(f, y), b.key_heads), b.key_size ** -0.5)
+                for f in (b.query, b.key))
+        o = delta64(q, k, split(linear(b.value, y), b.heads), linear(b.gate, y),
+                    linear(b.write, y), 1.0)
+        x = x + linear(b.project, o.reshape(x.shape))
+    mean = norm(model.norm, x).mean(1)
+    c = model.classifier
+    return mean @ p[id(c.weight)].reshape(c.weight.shape[:2]).T + p[id(c.bias)]
+
+
+def test_gradients_of_a_model_trained_by_reward():
+    """The draw's log probabilities are the model's; after a step, whose update moved the policy,
+    every parameter's gradient of the second step is the graph's."""
+    images, labels = images_of(16)
+    model = model_of()
+    step = sequence.RewardTraining(model, 16)
+    pixels = images.astype(np.float32).reshape(16, 1, 28, 28) / 255
+    step.images.copy_from(pixels)
+    actions = step.draw()
+    old, rewards = step._rows[1].host(), (actions == labels).astype(np.float64)
+    params = [leaf(p.host()) for p in model.parameters()]
+    logits = model64(model, params, c64(pixels[:, 0]))
+    at = torch.log_softmax(logits, 1)[torch.arange(16), torch.as_tensor(actions)]
+    close(old, at, "log probabilities")
+    step.step(rewards)
+    torch.cuda.synchronize()
+    params = [leaf(p.host()) for p in model.parameters()]
+    step.step(rewards)
+    advantages = step._rows[2].host()
+    L = policy64(model64(model, params, c64(pixels[:, 0])), actions, old, advantages)
+    L.backward()
+    assert abs(step.loss() - L.item()) <= 5e-4 * np.abs(advantages).mean()
+    for p, ref in zip(model.parameters(), params):
+        close(step.program.gradient(p.tensor()).host(), ref.grad, p.shape)
+
+
+def test_replays_equal_eager_steps():
+    images, labels = images_of(16)
+    x, y = images.astype(np.float32).reshape(16, 1, 28, 28) / 255, labels.astype(np.float32)
+    results = []
+    for replay in (True, False):
+        step = sequence.Training(model_of(), 16)
+        step.images.copy_from(x)
+        step.labels.copy_from(y)
+        losses = []
+        for _ in range(4):
+            step.step() if replay else step.program.run()
+            losses.append(step.loss())
+        results.append((losses, step.logits.host()))
+    assert results[0][0] == results[1][0] and np.array_equal(results[0][1], results[1][1])
+
+
+def test_an_action_that_is_no_class():
+    model = model_of()
+    step = sequence.RewardTraining(model, 4)
+    step.images.copy_from(np.zeros((4, 1, 28, 28), np.float32))
+    step.draw()
+    step._rows[0].copy_from(np.array([0, 10, 2, 3], np.float32))
+    step.step([1, 0, 0, 1])
+    with pytest.raises(ox.OxideError) as err:
+        step.loss()
+    assert err.value.kind == "InvalidShape"
+
+
+def test_compiled_block():
+    block, x = nn.DeltaRuleBlock(24, heads=4, key_heads=2, key_size=5), randn(2, 11, 24, seed=1)
+    module = jit.compile(block, x)
+    c = lambda m: c64(m.host())  # noqa: E731
+    lin = lambda m, v: v @ c(m.conv.weight)[:, :, 0, 0].T + c(m.conv.bias)  # noqa: E731
+    X = c64(x)
+    y = layer64(X, c(block.norm.weight), c(block.norm.bias))
+    q, k = (norm64(lin(f, y).reshape(2, 11, 2, 5), 5 ** -0.5) for f in (block.query, block.key))
+    o = delta64(q, k, lin(block.value, y).reshape(2, 11, 4, 6), lin(block.gate, y),
+                lin(block.write, y), 1.0)
+    ref = X + lin(block.project, o.reshape(2, 11, 24))
+    for _ in range(2):
+        close(np.asarray(module.run([x])).reshape(x.shape), ref, "block")
+
+
+@pytest.mark.parametrize("kind", [("delta",), ("delta", "reward"), ("reward",)])
+def test_example_on_idx_files(tmp_path, capsys, kind):
+    for name, count, seed in (("train", 256, 0), ("t10k", 100, 1)):
+        images, labels = images_of(count, seed)
+        (tmp_path / f"{name}-images-idx3-ubyte").write_bytes(_idx_images(images))
+        (tmp_path / f"{name}-labels-idx1-ubyte").write_bytes(_idx_labels(labels))
+    sequence.main(str(tmp_path), 2, *kind)
+    lines = capsys.readouterr().out.splitlines()
+    assert [line.split()[0] for line in lines] == ["epoch", "epoch", "test"]
+    assert math.isfinite(float(lines[1].split()[-1])) and 0 <= float(lines[2].split()[-1]) <= 1

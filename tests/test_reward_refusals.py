@@ -87,6 +87,9 @@ BAD_DIMS = [(dict(key_dim=0), b"key_dim"), (dict(key_dim=129), b"key_dim"),
             (dict(batch=60000, heads=60000, time=64), b"one call"),
             (dict(batch=1, heads=64000, key_heads=64000, value_dim=4096, time=64, dtype=1,
                   kept=1 << 62),
+             b"2^24"),
+            (dict(batch=1, heads=64000, key_heads=64000, value_dim=256, time=64, dtype=1,
+                  kept=1 << 62),
              b"workspace"), (dict(dtype=2), b"dtype")]
 
 
@@ -175,3 +178,98 @@ def test_policy_loss():
         refused(policy(**{name: at}), b"overlaps an operand")
     for name, at in (("lp", loss), ("g", lp), ("ws", g)):
         refused(policy(**{name: at}), b"two outputs")
+
+
+def test_net_builders():
+    """oxh_net_* of the three, before anything is allocated."""
+    import tensor
+
+    L, h, u32 = tensor._lib(), ctypes.c_void_p(), ctypes.c_uint32
+    none = tensor.NO_NODE
+    assert L.oxh_net_create(ctypes.byref(h)) == ox.OK
+
+    def leaf(*d):
+        n = u32()
+        shape = (ctypes.c_uint64 * len(d))(*d)
+        assert L.oxh_net_input(h, len(d), shape, 0, ctypes.byref(n)) == ox.OK
+        return n.value
+
+    n = u32()
+    out = ctypes.byref(n)
+    x, w, short = leaf(2, 3, 8), leaf(8), leaf(7)
+    for a, b, c in ((x, short, short), (x, w, short), (x, w, x), (x, 99, w), (99, w, w),
+                    (x, w, 99)):
+        assert L.oxh_net_layer_norm(h, a, b, c, 1e-5, out) == ox.INVALID_SHAPE
+    for eps in (-1.0, NAN, INF):
+        refused(L.oxh_net_layer_norm(h, x, w, w, eps, out), b"epsilon", ox.EXECUTION)
+    assert L.oxh_net_layer_norm(h, x, w, w, 0.0, out) == ox.OK
+
+    k, v, g = leaf(2, 5, 2, 8), leaf(2, 5, 4, 6), leaf(2, 5, 4)
+
+    def rule(query=k, key=k, value=v, gate=g, write=g, scale=1.0):
+        return L.oxh_net_gated_delta_rule(h, query, key, value, gate, write, scale, out)
+
+    for bad in (dict(query=leaf(2, 5, 2, 7)), dict(value=leaf(2, 4, 4, 6)), dict(value=x),
+                dict(value=leaf(3, 5, 4, 6)), dict(gate=leaf(2, 5, 2)), dict(write=x),
+                dict(key=99), dict(write=99)):
+        assert rule(**bad) == ox.INVALID_SHAPE, bad
+    odd = dict(value=leaf(2, 5, 3, 6), gate=leaf(2, 5, 3))
+    assert rule(**odd, write=odd["gate"]) == ox.INVALID_SHAPE  # 3 heads of 2 key heads
+    wide = leaf(2, 5, 2, 129)
+    refused(rule(query=wide, key=wide), b"key_dim")
+    refused(rule(scale=NAN), b"scale", ox.EXECUTION)
+    assert rule() == ox.OK
+    rank, dims = u32(), (ctypes.c_uint64 * 4)()
+    assert L.oxh_net_node_shape(h, n.value, ctypes.byref(rank), dims) == ox.OK
+    assert rank.value == 4 and list(dims) == [2, 5, 4, 6]
+
+    logits, row = leaf(6, 8), leaf(6)
+
+    def policy(a=logits, b=row, c=row, d=row, reference=none, weights=none, low=0.2, high=0.2,
+               kl=0.0):
+        return L.oxh_net_policy_loss(h, a, b, c, d, reference, weights, low, high, kl, out)
+
+    for bad in (dict(a=x), dict(b=short), dict(c=x), dict(d=99), dict(weights=short),
+                dict(weights=99), dict(reference=none - 1), dict(kl=0.1)):
+        assert policy(**bad) == ox.INVALID_SHAPE, bad
+    for bad in (dict(low=-0.1), dict(low=1.1), dict(high=INF), dict(kl=-1.0), dict(kl=NAN)):
+        assert policy(**bad) == ox.EXECUTION, bad
+    assert policy(reference=row, weights=row, kl=0.1) == ox.OK
+    assert policy(reference=row) == ox.OK
+    assert L.oxh_net_layer_norm(None, x, w, w, 0.0, out) == ox.INVALID_SHAPE
+    assert L.oxh_net_policy_loss(h, logits, row, row, row, none, none, 0.2, 0.2, 0.0,
+                                 None) == ox.INVALID_SHAPE
+    assert L.oxh_net_destroy(h) == ox.OK
+
+
+def test_tensor_methods():
+    """The Python graph's own checks."""
+    import nn
+    import tensor as tn
+
+    i = tn.input
+    for call in (lambda: i((2, 3)).layer_norm(i((2,)), i((2,))),
+                 lambda: i((2, 3)).layer_norm(i((3,)), i((2,))),
+                 lambda: i((2, 5, 2, 8)).gated_delta_rule(i((2, 5, 2, 7)), i((2, 5, 2, 3)),
+                                                          i((2, 5, 2)), i((2, 5, 2))),
+                 lambda: i((2, 5, 2, 8)).gated_delta_rule(i((2, 5, 2, 8)), i((2, 5, 3, 3)),
+                                                          i((2, 5, 3)), i((2, 5, 3))),
+                 lambda: i((2, 5, 2, 8)).gated_delta_rule(i((2, 5, 2, 8)), i((2, 5, 2, 3)),
+                                                          i((2, 5, 2)), i((2, 5, 1))),
+                 lambda: i((2, 5, 2, 129)).gated_delta_rule(i((2, 5, 2, 129)), i((2, 5, 2, 3)),
+                                                            i((2, 5, 2)), i((2, 5, 2))),
+                 lambda: i((4, 3)).policy_loss(i((4,)), i((4,)), i((3,))),
+                 lambda: i((4, 3)).policy_loss(i((4,)), i((4,)), i((4,)), kl=0.1),
+                 lambda: nn.LayerNorm(0), lambda: nn.DeltaRuleBlock(10, heads=4),
+                 lambda: nn.DeltaRuleBlock(12, heads=4, key_heads=3)):
+        with pytest.raises(ox.OxideError) as err:
+            call()
+        assert err.value.kind == "InvalidShape"
+    for call in (lambda: i((2, 3)).layer_norm(i((3,)), i((3,)), NAN),
+                 lambda: i((2, 5, 2, 8)).gated_delta_rule(i((2, 5, 2, 8)), i((2, 5, 2, 3)),
+                                                          i((2, 5, 2)), i((2, 5, 2)), INF),
+                 lambda: i((4, 3)).policy_loss(i((4,)), i((4,)), i((4,)), clip=(1.5, 0.2)),
+                 lambda: i((4, 3)).policy_loss(i((4,)), i((4,)), i((4,)), kl=-0.1)):
+        with pytest.raises(ox.OxideError) as err:
+            call()
+        assert err.value.kind == "Execution"
