@@ -80,6 +80,9 @@ __device__ __forceinline__ operand<T> rounded(f32x8 v) {
 }
 __device__ __forceinline__ f32x8 widened(bf16x8 v) { return __builtin_convertvector(v, f32x8); }
 __device__ __forceinline__ f32x8 widened(f32x8 v) { return v; }
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f32x4 widened(bf16x4 v) { return __builtin_convertvector(v, f32x4); }
+__device__ __forceinline__ f32x4 widened(f32x4 v) { return v; }
 
 // A float32 operand as bfloat16 ones that add up to it: to 2^-17 of each value with two.
 template <typename T, int Parts>
@@ -186,24 +189,30 @@ __device__ __forceinline__ int upper_place(int tile, int step) {
 // columns.
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+// Mixed: the slabs' lanes are the pair's columns in the order of index_of.
+template <bool Mixed>
 __device__ __forceinline__ bf16x8 turned(const bf16x8 *first, uint32_t apart, int half, uint32_t n,
                                          uint32_t g) {
   // 16 lanes read four columns' 16 rows, four of them each, and get a row of it
-  const bf16x8 *at = first + (g >> 1) * apart + (n & 3) * 16 + 8 * (g & 1) + (n >> 2);
   s16x4 v[2];
 #pragma unroll
-  for (int e = 0; e < 2; ++e)
-    v[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (lds_s16x4 *)(reinterpret_cast<const s16x4 *>(at + 4 * e) + half));
+  for (int e = 0; e < 2; ++e) {
+    const uint32_t at = Mixed ? e * apart + 4 * g : (g >> 1) * apart + 8 * (g & 1) + 4 * e;
+    v[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(
+        reinterpret_cast<const s16x4 *>(first + at + (n & 3) * 16 + (n >> 2)) + half));
+  }
   return __builtin_bit_cast(bf16x8, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
 }
+template <bool Mixed>
 __device__ __forceinline__ f32x8 turned(const f32x8 *first, uint32_t apart, int half, uint32_t n,
                                         uint32_t g) {
-  const f32x8 *at = first + (g >> 1) * apart + (n >> 2) * 16 + 8 * (g & 1);
   f32x8 v;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    v[i] = reinterpret_cast<const float *>(at + i)[4 * half + (n & 3)];
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t at = Mixed ? (i >> 2) * apart + 4 * g + (i & 3)
+                              : (g >> 1) * apart + 8 * (g & 1) + i;
+    v[i] = reinterpret_cast<const float *>(first + at + (n >> 2) * 16)[4 * half + (n & 3)];
+  }
   return v;
 }
 
@@ -225,8 +234,26 @@ __device__ __forceinline__ void lds_barrier() {
 // Stores to places of a buffer that begins anywhere (the same for the wave); those past its bytes,
 // kNowhere among them, do not happen.
 constexpr uint32_t kNowhere = 0xFFFFFFF0u;
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(void *p, uint32_t bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(p, 0, static_cast<int>(bytes), 0x00020000);
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void *p, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, static_cast<int>(bytes), 0x00020000);
+}
+// A lane's load from place `at` of a buffer, `further` (the same for the wave) behind it; 0 past the
+// buffer's end.
+template <typename V>
+__device__ __forceinline__ V load_from(__amdgpu_buffer_rsrc_t from, uint32_t at, uint32_t further) {
+  if constexpr (sizeof(V) == 2) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b16(from, at, further, 0));
+  } else if constexpr (sizeof(V) == 4) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b32(from, at, further, 0));
+  } else if constexpr (sizeof(V) == 16) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b128(from, at, further, 0));
+  } else {
+    struct Halves {
+      f32x4 low, high;
+    };
+    const Halves x = {load_from<f32x4>(from, at, further), load_from<f32x4>(from, at + 16, further)};
+    return __builtin_bit_cast(V, x);
+  }
 }
 template <typename V>
 __device__ __forceinline__ void store_to(__amdgpu_buffer_rsrc_t to, uint32_t at, V v) {
@@ -249,6 +276,86 @@ __device__ __forceinline__ void store_to(__amdgpu_buffer_rsrc_t to, uint32_t at,
     __builtin_amdgcn_raw_buffer_store_b128(x.high, to, at == kNowhere ? at : at + 16, 0, 0);
   }
 }
+
+// 64 rows of a head's keys or queries in shared memory, as they lie in memory: pieces of 16 bytes,
+// those of a row in an order by the row that lets 16 rows' same pieces come from different banks.
+// KT 0: none.
+template <typename T, int KT>
+struct RowTile {
+  static constexpr uint32_t per = 16 / sizeof(T), pieces = 32 * (KT == 0 ? 1 : KT) / per,
+                            span = KT == 3 ? 4 * pieces / 3 : pieces;
+  f32x4 piece[KT == 0 ? 1 : kChunk * span];
+  static __device__ __forceinline__ uint32_t place(uint32_t row, uint32_t piece) {
+    const uint32_t order = (row & 3) | ((row >> 1) & 12);
+    return row * span + (piece ^ (order * (sizeof(T) / 2) & (span - 1)));
+  }
+  // The operand of a sum over the keys: a lane its row, 8 keys of step s.
+  __device__ __forceinline__ operand<T> along(uint32_t row, int s, uint32_t g) const {
+    return *reinterpret_cast<const operand<T> *>(&piece[place(row, (4 * s + g) * 8 / per)]);
+  }
+  // The operand of a sum over the rows: a lane its key of a tile of 16, 8 rows of step s.
+  __device__ __forceinline__ operand<T> across(uint32_t tile, int s, uint32_t n, uint32_t g) const {
+    if constexpr (sizeof(T) == 2) {
+      s16x4 v[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const f32x4 *at = &piece[place(32 * s + 8 * g + 4 * e + (n >> 2), 4 * (tile >> 1) + (n & 3))];
+        v[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_s16x4 *)(reinterpret_cast<const s16x4 *>(at) + (tile & 1)));
+      }
+      return __builtin_bit_cast(
+          operand<T>, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      operand<T> v;
+      const uint32_t key = index_of(tile, n);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = piece[place(32 * s + 8 * g + i, key >> 2)][key & 3];
+      return v;
+    }
+  }
+};
+
+// The part of such a tile that one of 256 threads brings: by way of its registers, a load ahead.
+// Packed: 16 bytes at a time, else its elements. Rows past a chunk's and keys past the last are 0.
+template <typename T, int KT, bool Packed>
+struct RowPart {
+  using Tile = RowTile<T, KT>;
+  static constexpr int count = KT == 0 ? 1 : kChunk * Tile::pieces / 256;
+  struct Values {
+    f32x4 v[count];
+  };
+  uint32_t at[count], to[count];
+  __device__ __forceinline__ RowPart(uint32_t thread, uint32_t row_bytes, uint32_t keys) {
+#pragma unroll
+    for (int i = 0; i < count; ++i) {
+      const uint32_t id = 256 * i + thread, row = id / Tile::pieces, piece = id % Tile::pieces;
+      at[i] = piece * Tile::per < keys ? row * row_bytes + piece * 16 : kNowhere;
+      to[i] = Tile::place(row, piece);
+    }
+  }
+  __device__ __forceinline__ void load(Values &x, __amdgpu_buffer_rsrc_t from,
+                                       uint32_t keys) const {
+#pragma unroll
+    for (int i = 0; i < count; ++i) {
+      if constexpr (Packed) {
+        x.v[i] = load_from<f32x4>(from, at[i], 0);
+      } else {
+        typedef T part __attribute__((ext_vector_type(Tile::per)));
+        const uint32_t piece = (256 * i + threadIdx.x % 256) % Tile::pieces;
+        part y;
+#pragma unroll
+        for (uint32_t e = 0; e < Tile::per; ++e)
+          y[e] = load_from<T>(from, piece * Tile::per + e < keys ? at[i] + e * sizeof(T) : kNowhere,
+                              0);
+        x.v[i] = __builtin_bit_cast(f32x4, y);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(Tile &tile, const Values &x) const {
+#pragma unroll
+    for (int i = 0; i < count; ++i) tile.piece[to[i]] = x.v[i];
+  }
+};
 
 // exp of the decay's sums of a chunk: from its start (`since`), to its end (`until`), and b.
 struct Gates {

@@ -39,7 +39,7 @@ struct PrepareArgs {
   Dims d;
   const T *query, *key, *gate, *write;
   char *heads;  // Chunk<T> of (batch, head, chunk)
-  char *keys;   // operands of keys, queries and transposed keys of (batch, key head, chunk)
+  char *keys;   // operands of keys, queries and transposed keys of (batch, key head, chunk), or null
 };
 
 // A block per chunk and value head.
@@ -55,7 +55,8 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(PrepareArgs<T> a) {
   const T *query = a.query + at.key_row * d.keys;
   const uint64_t stride = static_cast<uint64_t>(d.key_heads) * d.keys;
   char *out = a.heads + at.head_chunk(d) * Chunk<T, P>::bytes;
-  const bool first_head = at.head % d.group == 0;  // brings what its key head's others share
+  // the first of a key head's value heads brings what they share
+  const bool copies = a.keys != nullptr && at.head % d.group == 0;
   Op *keys = reinterpret_cast<Op *>(a.keys) + at.key_chunk(d) * (12 * KT * 64) + lane;
   Op *queries = keys + 4 * KT * 64, *across = queries + 4 * KT * 64;
   solve<T, KT, Whole>(
@@ -68,7 +69,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(PrepareArgs<T> a) {
 #pragma unroll
           for (int s = 0; s < KT; ++s)
             q[s] = load_row<T, Whole>(query + min(t, at.rows - 1) * stride, 32 * s + 8 * g, d.keys);
-          if (first_head)
+          if (copies)
 #pragma unroll
             for (int s = 0; s < KT; ++s) queries[(ti * KT + s) * 64] = q[s];
           for (int step = 0; step <= static_cast<int>(ti >> 1); ++step) {
@@ -102,7 +103,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(PrepareArgs<T> a) {
     for (int q = 0; q < P; ++q)
       to[(p * P + q) * 64 + lane] = parts.part[q];
   }
-  if (!first_head) return;
+  if (!copies) return;
 #pragma unroll
   for (int s = 0; s < KT; ++s)
     keys[(wave * KT + s) * 64] = m.key_row(index_of(wave, n), s, g);
@@ -112,7 +113,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(PrepareArgs<T> a) {
 template <typename T>
 struct ScanArgs {
   Dims d;
-  const T *value;
+  const T *query, *key, *value;
   const char *heads, *keys;
   const float *from;  // states before the first chunk, null: 0
   float *to;          // and after the last, may be null
@@ -122,27 +123,35 @@ struct ScanArgs {
 };
 
 // What the block's waves hand each other, as operands: the state, b y, b e, exp(g_64 - g) b e, and e
-// for the backward.
+// for the backward; and a chunk's keys, queries and gates.
 template <typename T, int P, int KT, int C>
 struct Exchange {
   operand<T> state[KT][C][P][64], weighted[2][C][P][64], wrote[2][C][P][64], left[2][C][P][64],
       error[2][C][64];
+  Gates gates[2];                             // of the chunks with even and with odd numbers
+  RowTile<T, C == 2 ? KT : 0> keys[2], queries;  // where they are staged
 };
 
-// A block of four waves per C slabs of 16 columns of a head's values.  A wave takes 16 of a chunk's
-// steps and 32 of the keys: whatever stands on the left of a product (keys, queries, the chunk's
-// matrices) is one wave's alone and goes from memory to its registers, a chunk ahead, as soon as the
-// present chunk's is used; what stands on the right goes through shared memory, three times a
-// chunk.
-template <typename T, int P, int KT, int C>
-__global__ __launch_bounds__(256) void delta_scan_kernel(ScanArgs<T> a) {
+// A block of eight waves per C slabs of 16 columns of a head's values.  Each holds 16 of the keys;
+// the first four follow the errors of 16 of a chunk's steps each, the others form those steps'
+// outputs beside them, a stage behind.  What they form of each other's products goes through shared
+// memory, three times a chunk; what stands on the left of a product, or here of its transpose, is
+// one wave's alone, and is loaded a chunk ahead, as soon as the present chunk's is used.  The chunk's
+// matrices go straight to registers.  So do keys and queries with one slab, as operands that were
+// prepared: few blocks are as fast as a chunk's way through one.  Blocks of two slabs stage their
+// rows in shared memory, where the sums over the keys and those over the steps both find their
+// operands: of many blocks the bytes count, a third less without the copies.
+template <typename T, int P, int KT, int C, bool Packed>
+__global__ __launch_bounds__(512, Packed && sizeof(T) == 2 && C == 2 && P == 1 ? 4 : 2) void delta_scan_kernel(
+    ScanArgs<T> a) {
   using Op = operand<T>;
   using Kept = Chunk<T, P>;
   __shared__ Exchange<T, P, KT, C> m;
   const Dims &d = a.d;
   const uint32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-  const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = w & 1;
-  const int pair = w >> 1;  // of tiles of 16 steps: an operand of 32
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
+  const bool errs = wave < 4;
+  const int pair = w >> 1, half = w & 1;  // of tiles of 16 steps: an operand of 32
   // blocks of a head share what they read: on one XCD
   const oxh::BlockTile block = oxh::xcd_block();
   const uint32_t h = block.y, b = block.z, kh = h / d.group;
@@ -156,130 +165,65 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(ScanArgs<T> a) {
   T *outs = a.out + row0 * value_stride + static_cast<uint64_t>(h) * d.values;
   const char *chunks = a.heads + head * d.chunks * Kept::bytes;
   constexpr uint32_t kOperand = 64 * sizeof(Op), kKeys = 4 * KT * kOperand;
-  const char *keys =
+  constexpr bool kStaged = C == 2;
+  const char *copies =
       a.keys + (static_cast<uint64_t>(b) * d.key_heads + kh) * d.chunks * (3 * kKeys);
-  uint32_t cols[C];  // this lane's; those past the last are the last again, and not stored
-  bool in[C];
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const uint32_t column = 16 * (block.x * C + c) + n;
-    in[c] = column < d.values;
-    cols[c] = in[c] ? column : d.values - 1;
-  }
+  const uint32_t value_bytes = static_cast<uint32_t>(value_stride * sizeof(T));
+  // A lane's columns: of two slabs those that make its 4 rows of two results 8 in sequence.
+  auto column_of = [&](int c, uint32_t n) {
+    return C == 2 ? 32 * block.x + index_of(c, n) : 16 * block.x + n;
+  };
+  constexpr uint32_t kValue = sizeof(T);
   auto rows_of = [&](uint32_t chunk) -> uint32_t {
     return min(length - start - chunk * kChunk, static_cast<uint32_t>(kChunk));
   };
-  const bool holds = w < KT;  // keys 32 w on
+  const uint32_t tile = wave ^ 4;  // of 16 keys: half an operand
+  const bool holds = tile < 2 * KT;
   const uint64_t state_at = head * d.keys * d.values;
-  auto key_at = [&](int tile, int r) { return 32 * w + index_of(tile, 4 * g + r); };
-  f32x4 state[2][C];
+  auto key_at = [&](int r) { return index_of(tile, 4 * g + r); };
+  f32x4 state[C];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      state[i][c] = f32x4{};
-      if (a.from == nullptr || !holds) continue;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const uint32_t k = key_at(i, r), there = min(k, d.keys - 1);
-        const float v = a.from[state_at + static_cast<uint64_t>(there) * d.values + cols[c]];
-        state[i][c][r] = k < d.keys ? v : 0.0f;
-      }
-    }
-
-  // The left operands of a chunk's four products and its values, each loaded where the chunk before
-  // has used its own (not before: their registers are the same).  No load or store of the loop is behind a branch, so that each use waits for
-  // its own loads alone: the last chunk loads itself again, and stores that are not to be go past
-  // their buffer's end.
-  Op key[KT], query[KT], solve[2][P], scores[2], back[2][2];
-  T value[C][4];
-  f32x4 since, until, write;
-  float whole = 0.0f;
-  const uint32_t value_bytes = static_cast<uint32_t>(value_stride * sizeof(T));
-  const uint32_t lane_at = lane * sizeof(Op);
-  auto load_keys = [&](uint32_t chunk) {
-    const char *from = keys + (chunk * uint64_t{3 * kKeys} + w * (KT * kOperand));
-#pragma unroll
-    for (int s = 0; s < KT; ++s) key[s] = load_at<Op>(from + s * kOperand, lane_at);
-#pragma unroll
-    for (int s = 0; s < KT; ++s) query[s] = load_at<Op>(from + kKeys + s * kOperand, lane_at);
-  };
-  auto load_values = [&](uint32_t chunk) {
-    const uint32_t last = rows_of(chunk) - 1;
-    const char *from = reinterpret_cast<const char *>(values + chunk * kChunk * value_stride);
+  for (int c = 0; c < C; ++c) {
+    state[c] = f32x4{};
+    if (a.from == nullptr || !holds) continue;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const uint32_t row = min(index_of(w, 4 * g + r), last) * value_bytes;
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-        value[c][r] = load_at<T>(from, row + cols[c] * static_cast<uint32_t>(sizeof(T)));
+      const uint32_t k = key_at(r), there = min(k, d.keys - 1);
+      const float v = a.from[state_at + static_cast<uint64_t>(there) * d.values +
+                             min(column_of(c, n), d.values - 1)];
+      state[c][r] = k < d.keys ? v : 0.0f;
     }
+  }
+
+  // No load or store of the loop is behind a branch, so that each use waits for its own loads alone:
+  // the last chunk loads itself again, and stores that are not to be go past their buffer's end.
+  const uint32_t lane_at = lane * sizeof(Op);
+  Op back[2];
+  auto load_copies = [&](uint32_t chunk, uint32_t part, auto &to, uint32_t first) {
+    const auto from = buffer_of(copies + (chunk * uint64_t{3 * kKeys} + part * kKeys), kKeys);
+#pragma unroll
+    for (uint32_t s = 0; s < sizeof(to) / sizeof(Op); ++s)
+      to[s] = load_from<Op>(from, lane_at, (first + s) * kOperand);
   };
+  auto load_back = [&](uint32_t chunk) { load_copies(chunk, 2, back, 2 * min(tile, 2 * KT - 1u)); };
   auto operands_of = [&](uint32_t chunk, uint64_t part) {
-    return chunks + (chunk * Kept::bytes + part);
-  };
-  auto load_system = [&](uint32_t chunk) {
-    const char *from = operands_of(chunk, Kept::system);
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int p = 0; p < P; ++p)
-        solve[s][p] =
-            load_at<Op>(from + (lower_place(w, min(s, pair)) * P + p) * kOperand, lane_at);
-  };
-  auto load_rest = [&](uint32_t chunk) {
-    whole = load_at<float>(operands_of(chunk, Kept::gates) + offsetof(Gates, since),
-                           (kChunk - 1) * 4);
-    const char *from = operands_of(chunk, Kept::within);
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-      scores[s] = load_at<Op>(from + lower_place(w, min(s, pair)) * kOperand, lane_at);
-    const char *k = keys + (chunk * uint64_t{3 * kKeys} + 2 * kKeys + 4 * min(w, KT - 1u) * kOperand);
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-        back[i][s] = load_at<Op>(k + (2 * i + s) * kOperand, lane_at);
-  };
-  auto load_gates = [&](uint32_t chunk) {
-    const char *gates = operands_of(chunk, Kept::gates);
-    const uint32_t at = index_of(w, 4 * g) * 4;
-    since = load_at<f32x4>(gates + offsetof(Gates, since), at);
-    until = load_at<f32x4>(gates + offsetof(Gates, until), at);
-    write = load_at<f32x4>(gates + offsetof(Gates, write), at);
+    return buffer_of(chunks + (chunk * Kept::bytes + part),
+                     static_cast<uint32_t>(Kept::bytes - part));
   };
   typedef T quarter __attribute__((ext_vector_type(4)));
-  // a wave's half of an operand that two waves form, and the state's, which is its own
-  auto hand = [&](Op(&to)[P][64], f32x4 v) {
+  // a wave's half of an operand that two waves form
+  auto hand = [&](Op(&to)[P][64], f32x4 v, uint32_t half) {
 #pragma unroll
     for (int p = 0; p < P; ++p) {
       const quarter q = __builtin_convertvector(v, quarter);
       reinterpret_cast<quarter *>(&to[p][lane])[half] = q;
-      if (p + 1 < P) v -= __builtin_convertvector(q, f32x4);
+      if (p + 1 < P) v -= widened(q);
     }
   };
-  // what the backward reads of a chunk; a block of one slab brings its half of the pair's lanes
-  const uint32_t kept = (d.slabs + 1) / 2 * (2 * KT + 4) * kOperand;
-  auto saved_of = [&](uint32_t chunk) {
-    return buffer_of(a.saved + ((head * a.all + d.first + chunk) * kept), a.saved == nullptr ? 0 : kept);
-  };
-  const bool brings = C == 2 || (g >> 1) == (block.x & 1);
-  auto saved_at = [&](int place) {
-    return brings ? (block.x * C / 2 * (2 * KT + 4) + place) * kOperand + lane_at : kNowhere;
-  };
-  auto hand_state = [&](uint32_t chunk) {
+  auto hand_state = [&] {
     if (KT < 4 && !holds) return;
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const Split<T, P> st(join(state[0][c], state[1][c]));
-#pragma unroll
-      for (int p = 0; p < P; ++p) m.state[w][c][p][lane] = st.part[p];
-    }
-    if (a.saved == nullptr) return;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      store_to(saved_of(chunk), saved_at(2 * w + i),
-               turned(&m.state[w][0][0][0], C == 2 ? P * 64 : 0, i, n, g));
+    for (int c = 0; c < C; ++c) hand(m.state[tile >> 1][c], state[c], tile & 1);
   };
   // right operands of 64 steps, all of them on their way before the first is used
   auto read_pairs = [&](Op(&to)[2][C][P], const Op(&from)[2][C][P][64]) {
@@ -291,143 +235,340 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(ScanArgs<T> a) {
         for (int p = 0; p < P; ++p) to[s][c][p] = from[s][c][p][lane];
     __builtin_amdgcn_sched_barrier(0);
   };
-  if (live != 0) {
-    load_keys(0);
-    load_values(0);
-    load_gates(0);
-    load_system(0);
-    load_rest(0);
-    hand_state(0);
-  }
-  for (uint32_t chunk = 0; chunk < live; ++chunk) {
-    const uint32_t next = min(chunk + 1, live - 1);
-    lds_barrier();
-    f32x4 y[C] = {}, o[C] = {};
-    {
-      Op right[KT][C][P];
+  // S = exp(g_64) S0 + k' (exp(g_64 - g) b e)
+  auto advance = [&](uint32_t chunk) {
+    if (KT == 4 || holds) {
+      Op left[2][C][P];
+      const float whole = m.gates[chunk & 1].since[kChunk - 1];
+      if constexpr (kStaged)
 #pragma unroll
-      for (int s = 0; s < KT; ++s)
+        for (int s = 0; s < 2; ++s) back[s] = m.keys[chunk & 1].across(tile, s, n, g);
+      read_pairs(left, m.left);
 #pragma unroll
-        for (int c = 0; c < C; ++c)
+      for (int c = 0; c < C; ++c) state[c] *= whole;
 #pragma unroll
-          for (int p = 0; p < P; ++p) right[s][c][p] = m.state[s][c][p][lane];
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int s = 0; s < KT; ++s) {
+      for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int p = P - 1; p >= 0; --p)
 #pragma unroll
-          for (int c = 0; c < C; ++c) y[c] = product(key[s], right[s][c][p], y[c]);
+          for (int c = 0; c < C; ++c) state[c] = product(back[s], left[s][c][p], state[c]);
+    }
+    if constexpr (!kStaged) {
+      __builtin_amdgcn_sched_barrier(0);
+      load_back(min(chunk + 1, live - 1));
+    }
+    hand_state();
+  };
+  // a lane's 4 steps
+  auto gates_of = [&](uint32_t chunk, float(Gates::*which)[kChunk]) {
+    return *reinterpret_cast<const f32x4 *>(&(m.gates[chunk & 1].*which)[index_of(w, 4 * g)]);
+  };
+  if (live != 0) {
+    if constexpr (!kStaged) load_back(0);
+    hand_state();
+  }
+  if (errs) {
+    Op key[KT], solve[2][P];
+    // the values: a lane its columns of 4 steps, or in a row's order 8 columns of a step, which a
+    // product with columns of the identity brings there
+    constexpr bool kRows = Packed && sizeof(T) == 2 && kStaged;
+    T value[C][4];
+    Op row, unit[C];
+    uint32_t at[C][4], row_at = kNowhere;
+    if constexpr (kRows) {
+      const uint32_t first = 32 * (C == 2 ? block.x : block.x >> 1) + 8 * g;
+      if (first < d.values) row_at = index_of(w, n) * value_bytes + first * kValue;
 #pragma unroll
-        for (int c = 0; c < C; ++c) o[c] = product(query[s], right[s][c][0], o[c]);
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i)
+          unit[c][i] = static_cast<T>(first + i == column_of(c, n) ? 1.0f : 0.0f);
+    } else {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          at[c][r] = column_of(c, n) < d.values
+                         ? index_of(w, 4 * g + r) * value_bytes + column_of(c, n) * kValue
+                         : kNowhere;
+    }
+    auto read_keys = [&](uint32_t chunk) {
+      if constexpr (kStaged) {
+#pragma unroll
+        for (int s = 0; s < KT; ++s) key[s] = m.keys[chunk & 1].along(index_of(w, n), s, g);
+      } else {
+        load_copies(chunk, 0, key, w * KT);
       }
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    load_keys(next);
+    };
+    auto load_values = [&](uint32_t chunk) {
+      const auto from = buffer_of(values + chunk * kChunk * value_stride,
+                                  rows_of(chunk) * value_bytes);
+      if constexpr (kRows) {
+        row = load_from<Op>(from, row_at, 0);
+      } else {
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      f32x4 v;
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = widen(value[c][r]);
-      y[c] = v - since * y[c];
-      o[c] *= since * d.scale;
-      hand(m.weighted[pair][c], -write * y[c]);
+          for (int c = 0; c < C; ++c) value[c][r] = load_from<T>(from, at[c][r], 0);
+      }
+    };
+    auto load_system = [&](uint32_t chunk) {
+      const auto from = operands_of(chunk, Kept::system);
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+          solve[s][p] =
+              load_from<Op>(from, lane_at, (lower_place(w, min(s, pair)) * P + p) * kOperand);
+    };
+    if (live != 0) {
+      load_values(0);
+      load_system(0);
+      if constexpr (kStaged) lds_barrier();
+      read_keys(0);
     }
-    __builtin_amdgcn_sched_barrier(0);
-    load_values(next);
-    lds_barrier();
-    // e = y - N (b y)
-    {
-      Op right[2][C][P];
-      read_pairs(right, m.weighted);
+    for (uint32_t chunk = 0; chunk < live; ++chunk) {
+      const uint32_t next = min(chunk + 1, live - 1);
+      lds_barrier();
+      f32x4 y[C] = {}, v[C] = {};
+      {
+        Op right[KT][C][P];
+#pragma unroll
+        for (int s = 0; s < KT; ++s)
+#pragma unroll
+          for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int p = 0; p < P; ++p) right[s][c][p] = m.state[s][c][p][lane];
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int s = 0; s < KT; ++s)
+#pragma unroll
+          for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+            for (int c = 0; c < C; ++c) y[c] = product(key[s], right[s][c][p], y[c]);
+        if constexpr (kRows)
+#pragma unroll
+          for (int c = 0; c < C; ++c) v[c] = product(row, unit[c], v[c]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (!kStaged) read_keys(next);
+      const f32x4 since = gates_of(chunk, &Gates::since), write = gates_of(chunk, &Gates::write);
+      const f32x4 until = gates_of(chunk, &Gates::until);
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        if constexpr (!kRows)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[c][r] = widen(value[c][r]);
+        y[c] = v[c] - since * y[c];
+        hand(m.weighted[pair][c], -write * y[c], half);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      load_values(next);
+      lds_barrier();
+      // e = y - N (b y)
+      {
+        Op right[2][C][P];
+        read_pairs(right, m.weighted);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          if (s > pair) continue;
+#pragma unroll
+          for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+            for (int q = P - 1 - p; q >= 0; --q)
+#pragma unroll
+              for (int c = 0; c < C; ++c) y[c] = product(solve[s][p], right[s][c][q], y[c]);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      load_system(next);
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        if (a.saved != nullptr)
+          reinterpret_cast<quarter *>(&m.error[pair][c][lane])[half] =
+              __builtin_convertvector(y[c], quarter);
+        y[c] *= write;
+        hand(m.left[pair][c], until * y[c], half);
+        hand(m.wrote[pair][c], y[c], half);
+      }
+      lds_barrier();
+      if constexpr (kStaged) read_keys(next);
+      advance(chunk);
+    }
+  } else {
+    Op scores[2], query[KT];
+    f32x4 o[C] = {}, gates;  // and 4 of a chunk's gates, a lane
+    const uint32_t row_bytes = d.key_heads * d.keys * kValue;
+    using Part = RowPart<T, kStaged ? KT : 0, Packed>;
+    const Part part(threadIdx.x - 256, row_bytes, d.keys);
+    typename Part::Values key_part, query_part;
+    const uint64_t key_row0 = (row0 * d.key_heads + kh) * d.keys;
+    auto load_rows = [&](typename Part::Values &to, const T *from, uint32_t chunk) {
+      part.load(to, buffer_of(from + key_row0 + chunk * kChunk * static_cast<uint64_t>(d.key_heads) * d.keys,
+                              rows_of(chunk) * row_bytes), d.keys);
+    };
+    auto load_scores = [&](uint32_t chunk) {
+      const auto from = operands_of(chunk, Kept::within);
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        scores[s] = load_from<Op>(from, lane_at, lower_place(w, min(s, pair)) * kOperand);
+    };
+    // The outputs are formed transposed: a lane a step, its columns in sequence.
+    const uint32_t step = index_of(w, n), first = column_of(0, 4 * g);
+    // what the backward reads of a chunk; a block of one slab brings its half of the pair's lanes
+    const uint32_t kept = (d.slabs + 1) / 2 * (2 * KT + 4) * kOperand;
+    const bool brings = C == 2 || (g >> 1) == (block.x & 1);
+    auto saved_of = [&](uint32_t chunk, bool there) {
+      return buffer_of(a.saved + ((head * a.all + d.first + chunk) * kept), there ? kept : 0);
+    };
+    auto saved_at = [&](int place) {
+      return brings ? (block.x * C / 2 * (2 * KT + 4) + place) * kOperand + lane_at : kNowhere;
+    };
+    // o = exp(g) q S0 + (G o q k') (b e) of a chunk, the first part there
+    Op wrote[2][C][P];
+    auto finish = [&](uint32_t chunk, bool there) {
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         if (s > pair) continue;
 #pragma unroll
         for (int p = P - 1; p >= 0; --p)
 #pragma unroll
-          for (int q = P - 1 - p; q >= 0; --q)
-#pragma unroll
-            for (int c = 0; c < C; ++c) y[c] = product(solve[s][p], right[s][c][q], y[c]);
+          for (int c = 0; c < C; ++c) o[c] = product(wrote[s][c][p], scores[s], o[c]);
       }
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    load_system(next);
+      const auto to = buffer_of(outs + chunk * kChunk * value_stride,
+                                there ? rows_of(chunk) * value_bytes : 0);
+      const uint32_t at = step * value_bytes + first * kValue;
+      if constexpr (Packed && C == 2) {
+        store_to(to, first < d.values ? at : kNowhere, rounded<T>(join(o[0], o[1])));
+      } else {
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
+        for (int c = 0; c < C; ++c) {
+          if constexpr (Packed) {
+            store_to(to, first < d.values ? at : kNowhere, __builtin_convertvector(o[c], quarter));
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              store_to(to, first + 4 * c + r < d.values ? at + (4 * c + r) * kValue : kNowhere,
+                       static_cast<T>(o[c][r]));
+          }
+        }
+      }
+    };
+    auto load_gates = [&](uint32_t chunk) {
+      gates = load_from<f32x4>(buffer_of(chunks + (chunk * Kept::bytes + Kept::gates), sizeof(Gates)),
+                               lane * 16, 0);
+    };
+    auto hand_gates = [&](uint32_t chunk) {
+      if (w == 0 && lane < sizeof(Gates) / 16)
+        reinterpret_cast<f32x4 *>(&m.gates[chunk & 1])[lane] = gates;
+      __builtin_amdgcn_sched_barrier(0);
+      load_gates(min(chunk + 1, live - 1));
+    };
+    // the errors of a chunk for the backward
+    auto save_errors = [&](uint32_t chunk, bool there) {
       if (a.saved != nullptr)
-        reinterpret_cast<quarter *>(&m.error[pair][c][lane])[half] =
-            __builtin_convertvector(y[c], quarter);
-      y[c] *= write;
-      hand(m.wrote[pair][c], y[c]);
-      hand(m.left[pair][c], until * y[c]);
+        store_to(saved_of(chunk, there), saved_at(2 * KT + w),
+                 turned<C == 2>(&m.error[pair][0][0], C == 2 ? 64 : 0, half, n, g));
+    };
+    if (live != 0) {
+      load_scores(0);
+      load_gates(0);
+      if constexpr (kStaged) {
+        load_rows(key_part, a.key, 0);
+        part.store(m.keys[0], key_part);
+        __builtin_amdgcn_sched_barrier(0);
+        load_rows(key_part, a.key, min(1u, live - 1));
+        load_rows(query_part, a.query, 0);
+      } else {
+        load_copies(0, 1, query, w * KT);
+      }
+      hand_gates(0);
+      if constexpr (kStaged) lds_barrier();
     }
-    __builtin_amdgcn_sched_barrier(0);
-    load_gates(next);
-    lds_barrier();
-    // o = exp(g) q S0 + (G o q k') (b e);  S = exp(g_64) S0 + k' (exp(g_64 - g) b e)
-    Op left[2][C][P], wrote[2][C][P];
-    read_pairs(left, m.left);
-    read_pairs(wrote, m.wrote);
-    if (KT == 4 || holds) {
+    for (uint32_t chunk = 0; chunk < live; ++chunk) {
+      lds_barrier();
+      // the chunk before's outputs, while the others form this one's errors; before the first one
+      // nothing is there
+      const uint32_t before = max(chunk, 1u) - 1, next = min(chunk + 1, live - 1);
+      read_pairs(wrote, m.wrote);
+      if constexpr (kStaged) {
+        part.store(m.queries, query_part);
+        part.store(m.keys[(chunk + 1) & 1], key_part);
+        __builtin_amdgcn_sched_barrier(0);
+        load_rows(query_part, a.query, next);
+        load_rows(key_part, a.key, min(chunk + 2, live - 1));
+      } else {
+        finish(before, chunk != 0);
+        __builtin_amdgcn_sched_barrier(0);
+        load_scores(chunk);
+      }
+      save_errors(before, chunk != 0);
+      if (a.saved != nullptr && w < KT) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i)
+          store_to(saved_of(chunk, true), saved_at(2 * w + i),
+                   turned<C == 2>(&m.state[w][0][0][0], C == 2 ? P * 64 : 0, i, n, g));
+      }
+      lds_barrier();
+      if constexpr (kStaged) {
+        finish(before, chunk != 0);
+        __builtin_amdgcn_sched_barrier(0);
+        load_scores(chunk);
+      }
 #pragma unroll
-        for (int c = 0; c < C; ++c) state[i][c] *= whole;
+      for (int c = 0; c < C; ++c) o[c] = f32x4{};
+      constexpr int kAtOnce = kStaged && KT == 4 ? 2 : KT;  // more would leave registers for one block alone
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+      for (int from = 0; from < KT; from += kAtOnce) {
+        Op right[kAtOnce][C];
 #pragma unroll
-        for (int p = P - 1; p >= 0; --p)
+        for (int s = 0; s < kAtOnce; ++s) {
+          if constexpr (kStaged) query[from + s] = m.queries.along(step, from + s, g);
 #pragma unroll
-          for (int c = 0; c < C; ++c)
+          for (int c = 0; c < C; ++c) right[s][c] = m.state[from + s][c][0][lane];
+        }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) state[i][c] = product(back[i][s], left[s][c][p], state[i][c]);
+        for (int s = 0; s < kAtOnce; ++s)
+#pragma unroll
+          for (int c = 0; c < C; ++c) o[c] = product(right[s][c], query[from + s], o[c]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      const float since = m.gates[chunk & 1].since[step] * d.scale;
+#pragma unroll
+      for (int c = 0; c < C; ++c) o[c] *= since;
+      if constexpr (!kStaged) {
+        __builtin_amdgcn_sched_barrier(0);
+        load_copies(next, 1, query, w * KT);
+      }
+      lds_barrier();
+      advance(chunk);
+      hand_gates(chunk + 1);
     }
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      if (s > pair) continue;
-#pragma unroll
-      for (int p = P - 1; p >= 0; --p)
-#pragma unroll
-        for (int c = 0; c < C; ++c) o[c] = product(scores[s], wrote[s][c][p], o[c]);
+    if (live != 0) {
+      read_pairs(wrote, m.wrote);
+      save_errors(live - 1, true);
+      finish(live - 1, true);
     }
-    if (a.saved != nullptr)
-      store_to(saved_of(chunk), saved_at(2 * KT + w),
-               turned(&m.error[pair][0][0], C == 2 ? 64 : 0, half, n, g));
-    __builtin_amdgcn_sched_barrier(0);
-    load_rest(next);
-    const uint32_t rows = rows_of(chunk);
-    const auto to = buffer_of(outs + chunk * kChunk * value_stride, kChunk * value_bytes);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const uint32_t t = index_of(w, 4 * g + r);
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-        store_to(to, t < rows && in[c]
-                         ? t * value_bytes + cols[c] * static_cast<uint32_t>(sizeof(T))
-                         : kNowhere,
-                 static_cast<T>(o[c][r]));
-    }
-    if (chunk + 1 < live) hand_state(chunk + 1);
   }
   // steps past the row's end
   const uint32_t end = min(d.time - start, d.chunks * kChunk);
-  for (uint32_t t = (length <= start ? 0 : length - start) + 4 * w + g; t < end; t += 16) {
+  for (uint32_t t = (length <= start ? 0 : length - start) + 4 * wave + g; t < end; t += 32) {
 #pragma unroll
     for (int c = 0; c < C; ++c)
-      if (in[c]) outs[t * value_stride + cols[c]] = static_cast<T>(0.0f);
+      if (column_of(c, n) < d.values)
+        outs[t * value_stride + column_of(c, n)] = static_cast<T>(0.0f);
   }
   if (a.to == nullptr || !holds) return;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int r = 0; r < 4; ++r) {
+    const uint32_t k = key_at(r);
+    if (k >= d.keys) continue;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const uint32_t k = key_at(i, r);
-      if (k >= d.keys) continue;
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-        if (in[c]) a.to[state_at + static_cast<uint64_t>(k) * d.values + cols[c]] = state[i][c][r];
-    }
+    for (int c = 0; c < C; ++c)
+      if (column_of(c, n) < d.values)
+        a.to[state_at + static_cast<uint64_t>(k) * d.values + column_of(c, n)] = state[c][r];
+  }
 }
 
 template <typename T>
@@ -556,12 +697,15 @@ constexpr uint64_t kStepLimit = 16;
 template <typename T, int P>
 struct ForwardPlan {
   Plan p;
+  bool two;                                     // slabs of a block of the scan
   uint64_t head_bytes, key_bytes, state_bytes;  // of the workspace
   uint64_t bytes() const { return head_bytes + key_bytes + state_bytes; }
   ForwardPlan(const oxh_delta_shape &s, float scale, const int32_t *lengths)
       : p(s, scale, lengths) {
     const uint64_t head = s.batch * s.heads * Chunk<T, P>::bytes;
-    const uint64_t key = s.batch * s.key_heads * p.steps * 12 * kOperandBytes<T>;
+    // as many as leave a block for each compute unit
+    two = s.batch * s.heads * ((p.d.slabs + 1) / 2) >= oxh::kComputeUnits;
+    const uint64_t key = two ? 0 : s.batch * s.key_heads * p.steps * 12 * kOperandBytes<T>;
     p.divide(head + key);
     head_bytes = round_up(p.segment * head, 256);
     key_bytes = round_up(p.segment * key, 256);
@@ -591,31 +735,37 @@ oxh_status by_chunks(hipStream_t stream, const ForwardPlan<T, P> &plan, const T 
                      const T *gate, const T *write, const float *initial, T *out, float *final,
                      char *saved, char *workspace) {
   const Plan &p = plan.p;
-  char *heads = workspace, *keys = heads + plan.head_bytes;
-  float *between = reinterpret_cast<float *>(keys + plan.key_bytes);
-  // slabs of a block: as many as leave a block for each compute unit
-  const uint64_t all_heads = static_cast<uint64_t>(p.d.batch) * p.d.heads;
+  char *heads = workspace, *keys = plan.two ? nullptr : heads + plan.head_bytes;
+  float *between = reinterpret_cast<float *>(heads + plan.head_bytes + plan.key_bytes);
   const uint32_t pairs = (p.d.slabs + 1) / 2;
-  const bool two = all_heads * pairs >= oxh::kComputeUnits;
+  // whether 16 bytes of a row are loaded and stored at once
+  const bool packed = p.d.values % (16 / sizeof(T)) == 0 && p.d.keys % (16 / sizeof(T)) == 0 &&
+                      oxh::aligned16(query) && oxh::aligned16(key) && oxh::aligned16(value) &&
+                      oxh::aligned16(out);
   for (uint64_t first = 0; first < p.all; first += p.segment) {
     Dims d = p.d;
     d.first = static_cast<uint32_t>(first);
     d.chunks = static_cast<uint32_t>(std::min(p.segment, p.all - first));
     const bool last = first + p.segment >= p.all;
     const PrepareArgs<T> prepare{d, query, key, gate, write, heads, keys};
-    const ScanArgs<T> scan{d, value, heads, keys, first == 0 ? initial : between,
+    const ScanArgs<T> scan{d, query, key, value, heads, keys, first == 0 ? initial : between,
                            last ? final : between, out, saved, static_cast<uint32_t>(p.all)};
     with_keys(d.keys, d.keys % 32 == 0, [&](auto steps, auto whole) {
       constexpr int KT = decltype(steps)::value;
       constexpr bool W = decltype(whole)::value;
       oxh::launch(delta_prepare_kernel<T, P, KT, W>, dim3(d.chunks, d.heads, d.batch), dim3(256), 0,
                   stream, prepare);
-      if (two)
-        oxh::launch(delta_scan_kernel<T, P, KT, 2>, dim3(pairs, d.heads, d.batch), dim3(256), 0,
-                    stream, scan);
-      else
-        oxh::launch(delta_scan_kernel<T, P, KT, 1>, dim3(2 * pairs, d.heads, d.batch), dim3(256), 0,
-                    stream, scan);
+      auto go = [&](auto columns, auto packs) {
+        constexpr int C = decltype(columns)::value;
+        oxh::launch(delta_scan_kernel<T, P, KT, C, decltype(packs)::value>,
+                    dim3(2 / C * pairs, d.heads, d.batch), dim3(512), 0, stream, scan);
+      };
+      auto slabs = [&](auto packs) {
+        if (plan.two) go(std::integral_constant<int, 2>(), packs);
+        else go(std::integral_constant<int, 1>(), packs);
+      };
+      if (packed) slabs(std::true_type());
+      else slabs(std::false_type());
     });
     oxh_status st = oxh::launched("gated_delta_rule");
     if (st != OXH_OK) return st;

@@ -279,7 +279,7 @@ __global__ __launch_bounds__(256) void delta_backward_scan_kernel(Args<T> a) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
       store_to(pairs_at(chunk), pair_at(2 * w + i),
-               turned(&m.state[w][0][0], C == 2 ? 64 : 0, i, n, g));
+               turned<false>(&m.state[w][0][0], C == 2 ? 64 : 0, i, n, g));
   };
   auto read_pairs = [&](Op(&to)[2][C], const Op(&from)[2][C][64]) {
 #pragma unroll
@@ -390,7 +390,7 @@ __global__ __launch_bounds__(256) void delta_backward_scan_kernel(Args<T> a) {
           for (int i = 0; i < 2; ++i) ds[i][c] = product(back[i][s], taken[s][c], ds[i][c]);
     }
     store_to(pairs_at(chunk), pair_at(2 * KT + w),
-             turned(&m.x[pair][0][0], C == 2 ? 64 : 0, half, n, g));
+             turned<false>(&m.x[pair][0][0], C == 2 ? 64 : 0, half, n, g));
     __builtin_amdgcn_sched_barrier(0);
     load_rest(next);
     if (chunk != 0) hand_state(next);
