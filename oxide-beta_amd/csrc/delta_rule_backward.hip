@@ -56,7 +56,8 @@ struct Args {
   Dims d;
   const T *query, *key, *gate, *write, *gradient;
   const char *saved;
-  char *heads, *keys;   // Back<T> of (batch, head, chunk); keys, their transpose, queries' transpose
+  char *heads, *keys;   // Back<T> of (batch, head, chunk); keys, their transpose, queries' transpose,
+                        // or null
   const float *from;    // gradients of the states behind the launch's chunks, null: 0
   float *to;            // and before them, may be null
   T *dquery, *dkey, *dvalue, *dgate, *dwrite;
@@ -110,7 +111,7 @@ __global__ __launch_bounds__(256) void delta_backward_prepare_kernel(Args<T> a) 
     for (int j = 0; j < 8; ++j) v[j] = m.mat[32 * step + 8 * g + j][i];
     reinterpret_cast<Op *>(out + Back<T>::system)[p * 64 + lane] = rounded<T>(v);
   }
-  if (at.head % d.group != 0) return;
+  if (a.keys == nullptr || at.head % d.group != 0) return;
   Op *to = reinterpret_cast<Op *>(a.keys) + at.key_chunk(d) * (12 * KT * 64);
 #pragma unroll
   for (int s = 0; s < KT; ++s)
@@ -131,26 +132,29 @@ __device__ __forceinline__ float row_total(float v) {
   return v;
 }
 
-// What the block's waves hand each other, as operands: dS, do and scale exp(g) do (of this chunk and
-// the next), -b du, -exp(g) dv, and
-// x for the products.
+// What the block's waves hand each other, as operands: dS, do, scale exp(g) do, -b du, -exp(g) dv, x
+// for the products and dv; and a chunk's keys (of those with even and with odd numbers) and queries
+// where they are staged.
 template <typename T, int KT, int C>
 struct Exchange {
-  operand<T> state[KT][C][64], out[2][2][C][64], decayed[2][2][C][64], weighted[2][C][64],
-      taken[2][C][64], x[2][C][64];
+  operand<T> state[KT][C][64], out[2][C][64], decayed[2][C][64], weighted[2][C][64],
+      taken[2][C][64], x[2][C][64], dv[2][C][64];
+  RowTile<T, C == 2 ? KT : 0> keys[2], queries;
 };
 
-// A block of four waves per C slabs of 16 columns of a head's values, from the last chunk to the
-// first; the waves share a chunk as the forward's do.
-template <typename T, int KT, int C>
-__global__ __launch_bounds__(256) void delta_backward_scan_kernel(Args<T> a) {
+// A block of eight waves per C slabs of 16 columns of a head's values, from the last chunk to the
+// first.  They share a chunk as the forward's do: each holds 16 of the keys, the first four follow x,
+// the others bring the rows and do, and store what a chunk leaves a stage behind.
+template <typename T, int KT, int C, bool Packed>
+__global__ __launch_bounds__(512, Packed && sizeof(T) == 2 && C == 2 ? 4 : 2) void
+delta_backward_scan_kernel(Args<T> a) {
   using Op = operand<T>;
   using Kept = Back<T>;
   __shared__ Exchange<T, KT, C> m;
   const Dims &d = a.d;
   const uint32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-  const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = w & 1;
-  const int pair = w >> 1;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
+  const int pair = w >> 1, half = w & 1;
   const oxh::BlockTile block = oxh::xcd_block();
   const uint32_t h = block.y, b = block.z, kh = h / d.group;
   const uint32_t length = length_of(d, b), start = d.first * kChunk;
@@ -158,128 +162,69 @@ __global__ __launch_bounds__(256) void delta_backward_scan_kernel(Args<T> a) {
       length <= start ? 0 : min((length - start + kChunk - 1) / kChunk, d.chunks);
   const uint64_t head = static_cast<uint64_t>(b) * d.heads + h;
   const uint64_t value_stride = static_cast<uint64_t>(d.heads) * d.values;
-  const uint64_t value0 = (static_cast<uint64_t>(b) * d.time + start) * value_stride +
-                          static_cast<uint64_t>(h) * d.values;
+  const uint64_t row0 = static_cast<uint64_t>(b) * d.time + start;
+  const uint64_t value0 = row0 * value_stride + static_cast<uint64_t>(h) * d.values;
   const T *gradients = a.gradient + value0;
   T *dvalues = a.dvalue + value0;
   const uint64_t block_bytes = Kept::bytes(KT, a.pairs);
   char *chunks = a.heads + head * d.chunks * block_bytes;
-  constexpr uint32_t kOperand = 64 * sizeof(Op), kKeys = 4 * KT * kOperand;
-  const char *keys =
+  constexpr uint32_t kOperand = 64 * sizeof(Op), kKeys = 4 * KT * kOperand, kValue = sizeof(T);
+  constexpr bool kStaged = C == 2;
+  const char *copies =
       a.keys + (static_cast<uint64_t>(b) * d.key_heads + kh) * d.chunks * (3 * kKeys);
-  uint32_t cols[C];  // this lane's; those past the last are the last again, with gradients of 0
-  bool in[C];
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const uint32_t column = 16 * (block.x * C + c) + n;
-    in[c] = column < d.values;
-    cols[c] = in[c] ? column : d.values - 1;
-  }
+  const uint32_t value_bytes = static_cast<uint32_t>(value_stride * sizeof(T));
+  auto column_of = [&](int c) { return 16 * (block.x * C + c) + n; };
   auto rows_of = [&](uint32_t chunk) -> uint32_t {
     return min(length - start - chunk * kChunk, static_cast<uint32_t>(kChunk));
   };
-  const bool holds = w < KT;  // keys 32 w on
+  const uint32_t tile = wave ^ 4;  // of 16 keys: half an operand
+  const bool holds = tile < 2 * KT;
   const uint64_t state_at = head * d.keys * d.values;
-  auto key_at = [&](int tile, int r) { return 32 * w + index_of(tile, 4 * g + r); };
-  f32x4 ds[2][C];
+  auto key_at = [&](int r) { return index_of(tile, 4 * g + r); };
+  f32x4 ds[C];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int c = 0; c < C; ++c) {
+    ds[c] = f32x4{};
+    if (a.from == nullptr || !holds) continue;
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      ds[i][c] = f32x4{};
-      if (a.from == nullptr || !holds) continue;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const uint32_t k = key_at(i, r), there = min(k, d.keys - 1);
-        const float v = a.from[state_at + static_cast<uint64_t>(there) * d.values + cols[c]];
-        ds[i][c][r] = k < d.keys && in[c] ? v : 0.0f;
-      }
+    for (int r = 0; r < 4; ++r) {
+      const uint32_t k = key_at(r), there = min(k, d.keys - 1);
+      const float v = a.from[state_at + static_cast<uint64_t>(there) * d.values +
+                             min(column_of(c), d.values - 1)];
+      ds[c][r] = k < d.keys && column_of(c) < d.values ? v : 0.0f;
     }
+  }
 
   // Loaded and stored as the forward's.
   typedef T quarter __attribute__((ext_vector_type(4)));
-  Op key[KT], scores[2], solve[2], back[2][2], forth[2][2];
-  T gradient[C][4];
-  f32x4 since, until, write, since_next;
+  Op back[2], forth[2];
   float whole = 0.0f;
-  const uint32_t value_bytes = static_cast<uint32_t>(value_stride * sizeof(T));
   const uint32_t lane_at = lane * sizeof(Op);
   auto operands_of = [&](uint32_t chunk, uint64_t part) {
-    return chunks + (chunk * block_bytes + part);
+    return buffer_of(chunks + (chunk * block_bytes + part),
+                     static_cast<uint32_t>(Kept::pairs - part));
   };
-  auto load_keys = [&](uint32_t chunk) {
-    const char *from = keys + (chunk * uint64_t{3 * kKeys} + w * (KT * kOperand));
+  auto load_copies = [&](uint32_t chunk, uint32_t part, auto &to, uint32_t first) {
+    const auto from = buffer_of(copies + (chunk * uint64_t{3 * kKeys} + part * kKeys), kKeys);
 #pragma unroll
-    for (int s = 0; s < KT; ++s) key[s] = load_at<Op>(from + s * kOperand, lane_at);
-  };
-  auto load_triangle = [&](uint32_t chunk, uint64_t part, Op(&to)[2]) {
-    const char *from = operands_of(chunk, part);
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-      to[s] = load_at<Op>(from + upper_place(w, max(s, pair)) * kOperand, lane_at);
-  };
-  auto load_gradients = [&](uint32_t chunk) {
-    const uint32_t last = rows_of(chunk) - 1;
-    const char *from = reinterpret_cast<const char *>(gradients + chunk * kChunk * value_stride);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const uint32_t row = min(index_of(w, 4 * g + r), last) * value_bytes;
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-        gradient[c][r] = load_at<T>(from, row + cols[c] * static_cast<uint32_t>(sizeof(T)));
-    }
-    since_next = load_at<f32x4>(operands_of(chunk, Kept::gates) + offsetof(Gates, since),
-                                index_of(w, 4 * g) * 4);
-  };
-  auto load_gates = [&](uint32_t chunk) {
-    const char *gates = operands_of(chunk, Kept::gates);
-    const uint32_t at = index_of(w, 4 * g) * 4;
-    since = load_at<f32x4>(gates + offsetof(Gates, since), at);
-    until = load_at<f32x4>(gates + offsetof(Gates, until), at);
-    write = load_at<f32x4>(gates + offsetof(Gates, write), at);
+    for (uint32_t s = 0; s < sizeof(to) / sizeof(Op); ++s)
+      to[s] = load_from<Op>(from, lane_at, (first + s) * kOperand);
   };
   auto load_rest = [&](uint32_t chunk) {
-    whole = load_at<float>(operands_of(chunk, Kept::gates) + offsetof(Gates, since),
-                           (kChunk - 1) * 4);
-    const char *k = keys + (chunk * uint64_t{3 * kKeys} + kKeys + 4 * min(w, KT - 1u) * kOperand);
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        back[i][s] = load_at<Op>(k + (2 * i + s) * kOperand, lane_at);
-        forth[i][s] = load_at<Op>(k + kKeys + (2 * i + s) * kOperand, lane_at);
-      }
-  };
-  auto hand = [&](Op(&to)[64], f32x4 v) {
-    reinterpret_cast<quarter *>(&to[lane])[half] = __builtin_convertvector(v, quarter);
-  };
-  auto hand_gradients = [&](uint32_t chunk) {
-    const uint32_t rows = rows_of(chunk);
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      f32x4 v;
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        v[r] = in[c] && index_of(w, 4 * g + r) < rows ? widen(gradient[c][r]) : 0.0f;
-      hand(m.out[chunk & 1][pair][c], v);
-      hand(m.decayed[chunk & 1][pair][c], since_next * d.scale * v);
+    whole = load_from<float>(operands_of(chunk, Kept::gates),
+                             offsetof(Gates, since) + (kChunk - 1) * 4, 0);
+    if constexpr (!kStaged) {
+      load_copies(chunk, 1, back, 2 * min(tile, 2 * KT - 1u));
+      load_copies(chunk, 2, forth, 2 * min(tile, 2 * KT - 1u));
     }
   };
-  // what the products read of a chunk; a block of one slab brings its half of the pair's lanes
-  const uint32_t kept = a.pairs * static_cast<uint32_t>(Kept::pair(KT));
-  auto pairs_at = [&](uint32_t chunk) { return buffer_of(operands_of(chunk, Kept::pairs), kept); };
-  const bool brings = C == 2 || (g >> 1) == (block.x & 1);
-  auto pair_at = [&](int place) {
-    return brings ? (block.x * C / 2 * (2 * KT + 4) + place) * kOperand + lane_at : kNowhere;
+  auto hand = [&](Op(&to)[64], f32x4 v, uint32_t half) {
+    reinterpret_cast<quarter *>(&to[lane])[half] = __builtin_convertvector(v, quarter);
   };
-  auto hand_state = [&](uint32_t chunk) {
+  auto hand_state = [&] {
     if (KT < 4 && !holds) return;
 #pragma unroll
-    for (int c = 0; c < C; ++c) m.state[w][c][lane] = rounded<T>(join(ds[0][c], ds[1][c]));
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      store_to(pairs_at(chunk), pair_at(2 * w + i),
-               turned<false>(&m.state[w][0][0], C == 2 ? 64 : 0, i, n, g));
+    for (int c = 0; c < C; ++c) hand(m.state[tile >> 1][c], ds[c], tile & 1);
   };
   auto read_pairs = [&](Op(&to)[2][C], const Op(&from)[2][C][64]) {
 #pragma unroll
@@ -287,132 +232,299 @@ __global__ __launch_bounds__(256) void delta_backward_scan_kernel(Args<T> a) {
 #pragma unroll
       for (int c = 0; c < C; ++c) to[s][c] = from[s][c][lane];
   };
-  if (live != 0) {
-    const uint32_t last = live - 1;
-    load_gradients(last);
-    load_keys(last);
-    load_triangle(last, Kept::within, scores);
-    load_gates(last);
-    load_triangle(last, Kept::system, solve);
-    load_rest(last);
-    hand_gradients(last);
-    load_gradients(last == 0 ? 0 : last - 1);
-    hand_state(last);
-  }
-  for (uint32_t chunk = live; chunk-- != 0;) {
-    const uint32_t next = chunk == 0 ? 0 : chunk - 1, after = next == 0 ? 0 : next - 1;
-    lds_barrier();
-    // du = scale (G o q k')' do + exp(g_64 - g) k dS
-    f32x4 x[C] = {};
-    {
-      Op right[KT][C], out[2][C];
-#pragma unroll
-      for (int s = 0; s < KT; ++s)
-#pragma unroll
-        for (int c = 0; c < C; ++c) right[s][c] = m.state[s][c][lane];
-      read_pairs(out, m.out[chunk & 1]);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int s = 0; s < KT; ++s)
-#pragma unroll
-        for (int c = 0; c < C; ++c) x[c] = product(key[s], right[s][c], x[c]);
-#pragma unroll
-      for (int c = 0; c < C; ++c) x[c] *= until;
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        if (s < pair) continue;
-#pragma unroll
-        for (int c = 0; c < C; ++c) x[c] = product(scores[s], out[s][c], x[c]);
-      }
-    }
-#pragma unroll
-    for (int c = 0; c < C; ++c) hand(m.weighted[pair][c], -write * x[c]);
-    __builtin_amdgcn_sched_barrier(0);
-    load_keys(next);
-    load_triangle(next, Kept::within, scores);
-    lds_barrier();
-    // x = du - N' (b du);  dv = b x
-    {
-      Op right[2][C];
-      read_pairs(right, m.weighted);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        if (s < pair) continue;
-#pragma unroll
-        for (int c = 0; c < C; ++c) x[c] = product(solve[s], right[s][c], x[c]);
-      }
-    }
-    const uint32_t rows = rows_of(chunk);
-    const auto to = buffer_of(dvalues + chunk * kChunk * value_stride, kChunk * value_bytes);
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      hand(m.x[pair][c], x[c]);
-      x[c] *= write;
-      hand(m.taken[pair][c], -since * x[c]);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const uint32_t t = index_of(w, 4 * g + r);
-        store_to(to, t < rows && in[c]
-                         ? t * value_bytes + cols[c] * static_cast<uint32_t>(sizeof(T))
-                         : kNowhere,
-                 static_cast<T>(x[c][r]));
-      }
-    }
-    // the next chunk's gradients of the outputs
-    hand_gradients(next);
-    __builtin_amdgcn_sched_barrier(0);
-    load_triangle(next, Kept::system, solve);
-    load_gates(next);
-    load_gradients(after);
-    lds_barrier();
-    // dS0 = exp(g_64) dS + scale q' (exp(g) do) - k' (exp(g) dv)
-    Op decayed[2][C], taken[2][C];
-    read_pairs(decayed, m.decayed[chunk & 1]);
-    read_pairs(taken, m.taken);
-    __builtin_amdgcn_sched_barrier(0);
+  // dS0 = exp(g_64) dS + scale q' (exp(g) do) - k' (exp(g) dv)
+  auto advance = [&](uint32_t chunk, uint32_t next) {
     if (KT == 4 || holds) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int c = 0; c < C; ++c) ds[c] *= whole;
+      // one sum after the other: both sums' operands would take registers of a second block
+      {
+        Op right[2][C];
+        if constexpr (kStaged)
 #pragma unroll
-        for (int c = 0; c < C; ++c) ds[i][c] *= whole;
+          for (int s = 0; s < 2; ++s) forth[s] = m.queries.across(tile, s, n, g);
+        read_pairs(right, m.decayed);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+        for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int c = 0; c < C; ++c)
+          for (int c = 0; c < C; ++c) ds[c] = product(forth[s], right[s][c], ds[c]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      {
+        Op right[2][C];
+        if constexpr (kStaged)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) ds[i][c] = product(forth[i][s], decayed[s][c], ds[i][c]);
+          for (int s = 0; s < 2; ++s) back[s] = m.keys[chunk & 1].across(tile, s, n, g);
+        read_pairs(right, m.taken);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+        for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) ds[i][c] = product(back[i][s], taken[s][c], ds[i][c]);
+          for (int c = 0; c < C; ++c) ds[c] = product(back[s], right[s][c], ds[c]);
+      }
     }
-    store_to(pairs_at(chunk), pair_at(2 * KT + w),
-             turned<false>(&m.x[pair][0][0], C == 2 ? 64 : 0, half, n, g));
     __builtin_amdgcn_sched_barrier(0);
     load_rest(next);
-    if (chunk != 0) hand_state(next);
+    if (chunk != 0) hand_state();
+  };
+  if (live != 0) {
+    load_rest(live - 1);
+    hand_state();
+  }
+  if (wave < 4) {
+    Op key[KT], scores[2], solve[2];
+    f32x4 since, until, write;
+    auto read_keys = [&](uint32_t chunk) {
+      if constexpr (kStaged) {
+#pragma unroll
+        for (int s = 0; s < KT; ++s) key[s] = m.keys[chunk & 1].along(index_of(w, n), s, g);
+      } else {
+        load_copies(chunk, 0, key, w * KT);
+      }
+    };
+    auto load_triangle = [&](uint32_t chunk, uint64_t part, Op(&to)[2]) {
+      const auto from = operands_of(chunk, part);
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        to[s] = load_from<Op>(from, lane_at, upper_place(w, max(s, pair)) * kOperand);
+    };
+    auto load_gates = [&](uint32_t chunk) {
+      const auto from = operands_of(chunk, Kept::gates);
+      const uint32_t at = index_of(w, 4 * g) * 4;
+      since = load_from<f32x4>(from, at, offsetof(Gates, since));
+      until = load_from<f32x4>(from, at, offsetof(Gates, until));
+      write = load_from<f32x4>(from, at, offsetof(Gates, write));
+    };
+    if (live != 0) {
+      const uint32_t last = live - 1;
+      load_triangle(last, Kept::within, scores);
+      load_gates(last);
+      load_triangle(last, Kept::system, solve);
+      if constexpr (kStaged) lds_barrier();
+      read_keys(last);
+    }
+    for (uint32_t chunk = live; chunk-- != 0;) {
+      const uint32_t next = chunk == 0 ? 0 : chunk - 1;
+      lds_barrier();
+      // du = scale (G o q k')' do + exp(g_64 - g) k dS
+      f32x4 x[C] = {};
+      {
+        Op right[KT][C];
+#pragma unroll
+        for (int s = 0; s < KT; ++s)
+#pragma unroll
+          for (int c = 0; c < C; ++c) right[s][c] = m.state[s][c][lane];
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int s = 0; s < KT; ++s)
+#pragma unroll
+          for (int c = 0; c < C; ++c) x[c] = product(key[s], right[s][c], x[c]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      {
+        Op out[2][C];
+        read_pairs(out, m.out);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int c = 0; c < C; ++c) x[c] *= until;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          if (s < pair) continue;
+#pragma unroll
+          for (int c = 0; c < C; ++c) x[c] = product(scores[s], out[s][c], x[c]);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < C; ++c) hand(m.weighted[pair][c], -write * x[c], half);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (!kStaged) read_keys(next);
+      load_triangle(next, Kept::within, scores);
+      lds_barrier();
+      // x = du - N' (b du);  dv = b x
+      {
+        Op right[2][C];
+        read_pairs(right, m.weighted);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          if (s < pair) continue;
+#pragma unroll
+          for (int c = 0; c < C; ++c) x[c] = product(solve[s], right[s][c], x[c]);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        hand(m.x[pair][c], x[c], half);
+        x[c] *= write;
+        hand(m.taken[pair][c], -since * x[c], half);
+        hand(m.dv[pair][c], x[c], half);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      load_triangle(next, Kept::system, solve);
+      load_gates(next);
+      lds_barrier();
+      advance(chunk, next);
+      if constexpr (kStaged) read_keys(next);
+    }
+  } else {
+    // do, as the forward has its values
+    constexpr bool kRows = Packed && sizeof(T) == 2 && kStaged;
+    T gradient[C][4];
+    Op row, unit[C];
+    uint32_t at[C][4], row_at = kNowhere;
+    if constexpr (kRows) {
+      const uint32_t first = 32 * block.x + 8 * g;
+      if (first < d.values) row_at = index_of(w, n) * value_bytes + first * kValue;
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i)
+          unit[c][i] = static_cast<T>(first + i == column_of(c) ? 1.0f : 0.0f);
+    } else {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          at[c][r] = column_of(c) < d.values
+                         ? index_of(w, 4 * g + r) * value_bytes + column_of(c) * kValue
+                         : kNowhere;
+    }
+    f32x4 since, v[C] = {};
+    auto load_gradients = [&](uint32_t chunk) {
+      const auto from = buffer_of(gradients + chunk * kChunk * value_stride,
+                                  rows_of(chunk) * value_bytes);
+      if constexpr (kRows) {
+        row = load_from<Op>(from, row_at, 0);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int c = 0; c < C; ++c) gradient[c][r] = load_from<T>(from, at[c][r], 0);
+      }
+      since = load_from<f32x4>(operands_of(chunk, Kept::gates), index_of(w, 4 * g) * 4,
+                               offsetof(Gates, since));
+    };
+    auto hand_out = [&] {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        v[c] = f32x4{};
+        if constexpr (kRows) {
+          v[c] = product(row, unit[c], v[c]);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[c][r] = widen(gradient[c][r]);
+        }
+        hand(m.out[pair][c], v[c], half);
+        v[c] *= since * d.scale;
+      }
+    };
+    const uint32_t row_bytes = d.key_heads * d.keys * kValue;
+    using Part = RowPart<T, kStaged ? KT : 0, Packed>;
+    const Part part(threadIdx.x - 256, row_bytes, d.keys);
+    typename Part::Values key_part, query_part;
+    const uint64_t key_row0 = (row0 * d.key_heads + kh) * d.keys;
+    auto load_rows = [&](typename Part::Values &to, const T *from, uint32_t chunk) {
+      const uint64_t first = chunk * kChunk * static_cast<uint64_t>(d.key_heads) * d.keys;
+      part.load(to, buffer_of(from + key_row0 + first, rows_of(chunk) * row_bytes), d.keys);
+    };
+    // what the products read of a chunk; a block of one slab brings its half of the pair's lanes
+    const uint32_t kept = a.pairs * static_cast<uint32_t>(Kept::pair(KT));
+    auto pairs_at = [&](uint32_t chunk, bool there) {
+      return buffer_of(chunks + (chunk * block_bytes + Kept::pairs), there ? kept : 0);
+    };
+    const bool brings = C == 2 || (g >> 1) == (block.x & 1);
+    auto pair_at = [&](int place) {
+      return brings ? (block.x * C / 2 * (2 * KT + 4) + place) * kOperand + lane_at : kNowhere;
+    };
+    // x and dv of a chunk: a lane its step's 8 columns
+    auto finish = [&](uint32_t chunk, bool there) {
+      constexpr uint32_t kApart = C == 2 ? 64 : 0;
+      store_to(pairs_at(chunk, there), pair_at(2 * KT + w),
+               turned<false>(&m.x[pair][0][0], kApart, half, n, g));
+      const Op dv = turned<false>(&m.dv[pair][0][0], kApart, half, n, g);
+      const auto to = buffer_of(dvalues + chunk * kChunk * value_stride,
+                                there ? rows_of(chunk) * value_bytes : 0);
+      const uint32_t first = 32 * (C == 2 ? block.x : block.x >> 1) + 8 * g;
+      const uint32_t from = index_of(w, n) * value_bytes + first * kValue;
+      if constexpr (Packed) {
+        if constexpr (sizeof(T) == 2) {
+          store_to(to, brings && first < d.values ? from : kNowhere, dv);
+        } else {
+#pragma unroll
+          for (uint32_t i = 0; i < 8; i += 4)
+            store_to(to, brings && first + i < d.values ? from + i * kValue : kNowhere,
+                     f32x4{dv[i], dv[i + 1], dv[i + 2], dv[i + 3]});
+        }
+      } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i)
+          store_to(to, brings && first + i < d.values ? from + i * kValue : kNowhere,
+                   static_cast<T>(dv[i]));
+      }
+    };
+    if (live != 0) {
+      const uint32_t last = live - 1, next = last == 0 ? 0 : last - 1;
+      load_gradients(last);
+      if constexpr (kStaged) {
+        load_rows(key_part, a.key, last);
+        part.store(m.keys[last & 1], key_part);
+        __builtin_amdgcn_sched_barrier(0);
+        load_rows(key_part, a.key, next);
+        load_rows(query_part, a.query, last);
+      }
+      hand_out();
+      __builtin_amdgcn_sched_barrier(0);
+      load_gradients(next);
+      if constexpr (kStaged) lds_barrier();
+    }
+    for (uint32_t chunk = live; chunk-- != 0;) {
+      const uint32_t next = chunk == 0 ? 0 : chunk - 1, after = next == 0 ? 0 : next - 1;
+      lds_barrier();
+      // the chunk before's (it is the one behind this), while the others form this one's du; at the
+      // last chunk nothing is there
+      finish(min(chunk + 1, live - 1), chunk + 1 != live);
+#pragma unroll
+      for (int c = 0; c < C; ++c) hand(m.decayed[pair][c], v[c], half);
+      if constexpr (kStaged) {
+        part.store(m.queries, query_part);
+        part.store(m.keys[(chunk + 1) & 1], key_part);
+        __builtin_amdgcn_sched_barrier(0);
+        load_rows(query_part, a.query, next);
+        load_rows(key_part, a.key, after);
+      }
+      if (w < KT) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          store_to(pairs_at(chunk, true), pair_at(2 * w + i),
+                   turned<false>(&m.state[w][0][0], C == 2 ? 64 : 0, i, n, g));
+      }
+      lds_barrier();
+      hand_out();
+      __builtin_amdgcn_sched_barrier(0);
+      load_gradients(after);
+      lds_barrier();
+      advance(chunk, next);
+    }
+    if (live != 0) finish(0, true);
   }
   // steps past the row's end
   const uint32_t end = min(d.time - start, d.chunks * kChunk);
-  for (uint32_t t = (length <= start ? 0 : length - start) + 4 * w + g; t < end; t += 16) {
+  for (uint32_t t = (length <= start ? 0 : length - start) + 4 * wave + g; t < end; t += 32) {
 #pragma unroll
     for (int c = 0; c < C; ++c)
-      if (in[c]) dvalues[t * value_stride + cols[c]] = static_cast<T>(0.0f);
+      if (column_of(c) < d.values) dvalues[t * value_stride + column_of(c)] = static_cast<T>(0.0f);
   }
   if (a.to == nullptr || !holds) return;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int r = 0; r < 4; ++r) {
+    const uint32_t k = key_at(r);
+    if (k >= d.keys) continue;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const uint32_t k = key_at(i, r);
-      if (k >= d.keys) continue;
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-        if (in[c]) a.to[state_at + static_cast<uint64_t>(k) * d.values + cols[c]] = ds[i][c][r];
-    }
+    for (int c = 0; c < C; ++c)
+      if (column_of(c) < d.values)
+        a.to[state_at + static_cast<uint64_t>(k) * d.values + column_of(c)] = ds[c][r];
+  }
 }
 
 constexpr int kColumns = 32;  // of values that the products take at a time: a pair of slabs
@@ -426,6 +538,9 @@ struct Products {
   };
   union {
     Pair pairs[2];
+    struct {
+      RowTile<T, KT> keys, queries;
+    };
     alignas(16) float rows[kChunk][32 * KT + 4];
   };
   // past a row's 64 columns: what is not to be written
@@ -453,12 +568,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && !Shared ? 2 : 1) void delta_
   const uint32_t row = threadIdx.x >> 2, part = threadIdx.x & 3;  // of the results' rows
   const uint64_t stride = static_cast<uint64_t>(d.key_heads) * d.keys;
   const uint64_t value_stride = static_cast<uint64_t>(d.heads) * d.values;
-  constexpr uint32_t kOperand = 64 * sizeof(Op);
-  const uint32_t lane_at = lane * sizeof(Op);
   f32x8 sums_q[Shared ? KT : 1] = {}, sums_k[Shared ? KT : 1] = {};
   const Place first(d, chunk, kh * d.group, b);
   const uint32_t held = min(d.time - first.begin, static_cast<uint32_t>(kChunk)), rows = first.rows;
-  const char *keys = a.keys + first.key_chunk(d) * (12 * KT * kOperand);
+  const RowPart<T, KT, Whole> brings(threadIdx.x, static_cast<uint32_t>(stride * sizeof(T)), d.keys);
   const uint32_t t_row = index_of(w, n), t_read = rows == 0 ? 0 : min(t_row, rows - 1);
   const uint64_t to_keys = first.key_row * d.keys + row * stride;
   for (uint32_t turn = 0; turn < (Shared ? d.group : 1); ++turn) {
@@ -545,27 +658,28 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && !Shared ? 2 : 1) void delta_
             for (int j = 0; j < 8; ++j) across = fmaf(widen(state[k][j]), widen(gradient[k][j]), across);
       }
     }
+    // the chunk's keys and queries where the pairs were
+    {
+      typename RowPart<T, KT, Whole>::Values keys, queries;
+      const uint32_t bytes = rows * static_cast<uint32_t>(stride * sizeof(T));
+      brings.load(keys, buffer_of(a.key + at.key_row * d.keys, bytes), d.keys);
+      brings.load(queries, buffer_of(a.query + at.key_row * d.keys, bytes), d.keys);
+      lds_barrier();
+      brings.store(m.keys, keys);
+      brings.store(m.queries, queries);
+      lds_barrier();
+    }
     // q k' and k k' again, for what their pairs' decays are worth
     f32x4 qk[4] = {}, kk[4] = {};
-    {
-      const T *query = a.query + at.key_row * d.keys + t_read * stride;
-      Op q[KT], others[KT][4];
 #pragma unroll
-      for (int s = 0; s < KT; ++s) {
-        q[s] = load_row<T, Whole>(query, 32 * s + 8 * g, d.keys);
+    for (int s = 0; s < KT; ++s) {
+      const Op q = m.queries.along(t_row, s, g), k = m.keys.along(t_row, s, g);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) others[s][i] = load_at<Op>(keys + (i * KT + s) * kOperand, lane_at);
-      }
-      if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int s = 0; s < KT; ++s) {
-        const Op k = w == 0 ? others[s][0] : w == 1 ? others[s][1] : w == 2 ? others[s][2] : others[s][3];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if ((i >> 1) > pair) continue;
-          qk[i] = product(q[s], others[s][i], qk[i]);
-          kk[i] = product(k, others[s][i], kk[i]);
-        }
+      for (int i = 0; i < 4; ++i) {
+        if ((i >> 1) > pair) continue;
+        const Op other = m.keys.along(index_of(i, n), s, g);
+        qk[i] = product(q, other, qk[i]);
+        kk[i] = product(k, other, kk[i]);
       }
     }
     const uint32_t t0 = index_of(w, 4 * g);  // this lane's first row of the results
@@ -626,8 +740,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && !Shared ? 2 : 1) void delta_
       Op k[2], q[2];
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        k[s] = load_at<Op>(keys + (4 * KT + 2 * i + s) * kOperand, lane_at);
-        q[s] = load_at<Op>(keys + (8 * KT + 2 * i + s) * kOperand, lane_at);
+        k[s] = m.keys.across(i, s, n, g);
+        q[s] = m.queries.across(i, s, n, g);
       }
       // of the wave's own steps: a lane's four are half of its 8
       const Op own = pair == 0 ? k[0] : k[1], asked = pair == 0 ? q[0] : q[1];
@@ -714,12 +828,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && !Shared ? 2 : 1) void delta_
 template <typename T>
 struct BackPlan {
   Plan p;
+  bool two;  // slabs of a block of the scan, as the forward's
   uint64_t head_bytes, key_bytes, state_bytes;
   uint64_t bytes() const { return head_bytes + key_bytes + state_bytes; }
   explicit BackPlan(const oxh_delta_shape &s, float scale, const int32_t *lengths)
       : p(s, scale, lengths) {
     const uint64_t head = s.batch * s.heads * Back<T>::bytes(p.steps, pairs_of(s.value_dim));
-    const uint64_t key = s.batch * s.key_heads * p.steps * 12 * kOperandBytes<T>;
+    two = s.batch * s.heads * pairs_of(s.value_dim) >= oxh::kComputeUnits;
+    const uint64_t key = two ? 0 : s.batch * s.key_heads * p.steps * 12 * kOperandBytes<T>;
     p.divide(head + key);
     head_bytes = round_up(p.segment * head, 256);
     key_bytes = round_up(p.segment * key, 256);
@@ -731,13 +847,16 @@ template <typename T>
 oxh_status backward(hipStream_t stream, const BackPlan<T> &plan, Args<T> a, const float *final,
                     float *initial, char *workspace) {
   a.heads = workspace;
-  a.keys = a.heads + plan.head_bytes;
-  float *between = reinterpret_cast<float *>(a.keys + plan.key_bytes);
+  a.keys = plan.two ? nullptr : a.heads + plan.head_bytes;
+  float *between = reinterpret_cast<float *>(a.heads + plan.head_bytes + plan.key_bytes);
   const Plan &p = plan.p;
   a.all = static_cast<uint32_t>(p.all);
   const uint64_t launches = (p.all + p.segment - 1) / p.segment;
   a.pairs = (p.d.slabs + 1) / 2;
-  const bool two = static_cast<uint64_t>(p.d.batch) * p.d.heads * a.pairs >= oxh::kComputeUnits;
+  constexpr uint64_t kPack = 16 / sizeof(T);
+  const bool keys16 = oxh::aligned16(a.query) && oxh::aligned16(a.key);
+  const bool packed = p.d.values % kPack == 0 && p.d.keys % kPack == 0 && keys16 &&
+                      oxh::aligned16(a.gradient) && oxh::aligned16(a.dvalue);
   for (uint64_t i = launches; i-- != 0;) {
     const uint64_t first = i * p.segment;
     a.d = p.d;
@@ -746,17 +865,22 @@ oxh_status backward(hipStream_t stream, const BackPlan<T> &plan, Args<T> a, cons
     a.from = i + 1 == launches ? final : between;
     a.to = i == 0 ? initial : between;
     const Dims &d = a.d;
-    with_keys(d.keys, d.keys % 32 == 0, [&](auto steps, auto whole) {
+    with_keys(d.keys, d.keys % 32 == 0 && keys16, [&](auto steps, auto whole) {
       constexpr int KT = decltype(steps)::value;
       constexpr bool W = decltype(whole)::value;
       oxh::launch(delta_backward_prepare_kernel<T, KT, W>, dim3(d.chunks, d.heads, d.batch),
                   dim3(256), 0, stream, a);
-      if (two)
-        oxh::launch(delta_backward_scan_kernel<T, KT, 2>, dim3(a.pairs, d.heads, d.batch), dim3(256),
-                    0, stream, a);
-      else
-        oxh::launch(delta_backward_scan_kernel<T, KT, 1>, dim3(2 * a.pairs, d.heads, d.batch),
-                    dim3(256), 0, stream, a);
+      auto go = [&](auto columns, auto packs) {
+        constexpr int C = decltype(columns)::value;
+        oxh::launch(delta_backward_scan_kernel<T, KT, C, decltype(packs)::value>,
+                    dim3(2 / C * a.pairs, d.heads, d.batch), dim3(512), 0, stream, a);
+      };
+      auto slabs = [&](auto packs) {
+        if (plan.two) go(std::integral_constant<int, 2>(), packs);
+        else go(std::integral_constant<int, 1>(), packs);
+      };
+      if (packed) slabs(std::true_type());
+      else slabs(std::false_type());
       const dim3 grid(d.chunks, d.key_heads, d.batch);
       auto products = [&](auto values, auto shared) {
         oxh::launch(delta_backward_products_kernel<T, KT, W, decltype(values)::value,
