@@ -13,9 +13,21 @@
 //   o = scale (exp(g) q S0 + (G o q k') (b e));  S = exp(g_64) S0 + k' (exp(g_64 - g) b e)
 //
 // N and G o q k' depend on no state: delta_prepare_kernel forms them for all chunks at once.
-// delta_scan_kernel goes from chunk to chunk, a wave for each 16 columns of values, which never
-// meet: the state stays in its registers in the layout of the matrix cores' results, which is that
-// of their next operand, so that a chunk is products alone.  b is never divided by: it may be 0.
+// delta_scan_kernel goes from chunk to chunk; columns of values never meet, so a block takes 16 or 32
+// of them, its waves the state in the layout of the matrix cores' results, which is that of their next
+// operand.  b is never divided by: it may be 0.
+//
+// What is rounded.  float32 operands: nothing, the matrix cores take float32.  bfloat16 ones: q, k and
+// v as they are; the state, N, G o q k', b y and b e as operands of products, 8 bits each, their sums
+// and the state itself float32: outputs are 2.4e-3 off in the mean square, 1.7e-3 being their own
+// rounding.  A state that is handed on is formed from pairs of such operands that add up to 16 bits
+// (2^-17): rounding it to 8 at each of many chunks is no error of one output but of all later calls.
+//
+// Measured, bfloat16, heads of 128 keys and 128 values: 8 x 2048 x 16 heads with what the backward reads
+// 60 us to prepare (183 MB, 3.1 TB/s) and 144 to scan (511 MB, 3.5 TB/s): memory.  1 x 32768 x 16 heads
+// with a final state 3 x 64 and 3 x 220 us, 1.3 us a chunk: the way of a chunk through one block (its
+// three exchanges, about 300 instructions of a wave and 96 KB from the caches at 64 bytes a cycle),
+// on half of the compute units.  Loading the same two chunks again and again took as long.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -42,7 +54,9 @@ struct PrepareArgs {
   char *keys;   // operands of keys, queries and transposed keys of (batch, key head, chunk), or null
 };
 
-// A block per chunk and value head.
+// A block per chunk and value head.  Its own work is 64 x 64 products; what it reads and writes bounds
+// it, or for one chunk of few heads the inversion's 16 dependent steps and three more barriers
+// (float32 128 x 28 x 4 heads of 32: 14 us).
 template <typename T, int P, int KT, bool Whole>
 __global__ __launch_bounds__(256) void delta_prepare_kernel(PrepareArgs<T> a) {
   using Op = operand<T>;
@@ -134,13 +148,15 @@ struct Exchange {
 
 // A block of eight waves per C slabs of 16 columns of a head's values.  Each holds 16 of the keys;
 // the first four follow the errors of 16 of a chunk's steps each, the others form those steps'
-// outputs beside them, a stage behind.  What they form of each other's products goes through shared
-// memory, three times a chunk; what stands on the left of a product, or here of its transpose, is
-// one wave's alone, and is loaded a chunk ahead, as soon as the present chunk's is used.  The chunk's
-// matrices go straight to registers.  So do keys and queries with one slab, as operands that were
-// prepared: few blocks are as fast as a chunk's way through one.  Blocks of two slabs stage their
-// rows in shared memory, where the sums over the keys and those over the steps both find their
-// operands: of many blocks the bytes count, a third less without the copies.
+// outputs beside them, a stage behind (four waves with all of it: 250 us a launch where this takes
+// 220).  What they form of each other's products goes through shared memory, three times a chunk; what
+// stands on the left of a product, or here of its transpose, is one wave's alone, and is loaded a chunk
+// ahead, as soon as the present chunk's is used.  The chunk's matrices go straight to registers.  So do
+// keys and queries with one slab, as operands that were prepared: few blocks are as fast as a chunk's
+// way through one, and shared memory takes longer (1 x 32768 x 16 heads: 654 us of scans, 807 with
+// rows staged).  Blocks of two slabs stage their rows in shared memory, where the sums over the keys
+// and those over the steps both find their operands: of many blocks the bytes count, a third less
+// without the copies (8 x 2048 x 16 heads: 204 us prepared and scanned, 270 with copies).
 template <typename T, int P, int KT, int C, bool Packed>
 __global__ __launch_bounds__(512, Packed && sizeof(T) == 2 && C == 2 && P == 1 ? 4 : 2) void delta_scan_kernel(
     ScanArgs<T> a) {
@@ -581,7 +597,8 @@ struct StepArgs {
 };
 
 // A wave per 32 columns of a head's values: a lane R consecutive keys of 4 columns, kept in
-// registers from step to step.
+// registers from step to step.  One step reads and writes the state once, in 16 bytes a lane of a row
+// of 128: 64 rows of 32 heads of 128 x 128 in 57 us, 4.7 TB/s, which bounds it.
 template <typename T, int R, bool Whole>
 __global__ __launch_bounds__(256) void delta_step_kernel(StepArgs<T> a) {
   const Dims &d = a.d;
@@ -691,8 +708,15 @@ __global__ __launch_bounds__(256) void delta_step_kernel(StepArgs<T> a) {
 
 // ------------------------------------------------------------------------------------ host side
 
-// Steps taken one by one where no backward is to follow.
-constexpr uint64_t kStepLimit = 16;
+// Steps taken one by one where no backward is to follow: they cost about 1.5 us each, or with many
+// heads their products on the vector units; a chunk costs as much for one step as for 64.  (16 steps
+// of 16 heads: 28 us one by one, 16 by a chunk in bfloat16, and 25 and 23 in float32; of 512 heads 44
+// and 53, 38 and 96; 8 steps of 16 heads: 16 and 15, 14 and 23.)  float32 chunks are four times as
+// dear on the matrix cores, so many heads take more steps (48 of 512 heads: 88 us and 98).
+uint64_t step_limit(const oxh_delta_shape &s, bool f32) {
+  const uint64_t waves = s.batch * s.heads * ((s.value_dim + 31) / 32);
+  return f32 && waves >= 8 * oxh::kComputeUnits ? 48 : 16;
+}
 
 template <typename T, int P>
 struct ForwardPlan {
@@ -703,7 +727,9 @@ struct ForwardPlan {
   ForwardPlan(const oxh_delta_shape &s, float scale, const int32_t *lengths)
       : p(s, scale, lengths) {
     const uint64_t head = s.batch * s.heads * Chunk<T, P>::bytes;
-    // as many as leave a block for each compute unit
+    // Two where that leaves a block for each compute unit (a head of 128 values has 4 such blocks.
+    // Of 1024 steps, one and two slabs: bfloat16 128 blocks 41 and 48 us, 256 blocks 57 and 52, 512
+    // blocks 128 and 94; float32 73 and 111, 137 and 131, 305 and 263).
     two = s.batch * s.heads * ((p.d.slabs + 1) / 2) >= oxh::kComputeUnits;
     const uint64_t key = two ? 0 : s.batch * s.key_heads * p.steps * 12 * kOperandBytes<T>;
     p.divide(head + key);
@@ -773,8 +799,8 @@ oxh_status by_chunks(hipStream_t stream, const ForwardPlan<T, P> &plan, const T 
   return oxh::ok();
 }
 
-bool by_steps_alone(const oxh_delta_shape &s, bool saves) {
-  return s.time == 0 || (!saves && s.time <= kStepLimit);
+bool by_steps_alone(int dtype, const oxh_delta_shape &s, bool saves) {
+  return s.time == 0 || (!saves && s.time <= step_limit(s, dtype == OXH_F32));
 }
 
 template <typename T>
@@ -803,7 +829,7 @@ oxh_status oxh_gated_delta_rule_workspace_size(int dtype, const oxh_delta_shape 
   oxh_status st = check_shape(dtype, shape);
   if (st != OXH_OK) return st;
   *bytes = 0;
-  if (by_steps_alone(*shape, saves != 0)) return oxh::ok();
+  if (by_steps_alone(dtype, *shape, saves != 0)) return oxh::ok();
   *bytes = dtype == OXH_F32 ? ForwardPlan<float, 1>(*shape, 1.0f, nullptr).bytes()
                             : ForwardPlan<bf16, 2>(*shape, 1.0f, nullptr).bytes();
   return oxh::ok();
@@ -832,7 +858,7 @@ oxh_status oxh_gated_delta_rule_forward(oxh_stream stream, int dtype, const oxh_
                   "gated delta rule: null pointer");
   in.push_back({lengths, s.batch * 4, 4});
   out.push_back({final_state, z.state, 4});
-  const bool steps = by_steps_alone(s, saved != nullptr);
+  const bool steps = by_steps_alone(dtype, s, saved != nullptr);
   uint64_t needed = 0;
   if (!steps) {
     st = oxh_gated_delta_rule_workspace_size(dtype, shape, saved != nullptr, &needed);

@@ -17,8 +17,17 @@
 // themselves away to the last bit, whatever their operands were rounded to.
 //
 // Three kernels: what depends on no state, for all chunks at once; the state's gradient from the
-// last chunk to the first, a wave for each 16 columns of values; and the products over the values,
+// last chunk to the first, a block for 16 or 32 columns of values; and the products over the values,
 // a block per chunk and key head.  S0 and e are the forward's.
+//
+// Rounded as the forward's: of bfloat16 operands u, x, dS, S0, e, M1, M2 and the matrices keep 8 bits
+// where they are operands, sums and dS itself float32; gradients are up to 3.4e-3 off in the mean
+// square.  The gates' sums are float32 throughout but for those operands.
+//
+// Measured, bfloat16, 8 x 2048 x 16 heads of 128 keys and values, in two parts: 2 x 38 us to prepare, 2 x
+// 80 to scan (509 MB in both, 3.2 TB/s) and 2 x 105 for the products (721 MB, 3.4 TB/s; their matrix
+// work is 30 us): memory, with two blocks a compute unit.  float32 128 x 28 x 4 heads of 32, one chunk:
+// 15, 12 and 27 us, the chain of a block's stages.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -478,3 +478,91 @@ def test_wrong_tensors(module, dev):
                  dict(scale=float("nan"))):
         with pytest.raises(ox.OxideError):
             call(q, k, v, gate, write, out, **rest)
+
+
+def shifted(x):
+    """The same values one element behind an aligned place."""
+    room = torch.empty(x.numel() + 1, dtype=x.dtype, device=x.device)
+    room[1:] = x.flatten()
+    return room[1:].view(x.shape)
+
+
+# enough heads for blocks of 32 columns, whose rows are staged: rows of whole 16 bytes, odd ones,
+# every count of 32 keys, odd counts of 16 columns, shared heads, one chunk and several
+MANY = [(32, 66, 2, 4, 128, 40), (43, 130, 1, 6, 17, 7), (86, 65, 1, 3, 96, 24),
+        (32, 129, 4, 4, 64, 33), (256, 20, 1, 1, 32, 32)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", MANY)
+@pytest.mark.parametrize("aligned", [True, False])
+def test_many_heads(module, dev, shape, dtype, aligned):
+    t = TYPES[dtype]
+    batch, time, _, heads, keys, values = shape
+    place = (lambda x: x) if aligned else shifted
+    ops = [place(x) for x in operands(shape, t, dev)]
+    g = place(make((batch, time, heads, values), t, dev, 21))
+    lengths = [time - 7 * (b % 3) if b % 5 else (b * 37) % (time + 1) for b in range(batch)]
+    n = torch.tensor(lengths, dtype=torch.int32, device=dev)
+    for x in (*ops, g):
+        for b, end in enumerate(lengths):
+            x[b, end:] = float("nan")
+    state = (batch, heads, keys, values)
+    first, dfinal = make(state, F32, dev, 9) * 0.3, make(state, F32, dev, 22)
+    out, final, back = place(torch.empty_like(ops[2])), torch.empty_like(first), torch.empty_like(first)
+    saved = module.gated_delta_rule_saved(ops[1], ops[2])
+    module.gated_delta_rule_forward(*ops, out, initial_state=first, final_state=final, saved=saved,
+                                    lengths=n)
+    clean = [torch.nan_to_num(x) for x in ops]
+    ref = check_forward(clean, out, final, t, True, first, lengths)
+    # without the state's exact way, and without what the backward reads
+    out.fill_(3.0)
+    module.gated_delta_rule_forward(*ops, out, initial_state=first, lengths=n)
+    held(out, ref.out, ref.near, units_of(t, True)[0], t, "output alone")
+    module.gated_delta_rule_forward(*ops, out, initial_state=first, saved=saved, lengths=n)
+    outs = [place(torch.full_like(x, 7.0)) for x in ops]
+    module.gated_delta_rule_backward(g, *ops, saved, *outs, final_state_gradient=dfinal,
+                                     initial_state_gradient=back, lengths=n)
+    check_gradients(ref, torch.nan_to_num(g), outs, t, dfinal, back)
+
+
+@pytest.mark.parametrize("time", [17, 48, 49])
+def test_steps_of_many_heads(module, dev, time):
+    """float32 heads enough to be taken one by one further, and the first count of steps that is not."""
+    shape = (128, time, 8, 16, 32, 24)
+    ops = operands(shape, F32, dev, 61)
+    first = make((128, 16, 32, 24), F32, dev, 9) * 0.3
+    out, final = torch.empty_like(ops[2]), torch.empty_like(first)
+    module.gated_delta_rule_forward(*ops, out, initial_state=first, final_state=final)
+    check_forward(ops, out, final, F32, True, first)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_heads_in_parts(module, dev, dtype):
+    """More chunks of many heads than are prepared at once: to the bit what two calls give that hand
+    each other the state and its gradient."""
+    t, shape = TYPES[dtype], (64, 1024, 8, 16, 8, 8)
+    ops, g = operands(shape, t, dev, 71), make((64, 1024, 16, 8), t, dev, 72)
+    state = torch.empty(64, 16, 8, 8, device=dev)
+    whole, parts, back = (torch.empty_like(state) for _ in range(3))
+    dfinal = make(state.shape, F32, dev, 73)
+    out, saved = torch.empty_like(ops[2]), module.gated_delta_rule_saved(ops[1], ops[2])
+    module.gated_delta_rule_forward(*ops, out, final_state=whole, saved=saved)
+    outs = backward(module, ops, g, saved, final_state_gradient=dfinal, initial_state_gradient=back)
+    halves = [[x[:, i:i + 512].contiguous() for x in (*ops, g)] for i in (0, 512)]
+    kept = []
+    for i, (*half, _) in enumerate(halves):
+        o = torch.empty_like(half[2])
+        kept.append(module.gated_delta_rule_saved(half[1], half[2]))
+        module.gated_delta_rule_forward(*half, o, initial_state=parts if i else None,
+                                        final_state=parts, saved=kept[i])
+        assert torch.equal(o, out[:, 512 * i:512 * i + 512])
+    assert torch.equal(parts, whole)
+    into = dfinal.clone()
+    for i in (1, 0):
+        *half, gradient = halves[i]
+        got = backward(module, half, gradient, kept[i], final_state_gradient=into,
+                       initial_state_gradient=into)
+        for name, a, b in zip(("query", "key", "value", "gate", "write"), got, outs):
+            assert torch.equal(a, b[:, 512 * i:512 * i + 512]), name
+    assert torch.equal(into, back)
