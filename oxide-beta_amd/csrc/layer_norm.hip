@@ -10,7 +10,11 @@
 // is the mean of squared deviations from the row's own mean, not a difference of moments, so a row
 // far from zero keeps its digits.
 //
-// The bound is memory, so a row is read once and kept in registers over both of its statistics.
+// The bound is memory, so a row is read once and kept in registers over both of its statistics:
+// bfloat16 16384 x 4096 forward with the sum 96 us (537 MB, 5.6 TB/s), backward with the parameters'
+// gradients 105 us (537 MB, 5.1 TB/s; 98 and 7 for the blocks' shares).  Small ones are launches and a
+// row's load, sum and store: 1 x 2048 3.1 us of 6.5 a call, backward float32 1021 x 1537 12 and 4 of
+// 16.7 (its rows begin anywhere: 1021 x 1536 takes 8 and 4).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -320,7 +324,8 @@ __global__ __launch_bounds__(1024) void layer_norm_backward_long_kernel(Backward
   }
 }
 
-// Values of a row that a block's registers hold, the backward's with seven for each.
+// Values of a row that a block's registers hold, the backward's with seven for each (float32 1024 x
+// 16384 backward: 49 us, 104 in two passes over the row; bfloat16 4096 x 10240 86 and 248).
 template <typename T>
 constexpr uint64_t forward_limit() {
   return 1024 * 8 * (16 / sizeof(T));
