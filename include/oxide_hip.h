@@ -486,7 +486,7 @@ oxh_status oxh_layer_norm_backward(oxh_stream stream, int dtype, uint64_t rows, 
  * state in place.  lengths (device int32 [batch], may be NULL; clamped to 0..time): a row's steps
  * at or past its length give 0 and leave the state, whatever the operands hold there.
  * Keys of length 1 (or less) keep the state bounded.  A value of a row's own steps that is not
- * finite may reach the outputs of its whole chunk of 64 steps.  bfloat16 operands: products keep 8
+ * finite may reach every output of its head from its chunk of 64 steps on.  bfloat16 operands: products keep 8
  * bits of what is formed on the way, with a final_state 16 of what the state is made of.
  * `saved` (may be NULL) receives what the backward reads; a call without it takes up to 16 steps
  * (48 float32 ones of many heads) one by one, in float32.  OXH_INVALID_SHAPE above a key_dim of 128, a value_dim of 4096, a

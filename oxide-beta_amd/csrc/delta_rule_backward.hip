@@ -27,7 +27,7 @@
 // Measured, bfloat16, 8 x 2048 x 16 heads of 128 keys and values, in two parts: 2 x 38 us to prepare, 2 x
 // 80 to scan (509 MB in both, 3.2 TB/s) and 2 x 105 for the products (721 MB, 3.4 TB/s; their matrix
 // work is 30 us): memory, with two blocks a compute unit.  float32 128 x 28 x 4 heads of 32, one chunk:
-// 15, 12 and 27 us, the chain of a block's stages.
+// 15, 12 and 20 us, the chain of a block's stages.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -547,13 +547,15 @@ struct Products {
   };
   union {
     Pair pairs[2];
+    // then the chunk's keys and queries and the matrices over them; past a row's 64 columns what is
+    // not to be written
     struct {
       RowTile<T, KT> keys, queries;
+      alignas(32) T one[kChunk][kChunk + 8], one_t[kChunk][kChunk + 8], two[kChunk][kChunk + 8];
     };
+    // and the results' rows
     alignas(16) float rows[kChunk][32 * KT + 4];
   };
-  // past a row's 64 columns: what is not to be written
-  alignas(32) T one[kChunk][kChunk + 8], one_t[kChunk][kChunk + 8], two[kChunk][kChunk + 8];
   double sums[kChunk];
   float rows_at[kChunk], columns_at[4][kChunk], before[kChunk], errors[kChunk], across[4];
 };

@@ -313,6 +313,8 @@ class Tensor:
             raise _err(ox.INVALID_SHAPE,
                        "policy_loss expects [batch, classes] logits and one action, log "
                        "probability, advantage and weight a row")
+        if np.shape(clip) != (2,):
+            raise _err(ox.INVALID_SHAPE, "policy_loss clip is (low, high)")
         low, high = np.float32(clip)
         if not (np.isfinite(low) and np.isfinite(high) and 0 <= low <= 1 and high >= 0):
             raise _err(ox.EXECUTION, "policy_loss clips must be finite and non-negative, the low "

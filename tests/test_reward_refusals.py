@@ -260,6 +260,7 @@ def test_tensor_methods():
                                                             i((2, 5, 2)), i((2, 5, 2))),
                  lambda: i((4, 3)).policy_loss(i((4,)), i((4,)), i((3,))),
                  lambda: i((4, 3)).policy_loss(i((4,)), i((4,)), i((4,)), kl=0.1),
+                 lambda: i((4, 3)).policy_loss(i((4,)), i((4,)), i((4,)), clip=0.2),
                  lambda: nn.LayerNorm(0), lambda: nn.DeltaRuleBlock(10, heads=4),
                  lambda: nn.DeltaRuleBlock(12, heads=4, key_heads=3)):
         with pytest.raises(ox.OxideError) as err:
