@@ -296,3 +296,72 @@ def test_example_on_idx_files(tmp_path, capsys, kind):
     lines = capsys.readouterr().out.splitlines()
     assert [line.split()[0] for line in lines] == ["epoch", "epoch", "test"]
     assert math.isfinite(float(lines[1].split()[-1])) and 0 <= float(lines[2].split()[-1]) <= 1
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("batch", [3, 40])  # blocks of 16 columns, and of 32
+def test_launchers_in_one_graph(dtype, batch):
+    """Norm, rule, loss and their gradients recorded as one graph on one stream, replayed on others'
+    data with eager calls of the same launchers between: to the bit what eager calls give."""
+    module, dev = ox.LoadedModule(), torch.device("cuda")
+    heads, time, size = 8, 70, 32
+    width, shape = heads * size, (batch, time, heads, size)
+    zeros = lambda *s, t=dtype: torch.zeros(*s, dtype=t, device=dev)  # noqa: E731
+    f32 = torch.float32
+
+    def fill(a, seed):
+        g = torch.Generator(device=dev).manual_seed(seed)
+        for name, x in a.items():
+            x.copy_(torch.randn(x.shape, generator=g, device=dev))
+        for name in ("query", "key"):
+            a[name].copy_(torch.nn.functional.normalize(a[name].float(), dim=-1) * 0.99)
+        a["actions"].copy_((a["actions"].abs() * 60).clamp_(max=width - 1).floor())
+        a["old"].copy_(-5 + 0.3 * a["old"])
+
+    ins = {"x": zeros(batch * time, width), "residual": zeros(batch * time, width),
+           "query": zeros(*shape), "key": zeros(*shape), "gate": zeros(*shape[:3]),
+           "write": zeros(*shape[:3]), "weight": zeros(width, t=f32), "bias": zeros(width, t=f32),
+           "actions": zeros(batch * time, t=f32), "old": zeros(batch * time, t=f32),
+           "advantages": zeros(batch * time, t=f32)}
+    one = torch.ones(1, device=dev)
+
+    def outputs():
+        like = torch.empty_like
+        return {"sum": like(ins["x"]), "y": like(ins["x"]), "mean": like(ins["old"]),
+                "inverse": like(ins["old"]), "o": like(ins["x"]), "loss": like(one),
+                "dlogits": like(ins["x"]), "dq": like(ins["query"]), "dk": like(ins["key"]),
+                "dv": like(ins["x"]), "dgate": like(ins["gate"]), "dwrite": like(ins["write"]),
+                "dx": like(ins["x"]), "dw": like(ins["weight"]), "db": like(ins["bias"]),
+                "saved": module.gated_delta_rule_saved(ins["key"], ins["x"].view(shape))}
+
+    def run(o, stream=None):
+        s = dict(stream=stream)
+        heads_of = lambda x: x.view(shape)  # noqa: E731
+        module.layer_norm_forward(ins["x"], ins["weight"], ins["bias"], o["y"], o["mean"],
+                                  o["inverse"], ins["residual"], o["sum"], **s)
+        operands = ins["query"], ins["key"], heads_of(o["y"]), ins["gate"], ins["write"]
+        module.gated_delta_rule_forward(*operands, heads_of(o["o"]), saved=o["saved"], **s)
+        module.policy_loss(o["o"], ins["actions"], ins["old"], ins["advantages"], o["loss"],
+                           o["dlogits"], one, **s)
+        module.gated_delta_rule_backward(
+            heads_of(o["dlogits"]), *operands, o["saved"], o["dq"], o["dk"], heads_of(o["dv"]),
+            o["dgate"], o["dwrite"], **s)
+        module.layer_norm_backward(o["dv"], o["sum"], ins["weight"], o["mean"], o["inverse"],
+                                   o["dx"], o["dw"], o["db"], **s)
+
+    fill(ins, 1)
+    eager, captured = outputs(), outputs()
+    run(eager)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = ox.HipGraphExec.capture(stream, lambda: run(captured, stream))
+    for seed in (2, 3, 4):
+        fill(ins, seed)
+        torch.cuda.synchronize()
+        graph.launch(stream)
+        run(eager)
+        torch.cuda.synchronize()
+        for name, x in eager.items():
+            if name != "saved":
+                assert torch.equal(x, captured[name]), (seed, name)
+        assert math.isfinite(eager["loss"].item()) and eager["dw"].abs().sum() > 0
