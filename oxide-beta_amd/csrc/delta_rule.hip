@@ -207,7 +207,7 @@ __global__ __launch_bounds__(512, Packed && sizeof(T) == 2 && C == 2 && P == 1 ?
       const uint32_t k = key_at(r), there = min(k, d.keys - 1);
       const float v = a.from[state_at + static_cast<uint64_t>(there) * d.values +
                              min(column_of(c, n), d.values - 1)];
-      state[c][r] = k < d.keys ? v : 0.0f;
+      state[c][r] = k < d.keys && column_of(c, n) < d.values ? v : 0.0f;
     }
   }
 
