@@ -489,9 +489,9 @@ oxh_status oxh_layer_norm_backward(oxh_stream stream, int dtype, uint64_t rows, 
  * finite may reach every output of its head from its chunk of 64 steps on.  bfloat16 operands: products keep 8
  * bits of what is formed on the way, with a final_state 16 of what the state is made of.
  * `saved` (may be NULL) receives what the backward reads; a call without it takes up to 16 steps
- * (48 float32 ones of many heads) one by one, in float32.  OXH_INVALID_SHAPE above a key_dim of 128, a value_dim of 4096, a
- * batch or heads of 65535 or heads * value_dim of 2^24 - 1, or where one launch cannot number the
- * threads. */
+ * (48 float32 ones of many heads) one by one, in float32.  OXH_INVALID_SHAPE above a key_dim of
+ * 128, a value_dim of 4096, a batch or heads of 65535 or heads * value_dim of 2^24 - 1, or where
+ * one launch cannot number the threads. */
 typedef struct oxh_delta_shape {
   uint64_t batch, time, key_heads, heads, key_dim, value_dim;
 } oxh_delta_shape;

@@ -6,9 +6,9 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <initializer_list>
 #include <string>
 #include <type_traits>
-#include <vector>
 
 #include "common.h"
 #include "row_norm.h"
@@ -604,21 +604,31 @@ struct Span {
   const void *p;
   uint64_t bytes, align;
 };
+// A call's operands or outputs: no more than this many, and no memory that could be refused.
+struct Spans {
+  Span span[12];
+  int count = 0;
+  Spans(std::initializer_list<Span> from) {
+    for (const Span &x : from) push_back(x);
+  }
+  void push_back(const Span &x) { span[count++] = x; }
+  const Span *begin() const { return span; }
+  const Span *end() const { return span + count; }
+};
 // Aligned to their elements; no output over an operand or another output.
-inline oxh_status check_apart(const std::vector<Span> &in, const std::vector<Span> &out) {
+inline oxh_status check_apart(const Spans &in, const Spans &out) {
   for (const auto *list : {&in, &out})
     for (const Span &x : *list)
       OXH_REQUIRE(row_norm::aligned_to(x.p, x.align), OXH_INVALID_SHAPE,
                   "gated delta rule: a pointer is not aligned to its elements");
-  for (size_t o = 0; o < out.size(); ++o) {
-    if (out[o].p == nullptr) continue;
+  for (const Span &o : out) {
+    if (o.p == nullptr) continue;
     for (const Span &i : in)
-      OXH_REQUIRE(i.p == nullptr || !any_overlap(out[o].p, out[o].bytes, i.p, i.bytes),
+      OXH_REQUIRE(i.p == nullptr || !any_overlap(o.p, o.bytes, i.p, i.bytes),
                   OXH_INVALID_SHAPE,
                   "gated delta rule: an output, saved or the workspace overlaps an operand");
-    for (size_t k = 0; k < o; ++k)
-      OXH_REQUIRE(out[k].p == nullptr ||
-                      !any_overlap(out[o].p, out[o].bytes, out[k].p, out[k].bytes),
+    for (const Span *k = out.begin(); k != &o; ++k)
+      OXH_REQUIRE(k->p == nullptr || !any_overlap(o.p, o.bytes, k->p, k->bytes),
                   OXH_INVALID_SHAPE, "gated delta rule: two outputs overlap");
   }
   return ok();

@@ -34,7 +34,6 @@
 #include <cmath>
 #include <cstddef>
 #include <string>
-#include <vector>
 
 #include "common.h"
 #include "delta_rule.h"
@@ -158,8 +157,8 @@ struct Exchange {
 // and those over the steps both find their operands: of many blocks the bytes count, a third less
 // without the copies (8 x 2048 x 16 heads: 204 us prepared and scanned, 270 with copies).
 template <typename T, int P, int KT, int C, bool Packed>
-__global__ __launch_bounds__(512, Packed && sizeof(T) == 2 && C == 2 && P == 1 ? 4 : 2) void delta_scan_kernel(
-    ScanArgs<T> a) {
+__global__ __launch_bounds__(512, Packed && sizeof(T) == 2 && C == 2 && P == 1 ? 4 : 2) void
+delta_scan_kernel(ScanArgs<T> a) {
   using Op = operand<T>;
   using Kept = Chunk<T, P>;
   __shared__ Exchange<T, P, KT, C> m;
@@ -420,8 +419,8 @@ __global__ __launch_bounds__(512, Packed && sizeof(T) == 2 && C == 2 && P == 1 ?
     typename Part::Values key_part, query_part;
     const uint64_t key_row0 = (row0 * d.key_heads + kh) * d.keys;
     auto load_rows = [&](typename Part::Values &to, const T *from, uint32_t chunk) {
-      part.load(to, buffer_of(from + key_row0 + chunk * kChunk * static_cast<uint64_t>(d.key_heads) * d.keys,
-                              rows_of(chunk) * row_bytes), d.keys);
+      const uint64_t first = chunk * kChunk * static_cast<uint64_t>(d.key_heads) * d.keys;
+      part.load(to, buffer_of(from + key_row0 + first, rows_of(chunk) * row_bytes), d.keys);
     };
     auto load_scores = [&](uint32_t chunk) {
       const auto from = operands_of(chunk, Kept::within);
@@ -757,9 +756,9 @@ oxh_status by_steps(hipStream_t stream, const StepArgs<T> &a) {
 }
 
 template <typename T, int P>
-oxh_status by_chunks(hipStream_t stream, const ForwardPlan<T, P> &plan, const T *query, const T *key, const T *value,
-                     const T *gate, const T *write, const float *initial, T *out, float *final,
-                     char *saved, char *workspace) {
+oxh_status by_chunks(hipStream_t stream, const ForwardPlan<T, P> &plan, const T *query,
+                     const T *key, const T *value, const T *gate, const T *write,
+                     const float *initial, T *out, float *final, char *saved, char *workspace) {
   const Plan &p = plan.p;
   char *heads = workspace, *keys = plan.two ? nullptr : heads + plan.head_bytes;
   float *between = reinterpret_cast<float *>(heads + plan.head_bytes + plan.key_bytes);
@@ -848,10 +847,10 @@ oxh_status oxh_gated_delta_rule_forward(oxh_stream stream, int dtype, const oxh_
   OXH_REQUIRE(std::isfinite(scale), OXH_EXECUTION, "gated delta rule: scale must be finite");
   if (s.batch == 0) return oxh::ok();
   const Sizes z(dtype, s);
-  std::vector<Span> in = {{query, z.query, z.element}, {key, z.query, z.element},
-                          {value, z.value, z.element}, {gate, z.gate, z.element},
-                          {write, z.gate, z.element}};
-  std::vector<Span> out = {{output, z.value, z.element}};
+  Spans in = {{query, z.query, z.element}, {key, z.query, z.element},
+              {value, z.value, z.element}, {gate, z.gate, z.element},
+              {write, z.gate, z.element}};
+  Spans out = {{output, z.value, z.element}};
   for (const auto *list : {&in, &out})
     for (const Span &x : *list)
       OXH_REQUIRE(x.p != nullptr || x.bytes == 0, OXH_INVALID_SHAPE,

@@ -34,7 +34,6 @@
 #include <cmath>
 #include <cstddef>
 #include <string>
-#include <vector>
 
 #include "common.h"
 #include "delta_rule.h"
@@ -942,13 +941,13 @@ oxh_status oxh_gated_delta_rule_backward(
   st = oxh_gated_delta_rule_saved_size(dtype, shape, &kept);
   if (st == OXH_OK) st = oxh_gated_delta_rule_backward_workspace_size(dtype, shape, &needed);
   if (st != OXH_OK) return st;
-  std::vector<Span> in = {{gradient, z.value, z.element}, {query, z.query, z.element},
-                          {key, z.query, z.element},      {value, z.value, z.element},
-                          {gate, z.gate, z.element},      {write, z.gate, z.element},
-                          {saved, kept, 16}};
-  std::vector<Span> out = {{query_gradient, z.query, z.element}, {key_gradient, z.query, z.element},
-                           {value_gradient, z.value, z.element}, {gate_gradient, z.gate, z.element},
-                           {write_gradient, z.gate, z.element},  {workspace, needed, 16}};
+  Spans in = {{gradient, z.value, z.element}, {query, z.query, z.element},
+              {key, z.query, z.element},      {value, z.value, z.element},
+              {gate, z.gate, z.element},      {write, z.gate, z.element},
+              {saved, kept, 16}};
+  Spans out = {{query_gradient, z.query, z.element}, {key_gradient, z.query, z.element},
+               {value_gradient, z.value, z.element}, {gate_gradient, z.gate, z.element},
+               {write_gradient, z.gate, z.element},  {workspace, needed, 16}};
   for (const auto *list : {&in, &out})
     for (const Span &x : *list)
       OXH_REQUIRE(x.p != nullptr || x.bytes == 0, OXH_INVALID_SHAPE,
