@@ -798,6 +798,15 @@ oxh_status by_chunks(hipStream_t stream, const ForwardPlan<T, P> &plan, const T 
   return oxh::ok();
 }
 
+// Bytes of the workspace of every form that a call by chunks may take (P: it hands a state on or not).
+// The one of two operands' parts has the larger chunks, so it may prepare fewer of them at a time and
+// need less in all (8 x 6144 x 16 heads of 128: 126 MB, the other 160).
+template <typename T>
+uint64_t chunks_bytes(const oxh_delta_shape &s) {
+  const uint64_t one = ForwardPlan<T, 1>(s, 1.0f, nullptr).bytes();
+  return sizeof(T) == 4 ? one : std::max(one, ForwardPlan<T, 2>(s, 1.0f, nullptr).bytes());
+}
+
 bool by_steps_alone(int dtype, const oxh_delta_shape &s, bool saves) {
   return s.time == 0 || (!saves && s.time <= step_limit(s, dtype == OXH_F32));
 }
@@ -829,8 +838,7 @@ oxh_status oxh_gated_delta_rule_workspace_size(int dtype, const oxh_delta_shape 
   if (st != OXH_OK) return st;
   *bytes = 0;
   if (by_steps_alone(dtype, *shape, saves != 0)) return oxh::ok();
-  *bytes = dtype == OXH_F32 ? ForwardPlan<float, 1>(*shape, 1.0f, nullptr).bytes()
-                            : ForwardPlan<bf16, 2>(*shape, 1.0f, nullptr).bytes();
+  *bytes = dtype == OXH_F32 ? chunks_bytes<float>(*shape) : chunks_bytes<bf16>(*shape);
   return oxh::ok();
 }
 
