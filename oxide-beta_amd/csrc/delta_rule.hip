@@ -453,13 +453,15 @@ delta_scan_kernel(ScanArgs<T> a) {
       const auto to = buffer_of(outs + chunk * kChunk * value_stride,
                                 there ? rows_of(chunk) * value_bytes : 0);
       const uint32_t at = step * value_bytes + first * kValue;
-      if constexpr (Packed && C == 2) {
+      // 16 bytes at a time end with a row's values: 8 of bfloat16, 4 of float32
+      if constexpr (Packed && C == 2 && sizeof(T) == 2) {
         store_to(to, first < d.values ? at : kNowhere, rounded<T>(join(o[0], o[1])));
       } else {
 #pragma unroll
         for (int c = 0; c < C; ++c) {
           if constexpr (Packed) {
-            store_to(to, first < d.values ? at : kNowhere, __builtin_convertvector(o[c], quarter));
+            store_to(to, first + 4 * c < d.values ? at + 4 * c * kValue : kNowhere,
+                     __builtin_convertvector(o[c], quarter));
           } else {
 #pragma unroll
             for (int r = 0; r < 4; ++r)

@@ -4,11 +4,18 @@ against the steps in float64, with the tolerances of test_gpu_delta_rule."""
 
 import ctypes
 
+import numpy as np
 import pytest
 import torch
+import torch.nn.functional as F
 
+import nn
 import oxide_hip as ox
-from test_gpu_delta_rule import TYPES, check_forward, operands
+import sequence
+from test_gpu_delta_rule import TYPES, backward, check_forward, check_gradients, operands
+from test_gpu_reward_net import c64, model64
+from test_gpu_rms_norm import make
+from test_gpu_sequence_net import close, images_of, leaf
 
 pytestmark = pytest.mark.gpu
 F32, BF16 = torch.float32, torch.bfloat16
@@ -40,3 +47,54 @@ def test_workspace_without_a_final_state(module, dev, shape, saves):
         at(room), size))
     assert (room[size:] == 0x5A).all()
     check_forward(ops, out, None, BF16, True)
+
+
+# widths of every remainder by the columns that one access stores, of many heads (blocks of 32
+# columns) and of few (16)
+WIDTHS = [(64, 66, 2, 4, 32, 36), (256, 70, 1, 1, 32, 12), (32, 65, 4, 8, 20, 20),
+          (64, 70, 1, 1, 64, 100), (1, 130, 1, 256, 8, 28), (128, 28, 4, 4, 20, 20),
+          (86, 65, 1, 3, 12, 4), (32, 66, 2, 8, 16, 56), (2, 70, 1, 2, 8, 12), (1, 66, 2, 4, 4, 36)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", WIDTHS)
+def test_outputs_of_every_width(module, dev, shape, dtype):
+    """16-byte aligned rows, which are stored 16 bytes at a time, and nothing around them: outputs
+    and gradients, the same bits when asked again."""
+    t = TYPES[dtype]
+    ops = operands(shape, t, dev, 3)
+    g = make(ops[2].shape, t, dev, 21)
+    edge = 64  # elements
+    rooms = [torch.full((x.numel() + 2 * edge,), 7.0, dtype=t, device=dev)
+             for x in (ops[2], *ops)]
+    out, *grads = [r[edge:-edge].view(x.shape) for r, x in zip(rooms, (ops[2], *ops))]
+    assert out.data_ptr() % 16 == 0
+    saved = module.gated_delta_rule_saved(ops[1], ops[2])
+    module.gated_delta_rule_forward(*ops, out, saved=saved)
+    ref = check_forward(ops, out, None, t, True)
+    module.gated_delta_rule_backward(g, *ops, saved, *grads)
+    check_gradients(ref, g, grads, t)
+    for r in rooms:
+        assert (r[:edge] == 7).all() and (r[-edge:] == 7).all()
+    again = torch.full_like(out, 3.0)
+    module.gated_delta_rule_forward(*ops, again, saved=saved)
+    assert torch.equal(again, out)
+    for x, y in zip(backward(module, ops, g, saved), grads):
+        assert torch.equal(x, y)
+
+
+def test_classifier_of_20_columns_a_head():
+    """Its training forward and gradients, at the example's batch."""
+    images, labels = images_of(128)
+    pixels = images.astype(np.float32).reshape(128, 1, 28, 28) / 255
+    model = sequence.RowClassifier(features=80, depth=1, block=nn.DeltaRuleBlock, norm=nn.LayerNorm)
+    step = sequence.Training(model, 128)
+    step.images.copy_from(pixels)
+    step.labels.copy_from(labels.astype(np.float32))
+    params = [leaf(p.host()) for p in model.parameters()]
+    step.step()
+    logits = model64(model, params, c64(pixels[:, 0]))
+    F.cross_entropy(logits, torch.tensor(labels.astype(np.int64))).backward()
+    close(step.logits.host(), logits, "logits")
+    for p, ref in zip(model.parameters(), params):
+        close(step.program.gradient(p.tensor()).host(), ref.grad, p.shape)
