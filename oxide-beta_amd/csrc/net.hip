@@ -1028,7 +1028,11 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam,
   const bool root_fused_ce = is_loss(g.nodes[root].op) && want(g.nodes[root].in[0]);
   for (size_t r = n; r-- > 0;) {
     const Node &x = g.nodes[r];
-    if (!want(static_cast<int>(r)) || fused_bn[r] || pre_fused[r]) continue;
+    if (!want(static_cast<int>(r)) || fused_bn[r]) continue;
+    if (pre_fused[r]) {  // what its other consumers contribute, for the layer's launch to add
+      has_grad[r] = consumers[r] > 1;
+      continue;
+    }
     if (static_cast<int>(r) == root && root_fused_ce) continue;  // its outer gradient is 1
     if (x.op == Op::Param) continue;  // its gradient buffer is the optimizer's
     has_grad[r] = 1;
