@@ -935,7 +935,16 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam,
     else
       for (int k : x.in) needs[i] = needs[i] || needs[k];
   }
-  auto want = [&](int i) { return active[i] && needs[i]; };
+  // ... and which the root's gradient reaches: a loss passes it to its logits alone, so what only
+  // its other operands are made of takes none and is not trained
+  std::vector<char> reached(n, 0);
+  reached[root] = 1;
+  for (size_t r = static_cast<size_t>(root) + 1; r-- > 0;) {
+    const Node &x = g.nodes[r];
+    for (size_t k = 0; reached[r] && k < (is_loss(x.op) ? 1 : x.in.size()); ++k)
+      reached[x.in[k]] = 1;
+  }
+  auto want = [&](int i) { return reached[i] && needs[i]; };
 
   // consumers among the participating nodes
   std::vector<int> consumers(n, 0);
@@ -1014,6 +1023,7 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam,
     else if (g.nodes[cin].op == Op::Add && add_absorbed[cin])
       b1 = g.nodes[cin].in[0];
     if (b1 < 0 || dw_conv_of[b1] >= 0) continue;
+    if (want(b1) && !want(static_cast<int>(i))) continue;  // its gradient comes from elsewhere
     const oxh_conv2d_shape s = conv_shape(g, g.nodes[i]);
     if (!oxh_batch_norm_depthwise_conv_batch_norm_supported(&s)) continue;
     pre_bn_of[i] = b1;
@@ -1086,7 +1096,7 @@ oxh_status build_training(const Graph &g, int root, const AdamConfig *adam,
   // runtime.rs:1330-1332)
   std::vector<int> trained;
   for (int pn : g.params)
-    if (active[pn]) trained.push_back(pn);
+    if (reached[pn]) trained.push_back(pn);
   std::vector<std::array<int64_t, 3>> poff(trained.size());
   for (size_t k = 0; k < trained.size(); ++k) {
     const uint64_t bytes = node_bytes(g.nodes[trained[k]]);
