@@ -920,7 +920,8 @@ oxh_status oxh_program_op_count(const oxh_program *program, uint64_t *count);
 oxh_status oxh_program_op(const oxh_program *program, uint64_t index, oxh_op_info *info);
 oxh_status oxh_program_run_op(oxh_program *program, uint64_t index);
 /* Waits for the program's stream; OXH_INVALID_SHAPE (and the flag cleared) if a cross entropy
- * met a target that is not a class index since the last check (evaluation.rs:622-636). */
+ * met a target, or a policy loss an action, that is not a class index since the last check
+ * (evaluation.rs:622-636). */
 oxh_status oxh_program_check(oxh_program *program);
 /* The optimizer's device step counter after the enqueued work (0 without AdamW). */
 oxh_status oxh_program_steps(oxh_program *program, int32_t *steps);

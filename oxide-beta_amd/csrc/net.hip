@@ -2491,7 +2491,8 @@ oxh_status oxh_program_check(oxh_program *p) {
   OXH_HIP_CHECK(hipMemcpy(&flag, p->error_flag, 4, hipMemcpyDeviceToHost));
   if (flag != 0) {
     OXH_HIP_CHECK(hipMemset(p->error_flag, 0, 4));
-    return oxh::fail(OXH_INVALID_SHAPE, "cross entropy target is not a class index");
+    return oxh::fail(OXH_INVALID_SHAPE,
+                     "a cross entropy target or policy loss action is not a class index");
   }
   return oxh::ok();
 }

@@ -10,6 +10,7 @@ import torch
 import torch.nn.functional as F
 
 import nn
+import oxide_hip as ox
 import tensor as tn
 from test_gpu_reward_net import c64, drawn, policy64
 from test_gpu_sequence_net import close, kinds, leaf, randn, run_checked
@@ -108,3 +109,18 @@ def test_layers_of_a_branch_without_gradient():
     close(program.gradient(own.tensor()).host(), P.grad, "other logits")
     for p, was in zip(layer.parameters(), before):
         assert program.gradient(p.tensor()) is None and np.array_equal(p.host(), was)
+
+
+def test_what_the_check_says_of_an_action():
+    x, rows = tn.input((2, 3), requires_grad=True), [tn.input((2,)) for _ in range(3)]
+    program = tn.training_program(x.policy_loss(*rows))
+    for node in (x, *rows):
+        program.feed(node, np.zeros(node.shape))
+    program.feed(rows[0], np.array([1.0, 3.0]))
+    program.run()
+    with pytest.raises(ox.OxideError, match="action is not a class index") as err:
+        program.check()
+    assert err.value.kind == "InvalidShape"
+    program.feed(rows[0], np.array([1.0, 2.0]))
+    program.run()
+    program.check()
