@@ -49,6 +49,32 @@ def test_workspace_without_a_final_state(module, dev, shape, saves):
     check_forward(ops, out, None, BF16, True)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(2, 130, 1, 2, 64, 40), (64, 130, 4, 8, 40, 12),
+                                   (1, 9000, 16, 16, 128, 8), (64, 640, 8, 16, 8, 8)])
+def test_saved_and_both_workspaces(module, dev, shape, dtype):
+    """Training by a caller with buffers of exactly the sizes named: one part, and several."""
+    t, code = TYPES[dtype], {"f32": ox.F32, "bf16": ox.BF16}[dtype]
+    ops = operands(shape, t, dev, 6)
+    g = make(ops[2].shape, t, dev, 21)
+    out, grads = torch.empty_like(ops[2]), [torch.empty_like(x) for x in ops]
+    _, _, forward, kept, back = ox._delta_plan(code, *shape)
+    dims, scale, edge = ctypes.byref(ox.DeltaShape(*shape)), shape[4] ** -0.5, 1 << 20
+    saved, ws, ws_back = (torch.full((n + edge,), 0x5A, dtype=torch.uint8, device=dev)
+                          for n in (kept, forward, back))
+    stream = ox.current_stream()
+    ox.check(ox.lib().oxh_gated_delta_rule_forward(
+        stream, code, dims, scale, *[at(x) for x in ops], None, None, at(out), None, at(saved), kept,
+        at(ws), forward))
+    ox.check(ox.lib().oxh_gated_delta_rule_backward(
+        stream, code, dims, scale, at(g), *[at(x) for x in ops], at(saved), kept, None, None,
+        *[at(x) for x in grads], None, at(ws_back), back))
+    for x, n in ((saved, kept), (ws, forward), (ws_back, back)):
+        assert (x[n:] == 0x5A).all()
+    ref = check_forward(ops, out, None, t, True)
+    check_gradients(ref, g, grads, t)
+
+
 # widths of every remainder by the columns that one access stores, of many heads (blocks of 32
 # columns) and of few (16)
 WIDTHS = [(64, 66, 2, 4, 32, 36), (256, 70, 1, 1, 32, 12), (32, 65, 4, 8, 20, 20),
