@@ -189,6 +189,9 @@ def accuracy(model: RowClassifier, images, labels, batch=100) -> float:
 
 
 def main(directory: str, epochs: int = 1, *kinds: str) -> None:
+    unknown = set(kinds) - {"delta", "reward"}
+    if unknown:
+        raise ValueError(f"sequence.py takes delta and reward, not {', '.join(sorted(unknown))}")
     mnist = data.Mnist.load(directory)
     model = (RowClassifier(block=nn.DeltaRuleBlock, norm=nn.LayerNorm) if "delta" in kinds
              else RowClassifier())
