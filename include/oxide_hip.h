@@ -486,8 +486,9 @@ oxh_status oxh_layer_norm_backward(oxh_stream stream, int dtype, uint64_t rows, 
  * state in place.  lengths (device int32 [batch], may be NULL; clamped to 0..time): a row's steps
  * at or past its length give 0 and leave the state, whatever the operands hold there.
  * Keys of length 1 (or less) keep the state bounded.  A value of a row's own steps that is not
- * finite may reach every output of its head from its chunk of 64 steps on.  bfloat16 operands: products keep 8
- * bits of what is formed on the way, with a final_state 16 of what the state is made of.
+ * finite may reach every output of its head from its chunk of 64 steps on, earlier steps of that
+ * chunk among them.  bfloat16 operands: products keep 8 bits of what is formed on the way, with a
+ * final_state 16 of what the state is made of.
  * `saved` (may be NULL) receives what the backward reads; a call without it takes up to 16 steps
  * (48 float32 ones of many heads) one by one, in float32.  OXH_INVALID_SHAPE above a key_dim of
  * 128, a value_dim of 4096, a batch or heads of 65535 or heads * value_dim of 2^24 - 1, or where
@@ -531,7 +532,8 @@ oxh_status oxh_gated_delta_rule_backward(
  * (l; 0 for a row of weight 0) and gradient (of the logits, times outer_gradient[0]) may be NULL.
  * The clip's borders belong to its inside.  An action that is no class index makes the loss, its
  * row's gradient and log probability NaN and sets error_flag (may be NULL).  The workspace is the
- * loss's. */
+ * loss's.  OXH_INVALID_SHAPE without rows or classes, above 2^21 rows or from 2^31 - 65536 classes
+ * on. */
 oxh_status oxh_policy_loss_workspace_size(uint64_t rows, uint64_t classes, uint64_t *bytes);
 oxh_status oxh_policy_loss(oxh_stream stream, int dtype, uint64_t rows, uint64_t classes,
                            float clip_low, float clip_high, float kl, const void *logits,

@@ -19,9 +19,10 @@
 //
 // What is rounded.  float32 operands: nothing, the matrix cores take float32.  bfloat16 ones: q, k and
 // v as they are; the state, N, G o q k', b y and b e as operands of products, 8 bits each, their sums
-// and the state itself float32: outputs are 2.4e-3 off in the mean square, 1.7e-3 being their own
-// rounding.  A state that is handed on is formed from pairs of such operands that add up to 16 bits
-// (2^-17): rounding it to 8 at each of many chunks is no error of one output but of all later calls.
+// and the state itself float32: outputs are 2.4e-3 to 4.3e-3 off in the mean square, the more the longer
+// a state lasts and the narrower it is, 1.7e-3 being their own rounding.  A state that is handed on is
+// formed from pairs of such operands that add up to 16 bits (2^-17; 2e-6 to 6e-6 in the mean square):
+// rounding it to 8 at each of many chunks is no error of one output but of all later calls.
 //
 // Measured, bfloat16, heads of 128 keys and 128 values: 8 x 2048 x 16 heads with what the backward reads
 // 60 us to prepare (183 MB, 3.1 TB/s) and 144 to scan (511 MB, 3.5 TB/s): memory.  1 x 32768 x 16 heads
@@ -55,7 +56,7 @@ struct PrepareArgs {
 
 // A block per chunk and value head.  Its own work is 64 x 64 products; what it reads and writes bounds
 // it, or for one chunk of few heads the inversion's 16 dependent steps and three more barriers
-// (float32 128 x 28 x 4 heads of 32: 14 us).
+// (float32 128 x 28 x 4 heads of 32: 15 to 18 us).
 template <typename T, int P, int KT, bool Whole>
 __global__ __launch_bounds__(256) void delta_prepare_kernel(PrepareArgs<T> a) {
   using Op = operand<T>;
@@ -599,7 +600,8 @@ struct StepArgs {
 
 // A wave per 32 columns of a head's values: a lane R consecutive keys of 4 columns, kept in
 // registers from step to step.  One step reads and writes the state once, in 16 bytes a lane of a row
-// of 128: 64 rows of 32 heads of 128 x 128 in 57 us, 4.7 TB/s, which bounds it.
+// of 128: 64 rows of 32 heads of 128 x 128 in 57 us a call, 4.7 TB/s, which bounds it (48 us and 5.6
+// TB/s in a trace of two sets of states in turn, of which the caches keep a part).
 template <typename T, int R, bool Whole>
 __global__ __launch_bounds__(256) void delta_step_kernel(StepArgs<T> a) {
   const Dims &d = a.d;

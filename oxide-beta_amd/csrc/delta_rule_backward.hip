@@ -21,11 +21,12 @@
 // a block per chunk and key head.  S0 and e are the forward's.
 //
 // Rounded as the forward's: of bfloat16 operands u, x, dS, S0, e, M1, M2 and the matrices keep 8 bits
-// where they are operands, sums and dS itself float32; gradients are up to 3.4e-3 off in the mean
-// square.  The gates' sums are float32 throughout but for those operands.
+// where they are operands, sums and dS itself float32; gradients are 2.3e-3 to 4.3e-3 off in the
+// mean square, those of gates, whose terms cancel, up to 6.5e-3.  The gates' sums are float32 throughout
+// but for those operands.
 //
-// Measured, bfloat16, 8 x 2048 x 16 heads of 128 keys and values, in two parts: 2 x 38 us to prepare, 2 x
-// 80 to scan (509 MB in both, 3.2 TB/s) and 2 x 105 for the products (721 MB, 3.4 TB/s; their matrix
+// Measured, bfloat16, 8 x 2048 x 16 heads of 128 keys and values, in two parts: 2 x 37 us to prepare, 2 x
+// 82 to scan (509 MB in both, 3.1 TB/s) and 2 x 99 for the products (721 MB, 3.6 TB/s; their matrix
 // work is 30 us): memory, with two blocks a compute unit.  float32 128 x 28 x 4 heads of 32, one chunk:
 // 15, 12 and 20 us, the chain of a block's stages.
 #include <hip/hip_runtime.h>

@@ -11,10 +11,11 @@
 // far from zero keeps its digits.
 //
 // The bound is memory, so a row is read once and kept in registers over both of its statistics:
-// bfloat16 16384 x 4096 forward with the sum 96 us (537 MB, 5.6 TB/s), backward with the parameters'
-// gradients 105 us (537 MB, 5.1 TB/s; 98 and 7 for the blocks' shares).  Small ones are launches and a
-// row's load, sum and store: 1 x 2048 3.1 us of 6.5 a call, backward float32 1021 x 1537 12 and 4 of
-// 16.7 (its rows begin anywhere: 1021 x 1536 takes 8 and 4).
+// bfloat16 16384 x 4096 forward with the sum 97 to 103 us (537 MB, 5.2 to 5.5 TB/s), backward with the
+// parameters' gradients 105 us a call (537 MB, 5.1 TB/s; its kernels 99 to 103 and 7 for the blocks'
+// shares).  Small ones are launches and a row's load, sum and store: 1 x 2048 3 us of 6.5 a call,
+// backward float32 1021 x 1537 16.7 a call, its kernels 14 and 4 in a trace (its rows begin anywhere:
+// 1021 x 1536 takes 10 and 4 there).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -52,8 +53,8 @@ __device__ __forceinline__ void counted(const typename oxh::storage::Pack<T, N>:
 }
 
 // Stores access c of a row's lane.  A ragged row's last one goes value by value, in the one chunk that
-// holds it: the others have no such path to pass (float32 1021 x 1537 backward: 10.4 us, 13.1 with a
-// path in each).
+// holds it: the others have no such path to pass (float32 1021 x 1537 backward: 16.7 us a call, 17.5
+// with a path in each).
 template <typename T, int N, int Lanes, bool Ragged>
 __device__ __forceinline__ void store_chunk(T *row, int c, uint32_t lane, uint32_t columns,
                                             const float (&v)[N]) {

@@ -970,7 +970,8 @@ class LoadedModule:
         [1] = sum of weight * (-min(r A, clip(r) A) + kl (exp(d) - d - 1)) with l = log
         softmax(logits)[action], r = exp(l - old), d = reference - l; ``weights`` None: 1 / rows.
         ``actions`` are class indexes in float32, as cross entropy's targets; ``log_probs`` [rows]
-        receives l, ``gradient`` the logits' gradient times ``outer_gradient`` [1]."""
+        receives l, ``gradient`` the logits' gradient times ``outer_gradient`` [1].  At most 2^21
+        rows."""
         shape = logits.shape
         if len(shape) != 2:
             raise OxideError(INVALID_SHAPE, "policy_loss expects [rows, classes] logits")
@@ -1184,7 +1185,9 @@ class LoadedModule:
         ``query`` and ``key`` [batch, time, key_heads, key_dim], ``gate`` and ``write`` [batch,
         time, heads]; states [batch, heads, key_dim, value_dim] float32 (the final one may be
         written over the initial one), ``lengths`` [batch] int32, ``scale`` key_dim ** -0.5 unless
-        given; ``saved`` (``gated_delta_rule_saved``) receives what the backward reads."""
+        given; ``saved`` (``gated_delta_rule_saved``) receives what the backward reads.  A value
+        within a row's length that is not finite may reach every output of its head from its chunk
+        of 64 steps on, earlier steps of the chunk among them."""
         dims = _delta_dims(query, key, value)
         batch, time, _, heads, keys, values = dims
         code, query_at, key_at = _activations((query, key), query.shape, "gated_delta_rule")

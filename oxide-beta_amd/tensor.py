@@ -282,7 +282,8 @@ class Tensor:
         """The answers to these queries of a state that each step fades by sigmoid(gate) and moves
         by sigmoid(write) towards value at key, from a zero state; queries and keys [batch, time,
         key heads, key size], values [batch, time, heads, value size], gate and write [batch, time,
-        heads].  ``scale``: key size ** -0.5."""
+        heads].  ``scale``: key size ** -0.5.  What is not finite may reach its head's outputs from
+        its chunk of 64 steps on, earlier steps of the chunk among them."""
         if (len(self.shape) != 4 or key.shape != self.shape or len(value.shape) != 4
                 or value.shape[:2] != key.shape[:2]):
             raise _err(ox.INVALID_SHAPE,
